@@ -270,6 +270,132 @@ xm_status xm_gated_deltanet2_fwd(const xm_gated_deltanet2_attrs *attrs, const xm
 xm_status xm_gated_deltanet2_fwd_static_ws(const xm_gated_deltanet2_attrs *attrs, const xm_tensor *inputs,
                                            int32_t n_inputs, xm_tensor *output, void *cuda_stream);
 
+/* ---------------------------------------------------------------- Serving operators
+ * The operators around SelectiveScanFn in a served selective-scan model (no
+ * reference counterpart: the reference's SelectiveScanFn starts every call from
+ * a zero state, and its graphs run the convolution as an ONNX Conv): the short
+ * causal convolution and the scan over prompts, which continue cached states
+ * and may be packed with different lengths, and both for single tokens.
+ *
+ * Common to the four:
+ *  - Overloads are selected by the first input's type: float32, bfloat16 or
+ *    float16 activations. Parameters (weight, bias, A, D, delta_bias) and the
+ *    scan's state are float32, arithmetic is float32, outputs are rounded once.
+ *    The convolution's state holds copies of its inputs, in their type.
+ *  - A state tensor has one row per sequence (batch row, or packed sequence).
+ *    With state_indices (int32 or int64, one per sequence) it is a pool of
+ *    slots instead, and sequence i owns row state_indices[i]. An index that is
+ *    negative or not below the number of slots owns no row: a prompt then starts
+ *    from zeros and stores no final state; a single-token row is skipped, its
+ *    output row left as it was (padding of a captured graph's batch). Two
+ *    sequences of one call must not own the same slot: nothing outside the pool
+ *    is touched then, but which of the two states it holds is not defined.
+ *  - cu_seqlens (int32 or int64, [sequences + 1] ascending offsets [0, ...])
+ *    packs sequences into the single batch row; lengths of zero are allowed, and
+ *    positions behind the last offset are neither read nor written. Offsets are
+ *    clamped into the row, so malformed ones never address outside it.
+ *  - A state output may be the state input itself (same address, in place);
+ *    with state_indices it must be. Apart from that, an output that overlaps an
+ *    input or another output is rejected.
+ *  - Empty tensors are absent inputs. Tokens per call (batch x seqlen) and every
+ *    dimension are limited to 2^31 - 1.
+ */
+
+/* CausalConv1dFn: y[t, d] = act(bias[d] + sum_k weight[d, k] x[t - (width - 1) + k, d]),
+ * x before a sequence's first token taken from its state (zeros without one).
+ * Inputs (7, in order): x, weight, bias, initial_state, cu_seqlens,
+ *   state_indices, has_initial_state.
+ *   x [batch, dim, seqlen], or [batch, seqlen, dim] with channels_last; weight
+ *   [dim, width], width 2 to 4; bias [dim] or empty; initial_state
+ *   [sequences or slots, dim, width - 1], oldest input first, or empty;
+ *   has_initial_state (int32 or int64, [sequences], or empty): sequences with 0
+ *   start from zeros whatever their state row holds.
+ * Outputs: y (x's shape and type); with output_final_state the last width - 1
+ *   inputs of every sequence (its starting state counted in), same shape as
+ *   initial_state would have. */
+typedef struct xm_causal_conv1d_attrs {
+    int64_t silu;               /* default 1: y = v sigmoid(v); 0: y = v */
+    int64_t channels_last;      /* default 0: x is [batch, dim, seqlen] */
+    int64_t output_final_state; /* default 0 */
+} xm_causal_conv1d_attrs;
+
+void xm_causal_conv1d_attrs_default(xm_causal_conv1d_attrs *attrs);
+xm_status xm_causal_conv1d_check_attrs(const xm_causal_conv1d_attrs *attrs);
+xm_status xm_causal_conv1d_output_shape(const xm_causal_conv1d_attrs *attrs, const xm_tensor *inputs,
+                                        int32_t n_inputs, int64_t *out_shape, int32_t *out_rank);
+xm_status xm_causal_conv1d_workspace_size(const xm_causal_conv1d_attrs *attrs, const xm_tensor *inputs,
+                                          int32_t n_inputs, size_t *bytes);
+xm_status xm_causal_conv1d_fwd(const xm_causal_conv1d_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                               xm_tensor *output, void *workspace, size_t workspace_bytes, void *cuda_stream);
+
+/* CausalConv1dUpdateFn: CausalConv1dFn for one token per sequence.
+ * Inputs (5, in order): x [batch, dim], weight, bias, state
+ *   [batch or slots, dim, width - 1], state_indices.
+ * Outputs (2): y [batch, dim] and the state with x shifted in. */
+typedef struct xm_causal_conv1d_update_attrs {
+    int64_t silu; /* default 1 */
+} xm_causal_conv1d_update_attrs;
+
+void xm_causal_conv1d_update_attrs_default(xm_causal_conv1d_update_attrs *attrs);
+xm_status xm_causal_conv1d_update_check_attrs(const xm_causal_conv1d_update_attrs *attrs);
+xm_status xm_causal_conv1d_update_output_shape(const xm_causal_conv1d_update_attrs *attrs, const xm_tensor *inputs,
+                                               int32_t n_inputs, int64_t *out_shape, int32_t *out_rank);
+xm_status xm_causal_conv1d_update_workspace_size(const xm_causal_conv1d_update_attrs *attrs,
+                                                 const xm_tensor *inputs, int32_t n_inputs, size_t *bytes);
+xm_status xm_causal_conv1d_update_fwd(const xm_causal_conv1d_update_attrs *attrs, const xm_tensor *inputs,
+                                      int32_t n_inputs, xm_tensor *output, void *workspace, size_t workspace_bytes,
+                                      void *cuda_stream);
+
+/* SelectiveScanVarlenFn: SelectiveScanFn's recurrence over token-major tensors,
+ * continuing given states:
+ *   dt = softplus?(delta + delta_bias), h_n = exp(dt A_n) h_n + dt u B_n,
+ *   y = (D u + sum_n C_n h_n) silu(z).
+ * Inputs (12, in order): u, delta [batch, seqlen, dim], A [dim, d_state], B, C
+ *   [batch, seqlen, d_state] or [batch, seqlen, n_groups, d_state], D [dim] or
+ *   empty, z (u's shape) or empty, delta_bias [dim] or empty, initial_state
+ *   [sequences or slots, dim, d_state] or empty, cu_seqlens, state_indices,
+ *   has_initial_state (as in CausalConv1dFn). d_state 1 to 256.
+ * Outputs: y (u's shape and type; gated whenever z is given, unlike
+ *   SelectiveScanFn's reference quirk); with output_final_state the float32
+ *   state after every sequence's last token (its starting state when it is empty).
+ * The workspace holds the state at the end of each block of tokens where the
+ * sequences are split over the long axis. */
+typedef struct xm_selective_scan_varlen_attrs {
+    int64_t delta_softplus;     /* default 0 */
+    int64_t output_final_state; /* default 0 */
+} xm_selective_scan_varlen_attrs;
+
+void xm_selective_scan_varlen_attrs_default(xm_selective_scan_varlen_attrs *attrs);
+xm_status xm_selective_scan_varlen_check_attrs(const xm_selective_scan_varlen_attrs *attrs);
+xm_status xm_selective_scan_varlen_output_shape(const xm_selective_scan_varlen_attrs *attrs, const xm_tensor *inputs,
+                                                int32_t n_inputs, int64_t *out_shape, int32_t *out_rank);
+xm_status xm_selective_scan_varlen_workspace_size(const xm_selective_scan_varlen_attrs *attrs,
+                                                  const xm_tensor *inputs, int32_t n_inputs, size_t *bytes);
+xm_status xm_selective_scan_varlen_fwd(const xm_selective_scan_varlen_attrs *attrs, const xm_tensor *inputs,
+                                       int32_t n_inputs, xm_tensor *output, void *workspace, size_t workspace_bytes,
+                                       void *cuda_stream);
+
+/* SelectiveStateUpdateFn: SelectiveScanVarlenFn for one token per sequence.
+ * Inputs (10, in order): u, delta [batch, dim], A [dim, d_state], B, C
+ *   [batch, d_state] or [batch, n_groups, d_state], D, z [batch, dim],
+ *   delta_bias (each as above, or empty), state [batch or slots, dim, d_state]
+ *   float32, state_indices.
+ * Outputs (2): y [batch, dim] and the updated state. */
+typedef struct xm_selective_state_update_attrs {
+    int64_t delta_softplus; /* default 0 */
+} xm_selective_state_update_attrs;
+
+void xm_selective_state_update_attrs_default(xm_selective_state_update_attrs *attrs);
+xm_status xm_selective_state_update_check_attrs(const xm_selective_state_update_attrs *attrs);
+xm_status xm_selective_state_update_output_shape(const xm_selective_state_update_attrs *attrs,
+                                                 const xm_tensor *inputs, int32_t n_inputs, int64_t *out_shape,
+                                                 int32_t *out_rank);
+xm_status xm_selective_state_update_workspace_size(const xm_selective_state_update_attrs *attrs,
+                                                   const xm_tensor *inputs, int32_t n_inputs, size_t *bytes);
+xm_status xm_selective_state_update_fwd(const xm_selective_state_update_attrs *attrs, const xm_tensor *inputs,
+                                        int32_t n_inputs, xm_tensor *output, void *workspace, size_t workspace_bytes,
+                                        void *cuda_stream);
+
 /* ---------------------------------------------------------------- SoftmaxCPU
  * Host-memory float32 softmax over `axis` (default -1), replacing
  * SoftmaxCpuKernel::Compute (softmax_cpu_ort.cpp:26-82). Kept so that graphs

@@ -9,6 +9,11 @@ xmetai-onnx-plugins, csrc/register_op.cpp:20-39, domain "xmetai_plugins"):
     GatedDeltaNet2Fn(q, k, v, g, beta, w, initial_state)       gated_deltanet2_fn_ort.cpp
     SoftmaxCPU(input)                                          softmax_cpu_ort.cpp
 
+Around SelectiveScanFn stand the operators that serve such a model, without a
+reference counterpart: CausalConv1dFn and SelectiveScanVarlenFn for prompts
+(packed, continuing cached states), CausalConv1dUpdateFn and
+SelectiveStateUpdateFn for single tokens.
+
 Each function takes the op's inputs in the op's order and its attributes as
 keyword arguments with the op's names and defaults, calls the C ABI of
 libxm_ops.so (include/xm_ops.h) on the current CUDA stream and returns the
@@ -27,6 +32,7 @@ from __future__ import annotations
 import ctypes
 import os
 import pathlib
+import struct
 
 __all__ = [
     "XmError",
@@ -35,13 +41,18 @@ __all__ = [
     "SelectiveScanFn",
     "Mamba3SisoFn",
     "GatedDeltaNet2Fn",
+    "CausalConv1dFn",
+    "CausalConv1dUpdateFn",
+    "SelectiveScanVarlenFn",
+    "SelectiveStateUpdateFn",
     "SoftmaxCPU",
     "DOMAIN",
     "OP_NAMES",
 ]
 
 DOMAIN = "xmetai_plugins"
-OP_NAMES = ("SelectiveScanFn", "Mamba3SisoFn", "GatedDeltaNet2Fn", "SoftmaxCPU")
+OP_NAMES = ("SelectiveScanFn", "Mamba3SisoFn", "GatedDeltaNet2Fn", "SoftmaxCPU", "CausalConv1dFn",
+            "CausalConv1dUpdateFn", "SelectiveScanVarlenFn", "SelectiveStateUpdateFn")
 
 _PKG_DIR = pathlib.Path(__file__).resolve().parent
 MAX_RANK = 8
@@ -102,6 +113,29 @@ class GatedDeltaNet2Attrs(ctypes.Structure):
     ]
 
 
+class CausalConv1dAttrs(ctypes.Structure):
+    _fields_ = [
+        ("silu", ctypes.c_int64),
+        ("channels_last", ctypes.c_int64),
+        ("output_final_state", ctypes.c_int64),
+    ]
+
+
+class CausalConv1dUpdateAttrs(ctypes.Structure):
+    _fields_ = [("silu", ctypes.c_int64)]
+
+
+class SelectiveScanVarlenAttrs(ctypes.Structure):
+    _fields_ = [
+        ("delta_softplus", ctypes.c_int64),
+        ("output_final_state", ctypes.c_int64),
+    ]
+
+
+class SelectiveStateUpdateAttrs(ctypes.Structure):
+    _fields_ = [("delta_softplus", ctypes.c_int64)]
+
+
 _lib = None
 
 
@@ -126,6 +160,10 @@ def load_library() -> ctypes.CDLL:
         "selective_scan": SelectiveScanAttrs,
         "mamba3_siso": Mamba3SisoAttrs,
         "gated_deltanet2": GatedDeltaNet2Attrs,
+        "causal_conv1d": CausalConv1dAttrs,
+        "causal_conv1d_update": CausalConv1dUpdateAttrs,
+        "selective_scan_varlen": SelectiveScanVarlenAttrs,
+        "selective_state_update": SelectiveStateUpdateAttrs,
     }
     for name, attrs in sigs.items():
         f = getattr(lib, f"xm_{name}_fwd")
@@ -372,6 +410,210 @@ def GatedDeltaNet2Fn(q, k, v, g, beta, w, initial_state=None, *, scale: float = 
     sshapes = [(units, q.shape[2], q.shape[3], v.shape[3])] if output_final_state else []
     return _run("gated_deltanet2", attrs, t, io, q.device, stream, out, sshapes,
                 None if final_state is None else [final_state])
+
+
+# ---------------------------------------------------------------- serving operators
+#
+# A decode step calls these for every layer, so their host path is short: one
+# pass over the tensors packs the C descriptors, and validation happens once,
+# in the library.
+
+_TENSOR_BYTES = ctypes.sizeof(XmTensor)
+_PACK = [struct.Struct(f"=Q{r}q{8 * (MAX_RANK - r)}xii") for r in range(MAX_RANK + 1)]
+_ABSENT = _PACK[1]
+
+
+def _invalid(message):
+    raise XmError(XM_ERR_INVALID_ARGUMENT, message)
+
+
+_codes = None
+
+
+def _type_codes():
+    global _codes
+    if _codes is None:
+        import torch
+
+        _codes = {torch.float32: DTYPE_FLOAT, torch.bfloat16: DTYPE_BFLOAT16, torch.float16: DTYPE_FLOAT16,
+                  torch.int32: DTYPE_INT32, torch.int64: DTYPE_INT64}
+    return _codes
+
+
+def _serve(name, attrs, names, tensors, absent, inplace, out, state, state_shape, with_state, workspace, stream):
+    """Call xm_<name>_fwd on the device of tensors[0]. `names` label the tensors, `absent` holds the type codes of
+    absent ones; inplace: index of the state input, which is the default state output (`state`) where state_shape is
+    None and then has to be contiguous (a copy would lose the update). Everything allocated here belongs to the stream
+    the call runs on."""
+    import torch
+
+    lib, codes = load_library(), _type_codes()
+    x = tensors[0]
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        _invalid(f"{names[0]} must be a CUDA tensor")
+    device = x.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _serve(name, attrs, names, tensors, absent, inplace, out, state, state_shape, with_state,
+                          workspace, stream)
+    current = torch.cuda.current_stream()
+    if stream is not None and stream != current:
+        if stream.device != device:
+            _invalid("stream belongs to another device")
+        with torch.cuda.stream(stream):
+            return _serve(name, attrs, names, tensors, absent, inplace, out, state, state_shape, with_state,
+                          workspace, None)
+    n = len(tensors)
+    descs = (XmTensor * n)()
+    keep = []
+    for i, t in enumerate(tensors):
+        if t is None:
+            _ABSENT.pack_into(descs, i * _TENSOR_BYTES, 0, 0, 1, absent[i])
+            continue
+        if not isinstance(t, torch.Tensor) or t.device != device:
+            _invalid(f"{names[i]} must be a tensor on {device}")
+        if not t.is_contiguous():
+            if i == inplace and with_state and state_shape is None:
+                _invalid(f"{names[i]} is updated in place and must be contiguous")
+            t = t.contiguous()
+            keep.append(t)
+        rank = t.dim()
+        if rank > MAX_RANK:
+            _invalid("tensor rank above 8 is not supported")
+        _PACK[rank].pack_into(descs, i * _TENSOR_BYTES, t.data_ptr() if t.numel() else 0, *t.shape, rank,
+                              codes.get(t.dtype, 0))
+    outs = (XmTensor * 2)()
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if with_state and state is None:
+        state = tensors[inplace] if state_shape is None else torch.empty(
+            state_shape, dtype=torch.float32 if absent[inplace] == DTYPE_FLOAT else x.dtype, device=device)
+    for i, t in enumerate((out, state) if with_state else (out,)):
+        label = "out" if i == 0 else "the state output"
+        if not isinstance(t, torch.Tensor) or t.device != device:
+            _invalid(f"{label} must be a tensor on {device}")
+        if not t.is_contiguous():
+            _invalid(f"{label} must be contiguous")
+        rank = t.dim()
+        if rank > MAX_RANK:
+            _invalid("tensor rank above 8 is not supported")
+        _PACK[rank].pack_into(outs, i * _TENSOR_BYTES, t.data_ptr() if t.numel() else 0, *t.shape, rank,
+                              codes.get(t.dtype, 0))
+    ws, ws_bytes = None, 0
+    if workspace:
+        size = ctypes.c_size_t(0)
+        _check(getattr(lib, f"xm_{name}_workspace_size")(ctypes.byref(attrs), descs, n, ctypes.byref(size)))
+        ws_bytes = size.value
+        if ws_bytes:
+            keep.append(torch.empty(ws_bytes, dtype=torch.uint8, device=device))
+            ws = keep[-1].data_ptr()
+    status = getattr(lib, f"xm_{name}_fwd")(ctypes.byref(attrs), descs, n, outs, ws, ws_bytes, current.cuda_stream)
+    if status != XM_OK:
+        _check(status)
+    return (out, state) if with_state else out
+
+
+_CONV_NAMES = ("x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices", "has_initial_state")
+_CONV_UPDATE_NAMES = ("x", "weight", "bias", "state", "state_indices")
+_SCAN_NAMES = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "initial_state", "cu_seqlens", "state_indices",
+               "has_initial_state")
+_UPDATE_NAMES = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "state", "state_indices")
+
+
+def _io_code(x):
+    return _type_codes().get(getattr(x, "dtype", None), 0)
+
+
+def _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state, row):
+    """Shape of the state output that a prompt call allocates; None: the pool itself is the output."""
+    if state_indices is not None or (final_state is not None and final_state is initial_state):
+        return None
+    return (x.shape[0] if cu_seqlens is None else max(0, cu_seqlens.numel() - 1), *row)
+
+
+def CausalConv1dFn(x, weight, bias=None, initial_state=None, cu_seqlens=None, state_indices=None,
+                   has_initial_state=None, *, silu: int = 1, channels_last: int = 0, output_final_state: int = 0,
+                   stream=None, out=None, final_state=None):
+    """Short causal depthwise convolution over prompts: y_t = act(bias + sum_k weight[:, k] x_(t - (width - 1) + k)),
+    with act(v) = v sigmoid(v) (silu=0: identity).
+
+    x: float32, bfloat16 or float16, [batch, dim, seqlen] (SelectiveScanFn's layout), or [batch, seqlen, dim] with
+    channels_last=1 (the layout of SelectiveScanVarlenFn and the other operators). weight [dim, width] (width 2 to 4)
+    and bias [dim] are float32. Without states every sequence starts from zeros.
+
+    initial_state [sequences, dim, width - 1], x's type, holds the inputs before each sequence's first token, oldest
+    first; output_final_state=1 returns (out, final_state) with the last width - 1 inputs of every sequence, which
+    continue it in the next call or in CausalConv1dUpdateFn. cu_seqlens (int32 / int64 offsets [0, ...]) packs
+    sequences into the single batch row; positions behind the last offset are left as they were.
+
+    state_indices (int32 / int64, one per sequence) makes initial_state a pool [slots, dim, width - 1]: sequence i
+    continues row state_indices[i], or starts from zeros where has_initial_state[i] is 0, and with
+    output_final_state=1 its final state replaces that row in place (the result is (out, initial_state)). An index
+    outside the pool owns no row: zeros, and no final state is kept. Slots named twice leave one of the two states.
+    """
+    attrs = CausalConv1dAttrs(int(silu), int(channels_last), int(output_final_state))
+    shape = None
+    if output_final_state:
+        if getattr(x, "ndim", 0) != 3 or getattr(weight, "ndim", 0) != 2:
+            _invalid("x must have rank 3 and weight shape (dim, width)")
+        shape = _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state,
+                                    (x.shape[2 if channels_last else 1], max(0, weight.shape[1] - 1)))
+    return _serve("causal_conv1d", attrs, _CONV_NAMES,
+                  (x, weight, bias, initial_state, cu_seqlens, state_indices, has_initial_state),
+                  (0, 1, 1, _io_code(x), 7, 7, 7), 3, out, final_state, shape,
+                  bool(output_final_state), False, stream)
+
+
+def CausalConv1dUpdateFn(x, weight, bias=None, state=None, state_indices=None, *, silu: int = 1, stream=None,
+                         out=None, new_state=None):
+    """CausalConv1dFn for one token per sequence: x [batch, dim], state [batch, dim, width - 1], or with state_indices
+    a pool [slots, dim, width - 1]. Returns (out, state) with x shifted into the state in place; new_state (without
+    state_indices) receives it instead and leaves `state` as it was. Rows whose index is outside the pool are
+    skipped and their output rows left as they were."""
+    if state is None:
+        _invalid("CausalConv1dUpdateFn needs a state")
+    return _serve("causal_conv1d_update", CausalConv1dUpdateAttrs(int(silu)), _CONV_UPDATE_NAMES,
+                  (x, weight, bias, state, state_indices), (0, 1, 1, 0, 7), 3, out, new_state,
+                  None if new_state is None or new_state is state else (), True, False, stream)
+
+
+def SelectiveScanVarlenFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, initial_state=None, cu_seqlens=None,
+                          state_indices=None, has_initial_state=None, *, delta_softplus: int = 0,
+                          output_final_state: int = 0, stream=None, out=None, final_state=None):
+    """SelectiveScanFn's recurrence over token-major prompts that continue given states:
+    h = exp(dt A) h + dt u B, y = (D u + sum_n C_n h_n) silu(z), dt = softplus?(delta + delta_bias).
+
+    u, delta, z: [batch, seqlen, dim] in float32, bfloat16 or float16; B, C: [batch, seqlen, d_state] or
+    [batch, seqlen, n_groups, d_state]; A [dim, d_state], D, delta_bias [dim] float32. y is gated whenever z is given.
+    initial_state is float32 [sequences, dim, d_state] (SelectiveScanFn's last_state); output_final_state,
+    cu_seqlens, state_indices and has_initial_state work as in CausalConv1dFn.
+    """
+    attrs = SelectiveScanVarlenAttrs(int(delta_softplus), int(output_final_state))
+    shape = None
+    if output_final_state:
+        if getattr(u, "ndim", 0) != 3 or getattr(A, "ndim", 0) != 2:
+            _invalid("u must have rank 3 and A shape (dim, d_state)")
+        shape = _prompt_state_shape(u, cu_seqlens, state_indices, initial_state, final_state,
+                                    (u.shape[2], A.shape[1]))
+    io = _io_code(u)
+    return _serve("selective_scan_varlen", attrs, _SCAN_NAMES,
+                  (u, delta, A, B, C, D, z, delta_bias, initial_state, cu_seqlens, state_indices, has_initial_state),
+                  (0, 0, 1, 0, 0, 1, io, 1, 1, 7, 7, 7), 8, out, final_state, shape, bool(output_final_state), True,
+                  stream)
+
+
+def SelectiveStateUpdateFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, state_indices=None, *,
+                           delta_softplus: int = 0, stream=None, out=None, new_state=None):
+    """SelectiveScanVarlenFn for one token per sequence: u, delta, z [batch, dim], B, C [batch, d_state] or
+    [batch, n_groups, d_state], state float32 [batch, dim, d_state], or with state_indices a pool
+    [slots, dim, d_state]. Returns (out, state) with the state updated in place; new_state (without state_indices)
+    receives it instead. Rows whose index is outside the pool are skipped and their output rows left as they were."""
+    if state is None:
+        _invalid("SelectiveStateUpdateFn needs a state")
+    return _serve("selective_state_update", SelectiveStateUpdateAttrs(int(delta_softplus)), _UPDATE_NAMES,
+                  (u, delta, A, B, C, D, z, delta_bias, state, state_indices),
+                  (0, 0, 1, 0, 0, 1, _io_code(u), 1, 1, 7), 8, out, new_state,
+                  None if new_state is None or new_state is state else (), True, False, stream)
 
 
 def device_wait_failures() -> int:

@@ -570,6 +570,299 @@ M3Plan m3_plan(const xm_mamba3_siso_attrs *attrs, const xm_tensor *in, int32_t n
     return pl;
 }
 
+// ------------------------------------------------------------------ serving operators
+
+// Elements of a tensor, with dimensions bounded so that element and byte
+// offsets fit 64 bits.
+int64_t bounded_elements(const xm_tensor &t, const char *name) {
+    __int128 n = 1;
+    for (int i = 0; i < t.rank; ++i) {
+        if (t.shape[i] > static_cast<int64_t>(INT32_MAX))
+            throw Invalid{std::string(name) + " dimension is out of range"};
+        n *= t.shape[i];
+        if (n > (static_cast<__int128>(1) << 59)) throw Invalid{std::string(name) + " has too many elements"};
+    }
+    return static_cast<int64_t>(n);
+}
+
+size_t element_size(int32_t dtype) {
+    switch (dtype) {
+        case XM_DTYPE_FLOAT16:
+        case XM_DTYPE_BFLOAT16: return 2;
+        case XM_DTYPE_INT64: return 8;
+        default: return 4;
+    }
+}
+
+bool present(const xm_tensor &t) { return elements_of(t) > 0; }
+
+void check_inputs(const xm_tensor *in, int32_t n, int32_t want, const char *const *names, const char *op) {
+    if (in == nullptr || n != want)
+        throw Invalid{std::string(op) + " expects " + std::to_string(want) + " inputs"};
+    for (int i = 0; i < want; ++i) {
+        check_tensor(&in[i], names[i]);
+        bounded_elements(in[i], names[i]);
+    }
+}
+
+bool ranges_overlap(const xm_tensor &a, const xm_tensor &b) {
+    if (!present(a) || !present(b)) return false;
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.data), b0 = reinterpret_cast<uintptr_t>(b.data);
+    const uintptr_t a1 = a0 + static_cast<size_t>(elements_of(a)) * element_size(a.dtype);
+    const uintptr_t b1 = b0 + static_cast<size_t>(elements_of(b)) * element_size(b.dtype);
+    return a0 < b1 && b0 < a1;
+}
+
+// A parameter vector of `n` float32 elements, or absent.
+const float *optional_vector(const xm_tensor &t, int64_t n, const char *name, const char *dim) {
+    require_dtype(t, XM_DTYPE_FLOAT);
+    if (!present(t)) return nullptr;
+    if (shape_of(t) != Shape{n}) throw Invalid{std::string(name) + " must be empty or have shape (" + dim + ")"};
+    return static_cast<const float *>(t.data);
+}
+
+// An int32 or int64 vector of `n` elements, or absent.
+const void *optional_indices(const xm_tensor &t, int64_t n, const char *name, bool *is64) {
+    if (!present(t)) return nullptr;
+    if (t.dtype != XM_DTYPE_INT32 && t.dtype != XM_DTYPE_INT64)
+        throw Invalid{std::string(name) + " must be int32 or int64"};
+    if (shape_of(t) != Shape{n})
+        throw Invalid{std::string(name) + " must be empty or have one element per sequence"};
+    *is64 = t.dtype == XM_DTYPE_INT64;
+    return t.data;
+}
+
+// The sequences of a prompt call from cu_seqlens, state_indices and
+// has_initial_state; n_rows is set by the caller once the state is known.
+xm::SeqArgs sequences_of(int64_t batch, int64_t seqlen, const xm_tensor *cu, const xm_tensor *slots,
+                         const xm_tensor *live, const char *op) {
+    xm::SeqArgs q{};
+    int64_t units = batch;
+    if (cu != nullptr && present(*cu)) {
+        if (cu->dtype != XM_DTYPE_INT64 && cu->dtype != XM_DTYPE_INT32)
+            throw Invalid{"cu_seqlens must be int64 or int32"};
+        const Shape cs = shape_of(*cu);
+        if (cs.size() != 1 || cs[0] < 2) throw Invalid{"cu_seqlens must be 1-D with at least 2 offsets"};
+        if (batch != 1) throw Invalid{std::string(op) + " with cu_seqlens expects batch 1"};
+        units = cs[0] - 1;
+        q.cu = cu->data;
+        q.cu64 = cu->dtype == XM_DTYPE_INT64;
+    }
+    if (batch * seqlen > static_cast<int64_t>(INT32_MAX))
+        throw Unsupported{std::string(op) + " of more than 2^31 - 1 tokens is not supported"};
+    q.units = static_cast<int>(units);
+    q.seqlen = static_cast<int>(seqlen);
+    q.tokens = static_cast<int>(batch * seqlen);
+    q.slots = optional_indices(*slots, units, "state_indices", &q.slots64);
+    if (live != nullptr) q.live = optional_indices(*live, units, "has_initial_state", &q.live64);
+    return q;
+}
+
+// The state input: one row of `row` per sequence, or a pool addressed by
+// state_indices. Sets q.n_rows and returns the state's full shape.
+Shape state_shape_of(xm::SeqArgs &q, const xm_tensor &state, int32_t dtype, const Shape &row, const char *name,
+                     const char *row_text) {
+    Shape want{q.units};
+    want.insert(want.end(), row.begin(), row.end());
+    if (state.dtype != dtype)
+        throw Invalid{std::string(name) + (dtype == XM_DTYPE_FLOAT ? " must be float32" : " must have the type of x")};
+    if (present(state)) {
+        const Shape have = shape_of(state);
+        if (q.slots != nullptr && have.size() == want.size()) want[0] = have[0];
+        if (have != want)
+            throw Invalid{std::string(name) + " must have shape (" + (q.slots != nullptr ? "slots" : "sequences") +
+                          ", " + row_text + ")"};
+    } else if (q.slots != nullptr && row[0] * row[1] > 0) {
+        throw Invalid{std::string("state_indices needs a non-empty ") + name};
+    }
+    q.n_rows = want[0];
+    return want;
+}
+
+// The state output. It may be the state input itself, and is with state_indices.
+void check_state_output(const xm_tensor &out, const xm_tensor &in, const Shape &want, int32_t dtype, bool pool,
+                        const char *name) {
+    check_tensor(&out, name);
+    if (out.dtype != dtype || shape_of(out) != want)
+        throw Invalid{std::string(name) + " must have the shape and type of the state input"};
+    if (pool && out.data != in.data)
+        throw Invalid{std::string(name) + " must be the state input itself when state_indices is given"};
+    if (present(in) && out.data != in.data && ranges_overlap(out, in))
+        throw Invalid{std::string(name) + " must not overlap the state input unless it is the same tensor"};
+}
+
+// No output may overlap an input (except the state pair, `state_in`, which
+// check_state_output decides) or the other output.
+void check_overlap(const xm_tensor *in, int32_t n, int32_t state_in, const xm_tensor *out, int32_t n_out) {
+    for (int o = 0; o < n_out; ++o) {
+        for (int i = 0; i < n; ++i)
+            if (!(o == 1 && i == state_in) && ranges_overlap(out[o], in[i]))
+                throw Invalid{"an output must not overlap an input"};
+        if (o == 1 && ranges_overlap(out[0], out[1])) throw Invalid{"the outputs must not overlap"};
+    }
+}
+
+struct ConvPlan {
+    xm::ConvArgs args;
+    Shape out_shape, state_shape;
+    int32_t io_dtype;
+};
+
+void conv_weights(xm::ConvArgs &a, const xm_tensor &weight, const xm_tensor &bias, int64_t dim) {
+    require_dtype(weight, XM_DTYPE_FLOAT);
+    const Shape ws = shape_of(weight);
+    if (ws.size() != 2 || ws[0] != dim) throw Invalid{"weight must have shape (dim, width)"};
+    if (ws[1] < 2 || ws[1] > 4) throw Unsupported{"causal convolution width must be 2, 3 or 4"};
+    a.width = static_cast<int>(ws[1]);
+    a.dim = static_cast<int>(dim);
+    a.weight = static_cast<const float *>(weight.data);
+    a.bias = optional_vector(bias, dim, "bias", "dim");
+}
+
+ConvPlan conv_plan(const xm_causal_conv1d_attrs *attrs, const xm_tensor *in, int32_t n) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    static const char *const names[7] = {"x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices",
+                                         "has_initial_state"};
+    check_inputs(in, n, 7, names, "CausalConv1dFn");
+    const int32_t io = io_type_of(in[0]);
+    require_dtype(in[0], io);
+    const Shape x = shape_of(in[0]);
+    require_rank(x, 3, "x");
+    const bool last = attrs->channels_last != 0;
+    const int64_t batch = x[0], dim = x[last ? 2 : 1], seqlen = x[last ? 1 : 2];
+    ConvPlan pl{};
+    xm::ConvArgs &a = pl.args;
+    conv_weights(a, in[1], in[2], dim);
+    a.seq = sequences_of(batch, seqlen, &in[4], &in[5], &in[6], "CausalConv1dFn");
+    pl.state_shape =
+        state_shape_of(a.seq, in[3], io, Shape{dim, a.width - 1}, "initial_state", "dim, width - 1");
+    pl.out_shape = x;
+    pl.io_dtype = io;
+    a.silu = attrs->silu != 0;
+    a.channels_last = last;
+    a.io = to_io(io);
+    a.x = in[0].data;
+    a.init = present(in[3]) ? in[3].data : nullptr;
+    return pl;
+}
+
+ConvPlan conv_update_plan(const xm_causal_conv1d_update_attrs *attrs, const xm_tensor *in, int32_t n) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    static const char *const names[5] = {"x", "weight", "bias", "state", "state_indices"};
+    check_inputs(in, n, 5, names, "CausalConv1dUpdateFn");
+    const int32_t io = io_type_of(in[0]);
+    require_dtype(in[0], io);
+    const Shape x = shape_of(in[0]);
+    require_rank(x, 2, "x");
+    ConvPlan pl{};
+    xm::ConvArgs &a = pl.args;
+    conv_weights(a, in[1], in[2], x[1]);
+    a.seq = sequences_of(x[0], 1, nullptr, &in[4], nullptr, "CausalConv1dUpdateFn");
+    pl.state_shape = state_shape_of(a.seq, in[3], io, Shape{x[1], a.width - 1}, "state", "dim, width - 1");
+    if (present(in[0]) && !present(in[3])) throw Invalid{"CausalConv1dUpdateFn needs a non-empty state"};
+    pl.out_shape = x;
+    pl.io_dtype = io;
+    a.silu = attrs->silu != 0;
+    a.channels_last = true;
+    a.io = to_io(io);
+    a.x = in[0].data;
+    a.init = in[3].data;
+    return pl;
+}
+
+struct ScanPlan {
+    xm::ScanArgs args;
+    Shape out_shape, state_shape;
+    int32_t io_dtype;
+};
+
+// u, delta, A, B, C, D, z, delta_bias: in[0..7] of the scan and of its
+// single-token form, whose tensors have `lead` leading dimensions (batch and
+// seqlen, or batch alone).
+void scan_inputs(ScanPlan &pl, const xm_tensor *in, size_t lead) {
+    const int32_t io = io_type_of(in[0]);
+    const int32_t want[8] = {io, io, XM_DTYPE_FLOAT, io, io, XM_DTYPE_FLOAT, io, XM_DTYPE_FLOAT};
+    for (int i = 0; i < 8; ++i) require_dtype(in[i], want[i]);
+    const Shape u = shape_of(in[0]), A = shape_of(in[2]);
+    const std::string rows = lead == 2 ? "(batch, seqlen, " : "(batch, ";
+    require_rank(u, lead + 1, "u");
+    require_same_shape(shape_of(in[1]), u, "delta", "u");
+    const int64_t dim = u[lead];
+    if (A.size() != 2 || A[0] != dim) throw Invalid{"A must have shape (dim, d_state)"};
+    const int64_t dstate = A[1];
+    if (dstate < 1 || dstate > 256) throw Unsupported{"d_state must be 1 to 256"};
+    Shape B = shape_of(in[3]), C = shape_of(in[4]);
+    if (B.size() == lead + 1) B.insert(B.begin() + lead, 1);
+    if (C.size() == lead + 1) C.insert(C.begin() + lead, 1);
+    bool ok = B.size() == lead + 2 && B[lead + 1] == dstate;
+    for (size_t i = 0; ok && i < lead; ++i) ok = B[i] == u[i];
+    if (!ok) throw Invalid{"B must have shape " + rows + "n_groups, d_state)"};
+    if (C != B) throw Invalid{"C shape must match B"};
+    const int64_t groups = B[lead];
+    if (groups <= 0 || dim % groups != 0) throw Invalid{"dim must be divisible by n_groups"};
+    if (present(in[6])) require_same_shape(shape_of(in[6]), u, "z", "u");
+    xm::ScanArgs &a = pl.args;
+    a.D = optional_vector(in[5], dim, "D", "dim");
+    a.bias = optional_vector(in[7], dim, "delta_bias", "dim");
+    a.dim = static_cast<int>(dim);
+    a.dstate = static_cast<int>(dstate);
+    a.groups = static_cast<int>(groups);
+    a.io = to_io(io);
+    a.u = in[0].data;
+    a.delta = in[1].data;
+    a.A = static_cast<const float *>(in[2].data);
+    a.B = in[3].data;
+    a.C = in[4].data;
+    a.z = present(in[6]) ? in[6].data : nullptr;
+    pl.out_shape = u;
+    pl.io_dtype = io;
+}
+
+ScanPlan scan_plan(const xm_selective_scan_varlen_attrs *attrs, const xm_tensor *in, int32_t n) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    static const char *const names[12] = {"u", "delta",      "A",             "B",          "C",             "D",
+                                          "z", "delta_bias", "initial_state", "cu_seqlens", "state_indices",
+                                          "has_initial_state"};
+    check_inputs(in, n, 12, names, "SelectiveScanVarlenFn");
+    ScanPlan pl{};
+    scan_inputs(pl, in, 2);
+    xm::ScanArgs &a = pl.args;
+    a.seq = sequences_of(pl.out_shape[0], pl.out_shape[1], &in[9], &in[10], &in[11], "SelectiveScanVarlenFn");
+    pl.state_shape = state_shape_of(a.seq, in[8], XM_DTYPE_FLOAT, Shape{a.dim, a.dstate}, "initial_state",
+                                    "dim, d_state");
+    a.softplus = attrs->delta_softplus != 0;
+    a.init = present(in[8]) ? static_cast<const float *>(in[8].data) : nullptr;
+    return pl;
+}
+
+ScanPlan state_update_plan(const xm_selective_state_update_attrs *attrs, const xm_tensor *in, int32_t n) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    static const char *const names[10] = {"u", "delta", "A", "B", "C", "D", "z", "delta_bias", "state",
+                                          "state_indices"};
+    check_inputs(in, n, 10, names, "SelectiveStateUpdateFn");
+    ScanPlan pl{};
+    scan_inputs(pl, in, 1);
+    xm::ScanArgs &a = pl.args;
+    a.seq = sequences_of(pl.out_shape[0], 1, nullptr, &in[9], nullptr, "SelectiveStateUpdateFn");
+    pl.state_shape = state_shape_of(a.seq, in[8], XM_DTYPE_FLOAT, Shape{a.dim, a.dstate}, "state", "dim, d_state");
+    if (present(in[0]) && !present(in[8])) throw Invalid{"SelectiveStateUpdateFn needs a non-empty state"};
+    a.softplus = attrs->delta_softplus != 0;
+    a.init = static_cast<const float *>(in[8].data);
+    return pl;
+}
+
+// Output checks shared by the four: y, and the state output where there is one.
+template <typename Plan>
+void serving_outputs(Plan &pl, const xm_tensor *in, int32_t n, int32_t state_in, xm_tensor *output, bool with_state,
+                     int32_t state_dtype, const char *like, const char *state_name) {
+    require_output(output, pl.out_shape, pl.io_dtype, like);
+    if (with_state)
+        check_state_output(output[1], in[state_in], pl.state_shape, state_dtype, pl.args.seq.slots != nullptr,
+                           state_name);
+    check_overlap(in, n, state_in, output, with_state ? 2 : 1);
+    pl.args.out = output->data;
+}
+
 }  // namespace
 
 extern "C" {
@@ -815,6 +1108,186 @@ xm_status xm_gated_deltanet2_fwd_static_ws(const xm_gated_deltanet2_attrs *attrs
         void *scratch = nullptr;
         cudaError_t e = xm::gdn_static_scratch(&scratch);
         if (e == cudaSuccess) e = xm::launch_gated_deltanet2(pl.args, scratch, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_causal_conv1d_attrs_default(xm_causal_conv1d_attrs *a) {
+    if (!a) return;
+    a->silu = 1;
+    a->channels_last = 0;
+    a->output_final_state = 0;
+}
+
+xm_status xm_causal_conv1d_check_attrs(const xm_causal_conv1d_attrs *attrs) {
+    return guarded([&] {
+        if (attrs == nullptr) throw Invalid{"attributes are null"};
+        return XM_OK;
+    });
+}
+
+xm_status xm_causal_conv1d_output_shape(const xm_causal_conv1d_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(conv_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_causal_conv1d_workspace_size(const xm_causal_conv1d_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        conv_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = 0;
+        return XM_OK;
+    });
+}
+
+xm_status xm_causal_conv1d_fwd(const xm_causal_conv1d_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("CausalConv1dFn");
+    (void)workspace;
+    (void)workspace_bytes;
+    return guarded([&] {
+        ConvPlan pl = conv_plan(attrs, inputs, n_inputs);
+        const bool with_state = attrs->output_final_state != 0;
+        serving_outputs(pl, inputs, n_inputs, 3, output, with_state, pl.io_dtype, "x", "final_state");
+        pl.args.final_state = with_state && present(output[1]) ? output[1].data : nullptr;
+        if (!present(*output) && pl.args.final_state == nullptr) return XM_OK;
+        const cudaError_t e = xm::launch_causal_conv1d(pl.args, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_causal_conv1d_update_attrs_default(xm_causal_conv1d_update_attrs *a) {
+    if (!a) return;
+    a->silu = 1;
+}
+
+xm_status xm_causal_conv1d_update_check_attrs(const xm_causal_conv1d_update_attrs *attrs) {
+    return guarded([&] {
+        if (attrs == nullptr) throw Invalid{"attributes are null"};
+        return XM_OK;
+    });
+}
+
+xm_status xm_causal_conv1d_update_output_shape(const xm_causal_conv1d_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(conv_update_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_causal_conv1d_update_workspace_size(const xm_causal_conv1d_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        conv_update_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = 0;
+        return XM_OK;
+    });
+}
+
+xm_status xm_causal_conv1d_update_fwd(const xm_causal_conv1d_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("CausalConv1dUpdateFn");
+    (void)workspace;
+    (void)workspace_bytes;
+    return guarded([&] {
+        ConvPlan pl = conv_update_plan(attrs, inputs, n_inputs);
+        serving_outputs(pl, inputs, n_inputs, 3, output, true, pl.io_dtype, "x", "new_state");
+        pl.args.final_state = output[1].data;
+        if (!present(*output)) return XM_OK;
+        const cudaError_t e = xm::launch_causal_conv1d_update(pl.args, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_selective_scan_varlen_attrs_default(xm_selective_scan_varlen_attrs *a) {
+    if (!a) return;
+    a->delta_softplus = 0;
+    a->output_final_state = 0;
+}
+
+xm_status xm_selective_scan_varlen_check_attrs(const xm_selective_scan_varlen_attrs *attrs) {
+    return guarded([&] {
+        if (attrs == nullptr) throw Invalid{"attributes are null"};
+        return XM_OK;
+    });
+}
+
+xm_status xm_selective_scan_varlen_output_shape(const xm_selective_scan_varlen_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(scan_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_selective_scan_varlen_workspace_size(const xm_selective_scan_varlen_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        const ScanPlan pl = scan_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = xm::scan_varlen_workspace(pl.args);
+        return XM_OK;
+    });
+}
+
+xm_status xm_selective_scan_varlen_fwd(const xm_selective_scan_varlen_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("SelectiveScanVarlenFn");
+    return guarded([&] {
+        ScanPlan pl = scan_plan(attrs, inputs, n_inputs);
+        const bool with_state = attrs->output_final_state != 0;
+        serving_outputs(pl, inputs, n_inputs, 8, output, with_state, XM_DTYPE_FLOAT, "u", "final_state");
+        pl.args.final_state = with_state && present(output[1]) ? static_cast<float *>(output[1].data) : nullptr;
+        if (!present(*output) && pl.args.final_state == nullptr) return XM_OK;
+        require_workspace(workspace, workspace_bytes, xm::scan_varlen_workspace(pl.args));
+        const cudaError_t e = xm::launch_scan_varlen(pl.args, workspace, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_selective_state_update_attrs_default(xm_selective_state_update_attrs *a) {
+    if (!a) return;
+    a->delta_softplus = 0;
+}
+
+xm_status xm_selective_state_update_check_attrs(const xm_selective_state_update_attrs *attrs) {
+    return guarded([&] {
+        if (attrs == nullptr) throw Invalid{"attributes are null"};
+        return XM_OK;
+    });
+}
+
+xm_status xm_selective_state_update_output_shape(const xm_selective_state_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(state_update_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_selective_state_update_workspace_size(const xm_selective_state_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        state_update_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = 0;
+        return XM_OK;
+    });
+}
+
+xm_status xm_selective_state_update_fwd(const xm_selective_state_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("SelectiveStateUpdateFn");
+    (void)workspace;
+    (void)workspace_bytes;
+    return guarded([&] {
+        ScanPlan pl = state_update_plan(attrs, inputs, n_inputs);
+        serving_outputs(pl, inputs, n_inputs, 8, output, true, XM_DTYPE_FLOAT, "u", "new_state");
+        pl.args.final_state = static_cast<float *>(output[1].data);
+        if (!present(*output)) return XM_OK;
+        const cudaError_t e = xm::launch_selective_state_update(pl.args, static_cast<cudaStream_t>(cuda_stream));
         return e == cudaSuccess ? XM_OK : cuda_fail(e);
     });
 }

@@ -110,4 +110,59 @@ cudaError_t m3c_take_wait_failures(unsigned int *count);
 // times out (test hook); 0 disarms.
 void m3c_force_wait_timeout(int launches);
 
+// How the tokens of a call form sequences and which state rows they own
+// (CausalConv1dFn, SelectiveScanVarlenFn and their single-token forms). Tokens
+// are numbered over all batch rows; sequence i holds the tokens of batch row i,
+// or with cu the tokens [cu[i], cu[i + 1]) of the single row.
+struct SeqArgs {
+    int units;   // sequences
+    int seqlen;  // tokens of a batch row
+    int tokens;  // batch * seqlen
+    const void *cu;  // units + 1 offsets, or null
+    bool cu64;
+    const void *slots;  // state row of each sequence, or null: row i
+    bool slots64;
+    long long n_rows;  // rows of the state tensors
+    const void *live;  // 0: the sequence starts from zeros; or null
+    bool live64;
+};
+
+// Short causal convolution. The states are [n_rows, dim, width - 1] of the I/O
+// type; init and final may be the same memory.
+struct ConvArgs {
+    SeqArgs seq;
+    int dim, width;
+    bool silu, channels_last;
+    IoType io;
+    const void *x;
+    const float *weight, *bias;  // bias may be null
+    const void *init;            // or null
+    void *final_state;           // or null
+    void *out;
+};
+cudaError_t launch_causal_conv1d(const ConvArgs &a, cudaStream_t stream);
+// One token per sequence: x, out [units, dim]; init and final_state both given.
+cudaError_t launch_causal_conv1d_update(const ConvArgs &a, cudaStream_t stream);
+
+// Selective scan over token-major tensors ([tokens, dim], [tokens, groups,
+// dstate]). The states are float32 [n_rows, dim, dstate]; init and final may be
+// the same memory.
+struct ScanArgs {
+    SeqArgs seq;
+    int dim, dstate, groups;
+    bool softplus;
+    IoType io;
+    const void *u, *delta, *z;  // z may be null
+    const void *B, *C;
+    const float *A, *D, *bias;  // D, bias may be null
+    const float *init;          // or null
+    float *final_state;         // or null
+    void *out;
+};
+size_t scan_varlen_workspace(const ScanArgs &a);
+// `workspace` must hold scan_varlen_workspace(a) bytes, 256-byte aligned.
+cudaError_t launch_scan_varlen(const ScanArgs &a, void *workspace, cudaStream_t stream);
+// One token per sequence: u, delta, z, out [units, dim]; init and final_state both given.
+cudaError_t launch_selective_state_update(const ScanArgs &a, cudaStream_t stream);
+
 }  // namespace xm
