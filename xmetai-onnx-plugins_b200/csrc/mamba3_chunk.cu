@@ -52,7 +52,6 @@ constexpr int kC = 128;        // tokens per chunk (MMA M)
 constexpr int kThreads = 256;  // two threads per TMEM lane (halves of the columns)
 constexpr float kPi = 3.14159265358979323846f;
 constexpr float kTwoPi = 2.0f * kPi;
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct M3cDev {
     int T, H, G, P, A;

@@ -22,6 +22,32 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return y;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// softplus(x) = max(x, 0) + log1p(t), t = exp(-|x|) in (0, 1], on a pair of
+// values. log1p(t) = t q(t) with q a degree-8 polynomial fitted to log1p(t)/t
+// on [0, 1] in relative error (my own least-squares fit on Chebyshev nodes:
+// 3e-8 model error, 2e-7 after float32 Horner), so the only MUFU work is the
+// two ex2. t q(t) keeps full relative precision as t -> 0, and for x > 20
+// the correction is below half an ulp of x, so the result equals x there as
+// in the reference (selective_scan_fwd_kernel.cuh:156-159).
+__device__ __forceinline__ float2 softplus_pair(float2 x) {
+    const float2 t = make_float2(ex2_approx(-fabsf(x.x) * kLog2e), ex2_approx(-fabsf(x.y) * kLog2e));
+    constexpr float c[9] = {0.9999999403953552f, -0.4999949336051941f, 0.3331909775733948f,
+                            -0.2484298199415207f, 0.19106005132198334f, -0.13663242757320404f,
+                            0.07822591066360474f, -0.029505213722586632f, 0.0052326880395412445f};
+    float2 q = __ffma2_rn(t, make_float2(c[8], c[8]), make_float2(c[7], c[7]));
+#pragma unroll
+    for (int i = 6; i >= 0; --i) q = __ffma2_rn(t, q, make_float2(c[i], c[i]));
+    return __ffma2_rn(t, q, make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+}
+
 // Element conversion between the I/O dtype and float.
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
