@@ -420,7 +420,6 @@ def GatedDeltaNet2Fn(q, k, v, g, beta, w, initial_state=None, *, scale: float = 
 
 _TENSOR_BYTES = ctypes.sizeof(XmTensor)
 _PACK = [struct.Struct(f"=Q{r}q{8 * (MAX_RANK - r)}xii") for r in range(MAX_RANK + 1)]
-_ABSENT = _PACK[1]
 
 
 def _invalid(message):
@@ -440,88 +439,108 @@ def _type_codes():
     return _codes
 
 
-def _serve(name, attrs, names, tensors, absent, inplace, out, state, state_shape, with_state, workspace, stream):
-    """Call xm_<name>_fwd on the device of tensors[0]. `names` label the tensors, `absent` holds the type codes of
-    absent ones; inplace: index of the state input, which is the default state output (`state`) where state_shape is
-    None and then has to be contiguous (a copy would lose the update). Everything allocated here belongs to the stream
-    the call runs on."""
+class _ServeOp:
+    """What the calls of one serving operator share: its C entries, the tensors' names and the index of the state
+    input. `kinds` has a letter per input: x (the activations' type), f (float32) or i (int32 / int64)."""
+
+    def __init__(self, name, names, kinds, state, workspace=False):
+        self.name, self.names, self.kinds, self.state, self.workspace = name, names, kinds, state, workspace
+        self.fwd = self.array = None
+        self.blank = {}
+
+    def load(self):
+        lib = load_library()
+        self.size = getattr(lib, f"xm_{self.name}_workspace_size")
+        self.array = XmTensor * len(self.names)
+        for io in (0, *_type_codes().values()):
+            descs = self.array()
+            for i, k in enumerate(self.kinds):
+                descs[i].rank, descs[i].dtype = 1, {"x": io, "f": DTYPE_FLOAT, "i": DTYPE_INT64}[k]
+            self.blank[io] = bytes(descs)  # every input absent
+        self.fwd = getattr(lib, f"xm_{self.name}_fwd")
+
+
+_OUTS = XmTensor * 2
+
+
+def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
+    """Call xm_<op>_fwd on the device of tensors[0]. The state output is `state`, a new tensor of state_shape, or
+    (state_shape None) the state input itself, which then has to be contiguous: a copy would lose the update.
+    Everything allocated here belongs to the stream that the call runs on."""
     import torch
 
-    lib, codes = load_library(), _type_codes()
+    if op.fwd is None:
+        op.load()
+    Tensor, codes = torch.Tensor, _type_codes()
     x = tensors[0]
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        _invalid(f"{names[0]} must be a CUDA tensor")
-    device = x.device
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _serve(name, attrs, names, tensors, absent, inplace, out, state, state_shape, with_state,
-                          workspace, stream)
-    current = torch.cuda.current_stream()
-    if stream is not None and stream != current:
-        if stream.device != device:
+    index = x.get_device() if isinstance(x, Tensor) else -1
+    if index < 0:
+        _invalid(f"{op.names[0]} must be a CUDA tensor")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _serve(op, attrs, tensors, out, state, state_shape, with_state, stream)
+    handle = torch._C._cuda_getCurrentRawStream(index)
+    if stream is not None and stream.cuda_stream != handle:
+        if stream.device_index != index:
             _invalid("stream belongs to another device")
         with torch.cuda.stream(stream):
-            return _serve(name, attrs, names, tensors, absent, inplace, out, state, state_shape, with_state,
-                          workspace, None)
-    n = len(tensors)
-    descs = (XmTensor * n)()
-    keep = []
+            return _serve(op, attrs, tensors, out, state, state_shape, with_state, None)
+    descs = op.array.from_buffer_copy(op.blank[codes.get(x.dtype, 0)])
+    keep = None
+    at = 0
     for i, t in enumerate(tensors):
-        if t is None:
-            _ABSENT.pack_into(descs, i * _TENSOR_BYTES, 0, 0, 1, absent[i])
-            continue
-        if not isinstance(t, torch.Tensor) or t.device != device:
-            _invalid(f"{names[i]} must be a tensor on {device}")
-        if not t.is_contiguous():
-            if i == inplace and with_state and state_shape is None:
-                _invalid(f"{names[i]} is updated in place and must be contiguous")
-            t = t.contiguous()
-            keep.append(t)
-        rank = t.dim()
-        if rank > MAX_RANK:
-            _invalid("tensor rank above 8 is not supported")
-        _PACK[rank].pack_into(descs, i * _TENSOR_BYTES, t.data_ptr() if t.numel() else 0, *t.shape, rank,
-                              codes.get(t.dtype, 0))
-    outs = (XmTensor * 2)()
+        if t is not None:
+            if not isinstance(t, Tensor) or t.get_device() != index:
+                _invalid(f"{op.names[i]} must be a tensor on cuda:{index}")
+            if not t.is_contiguous():
+                if i == op.state and with_state and state_shape is None:
+                    _invalid(f"{op.names[i]} is updated in place and must be contiguous")
+                t = t.contiguous()
+                keep = (keep, t)
+            shape = t.shape
+            rank = len(shape)
+            if rank > MAX_RANK:
+                _invalid("tensor rank above 8 is not supported")
+            _PACK[rank].pack_into(descs, at, t.data_ptr(), *shape, rank, codes.get(t.dtype, 0))
+        at += _TENSOR_BYTES
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if with_state and state is None:
-        state = tensors[inplace] if state_shape is None else torch.empty(
-            state_shape, dtype=torch.float32 if absent[inplace] == DTYPE_FLOAT else x.dtype, device=device)
-    for i, t in enumerate((out, state) if with_state else (out,)):
-        label = "out" if i == 0 else "the state output"
-        if not isinstance(t, torch.Tensor) or t.device != device:
-            _invalid(f"{label} must be a tensor on {device}")
-        if not t.is_contiguous():
-            _invalid(f"{label} must be contiguous")
-        rank = t.dim()
+        state = tensors[op.state] if state_shape is None else torch.empty(
+            state_shape, dtype=torch.float32 if op.kinds[op.state] == "f" else x.dtype, device=x.device)
+    outs = _OUTS()
+    at = 0
+    for t in (out, state) if with_state else (out,):
+        if not isinstance(t, Tensor) or t.get_device() != index or not t.is_contiguous():
+            _invalid(f"{'out' if at == 0 else 'the state output'} must be a contiguous tensor on cuda:{index}")
+        shape = t.shape
+        rank = len(shape)
         if rank > MAX_RANK:
             _invalid("tensor rank above 8 is not supported")
-        _PACK[rank].pack_into(outs, i * _TENSOR_BYTES, t.data_ptr() if t.numel() else 0, *t.shape, rank,
-                              codes.get(t.dtype, 0))
+        _PACK[rank].pack_into(outs, at, t.data_ptr(), *shape, rank, codes.get(t.dtype, 0))
+        at += _TENSOR_BYTES
+    attrs = ctypes.byref(attrs)
     ws, ws_bytes = None, 0
-    if workspace:
+    if op.workspace:
         size = ctypes.c_size_t(0)
-        _check(getattr(lib, f"xm_{name}_workspace_size")(ctypes.byref(attrs), descs, n, ctypes.byref(size)))
+        _check(op.size(attrs, descs, len(descs), ctypes.byref(size)))
         ws_bytes = size.value
         if ws_bytes:
-            keep.append(torch.empty(ws_bytes, dtype=torch.uint8, device=device))
-            ws = keep[-1].data_ptr()
-    status = getattr(lib, f"xm_{name}_fwd")(ctypes.byref(attrs), descs, n, outs, ws, ws_bytes, current.cuda_stream)
+            scratch = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+            ws = scratch.data_ptr()
+    status = op.fwd(attrs, descs, len(descs), outs, ws, ws_bytes, handle)
     if status != XM_OK:
         _check(status)
     return (out, state) if with_state else out
 
 
-_CONV_NAMES = ("x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices", "has_initial_state")
-_CONV_UPDATE_NAMES = ("x", "weight", "bias", "state", "state_indices")
-_SCAN_NAMES = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "initial_state", "cu_seqlens", "state_indices",
-               "has_initial_state")
-_UPDATE_NAMES = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "state", "state_indices")
-
-
-def _io_code(x):
-    return _type_codes().get(getattr(x, "dtype", None), 0)
+_CONV = _ServeOp("causal_conv1d", ("x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices",
+                                    "has_initial_state"), "xffxiii", 3)
+_CONV_UPDATE = _ServeOp("causal_conv1d_update", ("x", "weight", "bias", "state", "state_indices"), "xffxi", 3)
+_SCAN = _ServeOp("selective_scan_varlen", ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "initial_state",
+                                           "cu_seqlens", "state_indices", "has_initial_state"), "xxfxxfxffiii", 8, True)
+_UPDATE = _ServeOp("selective_state_update", ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "state",
+                                              "state_indices"), "xxfxxfxffi", 8)
 
 
 def _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state, row):
@@ -558,10 +577,8 @@ def CausalConv1dFn(x, weight, bias=None, initial_state=None, cu_seqlens=None, st
             _invalid("x must have rank 3 and weight shape (dim, width)")
         shape = _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state,
                                     (x.shape[2 if channels_last else 1], max(0, weight.shape[1] - 1)))
-    return _serve("causal_conv1d", attrs, _CONV_NAMES,
-                  (x, weight, bias, initial_state, cu_seqlens, state_indices, has_initial_state),
-                  (0, 1, 1, _io_code(x), 7, 7, 7), 3, out, final_state, shape,
-                  bool(output_final_state), False, stream)
+    return _serve(_CONV, attrs, (x, weight, bias, initial_state, cu_seqlens, state_indices, has_initial_state), out,
+                  final_state, shape, bool(output_final_state), stream)
 
 
 def CausalConv1dUpdateFn(x, weight, bias=None, state=None, state_indices=None, *, silu: int = 1, stream=None,
@@ -572,9 +589,8 @@ def CausalConv1dUpdateFn(x, weight, bias=None, state=None, state_indices=None, *
     skipped and their output rows left as they were."""
     if state is None:
         _invalid("CausalConv1dUpdateFn needs a state")
-    return _serve("causal_conv1d_update", CausalConv1dUpdateAttrs(int(silu)), _CONV_UPDATE_NAMES,
-                  (x, weight, bias, state, state_indices), (0, 1, 1, 0, 7), 3, out, new_state,
-                  None if new_state is None or new_state is state else (), True, False, stream)
+    return _serve(_CONV_UPDATE, CausalConv1dUpdateAttrs(int(silu)), (x, weight, bias, state, state_indices), out,
+                  new_state, None if new_state is None or new_state is state else (), True, stream)
 
 
 def SelectiveScanVarlenFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, initial_state=None, cu_seqlens=None,
@@ -595,11 +611,8 @@ def SelectiveScanVarlenFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, in
             _invalid("u must have rank 3 and A shape (dim, d_state)")
         shape = _prompt_state_shape(u, cu_seqlens, state_indices, initial_state, final_state,
                                     (u.shape[2], A.shape[1]))
-    io = _io_code(u)
-    return _serve("selective_scan_varlen", attrs, _SCAN_NAMES,
-                  (u, delta, A, B, C, D, z, delta_bias, initial_state, cu_seqlens, state_indices, has_initial_state),
-                  (0, 0, 1, 0, 0, 1, io, 1, 1, 7, 7, 7), 8, out, final_state, shape, bool(output_final_state), True,
-                  stream)
+    return _serve(_SCAN, attrs, (u, delta, A, B, C, D, z, delta_bias, initial_state, cu_seqlens, state_indices,
+                                 has_initial_state), out, final_state, shape, bool(output_final_state), stream)
 
 
 def SelectiveStateUpdateFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, state_indices=None, *,
@@ -610,10 +623,9 @@ def SelectiveStateUpdateFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, s
     receives it instead. Rows whose index is outside the pool are skipped and their output rows left as they were."""
     if state is None:
         _invalid("SelectiveStateUpdateFn needs a state")
-    return _serve("selective_state_update", SelectiveStateUpdateAttrs(int(delta_softplus)), _UPDATE_NAMES,
-                  (u, delta, A, B, C, D, z, delta_bias, state, state_indices),
-                  (0, 0, 1, 0, 0, 1, _io_code(u), 1, 1, 7), 8, out, new_state,
-                  None if new_state is None or new_state is state else (), True, False, stream)
+    return _serve(_UPDATE, SelectiveStateUpdateAttrs(int(delta_softplus)),
+                  (u, delta, A, B, C, D, z, delta_bias, state, state_indices), out, new_state,
+                  None if new_state is None or new_state is state else (), True, stream)
 
 
 def device_wait_failures() -> int:
