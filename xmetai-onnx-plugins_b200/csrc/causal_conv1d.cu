@@ -36,6 +36,68 @@ __device__ __forceinline__ float conv_act(float v, bool silu) {
     return silu ? v * rcp_approx(1.0f + ex2_approx(-v * kLog2e)) : v;
 }
 
+// y[i] = act(b[i] + sum_k w[k][i] x_k[i]) over V values, in pairs (FFMA2) where V is even.
+template <int V, int W>
+__device__ __forceinline__ void conv_values(float (&y)[V], const float (&b)[V], const float (&w)[W][V],
+                                            const float (&x)[W][V], bool silu) {
+    if constexpr (V == 1) {
+        y[0] = b[0];
+#pragma unroll
+        for (int k = 0; k < W; ++k) y[0] = fmaf(w[k][0], x[k][0], y[0]);
+        y[0] = conv_act(y[0], silu);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            float2 v = make_float2(b[i], b[i + 1]);
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+                v = __ffma2_rn(make_float2(w[k][i], w[k][i + 1]), make_float2(x[k][i], x[k][i + 1]), v);
+            if (silu) {
+                const float2 t = __fmul2_rn(v, make_float2(-kLog2e, -kLog2e));
+                const float2 e = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.0f, 1.0f));
+                v = __fmul2_rn(v, make_float2(rcp_approx(e.x), rcp_approx(e.y)));
+            }
+            y[i] = v.x;
+            y[i + 1] = v.y;
+        }
+    }
+}
+
+// Weights and bias of channels [d, d + V), weights by tap. `words`: both 16-byte aligned.
+template <int V, int W>
+__device__ __forceinline__ void conv_load_weights(const ConvArgs &p, int d, bool words, float (&w)[W][V], float (&b)[V]) {
+    const float *src = p.weight + static_cast<size_t>(d) * W;
+    float flat[V * W];
+    if (V > 1 && words) {
+#pragma unroll
+        for (int i = 0; i + 4 <= V * W; i += 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4 *>(src + i));
+            flat[i] = v.x; flat[i + 1] = v.y; flat[i + 2] = v.z; flat[i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V * W; ++i) flat[i] = __ldg(src + i);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) w[k][i] = flat[i * W + k];
+        b[i] = 0.0f;
+    }
+    if (p.bias != nullptr) {
+        if (V > 1 && words) {
+#pragma unroll
+            for (int i = 0; i + 4 <= V; i += 4) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(p.bias + d + i));
+                b[i] = v.x; b[i + 1] = v.y; b[i + 2] = v.z; b[i + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) b[i] = __ldg(p.bias + d + i);
+        }
+    }
+}
+
 // Channels or tokens of one 16-byte word.
 template <typename T>
 constexpr int kWord = 16 / static_cast<int>(sizeof(T));
@@ -112,7 +174,7 @@ constexpr int kAheadTokens = 4;  // tokens whose loads are issued together
 // Thread: V channels from channel V * (blockIdx.x * threads + thread); blockIdx.y:
 // the block of `block` tokens. Each thread walks the sequences that meet it.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArgs p, int block, int nblocks) {
+__global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArgs p, int block, int nblocks, bool words) {
     const SeqArgs &q = p.seq;
     const int d = (blockIdx.x * kConvThreads + threadIdx.x) * V;
     if (d >= p.dim) return;
@@ -120,12 +182,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArg
     const T *const x = static_cast<const T *>(p.x) + d;
     T *const out = static_cast<T *>(p.out) + d;
     float w[W][V], b[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-#pragma unroll
-        for (int k = 0; k < W; ++k) w[k][i] = p.weight[static_cast<size_t>(d + i) * W + k];
-        b[i] = p.bias != nullptr ? p.bias[d + i] : 0.0f;
-    }
+    conv_load_weights<V, W>(p, d, words, w, b);
     for (int blk = blockIdx.y; blk < nblocks; blk += gridDim.y) {
         const int t0 = blk * block, t1 = t0 + min(block, q.tokens - t0);
         const bool last = blk == nblocks - 1;
@@ -164,13 +221,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArg
 #pragma unroll
                     for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
                 r.floats(win[W - 1]);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    y[i] = b[i];
-#pragma unroll
-                    for (int k = 0; k < W; ++k) y[i] = fmaf(w[k][i], win[k][i], y[i]);
-                    y[i] = conv_act(y[i], p.silu);
-                }
+                conv_values<V, W>(y, b, w, win, p.silu);
                 store_elems<T, V>(out + static_cast<size_t>(t) * D, y);
             };
             int t = from;
@@ -218,172 +269,208 @@ __global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArg
 
 // ------------------------------------------------------------------ channels first
 
-constexpr int kWordsPerThread = 4;  // words whose loads are issued together
+constexpr int kRuns = 4;  // runs of 32 words whose loads are issued together
+
+// One row of a [rows, seqlen] x: its channel, its sequences and their states.
+template <typename T, int W>
+struct ConvRow {
+    const ConvArgs &p;
+    const T *x;
+    T *out;
+    int ch, first;    // channel; number of the row's first token
+    int n, n_end;     // dense: the batch row's sequence
+    float w[W], b;
+
+    __device__ __forceinline__ ConvRow(const ConvArgs &args, long long row, long long batch, int channel)
+        : p(args), x(static_cast<const T *>(args.x) + row * args.seq.seqlen),
+          out(static_cast<T *>(args.out) + row * args.seq.seqlen), ch(channel) {
+        const bool packed = p.seq.cu != nullptr;
+        first = packed ? 0 : static_cast<int>(batch) * p.seq.seqlen;
+        n = packed ? 0 : static_cast<int>(batch);
+        n_end = packed ? p.seq.units : n + 1;
+#pragma unroll
+        for (int k = 0; k < W; ++k) w[k] = __ldg(p.weight + static_cast<size_t>(ch) * W + k);
+        b = p.bias != nullptr ? __ldg(p.bias + ch) : 0.0f;
+    }
+    __device__ __forceinline__ int begin(int i) const { return seq_start(p.seq, i) - first; }
+    __device__ __forceinline__ T state_at(long long row, int k) const {
+        return static_cast<const T *>(p.init)[(static_cast<size_t>(row) * p.dim + ch) * (W - 1) + k];
+    }
+    __device__ __forceinline__ bool live(int i, long long row) const { return p.init != nullptr && seq_live(p.seq, i, row); }
+    // The final state of sequence i = tokens [s, e) of the row.
+    __device__ __forceinline__ void finish(int s, int e, long long row, bool alive) const {
+        if (p.final_state == nullptr || row < 0) return;
+        T keep[W - 1];
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) {
+            const int at = e - (W - 1) + k;
+            if (at >= s) keep[k] = x[at];
+            else keep[k] = alive ? state_at(row, W - 1 + at - s) : from_f32<T>(0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k)
+            static_cast<T *>(p.final_state)[(static_cast<size_t>(row) * p.dim + ch) * (W - 1) + k] = keep[k];
+    }
+    // Tokens [t0, t1) of the row, sequence by sequence and token by token.
+    __device__ __forceinline__ void walk(int t0, int t1) const {
+        const int L = p.seq.seqlen;
+        int i = p.seq.cu != nullptr ? max(0, conv_first_from(p.seq, t0) - 1) : n;
+        for (; i < n_end; ++i) {
+            const int s = begin(i);
+            if (s >= t1 && t1 < L) break;
+            const int e = max(s, begin(i + 1));
+            const bool own = s >= t0;  // these tokens hold the sequence's first one
+            const int from = own ? s : max(t0, min(e, s + W - 1));
+            const int to = own ? max(min(e, t1), min(e, s + W - 1)) : min(e, t1);
+            const long long row = own ? seq_row(p.seq, i) : -1;
+            const bool alive = own && live(i, row);
+            for (int t = from; t < to; ++t) {
+                float y = b;
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    const int at = t - (W - 1) + k;
+                    const float in = at >= s ? to_f32<T>(x[at]) : alive ? to_f32<T>(state_at(row, W - 1 + at - s)) : 0.0f;
+                    y = fmaf(w[k], in, y);
+                }
+                out[t] = from_f32<T>(conv_act(y, p.silu));
+            }
+            if (own) finish(s, e, row, alive);
+        }
+    }
+};
+
+// Elements [f, end) of the flat x, row by row from (row, batch, ch, c).
+template <typename T, int W>
+__device__ __noinline__ void conv_any(const ConvArgs &p, long long f, long long end, long long row, long long batch,
+                                      unsigned ch, unsigned c) {
+    const unsigned L = p.seq.seqlen;
+    while (f < end) {
+        const int count = static_cast<int>(min(end - f, static_cast<long long>(L - c)));
+        const ConvRow<T, W> r(p, row, batch, static_cast<int>(ch));
+        r.walk(static_cast<int>(c), static_cast<int>(c) + count);
+        f += count;
+        ++row;
+        c = 0;
+        if (++ch == static_cast<unsigned>(p.dim) && p.seq.cu == nullptr) {
+            ch = 0;
+            ++batch;
+        }
+    }
+}
 
 // x as a flat [rows * seqlen] array, row = batch * dim + channel (or the channel,
-// packed). A warp takes kWordsPerThread runs of 32 words. `skew`: elements between
-// x's address and the 16-byte boundary below; words are counted from there.
+// packed). A warp takes kRuns runs of 32 words. A run that lies in one sequence
+// (or starts a dense row) goes word by word, each lane taking the W - 1 inputs
+// before its word from its neighbour; the others token by token. `skew`: elements
+// between x's address and the 16-byte boundary below; words are counted from there.
 template <typename T, int W>
 __global__ void __launch_bounds__(kConvThreads) conv_channels_kernel(const ConvArgs p, long long total, int skew,
                                                                        bool vec, long long items) {
     constexpr int V = kWord<T>;
+    constexpr int kRun = 32 * V;
     const SeqArgs &q = p.seq;
-    const int lane = threadIdx.x & 31, L = q.seqlen;
+    const int lane = threadIdx.x & 31;
+    const unsigned L = q.seqlen;
+    const bool packed = q.cu != nullptr;
     const T *const x = static_cast<const T *>(p.x);
-    T *const out = static_cast<T *>(p.out);
     for (long long item = static_cast<long long>(blockIdx.x) * (kConvThreads / 32) + (threadIdx.x >> 5); item < items;
          item += static_cast<long long>(gridDim.x) * (kConvThreads / 32)) {
-        const long long base = item * (32 * kWordsPerThread);  // the run's first word
-        // Row, channel and token of the run's first element; its words add a 32-bit offset to them.
-        const long long base0 = max(base * V - skew, 0LL);
-        const long long row_0 = base0 / L, batch_0 = q.cu != nullptr ? 0 : row_0 / p.dim;
+        const long long f_item = item * (kRun * kRuns) - skew;  // the item's first element
+        uint4 raw[kRuns], before = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < kRuns; ++m) {
+            const long long f0 = f_item + m * kRun + lane * V;
+            raw[m] = make_uint4(0, 0, 0, 0);
+            if (vec && f0 >= 0 && f0 + V <= total) raw[m] = __ldg(reinterpret_cast<const uint4 *>(x + f0));
+        }
+        if (vec && lane == 0 && f_item >= V && f_item <= total)
+            before = __ldg(reinterpret_cast<const uint4 *>(x + f_item - V));
+        // Row, channel and token of the item's first element; its runs add a 32-bit offset to them.
+        const long long base0 = max(f_item, 0LL);
+        const bool small = total <= 0xffffffffLL;
+        const long long row_0 = small ? static_cast<unsigned>(base0) / L : base0 / L;
+        const long long batch_0 = packed ? 0 : small ? static_cast<unsigned>(row_0) / static_cast<unsigned>(p.dim) : row_0 / p.dim;
         const unsigned c_0 = static_cast<unsigned>(base0 - row_0 * L);
         const unsigned ch_0 = static_cast<unsigned>(row_0 - batch_0 * p.dim);
-        uint4 raw[kWordsPerThread];
+        float tail[W - 1];  // lane 0: the inputs before the run's first word
+        {
+            float v[V];
+            word_floats<T>(before, v);
 #pragma unroll
-        for (int m = 0; m < kWordsPerThread; ++m) {
-            const long long f0 = (base + 32 * m + lane) * V - skew;
-            raw[m] = make_uint4(0, 0, 0, 0);
-            if (vec && f0 >= 0 && f0 + V <= total) {
-                raw[m] = __ldg(reinterpret_cast<const uint4 *>(x + f0));
-            } else if (f0 < total && f0 + V > 0) {
-                uint32_t e[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    e[i] = 0u;
-                    if (f0 + i >= 0 && f0 + i < total) {
-                        if constexpr (sizeof(T) == 4) e[i] = __float_as_uint(x[f0 + i]);
-                        else e[i] = reinterpret_cast<const unsigned short *>(x)[f0 + i];
-                    }
-                }
-                if constexpr (sizeof(T) == 4) raw[m] = make_uint4(e[0], e[1], e[2], e[3]);
-                else raw[m] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-            }
+            for (int k = 0; k < W - 1; ++k) tail[k] = v[V - (W - 1) + k];
         }
 #pragma unroll
-        for (int m = 0; m < kWordsPerThread; ++m) {
-            const long long f0 = (base + 32 * m + lane) * V - skew;
-            float v[V + W - 1];  // the W - 1 inputs before the word, then its own
-            float own_v[V];
+        for (int m = 0; m < kRuns; ++m) {
+            float own_v[V], hist[W - 1];
             word_floats<T>(raw[m], own_v);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[W - 1 + i] = own_v[i];
-#pragma unroll
             for (int k = 0; k < W - 1; ++k) {
-                v[k] = __shfl_up_sync(kFullMask, own_v[V - (W - 1) + k], 1);
-                if (lane == 0) {
-                    const long long at = f0 - (W - 1) + k;
-                    v[k] = at >= 0 && at < total ? to_f32<T>(x[at]) : 0.0f;
-                }
+                const float r = __shfl_sync(kFullMask, own_v[V - (W - 1) + k], (lane + 31) & 31);
+                hist[k] = lane == 0 ? tail[k] : r;
+                tail[k] = r;  // lane 0: lane 31's, which the next run's first word follows
             }
-            if (f0 >= total || f0 + V <= 0) continue;
-            const long long lo = max(f0, 0LL), hi = min(f0 + V, total);
-            unsigned c = c_0 + static_cast<unsigned>(lo - base0), ch = ch_0;
-            long long r = row_0, batch = batch_0;
-            if (c >= static_cast<unsigned>(L)) {
-                const unsigned rows = c / static_cast<unsigned>(L);
-                c -= rows * static_cast<unsigned>(L);
-                r += rows;
-                ch += rows;
-                if (q.cu == nullptr && ch >= static_cast<unsigned>(p.dim)) {
-                    const unsigned more = ch / static_cast<unsigned>(p.dim);
-                    batch += more;
-                    ch -= more * static_cast<unsigned>(p.dim);
+            const long long f_run = f_item + m * kRun;
+            if (f_run >= total) break;
+            auto place = [&](long long f, long long &row, long long &batch, unsigned &ch, unsigned &c) {
+                c = c_0 + static_cast<unsigned>(f - base0);
+                ch = ch_0;
+                row = row_0;
+                batch = batch_0;
+                if (c >= L) {
+                    const unsigned rows = c / L;
+                    c -= rows * L;
+                    row += rows;
+                    ch += rows;
+                    if (!packed && ch >= static_cast<unsigned>(p.dim)) {
+                        const unsigned more = ch / static_cast<unsigned>(p.dim);
+                        batch += more;
+                        ch -= more * static_cast<unsigned>(p.dim);
+                    }
                 }
+            };
+            long long row, batch;
+            unsigned ch, c;
+            place(max(f_run, 0LL), row, batch, ch, c);
+            // the run's sequence [s, e) of the row: dense rows are one
+            int n = static_cast<int>(batch), s = 0, e = static_cast<int>(L);
+            if (packed) {
+                n = conv_first_from(q, static_cast<int>(c) + 1) - 1;
+                s = n >= 0 ? seq_start(q, n) : 0;
+                e = n >= 0 ? seq_end(q, n, s) : 0;
             }
-            // Row by row (one, unless rows are shorter than a word).
-            for (long long f = lo; f < hi;) {
-                const int count = static_cast<int>(min(hi - f, static_cast<long long>(L) - c));  // its tokens here
-                const int tb = static_cast<int>(batch) * L;  // number of the row's first token (0 where packed)
-                const T *const xr = x + r * L;
-                T *const yr = out + r * L;
-                float w[W];
+            const int t0 = static_cast<int>(c), t1 = t0 + min(kRun, INT_MAX - t0);
+            if (vec && f_run >= 0 && f_run + kRun <= total && c + kRun <= L &&
+                (packed ? t0 - s >= W - 1 && e > t1 : t0 == 0 || t0 >= W - 1)) {
+                const ConvRow<T, W> r(p, row, batch, static_cast<int>(ch));
+                long long srow = -1;
+                bool alive = false;
+                if (t0 == s && lane == 0) {  // a dense row's start
+                    srow = seq_row(q, n);
+                    alive = r.live(n, srow);
 #pragma unroll
-                for (int k = 0; k < W; ++k) w[k] = __ldg(p.weight + static_cast<size_t>(ch) * W + k);
-                const float b = p.bias != nullptr ? __ldg(p.bias + ch) : 0.0f;
-                const int t0 = static_cast<int>(c), t1 = t0 + count;
-                // sequences of the row: dense rows have one, the batch's
-                int n = q.cu != nullptr ? conv_first_from(q, t0) : static_cast<int>(batch);
-                const int n_end = q.cu != nullptr ? q.units : n + 1;
-                if (q.cu != nullptr && n > 0) --n;
-                auto begin = [&](int i) { return seq_start(q, i) - tb; };
-                auto state_of = [&](int i, bool &live) {
-                    const long long row = seq_row(q, i);
-                    live = p.init != nullptr && seq_live(q, i, row);
-                    return row;
-                };
-                auto state_at = [&](long long row, int k) {
-                    return static_cast<const T *>(p.init)[(static_cast<size_t>(row) * p.dim + ch) * (W - 1) + k];
-                };
-                auto finish = [&](int i, int s, int e, long long row, bool live) {
-                    if (p.final_state == nullptr || row < 0) return;
-                    T keep[W - 1];
+                    for (int k = 0; k < W - 1; ++k) hist[k] = alive ? to_f32<T>(r.state_at(srow, k)) : 0.0f;
+                }
+                float y[V], in[W][V], ww[W][V], bb[V];
 #pragma unroll
-                    for (int k = 0; k < W - 1; ++k) {
-                        const int at = e - (W - 1) + k;
-                        if (at >= s) keep[k] = xr[at];
-                        else keep[k] = live ? state_at(row, W - 1 + at - s) : from_f32<T>(0.0f);
-                    }
+                for (int i = 0; i < V; ++i) {
+                    bb[i] = r.b;
 #pragma unroll
-                    for (int k = 0; k < W - 1; ++k)
-                        static_cast<T *>(p.final_state)[(static_cast<size_t>(row) * p.dim + ch) * (W - 1) + k] = keep[k];
-                };
-                const int s0 = n < n_end ? begin(n) : INT_MAX;
-                const int e0 = n < n_end ? max(s0, begin(n + 1)) : INT_MAX;
-                if (vec && count == V && e0 >= t1 && s0 <= t0 && (s0 == t0 || t0 - s0 >= W - 1) &&
-                    (q.cu == nullptr || (s0 < t0 && e0 > t1))) {
-                    // the whole word in one sequence, all its inputs here (or its state at the row's start)
-                    bool live = false;
-                    long long row = -1;
-                    if (s0 == t0) {
-                        row = state_of(n, live);
-#pragma unroll
-                        for (int k = 0; k < W - 1; ++k) v[k] = live ? to_f32<T>(state_at(row, k)) : 0.0f;
-                    }
-                    float y[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        y[i] = b;
-#pragma unroll
-                        for (int k = 0; k < W; ++k) y[i] = fmaf(w[k], v[i + k], y[i]);
-                        y[i] = conv_act(y[i], p.silu);
-                    }
-                    *reinterpret_cast<uint4 *>(yr + t0) = floats_word<T>(y);
-                    if (s0 == t0) finish(n, s0, e0, row, live);
-                } else {
-                    // sequence by sequence and token by token
-                    for (; n < n_end; ++n) {
-                        const int s = begin(n);
-                        if (s >= t1 && t1 < L) break;
-                        const int e = max(s, begin(n + 1));
-                        const bool own = s >= t0;  // this word holds the sequence's first token
-                        if (own && s >= t1 && s < L) break;
-                        if (s < 0) continue;
-                        const int from = own ? s : max(t0, min(e, s + W - 1));
-                        const int to = own ? max(min(e, t1), min(e, s + W - 1)) : min(e, t1);
-                        bool live = false;
-                        const long long row = own ? state_of(n, live) : -1;
-                        for (int t = from; t < to; ++t) {
-                            float y = b;
-#pragma unroll
-                            for (int k = 0; k < W; ++k) {
-                                const int at = t - (W - 1) + k;
-                                const float in = at >= s ? to_f32<T>(xr[at])
-                                                         : live ? to_f32<T>(state_at(row, W - 1 + at - s)) : 0.0f;
-                                y = fmaf(w[k], in, y);
-                            }
-                            yr[t] = from_f32<T>(conv_act(y, p.silu));
-                        }
-                        if (own) finish(n, s, e, row, live);
+                    for (int k = 0; k < W; ++k) {
+                        const int at = i + k - (W - 1);
+                        in[k][i] = at < 0 ? hist[at < 0 ? at + W - 1 : 0] : own_v[at < 0 ? 0 : at];
+                        ww[k][i] = r.w[k];
                     }
                 }
-                f += count;
-                ++r;
-                c = 0;
-                if (++ch == static_cast<unsigned>(p.dim) && q.cu == nullptr) {
-                    ch = 0;
-                    ++batch;
+                conv_values<V, W>(y, bb, ww, in, p.silu);
+                *reinterpret_cast<uint4 *>(r.out + t0 + lane * V) = floats_word<T>(y);
+                if (t0 == s && lane == 0) r.finish(s, e, srow, alive);
+            } else {
+                const long long lo = max(f_run + lane * V, 0LL), hi = min(f_run + (lane + 1) * V, total);
+                if (lo < hi) {
+                    place(lo, row, batch, ch, c);
+                    conv_any<T, W>(p, lo, hi, row, batch, ch, c);
                 }
+                __syncwarp();
             }
         }
     }
@@ -394,7 +481,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_channels_kernel(const ConvA
 // Thread: V channels, kRows sequences (loads issued together; the weights are
 // read once for all).
 template <typename T, int V, int W, int kRows>
-__global__ void __launch_bounds__(kConvThreads) conv_token_kernel(const ConvArgs p) {
+__global__ void __launch_bounds__(kConvThreads) conv_token_kernel(const ConvArgs p, bool words) {
     constexpr int S = V * (W - 1);  // state elements of the thread's channels in a row
     const int d = (blockIdx.x * kConvThreads + threadIdx.x) * V;
     if (d >= p.dim) return;
@@ -412,13 +499,8 @@ __global__ void __launch_bounds__(kConvThreads) conv_token_kernel(const ConvArgs
 #pragma unroll
             for (int k = 0; k < W - 1; ++k) s[r][k].load(from + k * V);
         }
-        float w[V][W], b[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-#pragma unroll
-            for (int k = 0; k < W; ++k) w[i][k] = __ldg(p.weight + static_cast<size_t>(d + i) * W + k);
-            b[i] = p.bias != nullptr ? __ldg(p.bias + d + i) : 0.0f;
-        }
+        float w[W][V], b[V];
+        conv_load_weights<V, W>(p, d, words, w, b);
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             if (row[r] < 0) continue;
@@ -432,16 +514,17 @@ __global__ void __launch_bounds__(kConvThreads) conv_token_kernel(const ConvArgs
                 for (int i = 0; i < V; ++i) old[k * V + i] = part[i];
             }
             float now[S];  // the state, x shifted in (exact: the values round back to what they were)
+            float win[W][V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                y[i] = b[i];
 #pragma unroll
                 for (int k = 0; k < W - 1; ++k) {
-                    y[i] = fmaf(w[i][k], old[i * (W - 1) + k], y[i]);
+                    win[k][i] = old[i * (W - 1) + k];
                     now[i * (W - 1) + k] = k + 1 < W - 1 ? old[i * (W - 1) + k + 1] : xv[i];
                 }
-                y[i] = conv_act(fmaf(w[i][W - 1], xv[i], y[i]), p.silu);
+                win[W - 1][i] = xv[i];
             }
+            conv_values<V, W>(y, b, w, win, p.silu);
             T *to = static_cast<T *>(p.final_state) + (static_cast<size_t>(row[r]) * D + d) * (W - 1);
 #pragma unroll
             for (int k = 0; k < W - 1; ++k) {
@@ -475,7 +558,7 @@ cudaError_t launch_tokens(const ConvArgs &a, cudaStream_t stream) {
     while (block > 4 && groups * ((a.seq.tokens + block - 1) / block) < 4 * sms) block /= 2;
     const int nblocks = std::max(1, static_cast<int>((static_cast<int64_t>(a.seq.tokens) + block - 1) / block));
     const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(std::min(nblocks, 65535)));
-    conv_tokens_kernel<T, V, W><<<grid, kConvThreads, 0, stream>>>(a, block, nblocks);
+    conv_tokens_kernel<T, V, W><<<grid, kConvThreads, 0, stream>>>(a, block, nblocks, aligned16(a.weight) && aligned16(a.bias));
     return cudaGetLastError();
 }
 
@@ -486,7 +569,7 @@ cudaError_t launch_channels(const ConvArgs &a, cudaStream_t stream) {
         (a.seq.cu != nullptr ? 1LL : static_cast<long long>(a.seq.units)) * a.dim * static_cast<long long>(a.seq.seqlen);
     const auto at = [](const void *p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T)); };
     const int skew = at(a.x);
-    const long long words = (total + skew + V - 1) / V, items = (words + 32 * kWordsPerThread - 1) / (32 * kWordsPerThread);
+    const long long words = (total + skew + V - 1) / V, items = (words + 32 * kRuns - 1) / (32 * kRuns);
     const long long blocks = (items + kConvThreads / 32 - 1) / (kConvThreads / 32);
     conv_channels_kernel<T, W><<<static_cast<unsigned>(std::min(blocks, 1LL << 30)), kConvThreads, 0, stream>>>(
         a, total, skew, at(a.out) == skew, items);
@@ -509,13 +592,14 @@ cudaError_t launch_token(const ConvArgs &a, cudaStream_t stream) {
     const int64_t blocks = (static_cast<int64_t>(a.dim) + V * kConvThreads - 1) / (V * kConvThreads);
     const int64_t groups = (static_cast<int64_t>(a.seq.units) + 3) / 4;
     const unsigned gx = static_cast<unsigned>(blocks);
+    const bool words = aligned16(a.weight) && aligned16(a.bias);
     // Four sequences per thread where that leaves each SM four blocks.
     if (blocks * groups >= 4LL * current_device_sm_count())
         conv_token_kernel<T, V, W, 4>
-            <<<dim3(gx, static_cast<unsigned>(std::min<int64_t>(groups, 65535))), kConvThreads, 0, stream>>>(a);
+            <<<dim3(gx, static_cast<unsigned>(std::min<int64_t>(groups, 65535))), kConvThreads, 0, stream>>>(a, words);
     else
         conv_token_kernel<T, V, W, 1>
-            <<<dim3(gx, static_cast<unsigned>(std::min(a.seq.units, 65535))), kConvThreads, 0, stream>>>(a);
+            <<<dim3(gx, static_cast<unsigned>(std::min(a.seq.units, 65535))), kConvThreads, 0, stream>>>(a, words);
     return cudaGetLastError();
 }
 
