@@ -15,11 +15,11 @@
 //   conv_token_kernel     one token per sequence: a thread owns the channels of
 //                         one word, their state and their weights.
 //
-// Where sequences are cut, over blocks of tokens or words, one thread does all
-// that touches a sequence's state of a channel: the one at the sequence's first
-// token. It computes the first W - 1 tokens, which alone see the starting state,
-// even where they reach into the next block or word, and then stores the final
-// state. So in-place states are safe and need no second launch.
+// The states may be updated in place. With tokens first, one thread does all that
+// touches a sequence's state of a channel: the one whose block holds the
+// sequence's first token. It computes the first W - 1 tokens, which alone see the
+// starting state, even where they reach into the next block, and then stores the
+// final state. With channels first a small second launch stores it.
 #include <algorithm>
 #include <climits>
 
@@ -286,7 +286,18 @@ __global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArg
 
 // ------------------------------------------------------------------ channels first
 
-constexpr int kRuns = 4;  // runs of 32 words whose loads are issued together
+// The state that sequence n of channel ch starts from (zeros where it starts anew).
+template <typename T, int W>
+__device__ __noinline__ float4 conv_start(const ConvArgs &p, int n, int ch) {
+    float f[3] = {0.0f, 0.0f, 0.0f};
+    const long long row = seq_row(p.seq, n);
+    if (seq_live(p.seq, n, row)) {
+        const T *s = static_cast<const T *>(p.init) + (static_cast<size_t>(row) * p.dim + ch) * (W - 1);
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) f[k] = to_f32<T>(s[k]);
+    }
+    return make_float4(f[0], f[1], f[2], 0.0f);
+}
 
 // One row of a [rows, seqlen] x: its channel, its sequences and their states.
 template <typename T, int W>
@@ -294,77 +305,92 @@ struct ConvRow {
     const ConvArgs &p;
     const T *x;
     T *out;
-    int ch, first;    // channel; number of the row's first token
-    int n, n_end;     // dense: the batch row's sequence
+    int ch;  // channel
+    int n0;  // dense: the batch row's sequence
     float w[W], b;
 
-    __device__ __forceinline__ ConvRow(const ConvArgs &args, long long row, long long batch, int channel)
-        : p(args), x(static_cast<const T *>(args.x) + row * args.seq.seqlen),
-          out(static_cast<T *>(args.out) + row * args.seq.seqlen), ch(channel) {
-        const bool packed = p.seq.cu != nullptr;
-        first = packed ? 0 : static_cast<int>(batch) * p.seq.seqlen;
-        n = packed ? 0 : static_cast<int>(batch);
-        n_end = packed ? p.seq.units : n + 1;
+    __device__ __forceinline__ ConvRow(const ConvArgs &args, long long row, long long batch, unsigned channel) : p(args) {
+        take(row, batch, channel);
+    }
+    __device__ __forceinline__ void take(long long row, long long batch, unsigned channel) {
+        x = static_cast<const T *>(p.x) + row * p.seq.seqlen;
+        out = static_cast<T *>(p.out) + row * p.seq.seqlen;
+        ch = static_cast<int>(channel);
+        n0 = p.seq.cu != nullptr ? 0 : static_cast<int>(batch);
 #pragma unroll
         for (int k = 0; k < W; ++k) w[k] = __ldg(p.weight + static_cast<size_t>(ch) * W + k);
         b = p.bias != nullptr ? __ldg(p.bias + ch) : 0.0f;
     }
-    __device__ __forceinline__ int begin(int i) const { return seq_start(p.seq, i) - first; }
-    __device__ __forceinline__ T state_at(long long row, int k) const {
-        return static_cast<const T *>(p.init)[(static_cast<size_t>(row) * p.dim + ch) * (W - 1) + k];
-    }
-    __device__ __forceinline__ bool live(int i, long long row) const { return p.init != nullptr && seq_live(p.seq, i, row); }
-    // The final state of sequence i = tokens [s, e) of the row.
-    __device__ __forceinline__ void finish(int s, int e, long long row, bool alive) const {
-        if (p.final_state == nullptr || row < 0) return;
-        T keep[W - 1];
+    // The W - 1 inputs before sequence n's first token: its state, or zeros.
+    __device__ __forceinline__ void start_of(int n, float (&h)[W - 1]) const {
+        const float4 v = p.init != nullptr ? conv_start<T, W>(p, n, ch) : make_float4(0, 0, 0, 0);
+        const float f[3] = {v.x, v.y, v.z};
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) {
-            const int at = e - (W - 1) + k;
-            if (at >= s) keep[k] = x[at];
-            else keep[k] = alive ? state_at(row, W - 1 + at - s) : from_f32<T>(0.0f);
-        }
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k)
-            static_cast<T *>(p.final_state)[(static_cast<size_t>(row) * p.dim + ch) * (W - 1) + k] = keep[k];
-    }
-    // Tokens [t0, t1) of the row, sequence by sequence and token by token.
-    __device__ __forceinline__ void walk(int t0, int t1) const {
-        const int L = p.seq.seqlen;
-        int i = p.seq.cu != nullptr ? max(0, conv_first_from(p.seq, t0) - 1) : n;
-        for (; i < n_end; ++i) {
-            const int s = begin(i);
-            if (s >= t1 && t1 < L) break;
-            const int e = max(s, begin(i + 1));
-            const bool own = s >= t0;  // these tokens hold the sequence's first one
-            const int from = own ? s : max(t0, min(e, s + W - 1));
-            const int to = own ? max(min(e, t1), min(e, s + W - 1)) : min(e, t1);
-            const long long row = own ? seq_row(p.seq, i) : -1;
-            const bool alive = own && live(i, row);
-            for (int t = from; t < to; ++t) {
-                float y = b;
-#pragma unroll
-                for (int k = 0; k < W; ++k) {
-                    const int at = t - (W - 1) + k;
-                    const float in = at >= s ? to_f32<T>(x[at]) : alive ? to_f32<T>(state_at(row, W - 1 + at - s)) : 0.0f;
-                    y = fmaf(w[k], in, y);
-                }
-                out[t] = from_f32<T>(conv_act(y, p.silu));
-            }
-            if (own) finish(s, e, row, alive);
-        }
+        for (int k = 0; k < W - 1; ++k) h[k] = f[k];
     }
 };
 
-// Elements [f, end) of the flat x, row by row from (row, batch, ch, c).
+// The sequence [s, e) of a row that holds a token; n outside [0, units): none.
+struct ConvSpan {
+    int n, s, e;
+    __device__ __forceinline__ void find(const SeqArgs &q, int t, int dense) {
+        if (q.cu == nullptr) {
+            n = dense, s = 0, e = q.seqlen;
+            return;
+        }
+        n = conv_first_from(q, t + 1) - 1;  // the last one that starts at or before t
+        s = n >= 0 ? seq_start(q, n) : 0;
+        e = n >= 0 ? seq_end(q, n, s) : 0;
+    }
+    __device__ __forceinline__ bool holds(int t) const { return n >= 0 && t >= s && t < e; }
+};
+
+// The W - 1 inputs before token t of sequence q, from the state where they lie before it.
+template <typename T, int W>
+__device__ __forceinline__ void conv_history(const ConvRow<T, W> &r, const ConvSpan &q, int t, float (&h)[W - 1]) {
+    if (!q.holds(t)) return;
+    float st[W - 1];
+    if (t - q.s < W - 1) r.start_of(q.n, st);
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+        const int at = t - (W - 1) + k;
+        if (at >= q.s) {
+            h[k] = to_f32<T>(r.x[at]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < W - 1; ++i)
+                if (W - 1 + at - q.s == i) h[k] = st[i];
+        }
+    }
+}
+
+// Elements [f, end) of the flat x, token by token from (row, batch, ch, c).
 template <typename T, int W>
 __device__ __noinline__ void conv_any(const ConvArgs &p, long long f, long long end, long long row, long long batch,
                                       unsigned ch, unsigned c) {
     const unsigned L = p.seq.seqlen;
     while (f < end) {
         const int count = static_cast<int>(min(end - f, static_cast<long long>(L - c)));
-        const ConvRow<T, W> r(p, row, batch, static_cast<int>(ch));
-        r.walk(static_cast<int>(c), static_cast<int>(c) + count);
+        const ConvRow<T, W> r(p, row, batch, ch);
+        ConvSpan q;
+        q.find(p.seq, static_cast<int>(c), r.n0);
+        float h[W - 1];
+        conv_history<T, W>(r, q, static_cast<int>(c), h);
+        for (int t = static_cast<int>(c); t < static_cast<int>(c) + count; ++t) {
+            if (t >= q.e) {
+                q.find(p.seq, t, r.n0);
+                conv_history<T, W>(r, q, t, h);
+            }
+            if (!q.holds(t)) continue;
+            const float in = to_f32<T>(r.x[t]);
+            float y = r.b;
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) y = fmaf(r.w[k], h[k], y);
+            r.out[t] = from_f32<T>(conv_act(fmaf(r.w[W - 1], in, y), p.silu));
+#pragma unroll
+            for (int k = 0; k + 2 < W; ++k) h[k] = h[k + 1];
+            h[W - 2] = in;
+        }
         f += count;
         ++row;
         c = 0;
@@ -376,11 +402,14 @@ __device__ __noinline__ void conv_any(const ConvArgs &p, long long f, long long 
 }
 
 // x as a flat [rows * seqlen] array, row = batch * dim + channel (or the channel,
-// packed). A warp takes kRuns runs of 32 words. A run that lies in one sequence
-// (or starts a dense row) goes word by word, each lane taking the W - 1 inputs
-// before its word from its neighbour; the others token by token. `skew`: elements
-// between x's address and the 16-byte boundary below; words are counted from there.
-template <typename T, int W>
+// packed). A warp takes an item of kRuns runs of 32 words, loaded together; a lane
+// takes the W - 1 inputs before its word from its neighbour lane. Items inside one
+// sequence do nothing else; in the others every lane looks up its word's row and
+// sequences, and a word that crosses into another row or sequence masks its taps.
+// Words that are not whole, and rows shorter than a word, go token by token.
+// `skew`: elements between x's address and the 16-byte boundary below; words are
+// counted from there. States are only read here; conv_final_kernel stores them.
+template <typename T, int W, int kRuns>
 __global__ void __launch_bounds__(kConvThreads) conv_channels_kernel(const ConvArgs p, long long total, int skew,
                                                                        bool vec, long long items) {
     constexpr int V = kWord<T>;
@@ -402,11 +431,12 @@ __global__ void __launch_bounds__(kConvThreads) conv_channels_kernel(const ConvA
         }
         if (vec && lane == 0 && f_item >= V && f_item <= total)
             before = __ldg(reinterpret_cast<const uint4 *>(x + f_item - V));
-        // Row, channel and token of the item's first element; its runs add a 32-bit offset to them.
+        // Row, channel and token of the item's first element; its words add a 32-bit offset to them.
         const long long base0 = max(f_item, 0LL);
         const bool small = total <= 0xffffffffLL;
         const long long row_0 = small ? static_cast<unsigned>(base0) / L : base0 / L;
-        const long long batch_0 = packed ? 0 : small ? static_cast<unsigned>(row_0) / static_cast<unsigned>(p.dim) : row_0 / p.dim;
+        const long long batch_0 =
+            packed ? 0 : small ? static_cast<unsigned>(row_0) / static_cast<unsigned>(p.dim) : row_0 / p.dim;
         const unsigned c_0 = static_cast<unsigned>(base0 - row_0 * L);
         const unsigned ch_0 = static_cast<unsigned>(row_0 - batch_0 * p.dim);
         float tail[W - 1];  // lane 0: the inputs before the run's first word
@@ -415,86 +445,79 @@ __global__ void __launch_bounds__(kConvThreads) conv_channels_kernel(const ConvA
             word_floats<T>(before, v);
 #pragma unroll
             for (int k = 0; k < W - 1; ++k) tail[k] = v[V - (W - 1) + k];
+            if (lane == 0 && skew > 0 && f_item > 0 && f_item < V) {  // the word before is cut by x's begin
+#pragma unroll
+                for (int k = 0; k < W - 1; ++k) {
+                    const long long at = f_item - (W - 1) + k;
+                    if (at >= 0 && at < total) tail[k] = to_f32<T>(x[at]);
+                }
+            }
         }
-        // the sequence [s, e) of the item's row around its first element: dense rows are one
-        auto sequence = [&](unsigned c, long long batch, int &n, int &s, int &e) {
-            n = static_cast<int>(batch), s = 0, e = static_cast<int>(L);
-            if (packed) {
-                n = conv_first_from(q, static_cast<int>(c) + 1) - 1;
-                s = n >= 0 ? seq_start(q, n) : 0;
-                e = n >= 0 ? seq_end(q, n, s) : 0;
+        // A run's inputs: the lane's own and the W - 1 before them.
+        auto run_inputs = [&](const uint4 &word, float (&v)[V + W - 1]) {
+            float own[V];
+            word_floats<T>(word, own);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[W - 1 + i] = own[i];
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) {
+                const float r = __shfl_sync(kFullMask, own[V - (W - 1) + k], (lane + 31) & 31);
+                v[k] = lane == 0 ? tail[k] : r;
+                tail[k] = r;  // lane 0: lane 31's, which the next run's first word follows
             }
         };
-        // Words [t0 + lane V, + V) of row r, which starts with lane 0's word when `start` (state of sequence n).
-        auto run_words = [&](const ConvRow<T, W> &r, int t0, bool start, int n, int e, const float (&own_v)[V],
-                             float (&hist)[W - 1]) {
-            long long srow = -1;
-            bool alive = false;
-            if (start && lane == 0) {
-                srow = seq_row(q, n);
-                alive = r.live(n, srow);
-#pragma unroll
-                for (int k = 0; k < W - 1; ++k) hist[k] = alive ? to_f32<T>(r.state_at(srow, k)) : 0.0f;
-            }
-            float y[V], in[W][V], ww[W][V], bb[V];
+        auto word_values = [&](const ConvRow<T, W> &r, const float (&v)[V + W - 1], float (&y)[V]) {
+            float in[W][V], ww[W][V], bb[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 bb[i] = r.b;
 #pragma unroll
                 for (int k = 0; k < W; ++k) {
-                    const int at = i + k - (W - 1);
-                    in[k][i] = at < 0 ? hist[at < 0 ? at + W - 1 : 0] : own_v[at < 0 ? 0 : at];
+                    in[k][i] = v[i + k];
                     ww[k][i] = r.w[k];
                 }
             }
             conv_values<V, W>(y, bb, ww, in, p.silu);
-            *reinterpret_cast<uint4 *>(r.out + t0 + lane * V) = floats_word<T>(y);
-            if (start && lane == 0) r.finish(0, e, srow, alive);
         };
         if (vec && f_item >= 0 && f_item + kRuns * kRun <= total && static_cast<uint64_t>(c_0) + kRuns * kRun <= L) {
-            int n, s, e;
-            sequence(c_0, batch_0, n, s, e);
-            const int t0 = static_cast<int>(c_0), t1 = t0 + kRuns * kRun;
-            if (packed ? t0 - s >= W - 1 && e > t1 : t0 == 0 || t0 >= W - 1) {
-                // the whole item in one sequence
-                const ConvRow<T, W> r(p, row_0, batch_0, static_cast<int>(ch_0));
+            const ConvRow<T, W> r(p, row_0, batch_0, ch_0);
+            const int t0 = static_cast<int>(c_0);
+            ConvSpan span;
+            span.find(q, t0, r.n0);
+            if (span.holds(t0) && t0 + kRuns * kRun <= span.e && (t0 == span.s || t0 - span.s >= W - 1)) {
 #pragma unroll
                 for (int m = 0; m < kRuns; ++m) {
-                    float own_v[V], hist[W - 1];
-                    word_floats<T>(raw[m], own_v);
+                    float v[V + W - 1], y[V];
+                    run_inputs(raw[m], v);
+                    if (m == 0 && t0 == span.s && lane == 0) {
+                        float h[W - 1];
+                        r.start_of(span.n, h);
 #pragma unroll
-                    for (int k = 0; k < W - 1; ++k) {
-                        const float v = __shfl_sync(kFullMask, own_v[V - (W - 1) + k], (lane + 31) & 31);
-                        hist[k] = lane == 0 ? tail[k] : v;
-                        tail[k] = v;  // lane 0: lane 31's, which the next run's first word follows
+                        for (int k = 0; k < W - 1; ++k) v[k] = h[k];
                     }
-                    run_words(r, t0 + m * kRun, !packed && m == 0 && t0 == 0, n, e, own_v, hist);
+                    word_values(r, v, y);
+                    *reinterpret_cast<uint4 *>(r.out + t0 + m * kRun + lane * V) = floats_word<T>(y);
                 }
                 continue;
             }
         }
-        // run by run (not unrolled: this code is rarely used and would crowd the instruction cache)
+        // word by word (not unrolled: this code would crowd the instruction cache)
+        ConvRow<T, W> r(p, row_0, batch_0, ch_0);
+        ConvSpan span{-1, 0, 0};
+        long long row_held = row_0;
 #pragma unroll 1
         for (int m = 0; m < kRuns; ++m) {
-            float own_v[V], hist[W - 1];
             uint4 word = raw[0];
 #pragma unroll
             for (int i = 1; i < kRuns; ++i)
                 if (m == i) word = raw[i];
-            word_floats<T>(word, own_v);
-#pragma unroll
-            for (int k = 0; k < W - 1; ++k) {
-                const float r = __shfl_sync(kFullMask, own_v[V - (W - 1) + k], (lane + 31) & 31);
-                hist[k] = lane == 0 ? tail[k] : r;
-                tail[k] = r;
-            }
-            const long long f_run = f_item + m * kRun;
-            if (f_run >= total) break;
-            auto place = [&](long long f, long long &row, long long &batch, unsigned &ch, unsigned &c) {
-                c = c_0 + static_cast<unsigned>(f - base0);
-                ch = ch_0;
-                row = row_0;
-                batch = batch_0;
+            float v[V + W - 1], y[V];
+            run_inputs(word, v);
+            const long long f0 = f_item + m * kRun + lane * V;
+            const long long lo = max(f0, 0LL), hi = min(f0 + V, total);
+            if (lo < hi) {
+                unsigned c = c_0 + static_cast<unsigned>(lo - base0), ch = ch_0;
+                long long row = row_0, batch = batch_0;
                 if (c >= L) {
                     const unsigned rows = c / L;
                     c -= rows * L;
@@ -506,26 +529,101 @@ __global__ void __launch_bounds__(kConvThreads) conv_channels_kernel(const ConvA
                         ch -= more * static_cast<unsigned>(p.dim);
                     }
                 }
-            };
-            long long row, batch;
-            unsigned ch, c;
-            place(max(f_run, 0LL), row, batch, ch, c);
-            int n, s, e;
-            sequence(c, batch, n, s, e);
-            const int t0 = static_cast<int>(c), t1 = t0 + min(kRun, INT_MAX - t0);
-            if (vec && f_run >= 0 && f_run + kRun <= total && static_cast<uint64_t>(c) + kRun <= L &&
-                (packed ? t0 - s >= W - 1 && e > t1 : t0 == 0 || t0 >= W - 1)) {
-                const ConvRow<T, W> r(p, row, batch, static_cast<int>(ch));
-                run_words(r, t0, !packed && t0 == 0, n, e, own_v, hist);
-            } else {
-                const long long lo = max(f_run + lane * V, 0LL), hi = min(f_run + (lane + 1) * V, total);
-                if (lo < hi) {
-                    place(lo, row, batch, ch, c);
+                if (!vec || lo != f0 || hi != f0 + V || L < V) {
                     conv_any<T, W>(p, lo, hi, row, batch, ch, c);
+                } else {
+                    if (row != row_held) {
+                        r.take(row, batch, ch);
+                        row_held = row;
+                        span.e = 0;
+                    }
+                    const int t0 = static_cast<int>(c);
+                    if (!span.holds(t0)) span.find(q, t0, r.n0);
+                    if (span.holds(t0) && t0 + V <= span.e && t0 - span.s >= W - 1) {
+                        word_values(r, v, y);
+                        *reinterpret_cast<uint4 *>(r.out + t0) = floats_word<T>(y);
+                    } else {
+                        // At most two rows: token by token in registers, the window taken from the state at
+                        // each sequence's start.
+                        const int here = static_cast<int>(min(static_cast<unsigned>(V), L - c));
+                        T *const to = static_cast<T *>(p.out) + f0;
+                        unsigned held = 0;
+                        float h[W - 1];
+#pragma unroll
+                        for (int k = 0; k < W - 1; ++k) h[k] = v[k];
+                        const int into = t0 - span.s;  // tokens of the sequence before the word
+                        if (span.holds(t0) && into > 0 && into < W - 1) {
+                            float st[W - 1];
+                            r.start_of(span.n, st);
+#pragma unroll
+                            for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+                                for (int i = 0; i < W - 1; ++i)
+                                    if (k + into < W - 1 && k + into == i) h[k] = st[i];
+                        }
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            if (i == here) {
+                                const bool wraps = !packed && ch + 1 == static_cast<unsigned>(p.dim);
+                                r.take(row + 1, wraps ? batch + 1 : batch, wraps ? 0 : ch + 1);
+                                row_held = row + 1;
+                                span.e = 0;
+                            }
+                            const int t = i >= here ? i - here : t0 + i;
+                            if (t >= span.e) span.find(q, t, r.n0);
+                            if (t == span.s && span.n >= 0) r.start_of(span.n, h);
+                            float a = r.b;
+#pragma unroll
+                            for (int k = 0; k < W - 1; ++k) a = fmaf(r.w[k], h[k], a);
+                            a = fmaf(r.w[W - 1], v[W - 1 + i], a);
+#pragma unroll
+                            for (int k = 0; k + 2 < W; ++k) h[k] = h[k + 1];
+                            h[W - 2] = v[W - 1 + i];
+                            y[i] = conv_act(a, p.silu);
+                            held |= span.holds(t) ? 1u << i : 0u;
+                        }
+                        if (held == (1u << V) - 1) {
+                            *reinterpret_cast<uint4 *>(to) = floats_word<T>(y);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < V; ++i)
+                                if (held >> i & 1) to[i] = from_f32<T>(y[i]);
+                        }
+                    }
                 }
-                __syncwarp();
             }
+            __syncwarp();
         }
+    }
+}
+
+// The final states behind conv_channels_kernel: a thread per (sequence, channel).
+// (A launch of its own: the state rows may be the ones that other words' first
+// tokens still read.)
+template <typename T, int W>
+__global__ void __launch_bounds__(kConvThreads) conv_final_kernel(const ConvArgs p) {
+    const SeqArgs &q = p.seq;
+    const long long count = static_cast<long long>(q.units) * p.dim;
+    for (long long i = static_cast<long long>(blockIdx.x) * kConvThreads + threadIdx.x; i < count;
+         i += static_cast<long long>(gridDim.x) * kConvThreads) {
+        const int n = static_cast<int>(i / p.dim), d = static_cast<int>(i - static_cast<long long>(n) * p.dim);
+        const long long row = seq_row(q, n);
+        if (row < 0) continue;
+        const bool live = p.init != nullptr && seq_live(q, n, row);
+        const int first = q.cu != nullptr ? 0 : n * q.seqlen;
+        const int s = seq_start(q, n) - first, e = seq_end(q, n, s + first) - first;
+        const T *const x =
+            static_cast<const T *>(p.x) + (static_cast<long long>(q.cu != nullptr ? 0 : n) * p.dim + d) * q.seqlen;
+        const size_t at0 = (static_cast<size_t>(row) * p.dim + d) * (W - 1);
+        T keep[W - 1];
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) {
+            const int at = e - (W - 1) + k;
+            if (at >= s) keep[k] = x[at];
+            else keep[k] = live ? static_cast<const T *>(p.init)[at0 + (W - 1) + at - s] : from_f32<T>(0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) static_cast<T *>(p.final_state)[at0 + k] = keep[k];
     }
 }
 
@@ -624,10 +722,20 @@ cudaError_t launch_channels(const ConvArgs &a, cudaStream_t stream) {
         (a.seq.cu != nullptr ? 1LL : static_cast<long long>(a.seq.units)) * a.dim * static_cast<long long>(a.seq.seqlen);
     const auto at = [](const void *p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T)); };
     const int skew = at(a.x);
-    const long long words = (total + skew + V - 1) / V, items = (words + 32 * kRuns - 1) / (32 * kRuns);
-    const long long blocks = (items + kConvThreads / 32 - 1) / (kConvThreads / 32);
-    conv_channels_kernel<T, W><<<static_cast<unsigned>(std::min(blocks, 1LL << 30)), kConvThreads, 0, stream>>>(
-        a, total, skew, at(a.out) == skew, items);
+    auto launch = [&](auto kernel, int runs) {
+        const long long words = (total + skew + V - 1) / V, items = (words + 32 * runs - 1) / (32 * runs);
+        const long long blocks = (items + kConvThreads / 32 - 1) / (kConvThreads / 32);
+        kernel<<<static_cast<unsigned>(std::min(blocks, 1LL << 30)), kConvThreads, 0, stream>>>(a, total, skew,
+                                                                                              at(a.out) == skew, items);
+        return cudaGetLastError();
+    };
+    // Eight runs share the item's arithmetic and cover more latency (8 rows of 4096 channels x 2048 tokens in
+    // bfloat16: 112, 79 and 65 us with two, four and eight), but an item that straddles rows goes run by run.
+    const cudaError_t e = a.seq.seqlen >= 8 * 32 * V ? launch(conv_channels_kernel<T, W, 8>, 8)
+                                                     : launch(conv_channels_kernel<T, W, 2>, 2);
+    if (e != cudaSuccess || a.final_state == nullptr) return e;
+    const long long blocks = (static_cast<long long>(a.seq.units) * a.dim + kConvThreads - 1) / kConvThreads;
+    conv_final_kernel<T, W><<<static_cast<unsigned>(std::min(blocks, 1LL << 20)), kConvThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
