@@ -729,10 +729,11 @@ cudaError_t launch_channels(const ConvArgs &a, cudaStream_t stream) {
                                                                                               at(a.out) == skew, items);
         return cudaGetLastError();
     };
-    // Eight runs share the item's arithmetic and cover more latency (8 rows of 4096 channels x 2048 tokens in
-    // bfloat16: 112, 79 and 65 us with two, four and eight), but an item that straddles rows goes run by run.
+    // Runs per item share its arithmetic and cover latency, but an item that straddles rows goes word by word.
+    // 4096 channels x 16384 tokens in bfloat16: rows of 2048 tokens 112, 79 and 62 us with two, four and eight
+    // runs; rows of 2000 164, 130 and 133 us, of 1024 124, 81 and 154 us, of 100 287, 265 and 323 us.
     const cudaError_t e = a.seq.seqlen >= 8 * 32 * V ? launch(conv_channels_kernel<T, W, 8>, 8)
-                                                     : launch(conv_channels_kernel<T, W, 2>, 2);
+                                                     : launch(conv_channels_kernel<T, W, 4>, 4);
     if (e != cudaSuccess || a.final_state == nullptr) return e;
     const long long blocks = (static_cast<long long>(a.seq.units) * a.dim + kConvThreads - 1) / kConvThreads;
     conv_final_kernel<T, W><<<static_cast<unsigned>(std::min(blocks, 1LL << 20)), kConvThreads, 0, stream>>>(a);
