@@ -32,7 +32,6 @@ from __future__ import annotations
 import ctypes
 import os
 import pathlib
-import struct
 
 __all__ = [
     "XmError",
@@ -414,29 +413,37 @@ def GatedDeltaNet2Fn(q, k, v, g, beta, w, initial_state=None, *, scale: float = 
 
 # ---------------------------------------------------------------- serving operators
 #
-# A decode step calls these for every layer, so their host path is short: one
-# pass over the tensors packs the C descriptors, and validation happens once,
-# in the library.
-
-_TENSOR_BYTES = ctypes.sizeof(XmTensor)
-_PACK = [struct.Struct(f"=Q{r}q{8 * (MAX_RANK - r)}xii") for r in range(MAX_RANK + 1)]
+# A decode step calls these for every layer, so their host path is short: the
+# descriptors are filled and the entry point is called in C (csrc/pycall.c), and
+# validation happens once, in the library.
 
 
 def _invalid(message):
     raise XmError(XM_ERR_INVALID_ARGUMENT, message)
 
 
-_codes = None
+_pycall = None
 
 
-def _type_codes():
-    global _codes
-    if _codes is None:
+def _load_pycall():
+    """The call path's module, built beside libxm_ops.so."""
+    global _pycall
+    if _pycall is None:
+        import importlib.util
+
         import torch
 
-        _codes = {torch.float32: DTYPE_FLOAT, torch.bfloat16: DTYPE_BFLOAT16, torch.float16: DTYPE_FLOAT16,
-                  torch.int32: DTYPE_INT32, torch.int64: DTYPE_INT64}
-    return _codes
+        path = _PKG_DIR / "_xm_call.so"
+        if not path.exists():
+            raise XmError(XM_ERR_UNSUPPORTED, f"{path} not found; build it with `make -C {_PKG_DIR}`")
+        spec = importlib.util.spec_from_file_location("_xm_call", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.setup(torch.Tensor, ((torch.float32, DTYPE_FLOAT), (torch.bfloat16, DTYPE_BFLOAT16),
+                                 (torch.float16, DTYPE_FLOAT16), (torch.int32, DTYPE_INT32),
+                                 (torch.int64, DTYPE_INT64)))
+        _pycall = mod
+    return _pycall
 
 
 class _ServeOp:
@@ -445,22 +452,23 @@ class _ServeOp:
 
     def __init__(self, name, names, kinds, state, workspace=False):
         self.name, self.names, self.kinds, self.state, self.workspace = name, names, kinds, state, workspace
-        self.fwd = self.array = None
-        self.blank = {}
+        self.call = None
 
     def load(self):
+        import torch
+
         lib = load_library()
-        self.size = getattr(lib, f"xm_{self.name}_workspace_size")
-        self.array = XmTensor * len(self.names)
-        for io in (0, *_type_codes().values()):
-            descs = self.array()
+        address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
+        self.fwd = address(getattr(lib, f"xm_{self.name}_fwd"))
+        self.size = address(getattr(lib, f"xm_{self.name}_workspace_size")) if self.workspace else 0
+        self.blank = {}  # by the activations' type: the descriptors of absent inputs
+        for io, code in ((torch.float32, DTYPE_FLOAT), (torch.bfloat16, DTYPE_BFLOAT16),
+                         (torch.float16, DTYPE_FLOAT16), (None, 0)):
+            descs = (XmTensor * len(self.names))()
             for i, k in enumerate(self.kinds):
-                descs[i].rank, descs[i].dtype = 1, {"x": io, "f": DTYPE_FLOAT, "i": DTYPE_INT64}[k]
-            self.blank[io] = bytes(descs)  # every input absent
-        self.fwd = getattr(lib, f"xm_{self.name}_fwd")
-
-
-_OUTS = XmTensor * 2
+                descs[i].rank, descs[i].dtype = 1, {"x": code, "f": DTYPE_FLOAT, "i": DTYPE_INT64}[k]
+            self.blank[io] = bytes(descs)
+        self.call = _load_pycall().call
 
 
 def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
@@ -469,11 +477,10 @@ def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
     Everything allocated here belongs to the stream that the call runs on."""
     import torch
 
-    if op.fwd is None:
+    if op.call is None:
         op.load()
-    Tensor, codes = torch.Tensor, _type_codes()
     x = tensors[0]
-    index = x.get_device() if isinstance(x, Tensor) else -1
+    index = x.get_device() if isinstance(x, torch.Tensor) else -1
     if index < 0:
         _invalid(f"{op.names[0]} must be a CUDA tensor")
     if index != torch.cuda.current_device():
@@ -485,53 +492,32 @@ def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
             _invalid("stream belongs to another device")
         with torch.cuda.stream(stream):
             return _serve(op, attrs, tensors, out, state, state_shape, with_state, None)
-    descs = op.array.from_buffer_copy(op.blank[codes.get(x.dtype, 0)])
-    keep = None
-    at = 0
-    for i, t in enumerate(tensors):
-        if t is not None:
-            if not isinstance(t, Tensor) or t.get_device() != index:
-                _invalid(f"{op.names[i]} must be a tensor on cuda:{index}")
-            if not t.is_contiguous():
-                if i == op.state and with_state and state_shape is None:
-                    _invalid(f"{op.names[i]} is updated in place and must be contiguous")
-                t = t.contiguous()
-                keep = (keep, t)
-            shape = t.shape
-            rank = len(shape)
-            if rank > MAX_RANK:
-                _invalid("tensor rank above 8 is not supported")
-            _PACK[rank].pack_into(descs, at, t.data_ptr(), *shape, rank, codes.get(t.dtype, 0))
-        at += _TENSOR_BYTES
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    if with_state and state is None:
-        state = tensors[op.state] if state_shape is None else torch.empty(
-            state_shape, dtype=torch.float32 if op.kinds[op.state] == "f" else x.dtype, device=x.device)
-    outs = _OUTS()
-    at = 0
-    for t in (out, state) if with_state else (out,):
-        if not isinstance(t, Tensor) or t.get_device() != index or not t.is_contiguous():
-            _invalid(f"{'out' if at == 0 else 'the state output'} must be a contiguous tensor on cuda:{index}")
-        shape = t.shape
-        rank = len(shape)
-        if rank > MAX_RANK:
-            _invalid("tensor rank above 8 is not supported")
-        _PACK[rank].pack_into(outs, at, t.data_ptr(), *shape, rank, codes.get(t.dtype, 0))
-        at += _TENSOR_BYTES
-    attrs = ctypes.byref(attrs)
-    ws, ws_bytes = None, 0
+    inplace = -1
+    outs = (out,)
+    if with_state:
+        if state_shape is None:
+            inplace = op.state
+        if state is None:
+            state = tensors[inplace] if state_shape is None else torch.empty(
+                state_shape, dtype=torch.float32 if op.kinds[op.state] == "f" else x.dtype, device=x.device)
+        outs = (out, state)
+    alloc = None
     if op.workspace:
-        size = ctypes.c_size_t(0)
-        _check(op.size(attrs, descs, len(descs), ctypes.byref(size)))
-        ws_bytes = size.value
-        if ws_bytes:
-            scratch = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-            ws = scratch.data_ptr()
-    status = op.fwd(attrs, descs, len(descs), outs, ws, ws_bytes, handle)
-    if status != XM_OK:
+        alloc = lambda n: torch.empty(n, dtype=torch.uint8, device=x.device)  # noqa: E731
+    blank = op.blank.get(x.dtype)
+    status, which = op.call(op.fwd, op.size, ctypes.addressof(attrs), tensors,
+                            op.blank[None] if blank is None else blank, outs, index, inplace, alloc, handle)
+    if status:
+        if status == -1:
+            _invalid(f"{op.names[which]} must be a tensor on cuda:{index}")
+        if status == -2:
+            _invalid(f"{op.names[which]} is updated in place and must be contiguous")
+        if status == -3:
+            _invalid(f"{'the state output' if which else 'out'} must be a contiguous tensor on cuda:{index}")
         _check(status)
-    return (out, state) if with_state else out
+    return outs if with_state else out
 
 
 _CONV = _ServeOp("causal_conv1d", ("x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices",
