@@ -145,6 +145,8 @@ xm_status guarded(F &&f) {
         return fail(XM_ERR_WORKSPACE, e.msg);
     } catch (const std::exception &e) {
         return fail(XM_ERR_INVALID_ARGUMENT, e.what());
+    } catch (...) {
+        return fail(XM_ERR_INVALID_ARGUMENT, "unknown error");
     }
 }
 

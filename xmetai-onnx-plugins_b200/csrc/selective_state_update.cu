@@ -27,27 +27,31 @@ namespace {
 
 constexpr int kUpdThreads = 128;
 
-// Four consecutive states from `p`, `left` of them below N (vec: all, one word).
-__device__ __forceinline__ float4 load_states(const float *p, int left, bool vec) {
+// A lane's four values of a group: one word of consecutive ones (vec), or every
+// `step`-th, so that neighbouring lanes still read neighbouring memory. The first
+// `left` of them are below N; the others read zero and are not stored.
+__device__ __forceinline__ float4 load_states(const float *p, int left, bool vec, int step) {
     if (vec) return left > 0 ? *reinterpret_cast<const float4 *>(p) : make_float4(0, 0, 0, 0);
-    return make_float4(left > 0 ? p[0] : 0.0f, left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
+    return make_float4(left > 0 ? p[0] : 0.0f, left > 1 ? p[step] : 0.0f, left > 2 ? p[2 * step] : 0.0f,
+                       left > 3 ? p[3 * step] : 0.0f);
 }
 
-__device__ __forceinline__ void store_states(float *p, int left, bool vec, const float4 &v) {
+__device__ __forceinline__ void store_states(float *p, int left, bool vec, int step, const float4 &v) {
     if (vec) {
         if (left > 0) *reinterpret_cast<float4 *>(p) = v;
         return;
     }
     if (left > 0) p[0] = v.x;
-    if (left > 1) p[1] = v.y;
-    if (left > 2) p[2] = v.z;
-    if (left > 3) p[3] = v.w;
+    if (left > 1) p[step] = v.y;
+    if (left > 2) p[2 * step] = v.z;
+    if (left > 3) p[3 * step] = v.w;
 }
 
-// Four consecutive values of the I/O type as floats, zeros from `left` on.
+// The same for values of the I/O type.
 template <typename T>
-__device__ __forceinline__ float4 load_io4(const T *p, int left, bool vec) {
-    if (vec && left > 0) {
+__device__ __forceinline__ float4 load_io4(const T *p, int left, bool vec, int step) {
+    if (vec) {
+        if (left <= 0) return make_float4(0, 0, 0, 0);
         if constexpr (sizeof(T) == 4) {
             return __ldg(reinterpret_cast<const float4 *>(p));
         } else {
@@ -56,8 +60,8 @@ __device__ __forceinline__ float4 load_io4(const T *p, int left, bool vec) {
             return make_float4(a.x, a.y, b.x, b.y);
         }
     }
-    return make_float4(left > 0 ? to_f32<T>(p[0]) : 0.0f, left > 1 ? to_f32<T>(p[1]) : 0.0f,
-                       left > 2 ? to_f32<T>(p[2]) : 0.0f, left > 3 ? to_f32<T>(p[3]) : 0.0f);
+    return make_float4(left > 0 ? to_f32<T>(p[0]) : 0.0f, left > 1 ? to_f32<T>(p[step]) : 0.0f,
+                       left > 2 ? to_f32<T>(p[2 * step]) : 0.0f, left > 3 ? to_f32<T>(p[3 * step]) : 0.0f);
 }
 
 // kFull: N = 4 kLanes kQuads and every access in words.
@@ -74,11 +78,15 @@ __global__ void __launch_bounds__(kUpdThreads) state_token_kernel(const ScanArgs
     const int d = active ? c : p.dim - 1;
     const int g = p.groups == 1 ? 0 : d / (p.dim / p.groups);
     const size_t row_elems = static_cast<size_t>(p.dim) * N, bc_elems = static_cast<size_t>(p.groups) * N;
-    const size_t here = static_cast<size_t>(d) * N + 4 * part;  // this lane's first state in a row
-    const int left0 = N - 4 * part;                             // states from there on
-    const T *const Bp = static_cast<const T *>(p.B) + static_cast<size_t>(g) * N + 4 * part;
-    const T *const Cp = static_cast<const T *>(p.C) + static_cast<size_t>(g) * N + 4 * part;
-    auto left = [&](int k) { return kFull ? 4 : left0 - 4 * kLanes * k; };
+    const int n0_lane = vec ? 4 * part : part;                      // this lane's first state
+    const size_t here = static_cast<size_t>(d) * N + n0_lane;       // and its place in a row
+    const T *const Bp = static_cast<const T *>(p.B) + static_cast<size_t>(g) * N + n0_lane;
+    const T *const Cp = static_cast<const T *>(p.C) + static_cast<size_t>(g) * N + n0_lane;
+    auto left = [&](int k) {  // how many of the lane's k-th four states are below N
+        if (kFull) return 4;
+        const int n = N - n0_lane - 4 * kLanes * k;
+        return vec ? n : (n + kLanes - 1) / kLanes;
+    };
     for (int n0 = blockIdx.y * kRows; n0 < p.seq.units; n0 += gridDim.y * kRows) {
         int row[kRows];  // rows of the state are numbered in 31 bits
 #pragma unroll
@@ -96,15 +104,15 @@ __global__ void __launch_bounds__(kUpdThreads) state_token_kernel(const ScanArgs
             const size_t bc = static_cast<size_t>(min(n0 + r, p.seq.units - 1)) * bc_elems;
 #pragma unroll
             for (int k = 0; k < kQuads; ++k) {
-                h[r][k] = load_states(s + 4 * kLanes * k, row[r] >= 0 ? left(k) : 0, vec);
-                b[r][k] = load_io4<T>(Bp + bc + 4 * kLanes * k, left(k), vec);
-                cc[r][k] = load_io4<T>(Cp + bc + 4 * kLanes * k, left(k), vec);
+                h[r][k] = load_states(s + 4 * kLanes * k, row[r] >= 0 ? left(k) : 0, vec, kLanes);
+                b[r][k] = load_io4<T>(Bp + bc + 4 * kLanes * k, left(k), vec, kLanes);
+                cc[r][k] = load_io4<T>(Cp + bc + 4 * kLanes * k, left(k), vec, kLanes);
             }
         }
         float4 a2[kQuads];
 #pragma unroll
         for (int k = 0; k < kQuads; ++k) {
-            a2[k] = load_states(p.A + here + 4 * kLanes * k, left(k), vec);
+            a2[k] = load_states(p.A + here + 4 * kLanes * k, left(k), vec, kLanes);
             a2[k] = make_float4(a2[k].x * kLog2e, a2[k].y * kLog2e, a2[k].z * kLog2e, a2[k].w * kLog2e);
         }
         float dt_own = delta + (p.bias != nullptr ? p.bias[d] : 0.0f);
@@ -133,7 +141,7 @@ __global__ void __launch_bounds__(kUpdThreads) state_token_kernel(const ScanArgs
             if (active && row[r] >= 0) {
                 float *s = p.final_state + static_cast<size_t>(row[r]) * row_elems + here;
 #pragma unroll
-                for (int k = 0; k < kQuads; ++k) store_states(s + 4 * kLanes * k, left(k), vec, h[r][k]);
+                for (int k = 0; k < kQuads; ++k) store_states(s + 4 * kLanes * k, left(k), vec, kLanes, h[r][k]);
             }
         }
         // Sum over the channel's lanes; the first steps leave each lane the sequence it owns.
