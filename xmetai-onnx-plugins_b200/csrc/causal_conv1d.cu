@@ -68,7 +68,7 @@ template <int V, int W>
 __device__ __forceinline__ void conv_load_weights(const ConvArgs &p, int d, bool words, float (&w)[W][V], float (&b)[V]) {
     const float *src = p.weight + static_cast<size_t>(d) * W;
     float flat[V * W];
-    if (V > 1 && words) {
+    if (V % 4 == 0 && words) {
 #pragma unroll
         for (int i = 0; i + 4 <= V * W; i += 4) {
             const float4 v = __ldg(reinterpret_cast<const float4 *>(src + i));
@@ -85,7 +85,7 @@ __device__ __forceinline__ void conv_load_weights(const ConvArgs &p, int d, bool
         b[i] = 0.0f;
     }
     if (p.bias != nullptr) {
-        if (V > 1 && words) {
+        if (V % 4 == 0 && words) {
 #pragma unroll
             for (int i = 0; i + 4 <= V; i += 4) {
                 const float4 v = __ldg(reinterpret_cast<const float4 *>(p.bias + d + i));
@@ -127,7 +127,7 @@ __device__ __forceinline__ uint4 floats_word(const float (&v)[kWord<T>]) {
         return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
 
-// V elements from p: one word when V is the word's, else a single element.
+// V elements from p: a 16-byte word, half of one, or a single element.
 template <typename T, int V>
 struct Elems {
     uint4 r;
@@ -135,6 +135,10 @@ struct Elems {
         if constexpr (V == 1) {
             if constexpr (sizeof(T) == 4) r.x = __float_as_uint(*p);
             else r.x = *reinterpret_cast<const unsigned short *>(p);
+        } else if constexpr (V * sizeof(T) == 8) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(p);
+            r.x = w.x;
+            r.y = w.y;
         } else {
             r = *reinterpret_cast<const uint4 *>(p);
         }
@@ -143,6 +147,14 @@ struct Elems {
         if constexpr (V == 1) {
             if constexpr (sizeof(T) == 4) v[0] = __uint_as_float(r.x);
             else v[0] = unpack2<T>(r.x).x;
+        } else if constexpr (V * sizeof(T) == 8) {
+            if constexpr (sizeof(T) == 4) {
+                v[0] = __uint_as_float(r.x);
+                v[1] = __uint_as_float(r.y);
+            } else {
+                const float2 a = unpack2<T>(r.x), b = unpack2<T>(r.y);
+                v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+            }
         } else {
             word_floats<T>(r, v);
         }
@@ -152,6 +164,9 @@ struct Elems {
 template <typename T, int V>
 __device__ __forceinline__ void store_elems(T *p, const float (&v)[V]) {
     if constexpr (V == 1) *p = from_f32<T>(v[0]);
+    else if constexpr (V * sizeof(T) == 8 && sizeof(T) == 2)
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    else if constexpr (V * sizeof(T) == 8) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
     else *reinterpret_cast<uint4 *>(p) = floats_word<T>(v);
 }
 
@@ -757,13 +772,17 @@ cudaError_t launch_token(const ConvArgs &a, cudaStream_t stream) {
     const int64_t groups = (static_cast<int64_t>(a.seq.units) + 3) / 4;
     const unsigned gx = static_cast<unsigned>(blocks);
     const bool words = aligned16(a.weight) && aligned16(a.bias);
-    // Four sequences per thread where that leaves each SM four blocks.
-    if (blocks * groups >= 4LL * current_device_sm_count())
+    // Four sequences per thread where that leaves each SM four blocks; below, one, and half words, which
+    // need half the registers and give twice the threads (256 sequences x 4096 channels: 5.6 us against 9.6).
+    if (blocks * groups >= 4LL * current_device_sm_count()) {
         conv_token_kernel<T, V, W, 4>
             <<<dim3(gx, static_cast<unsigned>(std::min<int64_t>(groups, 65535))), kConvThreads, 0, stream>>>(a, words);
-    else
-        conv_token_kernel<T, V, W, 1>
-            <<<dim3(gx, static_cast<unsigned>(std::min(a.seq.units, 65535))), kConvThreads, 0, stream>>>(a, words);
+    } else {
+        constexpr int H = V > 1 ? V / 2 : 1;
+        const unsigned hx = static_cast<unsigned>((static_cast<int64_t>(a.dim) + H * kConvThreads - 1) / (H * kConvThreads));
+        conv_token_kernel<T, H, W, 1>
+            <<<dim3(hx, static_cast<unsigned>(std::min(a.seq.units, 65535))), kConvThreads, 0, stream>>>(a, words);
+    }
     return cudaGetLastError();
 }
 
