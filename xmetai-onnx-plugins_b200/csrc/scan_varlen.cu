@@ -364,14 +364,27 @@ __global__ void __launch_bounds__(Shape<T, NS, kLanes>::kThreads) scan_block_ker
         if (e > t0) {
             const int bs = min(max(0, (s - row0) / g.bl), j - 1);
             load_row(g.H, b0 + bs, h);
-            for (int b = bs + 1; b < j; ++b) {
-                float2 v[NS];
-                load_row(g.H, b0 + b, v);
+            // four blocks' loads at a time: one by one, each would wait for the caches
+            constexpr int kJoin = 4;
+            for (int b = bs + 1; b < j; b += kJoin) {
+                float2 v[kJoin][NS];
+                float sd[kJoin][2];
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    const float sd = g.S[static_cast<size_t>(b0 + b) * p.dim + d[i / (NS / 2)]];
-                    const float2 x = __fmul2_rn(make_float2(sd, sd), a2[i]);
-                    h[i] = __ffma2_rn(make_float2(ex2_approx(x.x), ex2_approx(x.y)), h[i], v[i]);
+                for (int k = 0; k < kJoin; ++k) {
+                    const int at = b0 + min(b + k, j - 1);
+                    load_row(g.H, at, v[k]);
+                    sd[k][0] = g.S[static_cast<size_t>(at) * p.dim + d[0]];
+                    sd[k][1] = g.S[static_cast<size_t>(at) * p.dim + d[1]];
+                }
+#pragma unroll
+                for (int k = 0; k < kJoin; ++k) {
+                    if (b + k >= j) break;
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) {
+                        const float m = sd[k][i / (NS / 2)];
+                        const float2 x = __fmul2_rn(make_float2(m, m), a2[i]);
+                        h[i] = __ffma2_rn(make_float2(ex2_approx(x.x), ex2_approx(x.y)), h[i], v[k][i]);
+                    }
                 }
             }
         } else {
@@ -652,7 +665,7 @@ ScanPlan plan_scan(const ScanArgs &a) {
     // Cut rows into the number of blocks with the least estimated time, in clocks: a scheduler with w
     // warps takes walk(w) for a token of each (measured at d_state 16: 335 for one warp, 470 for two,
     // 640 for three, 212 for each of many), the first pass 0.76 of that, and a second launch with the
-    // join over the blocks 16000 + 500 per block. 8 rows of 2048 tokens x 4096 channels: 481 us uncut,
+    // join over the blocks 16000 + 200 per block. 8 rows of 2048 tokens x 4096 channels: 481 us uncut,
     // 660 to 685 us cut into 2 to 6. One row of 32768 x 2048: 1227 us in 9 blocks, 731 us in 55.
     // One row of 2048 x 4096: 347 us uncut, 124 us in 16 blocks.
     auto walk = [](int64_t w) { return std::max({335.0, 130.0 + 170.0 * w, 212.0 * w}); };
@@ -662,7 +675,7 @@ ScanPlan plan_scan(const ScanArgs &a) {
         const int64_t bl = std::max<int64_t>(kGroup, (each + kGroup - 1) / kGroup * kGroup);
         if (nbr > 1 && (g.row_tokens + bl - 1) / bl != nbr) continue;
         double cost = bl * walk((warps * nbr + slots - 1) / slots);
-        if (nbr > 1) cost += 0.76 * bl * walk((warps * (nbr - 1) + slots - 1) / slots) + 16000.0 + 500.0 * nbr;
+        if (nbr > 1) cost += 0.76 * bl * walk((warps * (nbr - 1) + slots - 1) / slots) + 16000.0 + 200.0 * nbr;
         if (nbr == 1 || cost < best) {
             best = cost;
             g.bl = static_cast<int>(std::min<int64_t>(bl, INT32_MAX));
