@@ -16,6 +16,9 @@
  *                     and its launcher gated_deltanet2_fwd.cu:237-304
  *   SoftmaxCPU        csrc/softmax_cpu/softmax_cpu_ort.cpp:20-114
  *
+ * CausalConv1dFn, CausalConv1dUpdateFn, SelectiveScanVarlenFn and
+ * SelectiveStateUpdateFn stand beside them without a counterpart there.
+ *
  * Conventions
  *  - Plain pointers and sizes only. Tensors are dense row-major, exactly as the
  *    reference assumes (csrc/utils/ort_common.h:105-141 recomputes contiguous
@@ -25,7 +28,8 @@
  *    mamba3_siso_fn_ort.cpp:80-81, gated_deltanet2_fn_ort.cpp:119).
  *  - The caller owns all memory: inputs, the output (shape from the
  *    *_output_shape query) and a workspace (size from the *_workspace_size
- *    query, 256-byte aligned; 0 bytes for SelectiveScanFn and Mamba3SisoFn).
+ *    query, 256-byte aligned; 0 bytes for SelectiveScanFn, Mamba3SisoFn, the
+ *    convolutions and SelectiveStateUpdateFn).
  *    The library allocates no memory and never synchronises the stream, so
  *    concurrent calls on different streams with separate workspaces are
  *    independent. Its only state is, per (host thread, device), two internal
