@@ -292,8 +292,8 @@ xm_status xm_gated_deltanet2_fwd_static_ws(const xm_gated_deltanet2_attrs *attrs
  *    negative or not below the number of slots owns no row: a prompt then starts
  *    from zeros and stores no final state; a single-token row is skipped, its
  *    output row left as it was (padding of a captured graph's batch). Two
- *    sequences of one call must not own the same slot: nothing outside the pool
- *    is touched then, but which of the two states it holds is not defined.
+ *    sequences of one call must not own the same slot: nothing else is touched
+ *    then, but their outputs and the slot's state are not defined.
  *  - cu_seqlens (int32 or int64, [sequences + 1] ascending offsets [0, ...])
  *    packs sequences into the single batch row; lengths of zero are allowed, and
  *    positions behind the last offset are neither read nor written. Offsets are
@@ -301,8 +301,8 @@ xm_status xm_gated_deltanet2_fwd_static_ws(const xm_gated_deltanet2_attrs *attrs
  *  - A state output may be the state input itself (same address, in place);
  *    with state_indices it must be. Apart from that, an output that overlaps an
  *    input or another output is rejected.
- *  - Empty tensors are absent inputs. Tokens per call (batch x seqlen) and every
- *    dimension are limited to 2^31 - 1.
+ *  - Empty tensors are absent inputs. Limits: fewer than 2^31 - 4096 tokens
+ *    (batch x seqlen) per call, dim at most 2^30, other dimensions below 2^31.
  */
 
 /* CausalConv1dFn: y[t, d] = act(bias[d] + sum_k weight[d, k] x[t - (width - 1) + k, d]),

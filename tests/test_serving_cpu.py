@@ -123,7 +123,11 @@ REFUSED = [
     ("causal_conv1d", dict(cu=(3,)), "CausalConv1dFn with cu_seqlens expects batch 1"),
     ("causal_conv1d", dict(x=(1, 8, 16), cu=(1,)), "cu_seqlens must be 1-D with at least 2 offsets"),
     ("causal_conv1d", dict(x=(1, 8, 16), cu=(3,), cudt=F32), "cu_seqlens must be int64 or int32"),
-    ("causal_conv1d", dict(x=(70000, 8, 40000)), "CausalConv1dFn of more than 2^31 - 1 tokens is not supported"),
+    ("causal_conv1d", dict(x=(70000, 8, 40000)), "CausalConv1dFn of 2^31 - 4096 tokens or more is not supported"),
+    ("causal_conv1d", dict(x=(1, 8, (1 << 31) - 4096)), "CausalConv1dFn of 2^31 - 4096 tokens or more is not supported"),
+    ("causal_conv1d", dict(x=(1, (1 << 30) + 1, 2), w=((1 << 30) + 1, 4), bias=(0,)), "dim above 2^30 is not supported"),
+    ("selective_state_update", dict(u=(1, (1 << 30) + 1), A=((1 << 30) + 1, 4), B=(1, 4), D=(0,),
+                                    state=(1, (1 << 30) + 1, 4)), "dim above 2^30 is not supported"),
     ("causal_conv1d", dict(x=(2, 8, 1 << 31)), "x dimension is out of range"),
     ("causal_conv1d", dict(x=(1 << 30, 1 << 30, 1 << 30)), "x has too many elements"),
     ("causal_conv1d", dict(x=(2, 8, -1)), "x has a negative dimension"),

@@ -534,6 +534,86 @@ def test_pools_past_32_bit_offsets(xm, cuda):
     close(last[1:], final, ferr)
 
 
+@pytest.mark.parametrize("channels_last", [0, 1])
+def test_more_sequences_than_a_grid_dimension(xm, cuda, channels_last):
+    """70001 sequences of one call equal the same ones in several calls, bit by bit."""
+    g = gen(61)
+    n, dim = 70001, 8
+    cuts = [(0, 30000), (30000, 65536), (65536, n)]
+    x, w, b = conv_inputs(g, n, 3, dim, 4, torch.bfloat16, channels_last)
+    x, w, b = dev(x), dev(w), dev(b)
+    y, last = xm.CausalConv1dFn(x, w, b, channels_last=channels_last, output_final_state=1)
+    parts = [xm.CausalConv1dFn(x[a:c], w, b, channels_last=channels_last, output_final_state=1) for a, c in cuts]
+    assert torch.equal(torch.cat([p[0] for p in parts]), y) and torch.equal(torch.cat([p[1] for p in parts]), last)
+    if not channels_last:
+        return
+    q = {k: dev(v) for k, v in scan_inputs(g, n, 3, dim, 16, torch.bfloat16).items()}
+    cut = lambda t, a, c: t[a:c] if t.dim() > 2 else t  # noqa: E731
+    y, last = xm.SelectiveScanVarlenFn(*[q[k] for k in SCAN], delta_softplus=1, output_final_state=1)
+    parts = [xm.SelectiveScanVarlenFn(*[cut(q[k], a, c) for k in SCAN], delta_softplus=1, output_final_state=1)
+             for a, c in cuts]
+    assert torch.equal(torch.cat([p[0] for p in parts]), y) and torch.equal(torch.cat([p[1] for p in parts]), last)
+    state = torch.randn(n, dim, 16, device="cuda")
+    tok = lambda t, a, c: t[a:c, 0].contiguous() if t.dim() > 2 else t  # noqa: E731
+    parts = [xm.SelectiveStateUpdateFn(*[tok(q[k], a, c) for k in SCAN], state[a:c].clone(), delta_softplus=1)
+             for a, c in cuts]
+    y, state = xm.SelectiveStateUpdateFn(*[tok(q[k], 0, n) for k in SCAN], state, delta_softplus=1)
+    assert torch.equal(torch.cat([p[0] for p in parts]), y) and torch.equal(torch.cat([p[1] for p in parts]), state)
+    cs = last_inputs = torch.randn(n, dim, 3, device="cuda").to(torch.bfloat16)
+    parts = [xm.CausalConv1dUpdateFn(x[a:c, 0].contiguous(), w, b, cs[a:c].clone()) for a, c in cuts]
+    y, cs = xm.CausalConv1dUpdateFn(x[:, 0].contiguous(), w, b, cs)
+    assert cs is last_inputs
+    assert torch.equal(torch.cat([p[0] for p in parts]), y) and torch.equal(torch.cat([p[1] for p in parts]), cs)
+    # packed: as many sequences, some empty, over one row
+    lens = torch.randint(0, 4, (n,), generator=g)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)])
+    total = int(cu[-1])
+    flat = x.reshape(1, -1, dim)[:, :total].contiguous()
+    y, last = xm.CausalConv1dFn(flat, w, b, None, cu.cuda(), channels_last=1, output_final_state=1)
+    half = int(cu[40000])
+    a = xm.CausalConv1dFn(flat[:, :half], w, b, None, cu[:40001].cuda(), channels_last=1, output_final_state=1)
+    c = xm.CausalConv1dFn(flat[:, half:], w, b, None, (cu[40000:] - half).cuda(), channels_last=1, output_final_state=1)
+    assert torch.equal(torch.cat([a[0], c[0]], 1), y) and torch.equal(torch.cat([a[1], c[1]]), last)
+
+
+def test_a_slot_named_twice_touches_nothing_else(xm, cuda):
+    x = _layer_inputs(62)
+    before = {k: x[k].clone() for k in ("cs", "ss")}
+    x["slots"] = torch.tensor([3, 3, 1], dtype=torch.int32).cuda()
+    _layer(xm, x, torch.bfloat16)
+    for k in ("cs", "ss"):
+        for i in (0, 2, 4):
+            assert torch.equal(x[k][i], before[k][i])
+        assert torch.isfinite(x[k].float()).all()
+
+
+def test_refusals_on_the_device(xm, cuda):
+    """What only a device tensor can show: strided states in place, host tensors among device ones, strided outputs."""
+    g = gen(63)
+    x, w, b = conv_inputs(g, 4, 6, 16, 4, torch.float32, 1)
+    x, w, b = dev(x), dev(w), dev(b)
+    wide = torch.zeros(4, 16, 6, device="cuda")
+    with pytest.raises(xm.XmError, match="state is updated in place and must be contiguous"):
+        xm.CausalConv1dUpdateFn(x[:, 0].contiguous(), w, b, wide[..., :3])
+    with pytest.raises(xm.XmError, match="initial_state is updated in place and must be contiguous"):
+        xm.CausalConv1dFn(x, w, b, wide[..., :3], None, torch.arange(4, device="cuda"), channels_last=1,
+                          output_final_state=1)
+    with pytest.raises(xm.XmError, match="weight must be a tensor on cuda:0"):
+        xm.CausalConv1dFn(x, w.cpu(), b, channels_last=1)
+    with pytest.raises(xm.XmError, match="out must be a contiguous tensor on cuda:0"):
+        xm.CausalConv1dFn(x, w, b, channels_last=1, out=torch.empty(4, 6, 32, device="cuda")[..., :16])
+    with pytest.raises(xm.XmError, match="an output must not overlap an input"):
+        xm.CausalConv1dFn(x, w, b, channels_last=1, out=x)
+    with pytest.raises(xm.XmError, match="the state output must be a contiguous tensor on cuda:0"):
+        xm.CausalConv1dUpdateFn(x[:, 0].contiguous(), w, b, wide[..., :3].contiguous(), new_state=wide[..., :3])
+    with pytest.raises(xm.XmError, match="has_initial_state must be int32 or int64"):
+        xm.CausalConv1dFn(x, w, b, torch.zeros(4, 16, 3, device="cuda"), None, None,
+                          torch.ones(4, dtype=torch.bool, device="cuda"), channels_last=1)
+    # a strided input state is copied where it is not written
+    got, new = xm.CausalConv1dFn(x, w, b, wide[..., :3], channels_last=1, output_final_state=1)
+    assert torch.equal(got, xm.CausalConv1dFn(x, w, b, channels_last=1)) and not torch.equal(new, wide[..., :3])
+
+
 def test_malformed_offsets_stay_inside(xm, cuda):
     """Offsets that descend or leave the row address nothing outside it (values are not defined)."""
     x = _layer_inputs(51)

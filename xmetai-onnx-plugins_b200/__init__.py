@@ -554,7 +554,7 @@ def CausalConv1dFn(x, weight, bias=None, initial_state=None, cu_seqlens=None, st
     state_indices (int32 / int64, one per sequence) makes initial_state a pool [slots, dim, width - 1]: sequence i
     continues row state_indices[i], or starts from zeros where has_initial_state[i] is 0, and with
     output_final_state=1 its final state replaces that row in place (the result is (out, initial_state)). An index
-    outside the pool owns no row: zeros, and no final state is kept. Slots named twice leave one of the two states.
+    outside the pool owns no row: zeros, and no final state is kept. No slot may be named twice in a call.
     """
     attrs = CausalConv1dAttrs(int(silu), int(channels_last), int(output_final_state))
     shape = None

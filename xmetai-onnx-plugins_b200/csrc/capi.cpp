@@ -587,6 +587,9 @@ int64_t bounded_elements(const xm_tensor &t, const char *name) {
     return static_cast<int64_t>(n);
 }
 
+// Channel counts, rounded up to a block's, are kept in 31 bits.
+constexpr int64_t kMaxServingDim = int64_t(1) << 30;
+
 size_t element_size(int32_t dtype) {
     switch (dtype) {
         case XM_DTYPE_FLOAT16:
@@ -650,8 +653,9 @@ xm::SeqArgs sequences_of(int64_t batch, int64_t seqlen, const xm_tensor *cu, con
         q.cu = cu->data;
         q.cu64 = cu->dtype == XM_DTYPE_INT64;
     }
-    if (batch * seqlen > static_cast<int64_t>(INT32_MAX))
-        throw Unsupported{std::string(op) + " of more than 2^31 - 1 tokens is not supported"};
+    // The kernels count tokens, and a few behind the last, in 31 bits.
+    if (batch * seqlen > static_cast<int64_t>(INT32_MAX) - 4096)
+        throw Unsupported{std::string(op) + " of 2^31 - 4096 tokens or more is not supported"};
     q.units = static_cast<int>(units);
     q.seqlen = static_cast<int>(seqlen);
     q.tokens = static_cast<int>(batch * seqlen);
@@ -714,6 +718,7 @@ void conv_weights(xm::ConvArgs &a, const xm_tensor &weight, const xm_tensor &bia
     require_dtype(weight, XM_DTYPE_FLOAT);
     const Shape ws = shape_of(weight);
     if (ws.size() != 2 || ws[0] != dim) throw Invalid{"weight must have shape (dim, width)"};
+    if (dim > kMaxServingDim) throw Unsupported{"dim above 2^30 is not supported"};
     if (ws[1] < 2 || ws[1] > 4) throw Unsupported{"causal convolution width must be 2, 3 or 4"};
     a.width = static_cast<int>(ws[1]);
     a.dim = static_cast<int>(dim);
@@ -791,6 +796,7 @@ void scan_inputs(ScanPlan &pl, const xm_tensor *in, size_t lead) {
     require_same_shape(shape_of(in[1]), u, "delta", "u");
     const int64_t dim = u[lead];
     if (A.size() != 2 || A[0] != dim) throw Invalid{"A must have shape (dim, d_state)"};
+    if (dim > kMaxServingDim) throw Unsupported{"dim above 2^30 is not supported"};
     const int64_t dstate = A[1];
     if (dstate < 1 || dstate > 256) throw Unsupported{"d_state must be 1 to 256"};
     Shape B = shape_of(in[3]), C = shape_of(in[4]);

@@ -156,8 +156,13 @@ __global__ void __launch_bounds__(kUpdThreads) state_token_kernel(const ScanArgs
             const float k1 = (hi ? y[3] : y[1]) + __shfl_xor_sync(kFullMask, hi ? y[1] : y[3], 2);
             v = (odd ? k1 : k0) + __shfl_xor_sync(kFullMask, odd ? k0 : k1, 1);
         }
+        // (one sequence per thread adds in the same order, so a row's result does not depend on the batch)
+        if constexpr (kRows == 1 && kLanes >= 4) {
+            v += __shfl_xor_sync(kFullMask, v, 2);
+            v += __shfl_xor_sync(kFullMask, v, 1);
+        }
 #pragma unroll
-        for (int o = kRows; o < kLanes; o *= 2) v += __shfl_xor_sync(kFullMask, v, o);
+        for (int o = kRows == 1 && kLanes >= 4 ? 4 : kRows; o < kLanes; o *= 2) v += __shfl_xor_sync(kFullMask, v, o);
         v = fmaf(p.D != nullptr ? p.D[d] : 0.0f, u, v);
         if (p.z != nullptr) v *= z * rcp_approx(1.0f + ex2_approx(-z * kLog2e));
         bool kept = row[0] >= 0;  // the owned sequence owns a state row
