@@ -5,15 +5,15 @@
 // its state, the last W - 1 inputs of the tokens that went before.
 //
 // Bound by memory: x is read and y written once, against 2 W + 4 operations per
-// element, so each layout's kernel moves 16-byte words and keeps enough of them
-// in flight:
-//   conv_tokens_kernel    [tokens, dim]: a thread owns the channels of one word
+// element, so each layout's kernel moves words or half words of 16 bytes and keeps
+// enough of them in flight:
+//   conv_tokens_kernel    [tokens, dim]: a thread owns the channels of half a word
 //                         and walks a block of tokens, the window in registers;
 //   conv_channels_kernel  [dim, tokens]: a thread owns a word of consecutive
 //                         tokens and takes the W - 1 before it from its
 //                         neighbour lane;
 //   conv_token_kernel     one token per sequence: a thread owns the channels of
-//                         one word, their state and their weights.
+//                         a word or half of one, their state and their weights.
 //
 // The states may be updated in place. With tokens first, one thread does all that
 // touches a sequence's state of a channel: the one whose block holds the
@@ -31,6 +31,11 @@ namespace xm {
 namespace {
 
 constexpr int kConvThreads = 128;
+
+__device__ __forceinline__ void cp_async8(void *smem, const void *gmem) {
+    const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(s), "l"(gmem));
+}
 
 __device__ __forceinline__ float conv_act(float v, bool silu) {
     return silu ? v * rcp_approx(1.0f + ex2_approx(-v * kLog2e)) : v;
@@ -192,10 +197,12 @@ constexpr int kFlights = 4;  // batches in flight or in use
 // words arrive by asynchronous copies in slots of shared memory that no other
 // thread touches, three batches of four tokens ahead, so nothing is waited for
 // but the batch in use and no barrier is needed. (Loads into registers, four or
-// eight tokens ahead, left 16384 tokens x 4096 channels at 69 to 79 us.)
+// eight tokens ahead, left 16384 tokens x 4096 channels at 69 to 79 us.) Half words
+// leave room for six CTAs per SM, whole words for four: 53 us against 57.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArgs p, int block, int nblocks, bool words) {
-    __shared__ uint4 conv_slots[V > 1 ? kFlights * kBatch * kConvThreads : 1];
+    __shared__ uint2 conv_slots[V > 1 ? kFlights * kBatch * kConvThreads : 1];
+    static_assert(V == 1 || V * sizeof(T) == 8, "a thread's channels are half a word");
     const SeqArgs &q = p.seq;
     const int d = (blockIdx.x * kConvThreads + threadIdx.x) * V;
     if (d >= p.dim) return;
@@ -248,13 +255,13 @@ __global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArg
             int t = from;
             if constexpr (V > 1) {
                 const int batches = (to - from) / kBatch;
-                uint4 *const slot = conv_slots + threadIdx.x;
+                uint2 *const slot = conv_slots + threadIdx.x;
                 auto bring = [&](int i) {
                     if (i < batches) {
 #pragma unroll
                         for (int k = 0; k < kBatch; ++k)
-                            cp_async16(slot + ((i % kFlights) * kBatch + k) * kConvThreads,
-                                       x + (static_cast<size_t>(from) + i * kBatch + k) * D, 16);
+                            cp_async8(slot + ((i % kFlights) * kBatch + k) * kConvThreads,
+                                      x + (static_cast<size_t>(from) + i * kBatch + k) * D);
                     }
                     cp_async_commit();
                 };
@@ -266,7 +273,11 @@ __global__ void __launch_bounds__(kConvThreads) conv_tokens_kernel(const ConvArg
                     cp_async_wait<kFlights - 2>();
                     Elems<T, V> cur[kBatch];
 #pragma unroll
-                    for (int k = 0; k < kBatch; ++k) cur[k].r = slot[((i % kFlights) * kBatch + k) * kConvThreads];
+                    for (int k = 0; k < kBatch; ++k) {
+                        const uint2 v = slot[((i % kFlights) * kBatch + k) * kConvThreads];
+                        cur[k].r.x = v.x;
+                        cur[k].r.y = v.y;
+                    }
                     bring(i + kFlights - 1);
 #pragma unroll
                     for (int k = 0; k < kBatch; ++k) step(t + k, cur[k]);
@@ -718,9 +729,10 @@ cudaError_t by_type(IoType io, F &&f) {
 template <typename T, int V, int W>
 cudaError_t launch_tokens(const ConvArgs &a, cudaStream_t stream) {
     const int64_t groups = (static_cast<int64_t>(a.dim) + V * kConvThreads - 1) / (V * kConvThreads);
-    // Four CTAs are resident per SM. Blocks of about 128 tokens, sized so that the grid is whole waves of
-    // them (16384 tokens x 4096 channels: 62 us in blocks of 64, which are 1.7 waves); 4 tokens at least.
-    const int64_t resident = 4LL * current_device_sm_count(), tokens = a.seq.tokens;
+    // Six CTAs are resident per SM. Blocks of about 128 tokens, sized so that the grid is whole waves of
+    // them (with four resident, 16384 tokens x 4096 channels took 62 us in blocks of 64, 1.7 waves, and 57 us
+    // so); 4 tokens at least.
+    const int64_t resident = 6LL * current_device_sm_count(), tokens = a.seq.tokens;
     const int64_t waves = std::max<int64_t>(1, (tokens * groups + 64 * resident) / (128 * resident));
     const int64_t want = std::max<int64_t>(1, resident * waves / groups);
     const int block = static_cast<int>(std::max<int64_t>(4, ((tokens + want - 1) / want + 3) / 4 * 4));
@@ -759,8 +771,9 @@ cudaError_t launch_channels(const ConvArgs &a, cudaStream_t stream) {
 // [0, 0) with the tokens-first kernel touch nothing but states.
 template <typename T, int W>
 cudaError_t launch_width(const ConvArgs &a, cudaStream_t stream) {
-    constexpr int V = kWord<T>;
-    const bool vec = a.dim % V == 0 && aligned16(a.x) && aligned16(a.out);
+    constexpr int V = kWord<T> / 2;
+    auto on8 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 8 == 0; };
+    const bool vec = a.dim % V == 0 && on8(a.x) && on8(a.out);
     if (a.channels_last || a.seq.tokens == 0)
         return vec ? launch_tokens<T, V, W>(a, stream) : launch_tokens<T, 1, W>(a, stream);
     return launch_channels<T, W>(a, stream);
