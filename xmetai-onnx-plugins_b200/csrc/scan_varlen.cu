@@ -59,7 +59,7 @@ struct ScanGeom {
     int chan_blocks;  // channel blocks of a group
     bool vec_io;      // u, delta, z, out rows in words of a warp's channels (16 bytes at most)
     bool vec_bc;      // B / C rows in 16-byte words
-    bool vec_state;   // state rows in 16-byte words
+    bool vec_state;   // rows of the states and of A in 16-byte words
     float *H, *I;     // [blocks][dim][dstate]: state at a block's end; start of the sequence that leaves it
     float *S;         // [blocks][dim]: sum of dt over a block that a sequence crosses
 };
@@ -271,18 +271,7 @@ __global__ void __launch_bounds__(Shape<T, NS, kLanes>::kThreads) scan_block_ker
     };
 
     float2 h[NS], a2[NS];  // [channel][state pair]
-    unsigned real = 0;     // which of a channel's NS states here are below N
     auto state_of = [&](int i) { return 4 * ((i >> 2) * kLanes + part) + (i & 3); };  // i-th state of this lane
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int n = state_of(i);
-            const float a = n < N ? p.A[static_cast<size_t>(d[m]) * N + n] * kLog2e : 0.0f;
-            float2 &v = a2[m * (NS / 2) + i / 2];
-            (i & 1 ? v.y : v.x) = a;
-            real |= n < N ? 1u << i : 0u;
-        }
     auto zero = [&] {
 #pragma unroll
         for (int i = 0; i < NS; ++i) h[i] = make_float2(0.0f, 0.0f);
@@ -341,7 +330,7 @@ __global__ void __launch_bounds__(Shape<T, NS, kLanes>::kThreads) scan_block_ker
     int n, e, t, stop;
     float ssum[2] = {0.0f, 0.0f};
     bool crossing = false;  // kEnds: the sequence began before this block
-    zero();
+    int from_block = -1;    // outputs: the block in which the sequence that reaches into this one begins
     if constexpr (kEnds) {
         n = first_from(q, t1, row, false) - 1;
         if (n < 0) return;
@@ -351,10 +340,6 @@ __global__ void __launch_bounds__(Shape<T, NS, kLanes>::kThreads) scan_block_ker
         crossing = s < t0;
         t = max(s, t0);
         stop = t1;
-        if (!crossing) {
-            load_start(n);
-            store_row(g.I, b0 + j, h);
-        }
     } else {
         n = first_from(q, t0, row, j == 0) - 1;
         int s = n >= 0 ? seq_start(q, n) : 0;
@@ -362,31 +347,7 @@ __global__ void __launch_bounds__(Shape<T, NS, kLanes>::kThreads) scan_block_ker
         stop = q.cu != nullptr ? min(t1, seq_start(q, units)) : t1;
         t = t0;
         if (e > t0) {
-            const int bs = min(max(0, (s - row0) / g.bl), j - 1);
-            load_row(g.H, b0 + bs, h);
-            // four blocks' loads at a time: one by one, each would wait for the caches
-            constexpr int kJoin = 4;
-            for (int b = bs + 1; b < j; b += kJoin) {
-                float2 v[kJoin][NS];
-                float sd[kJoin][2];
-#pragma unroll
-                for (int k = 0; k < kJoin; ++k) {
-                    const int at = b0 + min(b + k, j - 1);
-                    load_row(g.H, at, v[k]);
-                    sd[k][0] = g.S[static_cast<size_t>(at) * p.dim + d[0]];
-                    sd[k][1] = g.S[static_cast<size_t>(at) * p.dim + d[1]];
-                }
-#pragma unroll
-                for (int k = 0; k < kJoin; ++k) {
-                    if (b + k >= j) break;
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) {
-                        const float m = sd[k][i / (NS / 2)];
-                        const float2 x = __fmul2_rn(make_float2(m, m), a2[i]);
-                        h[i] = __ffma2_rn(make_float2(ex2_approx(x.x), ex2_approx(x.y)), h[i], v[k][i]);
-                    }
-                }
-            }
+            from_block = min(max(0, (s - row0) / g.bl), j - 1);
         } else {
             t = n + 1 < units ? max(t0, seq_start(q, n + 1)) : t0;
             e = t;  // the event at t takes up sequence n + 1
@@ -486,9 +447,48 @@ __global__ void __launch_bounds__(Shape<T, NS, kLanes>::kThreads) scan_block_ker
         barrier();
     }
 
+    // The first groups are on their way before the states and A are waited for.
     if (t < stop) {
         fetch(t, 0);
         fetch(t + kGroup, 1);
+    }
+    unsigned real = 0;  // which of a channel's NS states here are below N
+#pragma unroll
+    for (int i = 0; i < NS; ++i) real |= state_of(i) < N ? 1u << i : 0u;
+    load_row(p.A, 0, a2);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) a2[i] = __fmul2_rn(a2[i], make_float2(kLog2e, kLog2e));
+    zero();
+    if constexpr (kEnds) {
+        if (!crossing) {
+            load_start(n);
+            store_row(g.I, b0 + j, h);
+        }
+    } else if (from_block >= 0) {
+        load_row(g.H, b0 + from_block, h);
+        // four blocks' loads at a time: one by one, each would wait for the caches
+        constexpr int kJoin = 4;
+        for (int b = from_block + 1; b < j; b += kJoin) {
+            float2 v[kJoin][NS];
+            float sd[kJoin][2];
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k) {
+                const int at = b0 + min(b + k, j - 1);
+                load_row(g.H, at, v[k]);
+                sd[k][0] = g.S[static_cast<size_t>(at) * p.dim + d[0]];
+                sd[k][1] = g.S[static_cast<size_t>(at) * p.dim + d[1]];
+            }
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k) {
+                if (b + k >= j) break;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const float m = sd[k][i / (NS / 2)];
+                    const float2 x = __fmul2_rn(make_float2(m, m), a2[i]);
+                    h[i] = __ffma2_rn(make_float2(ex2_approx(x.x), ex2_approx(x.y)), h[i], v[k][i]);
+                }
+            }
+        }
     }
     int st = 0;  // stage of the group at t
     for (; t < stop; t += kGroup) {
@@ -662,20 +662,29 @@ ScanPlan plan_scan(const ScanArgs &a) {
     g.row_tokens = a.seq.cu != nullptr ? a.seq.tokens : a.seq.seqlen;
     const int64_t ctas = std::max<int64_t>(1, static_cast<int64_t>(g.chan_blocks) * a.groups * rows);
     const int64_t warps = ctas * (N > 16 ? 4 : 1), slots = 4LL * current_device_sm_count();
-    // Cut rows into the number of blocks with the least estimated time, in clocks: a scheduler with w
-    // warps takes walk(w) for a token of each (measured at d_state 16: 335 for one warp, 470 for two,
-    // 640 for three, 212 for each of many), the first pass 0.76 of that, and a second launch with the
-    // join over the blocks 16000 + 200 per block. 8 rows of 2048 tokens x 4096 channels: 481 us uncut,
-    // 660 to 685 us cut into 2 to 6. One row of 32768 x 2048: 1227 us in 9 blocks, 731 us in 55.
-    // One row of 2048 x 4096: 347 us uncut, 124 us in 16 blocks.
-    auto walk = [](int64_t w) { return std::max({335.0, 130.0 + 170.0 * w, 212.0 * w}); };
+    // Cut rows into the number of blocks with the least estimated time, in clocks (measured at d_state 16):
+    // a scheduler with w warps takes walk[w] for a token of each; it holds 3 of the second pass and 4 of
+    // the first, whose tokens cost 0.76 as much; a CTA spends 7000 before and behind its tokens, a second
+    // launch 5000, and the last block's join 450 per block.
+    // Microseconds by number of blocks: a row of 512 tokens x 4096 channels 89 uncut, 37 in 8, 34 by the rule
+    // (13), 52 in 32; 4096 x 256: 682, 173 in 8, 45 (74), 56 in 128; 8192 x 2048: 1376, 342 in 8, 196 (27),
+    // 304 in 128; four rows of 1024 x 1024: 175, 65 in 8, 58 (13), 78 in 32; eight rows of 2048 x 4096: 480
+    // uncut (the rule's), 660 to 685 in 2 to 6.
+    constexpr double kWalk[5] = {0.0, 335.0, 470.0, 640.0, 848.0};
+    auto pass = [&](int64_t count, int64_t bl, int cap, double factor) {
+        const int64_t full = count / (cap * slots), rest = count % (cap * slots);
+        const double start = 7000.0;
+        double t = full * (factor * bl * kWalk[cap] + start);
+        if (rest > 0) t += factor * bl * kWalk[(rest + slots - 1) / slots] + start;
+        return t;
+    };
     double best = 0.0;
     for (int nbr = 1; nbr <= 128; ++nbr) {
         const int64_t each = (static_cast<int64_t>(g.row_tokens) + nbr - 1) / nbr;
         const int64_t bl = std::max<int64_t>(kGroup, (each + kGroup - 1) / kGroup * kGroup);
         if (nbr > 1 && (g.row_tokens + bl - 1) / bl != nbr) continue;
-        double cost = bl * walk((warps * nbr + slots - 1) / slots);
-        if (nbr > 1) cost += 0.76 * bl * walk((warps * (nbr - 1) + slots - 1) / slots) + 16000.0 + 200.0 * nbr;
+        double cost = pass(warps * nbr, bl, 3, 1.0);
+        if (nbr > 1) cost += pass(warps * (nbr - 1), bl, 4, 0.76) + 5000.0 + 450.0 * nbr;
         if (nbr == 1 || cost < best) {
             best = cost;
             g.bl = static_cast<int>(std::min<int64_t>(bl, INT32_MAX));
@@ -715,7 +724,7 @@ cudaError_t launch_passes(const ScanArgs &a, const ScanPlan &pl, cudaStream_t st
     auto on = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % (S::kCopy * sizeof(T)) == 0; };
     g.vec_io = a.dim / a.groups % std::max(S::kCopy, S::V) == 0 && on(a.u) && on(a.delta) && on(a.z) && on(a.out);
     g.vec_bc = a.dstate % S::kPer == 0 && aligned16(a.B) && aligned16(a.C);
-    g.vec_state = a.dstate % 4 == 0 && aligned16(a.init) && aligned16(a.final_state);
+    g.vec_state = a.dstate % 4 == 0 && aligned16(a.A) && aligned16(a.init) && aligned16(a.final_state);
     if (pl.ends) {
         const cudaError_t e = launch_pass<T, NS, kLanes, true>(a, g, stream);
         if (e != cudaSuccess) return e;
