@@ -500,12 +500,12 @@ def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
         if state_shape is None:
             inplace = op.state
         if state is None:
-            state = tensors[inplace] if state_shape is None else torch.empty(
-                state_shape, dtype=torch.float32 if op.kinds[op.state] == "f" else x.dtype, device=x.device)
+            state = tensors[inplace] if state_shape is None else x.new_empty(
+                state_shape, dtype=torch.float32 if op.kinds[op.state] == "f" else x.dtype)
         outs = (out, state)
     alloc = None
     if op.workspace:
-        alloc = lambda n: torch.empty(n, dtype=torch.uint8, device=x.device)  # noqa: E731
+        alloc = lambda n: x.new_empty(n, dtype=torch.uint8)  # noqa: E731
     blank = op.blank.get(x.dtype)
     status, which = op.call(op.fwd, op.size, ctypes.addressof(attrs), tensors,
                             op.blank[None] if blank is None else blank, outs, index, inplace, alloc, handle)

@@ -679,7 +679,8 @@ ScanPlan plan_scan(const ScanArgs &a) {
         return t;
     };
     double best = 0.0;
-    for (int nbr = 1; nbr <= 128; ++nbr) {
+    const int most = std::min(128, 1 + g.row_tokens / kGroup);
+    for (int nbr = 1; nbr <= most; ++nbr) {
         const int64_t each = (static_cast<int64_t>(g.row_tokens) + nbr - 1) / nbr;
         const int64_t bl = std::max<int64_t>(kGroup, (each + kGroup - 1) / kGroup * kGroup);
         if (nbr > 1 && (g.row_tokens + bl - 1) / bl != nbr) continue;
