@@ -1,0 +1,53 @@
+"""Calls of the serving operators at the edges of what their documentation
+allows, on the GPU, against the float64 definitions of serving_reference.py."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import serving_reference as R
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+def close(got, want, bound):
+    e = R.excess(got, want, bound)
+    assert e <= 0, f"off by {e} more than the bound"
+
+
+# ------------------------------------------------------------------ CausalConv1dFn, addresses
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("width", [2, 3, 4])
+@pytest.mark.parametrize("batch,seqlen,cu", [(2, 50, None), (1, 9, None), (3, 5, None), (1, 2500, None),
+                                             (1, 300, [0, 3, 4, 40, 290]), (1, 40, [6, 9, 33, 40])])
+def test_conv_input_and_output_equally_misaligned(xm, cuda, dt, width, batch, seqlen, cu):
+    """Channel-major x and out at the same offset from a 16-byte boundary: the first word is cut by x's begin."""
+    g = gen(seqlen + width)
+    dim = 3
+    x, w, b = normal(g, batch, dim, seqlen, dtype=DT[dt]), normal(g, dim, width), normal(g, dim)
+    state = normal(g, batch if cu is None else len(cu) - 1, dim, width - 1, dtype=DT[dt])
+    before = torch.full_like(x, 5.0)
+    y, bound, final = R.conv(x, w, b, state, cu, out=before)
+    cud = None if cu is None else torch.tensor(cu, dtype=torch.int32).cuda()
+    for o in range(1, 16 // x.element_size()):
+        src = torch.full((x.numel() + 32,), float("nan"), dtype=x.dtype, device="cuda")
+        dst = torch.full((x.numel() + 32,), 5.0, dtype=x.dtype, device="cuda")
+        xs, ys = src[o:o + x.numel()].view(x.shape), dst[o:o + x.numel()].view(x.shape)
+        xs.copy_(x)
+        _, last = xm.CausalConv1dFn(xs, w.cuda(), b.cuda(), state.cuda(), cud, output_final_state=1, out=ys)
+        close(ys, y, bound)
+        assert torch.equal(last.cpu(), final)
+        assert bool((dst[:o] == 5).all()) and bool((dst[o + x.numel():] == 5).all())

@@ -432,7 +432,8 @@ __device__ __noinline__ void conv_any(const ConvArgs &p, long long f, long long 
 // takes the W - 1 inputs before its word from its neighbour lane. Items inside one
 // sequence do nothing else; in the others every lane looks up its word's row and
 // sequences, and a word that crosses into another row or sequence masks its taps.
-// Words that are not whole, and rows shorter than a word, go token by token.
+// Words that are not whole, the word behind a cut first one, and rows shorter than
+// a word, go token by token.
 // `skew`: elements between x's address and the 16-byte boundary below; words are
 // counted from there. States are only read here; conv_final_kernel stores them.
 template <typename T, int W, int kRuns>
@@ -471,13 +472,6 @@ __global__ void __launch_bounds__(kConvThreads) conv_channels_kernel(const ConvA
             word_floats<T>(before, v);
 #pragma unroll
             for (int k = 0; k < W - 1; ++k) tail[k] = v[V - (W - 1) + k];
-            if (lane == 0 && skew > 0 && f_item > 0 && f_item < V) {  // the word before is cut by x's begin
-#pragma unroll
-                for (int k = 0; k < W - 1; ++k) {
-                    const long long at = f_item - (W - 1) + k;
-                    if (at >= 0 && at < total) tail[k] = to_f32<T>(x[at]);
-                }
-            }
         }
         // A run's inputs: the lane's own and the W - 1 before them.
         auto run_inputs = [&](const uint4 &word, float (&v)[V + W - 1]) {
@@ -555,7 +549,8 @@ __global__ void __launch_bounds__(kConvThreads) conv_channels_kernel(const ConvA
                         ch -= more * static_cast<unsigned>(p.dim);
                     }
                 }
-                if (!vec || lo != f0 || hi != f0 + V || L < V) {
+                // (0 < f0 < V: the word before is cut by x's begin, so the neighbour lane holds no inputs for this one)
+                if (!vec || lo != f0 || hi != f0 + V || L < V || (f0 > 0 && f0 < V)) {
                     conv_any<T, W>(p, lo, hi, row, batch, ch, c);
                 } else {
                     if (row != row_held) {
