@@ -51,3 +51,30 @@ def test_conv_input_and_output_equally_misaligned(xm, cuda, dt, width, batch, se
         close(ys, y, bound)
         assert torch.equal(last.cpu(), final)
         assert bool((dst[:o] == 5).all()) and bool((dst[o + x.numel():] == 5).all())
+
+
+# ------------------------------------------------------------------ empty index tensors
+
+
+def test_empty_index_tensors_are_absent(xm, cuda):
+    """Empty state_indices, cu_seqlens and has_initial_state are absent inputs: the given states stay as they were."""
+    g = gen(71)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    x, w = normal(g, 2, 20, 8).cuda(), normal(g, 8, 4).cuda()
+    state = normal(g, 2, 8, 3).cuda()
+    kept = state.clone()
+    want = xm.CausalConv1dFn(x, w, None, state, channels_last=1, output_final_state=1)
+    got = xm.CausalConv1dFn(x, w, None, state, none, none, none, channels_last=1, output_final_state=1)
+    assert got[1] is not state and torch.equal(state, kept)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = xm.CausalConv1dFn(x, w, None, None, none, none, none, channels_last=1, output_final_state=1)
+    want = xm.CausalConv1dFn(x, w, channels_last=1, output_final_state=1)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    A, B, C = -torch.rand(8, 4).cuda(), normal(g, 2, 20, 4).cuda(), normal(g, 2, 20, 4).cuda()
+    state = normal(g, 2, 8, 4).cuda()
+    kept = state.clone()
+    want = xm.SelectiveScanVarlenFn(x, x, A, B, C, None, None, None, state, delta_softplus=1, output_final_state=1)
+    got = xm.SelectiveScanVarlenFn(x, x, A, B, C, None, None, None, state, none, none, none, delta_softplus=1,
+                                   output_final_state=1)
+    assert got[1] is not state and torch.equal(state, kept)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -529,11 +529,16 @@ _UPDATE = _ServeOp("selective_state_update", ("u", "delta", "A", "B", "C", "D", 
                                               "state_indices"), "xxfxxfxffi", 8)
 
 
+def _given(t):
+    """Whether an optional input takes part: an empty tensor is an absent one."""
+    return t is not None and not (hasattr(t, "numel") and t.numel() == 0)
+
+
 def _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state, row):
     """Shape of the state output that a prompt call allocates; None: the pool itself is the output."""
-    if state_indices is not None or (final_state is not None and final_state is initial_state):
+    if _given(state_indices) or (final_state is not None and final_state is initial_state):
         return None
-    return (x.shape[0] if cu_seqlens is None else max(0, cu_seqlens.numel() - 1), *row)
+    return (cu_seqlens.numel() - 1 if _given(cu_seqlens) else x.shape[0], *row)
 
 
 def CausalConv1dFn(x, weight, bias=None, initial_state=None, cu_seqlens=None, state_indices=None,
