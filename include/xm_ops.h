@@ -293,7 +293,9 @@ xm_status xm_gated_deltanet2_fwd_static_ws(const xm_gated_deltanet2_attrs *attrs
  *    from zeros and stores no final state; a single-token row is skipped, its
  *    output row left as it was (padding of a captured graph's batch). Two
  *    sequences of one call must not own the same slot: nothing else is touched
- *    then, but their outputs and the slot's state are not defined.
+ *    then, but their outputs and the slot's state are not defined. A call
+ *    without sequences (batch 0, empty state_indices) takes a pool of any size
+ *    and leaves it as it was.
  *  - cu_seqlens (int32 or int64, [sequences + 1] ascending offsets [0, ...])
  *    packs sequences into the single batch row; lengths of zero are allowed, and
  *    positions behind the last offset are neither read nor written. Offsets are

@@ -3,6 +3,7 @@ means, limits, and what the sources promise to the compiler."""
 
 from __future__ import annotations
 
+import test_serving_cpu as C
 import torch
 
 
@@ -18,3 +19,29 @@ def test_empty_indices_allocate_the_state_output(xm):
             assert shape(x, cu, slots, state, None, row) is None
             assert shape(x, cu, empty, state, state, row) is None
         assert shape(x[:1], torch.tensor([0, 4, 20]), empty, None, None, row) == (2, 8, 4)
+
+
+# ------------------------------------------------------------------ calls without sequences
+
+
+def test_no_sequences_over_a_pool(xm):
+    """Batch 0 with empty state_indices takes a pool of any size and needs no device."""
+    m = C.Maker(xm)
+    calls = [
+        ("causal_conv1d", xm.CausalConv1dAttrs(1, 0, 1), C.conv_in(m, x=(0, 8, 16), init=(64, 8, 3)), 3, (0, 8, 16)),
+        ("causal_conv1d", xm.CausalConv1dAttrs(1, 1, 1), C.conv_in(m, x=(0, 16, 8), init=(64, 8, 3)), 3, (0, 16, 8)),
+        ("selective_scan_varlen", xm.SelectiveScanVarlenAttrs(1, 1),
+         C.scan_in(m, u=(0, 16, 8), B=(0, 16, 1, 4), init=(64, 8, 4)), 8, (0, 16, 8)),
+        ("causal_conv1d_update", xm.CausalConv1dUpdateAttrs(1), C.conv_update_in(m, x=(0, 8), state=(64, 8, 3)), 3, (0, 8)),
+        ("selective_state_update", xm.SelectiveStateUpdateAttrs(1),
+         C.update_in(m, u=(0, 8), B=(0, 4), state=(64, 8, 4)), 8, (0, 8)),
+    ]
+    for op, attrs, tensors, state, shape in calls:
+        assert C.shape_query(xm, op, attrs, tensors)[::2] == (0, shape)
+        assert C.fwd(xm, op, attrs, tensors, [m(shape, C.BF16), tensors[state]])[0] == 0
+        wrong = list(tensors)
+        wrong[state] = m((64, 8, 5), tensors[state].dtype)
+        assert "must have shape (sequences, dim" in C.shape_query(xm, op, attrs, wrong)[1]
+    state, none = torch.zeros(64, 8, 4), torch.empty(0, dtype=torch.int32)
+    assert xm._prompt_state_shape(torch.zeros(0, 6, 8), None, none, state, None, (8, 4)) is None
+    assert xm._prompt_state_shape(torch.zeros(0, 6, 8), None, none, None, None, (8, 4)) == (0, 8, 4)

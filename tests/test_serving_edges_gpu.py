@@ -78,3 +78,24 @@ def test_empty_index_tensors_are_absent(xm, cuda):
                                    output_final_state=1)
     assert got[1] is not state and torch.equal(state, kept)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_empty_batch_over_a_pool(xm, cuda):
+    """A step without sequences: empty outputs, the pool returned as it was."""
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    w, A = torch.rand(8, 4, device="cuda"), -torch.rand(8, 4, device="cuda")
+    cs, ss = torch.rand(5, 8, 3, device="cuda"), torch.rand(5, 8, 4, device="cuda")
+    kc, ks = cs.clone(), ss.clone()
+    x2, b2 = torch.empty(0, 8, device="cuda"), torch.empty(0, 4, device="cuda")
+    x3, b3 = torch.empty(0, 6, 8, device="cuda"), torch.empty(0, 6, 4, device="cuda")
+    y, s = xm.CausalConv1dUpdateFn(x2, w, None, cs, none)
+    assert y.shape == x2.shape and s is cs
+    y, s = xm.SelectiveStateUpdateFn(x2, x2, A, b2, b2, state=ss, state_indices=none)
+    assert y.shape == x2.shape and s is ss
+    y, s = xm.CausalConv1dFn(x3, w, None, cs, None, none, none, channels_last=1, output_final_state=1)
+    assert y.shape == x3.shape and s is cs
+    y, s = xm.SelectiveScanVarlenFn(x3, x3, A, b3, b3, None, None, None, ss, None, none, none, output_final_state=1)
+    assert y.shape == x3.shape and s is ss
+    y, s = xm.SelectiveScanVarlenFn(x3, x3, A, b3, b3, output_final_state=1)
+    assert y.shape == x3.shape and s.shape == (0, 8, 4)
+    assert torch.equal(cs, kc) and torch.equal(ss, ks)

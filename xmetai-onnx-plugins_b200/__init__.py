@@ -536,9 +536,11 @@ def _given(t):
 
 def _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state, row):
     """Shape of the state output that a prompt call allocates; None: the pool itself is the output."""
-    if _given(state_indices) or (final_state is not None and final_state is initial_state):
+    units = cu_seqlens.numel() - 1 if _given(cu_seqlens) else x.shape[0]
+    pool = _given(state_indices) or (state_indices is not None and units == 0 and _given(initial_state))
+    if pool or (final_state is not None and final_state is initial_state):
         return None
-    return (cu_seqlens.numel() - 1 if _given(cu_seqlens) else x.shape[0], *row)
+    return (units, *row)
 
 
 def CausalConv1dFn(x, weight, bias=None, initial_state=None, cu_seqlens=None, state_indices=None,

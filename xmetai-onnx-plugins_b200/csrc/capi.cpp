@@ -674,7 +674,8 @@ Shape state_shape_of(xm::SeqArgs &q, const xm_tensor &state, int32_t dtype, cons
         throw Invalid{std::string(name) + (dtype == XM_DTYPE_FLOAT ? " must be float32" : " must have the type of x")};
     if (present(state)) {
         const Shape have = shape_of(state);
-        if (q.slots != nullptr && have.size() == want.size()) want[0] = have[0];
+        // without sequences, a pool's state_indices are empty
+        if ((q.slots != nullptr || q.units == 0) && have.size() == want.size()) want[0] = have[0];
         if (have != want)
             throw Invalid{std::string(name) + " must have shape (" + (q.slots != nullptr ? "slots" : "sequences") +
                           ", " + row_text + ")"};
@@ -1161,7 +1162,7 @@ xm_status xm_causal_conv1d_fwd(const xm_causal_conv1d_attrs *attrs, const xm_ten
         const bool with_state = attrs->output_final_state != 0;
         serving_outputs(pl, inputs, n_inputs, 3, output, with_state, pl.io_dtype, "x", "final_state");
         pl.args.final_state = with_state && present(output[1]) ? output[1].data : nullptr;
-        if (!present(*output) && pl.args.final_state == nullptr) return XM_OK;
+        if (pl.args.seq.units == 0 || (!present(*output) && pl.args.final_state == nullptr)) return XM_OK;
         const cudaError_t e = xm::launch_causal_conv1d(pl.args, static_cast<cudaStream_t>(cuda_stream));
         return e == cudaSuccess ? XM_OK : cuda_fail(e);
     });
@@ -1249,7 +1250,7 @@ xm_status xm_selective_scan_varlen_fwd(const xm_selective_scan_varlen_attrs *att
         const bool with_state = attrs->output_final_state != 0;
         serving_outputs(pl, inputs, n_inputs, 8, output, with_state, XM_DTYPE_FLOAT, "u", "final_state");
         pl.args.final_state = with_state && present(output[1]) ? static_cast<float *>(output[1].data) : nullptr;
-        if (!present(*output) && pl.args.final_state == nullptr) return XM_OK;
+        if (pl.args.seq.units == 0 || (!present(*output) && pl.args.final_state == nullptr)) return XM_OK;
         require_workspace(workspace, workspace_bytes, xm::scan_varlen_workspace(pl.args));
         const cudaError_t e = xm::launch_scan_varlen(pl.args, workspace, static_cast<cudaStream_t>(cuda_stream));
         return e == cudaSuccess ? XM_OK : cuda_fail(e);
