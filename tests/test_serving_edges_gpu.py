@@ -99,3 +99,41 @@ def test_empty_batch_over_a_pool(xm, cuda):
     y, s = xm.SelectiveScanVarlenFn(x3, x3, A, b3, b3, output_final_state=1)
     assert y.shape == x3.shape and s.shape == (0, 8, 4)
     assert torch.equal(cs, kc) and torch.equal(ss, ks)
+
+
+# ------------------------------------------------------------------ counts near 2^31
+
+
+def test_single_tokens_of_as_many_sequences_as_allowed(xm, cuda):
+    """2^31 - 4097 sequences of one channel, all but a few without a slot: those few are updated once, the others'
+    outputs stay as they were. (The counters step past 2^31 behind the last sequence.)"""
+    n = 2**31 - 4097
+    at = [0, 5, 2**30 + 1, n - 262141, n - 65536, n - 3, n - 1]
+    k = len(at)
+    pos = torch.tensor(at, device="cuda")
+    slots = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    slots[pos] = torch.arange(k, dtype=torch.int32, device="cuda")
+    g = gen(91)
+    tok = normal(g, k, 1, 1, dtype=torch.bfloat16)
+    x = torch.full((n, 1), float("nan"), dtype=torch.bfloat16, device="cuda")
+    x[pos] = tok[:, 0].cuda()
+    out = torch.full((n, 1), 7.0, dtype=torch.bfloat16, device="cuda")
+
+    def untouched():
+        changed = sum(int((part != 7).sum()) for part in out.split(2**28))
+        return changed == int((out[pos] != 7).sum())
+
+    w, state = normal(g, 1, 4), normal(g, k, 1, 3, dtype=torch.bfloat16)
+    y, bound, final = R.conv(tok, w, None, state, channels_last=True)
+    pool = state.cuda()
+    xm.CausalConv1dUpdateFn(x, w.cuda(), None, pool, slots, out=out)
+    close(out[pos].unsqueeze(1), y, bound)
+    assert torch.equal(pool.cpu(), final) and untouched()
+    out.fill_(7.0)
+    A, D, state = -torch.rand(1, 1, generator=g), normal(g, 1), normal(g, k, 1, 1)
+    y, bound, final, ferr = R.scan(tok, tok, A, tok, tok, D, None, None, state)
+    pool = state.cuda()
+    xm.SelectiveStateUpdateFn(x, x, A.cuda(), x, x, D.cuda(), None, None, pool, slots, delta_softplus=1, out=out)
+    close(out[pos].unsqueeze(1), y, bound)
+    close(pool, final, ferr)
+    assert untouched()

@@ -653,7 +653,8 @@ xm::SeqArgs sequences_of(int64_t batch, int64_t seqlen, const xm_tensor *cu, con
         q.cu = cu->data;
         q.cu64 = cu->dtype == XM_DTYPE_INT64;
     }
-    // The kernels count tokens, and a few behind the last, in 31 bits.
+    // The kernels count tokens, and a few behind the last, in 31 bits (the single-token ones, which step
+    // further past it, in 32).
     if (batch * seqlen > static_cast<int64_t>(INT32_MAX) - 4096)
         throw Unsupported{std::string(op) + " of 2^31 - 4096 tokens or more is not supported"};
     q.units = static_cast<int>(units);

@@ -658,11 +658,13 @@ __global__ void __launch_bounds__(kConvThreads) conv_token_kernel(const ConvArgs
     const int d = (blockIdx.x * kConvThreads + threadIdx.x) * V;
     if (d >= p.dim) return;
     const size_t D = p.dim;
-    for (int n0 = blockIdx.y * kRows; n0 < p.seq.units; n0 += gridDim.y * kRows) {
+    // (sequences are counted in 31 bits, the steps past the last one need the 32nd)
+    const unsigned units = p.seq.units;
+    for (unsigned n0 = blockIdx.y * kRows; n0 < units; n0 += gridDim.y * kRows) {
         long long row[kRows];
         Elems<T, V> x[kRows], s[kRows][W - 1];
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) row[r] = n0 + r < p.seq.units ? seq_row(p.seq, n0 + r) : -1;
+        for (int r = 0; r < kRows; ++r) row[r] = n0 + r < units ? seq_row(p.seq, n0 + r) : -1;
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             if (row[r] < 0) continue;

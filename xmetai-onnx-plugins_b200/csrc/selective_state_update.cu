@@ -99,12 +99,13 @@ __global__ void __launch_bounds__(kUpdThreads) state_token_kernel(const ScanArgs
         const int n = N - n0_lane - 4 * kLanes * k;
         return vec ? n : (n + kLanes - 1) / kLanes;
     };
-    for (int n0 = blockIdx.y * kRows; n0 < p.seq.units; n0 += gridDim.y * kRows) {
+    // (sequences are counted in 31 bits, the steps past the last one need the 32nd)
+    const unsigned units = p.seq.units;
+    for (unsigned n0 = blockIdx.y * kRows; n0 < units; n0 += gridDim.y * kRows) {
         int row[kRows];  // rows of the state are numbered in 31 bits
 #pragma unroll
-        for (int r = 0; r < kRows; ++r)
-            row[r] = n0 + r < p.seq.units ? static_cast<int>(seq_row(p.seq, n0 + r)) : -1;
-        const int mine = min(n0 + own, p.seq.units - 1);
+        for (int r = 0; r < kRows; ++r) row[r] = n0 + r < units ? static_cast<int>(seq_row(p.seq, n0 + r)) : -1;
+        const unsigned mine = min(n0 + own, units - 1);
         const size_t at = static_cast<size_t>(mine) * p.dim + d;
         const float delta = to_f32<T>(static_cast<const T *>(p.delta)[at]);
         const float u = to_f32<T>(static_cast<const T *>(p.u)[at]);
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(kUpdThreads) state_token_kernel(const ScanArgs
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const float *s = p.init + static_cast<size_t>(max(row[r], 0)) * row_elems + here;
-            const size_t bc = static_cast<size_t>(min(n0 + r, p.seq.units - 1)) * bc_elems;
+            const size_t bc = static_cast<size_t>(min(n0 + r, units - 1)) * bc_elems;
 #pragma unroll
             for (int k = 0; k < kQuads; ++k) {
                 h[r][k] = load_states<(kRows > 1)>(s + 4 * kLanes * k, row[r] >= 0 ? left(k) : 0, vec, kLanes);
