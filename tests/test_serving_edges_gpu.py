@@ -137,3 +137,19 @@ def test_single_tokens_of_as_many_sequences_as_allowed(xm, cuda):
     close(out[pos].unsqueeze(1), y, bound)
     close(pool, final, ferr)
     assert untouched()
+
+
+@pytest.mark.parametrize("channels_last", [0, 1])
+def test_more_packed_sequences_than_30_bits(xm, cuda, channels_last):
+    """2^30 + 4097 sequences of one token, each starting from zeros: y = w_last x, rounded once."""
+    n = 2**30 + 4097
+    gcuda = torch.Generator(device="cuda").manual_seed(92)
+    x = torch.empty(1, n, dtype=torch.bfloat16, device="cuda")
+    for part in x[0].split(2**28):
+        part.normal_(generator=gcuda)
+    w = torch.tensor([[0.7, -1.3]], device="cuda")
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    shape = (1, n, 1) if channels_last else (1, 1, n)
+    y = xm.CausalConv1dFn(x.view(shape), w, None, None, cu, silu=0, channels_last=channels_last)
+    for a, b in zip(y.view(-1).split(2**28), x.view(-1).split(2**28)):
+        assert torch.equal(a, (b.float() * w[0, 1]).to(torch.bfloat16))

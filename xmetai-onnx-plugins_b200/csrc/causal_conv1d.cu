@@ -178,13 +178,7 @@ __device__ __forceinline__ void store_elems(T *p, const float (&v)[V]) {
 // First sequence that starts at or behind t (units: none).
 __device__ __forceinline__ int conv_first_from(const SeqArgs &q, int t) {
     if (q.cu == nullptr) return q.seqlen > 0 ? static_cast<int>((static_cast<long long>(t) + q.seqlen - 1) / q.seqlen) : 0;
-    int lo = 0, hi = q.units;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (seq_start(q, mid) >= t) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo;
+    return seq_first_from(q, t);
 }
 
 // ------------------------------------------------------------------ tokens first

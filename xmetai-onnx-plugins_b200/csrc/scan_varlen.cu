@@ -223,13 +223,7 @@ __device__ __forceinline__ float2 scan_token(float2 (&h)[NS], const float2 (&a2)
 // First sequence whose start is at or behind t (units: none); dense rows directly.
 __device__ __forceinline__ int first_from(const SeqArgs &q, int t, int row, bool at_row_start) {
     if (q.cu == nullptr) return at_row_start ? row : row + 1;
-    int lo = 0, hi = q.units;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (seq_start(q, mid) >= t) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo;
+    return seq_first_from(q, t);
 }
 
 // kEnds: the first pass.

@@ -21,6 +21,17 @@ __device__ __forceinline__ int seq_start(const SeqArgs &q, int i) {
 // End of sequence i that starts at `start`; offsets that descend give an empty sequence.
 __device__ __forceinline__ int seq_end(const SeqArgs &q, int i, int start) { return max(start, seq_start(q, i + 1)); }
 
+// First packed sequence that starts at or behind t (units: none).
+__device__ __forceinline__ int seq_first_from(const SeqArgs &q, int t) {
+    int lo = 0, hi = q.units;
+    while (lo < hi) {
+        const int mid = lo + ((hi - lo) >> 1);  // lo + hi would pass 31 bits
+        if (seq_start(q, mid) >= t) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
 // State row of sequence i, or -1 where it owns none.
 __device__ __forceinline__ long long seq_row(const SeqArgs &q, int i) {
     if (q.slots == nullptr) return i;
