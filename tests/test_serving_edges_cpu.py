@@ -6,6 +6,8 @@ from __future__ import annotations
 import test_serving_cpu as C
 import torch
 
+from conftest import ROOT
+
 
 def test_empty_indices_allocate_the_state_output(xm):
     """An empty state_indices or cu_seqlens counts as absent, in the Python mirror as in the library."""
@@ -45,3 +47,18 @@ def test_no_sequences_over_a_pool(xm):
     state, none = torch.zeros(64, 8, 4), torch.empty(0, dtype=torch.int32)
     assert xm._prompt_state_shape(torch.zeros(0, 6, 8), None, none, state, None, (8, 4)) is None
     assert xm._prompt_state_shape(torch.zeros(0, 6, 8), None, none, None, None, (8, 4)) == (0, 8, 4)
+
+
+# ------------------------------------------------------------------ what the sources promise
+
+
+def test_asynchronous_copies_declare_that_they_touch_memory():
+    """Plain loads behind a wait, and stores before a copy, are ordered only where the asm statement says so."""
+    import re
+
+    statements = []
+    for path in sorted((ROOT / "xmetai-onnx-plugins_b200" / "csrc").glob("*.cu*")):
+        for m in re.finditer(r'asm volatile\("cp\.async(.*?)\);', path.read_text(), re.S):
+            statements.append((path.name, m.group(1)))
+    assert len(statements) >= 9
+    assert [s for s in statements if '"memory"' not in s[1]] == []

@@ -34,7 +34,7 @@ constexpr int kConvThreads = 128;
 
 __device__ __forceinline__ void cp_async8(void *smem, const void *gmem) {
     const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(s), "l"(gmem));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(s), "l"(gmem) : "memory");
 }
 
 __device__ __forceinline__ float conv_act(float v, bool silu) {

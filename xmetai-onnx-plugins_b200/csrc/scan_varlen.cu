@@ -68,9 +68,9 @@ template <int kBytes>
 __device__ __forceinline__ void copy_async(void *smem, const void *gmem) {
     const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
     if constexpr (kBytes == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(s), "l"(gmem));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(s), "l"(gmem) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(s), "l"(gmem), "n"(kBytes));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(s), "l"(gmem), "n"(kBytes) : "memory");
 }
 
 __device__ __forceinline__ float scan_silu(float z) { return z * rcp_approx(1.0f + ex2_approx(-z * kLog2e)); }

@@ -295,19 +295,20 @@ __device__ __forceinline__ void unpack8(const Raw8<__half> &r, float (&out)[8]) 
     }
 }
 
-// Asynchronous global->shared copies (cp.async, Ampere+ and sm_100a).
+// Asynchronous global->shared copies (cp.async, Ampere+ and sm_100a). All declare "memory": the copies write shared
+// memory that no C++ statement does, and a wait orders the plain loads behind it also where no barrier follows.
 // `src_bytes` < size zero-fills the tail, so out-of-range rows read as 0.
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem, int src_bytes) {
     const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(gmem), "r"(src_bytes));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(gmem), "r"(src_bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async4(void *smem, const void *gmem, int src_bytes) {
     const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(s), "l"(gmem), "r"(src_bytes));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(s), "l"(gmem), "r"(src_bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 // Token span of work unit n over tensors laid out [batch, seqlen, ...]. Without
 // cu_seqlens unit n is batch row n; with cu_seqlens (batch 1) it is packed
