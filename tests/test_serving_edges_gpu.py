@@ -153,3 +153,54 @@ def test_more_packed_sequences_than_30_bits(xm, cuda, channels_last):
     y = xm.CausalConv1dFn(x.view(shape), w, None, None, cu, silu=0, channels_last=channels_last)
     for a, b in zip(y.view(-1).split(2**28), x.view(-1).split(2**28)):
         assert torch.equal(a, (b.float() * w[0, 1]).to(torch.bfloat16))
+
+
+# ------------------------------------------------------------------ the scan's join over blocks
+
+
+SCAN = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")
+
+
+def _run_scan(xm, x, state):
+    return xm.SelectiveScanVarlenFn(*[None if x[k] is None else x[k].cuda() for k in SCAN], state.cuda(),
+                                    output_final_state=1)
+
+
+@pytest.mark.parametrize("N", [5, 16])
+def test_scan_steps_whose_sum_overflows(xm, cuda, N):
+    """Steps of 3e38 over a split axis: each block's sum passes float32's range. The states decay to zero, those with
+    A = 0 keep their value, and nothing turns into NaN."""
+    g = gen(81)
+    tokens, dim = 4096, 6
+    x = dict(u=normal(g, 1, tokens, dim), delta=torch.rand(1, tokens, dim, generator=g) * 0.1,
+             A=-torch.rand(dim, N, generator=g) - 0.1, B=normal(g, 1, tokens, N), C=normal(g, 1, tokens, N),
+             D=None, z=None, delta_bias=None)
+    x["A"][:, 0] = 0.0
+    huge = slice(500, 2500)
+    x["delta"][:, huge] = 3e38
+    x["u"][:, huge] = 0.0
+    state = normal(g, 1, dim, N)
+    y, bound, final, ferr = R.scan(**x, state=state, softplus=False)
+    assert torch.isfinite(y).all() and torch.isfinite(final).all()
+    got, last = _run_scan(xm, x, state)
+    close(got, y, bound)
+    close(last, final, ferr)
+
+
+def test_scan_growth_past_float_range_in_a_block(xm, cuda):
+    """Growing states whose factor over a block is above 2^128: zero states stay zero, tiny ones grow to the value that
+    token by token gives."""
+    g = gen(82)
+    tokens, dim, N = 4096, 24, 3
+    x = dict(u=torch.zeros(1, tokens, dim), delta=torch.zeros(1, tokens, dim), A=torch.ones(dim, N),
+             B=normal(g, 1, tokens, N), C=normal(g, 1, tokens, N), D=None, z=None, delta_bias=None)
+    for c in range(dim):
+        x["delta"][:, 1000 + 8 * c:1050 + 8 * c, c] = 2.2
+    state = torch.zeros(1, dim, N)
+    state[:, :, 1] = 1e-30
+    state[:, :, 2] = -1e-35
+    y, bound, final, ferr = R.scan(**x, state=state, softplus=False)
+    assert torch.isfinite(y).all() and float(final.abs().max()) > 1e17
+    got, last = _run_scan(xm, x, state)
+    close(got, y, bound)
+    close(last, final, ferr)

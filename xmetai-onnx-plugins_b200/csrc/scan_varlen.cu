@@ -41,6 +41,7 @@
 // where a later block stores the final state into it, so in-place states are
 // never read after another block's store.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 #include "xm_common.cuh"
@@ -475,11 +476,15 @@ __global__ void __launch_bounds__(Shape<T, NS, kLanes>::kThreads) scan_block_ker
 #pragma unroll
             for (int k = 0; k < kJoin; ++k) {
                 if (b + k >= j) break;
+                // In two factors of half the exponent: a block's growth may pass float32's range where zero has to
+                // stay zero and a small state grow to what token by token gives (2^254 takes every state there is
+                // to infinity).
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    const float m = sd[k][i / (NS / 2)];
+                    const float m = 0.5f * sd[k][i / (NS / 2)];
                     const float2 x = __fmul2_rn(make_float2(m, m), a2[i]);
-                    h[i] = __ffma2_rn(make_float2(ex2_approx(x.x), ex2_approx(x.y)), h[i], v[k][i]);
+                    const float2 e = make_float2(ex2_approx(fminf(x.x, 127.0f)), ex2_approx(fminf(x.y, 127.0f)));
+                    h[i] = __ffma2_rn(e, __fmul2_rn(e, h[i]), v[k][i]);
                 }
             }
         }
@@ -626,8 +631,9 @@ __global__ void __launch_bounds__(Shape<T, NS, kLanes>::kThreads) scan_block_ker
         store_row(g.H, b0 + j, h);
         if (crossing && part == 0) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-                if (active[m]) g.S[static_cast<size_t>(b0 + j) * p.dim + d[m]] = ssum[m];
+            for (int m = 0; m < 2; ++m)  // a sum past float32's range stays finite: times A = 0 it has to be 0
+                if (active[m])
+                    g.S[static_cast<size_t>(b0 + j) * p.dim + d[m]] = fminf(fmaxf(ssum[m], -FLT_MAX), FLT_MAX);
         }
     } else if (e <= stop || !holding) {
         event(stop);
