@@ -364,6 +364,9 @@ xm_status xm_causal_conv1d_update_fwd(const xm_causal_conv1d_update_attrs *attrs
  * Outputs: y (u's shape and type; gated whenever z is given, unlike
  *   SelectiveScanFn's reference quirk); with output_final_state the float32
  *   state after every sequence's last token (its starting state when it is empty).
+ * Limit: fewer than 2^31 blocks of channels, batch x n_groups x (dim / n_groups)
+ * over 32 channels, rounded up (64 channels for d_state 17 to 32, 16 for 65 to
+ * 128, 8 above).
  * The workspace holds the state at the end of each block of tokens where the
  * sequences are split over the long axis. */
 typedef struct xm_selective_scan_varlen_attrs {

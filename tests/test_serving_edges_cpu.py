@@ -3,6 +3,8 @@ means, limits, and what the sources promise to the compiler."""
 
 from __future__ import annotations
 
+import ctypes
+
 import test_serving_cpu as C
 import torch
 
@@ -62,3 +64,25 @@ def test_asynchronous_copies_declare_that_they_touch_memory():
             statements.append((path.name, m.group(1)))
     assert len(statements) >= 9
     assert [s for s in statements if '"memory"' not in s[1]] == []
+
+
+# ------------------------------------------------------------------ limits
+
+
+def test_scan_refuses_more_channel_blocks_than_a_grid_holds(xm):
+    """2^31 blocks of channels are refused by every entry, one sequence less is not."""
+    attrs = xm.SelectiveScanVarlenAttrs(1, 0)
+    for n, message in ((2**30, "SelectiveScanVarlenFn of 2^31 or more blocks of channels is not supported"),
+                       (2**30 - 1, None)):
+        m = C.Maker(xm)
+        tensors = C.scan_in(m, u=(n, 1, 2), A=(2, 1), B=(n, 1, 2, 1), D=(2,), bias=(0,))
+        rc, msg, shape = C.shape_query(xm, "selective_scan_varlen", attrs, tensors)
+        ws = ctypes.c_size_t(7)
+        size_rc = xm.load_library().xm_selective_scan_varlen_workspace_size(
+            ctypes.byref(attrs), C._array(xm, tensors), len(tensors), ctypes.byref(ws))
+        if message is None:
+            assert (rc, shape, size_rc, ws.value) == (0, (n, 1, 2), 0, 0)
+        else:
+            assert rc == size_rc == xm.XM_ERR_UNSUPPORTED and msg == message
+            rc, msg = C.fwd(xm, "selective_scan_varlen", attrs, tensors, [m((n, 1, 2), C.BF16)])
+            assert rc == xm.XM_ERR_UNSUPPORTED and msg == message

@@ -840,6 +840,8 @@ ScanPlan scan_plan(const xm_selective_scan_varlen_attrs *attrs, const xm_tensor 
     a.seq = sequences_of(pl.out_shape[0], pl.out_shape[1], &in[9], &in[10], &in[11], "SelectiveScanVarlenFn");
     pl.state_shape = state_shape_of(a.seq, in[8], XM_DTYPE_FLOAT, Shape{a.dim, a.dstate}, "initial_state",
                                     "dim, d_state");
+    if (xm::scan_varlen_blocks(a) > static_cast<int64_t>(INT32_MAX))
+        throw Unsupported{"SelectiveScanVarlenFn of 2^31 or more blocks of channels is not supported"};
     a.softplus = attrs->delta_softplus != 0;
     a.init = present(in[8]) ? static_cast<const float *>(in[8].data) : nullptr;
     return pl;

@@ -649,15 +649,21 @@ struct ScanPlan {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-ScanPlan plan_scan(const ScanArgs &a) {
-    ScanPlan pl{};
-    ScanGeom &g = pl.g;
+// Lanes per channel pair, states per lane and the channel blocks of a group.
+void plan_channels(const ScanArgs &a, ScanPlan &pl) {
     const int N = a.dstate;
     pl.ns = N <= 8 ? 4 : 8;
     pl.lanes = 2;
     while (pl.lanes * pl.ns < N) pl.lanes *= 2;
     const int cpb = 64 / pl.lanes * (N > 16 ? 4 : 1), dpg = a.dim / a.groups;
-    g.chan_blocks = std::max(1, (dpg + cpb - 1) / cpb);
+    pl.g.chan_blocks = std::max(1, (dpg + cpb - 1) / cpb);
+}
+
+ScanPlan plan_scan(const ScanArgs &a) {
+    ScanPlan pl{};
+    ScanGeom &g = pl.g;
+    const int N = a.dstate;
+    plan_channels(a, pl);
     const int rows = a.seq.cu != nullptr ? 1 : a.seq.units;
     g.row_tokens = a.seq.cu != nullptr ? a.seq.tokens : a.seq.seqlen;
     const int64_t ctas = std::max<int64_t>(1, static_cast<int64_t>(g.chan_blocks) * a.groups * rows);
@@ -707,7 +713,6 @@ cudaError_t launch_pass(const ScanArgs &a, const ScanGeom &g, cudaStream_t strea
     using S = Shape<T, NS, kLanes>;
     const int64_t rows = a.seq.cu != nullptr ? 1 : a.seq.units;
     const int64_t ctas = rows * (kEnds ? g.nbr - 1 : g.nbr) * g.chan_blocks * a.groups;
-    if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;
     if constexpr (S::kSmem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(scan_block_kernel<T, NS, kLanes, kEnds>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -746,6 +751,12 @@ cudaError_t launch_type(const ScanArgs &a, const ScanPlan &pl, cudaStream_t stre
 }
 
 }  // namespace
+
+int64_t scan_varlen_blocks(const ScanArgs &a) {
+    ScanPlan pl{};
+    plan_channels(a, pl);
+    return static_cast<int64_t>(pl.g.chan_blocks) * a.groups * (a.seq.cu != nullptr ? 1 : a.seq.units);
+}
 
 size_t scan_varlen_workspace(const ScanArgs &a) { return plan_scan(a).total; }
 

@@ -159,6 +159,9 @@ struct ScanArgs {
     float *final_state;         // or null
     void *out;
 };
+// Thread blocks of an uncut call; launch_scan_varlen takes fewer than 2^31 of them (and cuts rows only where
+// there are few).
+int64_t scan_varlen_blocks(const ScanArgs &a);
 size_t scan_varlen_workspace(const ScanArgs &a);
 // `workspace` must hold scan_varlen_workspace(a) bytes, 256-byte aligned.
 cudaError_t launch_scan_varlen(const ScanArgs &a, void *workspace, cudaStream_t stream);
