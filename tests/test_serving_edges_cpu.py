@@ -4,6 +4,9 @@ means, limits, and what the sources promise to the compiler."""
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
+import sysconfig
 
 import test_serving_cpu as C
 import torch
@@ -86,3 +89,27 @@ def test_scan_refuses_more_channel_blocks_than_a_grid_holds(xm):
             assert rc == size_rc == xm.XM_ERR_UNSUPPORTED and msg == message
             rc, msg = C.fwd(xm, "selective_scan_varlen", attrs, tensors, [m((n, 1, 2), C.BF16)])
             assert rc == xm.XM_ERR_UNSUPPORTED and msg == message
+
+
+# ------------------------------------------------------------------ building
+
+
+def _make_plan(*args):
+    return subprocess.run(["make", "-n", "-B", "-C", str(ROOT / "xmetai-onnx-plugins_b200"), *args], check=True,
+                          capture_output=True, text=True).stdout
+
+
+def test_the_c_library_builds_without_python_headers():
+    """`make` leaves the Python call path out where there are no headers for it, and names it by its Python."""
+    alone = _make_plan("PYTHON=false")
+    assert "-o libxm_ops.so" in alone and "pycall.c" not in alone
+    assert "_xm_call" + sysconfig.get_config_var("EXT_SUFFIX") in _make_plan(f"PYTHON={sys.executable}")
+
+
+def test_build_makes_the_call_path_for_this_python(monkeypatch):
+    import __graft_entry__ as entry
+
+    made = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda args, **kw: made.append(args))
+    entry.build()
+    assert f"PYTHON={sys.executable}" in made[0]

@@ -430,12 +430,15 @@ def _load_pycall():
     global _pycall
     if _pycall is None:
         import importlib.util
+        import sys
+        import sysconfig
 
         import torch
 
-        path = _PKG_DIR / "_xm_call.so"
+        path = _PKG_DIR / ("_xm_call" + sysconfig.get_config_var("EXT_SUFFIX"))
         if not path.exists():
-            raise XmError(XM_ERR_UNSUPPORTED, f"{path} not found; build it with `make -C {_PKG_DIR}`")
+            raise XmError(XM_ERR_UNSUPPORTED, f"{path} not found; build it with `make -C {_PKG_DIR} "
+                                              f"PYTHON={sys.executable}` (needs this Python's headers)")
         spec = importlib.util.spec_from_file_location("_xm_call", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
