@@ -7,6 +7,8 @@ import ctypes
 import subprocess
 import sys
 import sysconfig
+import threading
+import time
 
 import test_serving_cpu as C
 import torch
@@ -113,3 +115,15 @@ def test_build_makes_the_call_path_for_this_python(monkeypatch):
     monkeypatch.setattr(entry.subprocess, "run", lambda args, **kw: made.append(args))
     entry.build()
     assert f"PYTHON={sys.executable}" in made[0]
+
+
+def test_the_call_path_lets_other_threads_run(xm):
+    """While an operator's entry point runs, the interpreter is free (libc's usleep stands in for one)."""
+    entry = ctypes.cast(ctypes.CDLL(None).usleep, ctypes.c_void_p).value
+    ran = []
+    other = threading.Thread(target=lambda: (time.sleep(0.05), ran.append(time.monotonic())))
+    other.start()
+    assert xm._load_pycall().call(entry, 0, 900_000, (), b"", (), 0, -1, None, 0) == (0, 0)
+    done = time.monotonic()
+    other.join()
+    assert ran[0] < done - 0.1

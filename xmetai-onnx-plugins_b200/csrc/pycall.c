@@ -187,7 +187,10 @@ static PyObject *call(PyObject *self, PyObject *const *a, Py_ssize_t n) {
                 ws = (void *)(uintptr_t)ptr;
             }
         }
+        /* a launch may wait for room in its queue: other threads run meanwhile (the caller's tuples hold the tensors) */
+        PyThreadState *const thread = PyEval_SaveThread();
         status = fwd(attrs, in, (int32_t)n_in, out, ws, bytes, stream);
+        PyEval_RestoreThread(thread);
     }
 answer:
     result = Py_BuildValue("(ll)", status, which);
