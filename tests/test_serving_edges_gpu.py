@@ -204,3 +204,18 @@ def test_scan_growth_past_float_range_in_a_block(xm, cuda):
     got, last = _run_scan(xm, x, state)
     close(got, y, bound)
     close(last, final, ferr)
+
+
+# ------------------------------------------------------------------ streams
+
+
+def test_streams_of_other_devices_are_refused(xm, cuda):
+    """Also the default stream of another device, whose handle equals this one's (a stand-in, so that one GPU does)."""
+    from types import SimpleNamespace
+
+    x, w = torch.rand(1, 8, 20, device="cuda"), torch.rand(8, 4, device="cuda")
+    here = torch.cuda.default_stream(0)
+    assert torch.equal(xm.CausalConv1dFn(x, w, stream=here), xm.CausalConv1dFn(x, w))
+    for handle in (here.cuda_stream, torch.cuda.Stream().cuda_stream):
+        with pytest.raises(xm.XmError, match="stream belongs to another device"):
+            xm.CausalConv1dFn(x, w, stream=SimpleNamespace(device_index=1, cuda_stream=handle))

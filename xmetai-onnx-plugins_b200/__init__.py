@@ -490,11 +490,12 @@ def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
         with torch.cuda.device(index):
             return _serve(op, attrs, tensors, out, state, state_shape, with_state, stream)
     handle = torch._C._cuda_getCurrentRawStream(index)
-    if stream is not None and stream.cuda_stream != handle:
-        if stream.device_index != index:
+    if stream is not None:
+        if stream.device_index != index:  # (default streams of all devices have the same handle)
             _invalid("stream belongs to another device")
-        with torch.cuda.stream(stream):
-            return _serve(op, attrs, tensors, out, state, state_shape, with_state, None)
+        if stream.cuda_stream != handle:
+            with torch.cuda.stream(stream):
+                return _serve(op, attrs, tensors, out, state, state_shape, with_state, None)
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     inplace = -1
