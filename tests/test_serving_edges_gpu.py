@@ -219,3 +219,22 @@ def test_streams_of_other_devices_are_refused(xm, cuda):
     for handle in (here.cuda_stream, torch.cuda.Stream().cuda_stream):
         with pytest.raises(xm.XmError, match="stream belongs to another device"):
             xm.CausalConv1dFn(x, w, stream=SimpleNamespace(device_index=1, cuda_stream=handle))
+
+
+# ------------------------------------------------------------------ CausalConv1dFn, long rows
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("seqlen,cu", [(1024, None), (2048, None), (2049, None), (8192, None), (8196, None), (16384, None),
+                                       (16400, None), (20000, [0, 20000]), (40000, [0, 17000, 17003, 40000])])
+def test_conv_rows_around_the_choice_of_runs(xm, cuda, dt, seqlen, cu):
+    """Channel-major rows of whole items, of many, and in between, and packed ones, with states."""
+    g = gen(seqlen)
+    batch = 2 if cu is None else 1
+    x, w, b = normal(g, batch, 3, seqlen, dtype=DT[dt]), normal(g, 3, 4), normal(g, 3)
+    state = normal(g, batch if cu is None else len(cu) - 1, 3, 3, dtype=DT[dt])
+    y, bound, final = R.conv(x, w, b, state, cu)
+    got, last = xm.CausalConv1dFn(x.cuda(), w.cuda(), b.cuda(), state.cuda(), None if cu is None else
+                                  torch.tensor(cu).cuda(), output_final_state=1)
+    close(got, y, bound)
+    assert torch.equal(last.cpu(), final)

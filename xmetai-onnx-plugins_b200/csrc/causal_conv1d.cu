@@ -747,11 +747,18 @@ cudaError_t launch_channels(const ConvArgs &a, cudaStream_t stream) {
                                                                                               at(a.out) == skew, items);
         return cudaGetLastError();
     };
-    // Runs per item share its arithmetic and cover latency, but an item that straddles rows goes word by word.
-    // 4096 channels x 16384 tokens in bfloat16: rows of 2048 tokens 112, 79 and 62 us with two, four and eight
-    // runs; rows of 2000 164, 130 and 133 us, of 1024 124, 81 and 154 us, of 100 287, 265 and 323 us.
-    const cudaError_t e = a.seq.seqlen >= 8 * 32 * V ? launch(conv_channels_kernel<T, W, 8>, 8)
-                                                     : launch(conv_channels_kernel<T, W, 4>, 4);
+    // Runs per item share its arithmetic and cover latency, but an item that straddles rows or sequences goes word
+    // by word. Eight runs where none does (rows of whole items) or few do (rows, or sequences on average, of eight
+    // items or more), else four. Microseconds per 2^26 elements in bfloat16 (items of 2048), four and eight: rows of
+    // 2048 tokens 76 and 58, of 4096 76 and 58, of 2000 129 and 134, 2500 129 and 142, 5000 110 and 125, 8200 96 and
+    // 106, 16400 88 and 85, 24000 83 and 77; rows of 2048 off a 16-byte boundary 129 and 135; packed sequences of
+    // 800 on average 253 and 275, 8192 114 and 116, 16384 101 and 95, 32768 92 and 78. float32 (items of 1024) turns
+    // between 4100 (158 and 168) and 8196 (146 and 134).
+    const int64_t item = 8 * 32 * V;
+    const int64_t length = a.seq.cu != nullptr ? a.seq.tokens / a.seq.units : a.seq.seqlen;
+    const bool whole = a.seq.cu == nullptr && skew == 0 && length % item == 0;
+    const cudaError_t e = whole || length >= 8 * item ? launch(conv_channels_kernel<T, W, 8>, 8)
+                                                      : launch(conv_channels_kernel<T, W, 4>, 4);
     if (e != cudaSuccess || a.final_state == nullptr) return e;
     const long long blocks = (static_cast<long long>(a.seq.units) * a.dim + kConvThreads - 1) / kConvThreads;
     conv_final_kernel<T, W><<<static_cast<unsigned>(std::min(blocks, 1LL << 20)), kConvThreads, 0, stream>>>(a);
