@@ -16,8 +16,10 @@
  *                     and its launcher gated_deltanet2_fwd.cu:237-304
  *   SoftmaxCPU        csrc/softmax_cpu/softmax_cpu_ort.cpp:20-114
  *
- * CausalConv1dFn, CausalConv1dUpdateFn, SelectiveScanVarlenFn and
- * SelectiveStateUpdateFn stand beside them without a counterpart there.
+ * CausalConv1dFn, CausalConv1dUpdateFn, SelectiveScanVarlenFn,
+ * SelectiveStateUpdateFn, GatedRecurrenceFn, GatedRecurrenceGradFn,
+ * GatedRecurrenceUpdateFn, LayerNormFn and LayerNormGradFn stand beside them
+ * without a counterpart there.
  *
  * Conventions
  *  - Plain pointers and sizes only. Tensors are dense row-major, exactly as the
@@ -29,7 +31,8 @@
  *  - The caller owns all memory: inputs, the output (shape from the
  *    *_output_shape query) and a workspace (size from the *_workspace_size
  *    query, 256-byte aligned; 0 bytes for SelectiveScanFn, Mamba3SisoFn, the
- *    convolutions and SelectiveStateUpdateFn).
+ *    convolutions, SelectiveStateUpdateFn, GatedRecurrenceFn,
+ *    GatedRecurrenceUpdateFn and LayerNormFn).
  *    The library allocates no memory and never synchronises the stream, so
  *    concurrent calls on different streams with separate workspaces are
  *    independent. Its only state is, per (host thread, device), two internal
@@ -404,6 +407,139 @@ xm_status xm_selective_state_update_workspace_size(const xm_selective_state_upda
 xm_status xm_selective_state_update_fwd(const xm_selective_state_update_attrs *attrs, const xm_tensor *inputs,
                                         int32_t n_inputs, xm_tensor *output, void *workspace, size_t workspace_bytes,
                                         void *cuda_stream);
+
+/* ---------------------------------------------------------------- Gated linear recurrence
+ * A diagonal recurrence whose gate comes from the input (no reference
+ * counterpart), for training and serving: per channel
+ *   a_t = lower_bound + (1 - lower_bound) sigmoid(f_t),
+ *   h_t = a_t h_(t-1) + (1 - a_t) x_t,   y_t = h_t.
+ * Types, sequences (cu_seqlens, state_indices, has_initial_state), states,
+ * absent inputs, overlap and limits are those of the serving operators; the
+ * states and lower_bound ([dim], at least 0 and below 1; empty: 0) are float32.
+ */
+
+/* GatedRecurrenceFn. Inputs (7, in order): x, f [batch, seqlen, dim],
+ *   lower_bound [dim] or empty, initial_state [sequences or slots, dim] or
+ *   empty, cu_seqlens, state_indices, has_initial_state.
+ * Outputs: y (x's shape and type); with output_final_state the float32 state
+ *   after every sequence's last token (its starting state when it is empty). */
+typedef struct xm_gated_recurrence_attrs {
+    int64_t output_final_state; /* default 0 */
+} xm_gated_recurrence_attrs;
+
+void xm_gated_recurrence_attrs_default(xm_gated_recurrence_attrs *attrs);
+xm_status xm_gated_recurrence_check_attrs(const xm_gated_recurrence_attrs *attrs);
+xm_status xm_gated_recurrence_output_shape(const xm_gated_recurrence_attrs *attrs, const xm_tensor *inputs,
+                                           int32_t n_inputs, int64_t *out_shape, int32_t *out_rank);
+xm_status xm_gated_recurrence_workspace_size(const xm_gated_recurrence_attrs *attrs, const xm_tensor *inputs,
+                                             int32_t n_inputs, size_t *bytes);
+xm_status xm_gated_recurrence_fwd(const xm_gated_recurrence_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                  xm_tensor *output, void *workspace, size_t workspace_bytes, void *cuda_stream);
+
+/* GatedRecurrenceGradFn: the backward pass. With G_t = dy_t + a_(t+1) G_(t+1),
+ * d_final_state taking the place of a G behind a sequence's last token:
+ *   dx_t = (1 - a_t) G_t,   df_t = G_t (h_(t-1) - x_t) (1 - a_t) sigmoid(f_t),
+ *   d_lower_bound = sum_t G_t (h_(t-1) - x_t) sigmoid(-f_t),
+ *   d_initial_state = a_1 G_1 of the sequence's first token.
+ * Inputs (8, in order): dy, x, f, y (GatedRecurrenceFn's output: h_(t-1) is the
+ *   y before, as it was rounded), lower_bound or empty, initial_state
+ *   [sequences, dim] or empty, cu_seqlens, d_final_state [sequences, dim] or
+ *   empty. There are no slots: a training step keeps its states per sequence.
+ * Outputs, in order: dx, df (x's shape and type); with output_lower_bound_grad
+ *   (which needs lower_bound) d_lower_bound, float32 [dim]; with
+ *   output_initial_state_grad d_initial_state, float32 [sequences, dim]
+ *   (d_final_state's row where the sequence is empty). Sums are taken in a fixed
+ *   order: equal calls give equal bits. Positions behind the last offset are
+ *   neither read nor written.
+ * The workspace holds d_lower_bound's partial sums. */
+typedef struct xm_gated_recurrence_grad_attrs {
+    int64_t output_lower_bound_grad;   /* default 0 */
+    int64_t output_initial_state_grad; /* default 0 */
+} xm_gated_recurrence_grad_attrs;
+
+void xm_gated_recurrence_grad_attrs_default(xm_gated_recurrence_grad_attrs *attrs);
+xm_status xm_gated_recurrence_grad_check_attrs(const xm_gated_recurrence_grad_attrs *attrs);
+xm_status xm_gated_recurrence_grad_output_shape(const xm_gated_recurrence_grad_attrs *attrs, const xm_tensor *inputs,
+                                                int32_t n_inputs, int64_t *out_shape, int32_t *out_rank);
+xm_status xm_gated_recurrence_grad_workspace_size(const xm_gated_recurrence_grad_attrs *attrs,
+                                                  const xm_tensor *inputs, int32_t n_inputs, size_t *bytes);
+xm_status xm_gated_recurrence_grad_fwd(const xm_gated_recurrence_grad_attrs *attrs, const xm_tensor *inputs,
+                                       int32_t n_inputs, xm_tensor *output, void *workspace, size_t workspace_bytes,
+                                       void *cuda_stream);
+
+/* GatedRecurrenceUpdateFn: GatedRecurrenceFn for one token per sequence.
+ * Inputs (5, in order): x, f [batch, dim], lower_bound or empty, state
+ *   [batch or slots, dim], state_indices.
+ * Outputs (2): y [batch, dim] and the updated state. */
+typedef struct xm_gated_recurrence_update_attrs {
+    int64_t reserved; /* must be 0 */
+} xm_gated_recurrence_update_attrs;
+
+void xm_gated_recurrence_update_attrs_default(xm_gated_recurrence_update_attrs *attrs);
+xm_status xm_gated_recurrence_update_check_attrs(const xm_gated_recurrence_update_attrs *attrs);
+xm_status xm_gated_recurrence_update_output_shape(const xm_gated_recurrence_update_attrs *attrs,
+                                                  const xm_tensor *inputs, int32_t n_inputs, int64_t *out_shape,
+                                                  int32_t *out_rank);
+xm_status xm_gated_recurrence_update_workspace_size(const xm_gated_recurrence_update_attrs *attrs,
+                                                    const xm_tensor *inputs, int32_t n_inputs, size_t *bytes);
+xm_status xm_gated_recurrence_update_fwd(const xm_gated_recurrence_update_attrs *attrs, const xm_tensor *inputs,
+                                         int32_t n_inputs, xm_tensor *output, void *workspace,
+                                         size_t workspace_bytes, void *cuda_stream);
+
+/* ---------------------------------------------------------------- Layer norm
+ * The norm around a recurrent layer with the residual sum that it is taken of
+ * (no reference counterpart), over x's last axis (dim, at most 2^30; the leading
+ * axes together fewer than 2^31 rows):
+ *   s = x + residual (x without one), rounded to x's type once and normalised as
+ *   it is stored; mean = average of s (0 with rms), rstd = 1 / sqrt(average of
+ *   (s - mean)^2 + eps); y = (s - mean) rstd weight + bias.
+ * Overloads by x's type as for the serving operators; weight and bias are
+ * float32, arithmetic is float32, the variance is taken of s - mean.
+ */
+
+/* LayerNormFn. Inputs (4, in order): x [..., dim], weight [dim] or empty (1),
+ *   bias [dim] or empty (0), residual (x's shape and type) or empty.
+ * Outputs, in order: y (x's shape and type); with a residual s (the same; it may
+ *   be the residual itself, in place); with output_stats float32 [..., 2]: mean
+ *   and rstd of every row. Other overlaps are rejected. */
+typedef struct xm_layer_norm_attrs {
+    float eps;            /* default 1e-5; finite, not negative */
+    int64_t rms;          /* default 0; non-zero: the mean counts as 0 */
+    int64_t output_stats; /* default 0 */
+} xm_layer_norm_attrs;
+
+void xm_layer_norm_attrs_default(xm_layer_norm_attrs *attrs);
+xm_status xm_layer_norm_check_attrs(const xm_layer_norm_attrs *attrs);
+xm_status xm_layer_norm_output_shape(const xm_layer_norm_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                     int64_t *out_shape, int32_t *out_rank);
+xm_status xm_layer_norm_workspace_size(const xm_layer_norm_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                       size_t *bytes);
+xm_status xm_layer_norm_fwd(const xm_layer_norm_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                            xm_tensor *output, void *workspace, size_t workspace_bytes, void *cuda_stream);
+
+/* LayerNormGradFn: the backward pass. With xhat = (x - mean) rstd and g = dy weight:
+ *   dx = rstd (g - average(g) - xhat average(g xhat)) + d_residual (no average(g) with rms),
+ *   d_weight = sum over rows of dy xhat,   d_bias = sum over rows of dy.
+ * Inputs (5, in order): dy, x (what was normalised: LayerNormFn's s where there
+ *   was a residual), weight or empty, stats [..., 2] (LayerNormFn's), d_residual
+ *   (x's shape and type: the gradient that reaches s from elsewhere) or empty.
+ * Outputs, in order: dx (x's shape and type; the gradient of x and of residual
+ *   alike); with a weight d_weight, float32 [dim]; with output_bias_grad d_bias,
+ *   float32 [dim]. Sums are taken in a fixed order: equal calls give equal bits.
+ * The workspace holds the partial sums of d_weight and d_bias. */
+typedef struct xm_layer_norm_grad_attrs {
+    int64_t rms;              /* default 0 */
+    int64_t output_bias_grad; /* default 0 */
+} xm_layer_norm_grad_attrs;
+
+void xm_layer_norm_grad_attrs_default(xm_layer_norm_grad_attrs *attrs);
+xm_status xm_layer_norm_grad_check_attrs(const xm_layer_norm_grad_attrs *attrs);
+xm_status xm_layer_norm_grad_output_shape(const xm_layer_norm_grad_attrs *attrs, const xm_tensor *inputs,
+                                          int32_t n_inputs, int64_t *out_shape, int32_t *out_rank);
+xm_status xm_layer_norm_grad_workspace_size(const xm_layer_norm_grad_attrs *attrs, const xm_tensor *inputs,
+                                            int32_t n_inputs, size_t *bytes);
+xm_status xm_layer_norm_grad_fwd(const xm_layer_norm_grad_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 xm_tensor *output, void *workspace, size_t workspace_bytes, void *cuda_stream);
 
 /* ---------------------------------------------------------------- SoftmaxCPU
  * Host-memory float32 softmax over `axis` (default -1), replacing

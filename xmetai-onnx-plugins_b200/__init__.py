@@ -12,7 +12,10 @@ xmetai-onnx-plugins, csrc/register_op.cpp:20-39, domain "xmetai_plugins"):
 Around SelectiveScanFn stand the operators that serve such a model, without a
 reference counterpart: CausalConv1dFn and SelectiveScanVarlenFn for prompts
 (packed, continuing cached states), CausalConv1dUpdateFn and
-SelectiveStateUpdateFn for single tokens.
+SelectiveStateUpdateFn for single tokens. A gated linear recurrence
+(GatedRecurrenceFn, its backward pass GatedRecurrenceGradFn and its single-token
+form GatedRecurrenceUpdateFn) and layer norm (LayerNormFn, LayerNormGradFn) serve
+training and serving alike, without a reference counterpart either.
 
 Each function takes the op's inputs in the op's order and its attributes as
 keyword arguments with the op's names and defaults, calls the C ABI of
@@ -44,6 +47,11 @@ __all__ = [
     "CausalConv1dUpdateFn",
     "SelectiveScanVarlenFn",
     "SelectiveStateUpdateFn",
+    "GatedRecurrenceFn",
+    "GatedRecurrenceGradFn",
+    "GatedRecurrenceUpdateFn",
+    "LayerNormFn",
+    "LayerNormGradFn",
     "SoftmaxCPU",
     "DOMAIN",
     "OP_NAMES",
@@ -51,7 +59,8 @@ __all__ = [
 
 DOMAIN = "xmetai_plugins"
 OP_NAMES = ("SelectiveScanFn", "Mamba3SisoFn", "GatedDeltaNet2Fn", "SoftmaxCPU", "CausalConv1dFn",
-            "CausalConv1dUpdateFn", "SelectiveScanVarlenFn", "SelectiveStateUpdateFn")
+            "CausalConv1dUpdateFn", "SelectiveScanVarlenFn", "SelectiveStateUpdateFn", "GatedRecurrenceFn",
+            "GatedRecurrenceGradFn", "GatedRecurrenceUpdateFn", "LayerNormFn", "LayerNormGradFn")
 
 _PKG_DIR = pathlib.Path(__file__).resolve().parent
 MAX_RANK = 8
@@ -135,6 +144,36 @@ class SelectiveStateUpdateAttrs(ctypes.Structure):
     _fields_ = [("delta_softplus", ctypes.c_int64)]
 
 
+class GatedRecurrenceAttrs(ctypes.Structure):
+    _fields_ = [("output_final_state", ctypes.c_int64)]
+
+
+class GatedRecurrenceGradAttrs(ctypes.Structure):
+    _fields_ = [
+        ("output_lower_bound_grad", ctypes.c_int64),
+        ("output_initial_state_grad", ctypes.c_int64),
+    ]
+
+
+class GatedRecurrenceUpdateAttrs(ctypes.Structure):
+    _fields_ = [("reserved", ctypes.c_int64)]
+
+
+class LayerNormAttrs(ctypes.Structure):
+    _fields_ = [
+        ("eps", ctypes.c_float),
+        ("rms", ctypes.c_int64),
+        ("output_stats", ctypes.c_int64),
+    ]
+
+
+class LayerNormGradAttrs(ctypes.Structure):
+    _fields_ = [
+        ("rms", ctypes.c_int64),
+        ("output_bias_grad", ctypes.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -163,6 +202,11 @@ def load_library() -> ctypes.CDLL:
         "causal_conv1d_update": CausalConv1dUpdateAttrs,
         "selective_scan_varlen": SelectiveScanVarlenAttrs,
         "selective_state_update": SelectiveStateUpdateAttrs,
+        "gated_recurrence": GatedRecurrenceAttrs,
+        "gated_recurrence_grad": GatedRecurrenceGradAttrs,
+        "gated_recurrence_update": GatedRecurrenceUpdateAttrs,
+        "layer_norm": LayerNormAttrs,
+        "layer_norm_grad": LayerNormGradAttrs,
     }
     for name, attrs in sigs.items():
         f = getattr(lib, f"xm_{name}_fwd")
@@ -422,6 +466,12 @@ def _invalid(message):
     raise XmError(XM_ERR_INVALID_ARGUMENT, message)
 
 
+def _float32():
+    import torch
+
+    return torch.float32
+
+
 _pycall = None
 
 
@@ -451,10 +501,12 @@ def _load_pycall():
 
 class _ServeOp:
     """What the calls of one serving operator share: its C entries, the tensors' names and the index of the state
-    input. `kinds` has a letter per input: x (the activations' type), f (float32) or i (int32 / int64)."""
+    input. `kinds` has a letter per input: x (the activations' type), f (float32) or i (int32 / int64). `outs` names
+    the outputs."""
 
-    def __init__(self, name, names, kinds, state, workspace=False):
+    def __init__(self, name, names, kinds, state, workspace=False, outs=("out", "the state output")):
         self.name, self.names, self.kinds, self.state, self.workspace = name, names, kinds, state, workspace
+        self.outs = outs
         self.call = None
 
     def load(self):
@@ -507,6 +559,15 @@ def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
             state = tensors[inplace] if state_shape is None else x.new_empty(
                 state_shape, dtype=torch.float32 if op.kinds[op.state] == "f" else x.dtype)
         outs = (out, state)
+    _launch(op, attrs, tensors, outs, index, inplace, handle)
+    return outs if with_state else out
+
+
+def _launch(op, attrs, tensors, outs, index, inplace, handle):
+    """Call xm_<op>_fwd on the current device `index` and the current stream `handle`."""
+    import torch
+
+    x = tensors[0]
     alloc = None
     if op.workspace:
         alloc = lambda n: x.new_empty(n, dtype=torch.uint8)  # noqa: E731
@@ -519,9 +580,34 @@ def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
         if status == -2:
             _invalid(f"{op.names[which]} is updated in place and must be contiguous")
         if status == -3:
-            _invalid(f"{'the state output' if which else 'out'} must be a contiguous tensor on cuda:{index}")
+            _invalid(f"{op.outs[which]} must be a contiguous tensor on cuda:{index}")
         _check(status)
-    return outs if with_state else out
+
+
+def _serve_many(op, attrs, tensors, outputs, stream, inplace=-1):
+    """_serve for operators with other outputs than a tensor and a state: `outputs` holds what the caller gave, or
+    (shape, dtype) of a tensor to allocate. Returns them."""
+    import torch
+
+    if op.call is None:
+        op.load()
+    x = tensors[0]
+    index = x.get_device() if isinstance(x, torch.Tensor) else -1
+    if index < 0:
+        _invalid(f"{op.names[0]} must be a CUDA tensor")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _serve_many(op, attrs, tensors, outputs, stream, inplace)
+    handle = torch._C._cuda_getCurrentRawStream(index)
+    if stream is not None:
+        if stream.device_index != index:
+            _invalid("stream belongs to another device")
+        if stream.cuda_stream != handle:
+            with torch.cuda.stream(stream):
+                return _serve_many(op, attrs, tensors, outputs, None, inplace)
+    outs = tuple([x.new_empty(o[0], dtype=o[1]) if type(o) is tuple else o for o in outputs])
+    _launch(op, attrs, tensors, outs, index, inplace, handle)
+    return outs
 
 
 _CONV = _ServeOp("causal_conv1d", ("x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices",
@@ -623,6 +709,130 @@ def SelectiveStateUpdateFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, s
     return _serve(_UPDATE, SelectiveStateUpdateAttrs(int(delta_softplus)),
                   (u, delta, A, B, C, D, z, delta_bias, state, state_indices), out, new_state,
                   None if new_state is None or new_state is state else (), True, stream)
+
+
+# ---------------------------------------------------------------- gated linear recurrence, layer norm
+
+_GATE = _ServeOp("gated_recurrence", ("x", "f", "lower_bound", "initial_state", "cu_seqlens", "state_indices",
+                                      "has_initial_state"), "xxffiii", 3)
+_GATE_GRAD = _ServeOp("gated_recurrence_grad", ("dy", "x", "f", "y", "lower_bound", "initial_state", "cu_seqlens",
+                                                "d_final_state"), "xxxxffif", 5, True, ("an output",) * 4)
+_GATE_UPDATE = _ServeOp("gated_recurrence_update", ("x", "f", "lower_bound", "state", "state_indices"), "xxffi", 3)
+_NORM = _ServeOp("layer_norm", ("x", "weight", "bias", "residual"), "xffx", 3, outs=("an output",) * 3)
+_NORM_GRAD = _ServeOp("layer_norm_grad", ("dy", "x", "weight", "stats", "d_residual"), "xxffx", 3, True,
+                      ("an output",) * 3)
+
+
+def GatedRecurrenceFn(x, f, lower_bound=None, initial_state=None, cu_seqlens=None, state_indices=None,
+                      has_initial_state=None, *, output_final_state: int = 0, stream=None, out=None, final_state=None):
+    """Gated linear recurrence over sequences: h_t = a_t h_(t-1) + (1 - a_t) x_t with
+    a_t = lower_bound + (1 - lower_bound) sigmoid(f_t); returns y = h.
+
+    x, f: [batch, seqlen, dim] in float32, bfloat16 or float16; lower_bound [dim], at least 0 and below 1, and the
+    states [sequences, dim] are float32. output_final_state, cu_seqlens, state_indices and has_initial_state work as in
+    CausalConv1dFn.
+    """
+    shape = None
+    if output_final_state:
+        if getattr(x, "ndim", 0) != 3:
+            _invalid("x must have rank 3")
+        shape = _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state, (x.shape[2],))
+    return _serve(_GATE, GatedRecurrenceAttrs(int(output_final_state)),
+                  (x, f, lower_bound, initial_state, cu_seqlens, state_indices, has_initial_state), out, final_state,
+                  shape, bool(output_final_state), stream)
+
+
+def GatedRecurrenceGradFn(dy, x, f, y, lower_bound=None, initial_state=None, cu_seqlens=None, d_final_state=None, *,
+                          output_lower_bound_grad: int | None = None, output_initial_state_grad: int | None = None,
+                          stream=None, out=None):
+    """GatedRecurrenceFn's backward pass: returns (dx, df, d_lower_bound, d_initial_state).
+
+    dy is the gradient of y, d_final_state (float32 [sequences, dim], None: zero) that of the final states; x, f,
+    lower_bound, initial_state and cu_seqlens are what the forward call took, y what it returned. d_lower_bound [dim]
+    and d_initial_state [sequences, dim] are float32 and by default there where lower_bound / initial_state are given,
+    else None. A sequence that started from zeros has a row of zeros in initial_state. out: a tuple of outputs in the
+    same order, None where one is to be allocated.
+    """
+    if getattr(dy, "ndim", 0) != 3:
+        _invalid("dy must have rank 3")
+    units = cu_seqlens.numel() - 1 if _given(cu_seqlens) else dy.shape[0]
+    lb = _given(lower_bound) if output_lower_bound_grad is None else bool(output_lower_bound_grad)
+    st = bool(output_initial_state_grad) if output_initial_state_grad is not None else (
+        _given(initial_state) or (initial_state is not None and units == 0))
+    f32 = _float32()
+    want = [(tuple(dy.shape), dy.dtype)] * 2 + [((dy.shape[2],), f32) if lb else None,
+                                                ((units, dy.shape[2]), f32) if st else None]
+    if out is not None:
+        if len(out) != 4:
+            _invalid("out must hold 4 outputs (None: allocate)")
+        want = [w if o is None or w is None else o for o, w in zip(out, want)]
+    got = iter(_serve_many(_GATE_GRAD, GatedRecurrenceGradAttrs(int(lb), int(st)),
+                           (dy, x, f, y, lower_bound, initial_state, cu_seqlens, d_final_state),
+                           [w for w in want if w is not None], stream))
+    return tuple([None if w is None else next(got) for w in want])
+
+
+def GatedRecurrenceUpdateFn(x, f, lower_bound=None, state=None, state_indices=None, *, stream=None, out=None,
+                            new_state=None):
+    """GatedRecurrenceFn for one token per sequence: x, f [batch, dim], state float32 [batch, dim], or with
+    state_indices a pool [slots, dim]. Returns (out, state) with the state updated in place; new_state (without
+    state_indices) receives it instead. Rows whose index is outside the pool are skipped and their output rows left as
+    they were."""
+    if state is None:
+        _invalid("GatedRecurrenceUpdateFn needs a state")
+    return _serve(_GATE_UPDATE, GatedRecurrenceUpdateAttrs(0), (x, f, lower_bound, state, state_indices), out, new_state,
+                  None if new_state is None or new_state is state else (), True, stream)
+
+
+def LayerNormFn(x, weight=None, bias=None, residual=None, *, eps: float = 1e-5, rms: int = 0, output_stats: int = 0,
+                stream=None, out=None, residual_out=None, stats=None):
+    """Layer norm over x's last axis, of x + residual where a residual is given: s = x + residual in x's type,
+    y = (s - mean) rstd weight + bias; with rms=1 the mean counts as 0.
+
+    x: float32, bfloat16 or float16, any number of leading axes; weight and bias [dim] are float32. Returns y, or a
+    tuple: (y, s) with a residual, and with output_stats=1 the float32 [..., 2] of every row's mean and rstd at its
+    end, which LayerNormGradFn takes. residual_out may be the residual itself: the residual stream in place.
+    """
+    if not hasattr(x, "shape") or len(x.shape) == 0:
+        _invalid("x must have at least one axis")
+    if residual is not None and not _given(residual) and not _given(x):  # no rows: the sum is as empty as its terms
+        y = LayerNormFn(x, weight, bias, eps=eps, rms=rms, output_stats=output_stats, stream=stream, out=out, stats=stats)
+        y = y if output_stats else (y,)
+        return y[:1] + (x.new_empty(x.shape) if residual_out is None else residual_out,) + y[1:]
+    many = _given(residual)
+    shape = tuple(x.shape)
+    outs = [(shape, x.dtype) if out is None else out]
+    if many:
+        outs.append((shape, x.dtype) if residual_out is None else residual_out)
+    if output_stats:
+        outs.append((shape[:-1] + (2,), _float32()) if stats is None else stats)
+    got = _serve_many(_NORM, LayerNormAttrs(float(eps), int(rms), int(output_stats)), (x, weight, bias, residual), outs,
+                      stream, 3 if many and residual_out is residual else -1)
+    return got if len(got) > 1 else got[0]
+
+
+def LayerNormGradFn(dy, x, weight=None, stats=None, d_residual=None, *, rms: int = 0, output_bias_grad: int = 0,
+                    stream=None, out=None):
+    """LayerNormFn's backward pass: returns (dx, d_weight, d_bias).
+
+    dy is the gradient of y, d_residual (None: zero) that of the residual sum; x is what was normalised (the residual
+    sum where there was a residual), weight what the forward call took, stats what it returned. dx is the gradient of
+    x and of the residual alike. d_weight is there where weight is given, d_bias with output_bias_grad=1, else None;
+    both float32 [dim]. out: a tuple of outputs in the same order, None where one is to be allocated.
+    """
+    if stats is None:
+        _invalid("LayerNormGradFn needs the forward call's stats")
+    if not hasattr(dy, "shape") or len(dy.shape) == 0:
+        _invalid("dy must have at least one axis")
+    row = ((dy.shape[-1],), _float32())
+    want = [(tuple(dy.shape), dy.dtype), row if _given(weight) else None, row if output_bias_grad else None]
+    if out is not None:
+        if len(out) != 3:
+            _invalid("out must hold 3 outputs (None: allocate)")
+        want = [w if o is None or w is None else o for o, w in zip(out, want)]
+    got = iter(_serve_many(_NORM_GRAD, LayerNormGradAttrs(int(rms), int(output_bias_grad)),
+                           (dy, x, weight, stats, d_residual), [w for w in want if w is not None], stream))
+    return tuple([None if w is None else next(got) for w in want])
 
 
 def device_wait_failures() -> int:

@@ -680,7 +680,7 @@ Shape state_shape_of(xm::SeqArgs &q, const xm_tensor &state, int32_t dtype, cons
         if (have != want)
             throw Invalid{std::string(name) + " must have shape (" + (q.slots != nullptr ? "slots" : "sequences") +
                           ", " + row_text + ")"};
-    } else if (q.slots != nullptr && row[0] * row[1] > 0) {
+    } else if (q.slots != nullptr && std::find(row.begin(), row.end(), 0) == row.end()) {
         throw Invalid{std::string("state_indices needs a non-empty ") + name};
     }
     q.n_rows = want[0];
@@ -873,6 +873,220 @@ void serving_outputs(Plan &pl, const xm_tensor *in, int32_t n, int32_t state_in,
                            state_name);
     check_overlap(in, n, state_in, output, with_state ? 2 : 1);
     pl.args.out = output->data;
+}
+
+// ------------------------------------------------------------------ gated linear recurrence
+
+struct GatePlan {
+    xm::GateArgs args;
+    Shape out_shape, state_shape;
+    int32_t io_dtype;
+};
+
+// x, f and lower_bound: in[0..2] of the recurrence and of its single-token form.
+void gate_inputs(GatePlan &pl, const xm_tensor *in, size_t lead) {
+    const int32_t io = io_type_of(in[0]);
+    require_dtype(in[0], io);
+    require_dtype(in[1], io);
+    const Shape x = shape_of(in[0]);
+    require_rank(x, lead + 1, "x");
+    require_same_shape(shape_of(in[1]), x, "f", "x");
+    if (x[lead] > kMaxServingDim) throw Unsupported{"dim above 2^30 is not supported"};
+    xm::GateArgs &a = pl.args;
+    a.bound = optional_vector(in[2], x[lead], "lower_bound", "dim");
+    a.dim = static_cast<int>(x[lead]);
+    a.io = to_io(io);
+    a.x = in[0].data;
+    a.f = in[1].data;
+    pl.out_shape = x;
+    pl.io_dtype = io;
+}
+
+GatePlan gate_plan(const xm_gated_recurrence_attrs *attrs, const xm_tensor *in, int32_t n) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    static const char *const names[7] = {"x", "f", "lower_bound", "initial_state", "cu_seqlens", "state_indices",
+                                         "has_initial_state"};
+    check_inputs(in, n, 7, names, "GatedRecurrenceFn");
+    GatePlan pl{};
+    gate_inputs(pl, in, 2);
+    xm::GateArgs &a = pl.args;
+    a.seq = sequences_of(pl.out_shape[0], pl.out_shape[1], &in[4], &in[5], &in[6], "GatedRecurrenceFn");
+    pl.state_shape = state_shape_of(a.seq, in[3], XM_DTYPE_FLOAT, Shape{a.dim}, "initial_state", "dim");
+    a.init = present(in[3]) ? static_cast<const float *>(in[3].data) : nullptr;
+    return pl;
+}
+
+void gate_update_check_attrs(const xm_gated_recurrence_update_attrs *attrs) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    if (attrs->reserved != 0) throw Invalid{"GatedRecurrenceUpdateFn has no attributes; reserved must be 0"};
+}
+
+GatePlan gate_update_plan(const xm_gated_recurrence_update_attrs *attrs, const xm_tensor *in, int32_t n) {
+    gate_update_check_attrs(attrs);
+    static const char *const names[5] = {"x", "f", "lower_bound", "state", "state_indices"};
+    check_inputs(in, n, 5, names, "GatedRecurrenceUpdateFn");
+    GatePlan pl{};
+    gate_inputs(pl, in, 1);
+    xm::GateArgs &a = pl.args;
+    a.seq = sequences_of(pl.out_shape[0], 1, nullptr, &in[4], nullptr, "GatedRecurrenceUpdateFn");
+    pl.state_shape = state_shape_of(a.seq, in[3], XM_DTYPE_FLOAT, Shape{a.dim}, "state", "dim");
+    if (present(in[0]) && !present(in[3])) throw Invalid{"GatedRecurrenceUpdateFn needs a non-empty state"};
+    a.init = static_cast<const float *>(in[3].data);
+    return pl;
+}
+
+// A gradient that an operator returns in float32.
+float *gradient_output(const xm_tensor &out, const Shape &want, const char *name, const char *text) {
+    check_tensor(&out, name);
+    if (out.dtype != XM_DTYPE_FLOAT || shape_of(out) != want)
+        throw Invalid{std::string(name) + " must be float32 with shape " + text};
+    return static_cast<float *>(out.data);
+}
+
+// No output may overlap an input or another output; output `same_out` may be
+// input `same_in` itself (-1: none).
+void check_disjoint(const xm_tensor *in, int32_t n, const xm_tensor *out, int32_t n_out, int32_t same_in = -1,
+                    int32_t same_out = -1) {
+    for (int o = 0; o < n_out; ++o) {
+        for (int i = 0; i < n; ++i)
+            if (ranges_overlap(out[o], in[i]) && !(o == same_out && i == same_in && out[o].data == in[i].data))
+                throw Invalid{"an output must not overlap an input"};
+        for (int k = 0; k < o; ++k)
+            if (ranges_overlap(out[o], out[k])) throw Invalid{"the outputs must not overlap"};
+    }
+}
+
+struct GateGradPlan {
+    xm::GateGradArgs args;
+    Shape out_shape, state_shape;
+    int32_t io_dtype;
+};
+
+GateGradPlan gate_grad_plan(const xm_gated_recurrence_grad_attrs *attrs, const xm_tensor *in, int32_t n) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    static const char *const names[8] = {"dy",          "x",             "f",          "y",
+                                         "lower_bound", "initial_state", "cu_seqlens", "d_final_state"};
+    check_inputs(in, n, 8, names, "GatedRecurrenceGradFn");
+    const int32_t io = io_type_of(in[0]);
+    const Shape shape = shape_of(in[0]);
+    require_rank(shape, 3, "dy");
+    for (int i = 0; i < 4; ++i) {
+        require_dtype(in[i], io);
+        require_same_shape(shape_of(in[i]), shape, names[i], "dy");
+    }
+    if (shape[2] > kMaxServingDim) throw Unsupported{"dim above 2^30 is not supported"};
+    GateGradPlan pl{};
+    xm::GateGradArgs &a = pl.args;
+    a.dim = static_cast<int>(shape[2]);
+    a.bound = optional_vector(in[4], shape[2], "lower_bound", "dim");
+    if (attrs->output_lower_bound_grad != 0 && a.bound == nullptr && shape[2] > 0)
+        throw Invalid{"output_lower_bound_grad requires a non-empty lower_bound"};
+    const xm_tensor none{nullptr, {0}, 1, XM_DTYPE_INT64};
+    a.seq = sequences_of(shape[0], shape[1], &in[6], &none, nullptr, "GatedRecurrenceGradFn");
+    pl.state_shape = state_shape_of(a.seq, in[5], XM_DTYPE_FLOAT, Shape{a.dim}, "initial_state", "dim");
+    state_shape_of(a.seq, in[7], XM_DTYPE_FLOAT, Shape{a.dim}, "d_final_state", "dim");
+    pl.state_shape[0] = a.seq.n_rows = a.seq.units;  // (without sequences, a state of any length counts as a pool above)
+    a.io = to_io(io);
+    a.dy = in[0].data;
+    a.x = in[1].data;
+    a.f = in[2].data;
+    a.y = in[3].data;
+    a.init = present(in[5]) ? static_cast<const float *>(in[5].data) : nullptr;
+    a.dfinal = present(in[7]) ? static_cast<const float *>(in[7].data) : nullptr;
+    pl.out_shape = shape;
+    pl.io_dtype = io;
+    a.want_dbound = attrs->output_lower_bound_grad != 0;
+    return pl;
+}
+
+// ------------------------------------------------------------------ layer norm
+
+void norm_check_attrs(const xm_layer_norm_attrs *attrs) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    if (!std::isfinite(attrs->eps) || attrs->eps < 0.0f) throw Invalid{"LayerNormFn requires a finite eps of at least 0"};
+}
+
+// Rows and dim of a tensor normalised over its last axis.
+void norm_shape(const Shape &x, const char *name, const char *op, int *rows, int *dim) {
+    if (x.empty()) throw Invalid{std::string(name) + " must have at least one axis"};
+    if (x.back() > kMaxServingDim) throw Unsupported{"dim above 2^30 is not supported"};
+    __int128 n = 1;
+    for (size_t i = 0; i + 1 < x.size(); ++i) {
+        if (x[i] == 0) n = 0;
+        else if (n <= INT32_MAX) n *= x[i];
+    }
+    if (n > INT32_MAX) throw Unsupported{std::string(op) + " of 2^31 rows or more is not supported"};
+    *rows = static_cast<int>(n);
+    *dim = static_cast<int>(x.back());
+}
+
+Shape stats_shape_of(Shape x) {
+    x.back() = 2;
+    return x;
+}
+
+struct NormPlan {
+    xm::NormArgs args;
+    Shape out_shape;
+    int32_t io_dtype;
+};
+
+NormPlan norm_plan(const xm_layer_norm_attrs *attrs, const xm_tensor *in, int32_t n) {
+    norm_check_attrs(attrs);
+    static const char *const names[4] = {"x", "weight", "bias", "residual"};
+    check_inputs(in, n, 4, names, "LayerNormFn");
+    const int32_t io = io_type_of(in[0]);
+    require_dtype(in[0], io);
+    require_dtype(in[3], io);
+    NormPlan pl{};
+    xm::NormArgs &a = pl.args;
+    pl.out_shape = shape_of(in[0]);
+    pl.io_dtype = io;
+    norm_shape(pl.out_shape, "x", "LayerNormFn", &a.rows, &a.dim);
+    a.weight = optional_vector(in[1], a.dim, "weight", "dim");
+    a.bias = optional_vector(in[2], a.dim, "bias", "dim");
+    if (present(in[3])) require_same_shape(shape_of(in[3]), pl.out_shape, "residual", "x");
+    a.eps = attrs->eps;
+    a.rms = attrs->rms != 0;
+    a.io = to_io(io);
+    a.x = in[0].data;
+    a.residual = present(in[3]) ? in[3].data : nullptr;
+    return pl;
+}
+
+struct NormGradPlan {
+    xm::NormGradArgs args;
+    Shape out_shape;
+    int32_t io_dtype;
+};
+
+NormGradPlan norm_grad_plan(const xm_layer_norm_grad_attrs *attrs, const xm_tensor *in, int32_t n) {
+    if (attrs == nullptr) throw Invalid{"attributes are null"};
+    static const char *const names[5] = {"dy", "x", "weight", "stats", "d_residual"};
+    check_inputs(in, n, 5, names, "LayerNormGradFn");
+    const int32_t io = io_type_of(in[0]);
+    require_dtype(in[0], io);
+    require_dtype(in[1], io);
+    require_dtype(in[3], XM_DTYPE_FLOAT);
+    require_dtype(in[4], io);
+    NormGradPlan pl{};
+    xm::NormGradArgs &a = pl.args;
+    pl.out_shape = shape_of(in[0]);
+    pl.io_dtype = io;
+    norm_shape(pl.out_shape, "dy", "LayerNormGradFn", &a.rows, &a.dim);
+    require_same_shape(shape_of(in[1]), pl.out_shape, "x", "dy");
+    a.weight = optional_vector(in[2], a.dim, "weight", "dim");
+    if (shape_of(in[3]) != stats_shape_of(pl.out_shape))
+        throw Invalid{"stats must have x's leading axes and a last one of 2 (mean, rstd)"};
+    if (present(in[4])) require_same_shape(shape_of(in[4]), pl.out_shape, "d_residual", "dy");
+    a.rms = attrs->rms != 0;
+    a.io = to_io(io);
+    a.dy = in[0].data;
+    a.x = in[1].data;
+    a.stats = static_cast<const float *>(in[3].data);
+    a.dres = present(in[4]) ? in[4].data : nullptr;
+    a.want_dbias = attrs->output_bias_grad != 0;
+    return pl;
 }
 
 }  // namespace
@@ -1300,6 +1514,254 @@ xm_status xm_selective_state_update_fwd(const xm_selective_state_update_attrs *a
         pl.args.final_state = static_cast<float *>(output[1].data);
         if (!present(*output)) return XM_OK;
         const cudaError_t e = xm::launch_selective_state_update(pl.args, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_gated_recurrence_attrs_default(xm_gated_recurrence_attrs *a) {
+    if (!a) return;
+    a->output_final_state = 0;
+}
+
+xm_status xm_gated_recurrence_check_attrs(const xm_gated_recurrence_attrs *attrs) {
+    return guarded([&] {
+        if (attrs == nullptr) throw Invalid{"attributes are null"};
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_output_shape(const xm_gated_recurrence_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(gate_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_workspace_size(const xm_gated_recurrence_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        gate_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = 0;
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_fwd(const xm_gated_recurrence_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("GatedRecurrenceFn");
+    (void)workspace;
+    (void)workspace_bytes;
+    return guarded([&] {
+        GatePlan pl = gate_plan(attrs, inputs, n_inputs);
+        const bool with_state = attrs->output_final_state != 0;
+        serving_outputs(pl, inputs, n_inputs, 3, output, with_state, XM_DTYPE_FLOAT, "x", "final_state");
+        pl.args.final_state = with_state && present(output[1]) ? static_cast<float *>(output[1].data) : nullptr;
+        if (pl.args.seq.units == 0 || (!present(*output) && pl.args.final_state == nullptr)) return XM_OK;
+        const cudaError_t e = xm::launch_gated_recurrence(pl.args, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_gated_recurrence_grad_attrs_default(xm_gated_recurrence_grad_attrs *a) {
+    if (!a) return;
+    a->output_lower_bound_grad = 0;
+    a->output_initial_state_grad = 0;
+}
+
+xm_status xm_gated_recurrence_grad_check_attrs(const xm_gated_recurrence_grad_attrs *attrs) {
+    return guarded([&] {
+        if (attrs == nullptr) throw Invalid{"attributes are null"};
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_grad_output_shape(const xm_gated_recurrence_grad_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(gate_grad_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_grad_workspace_size(const xm_gated_recurrence_grad_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        const GateGradPlan pl = gate_grad_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = xm::gated_recurrence_grad_workspace(pl.args);
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_grad_fwd(const xm_gated_recurrence_grad_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("GatedRecurrenceGradFn");
+    return guarded([&] {
+        GateGradPlan pl = gate_grad_plan(attrs, inputs, n_inputs);
+        xm::GateGradArgs &a = pl.args;
+        require_output(output, pl.out_shape, pl.io_dtype, "dy");
+        require_output(&output[1], pl.out_shape, pl.io_dtype, "dy");
+        int32_t outs = 2;
+        if (a.want_dbound)
+            a.dbound = gradient_output(output[outs++], Shape{a.dim}, "d_lower_bound", "(dim)");
+        if (attrs->output_initial_state_grad != 0)
+            a.dinit = gradient_output(output[outs++], pl.state_shape, "d_initial_state", "(sequences, dim)");
+        check_disjoint(inputs, n_inputs, output, outs);
+        a.dx = output[0].data;
+        a.df = output[1].data;
+        if (a.dim == 0 || (a.seq.units == 0 && !a.want_dbound)) return XM_OK;
+        require_workspace(workspace, workspace_bytes, xm::gated_recurrence_grad_workspace(a));
+        const cudaError_t e = xm::launch_gated_recurrence_grad(a, workspace, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_gated_recurrence_update_attrs_default(xm_gated_recurrence_update_attrs *a) {
+    if (!a) return;
+    a->reserved = 0;
+}
+
+xm_status xm_gated_recurrence_update_check_attrs(const xm_gated_recurrence_update_attrs *attrs) {
+    return guarded([&] {
+        gate_update_check_attrs(attrs);
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_update_output_shape(const xm_gated_recurrence_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(gate_update_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_update_workspace_size(const xm_gated_recurrence_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        gate_update_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = 0;
+        return XM_OK;
+    });
+}
+
+xm_status xm_gated_recurrence_update_fwd(const xm_gated_recurrence_update_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("GatedRecurrenceUpdateFn");
+    (void)workspace;
+    (void)workspace_bytes;
+    return guarded([&] {
+        GatePlan pl = gate_update_plan(attrs, inputs, n_inputs);
+        serving_outputs(pl, inputs, n_inputs, 3, output, true, XM_DTYPE_FLOAT, "x", "new_state");
+        pl.args.final_state = static_cast<float *>(output[1].data);
+        if (!present(*output)) return XM_OK;
+        const cudaError_t e = xm::launch_gated_recurrence_update(pl.args, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_layer_norm_attrs_default(xm_layer_norm_attrs *a) {
+    if (!a) return;
+    a->eps = 1e-5f;
+    a->rms = 0;
+    a->output_stats = 0;
+}
+
+xm_status xm_layer_norm_check_attrs(const xm_layer_norm_attrs *attrs) {
+    return guarded([&] {
+        norm_check_attrs(attrs);
+        return XM_OK;
+    });
+}
+
+xm_status xm_layer_norm_output_shape(const xm_layer_norm_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(norm_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_layer_norm_workspace_size(const xm_layer_norm_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        norm_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = 0;
+        return XM_OK;
+    });
+}
+
+xm_status xm_layer_norm_fwd(const xm_layer_norm_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("LayerNormFn");
+    (void)workspace;
+    (void)workspace_bytes;
+    return guarded([&] {
+        NormPlan pl = norm_plan(attrs, inputs, n_inputs);
+        xm::NormArgs &a = pl.args;
+        require_output(output, pl.out_shape, pl.io_dtype, "x");
+        int32_t outs = 1, sum = -1;
+        if (a.residual != nullptr) {
+            sum = outs++;
+            require_output(&output[sum], pl.out_shape, pl.io_dtype, "x");
+            a.sum = output[sum].data;
+        }
+        if (attrs->output_stats != 0)
+            a.stats = gradient_output(output[outs++], stats_shape_of(pl.out_shape), "stats", "x's with a last axis of 2");
+        check_disjoint(inputs, n_inputs, output, outs, 3, sum);
+        a.out = output->data;
+        if (a.rows == 0 || (a.dim == 0 && a.stats == nullptr)) return XM_OK;
+        if (a.dim == 0) throw Invalid{"stats of rows without elements are not defined"};
+        const cudaError_t e = xm::launch_layer_norm(a, static_cast<cudaStream_t>(cuda_stream));
+        return e == cudaSuccess ? XM_OK : cuda_fail(e);
+    });
+}
+
+void xm_layer_norm_grad_attrs_default(xm_layer_norm_grad_attrs *a) {
+    if (!a) return;
+    a->rms = 0;
+    a->output_bias_grad = 0;
+}
+
+xm_status xm_layer_norm_grad_check_attrs(const xm_layer_norm_grad_attrs *attrs) {
+    return guarded([&] {
+        if (attrs == nullptr) throw Invalid{"attributes are null"};
+        return XM_OK;
+    });
+}
+
+xm_status xm_layer_norm_grad_output_shape(const xm_layer_norm_grad_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                 int64_t *out_shape, int32_t *out_rank) {
+    return guarded([&] {
+        write_shape(norm_grad_plan(attrs, inputs, n_inputs).out_shape, out_shape, out_rank);
+        return XM_OK;
+    });
+}
+
+xm_status xm_layer_norm_grad_workspace_size(const xm_layer_norm_grad_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
+                                   size_t *bytes) {
+    return guarded([&] {
+        const NormGradPlan pl = norm_grad_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = xm::layer_norm_grad_workspace(pl.args);
+        return XM_OK;
+    });
+}
+
+xm_status xm_layer_norm_grad_fwd(const xm_layer_norm_grad_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
+                        void *workspace, size_t workspace_bytes, void *cuda_stream) {
+    XM_NVTX_RANGE("LayerNormGradFn");
+    return guarded([&] {
+        NormGradPlan pl = norm_grad_plan(attrs, inputs, n_inputs);
+        xm::NormGradArgs &a = pl.args;
+        require_output(output, pl.out_shape, pl.io_dtype, "dy");
+        int32_t outs = 1;
+        if (a.weight != nullptr) a.dweight = gradient_output(output[outs++], Shape{a.dim}, "d_weight", "(dim)");
+        if (a.want_dbias) a.dbias = gradient_output(output[outs++], Shape{a.dim}, "d_bias", "(dim)");
+        check_disjoint(inputs, n_inputs, output, outs);
+        a.dx = output->data;
+        if (a.dim == 0 || (a.rows == 0 && a.weight == nullptr && !a.want_dbias)) return XM_OK;
+        require_workspace(workspace, workspace_bytes, xm::layer_norm_grad_workspace(a));
+        const cudaError_t e = xm::launch_layer_norm_grad(a, workspace, static_cast<cudaStream_t>(cuda_stream));
         return e == cudaSuccess ? XM_OK : cuda_fail(e);
     });
 }

@@ -168,4 +168,64 @@ cudaError_t launch_scan_varlen(const ScanArgs &a, void *workspace, cudaStream_t 
 // One token per sequence: u, delta, z, out [units, dim]; init and final_state both given.
 cudaError_t launch_selective_state_update(const ScanArgs &a, cudaStream_t stream);
 
+// Gated linear recurrence over token-major tensors [tokens, dim]. The states are
+// float32 [n_rows, dim]; init and final may be the same memory.
+struct GateArgs {
+    SeqArgs seq;
+    int dim;
+    IoType io;
+    const void *x, *f;
+    const float *bound;  // lower bounds, or null
+    const float *init;   // or null
+    float *final_state;  // or null
+    void *out;
+};
+cudaError_t launch_gated_recurrence(const GateArgs &a, cudaStream_t stream);
+// One token per sequence: x, f, out [units, dim]; init and final_state both given.
+cudaError_t launch_gated_recurrence_update(const GateArgs &a, cudaStream_t stream);
+
+// Its backward pass; state rows are numbered by sequence (seq.slots and seq.live null).
+struct GateGradArgs {
+    SeqArgs seq;
+    int dim;
+    IoType io;
+    const void *dy, *x, *f, *y;
+    const float *bound, *init, *dfinal;  // or null
+    void *dx, *df;
+    bool want_dbound;  // the gradient of the lower bounds is an output
+    float *dbound, *dinit;  // or null
+};
+size_t gated_recurrence_grad_workspace(const GateGradArgs &a);
+// `workspace` must hold gated_recurrence_grad_workspace(a) bytes, 256-byte aligned.
+cudaError_t launch_gated_recurrence_grad(const GateGradArgs &a, void *workspace, cudaStream_t stream);
+
+// Layer norm over rows of dim elements.
+struct NormArgs {
+    int rows, dim;
+    float eps;
+    bool rms;
+    IoType io;
+    const void *x, *residual;    // residual may be null
+    const float *weight, *bias;  // or null
+    void *out, *sum;             // sum = x + residual, null without a residual; may be the residual
+    float *stats;                // [rows][2] mean, rstd, or null
+};
+cudaError_t launch_layer_norm(const NormArgs &a, cudaStream_t stream);
+
+// Its backward pass.
+struct NormGradArgs {
+    int rows, dim;
+    bool rms;
+    IoType io;
+    const void *dy, *x, *dres;  // dres may be null
+    const float *weight;        // or null; its gradient is an output where it is given
+    const float *stats;
+    void *dx;
+    bool want_dbias;  // the bias' gradient is an output
+    float *dweight, *dbias;
+};
+size_t layer_norm_grad_workspace(const NormGradArgs &a);
+// `workspace` must hold layer_norm_grad_workspace(a) bytes, 256-byte aligned.
+cudaError_t launch_layer_norm_grad(const NormGradArgs &a, void *workspace, cudaStream_t stream);
+
 }  // namespace xm
