@@ -29,10 +29,10 @@ def gate(f, bound):
     er = RCP + U + t / (1 + t) * et  # r = 1 / (1 + t)
     es = er + et + U  # t r
     ek, ee = torch.where(f >= 0, er, es), torch.where(f >= 0, es, er)
-    # 1 - low is rounded once, times take again; keep enters a by one fused multiply-add
+    # 1 - low is rounded, its products with keep and with take (or with r and then with t) are, and the sum is
     a = low + (1 - low) * keep
-    ea = ((1 - low) * keep * (ek + U)) / a.clamp(min=1e-300) + U
-    return dict(a=a, u=(1 - low) * take, ea=ea, eu=ee + 2 * U, keep=keep, take=take, ek=ek, et=ee)
+    ea = ((1 - low) * keep * (ek + 2 * U)) / a.clamp(min=1e-300) + U
+    return dict(a=a, u=(1 - low) * take, ea=ea, eu=ee + 3 * U, keep=keep, take=take, ek=ek, et=ee + U)
 
 
 def recurrence(x, f, bound=None, state=None, cu=None, slots=None, live=None, out=None, final=None):

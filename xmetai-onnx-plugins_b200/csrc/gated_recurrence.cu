@@ -11,129 +11,89 @@
 namespace xm {
 namespace {
 
-constexpr int kStages = 2;
+constexpr int kStages = 3;  // tiles of x and f in use and under way
 
-template <typename T, int V>
+template <typename T, bool kWords>
 struct ScanSmem {
-    GateJoin<V> join;
-    // words of x and f, each read only by the thread that copied it
-    uint32_t ring[V * sizeof(T) == 4 ? kStages : 0][2][kGateSteps][kGateThreads];
+    GateJoin join;
+    GateTile<T> ring[kWords ? kStages : 0][2];
 };
 
-// V channels per lane: two of the 16-bit types in a word (rows of even length, aligned
-// to words), else one. Words come by asynchronous copies a step ahead.
-template <typename T, int V>
+template <typename T, bool kWords>
 __global__ void __launch_bounds__(kGateThreads, 3) gate_kernel(const GateArgs p, const GateSpans g) {
     extern __shared__ float4 smem_f4[];
-    constexpr bool kAsync = V * sizeof(T) == 4;
-    auto &sm = *reinterpret_cast<ScanSmem<T, V> *>(smem_f4);
+    auto &sm = *reinterpret_cast<ScanSmem<T, kWords> *>(smem_f4);
     const SeqArgs &q = p.seq;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned rank = g.cluster > 1 ? cluster_rank() : 0;
-    const int id = blockIdx.x / g.cluster, tile = id % g.tiles, width = gridDim.x / g.cluster / g.tiles;
-    const int c0 = (tile * 32 + lane) * V;
-    const bool active = c0 < p.dim;  // (V divides dim)
-    const int c = active ? c0 : 0;
-    float low[V], rest[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        low[v] = p.bound != nullptr ? p.bound[c + v] : 0.0f;
-        rest[v] = 1.0f - low[v];
-    }
-    const T *const X = static_cast<const T *>(p.x) + c, *const F = static_cast<const T *>(p.f) + c;
-    T *const Y = static_cast<T *>(p.out) + c;
-    auto init_of = [&](int seq, float (&h)[V]) {
+    const int id = blockIdx.x / g.cluster, tile = id % g.tiles, slot = id / g.tiles;
+    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
+    T *const Y = static_cast<T *>(p.out);
+    auto init_of = [&](int seq) {
         const long long row = seq_row(q, seq);
-        const bool live = p.init != nullptr && seq_live(q, seq, row);
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = live ? p.init[row * p.dim + c + v] : 0.0f;
+        return ch.floats(p.init != nullptr && seq_live(q, seq, row) ? p.init + row * p.dim : nullptr, 0.0f);
     };
-    auto store_final = [&](int seq, const float (&h)[V]) {
+    auto store_final = [&](int seq, float2 h) {
         const long long row = seq_row(q, seq);
-        if (p.final_state == nullptr || row < 0 || !active) return;
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.final_state[row * p.dim + c + v] = h[v];
+        if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
     };
-    // sequences without tokens keep their starting states
-    if (p.final_state != nullptr && (q.cu != nullptr || q.seqlen == 0)) {
-        const int first = id / g.tiles * g.cluster + rank;
-        for (long long s0 = (static_cast<long long>(first) * kGateWarps + warp) * 32; s0 < q.units;
-             s0 += 32LL * kGateWarps * g.cluster * width) {
-            const int s = static_cast<int>(s0) + lane;
-            bool empty = false;
-            if (s < q.units) {
-                const int t = seq_start(q, s);
-                empty = seq_end(q, s, t) == t;
-            }
-            for (unsigned left = __ballot_sync(kFullMask, empty); left != 0; left &= left - 1) {
-                const int e = static_cast<int>(s0) + __ffs(left) - 1;
-                float h[V];
-                init_of(e, h);
-                store_final(e, h);
-            }
-        }
-    }
+    if (p.final_state != nullptr)  // sequences without tokens keep their starting states
+        for_empty_sequences(q, slot * g.cluster + rank, g.width * g.cluster, [&](int s) { store_final(s, init_of(s)); });
     if (g.cluster > 1) cluster_barrier();  // every block has begun before another writes into its shared memory
     const int stride = g.cluster * kGateTokens;  // tokens of a step
     int parity = 0;
-    for (int i = id / g.tiles; i < g.rows; i += width) {
+    for (int i = slot; i < g.rows; i += g.width) {
         const Span span = gate_span(q, g, i);
-        const int mine = span.lo + rank * kGateTokens + warp * kGateSteps;
-        auto copy = [&](int t0, int stage) {
-            if constexpr (kAsync) {
-                if (active) {
-#pragma unroll
-                    for (int k = 0; k < kGateSteps; ++k) {
-                        if (t0 + k < span.hi) {
-                            const size_t at = static_cast<size_t>(t0 + k) * p.dim;
-                            cp_async4(&sm.ring[stage][0][k][tid], X + at, 4);
-                            cp_async4(&sm.ring[stage][1][k][tid], F + at, 4);
-                        }
-                    }
+        const int first = span.lo + rank * kGateTokens;  // the block's first token
+        auto copy = [&](int step) {
+            if constexpr (kWords) {
+                const int t = first + step * stride, stage = step % kStages;
+                if (t < span.hi) {
+                    copy_tile<T>(sm.ring[stage][0], X, t, 0, span.hi, p.dim, tile);
+                    copy_tile<T>(sm.ring[stage][1], F, t, 0, span.hi, p.dim, tile);
                 }
                 cp_async_commit();
             }
         };
-        for (int k = 0; k < kStages; ++k) copy(mine + k * stride, k);
-        float carry[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = 0.0f;
+        if constexpr (kWords) {
+            for (int k = 0; k < kStages; ++k) copy(k);
+            cp_async_wait<kStages - 1>();
+            __syncthreads();
+        }
+        float2 carry = both(0.0f);
         SeqAt seq{0, 0, 0};
         int step = 0;
-        for (int base = span.lo; base < span.hi; base += stride, ++step) {
-            const int t0 = mine + step * stride, left = span.hi - t0;
-            const int stage = step % kStages;
-            cp_async_wait<kStages - 1>();
-            float P[kGateSteps][V], h[kGateSteps][V];
-            auto token = [&](int k, float (&x)[V], float (&f)[V]) {
-                if constexpr (kAsync) {
-                    unpack_word<T, V>(&sm.ring[stage][0][k][tid], x);
-                    unpack_word<T, V>(&sm.ring[stage][1][k][tid], f);
+        for (int base = span.lo; base < span.hi; base += stride, ++step, parity ^= 1) {
+            const int t0 = first + step * stride + warp * kGateSteps, left = span.hi - t0;
+            float2 P[kGateSteps], h[kGateSteps];
+            auto token = [&](int k, float2 &x, float2 &f) {
+                if constexpr (kWords) {
+                    const GateTile<T>(&tiles)[2] = sm.ring[step % kStages];
+                    x = tiles[0].at(warp * kGateSteps + k, lane);
+                    f = tiles[1].at(warp * kGateSteps + k, lane);
                 } else {
                     const size_t at = static_cast<size_t>(t0 + k) * p.dim;
-                    unpack_word<T, V>(X + at, x);
-                    unpack_word<T, V>(F + at, f);
+                    x = ch.load(X + at);
+                    f = ch.load(F + at);
                 }
             };
             if (left > 0 && seq.end <= t0) seq = seq_at(q, t0);
+            // no sequence starts or ends in the warp's tokens
             const bool inside = left >= kGateSteps && seq.start < t0 && seq.end > t0 + kGateSteps;
-            float rp[V], rh[V];  // the running pair
-#pragma unroll
-            for (int v = 0; v < V; ++v) rp[v] = 1.0f, rh[v] = 0.0f;
+            GatePair run{both(1.0f), both(0.0f)};
+            bool cut = false;
             if (inside) {
 #pragma unroll
                 for (int k = 0; k < kGateSteps; ++k) {
-                    float x[V], f[V];
+                    float2 x, f;
                     token(k, x, f);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const Gate gate = gate_of(f[v]);
-                        const float a = fmaf(rest[v], gate.keep, low[v]);
-                        rh[v] = fmaf(a, rh[v], rest[v] * gate.take * x[v]);
-                        rp[v] *= a;
-                        P[k][v] = rp[v];
-                        h[k][v] = rh[v];
-                    }
+                    const Gate2 gate = gate_of(f, low, rest);
+                    run.h = __ffma2_rn(gate.a, run.h, __fmul2_rn(gate.u, x));
+                    run.P = __fmul2_rn(run.P, gate.a);
+                    P[k] = run.P;
+                    h[k] = run.h;
                 }
             } else {
                 SeqAt at = seq;
@@ -142,59 +102,41 @@ __global__ void __launch_bounds__(kGateThreads, 3) gate_kernel(const GateArgs p,
                     if (k < left) {
                         if (at.end <= t0 + k) at = seq_at(q, t0 + k);
                         if (at.start == t0 + k) {
-                            init_of(at.seq, rh);
-#pragma unroll
-                            for (int v = 0; v < V; ++v) rp[v] = kCut;
+                            run.h = init_of(at.seq);
+                            cut = true;
                         }
-                        float x[V], f[V];
+                        float2 x, f;
                         token(k, x, f);
-#pragma unroll
-                        for (int v = 0; v < V; ++v) {
-                            const Gate gate = gate_of(f[v]);
-                            const float a = fmaf(rest[v], gate.keep, low[v]);
-                            rh[v] = fmaf(a, rh[v], rest[v] * gate.take * x[v]);
-                            rp[v] = rp[v] < 0.0f ? kCut : rp[v] * a;
-                        }
+                        const Gate2 gate = gate_of(f, low, rest);
+                        run.h = __ffma2_rn(gate.a, run.h, __fmul2_rn(gate.u, x));
+                        run.P = cut ? both(kCut) : __fmul2_rn(run.P, gate.a);
                     }
-#pragma unroll
-                    for (int v = 0; v < V; ++v) P[k][v] = rp[v], h[k][v] = rh[v];
+                    P[k] = run.P;
+                    h[k] = run.h;
                 }
             }
-            copy(t0 + kStages * stride, stage);
-            float start[V];
+            run.P = above_zero(run.P);
+            cp_async_wait<kStages - 2>();  // the next step's tile, which the join's barrier makes everyone's
+            const float2 start = gate_join(sm.join, parity, g.cluster, rank, run, cut, carry);
+            copy(step + kStages);  // into this step's tile: all have read it
+            if (inside && __all_sync(kFullMask, finite2(start) || !ch.active[0])) {
+                T *y = Y + static_cast<size_t>(t0) * p.dim;
 #pragma unroll
-            for (int v = 0; v < V; ++v) rp[v] = rp[v] < 0.0f ? kCut : fmaxf(rp[v], kLeast);
-            gate_join<V>(sm.join, parity, g.cluster, rank, rp, rh, carry, start);
-            parity ^= 1;
-            bool finite = true;
-#pragma unroll
-            for (int v = 0; v < V; ++v) finite = finite && fabsf(start[v]) <= 3.4028235e38f;
-            finite = finite || !active;
-            if (inside && __all_sync(kFullMask, finite)) {
-                if (active) {
-#pragma unroll
-                    for (int k = 0; k < kGateSteps; ++k) {
-                        float y[V];
-#pragma unroll
-                        for (int v = 0; v < V; ++v) y[v] = fmaf(P[k][v], start[v], h[k][v]);
-                        store_word<T, V>(Y + static_cast<size_t>(t0 + k) * p.dim, y);
-                    }
-                }
+                for (int k = 0; k < kGateSteps; ++k, y += p.dim) ch.store(y, __ffma2_rn(P[k], start, h[k]));
             } else {
                 SeqAt at = seq;
 #pragma unroll
                 for (int k = 0; k < kGateSteps; ++k) {
                     if (k >= left) break;
                     if (at.end <= t0 + k) at = seq_at(q, t0 + k);
-                    float y[V];
-#pragma unroll
-                    for (int v = 0; v < V; ++v) y[v] = through(P[k][v], start[v]) + h[k][v];
-                    if (active) store_word<T, V>(Y + static_cast<size_t>(t0 + k) * p.dim, y);
+                    const float2 y = make_float2(through(P[k].x, start.x) + h[k].x, through(P[k].y, start.y) + h[k].y);
+                    ch.store(Y + static_cast<size_t>(t0 + k) * p.dim, y);
                     if (at.end == t0 + k + 1) store_final(at.seq, y);
                 }
             }
         }
         cp_async_wait<0>();
+        __syncthreads();  // (the ring is filled anew)
     }
 }
 
@@ -204,32 +146,25 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) gate_token_kernel(const GateArgs p) {
     const int d = blockIdx.x * kThreads + threadIdx.x;
     if (d >= p.dim) return;
-    const float low = p.bound != nullptr ? p.bound[d] : 0.0f, rest = 1.0f - low;
+    const float low = p.bound != nullptr ? p.bound[d] : 0.0f;
     for (unsigned i = blockIdx.y; i < static_cast<unsigned>(p.seq.units); i += gridDim.y) {
         const long long row = seq_row(p.seq, i);
         if (row < 0) continue;
         const size_t at = static_cast<size_t>(i) * p.dim + d;
-        const Gate g = gate_of(to_f32<T>(static_cast<const T *>(p.f)[at]));
+        const Gate2 g = gate_of(both(to_f32<T>(static_cast<const T *>(p.f)[at])), both(low), both(1.0f - low));
         const float x = to_f32<T>(static_cast<const T *>(p.x)[at]);
-        const float h = fmaf(fmaf(rest, g.keep, low), p.init[row * p.dim + d], rest * g.take * x);
+        const float h = fmaf(g.a.x, p.init[row * p.dim + d], g.u.x * x);
         p.final_state[row * p.dim + d] = h;
         static_cast<T *>(p.out)[at] = from_f32<T>(h);
     }
 }
 
-template <typename T, int V>
-cudaError_t launch_words(const GateArgs &a, cudaStream_t stream) {
-    const GateSpans g = gate_spans(a.seq, a.dim, 32 * V);
-    return launch_gate_clusters(gate_kernel<T, V>, sizeof(ScanSmem<T, V>), g, stream, a, g);
-}
-
 template <typename T>
 cudaError_t launch_type(const GateArgs &a, cudaStream_t stream) {
-    if constexpr (sizeof(T) == 2) {
-        auto words = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; };
-        if (a.dim % 2 == 0 && words(a.x) && words(a.f) && words(a.out)) return launch_words<T, 2>(a, stream);
-    }
-    return launch_words<T, 1>(a, stream);
+    const GateSpans g = gate_spans(a.seq, a.dim);
+    if (a.dim * sizeof(T) % 16 == 0 && aligned16(a.x) && aligned16(a.f) && aligned16(a.out))
+        return launch_gate_clusters(gate_kernel<T, true>, sizeof(ScanSmem<T, true>), g, stream, a, g);
+    return launch_gate_clusters(gate_kernel<T, false>, sizeof(ScanSmem<T, false>), g, stream, a, g);
 }
 
 template <typename T>
@@ -241,23 +176,25 @@ cudaError_t launch_token_type(const GateArgs &a, cudaStream_t stream) {
 
 }  // namespace
 
-GateSpans gate_spans(const SeqArgs &q, int dim, int channels) {
+GateSpans gate_spans(const SeqArgs &q, int dim) {
     GateSpans g{};
-    g.tiles = (dim + channels - 1) / channels;
+    g.tiles = (dim + kGateChannels - 1) / kGateChannels;
     const int64_t want = 4LL * current_device_sm_count();  // blocks that fill the device
     if (q.cu != nullptr) {
         g.rows = 1;
         g.length = q.tokens;
     } else {
-        // rows shorter than a block's tokens share a span, as long as there are blocks enough
+        // rows shorter than a block's tokens share a span
         const int64_t per = q.seqlen > 0 ? std::max<int64_t>(1, kGateTokens / q.seqlen) : q.units;
         g.length = static_cast<int>(std::min<int64_t>(per * q.seqlen, q.tokens));
-        g.rows = g.length > 0 ? static_cast<int>((q.tokens + g.length - 1) / g.length) : 1;
+        g.rows = g.length > 0 ? static_cast<int>((static_cast<int64_t>(q.tokens) + g.length - 1) / g.length) : 1;
     }
     g.cluster = 1;
     while (g.cluster < kGateMaxCluster && g.cluster * kGateTokens < g.length &&
            static_cast<int64_t>(g.rows) * g.tiles * g.cluster < want)
         g.cluster *= 2;
+    const int64_t most = std::max<int64_t>(1, (int64_t(1) << 30) / (static_cast<int64_t>(g.tiles) * g.cluster));
+    g.width = static_cast<int>(std::min<int64_t>(g.rows, most));
     return g;
 }
 

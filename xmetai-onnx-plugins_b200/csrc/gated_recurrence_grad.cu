@@ -5,6 +5,8 @@
 //   G_t = dy_t + c,  dx_t = (1 - a_t) G_t,  c <- a_t G_t,
 //   df_t = G_t (h_(t-1) - x_t) (1 - a_t) sigmoid(f_t),
 //   d_bound += G_t (h_(t-1) - x_t) sigmoid(-f_t).
+// The recurrence of c is scanned as xm_gate.cuh says, from the last token to the
+// first.
 #include <algorithm>
 
 #include "xm_common.cuh"
@@ -15,53 +17,183 @@
 namespace xm {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kStages = 3;  // tiles in use and under way
 
-// A thread per channel walks all sequences backwards.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) gate_grad_kernel(const GateGradArgs p) {
-    const int d = blockIdx.x * kThreads + threadIdx.x;
-    if (d >= p.dim) return;
-    const float low = p.bound != nullptr ? p.bound[d] : 0.0f, rest = 1.0f - low;
-    float sum = 0.0f;
-    for (int i = 0; i < p.seq.units; ++i) {
-        const int t0 = seq_start(p.seq, i), t1 = seq_end(p.seq, i, t0);
-        const size_t srow = static_cast<size_t>(i) * p.dim + d;
-        float c = p.dfinal != nullptr ? p.dfinal[srow] : 0.0f;
-        for (int t = t1 - 1; t >= t0; --t) {
-            const size_t at = static_cast<size_t>(t) * p.dim + d;
-            const Gate g = gate_of(to_f32<T>(static_cast<const T *>(p.f)[at]));
-            const float x = to_f32<T>(static_cast<const T *>(p.x)[at]);
-            const float before = t > t0 ? to_f32<T>(static_cast<const T *>(p.y)[at - p.dim])
-                                        : (p.init != nullptr ? p.init[srow] : 0.0f);
-            const float G = to_f32<T>(static_cast<const T *>(p.dy)[at]) + c;
-            const float take = rest * g.take, da = G * (before - x);
-            static_cast<T *>(p.dx)[at] = from_f32<T>(take * G);
-            static_cast<T *>(p.df)[at] = from_f32<T>(da * take * g.keep);
-            sum = fmaf(da, g.take, sum);
-            c = fmaf(rest, g.keep, low) * G;
+template <typename T, bool kWords>
+struct GradSmem {
+    GateJoin join;
+    GateTile<T> ring[kWords ? kStages : 0][4];  // dy, x, f, and y of the token before
+};
+
+// part: [width x cluster][dim] sums of d_bound, or null.
+template <typename T, bool kWords>
+__global__ void __launch_bounds__(kGateThreads, 2) gate_grad_kernel(const GateGradArgs p, const GateSpans g, float *part) {
+    extern __shared__ float4 smem_f4[];
+    auto &sm = *reinterpret_cast<GradSmem<T, kWords> *>(smem_f4);
+    const SeqArgs &q = p.seq;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned rank = g.cluster > 1 ? cluster_rank() : 0;
+    const int id = blockIdx.x / g.cluster, tile = id % g.tiles, slot = id / g.tiles;
+    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
+                   *const F = static_cast<const T *>(p.f), *const H = static_cast<const T *>(p.y);
+    T *const DX = static_cast<T *>(p.dx), *const DF = static_cast<T *>(p.df);
+    auto state_row = [&](const float *base, int seq) {
+        return ch.floats(base != nullptr ? base + static_cast<size_t>(seq) * p.dim : nullptr, 0.0f);
+    };
+    auto store_dinit = [&](int seq, float2 c) {
+        if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
+    };
+    if (p.dinit != nullptr)  // sequences without tokens: the gradient passes through
+        for_empty_sequences(q, slot * g.cluster + rank, g.width * g.cluster,
+                            [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
+    if (g.cluster > 1) cluster_barrier();  // every block has begun before another writes into its shared memory
+    const int stride = g.cluster * kGateTokens;  // tokens of a step
+    float2 dlow = both(0.0f);                    // sum of da (1 - a)
+    int parity = 0;
+    for (int i = slot; i < g.rows; i += g.width) {
+        const Span span = gate_span(q, g, i);
+        const int first = span.hi - (rank + 1) * kGateTokens;  // the block's lowest token of the first step
+        auto copy = [&](int step) {
+            if constexpr (kWords) {
+                const int t = first - step * stride, stage = step % kStages;
+                if (t + kGateTokens > span.lo) {
+                    copy_tile<T>(sm.ring[stage][0], DY, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile<T>(sm.ring[stage][1], X, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile<T>(sm.ring[stage][2], F, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile<T>(sm.ring[stage][3], H, t - 1, span.lo, span.hi, p.dim, tile);
+                }
+                cp_async_commit();
+            }
+        };
+        if constexpr (kWords) {
+            for (int k = 0; k < kStages - 1; ++k) copy(k);
+            cp_async_wait<kStages - 2>();
+            __syncthreads();
         }
-        if (p.dinit != nullptr) p.dinit[srow] = c;
+        float2 carry = both(0.0f);
+        SeqAt seq{0, span.hi, 0};
+        int step = 0;
+        for (int base = span.lo; base < span.hi; base += stride, ++step, parity ^= 1) {
+            // the warp's tokens are t1, t1 - 1, ...; k counts them
+            const int row1 = kGateTokens - 1 - warp * kGateSteps;
+            const int t1 = first - step * stride + row1, left = t1 + 1 - span.lo;
+            auto load = [&](int which, const T *base_ptr, int k, int back) {
+                if constexpr (kWords) return sm.ring[step % kStages][which].at(row1 - k, lane);
+                else return ch.load(base_ptr + static_cast<size_t>(t1 - k - back) * p.dim);
+            };
+            if (left > 0 && seq.start > t1) seq = seq_at(q, t1);
+            // no sequence starts or ends in the warp's tokens
+            const bool inside = left >= kGateSteps && seq.end > t1 + 1 && seq.start < t1 + 1 - kGateSteps;
+            float2 P[kGateSteps], G[kGateSteps], u[kGateSteps], r[kGateSteps];  // P and G before the start is known
+            GatePair run{both(1.0f), both(0.0f)};
+            bool cut = false;
+            if (inside) {
+#pragma unroll
+                for (int k = 0; k < kGateSteps; ++k) {
+                    const Gate2 gate = gate_of(load(2, F, k, 0), low, rest);
+                    u[k] = gate.u;
+                    r[k] = gate.r;
+                    P[k] = run.P;
+                    G[k] = __fadd2_rn(load(0, DY, k, 0), run.h);
+                    run.h = __fmul2_rn(gate.a, G[k]);
+                    run.P = __fmul2_rn(run.P, gate.a);
+                }
+            } else {
+                SeqAt at = seq;
+#pragma unroll
+                for (int k = 0; k < kGateSteps; ++k) {
+                    u[k] = r[k] = P[k] = G[k] = both(0.0f);
+                    if (k < left) {
+                        if (at.start > t1 - k) at = seq_at(q, t1 - k);
+                        if (at.end == t1 - k + 1) {
+                            run.h = state_row(p.dfinal, at.seq);
+                            cut = true;
+                        }
+                        const Gate2 gate = gate_of(load(2, F, k, 0), low, rest);
+                        u[k] = gate.u;
+                        r[k] = gate.r;
+                        P[k] = cut ? both(kCut) : run.P;
+                        G[k] = __fadd2_rn(load(0, DY, k, 0), run.h);
+                        run.h = __fmul2_rn(gate.a, G[k]);
+                        run.P = __fmul2_rn(run.P, gate.a);
+                    }
+                }
+            }
+            run.P = above_zero(run.P);
+            cp_async_wait<kStages - 3>();  // the next step's tiles, which the join's barrier makes everyone's
+            const float2 start = gate_join(sm.join, parity, g.cluster, rank, run, cut, carry);
+            copy(step + kStages - 1);  // into the tiles of the step before: all are done with them
+            auto finish = [&](int k, float2 Gk, float2 before) {
+                const size_t at = static_cast<size_t>(t1 - k) * p.dim;
+                const float2 x = load(1, X, k, 0);
+                const float2 diff = make_float2(before.x - x.x, before.y - x.y);
+                const float2 w = __fmul2_rn(__fmul2_rn(Gk, diff), u[k]);
+                ch.store(DX + at, __fmul2_rn(u[k], Gk));
+                ch.store(DF + at, __fmul2_rn(w, r[k]));
+                dlow = __fadd2_rn(dlow, w);
+            };
+            if (inside && __all_sync(kFullMask, finite2(start) || !ch.active[0])) {
+#pragma unroll
+                for (int k = 0; k < kGateSteps; ++k) finish(k, __ffma2_rn(P[k], start, G[k]), load(3, H, k, 1));
+            } else {
+                SeqAt at = seq;
+#pragma unroll
+                for (int k = 0; k < kGateSteps; ++k) {
+                    if (k >= left) break;
+                    if (at.start > t1 - k) at = seq_at(q, t1 - k);
+                    const float2 Gk = make_float2(G[k].x + through(P[k].x, start.x), G[k].y + through(P[k].y, start.y));
+                    const bool begins = at.start == t1 - k;
+                    finish(k, Gk, begins ? state_row(p.init, at.seq) : load(3, H, k, 1));
+                    if (begins) store_dinit(at.seq, __fmul2_rn(__ffma2_rn(rest, r[k], low), Gk));
+                }
+            }
+        }
+        cp_async_wait<0>();
+        __syncthreads();  // (the ring is filled anew)
     }
-    if (p.dbound != nullptr) p.dbound[d] = sum;
+    if (part != nullptr) {  // the block's sum, the warps' added in order
+        sm.join.warp[0][warp][lane].h = dlow;
+        __syncthreads();
+        if (warp == 0) {
+            float2 sum = both(0.0f);
+            for (int w = 0; w < kGateWarps; ++w) sum = __fadd2_rn(sum, sm.join.warp[0][w][lane].h);
+            sum = make_float2(sum.x / rest.x, sum.y / rest.y);  // da (1 - a) = da (1 - bound) sigmoid(-f)
+            ch.store_floats(part + static_cast<size_t>(slot * g.cluster + rank) * p.dim, sum);
+        }
+    }
 }
 
 template <typename T>
-cudaError_t launch_type(const GateGradArgs &a, cudaStream_t stream) {
-    gate_grad_kernel<T><<<(a.dim + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+cudaError_t launch_type(const GateGradArgs &a, float *part, const GateSpans &g, cudaStream_t stream) {
+    if (a.dim * sizeof(T) % 16 == 0 && aligned16(a.dy) && aligned16(a.x) && aligned16(a.f) && aligned16(a.y) &&
+        aligned16(a.dx) && aligned16(a.df))
+        return launch_gate_clusters(gate_grad_kernel<T, true>, sizeof(GradSmem<T, true>), g, stream, a, g, part);
+    return launch_gate_clusters(gate_grad_kernel<T, false>, sizeof(GradSmem<T, false>), g, stream, a, g, part);
 }
 
 }  // namespace
 
-size_t gated_recurrence_grad_workspace(const GateGradArgs &) { return 0; }
+size_t gated_recurrence_grad_workspace(const GateGradArgs &a) {
+    if (!a.want_dbound || a.dim == 0) return 0;
+    const GateSpans g = gate_spans(a.seq, a.dim);
+    const size_t parts = static_cast<size_t>(g.width) * g.cluster;
+    return parts > 1 ? parts * a.dim * sizeof(float) : 0;
+}
 
-cudaError_t launch_gated_recurrence_grad(const GateGradArgs &a, void *, cudaStream_t stream) {
+cudaError_t launch_gated_recurrence_grad(const GateGradArgs &a, void *workspace, cudaStream_t stream) {
+    const GateSpans g = gate_spans(a.seq, a.dim);
+    const int parts = g.width * g.cluster;
+    float *part = a.dbound == nullptr ? nullptr : parts > 1 ? static_cast<float *>(workspace) : a.dbound;
+    cudaError_t e;
     switch (a.io) {
-        case IoType::kBF16: return launch_type<__nv_bfloat16>(a, stream);
-        case IoType::kF16: return launch_type<__half>(a, stream);
-        default: return launch_type<float>(a, stream);
+        case IoType::kBF16: e = launch_type<__nv_bfloat16>(a, part, g, stream); break;
+        case IoType::kF16: e = launch_type<__half>(a, part, g, stream); break;
+        default: e = launch_type<float>(a, part, g, stream);
     }
+    if (e != cudaSuccess || a.dbound == nullptr || parts == 1) return e;
+    return launch_column_sums(part, nullptr, parts, a.dim, a.dbound, nullptr, stream);
 }
 
 }  // namespace xm
