@@ -1099,10 +1099,12 @@ int32_t xm_abi_version(void) { return XM_ABI_VERSION; }
 
 xm_status xm_device_wait_failures(uint32_t *count) {
     if (count == nullptr) return fail(XM_ERR_INVALID_ARGUMENT, "count is null");
-    unsigned int n = 0, n2 = 0;
+    unsigned int n = 0, n2 = 0, n3 = 0, n4 = 0;
     cudaError_t e = xm::m3c_take_wait_failures(&n);
     if (e == cudaSuccess) e = xm::gdn_tc_take_wait_failures(&n2);
-    *count = n + n2;
+    if (e == cudaSuccess) e = xm::gate_take_wait_failures(&n3);
+    if (e == cudaSuccess) e = xm::gate_grad_take_wait_failures(&n4);
+    *count = n + n2 + n3 + n4;
     return e == cudaSuccess ? XM_OK : cuda_fail(e);
 }
 

@@ -11,16 +11,22 @@
 namespace xm {
 namespace {
 
-constexpr int kStages = 3;  // tiles of x and f in use and under way
+constexpr int kWarps = 4, kThreads = 32 * kWarps;  // a block's warps follow one another along the tokens
+constexpr int kSteps = 16;                         // tokens of a warp
+constexpr int kTokens = kWarps * kSteps;           // tokens of a block
+constexpr int kStages = 3;                         // tiles of x and f in use and under way
+
+__device__ unsigned int g_gate_wait_failures, g_gate_failures_taken;
+__global__ void gate_swap_failures() { g_gate_failures_taken = atomicExch(&g_gate_wait_failures, 0u); }
 
 template <typename T, bool kWords>
 struct ScanSmem {
-    GateJoin join;
-    GateTile<T> ring[kWords ? kStages : 0][2];
+    GateJoin<kWarps> join;
+    GateTile<T, kTokens> ring[kWords ? kStages : 0][2];
 };
 
 template <typename T, bool kWords>
-__global__ void __launch_bounds__(kGateThreads, 3) gate_kernel(const GateArgs p, const GateSpans g) {
+__global__ void __launch_bounds__(kThreads, 4) gate_kernel(const GateArgs p, const GateSpans g) {
     extern __shared__ float4 smem_f4[];
     auto &sm = *reinterpret_cast<ScanSmem<T, kWords> *>(smem_f4);
     const SeqArgs &q = p.seq;
@@ -40,39 +46,41 @@ __global__ void __launch_bounds__(kGateThreads, 3) gate_kernel(const GateArgs p,
         if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
     };
     if (p.final_state != nullptr)  // sequences without tokens keep their starting states
-        for_empty_sequences(q, slot * g.cluster + rank, g.width * g.cluster, [&](int s) { store_final(s, init_of(s)); });
-    if (g.cluster > 1) cluster_barrier();  // every block has begun before another writes into its shared memory
-    const int stride = g.cluster * kGateTokens;  // tokens of a step
-    int parity = 0;
+        for_empty_sequences<kWarps>(q, slot * g.cluster + rank, g.width * g.cluster, [&](int s) { store_final(s, init_of(s)); });
+    if (g.cluster > 1) gate_join_begin(sm.join);
+    if constexpr (kWords) clear_ring(sm.ring, p.dim, tile);
+    const int stride = g.cluster * kTokens;  // tokens of a step
+    unsigned turn = 0;
+    bool lost = false;
     for (int i = slot; i < g.rows; i += g.width) {
         const Span span = gate_span(q, g, i);
-        const int first = span.lo + rank * kGateTokens;  // the block's first token
-        auto copy = [&](int step) {
+        const int first = span.lo + rank * kTokens;  // the block's first token
+        auto copy = [&](int step, int stage) {
             if constexpr (kWords) {
-                const int t = first + step * stride, stage = step % kStages;
+                const int t = first + step * stride;
                 if (t < span.hi) {
-                    copy_tile<T>(sm.ring[stage][0], X, t, 0, span.hi, p.dim, tile);
-                    copy_tile<T>(sm.ring[stage][1], F, t, 0, span.hi, p.dim, tile);
+                    copy_tile<kThreads>(sm.ring[stage][0], X, t, 0, span.hi, p.dim, tile);
+                    copy_tile<kThreads>(sm.ring[stage][1], F, t, 0, span.hi, p.dim, tile);
                 }
                 cp_async_commit();
             }
         };
         if constexpr (kWords) {
-            for (int k = 0; k < kStages; ++k) copy(k);
+            for (int k = 0; k < kStages; ++k) copy(k, k);
             cp_async_wait<kStages - 1>();
             __syncthreads();
         }
         float2 carry = both(0.0f);
         SeqAt seq{0, 0, 0};
-        int step = 0;
-        for (int base = span.lo; base < span.hi; base += stride, ++step, parity ^= 1) {
-            const int t0 = first + step * stride + warp * kGateSteps, left = span.hi - t0;
-            float2 P[kGateSteps], h[kGateSteps];
+        int step = 0, stage = 0;
+        for (int base = span.lo; base < span.hi; base += stride, ++step, ++turn, stage = stage + 1 == kStages ? 0 : stage + 1) {
+            const int t0 = first + step * stride + warp * kSteps, left = span.hi - t0;
+            float2 P[kSteps], h[kSteps];
             auto token = [&](int k, float2 &x, float2 &f) {
                 if constexpr (kWords) {
-                    const GateTile<T>(&tiles)[2] = sm.ring[step % kStages];
-                    x = tiles[0].at(warp * kGateSteps + k, lane);
-                    f = tiles[1].at(warp * kGateSteps + k, lane);
+                    const GateTile<T, kTokens>(&tiles)[2] = sm.ring[stage];
+                    x = tiles[0].at(warp * kSteps + k, lane);
+                    f = tiles[1].at(warp * kSteps + k, lane);
                 } else {
                     const size_t at = static_cast<size_t>(t0 + k) * p.dim;
                     x = ch.load(X + at);
@@ -81,12 +89,12 @@ __global__ void __launch_bounds__(kGateThreads, 3) gate_kernel(const GateArgs p,
             };
             if (left > 0 && seq.end <= t0) seq = seq_at(q, t0);
             // no sequence starts or ends in the warp's tokens
-            const bool inside = left >= kGateSteps && seq.start < t0 && seq.end > t0 + kGateSteps;
+            const bool inside = left >= kSteps && seq.start < t0 && seq.end > t0 + kSteps;
             GatePair run{both(1.0f), both(0.0f)};
             bool cut = false;
             if (inside) {
 #pragma unroll
-                for (int k = 0; k < kGateSteps; ++k) {
+                for (int k = 0; k < kSteps; ++k) {
                     float2 x, f;
                     token(k, x, f);
                     const Gate2 gate = gate_of(f, low, rest);
@@ -98,7 +106,7 @@ __global__ void __launch_bounds__(kGateThreads, 3) gate_kernel(const GateArgs p,
             } else {
                 SeqAt at = seq;
 #pragma unroll
-                for (int k = 0; k < kGateSteps; ++k) {
+                for (int k = 0; k < kSteps; ++k) {
                     if (k < left) {
                         if (at.end <= t0 + k) at = seq_at(q, t0 + k);
                         if (at.start == t0 + k) {
@@ -109,28 +117,30 @@ __global__ void __launch_bounds__(kGateThreads, 3) gate_kernel(const GateArgs p,
                         token(k, x, f);
                         const Gate2 gate = gate_of(f, low, rest);
                         run.h = __ffma2_rn(gate.a, run.h, __fmul2_rn(gate.u, x));
-                        run.P = cut ? both(kCut) : __fmul2_rn(run.P, gate.a);
+                        run.P = cut ? both(0.0f) : above_zero(__fmul2_rn(run.P, gate.a));
                     }
                     P[k] = run.P;
                     h[k] = run.h;
                 }
             }
-            run.P = above_zero(run.P);
-            cp_async_wait<kStages - 2>();  // the next step's tile, which the join's barrier makes everyone's
-            const float2 start = gate_join(sm.join, parity, g.cluster, rank, run, cut, carry);
-            copy(step + kStages);  // into this step's tile: all have read it
-            if (inside && __all_sync(kFullMask, finite2(start) || !ch.active[0])) {
-                T *y = Y + static_cast<size_t>(t0) * p.dim;
+            if (inside) run.P = above_zero(run.P);
+            if constexpr (kWords) cp_async_wait<kStages - 2>();  // the next tiles, which the join's barrier makes everyone's
+            const float2 start = gate_join(sm.join, turn, g.cluster, rank, run, carry, lost);
+            copy(step + kStages, stage);  // into this step's tiles: all have read them
+            if (inside && __all_sync(kFullMask, finite2(start))) {
+                if (ch.active[0]) {
+                    T *y = Y + static_cast<size_t>(t0) * p.dim;
 #pragma unroll
-                for (int k = 0; k < kGateSteps; ++k, y += p.dim) ch.store(y, __ffma2_rn(P[k], start, h[k]));
+                    for (int k = 0; k < kSteps; ++k, y += p.dim) ch.store(y, __ffma2_rn(P[k], start, h[k]));
+                }
             } else {
                 SeqAt at = seq;
 #pragma unroll
-                for (int k = 0; k < kGateSteps; ++k) {
+                for (int k = 0; k < kSteps; ++k) {
                     if (k >= left) break;
                     if (at.end <= t0 + k) at = seq_at(q, t0 + k);
-                    const float2 y = make_float2(through(P[k].x, start.x) + h[k].x, through(P[k].y, start.y) + h[k].y);
-                    ch.store(Y + static_cast<size_t>(t0 + k) * p.dim, y);
+                    const float2 y = join_any(GatePair{inside ? above_zero(P[k]) : P[k], h[k]}, start);
+                    if (ch.active[0]) ch.store(Y + static_cast<size_t>(t0 + k) * p.dim, y);
                     if (at.end == t0 + k + 1) store_final(at.seq, y);
                 }
             }
@@ -138,13 +148,17 @@ __global__ void __launch_bounds__(kGateThreads, 3) gate_kernel(const GateArgs p,
         cp_async_wait<0>();
         __syncthreads();  // (the ring is filled anew)
     }
+    if (g.cluster > 1) {
+        if (lost && threadIdx.x == 0) atomicAdd(&g_gate_wait_failures, 1u);
+        cluster_barrier();
+    }
 }
 
-constexpr int kThreads = 128;
+constexpr int kTokenThreads = 128;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) gate_token_kernel(const GateArgs p) {
-    const int d = blockIdx.x * kThreads + threadIdx.x;
+__global__ void __launch_bounds__(kTokenThreads) gate_token_kernel(const GateArgs p) {
+    const int d = blockIdx.x * kTokenThreads + threadIdx.x;
     if (d >= p.dim) return;
     const float low = p.bound != nullptr ? p.bound[d] : 0.0f;
     for (unsigned i = blockIdx.y; i < static_cast<unsigned>(p.seq.units); i += gridDim.y) {
@@ -161,22 +175,22 @@ __global__ void __launch_bounds__(kThreads) gate_token_kernel(const GateArgs p) 
 
 template <typename T>
 cudaError_t launch_type(const GateArgs &a, cudaStream_t stream) {
-    const GateSpans g = gate_spans(a.seq, a.dim);
+    const GateSpans g = gate_spans(a.seq, a.dim, kTokens);
     if (a.dim * sizeof(T) % 16 == 0 && aligned16(a.x) && aligned16(a.f) && aligned16(a.out))
-        return launch_gate_clusters(gate_kernel<T, true>, sizeof(ScanSmem<T, true>), g, stream, a, g);
-    return launch_gate_clusters(gate_kernel<T, false>, sizeof(ScanSmem<T, false>), g, stream, a, g);
+        return launch_gate_clusters(gate_kernel<T, true>, kThreads, sizeof(ScanSmem<T, true>), g, stream, a, g);
+    return launch_gate_clusters(gate_kernel<T, false>, kThreads, sizeof(ScanSmem<T, false>), g, stream, a, g);
 }
 
 template <typename T>
 cudaError_t launch_token_type(const GateArgs &a, cudaStream_t stream) {
-    const dim3 grid((a.dim + kThreads - 1) / kThreads, std::min(a.seq.units, 65535));
-    gate_token_kernel<T><<<grid, kThreads, 0, stream>>>(a);
+    const dim3 grid((a.dim + kTokenThreads - 1) / kTokenThreads, std::min(a.seq.units, 65535));
+    gate_token_kernel<T><<<grid, kTokenThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
 }  // namespace
 
-GateSpans gate_spans(const SeqArgs &q, int dim) {
+GateSpans gate_spans(const SeqArgs &q, int dim, int tokens) {
     GateSpans g{};
     g.tiles = (dim + kGateChannels - 1) / kGateChannels;
     const int64_t want = 4LL * current_device_sm_count();  // blocks that fill the device
@@ -185,17 +199,26 @@ GateSpans gate_spans(const SeqArgs &q, int dim) {
         g.length = q.tokens;
     } else {
         // rows shorter than a block's tokens share a span
-        const int64_t per = q.seqlen > 0 ? std::max<int64_t>(1, kGateTokens / q.seqlen) : q.units;
+        const int64_t per = q.seqlen > 0 ? std::max<int64_t>(1, tokens / q.seqlen) : q.units;
         g.length = static_cast<int>(std::min<int64_t>(per * q.seqlen, q.tokens));
         g.rows = g.length > 0 ? static_cast<int>((static_cast<int64_t>(q.tokens) + g.length - 1) / g.length) : 1;
     }
     g.cluster = 1;
-    while (g.cluster < kGateMaxCluster && g.cluster * kGateTokens < g.length &&
+    while (g.cluster < kGateMaxCluster && g.cluster * tokens < g.length &&
            static_cast<int64_t>(g.rows) * g.tiles * g.cluster < want)
         g.cluster *= 2;
     const int64_t most = std::max<int64_t>(1, (int64_t(1) << 30) / (static_cast<int64_t>(g.tiles) * g.cluster));
     g.width = static_cast<int>(std::min<int64_t>(g.rows, most));
     return g;
+}
+
+cudaError_t gate_take_wait_failures(unsigned int *count) {
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) {
+        gate_swap_failures<<<1, 1>>>();
+        e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? cudaMemcpyFromSymbol(count, g_gate_failures_taken, sizeof(*count)) : e;
 }
 
 cudaError_t launch_gated_recurrence(const GateArgs &a, cudaStream_t stream) {

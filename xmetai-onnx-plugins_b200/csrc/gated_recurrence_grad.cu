@@ -17,17 +17,23 @@
 namespace xm {
 namespace {
 
-constexpr int kStages = 3;  // tiles in use and under way
+constexpr int kWarps = 8, kThreads = 32 * kWarps;  // a block's warps follow one another along the tokens
+constexpr int kSteps = 8;                          // tokens of a warp
+constexpr int kTokens = kWarps * kSteps;           // tokens of a block
+constexpr int kStages = 3;                         // tiles in use and under way
+
+__device__ unsigned int g_gate_grad_wait_failures, g_gate_grad_failures_taken;
+__global__ void gate_grad_swap_failures() { g_gate_grad_failures_taken = atomicExch(&g_gate_grad_wait_failures, 0u); }
 
 template <typename T, bool kWords>
 struct GradSmem {
-    GateJoin join;
-    GateTile<T> ring[kWords ? kStages : 0][4];  // dy, x, f, and y of the token before
+    GateJoin<kWarps> join;
+    GateTile<T, kTokens> ring[kWords ? kStages : 0][4];  // dy, x, f, and y of the token before
 };
 
 // part: [width x cluster][dim] sums of d_bound, or null.
 template <typename T, bool kWords>
-__global__ void __launch_bounds__(kGateThreads, 2) gate_grad_kernel(const GateGradArgs p, const GateSpans g, float *part) {
+__global__ void __launch_bounds__(kThreads, 2) gate_grad_kernel(const GateGradArgs p, const GateSpans g, float *part) {
     extern __shared__ float4 smem_f4[];
     auto &sm = *reinterpret_cast<GradSmem<T, kWords> *>(smem_f4);
     const SeqArgs &q = p.seq;
@@ -46,52 +52,54 @@ __global__ void __launch_bounds__(kGateThreads, 2) gate_grad_kernel(const GateGr
         if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
     };
     if (p.dinit != nullptr)  // sequences without tokens: the gradient passes through
-        for_empty_sequences(q, slot * g.cluster + rank, g.width * g.cluster,
+        for_empty_sequences<kWarps>(q, slot * g.cluster + rank, g.width * g.cluster,
                             [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
-    if (g.cluster > 1) cluster_barrier();  // every block has begun before another writes into its shared memory
-    const int stride = g.cluster * kGateTokens;  // tokens of a step
+    if (g.cluster > 1) gate_join_begin(sm.join);
+    if constexpr (kWords) clear_ring(sm.ring, p.dim, tile);
+    const int stride = g.cluster * kTokens;  // tokens of a step
     float2 dlow = both(0.0f);                    // sum of da (1 - a)
-    int parity = 0;
+    unsigned turn = 0;
+    bool lost = false;
     for (int i = slot; i < g.rows; i += g.width) {
         const Span span = gate_span(q, g, i);
-        const int first = span.hi - (rank + 1) * kGateTokens;  // the block's lowest token of the first step
-        auto copy = [&](int step) {
+        const int first = span.hi - (rank + 1) * kTokens;  // the block's lowest token of the first step
+        auto copy = [&](int step, int stage) {
             if constexpr (kWords) {
-                const int t = first - step * stride, stage = step % kStages;
-                if (t + kGateTokens > span.lo) {
-                    copy_tile<T>(sm.ring[stage][0], DY, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile<T>(sm.ring[stage][1], X, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile<T>(sm.ring[stage][2], F, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile<T>(sm.ring[stage][3], H, t - 1, span.lo, span.hi, p.dim, tile);
+                const int t = first - step * stride;
+                if (t + kTokens > span.lo) {
+                    copy_tile<kThreads>(sm.ring[stage][0], DY, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile<kThreads>(sm.ring[stage][1], X, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile<kThreads>(sm.ring[stage][2], F, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile<kThreads>(sm.ring[stage][3], H, t - 1, span.lo, span.hi, p.dim, tile);
                 }
                 cp_async_commit();
             }
         };
         if constexpr (kWords) {
-            for (int k = 0; k < kStages - 1; ++k) copy(k);
+            for (int k = 0; k < kStages - 1; ++k) copy(k, k);
             cp_async_wait<kStages - 2>();
             __syncthreads();
         }
         float2 carry = both(0.0f);
         SeqAt seq{0, span.hi, 0};
-        int step = 0;
-        for (int base = span.lo; base < span.hi; base += stride, ++step, parity ^= 1) {
+        int step = 0, stage = 0;
+        for (int base = span.lo; base < span.hi; base += stride, ++step, ++turn, stage = stage + 1 == kStages ? 0 : stage + 1) {
             // the warp's tokens are t1, t1 - 1, ...; k counts them
-            const int row1 = kGateTokens - 1 - warp * kGateSteps;
+            const int row1 = kTokens - 1 - warp * kSteps;
             const int t1 = first - step * stride + row1, left = t1 + 1 - span.lo;
             auto load = [&](int which, const T *base_ptr, int k, int back) {
-                if constexpr (kWords) return sm.ring[step % kStages][which].at(row1 - k, lane);
+                if constexpr (kWords) return sm.ring[stage][which].at(row1 - k, lane);
                 else return ch.load(base_ptr + static_cast<size_t>(t1 - k - back) * p.dim);
             };
             if (left > 0 && seq.start > t1) seq = seq_at(q, t1);
             // no sequence starts or ends in the warp's tokens
-            const bool inside = left >= kGateSteps && seq.end > t1 + 1 && seq.start < t1 + 1 - kGateSteps;
-            float2 P[kGateSteps], G[kGateSteps], u[kGateSteps], r[kGateSteps];  // P and G before the start is known
+            const bool inside = left >= kSteps && seq.end > t1 + 1 && seq.start < t1 + 1 - kSteps;
+            float2 P[kSteps], G[kSteps], u[kSteps], r[kSteps];  // P and G before the start is known
             GatePair run{both(1.0f), both(0.0f)};
             bool cut = false;
             if (inside) {
 #pragma unroll
-                for (int k = 0; k < kGateSteps; ++k) {
+                for (int k = 0; k < kSteps; ++k) {
                     const Gate2 gate = gate_of(load(2, F, k, 0), low, rest);
                     u[k] = gate.u;
                     r[k] = gate.r;
@@ -103,7 +111,7 @@ __global__ void __launch_bounds__(kGateThreads, 2) gate_grad_kernel(const GateGr
             } else {
                 SeqAt at = seq;
 #pragma unroll
-                for (int k = 0; k < kGateSteps; ++k) {
+                for (int k = 0; k < kSteps; ++k) {
                     u[k] = r[k] = P[k] = G[k] = both(0.0f);
                     if (k < left) {
                         if (at.start > t1 - k) at = seq_at(q, t1 - k);
@@ -114,36 +122,39 @@ __global__ void __launch_bounds__(kGateThreads, 2) gate_grad_kernel(const GateGr
                         const Gate2 gate = gate_of(load(2, F, k, 0), low, rest);
                         u[k] = gate.u;
                         r[k] = gate.r;
-                        P[k] = cut ? both(kCut) : run.P;
+                        if (cut) run.P = both(0.0f);
+                        P[k] = run.P;
                         G[k] = __fadd2_rn(load(0, DY, k, 0), run.h);
                         run.h = __fmul2_rn(gate.a, G[k]);
-                        run.P = __fmul2_rn(run.P, gate.a);
+                        run.P = cut ? both(0.0f) : above_zero(__fmul2_rn(run.P, gate.a));
                     }
                 }
             }
-            run.P = above_zero(run.P);
-            cp_async_wait<kStages - 3>();  // the next step's tiles, which the join's barrier makes everyone's
-            const float2 start = gate_join(sm.join, parity, g.cluster, rank, run, cut, carry);
-            copy(step + kStages - 1);  // into the tiles of the step before: all are done with them
+            if (inside) run.P = above_zero(run.P);
+            if constexpr (kWords) cp_async_wait<kStages - 3>();  // the next tiles, which the join's barrier makes everyone's
+            const float2 start = gate_join(sm.join, turn, g.cluster, rank, run, carry, lost);
+            copy(step + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);  // into the tiles of the step before: all are done with them
             auto finish = [&](int k, float2 Gk, float2 before) {
                 const size_t at = static_cast<size_t>(t1 - k) * p.dim;
                 const float2 x = load(1, X, k, 0);
                 const float2 diff = make_float2(before.x - x.x, before.y - x.y);
                 const float2 w = __fmul2_rn(__fmul2_rn(Gk, diff), u[k]);
-                ch.store(DX + at, __fmul2_rn(u[k], Gk));
-                ch.store(DF + at, __fmul2_rn(w, r[k]));
+                if (ch.active[0]) {
+                    ch.store(DX + at, __fmul2_rn(u[k], Gk));
+                    ch.store(DF + at, __fmul2_rn(w, r[k]));
+                }
                 dlow = __fadd2_rn(dlow, w);
             };
-            if (inside && __all_sync(kFullMask, finite2(start) || !ch.active[0])) {
+            if (inside && __all_sync(kFullMask, finite2(start))) {
 #pragma unroll
-                for (int k = 0; k < kGateSteps; ++k) finish(k, __ffma2_rn(P[k], start, G[k]), load(3, H, k, 1));
+                for (int k = 0; k < kSteps; ++k) finish(k, __ffma2_rn(P[k], start, G[k]), load(3, H, k, 1));
             } else {
                 SeqAt at = seq;
 #pragma unroll
-                for (int k = 0; k < kGateSteps; ++k) {
+                for (int k = 0; k < kSteps; ++k) {
                     if (k >= left) break;
                     if (at.start > t1 - k) at = seq_at(q, t1 - k);
-                    const float2 Gk = make_float2(G[k].x + through(P[k].x, start.x), G[k].y + through(P[k].y, start.y));
+                    const float2 Gk = join_any(GatePair{inside ? above_zero(P[k]) : P[k], G[k]}, start);
                     const bool begins = at.start == t1 - k;
                     finish(k, Gk, begins ? state_row(p.init, at.seq) : load(3, H, k, 1));
                     if (begins) store_dinit(at.seq, __fmul2_rn(__ffma2_rn(rest, r[k], low), Gk));
@@ -153,12 +164,16 @@ __global__ void __launch_bounds__(kGateThreads, 2) gate_grad_kernel(const GateGr
         cp_async_wait<0>();
         __syncthreads();  // (the ring is filled anew)
     }
+    if (g.cluster > 1) {
+        if (lost && threadIdx.x == 0) atomicAdd(&g_gate_grad_wait_failures, 1u);
+        cluster_barrier();
+    }
     if (part != nullptr) {  // the block's sum, the warps' added in order
         sm.join.warp[0][warp][lane].h = dlow;
         __syncthreads();
         if (warp == 0) {
             float2 sum = both(0.0f);
-            for (int w = 0; w < kGateWarps; ++w) sum = __fadd2_rn(sum, sm.join.warp[0][w][lane].h);
+            for (int w = 0; w < kWarps; ++w) sum = __fadd2_rn(sum, sm.join.warp[0][w][lane].h);
             sum = make_float2(sum.x / rest.x, sum.y / rest.y);  // da (1 - a) = da (1 - bound) sigmoid(-f)
             ch.store_floats(part + static_cast<size_t>(slot * g.cluster + rank) * p.dim, sum);
         }
@@ -169,21 +184,30 @@ template <typename T>
 cudaError_t launch_type(const GateGradArgs &a, float *part, const GateSpans &g, cudaStream_t stream) {
     if (a.dim * sizeof(T) % 16 == 0 && aligned16(a.dy) && aligned16(a.x) && aligned16(a.f) && aligned16(a.y) &&
         aligned16(a.dx) && aligned16(a.df))
-        return launch_gate_clusters(gate_grad_kernel<T, true>, sizeof(GradSmem<T, true>), g, stream, a, g, part);
-    return launch_gate_clusters(gate_grad_kernel<T, false>, sizeof(GradSmem<T, false>), g, stream, a, g, part);
+        return launch_gate_clusters(gate_grad_kernel<T, true>, kThreads, sizeof(GradSmem<T, true>), g, stream, a, g, part);
+    return launch_gate_clusters(gate_grad_kernel<T, false>, kThreads, sizeof(GradSmem<T, false>), g, stream, a, g, part);
 }
 
 }  // namespace
 
+cudaError_t gate_grad_take_wait_failures(unsigned int *count) {
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) {
+        gate_grad_swap_failures<<<1, 1>>>();
+        e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? cudaMemcpyFromSymbol(count, g_gate_grad_failures_taken, sizeof(*count)) : e;
+}
+
 size_t gated_recurrence_grad_workspace(const GateGradArgs &a) {
     if (!a.want_dbound || a.dim == 0) return 0;
-    const GateSpans g = gate_spans(a.seq, a.dim);
+    const GateSpans g = gate_spans(a.seq, a.dim, kTokens);
     const size_t parts = static_cast<size_t>(g.width) * g.cluster;
     return parts > 1 ? parts * a.dim * sizeof(float) : 0;
 }
 
 cudaError_t launch_gated_recurrence_grad(const GateGradArgs &a, void *workspace, cudaStream_t stream) {
-    const GateSpans g = gate_spans(a.seq, a.dim);
+    const GateSpans g = gate_spans(a.seq, a.dim, kTokens);
     const int parts = g.width * g.cluster;
     float *part = a.dbound == nullptr ? nullptr : parts > 1 ? static_cast<float *>(workspace) : a.dbound;
     cudaError_t e;

@@ -2,7 +2,7 @@
 // gate, the walk over sequences, and the scan over the token axis.
 //
 // Both are first-order recurrences per channel, h <- a h + b, forwards over the
-// tokens or backwards. A lane holds two channels, a warp kGateSteps consecutive
+// tokens or backwards. A lane holds two channels, a warp some consecutive
 // tokens of 64 channels; the block's warps follow one another along the axis, and so
 // do the blocks of a cluster. Each warp runs its tokens from zero and keeps, per
 // token, h and the product P of the a up to it, so that the value with the true start
@@ -17,6 +17,7 @@
 
 #include "xm_common.cuh"
 #include "xm_sequences.cuh"
+#include "xm_umma.cuh"
 
 namespace xm {
 
@@ -47,11 +48,7 @@ __device__ __forceinline__ Gate2 gate_of(float2 f, float2 low, float2 rest) {
     return g;
 }
 
-constexpr int kGateWarps = 8;  // warps of a block along the tokens
-constexpr int kGateThreads = 32 * kGateWarps;
-constexpr int kGateSteps = 8;                         // tokens of a warp
-constexpr int kGateTokens = kGateWarps * kGateSteps;  // tokens of a block
-constexpr int kGateChannels = 64;                     // channels of a block
+constexpr int kGateChannels = 64;  // channels of a block
 constexpr int kGateMaxCluster = 8;
 
 // The tokens that a cluster walks: a batch row, several short ones, or the packed row.
@@ -87,12 +84,12 @@ __device__ __forceinline__ SeqAt seq_at(const SeqArgs &q, int t) {
 
 // Calls f(sequence) for the sequences without tokens, shared out over the warps of all
 // blocks with the same channels (block `block` of `blocks`).
-template <typename F>
+template <int kWarps, typename F>
 __device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int block, int blocks, F &&f) {
     if (q.cu == nullptr && q.seqlen > 0) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (long long s0 = (static_cast<long long>(block) * kGateWarps + warp) * 32; s0 < q.units;
-         s0 += 32LL * kGateWarps * blocks) {
+    for (long long s0 = (static_cast<long long>(block) * kWarps + warp) * 32; s0 < q.units;
+         s0 += 32LL * kWarps * blocks) {
         const int s = static_cast<int>(s0) + lane;
         bool empty = false;
         if (s < q.units) {
@@ -104,32 +101,38 @@ __device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int block,
     }
 }
 
-// A (P, h) pair stands for h0 -> P h0 + h. Where a sequence starts inside, nothing of
-// h0 gets through, whatever it is (infinities and NaN too): a token's P is then kCut,
-// and a warp's pair is flagged. Products of gates are kept above zero, so that an
-// infinite h0 outlasts their underflow as it does step by step.
-constexpr float kCut = -1.0f;
-constexpr float kLeast = 1.4e-45f;
-__device__ __forceinline__ float2 above_zero(float2 P) { return make_float2(fmaxf(P.x, kLeast), fmaxf(P.y, kLeast)); }
-
+// A (P, h) pair stands for h0 -> P h0 + h. Where a sequence starts inside, P is zero
+// and nothing of h0 may get through; elsewhere products of gates are kept above zero,
+// so that an infinite h0 outlasts their underflow as it does step by step. As long as
+// h0 is finite a multiply-add does both, and it only gives a finite value if h0 was
+// one; values that come out infinite or NaN are joined once more with `join_any`.
 struct GatePair {
     float2 P, h;
 };
+constexpr float kLeast = 1.4e-45f;
+__device__ __forceinline__ float2 above_zero(float2 P) { return make_float2(fmaxf(P.x, kLeast), fmaxf(P.y, kLeast)); }
+__device__ __forceinline__ bool finite2(float2 v) { return fabsf(v.x) <= 3.4028235e38f && fabsf(v.y) <= 3.4028235e38f; }
+__device__ __forceinline__ float2 join(const GatePair &p, float2 h0) { return __ffma2_rn(p.P, h0, p.h); }
+__device__ __forceinline__ float2 join_any(const GatePair &p, float2 h0) {
+    return make_float2(p.P.x == 0.0f ? p.h.x : fmaf(p.P.x, h0.x, p.h.x), p.P.y == 0.0f ? p.h.y : fmaf(p.P.y, h0.y, p.h.y));
+}
+__device__ __forceinline__ float2 product(float2 P, float2 before) {
+    const float2 v = __fmul2_rn(P, before);
+    return make_float2(P.x == 0.0f || before.x == 0.0f ? 0.0f : fmaxf(v.x, kLeast),
+                       P.y == 0.0f || before.y == 0.0f ? 0.0f : fmaxf(v.y, kLeast));
+}
 
 // Shared memory of the join; parity alternates from step to step.
+template <int kWarps>
 struct GateJoin {
-    GatePair warp[2][kGateWarps][32];
+    GatePair warp[2][kWarps][32];
     GatePair block[2][kGateMaxCluster][32];
-    unsigned char warp_cut[2][kGateWarps];
-    int block_cut[2][kGateMaxCluster];
+    uint64_t arrived[2];  // the cluster's pairs of a step are here
 };
 
 __device__ __forceinline__ GatePair load_pair(const GatePair &p) {
     const float4 w = *reinterpret_cast<const float4 *>(&p);
     return GatePair{make_float2(w.x, w.y), make_float2(w.z, w.w)};
-}
-__device__ __forceinline__ float2 apply(const GatePair &p, bool cut, float2 h0) {
-    return cut ? p.h : __ffma2_rn(p.P, h0, p.h);
 }
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -137,7 +140,6 @@ __device__ __forceinline__ unsigned cluster_rank() {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-// All threads of the cluster: what each wrote before, into any block's shared memory, is visible behind it.
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
@@ -148,65 +150,119 @@ __device__ __forceinline__ uint32_t address_in_block(const void *smem, unsigned 
         : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "r"(rank));
     return there;
 }
+// A pair into another block's shared memory; its bytes count on that block's `arrived`. (A cluster barrier per step,
+// whose release waits for the block's own stores to global memory, took two to five microseconds under load.)
+__device__ __forceinline__ void send_pair(uint32_t there, uint32_t arrived, const GatePair &p) {
+    asm volatile(
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there),
+        "f"(p.P.x), "f"(p.P.y), "f"(p.h.x), "f"(p.h.y), "r"(arrived)
+        : "memory");
+}
+// Waits for a phase of `arrived`, a bounded number of times.
+__device__ __forceinline__ bool wait_arrived(uint64_t *arrived, uint32_t phase) {
+    const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(arrived));
+    for (uint32_t i = 0; i < (1u << 22); ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "}\n"
+            : "=r"(done)
+            : "r"(a), "r"(phase)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
 
-// Joins the warps' pairs of one step. Returns the value that this warp's tokens start
-// from and moves `carry` from the step's start to its end. Called by all threads of
-// the cluster; also a __syncthreads() of the block.
-__device__ __forceinline__ float2 gate_join(GateJoin &s, int parity, int cluster, unsigned rank, const GatePair &mine,
-                                            bool cut, float2 &carry) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Before the first join and behind the last, by all threads of a cluster of several blocks: every block has begun, and
+// none has left, while others write into its shared memory.
+template <int kWarps>
+__device__ __forceinline__ void gate_join_begin(GateJoin<kWarps> &s) {
+    if (threadIdx.x == 0) {
+        umma::mbar_init(&s.arrived[0], 1);
+        umma::mbar_init(&s.arrived[1], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    cluster_barrier();
+}
+
+// The values before and behind this block's part of the step.
+template <int K, int kWarps>
+__device__ __forceinline__ void join_blocks(const GateJoin<kWarps> &s, int parity, unsigned rank, float2 &start,
+                                            float2 &carry) {
+    const int lane = threadIdx.x & 31;
+    GatePair p[K];
+#pragma unroll
+    for (int r = 0; r < K; ++r) p[r] = load_pair(s.block[parity][r][lane]);
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+        if (r == static_cast<int>(rank)) start = carry;
+        carry = join(p[r], carry);
+    }
+}
+
+// Joins the warps' pairs of step `turn`, counted from 0 over the kernel. Returns the
+// value that this warp's tokens start from and moves `carry` from the step's start to
+// its end. Called by all threads of the cluster; also a __syncthreads() of the block.
+// `lost`: a wait gave up, here or before.
+template <int kWarps>
+__device__ __forceinline__ float2 gate_join(GateJoin<kWarps> &s, unsigned turn, int cluster, unsigned rank,
+                                            const GatePair &mine, float2 &carry, bool &lost) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, parity = turn & 1;
     *reinterpret_cast<float4 *>(&s.warp[parity][warp][lane]) = make_float4(mine.P.x, mine.P.y, mine.h.x, mine.h.y);
-    if (lane == 0) s.warp_cut[parity][warp] = cut;
     __syncthreads();
-    const uint2 cuts = *reinterpret_cast<const uint2 *>(&s.warp_cut[parity][0]);
-    auto cut_of = [&](int w) { return ((w < 4 ? cuts.x : cuts.y) >> (8 * (w & 3)) & 1) != 0; };
-    float2 start = carry;
+    float2 start = carry, behind = carry;
     if (cluster > 1) {
-        if (warp == kGateWarps - 1) {  // the block's pair, to every block
-            GatePair b = load_pair(s.warp[parity][0][lane]);
+        if (warp == kWarps - 1) {  // the block's pair, to every block
+            GatePair p[kWarps];
 #pragma unroll
-            for (int w = 1; w < kGateWarps; ++w) {
-                const GatePair p = load_pair(s.warp[parity][w][lane]);
-                b.h = apply(p, cut_of(w), b.h);
-                b.P = above_zero(__fmul2_rn(b.P, p.P));
-            }
-            for (int r = 0; r < cluster; ++r) {
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                 address_in_block(&s.block[parity][rank][lane], r)),
-                             "f"(b.P.x), "f"(b.P.y), "f"(b.h.x), "f"(b.h.y)
-                             : "memory");
-                if (lane == 0)
-                    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(
-                                     address_in_block(&s.block_cut[parity][rank], r)),
-                                 "r"((cuts.x | cuts.y) != 0 ? 1 : 0)
-                                 : "memory");
-            }
-        }
-        cluster_barrier();
-        for (int r = 0; r < cluster; ++r) {
-            if (r == static_cast<int>(rank)) start = carry;
-            carry = apply(load_pair(s.block[parity][r][lane]), s.block_cut[parity][r] != 0, carry);
-        }
+            for (int w = 0; w < kWarps; ++w) p[w] = load_pair(s.warp[parity][w][lane]);
+            GatePair b = p[0];
 #pragma unroll
-        for (int w = 0; w < kGateWarps - 1; ++w) {
-            if (w < warp) start = apply(load_pair(s.warp[parity][w][lane]), cut_of(w), start);
+            for (int w = 1; w < kWarps; ++w) b.h = join(p[w], b.h), b.P = product(p[w].P, b.P);
+            if (!finite2(b.h)) {
+                b.h = p[0].h;
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) b.h = join_any(p[w], b.h);
+            }
+            for (int r = 0; r < cluster; ++r)
+                send_pair(address_in_block(&s.block[parity][rank][lane], r), address_in_block(&s.arrived[parity], r), b);
+            if (lane == 0) umma::mbar_arrive_expect_tx(&s.arrived[parity], cluster * 32 * sizeof(GatePair));
         }
+        if (!lost) lost = !wait_arrived(&s.arrived[parity], turn >> 1 & 1);
+        if (cluster == 2) join_blocks<2>(s, parity, rank, start, behind);
+        else if (cluster == 4) join_blocks<4>(s, parity, rank, start, behind);
+        else join_blocks<8>(s, parity, rank, start, behind);
+#pragma unroll
+        for (int w = 0; w < kWarps - 1; ++w)
+            if (w < warp) start = join(load_pair(s.warp[parity][w][lane]), start);
     } else {
+        GatePair p[kWarps];
 #pragma unroll
-        for (int w = 0; w < kGateWarps; ++w) {
-            if (w == warp) start = carry;
-            carry = apply(load_pair(s.warp[parity][w][lane]), cut_of(w), carry);
+        for (int w = 0; w < kWarps; ++w) p[w] = load_pair(s.warp[parity][w][lane]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) start = behind;
+            behind = join(p[w], behind);
         }
     }
+    if (!__all_sync(kFullMask, finite2(start) && finite2(behind))) {
+        behind = start = carry;
+        for (int r = 0; r < (cluster > 1 ? cluster : 0); ++r) {
+            if (r == static_cast<int>(rank)) start = behind;
+            behind = join_any(load_pair(s.block[parity][r][lane]), behind);
+        }
+        for (int w = 0; w < kWarps; ++w) {
+            if (cluster == 1) behind = join_any(load_pair(s.warp[parity][w][lane]), behind);
+            if (w < warp) start = join_any(load_pair(s.warp[parity][w][lane]), start);
+        }
+    }
+    carry = behind;
     return start;
 }
-
-// A token's part of its warp's start: h0 -> P h0, with the care of kCut and kLeast.
-__device__ __forceinline__ float through(float P, float h0) {
-    if (P < 0.0f) return 0.0f;
-    return P == 0.0f && !(fabsf(h0) <= 3.4028235e38f) ? h0 : P * h0;
-}
-__device__ __forceinline__ bool finite2(float2 v) { return fabsf(v.x) <= 3.4028235e38f && fabsf(v.y) <= 3.4028235e38f; }
 
 // A lane's two channels: neighbours, moved as one word (kWords: rows of whole 16-byte
 // words, aligned to them), else 32 apart and moved one by one.
@@ -231,9 +287,9 @@ struct Lane {
     }
     // `row`: a token's first channel
     __device__ __forceinline__ float2 load(const T *row) const { return make_float2(to_f32<T>(row[c[0]]), to_f32<T>(row[c[1]])); }
+    // (words: only by active lanes)
     __device__ __forceinline__ void store(T *row, float2 v) const {
         if constexpr (kWords) {
-            if (!active[0]) return;
             if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t *>(row + c[0]) = pack2<T>(v.x, v.y);
             else *reinterpret_cast<float2 *>(row + c[0]) = v;
         } else {
@@ -245,41 +301,56 @@ struct Lane {
 
 // A block's tokens of one tensor in shared memory, and the copy that fills it: 16-byte
 // words of consecutive threads.
-template <typename T>
+template <typename T, int kTokens>
 struct GateTile {
-    T v[kGateTokens][kGateChannels];
+    T v[kTokens][kGateChannels];
     __device__ __forceinline__ float2 at(int row, int lane) const {
         if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][2 * lane]));
         else return *reinterpret_cast<const float2 *>(&v[row][2 * lane]);
     }
 };
-// Rows first + 0 .. kGateTokens - 1 of a tensor's channels; those outside [lo, hi) are left out.
-template <typename T>
-__device__ __forceinline__ void copy_tile(GateTile<T> &dst, const T *src, int first, int lo, int hi, int dim, int tile) {
+// Rows first + 0 .. kTokens - 1 of a tensor's channels; those outside [lo, hi) are left out.
+template <int kThreads, typename T, int kTokens>
+__device__ __forceinline__ void copy_tile(GateTile<T, kTokens> &dst, const T *src, int first, int lo, int hi, int dim,
+                                          int tile) {
     constexpr int kPer = 16 / static_cast<int>(sizeof(T)), kWordsRow = kGateChannels / kPer;
-    constexpr int kRows = kGateThreads / kWordsRow;  // rows per pass
+    constexpr int kRows = kThreads / kWordsRow;  // rows per pass
     const int col = threadIdx.x % kWordsRow * kPer, row = threadIdx.x / kWordsRow;
     if (tile * kGateChannels + col >= dim) return;
     const T *p = src + static_cast<int64_t>(first + row) * dim + tile * kGateChannels + col;
+    if (first >= lo && first + kTokens <= hi) {
 #pragma unroll
-    for (int k = 0; k < kGateTokens; k += kRows) {
+        for (int k = 0; k < kTokens; k += kRows, p += static_cast<int64_t>(kRows) * dim) cp_async16(&dst.v[row + k][col], p, 16);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < kTokens; k += kRows, p += static_cast<int64_t>(kRows) * dim) {
         const int t = first + row + k;
         if (t >= lo && t < hi) cp_async16(&dst.v[row + k][col], p, 16);
-        p += static_cast<int64_t>(kRows) * dim;
     }
 }
 
-// How a call is cut: blocks of channels, spans, and the cluster along the tokens.
-GateSpans gate_spans(const SeqArgs &q, int dim);
+// Zeros where copy_tile leaves channels behind the last one out: what is computed of them stays finite.
+template <typename R>
+__device__ __forceinline__ void clear_ring(R &ring, int dim, int tile) {
+    if ((tile + 1) * kGateChannels <= dim) return;
+    for (unsigned i = threadIdx.x; i < sizeof(R) / 16; i += blockDim.x)
+        reinterpret_cast<float4 *>(&ring)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __syncthreads();
+}
+
+// How a call is cut: blocks of channels, spans, and the cluster along the tokens, of which a block takes `tokens` at a
+// time.
+GateSpans gate_spans(const SeqArgs &q, int dim, int tokens);
 
 template <typename... Params, typename... Args>
-cudaError_t launch_gate_clusters(void (*kernel)(Params...), size_t smem, const GateSpans &g, cudaStream_t stream,
+cudaError_t launch_gate_clusters(void (*kernel)(Params...), int threads, size_t smem, const GateSpans &g, cudaStream_t stream,
                                  const Args &...args) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(g.width) * g.tiles * g.cluster);
-    cfg.blockDim = dim3(kGateThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
