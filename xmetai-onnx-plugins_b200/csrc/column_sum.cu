@@ -1,7 +1,7 @@
 // column_sum.cu -- sums of partial gradients over the blocks that left them, in a fixed
 // order, for GatedRecurrenceGradFn and LayerNormGradFn.
 //
-// A block takes 32 columns; its 8 warps take the rows in turn, four loads at a time,
+// A block takes 32 columns; its 32 warps take the rows in turn, four loads at a time,
 // and their sums are added in order. The partials were written just before and come
 // from L2.
 #include "xm_common.cuh"
@@ -10,7 +10,7 @@
 namespace xm {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 32;
 
 __global__ void __launch_bounds__(32 * kWarps) column_sum_kernel(const float *part0, const float *part1, int rows, int dim,
                                                                float *out0, float *out1) {

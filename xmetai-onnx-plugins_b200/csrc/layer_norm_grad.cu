@@ -3,88 +3,250 @@
 // Math, per row with xhat = (x - mean) rstd and g = dy weight:
 //   dx = rstd (g - average(g) - xhat average(g xhat)) + d_residual,
 // and over the rows d_weight = sum dy xhat, d_bias = sum dy.
+//
+// Bound by memory: dy, x and d_residual are read once and dx written once. A thread
+// keeps the same columns for all rows that its block walks, so the sums over rows stay
+// in registers next to the row itself; each block leaves one row of partial sums, which
+// column_sum.cu adds in a fixed order. Rows that do not fit (above 8192 elements of the
+// 16-bit types, 4096 of float32 or unaligned) take a kernel for dx and one for the
+// columns.
 #include <algorithm>
 
 #include "xm_common.cuh"
 #include "xm_kernels.h"
+#include "xm_rows.cuh"
 
 namespace xm {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int threads_of(int group) { return group < 128 ? 128 : group; }
 
-__device__ __forceinline__ float block_sum(float v, float *part) {
+// part: [2][blocks][dim] partial sums of d_weight and d_bias, written where they are wanted.
+template <typename T, int VE, int kGroup>
+__global__ void __launch_bounds__(threads_of(kGroup), 512 / threads_of(kGroup)) norm_grad_kernel(const NormGradArgs p, float *part_w,
+                                                                                                 float *part_b) {
+    constexpr int kThreads = threads_of(kGroup), kRows = kThreads / kGroup;
+    using Part = RowPart<T, VE, kGroup>;
+    constexpr int kElems = Part::kElems, kPairs = kElems / 2;
+    __shared__ float2 part[kGroup > 32 ? 2 * (kGroup / 32) : 1];
+    __shared__ float2 sums[kRows > 1 ? kThreads * kPairs : 1];
+    const int g = threadIdx.x % kGroup, dim = p.dim;
+    const float inv = 1.0f / static_cast<float>(dim);
+    const unsigned rows = p.rows;
+    const unsigned stride = gridDim.x * kRows;
+    unsigned row = blockIdx.x * kRows + threadIdx.x / kGroup;
+    const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
+                   *const DR = static_cast<const T *>(p.dres);
+    float2 weight[kPairs], sw[kPairs], sb[kPairs];
+    Part::vector(p.weight, g, dim, 1.0f, weight);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = part[threadIdx.x & (kThreads / 32 - 1)];
+    for (int i = 0; i < kPairs; ++i) sw[i] = sb[i] = twice(0.0f);
+    Part next_dy, next_x, next_dr;
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    next_dy.clear();
+    next_x.clear();
+    next_dr.clear();
+    auto load = [&](unsigned i) {
+        if (i >= rows) return;
+        next_dy.load(DY + static_cast<size_t>(i) * dim, g, dim);
+        next_x.load(X + static_cast<size_t>(i) * dim, g, dim);
+        if (DR != nullptr) next_dr.load(DR + static_cast<size_t>(i) * dim, g, dim);
+        if (!p.rms) next_mean = p.stats[2 * static_cast<size_t>(i)];
+        next_rstd = p.stats[2 * static_cast<size_t>(i) + 1];
+    };
+    load(row);
+    int turn = 0;
+    // (all groups of a block make the same number of turns: their sums share barriers or shuffles)
+    for (unsigned first = blockIdx.x * kRows; first < rows; first += stride, row += stride, turn ^= 1) {
+        const bool there = row < rows;
+        // as they are stored: a row's values are unpacked twice rather than held in twice the registers
+        const Part dy = next_dy, x = next_x, dr = next_dr;
+        const float rstd = next_rstd;
+        const float2 mean2 = twice(-next_mean), rstd2 = twice(rstd);
+        load(row + stride);
+        float2 total = twice(0.0f);
+        if (there) {
+            float2 sg = twice(0.0f), sx = twice(0.0f), v[kPairs], h[kPairs];
+            dy.floats(v);
+            x.floats(h);
 #pragma unroll
-    for (int o = kThreads / 64; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-    return v;
+            for (int i = 0; i < kPairs; ++i) {
+                h[i] = __fmul2_rn(__fadd2_rn(h[i], mean2), rstd2);
+                sw[i] = __ffma2_rn(v[i], h[i], sw[i]);
+                sb[i] = __fadd2_rn(sb[i], v[i]);
+                v[i] = __fmul2_rn(v[i], weight[i]);
+                sg = __fadd2_rn(sg, v[i]);
+                sx = __ffma2_rn(v[i], h[i], sx);
+            }
+            total = make_float2(sg.x + sg.y, sx.x + sx.y);
+        }
+        total = group_sum<kGroup>(total, part, turn);
+        if (there) {
+            const float2 ag = twice(p.rms ? 0.0f : -total.x * inv), ax = twice(-total.y * inv);
+            float2 v[kPairs], h[kPairs], more[kPairs];
+            dy.floats(v);
+            x.floats(h);
+            dr.floats(more);
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+                h[i] = __fmul2_rn(__fadd2_rn(h[i], mean2), rstd2);
+                v[i] = __ffma2_rn(h[i], ax, __ffma2_rn(v[i], weight[i], ag));
+                v[i] = __ffma2_rn(v[i], rstd2, more[i]);
+            }
+            Part out;
+            out.from(v);
+            out.store(static_cast<T *>(p.dx) + static_cast<size_t>(row) * dim, g, dim);
+        }
+    }
+    // the block's sums
+    auto leave = [&](float *out, float2 (&s)[kPairs]) {
+        if constexpr (kRows > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) sums[i * kThreads + threadIdx.x] = s[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+                s[i] = twice(0.0f);
+                for (int r = 0; r < kRows; ++r) s[i] = __fadd2_rn(s[i], sums[i * kThreads + r * kGroup + g]);
+            }
+        }
+        if (threadIdx.x < kGroup) Part::store_vector(out + static_cast<size_t>(blockIdx.x) * dim, g, dim, s);
+    };
+    if (part_w != nullptr) leave(part_w, sw);
+    if (part_b != nullptr) leave(part_b, sb);
 }
 
-// A block per row, two passes over it.
+constexpr int kWideThreads = 1024;
+
+// Rows of any length: a block per row, two passes over it.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_grad_rows_kernel(const NormGradArgs p) {
-    __shared__ float part[kThreads / 32];
-    for (unsigned row = blockIdx.x; row < static_cast<unsigned>(p.rows); row += gridDim.x) {
+__global__ void __launch_bounds__(kWideThreads) norm_grad_wide_kernel(const NormGradArgs p) {
+    __shared__ float2 part[2 * (kWideThreads / 32)];
+    const float inv = 1.0f / static_cast<float>(p.dim);
+    int turn = 0;
+    for (unsigned row = blockIdx.x; row < static_cast<unsigned>(p.rows); row += gridDim.x, turn ^= 1) {
         const size_t at = static_cast<size_t>(row) * p.dim;
         const float mean = p.rms ? 0.0f : p.stats[2 * static_cast<size_t>(row)];
         const float rstd = p.stats[2 * static_cast<size_t>(row) + 1];
-        float sg = 0.0f, sx = 0.0f;
-        for (int d = threadIdx.x; d < p.dim; d += kThreads) {
+        float2 sum = make_float2(0.0f, 0.0f);
+        for (int d = threadIdx.x; d < p.dim; d += kWideThreads) {
             const float g = to_f32<T>(static_cast<const T *>(p.dy)[at + d]) * (p.weight != nullptr ? p.weight[d] : 1.0f);
-            sg += g;
-            sx = fmaf(g, (to_f32<T>(static_cast<const T *>(p.x)[at + d]) - mean) * rstd, sx);
+            sum.x += g;
+            sum.y = fmaf(g, (to_f32<T>(static_cast<const T *>(p.x)[at + d]) - mean) * rstd, sum.y);
         }
-        sg = p.rms ? 0.0f : block_sum(sg, part) / p.dim;
-        sx = block_sum(sx, part) / p.dim;
-        for (int d = threadIdx.x; d < p.dim; d += kThreads) {
+        sum = group_sum<kWideThreads>(sum, part, turn);
+        const float ag = p.rms ? 0.0f : sum.x * inv, ax = sum.y * inv;
+        for (int d = threadIdx.x; d < p.dim; d += kWideThreads) {
             const float g = to_f32<T>(static_cast<const T *>(p.dy)[at + d]) * (p.weight != nullptr ? p.weight[d] : 1.0f);
             const float xhat = (to_f32<T>(static_cast<const T *>(p.x)[at + d]) - mean) * rstd;
             const float more = p.dres != nullptr ? to_f32<T>(static_cast<const T *>(p.dres)[at + d]) : 0.0f;
-            static_cast<T *>(p.dx)[at + d] = from_f32<T>(fmaf(rstd, g - sg - xhat * sx, more));
+            static_cast<T *>(p.dx)[at + d] = from_f32<T>(fmaf(rstd, g - ag - xhat * ax, more));
         }
     }
 }
 
-// A thread per column walks the rows.
+constexpr int kColThreads = 256;
+
+// Partial sums of a block of columns over a range of rows.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(const NormGradArgs p) {
-    const int d = blockIdx.x * kThreads + threadIdx.x;
+__global__ void __launch_bounds__(kColThreads) norm_grad_columns_kernel(const NormGradArgs p, float *part_w, float *part_b) {
+    const int d = blockIdx.x * kColThreads + threadIdx.x;
     if (d >= p.dim) return;
     float sw = 0.0f, sb = 0.0f;
-    for (int row = 0; row < p.rows; ++row) {
-        const float dy = to_f32<T>(static_cast<const T *>(p.dy)[static_cast<size_t>(row) * p.dim + d]);
-        const float x = to_f32<T>(static_cast<const T *>(p.x)[static_cast<size_t>(row) * p.dim + d]);
+    for (unsigned row = blockIdx.y; row < static_cast<unsigned>(p.rows); row += gridDim.y) {
+        const size_t at = static_cast<size_t>(row) * p.dim + d;
+        const float dy = to_f32<T>(static_cast<const T *>(p.dy)[at]);
         const float mean = p.rms ? 0.0f : p.stats[2 * static_cast<size_t>(row)];
-        sw = fmaf(dy, (x - mean) * p.stats[2 * static_cast<size_t>(row) + 1], sw);
+        sw = fmaf(dy, (to_f32<T>(static_cast<const T *>(p.x)[at]) - mean) * p.stats[2 * static_cast<size_t>(row) + 1], sw);
         sb += dy;
     }
-    if (p.dweight != nullptr) p.dweight[d] = sw;
-    if (p.dbias != nullptr) p.dbias[d] = sb;
+    if (part_w != nullptr) part_w[static_cast<size_t>(blockIdx.y) * p.dim + d] = sw;
+    if (part_b != nullptr) part_b[static_cast<size_t>(blockIdx.y) * p.dim + d] = sb;
+}
+
+// Threads per row; 0: the rows do not fit.
+int group_of(int dim, int elems) {
+    for (int group : {8, 32, 128, 256, 512})
+        if (dim <= group * elems) return group;
+    return 0;
+}
+
+// Whether all tensors move in words.
+bool words_of(const NormGradArgs &a) {
+    return a.dim % (a.io == IoType::kF32 ? 4 : 8) == 0 && aligned16(a.dy) && aligned16(a.x) && aligned16(a.dres) &&
+           aligned16(a.weight);
+}
+int elems_of(const NormGradArgs &a, bool words) {
+    return !words ? kRowElems<float, 1> : a.io == IoType::kF32 ? kRowElems<float, 4> : kRowElems<__half, 8>;
+}
+
+// Blocks that leave partial sums: as many as are resident, fewer for few rows.
+int parts_of(const NormGradArgs &a, bool words) {
+    const int group = group_of(a.dim, elems_of(a, words)), sms = current_device_sm_count();
+    if (group == 0) {
+        const int tiles = (a.dim + kColThreads - 1) / kColThreads;
+        return std::max(1, std::min(a.rows, (8 * sms + tiles - 1) / tiles));
+    }
+    const int threads = threads_of(group), rows = threads / group;
+    return std::max(1, std::min((a.rows + rows - 1) / rows, sms * (512 / threads)));
+}
+
+template <typename T, int VE, int kGroup>
+void launch_group(const NormGradArgs &a, int parts, float *part_w, float *part_b, cudaStream_t stream) {
+    norm_grad_kernel<T, VE, kGroup><<<parts, threads_of(kGroup), 0, stream>>>(a, part_w, part_b);
+}
+
+template <typename T, int VE>
+void launch_rows(const NormGradArgs &a, int parts, float *part_w, float *part_b, cudaStream_t stream) {
+    switch (group_of(a.dim, kRowElems<T, VE>)) {
+        case 8: return launch_group<T, VE, 8>(a, parts, part_w, part_b, stream);
+        case 32: return launch_group<T, VE, 32>(a, parts, part_w, part_b, stream);
+        case 128: return launch_group<T, VE, 128>(a, parts, part_w, part_b, stream);
+        case 256: return launch_group<T, VE, 256>(a, parts, part_w, part_b, stream);
+        case 512: return launch_group<T, VE, 512>(a, parts, part_w, part_b, stream);
+    }
+    if (a.rows > 0)
+        norm_grad_wide_kernel<T><<<std::min(a.rows, 2 * current_device_sm_count()), kWideThreads, 0, stream>>>(a);
+    if (part_w != nullptr || part_b != nullptr)
+        norm_grad_columns_kernel<T><<<dim3((a.dim + kColThreads - 1) / kColThreads, parts), kColThreads, 0, stream>>>(
+            a, part_w, part_b);
 }
 
 template <typename T>
-cudaError_t launch_type(const NormGradArgs &a, cudaStream_t stream) {
-    if (a.rows > 0) norm_grad_rows_kernel<T><<<std::min(a.rows, 148 * 8), kThreads, 0, stream>>>(a);
-    if (a.dweight != nullptr || a.dbias != nullptr)
-        norm_grad_columns_kernel<T><<<(a.dim + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+void launch_type(const NormGradArgs &a, bool words, int parts, float *part_w, float *part_b, cudaStream_t stream) {
+    if (words) launch_rows<T, 16 / static_cast<int>(sizeof(T))>(a, parts, part_w, part_b, stream);
+    else launch_rows<T, 1>(a, parts, part_w, part_b, stream);
 }
 
 }  // namespace
 
-size_t layer_norm_grad_workspace(const NormGradArgs &) { return 0; }
+// (The partial sums' number depends on alignment; the larger of both.)
+size_t layer_norm_grad_workspace(const NormGradArgs &a) {
+    const int sums = (a.weight != nullptr) + a.want_dbias, parts = std::max(parts_of(a, true), parts_of(a, false));
+    // rows of the two sums begin on 16-byte words
+    return parts > 1 ? static_cast<size_t>(sums) * ((static_cast<size_t>(parts) * a.dim + 3) / 4 * 4) * sizeof(float) : 0;
+}
 
-cudaError_t launch_layer_norm_grad(const NormGradArgs &a, void *, cudaStream_t stream) {
-    switch (a.io) {
-        case IoType::kBF16: return launch_type<__nv_bfloat16>(a, stream);
-        case IoType::kF16: return launch_type<__half>(a, stream);
-        default: return launch_type<float>(a, stream);
+cudaError_t launch_layer_norm_grad(const NormGradArgs &a, void *workspace, cudaStream_t stream) {
+    bool words = words_of(a) && aligned16(a.dx);
+    if (parts_of(a, words) == 1) words = words && aligned16(a.dweight) && aligned16(a.dbias);
+    const int parts = parts_of(a, words);
+    float *part_w = a.dweight, *part_b = a.dbias;
+    if (parts > 1) {
+        float *next = static_cast<float *>(workspace);
+        if (part_w != nullptr) part_w = next, next += (static_cast<size_t>(parts) * a.dim + 3) / 4 * 4;
+        if (part_b != nullptr) part_b = next;
     }
+    switch (a.io) {
+        case IoType::kBF16: launch_type<__nv_bfloat16>(a, words, parts, part_w, part_b, stream); break;
+        case IoType::kF16: launch_type<__half>(a, words, parts, part_w, part_b, stream); break;
+        default: launch_type<float>(a, words, parts, part_w, part_b, stream);
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || parts == 1 || (part_w == nullptr && part_b == nullptr)) return e;
+    if (part_w == nullptr) return launch_column_sums(part_b, nullptr, parts, a.dim, a.dbias, nullptr, stream);
+    return launch_column_sums(part_w, part_b, parts, a.dim, a.dweight, a.dbias, stream);
 }
 
 }  // namespace xm
