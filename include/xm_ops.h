@@ -31,8 +31,8 @@
  *  - The caller owns all memory: inputs, the output (shape from the
  *    *_output_shape query) and a workspace (size from the *_workspace_size
  *    query, 256-byte aligned; 0 bytes for SelectiveScanFn, Mamba3SisoFn, the
- *    convolutions, SelectiveStateUpdateFn, GatedRecurrenceFn,
- *    GatedRecurrenceUpdateFn and LayerNormFn).
+ *    convolutions, SelectiveStateUpdateFn, GatedRecurrenceUpdateFn and
+ *    LayerNormFn).
  *    The library allocates no memory and never synchronises the stream, so
  *    concurrent calls on different streams with separate workspaces are
  *    independent. Its only state is, per (host thread, device), two internal
@@ -422,7 +422,9 @@ xm_status xm_selective_state_update_fwd(const xm_selective_state_update_attrs *a
  *   lower_bound [dim] or empty, initial_state [sequences or slots, dim] or
  *   empty, cu_seqlens, state_indices, has_initial_state.
  * Outputs: y (x's shape and type); with output_final_state the float32 state
- *   after every sequence's last token (its starting state when it is empty). */
+ *   after every sequence's last token (its starting state when it is empty).
+ * The workspace holds the segments' end states where a row is cut along its
+ * tokens. */
 typedef struct xm_gated_recurrence_attrs {
     int64_t output_final_state; /* default 0 */
 } xm_gated_recurrence_attrs;
@@ -451,7 +453,8 @@ xm_status xm_gated_recurrence_fwd(const xm_gated_recurrence_attrs *attrs, const 
  *   (d_final_state's row where the sequence is empty). Sums are taken in a fixed
  *   order: equal calls give equal bits. Positions behind the last offset are
  *   neither read nor written.
- * The workspace holds d_lower_bound's partial sums. */
+ * The workspace holds d_lower_bound's partial sums and, where a row is cut
+ * along its tokens, what each segment passes on. */
 typedef struct xm_gated_recurrence_grad_attrs {
     int64_t output_lower_bound_grad;   /* default 0 */
     int64_t output_initial_state_grad; /* default 0 */

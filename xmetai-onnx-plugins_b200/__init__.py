@@ -714,7 +714,7 @@ def SelectiveStateUpdateFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, s
 # ---------------------------------------------------------------- gated linear recurrence, layer norm
 
 _GATE = _ServeOp("gated_recurrence", ("x", "f", "lower_bound", "initial_state", "cu_seqlens", "state_indices",
-                                      "has_initial_state"), "xxffiii", 3)
+                                      "has_initial_state"), "xxffiii", 3, True)
 _GATE_GRAD = _ServeOp("gated_recurrence_grad", ("dy", "x", "f", "y", "lower_bound", "initial_state", "cu_seqlens",
                                                 "d_final_state"), "xxxxffif", 5, True, ("an output",) * 4)
 _GATE_UPDATE = _ServeOp("gated_recurrence_update", ("x", "f", "lower_bound", "state", "state_indices"), "xxffi", 3)

@@ -1099,12 +1099,10 @@ int32_t xm_abi_version(void) { return XM_ABI_VERSION; }
 
 xm_status xm_device_wait_failures(uint32_t *count) {
     if (count == nullptr) return fail(XM_ERR_INVALID_ARGUMENT, "count is null");
-    unsigned int n = 0, n2 = 0, n3 = 0, n4 = 0;
+    unsigned int n = 0, n2 = 0;
     cudaError_t e = xm::m3c_take_wait_failures(&n);
     if (e == cudaSuccess) e = xm::gdn_tc_take_wait_failures(&n2);
-    if (e == cudaSuccess) e = xm::gate_take_wait_failures(&n3);
-    if (e == cudaSuccess) e = xm::gate_grad_take_wait_failures(&n4);
-    *count = n + n2 + n3 + n4;
+    *count = n + n2;
     return e == cudaSuccess ? XM_OK : cuda_fail(e);
 }
 
@@ -1543,8 +1541,8 @@ xm_status xm_gated_recurrence_output_shape(const xm_gated_recurrence_attrs *attr
 xm_status xm_gated_recurrence_workspace_size(const xm_gated_recurrence_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs,
                                    size_t *bytes) {
     return guarded([&] {
-        gate_plan(attrs, inputs, n_inputs);
-        if (bytes) *bytes = 0;
+        const GatePlan pl = gate_plan(attrs, inputs, n_inputs);
+        if (bytes) *bytes = xm::gated_recurrence_workspace(pl.args);
         return XM_OK;
     });
 }
@@ -1552,15 +1550,14 @@ xm_status xm_gated_recurrence_workspace_size(const xm_gated_recurrence_attrs *at
 xm_status xm_gated_recurrence_fwd(const xm_gated_recurrence_attrs *attrs, const xm_tensor *inputs, int32_t n_inputs, xm_tensor *output,
                         void *workspace, size_t workspace_bytes, void *cuda_stream) {
     XM_NVTX_RANGE("GatedRecurrenceFn");
-    (void)workspace;
-    (void)workspace_bytes;
     return guarded([&] {
         GatePlan pl = gate_plan(attrs, inputs, n_inputs);
         const bool with_state = attrs->output_final_state != 0;
         serving_outputs(pl, inputs, n_inputs, 3, output, with_state, XM_DTYPE_FLOAT, "x", "final_state");
         pl.args.final_state = with_state && present(output[1]) ? static_cast<float *>(output[1].data) : nullptr;
         if (pl.args.seq.units == 0 || (!present(*output) && pl.args.final_state == nullptr)) return XM_OK;
-        const cudaError_t e = xm::launch_gated_recurrence(pl.args, static_cast<cudaStream_t>(cuda_stream));
+        require_workspace(workspace, workspace_bytes, xm::gated_recurrence_workspace(pl.args));
+        const cudaError_t e = xm::launch_gated_recurrence(pl.args, workspace, static_cast<cudaStream_t>(cuda_stream));
         return e == cudaSuccess ? XM_OK : cuda_fail(e);
     });
 }

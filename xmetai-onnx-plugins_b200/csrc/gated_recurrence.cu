@@ -2,6 +2,7 @@
 //
 // Math, per channel: a_t = b + (1 - b) sigmoid(f_t), h_t = a_t h_(t-1) + (1 - a_t) x_t.
 #include <algorithm>
+#include <climits>
 
 #include "xm_common.cuh"
 #include "xm_gate.cuh"
@@ -11,146 +12,149 @@
 namespace xm {
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps;  // a block's warps follow one another along the tokens
-constexpr int kSteps = 16;                         // tokens of a warp
-constexpr int kTokens = kWarps * kSteps;           // tokens of a block
-constexpr int kStages = 3;                         // tiles of x and f in use and under way
-
-__device__ unsigned int g_gate_wait_failures, g_gate_failures_taken;
-__global__ void gate_swap_failures() { g_gate_failures_taken = atomicExch(&g_gate_wait_failures, 0u); }
+constexpr int kStages = 6;  // groups of x and f in use and under way
 
 template <typename T, bool kWords>
 struct ScanSmem {
-    GateJoin<kWarps> join;
-    GateTile<T, kTokens> ring[kWords ? kStages : 0][2];
+    GateTile<T> ring[kWords ? kStages : 0][2];
 };
 
-template <typename T, bool kWords>
-__global__ void __launch_bounds__(kThreads, 4) gate_kernel(const GateArgs p, const GateSpans g) {
+// kEnds: the first pass over segments (all but a span's last).
+template <typename T, bool kWords, bool kEnds>
+__global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const GateCut g) {
     extern __shared__ float4 smem_f4[];
     auto &sm = *reinterpret_cast<ScanSmem<T, kWords> *>(smem_f4);
     const SeqArgs &q = p.seq;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned rank = g.cluster > 1 ? cluster_rank() : 0;
-    const int id = blockIdx.x / g.cluster, tile = id % g.tiles, slot = id / g.tiles;
-    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
+    const int j = blockIdx.x / g.tiles % segs, slot = blockIdx.x / g.tiles / segs;
+    const Lane<T, kWords> ch(tile, threadIdx.x, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
     T *const Y = static_cast<T *>(p.out);
-    auto init_of = [&](int seq) {
-        const long long row = seq_row(q, seq);
+    auto init_of = [&](int seq, long long row) {
         return ch.floats(p.init != nullptr && seq_live(q, seq, row) ? p.init + row * p.dim : nullptr, 0.0f);
     };
-    auto store_final = [&](int seq, float2 h) {
-        const long long row = seq_row(q, seq);
+    auto store_final = [&](long long row, float2 h) {
         if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
     };
-    if (p.final_state != nullptr)  // sequences without tokens keep their starting states
-        for_empty_sequences<kWarps>(q, slot * g.cluster + rank, g.width * g.cluster, [&](int s) { store_final(s, init_of(s)); });
-    if (g.cluster > 1) gate_join_begin(sm.join);
-    if constexpr (kWords) clear_ring(sm.ring, p.dim, tile);
-    const int stride = g.cluster * kTokens;  // tokens of a step
-    unsigned turn = 0;
-    bool lost = false;
-    for (int i = slot; i < g.rows; i += g.width) {
+    if (!kEnds && p.final_state != nullptr)  // sequences without tokens keep their starting states
+        for_empty_sequences(q, slot * segs + j, g.width * segs, [&](int s) {
+            const long long row = seq_row(q, s);
+            store_final(row, init_of(s, row));
+        });
+    for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(q, g, i);
-        const int first = span.lo + rank * kTokens;  // the block's first token
-        auto copy = [&](int step, int stage) {
+        const int length = segment_length(g, span);
+        const int s0 = span.lo + min(static_cast<long long>(j) * length, static_cast<long long>(max(span.hi - span.lo, 0)));
+        const int s1 = min(static_cast<long long>(s0) + length, static_cast<long long>(span.hi));
+        if (s0 >= s1) continue;
+        auto pair = [&](int k) { return ((static_cast<size_t>(i) * g.segments + k) * g.tiles + tile) * 32 + threadIdx.x; };
+        int begin = s0;
+        SeqAt seq = seq_at(q, kEnds ? s1 - 1 : s0);
+        if (kEnds) {
+            if (seq.end <= s1 || s1 >= span.hi) continue;  // no sequence leaves the segment
+            begin = max(s0, seq.start);
+        }
+        auto copy = [&](int t, int stage) {
             if constexpr (kWords) {
-                const int t = first + step * stride;
-                if (t < span.hi) {
-                    copy_tile<kThreads>(sm.ring[stage][0], X, t, 0, span.hi, p.dim, tile);
-                    copy_tile<kThreads>(sm.ring[stage][1], F, t, 0, span.hi, p.dim, tile);
+                if (t < s1) {
+                    copy_tile(sm.ring[stage][0], X, t, 0, s1, p.dim, tile);
+                    copy_tile(sm.ring[stage][1], F, t, 0, s1, p.dim, tile);
                 }
                 cp_async_commit();
             }
         };
-        if constexpr (kWords) {
-            for (int k = 0; k < kStages; ++k) copy(k, k);
-            cp_async_wait<kStages - 1>();
-            __syncthreads();
+        for (int k = 0; k < kStages - 1; ++k) copy(begin + k * kGateGroup, k);
+        float2 h = both(0.0f), P = both(1.0f);
+        long long row = seq_row(q, seq.seq);
+        // where the warp's first token does not begin a sequence, the state comes from the segments before
+        SeqAt next{0, 0, 0};
+        long long next_row = -1;
+        float2 next_h = both(0.0f);
+        if (seq.start >= begin) {  // (== unless the offsets descend)
+            h = init_of(seq.seq, row);
+            if (kEnds) g.start[pair(j)] = h;
+            else if (seq.end > s1 && g.segments > 1) h = g.start[pair(j)];
+        } else if (!kEnds && j > 0) {
+            int k = max(seq.start - span.lo, 0) / length;
+            h = g.h[pair(k)];
+            for (++k; k < j; ++k) h = __ffma2_rn(g.P[pair(k)], h, g.h[pair(k)]);
         }
-        float2 carry = both(0.0f);
-        SeqAt seq{0, 0, 0};
-        int step = 0, stage = 0;
-        for (int base = span.lo; base < span.hi; base += stride, ++step, ++turn, stage = stage + 1 == kStages ? 0 : stage + 1) {
-            const int t0 = first + step * stride + warp * kSteps, left = span.hi - t0;
-            float2 P[kSteps], h[kSteps];
+        auto look_ahead = [&] {  // the sequence behind this one, and its starting state
+            if (kEnds || seq.end >= s1) return;
+            next = seq_behind(q, seq);
+            next_row = seq_row(q, next.seq);
+            // one that leaves the segment: its last warp may have stored its final state in the same place
+            next_h = next.end > s1 && g.segments > 1 ? g.start[pair(j)] : init_of(next.seq, next_row);
+        };
+        look_ahead();
+        int stage = 0;
+        for (int t = begin; t < s1; t += kGateGroup) {
+            if constexpr (kWords) {
+                cp_async_wait<kStages - 2>();
+                __syncwarp();
+            }
+            copy(t + (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
             auto token = [&](int k, float2 &x, float2 &f) {
                 if constexpr (kWords) {
-                    const GateTile<T, kTokens>(&tiles)[2] = sm.ring[stage];
-                    x = tiles[0].at(warp * kSteps + k, lane);
-                    f = tiles[1].at(warp * kSteps + k, lane);
+                    x = sm.ring[stage][0].at(k);
+                    f = sm.ring[stage][1].at(k);
                 } else {
-                    const size_t at = static_cast<size_t>(t0 + k) * p.dim;
+                    const size_t at = static_cast<size_t>(t + k) * p.dim;
                     x = ch.load(X + at);
                     f = ch.load(F + at);
                 }
             };
-            if (left > 0 && seq.end <= t0) seq = seq_at(q, t0);
-            // no sequence starts or ends in the warp's tokens
-            const bool inside = left >= kSteps && seq.start < t0 && seq.end > t0 + kSteps;
-            GatePair run{both(1.0f), both(0.0f)};
-            bool cut = false;
-            if (inside) {
+            if (t + kGateGroup <= s1 && (kEnds || seq.end > t + kGateGroup)) {
+                float2 a[kGateGroup], b[kGateGroup];
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
+                for (int k = 0; k < kGateGroup; ++k) {
                     float2 x, f;
                     token(k, x, f);
                     const Gate2 gate = gate_of(f, low, rest);
-                    run.h = __ffma2_rn(gate.a, run.h, __fmul2_rn(gate.u, x));
-                    run.P = __fmul2_rn(run.P, gate.a);
-                    P[k] = run.P;
-                    h[k] = run.h;
+                    a[k] = gate.a;
+                    b[k] = __fmul2_rn(gate.u, x);
+                }
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k) {
+                    h = __ffma2_rn(a[k], h, b[k]);
+                    if (kEnds) P = __fmul2_rn(P, a[k]);
+                    b[k] = h;
+                }
+                if (!kEnds && ch.active[0]) {
+                    T *y = Y + static_cast<size_t>(t) * p.dim;
+#pragma unroll
+                    for (int k = 0; k < kGateGroup; ++k, y += p.dim) ch.store(y, b[k]);
                 }
             } else {
-                SeqAt at = seq;
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    if (k < left) {
-                        if (at.end <= t0 + k) at = seq_at(q, t0 + k);
-                        if (at.start == t0 + k) {
-                            run.h = init_of(at.seq);
-                            cut = true;
-                        }
-                        float2 x, f;
-                        token(k, x, f);
-                        const Gate2 gate = gate_of(f, low, rest);
-                        run.h = __ffma2_rn(gate.a, run.h, __fmul2_rn(gate.u, x));
-                        run.P = cut ? both(0.0f) : above_zero(__fmul2_rn(run.P, gate.a));
+#pragma unroll 1
+                for (int k = 0; k < kGateGroup && t + k < s1; ++k) {
+                    float2 x, f;
+                    token(k, x, f);
+                    const Gate2 gate = gate_of(f, low, rest);
+                    h = __ffma2_rn(gate.a, h, __fmul2_rn(gate.u, x));
+                    if (kEnds) {
+                        P = __fmul2_rn(P, gate.a);
+                        continue;
                     }
-                    P[k] = run.P;
-                    h[k] = run.h;
+                    if (ch.active[0]) ch.store(Y + static_cast<size_t>(t + k) * p.dim, h);
+                    if (seq.end == t + k + 1) {
+                        store_final(row, h);
+                        seq = next;
+                        row = next_row;
+                        h = next_h;
+                        look_ahead();
+                    }
                 }
             }
-            if (inside) run.P = above_zero(run.P);
-            if constexpr (kWords) cp_async_wait<kStages - 2>();  // the next tiles, which the join's barrier makes everyone's
-            const float2 start = gate_join(sm.join, turn, g.cluster, rank, run, carry, lost);
-            copy(step + kStages, stage);  // into this step's tiles: all have read them
-            if (inside && __all_sync(kFullMask, finite2(start))) {
-                if (ch.active[0]) {
-                    T *y = Y + static_cast<size_t>(t0) * p.dim;
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k, y += p.dim) ch.store(y, __ffma2_rn(P[k], start, h[k]));
-                }
-            } else {
-                SeqAt at = seq;
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    if (k >= left) break;
-                    if (at.end <= t0 + k) at = seq_at(q, t0 + k);
-                    const float2 y = join_any(GatePair{inside ? above_zero(P[k]) : P[k], h[k]}, start);
-                    if (ch.active[0]) ch.store(Y + static_cast<size_t>(t0 + k) * p.dim, y);
-                    if (at.end == t0 + k + 1) store_final(at.seq, y);
-                }
-            }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+        if (kEnds) {
+            g.P[pair(j)] = above_zero(P);
+            g.h[pair(j)] = h;
         }
         cp_async_wait<0>();
-        __syncthreads();  // (the ring is filled anew)
-    }
-    if (g.cluster > 1) {
-        if (lost && threadIdx.x == 0) atomicAdd(&g_gate_wait_failures, 1u);
-        cluster_barrier();
+        __syncwarp();  // (the ring is filled anew)
     }
 }
 
@@ -173,12 +177,21 @@ __global__ void __launch_bounds__(kTokenThreads) gate_token_kernel(const GateArg
     }
 }
 
+template <typename T, bool kWords>
+cudaError_t launch_words(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
+    constexpr size_t kSmem = sizeof(ScanSmem<T, kWords>);
+    if (g.segments > 1) {
+        const cudaError_t e = launch_gate(gate_kernel<T, kWords, true>, kSmem, g, g.segments - 1, stream, a, g);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_gate(gate_kernel<T, kWords, false>, kSmem, g, g.segments, stream, a, g);
+}
+
 template <typename T>
-cudaError_t launch_type(const GateArgs &a, cudaStream_t stream) {
-    const GateSpans g = gate_spans(a.seq, a.dim, kTokens);
+cudaError_t launch_type(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
     if (a.dim * sizeof(T) % 16 == 0 && aligned16(a.x) && aligned16(a.f) && aligned16(a.out))
-        return launch_gate_clusters(gate_kernel<T, true>, kThreads, sizeof(ScanSmem<T, true>), g, stream, a, g);
-    return launch_gate_clusters(gate_kernel<T, false>, kThreads, sizeof(ScanSmem<T, false>), g, stream, a, g);
+        return launch_words<T, true>(a, g, stream);
+    return launch_words<T, false>(a, g, stream);
 }
 
 template <typename T>
@@ -190,42 +203,40 @@ cudaError_t launch_token_type(const GateArgs &a, cudaStream_t stream) {
 
 }  // namespace
 
-GateSpans gate_spans(const SeqArgs &q, int dim, int tokens) {
-    GateSpans g{};
+GateCut gate_cut(const SeqArgs &q, int dim, int parts) {
+    GateCut g{};
     g.tiles = (dim + kGateChannels - 1) / kGateChannels;
-    const int64_t want = 4LL * current_device_sm_count();  // blocks that fill the device
+    constexpr int kShort = 64;  // rows shorter than this share a span
     if (q.cu != nullptr) {
-        g.rows = 1;
+        g.spans = 1;
         g.length = q.tokens;
     } else {
-        // rows shorter than a block's tokens share a span
-        const int64_t per = q.seqlen > 0 ? std::max<int64_t>(1, tokens / q.seqlen) : q.units;
+        const int64_t per = q.seqlen > 0 ? std::max<int64_t>(1, kShort / q.seqlen) : q.units;
         g.length = static_cast<int>(std::min<int64_t>(per * q.seqlen, q.tokens));
-        g.rows = g.length > 0 ? static_cast<int>((static_cast<int64_t>(q.tokens) + g.length - 1) / g.length) : 1;
+        g.spans = g.length > 0 ? static_cast<int>((static_cast<int64_t>(q.tokens) + g.length - 1) / g.length) : 1;
     }
-    g.cluster = 1;
-    while (g.cluster < kGateMaxCluster && g.cluster * tokens < g.length &&
-           static_cast<int64_t>(g.rows) * g.tiles * g.cluster < want)
-        g.cluster *= 2;
-    const int64_t most = std::max<int64_t>(1, (int64_t(1) << 30) / (static_cast<int64_t>(g.tiles) * g.cluster));
-    g.width = static_cast<int>(std::min<int64_t>(g.rows, most));
+    const int64_t warps = static_cast<int64_t>(g.spans) * g.tiles, sms = current_device_sm_count();
+    g.segments = 1;
+    if (warps * 10 < sms * 24 && g.length > 128)
+        g.segments = static_cast<int>(std::min<int64_t>((8 * sms + warps - 1) / warps, (g.length + 63) / 64));
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(parts, (int64_t(1) << 30) / g.tiles) / g.segments);
+    g.width = static_cast<int>(std::min<int64_t>(g.spans, most));
     return g;
 }
 
-cudaError_t gate_take_wait_failures(unsigned int *count) {
-    cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) {
-        gate_swap_failures<<<1, 1>>>();
-        e = cudaGetLastError();
-    }
-    return e == cudaSuccess ? cudaMemcpyFromSymbol(count, g_gate_failures_taken, sizeof(*count)) : e;
+size_t gated_recurrence_workspace(const GateArgs &a) {
+    return a.dim == 0 ? 0 : 3 * gate_pairs(gate_cut(a.seq, a.dim, INT_MAX)) * sizeof(float2);
 }
 
-cudaError_t launch_gated_recurrence(const GateArgs &a, cudaStream_t stream) {
+cudaError_t launch_gated_recurrence(const GateArgs &a, void *workspace, cudaStream_t stream) {
+    GateCut g = gate_cut(a.seq, a.dim, INT_MAX);
+    g.P = static_cast<float2 *>(workspace);
+    g.h = g.P + gate_pairs(g);
+    g.start = g.h + gate_pairs(g);
     switch (a.io) {
-        case IoType::kBF16: return launch_type<__nv_bfloat16>(a, stream);
-        case IoType::kF16: return launch_type<__half>(a, stream);
-        default: return launch_type<float>(a, stream);
+        case IoType::kBF16: return launch_type<__nv_bfloat16>(a, g, stream);
+        case IoType::kF16: return launch_type<__half>(a, g, stream);
+        default: return launch_type<float>(a, g, stream);
     }
 }
 

@@ -5,9 +5,10 @@
 //   G_t = dy_t + c,  dx_t = (1 - a_t) G_t,  c <- a_t G_t,
 //   df_t = G_t (h_(t-1) - x_t) (1 - a_t) sigmoid(f_t),
 //   d_bound += G_t (h_(t-1) - x_t) sigmoid(-f_t).
-// The recurrence of c is scanned as xm_gate.cuh says, from the last token to the
+// The recurrence of c is walked as xm_gate.cuh says, from the last token to the
 // first.
 #include <algorithm>
+#include <climits>
 
 #include "xm_common.cuh"
 #include "xm_gate.cuh"
@@ -17,30 +18,26 @@
 namespace xm {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;  // a block's warps follow one another along the tokens
-constexpr int kSteps = 8;                          // tokens of a warp
-constexpr int kTokens = kWarps * kSteps;           // tokens of a block
-constexpr int kStages = 3;                         // tiles in use and under way
+constexpr int kMaxParts = 1024;  // partial sums of d_bound per channel
 
-__device__ unsigned int g_gate_grad_wait_failures, g_gate_grad_failures_taken;
-__global__ void gate_grad_swap_failures() { g_gate_grad_failures_taken = atomicExch(&g_gate_grad_wait_failures, 0u); }
-
-template <typename T, bool kWords>
+template <typename T, bool kWords, bool kEnds>
 struct GradSmem {
-    GateJoin<kWarps> join;
-    GateTile<T, kTokens> ring[kWords ? kStages : 0][4];  // dy, x, f, and y of the token before
+    static constexpr int kStages = sizeof(T) == 4 ? 3 : 5;  // groups in use and under way
+    static constexpr int kTensors = kEnds ? 2 : 4;          // f, dy; x, and y of the token before
+    GateTile<T> ring[kWords ? kStages : 0][kTensors];
 };
 
-// part: [width x cluster][dim] sums of d_bound, or null.
-template <typename T, bool kWords>
-__global__ void __launch_bounds__(kThreads, 2) gate_grad_kernel(const GateGradArgs p, const GateSpans g, float *part) {
+// kEnds: the first pass over segments (all but a span's first).
+// part: [width x segments][dim] sums of d_bound, or null.
+template <typename T, bool kWords, bool kEnds>
+__global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, const GateCut g, float *part) {
     extern __shared__ float4 smem_f4[];
-    auto &sm = *reinterpret_cast<GradSmem<T, kWords> *>(smem_f4);
+    auto &sm = *reinterpret_cast<GradSmem<T, kWords, kEnds> *>(smem_f4);
+    constexpr int kStages = GradSmem<T, kWords, kEnds>::kStages;
     const SeqArgs &q = p.seq;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned rank = g.cluster > 1 ? cluster_rank() : 0;
-    const int id = blockIdx.x / g.cluster, tile = id % g.tiles, slot = id / g.tiles;
-    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
+    const int j = blockIdx.x / g.tiles % segs + (kEnds ? 1 : 0), slot = blockIdx.x / g.tiles / segs;
+    const Lane<T, kWords> ch(tile, threadIdx.x, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
                    *const F = static_cast<const T *>(p.f), *const H = static_cast<const T *>(p.y);
@@ -51,170 +48,191 @@ __global__ void __launch_bounds__(kThreads, 2) gate_grad_kernel(const GateGradAr
     auto store_dinit = [&](int seq, float2 c) {
         if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
     };
-    if (p.dinit != nullptr)  // sequences without tokens: the gradient passes through
-        for_empty_sequences<kWarps>(q, slot * g.cluster + rank, g.width * g.cluster,
-                            [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
-    if (g.cluster > 1) gate_join_begin(sm.join);
-    if constexpr (kWords) clear_ring(sm.ring, p.dim, tile);
-    const int stride = g.cluster * kTokens;  // tokens of a step
-    float2 dlow = both(0.0f);                    // sum of da (1 - a)
-    unsigned turn = 0;
-    bool lost = false;
-    for (int i = slot; i < g.rows; i += g.width) {
+    if (!kEnds && p.dinit != nullptr)  // sequences without tokens: the gradient passes through
+        for_empty_sequences(q, slot * segs + j, g.width * segs, [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
+    float2 dlow = both(0.0f);  // sum of da (1 - a)
+    for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(q, g, i);
-        const int first = span.hi - (rank + 1) * kTokens;  // the block's lowest token of the first step
-        auto copy = [&](int step, int stage) {
+        const int length = segment_length(g, span);
+        const int s0 = span.lo + min(static_cast<long long>(j) * length, static_cast<long long>(max(span.hi - span.lo, 0)));
+        const int s1 = min(static_cast<long long>(s0) + length, static_cast<long long>(span.hi));
+        if (s0 >= s1) continue;
+        auto pair = [&](int k) { return ((static_cast<size_t>(i) * g.segments + k) * g.tiles + tile) * 32 + threadIdx.x; };
+        int end = s1;
+        SeqAt seq = seq_at(q, kEnds ? s0 : s1 - 1);
+        if (kEnds) {
+            if (seq.start >= s0) continue;  // no sequence enters the segment
+            end = min(s1, seq.end);
+        }
+        auto copy = [&](int hi, int stage) {
             if constexpr (kWords) {
-                const int t = first - step * stride;
-                if (t + kTokens > span.lo) {
-                    copy_tile<kThreads>(sm.ring[stage][0], DY, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile<kThreads>(sm.ring[stage][1], X, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile<kThreads>(sm.ring[stage][2], F, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile<kThreads>(sm.ring[stage][3], H, t - 1, span.lo, span.hi, p.dim, tile);
+                const int t = hi - kGateGroup;
+                if (hi > s0) {
+                    copy_tile(sm.ring[stage][0], F, t, s0, s1, p.dim, tile);
+                    copy_tile(sm.ring[stage][1], DY, t, s0, s1, p.dim, tile);
+                    if constexpr (!kEnds) {
+                        copy_tile(sm.ring[stage][2], X, t, s0, s1, p.dim, tile);
+                        copy_tile(sm.ring[stage][3], H, t - 1, span.lo, s1, p.dim, tile);
+                    }
                 }
                 cp_async_commit();
             }
         };
-        if constexpr (kWords) {
-            for (int k = 0; k < kStages - 1; ++k) copy(k, k);
-            cp_async_wait<kStages - 2>();
-            __syncthreads();
+        for (int k = 0; k < kStages - 1; ++k) copy(end - k * kGateGroup, k);
+        float2 c = both(0.0f), P = both(1.0f);
+        if (seq.end <= end) {  // (== unless the offsets descend)
+            c = state_row(p.dfinal, seq.seq);
+        } else if (!kEnds && j + 1 < g.segments) {  // what comes from the segments behind
+            int k = min(max(seq.end - 1 - span.lo, 0) / length, g.segments - 1);
+            c = g.h[pair(k)];
+            for (--k; k > j; --k) c = __ffma2_rn(g.P[pair(k)], c, g.h[pair(k)]);
         }
-        float2 carry = both(0.0f);
-        SeqAt seq{0, span.hi, 0};
-        int step = 0, stage = 0;
-        for (int base = span.lo; base < span.hi; base += stride, ++step, ++turn, stage = stage + 1 == kStages ? 0 : stage + 1) {
-            // the warp's tokens are t1, t1 - 1, ...; k counts them
-            const int row1 = kTokens - 1 - warp * kSteps;
-            const int t1 = first - step * stride + row1, left = t1 + 1 - span.lo;
-            auto load = [&](int which, const T *base_ptr, int k, int back) {
-                if constexpr (kWords) return sm.ring[stage][which].at(row1 - k, lane);
-                else return ch.load(base_ptr + static_cast<size_t>(t1 - k - back) * p.dim);
+        SeqAt next{0, 0, 0};
+        float2 next_c = both(0.0f), first_h = both(0.0f);
+        auto look_ahead = [&] {  // this sequence's starting state, and the sequence before it
+            if (kEnds || seq.start < s0) return;
+            first_h = state_row(p.init, seq.seq);
+            if (seq.start == s0) return;
+            next = seq_before(q, seq);
+            next_c = state_row(p.dfinal, next.seq);
+        };
+        look_ahead();
+        int stage = 0;
+        for (int hi = end; hi > s0; hi -= kGateGroup) {
+            if constexpr (kWords) {
+                cp_async_wait<kStages - 2>();
+                __syncwarp();
+            }
+            copy(hi - (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
+            // token hi - 1 - k of a tensor
+            auto load = [&](int which, const T *base, int k, int back) {
+                if constexpr (kWords) return sm.ring[stage][which].at(kGateGroup - 1 - k);
+                else return ch.load(base + static_cast<size_t>(hi - 1 - k - back) * p.dim);
             };
-            if (left > 0 && seq.start > t1) seq = seq_at(q, t1);
-            // no sequence starts or ends in the warp's tokens
-            const bool inside = left >= kSteps && seq.end > t1 + 1 && seq.start < t1 + 1 - kSteps;
-            float2 P[kSteps], G[kSteps], u[kSteps], r[kSteps];  // P and G before the start is known
-            GatePair run{both(1.0f), both(0.0f)};
-            bool cut = false;
-            if (inside) {
+            if (hi - kGateGroup >= s0 && (kEnds || seq.start < hi - kGateGroup)) {
+                if constexpr (kEnds) {
+                    float2 a[kGateGroup], b[kGateGroup];
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    const Gate2 gate = gate_of(load(2, F, k, 0), low, rest);
-                    u[k] = gate.u;
-                    r[k] = gate.r;
-                    P[k] = run.P;
-                    G[k] = __fadd2_rn(load(0, DY, k, 0), run.h);
-                    run.h = __fmul2_rn(gate.a, G[k]);
-                    run.P = __fmul2_rn(run.P, gate.a);
-                }
-            } else {
-                SeqAt at = seq;
+                    for (int k = 0; k < kGateGroup; ++k) {
+                        a[k] = gate_of(load(0, F, k, 0), low, rest).a;
+                        b[k] = __fmul2_rn(a[k], load(1, DY, k, 0));
+                    }
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    u[k] = r[k] = P[k] = G[k] = both(0.0f);
-                    if (k < left) {
-                        if (at.start > t1 - k) at = seq_at(q, t1 - k);
-                        if (at.end == t1 - k + 1) {
-                            run.h = state_row(p.dfinal, at.seq);
-                            cut = true;
-                        }
-                        const Gate2 gate = gate_of(load(2, F, k, 0), low, rest);
+                    for (int k = 0; k < kGateGroup; ++k) {
+                        c = __ffma2_rn(a[k], c, b[k]);
+                        P = __fmul2_rn(P, a[k]);
+                    }
+                } else {
+                    float2 G[kGateGroup], u[kGateGroup], r[kGateGroup];
+#pragma unroll
+                    for (int k = 0; k < kGateGroup; ++k) {
+                        const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
+                        G[k] = gate.a;
                         u[k] = gate.u;
                         r[k] = gate.r;
-                        if (cut) run.P = both(0.0f);
-                        P[k] = run.P;
-                        G[k] = __fadd2_rn(load(0, DY, k, 0), run.h);
-                        run.h = __fmul2_rn(gate.a, G[k]);
-                        run.P = cut ? both(0.0f) : above_zero(__fmul2_rn(run.P, gate.a));
+                    }
+#pragma unroll
+                    for (int k = 0; k < kGateGroup; ++k) {
+                        const float2 v = __fadd2_rn(load(1, DY, k, 0), c);
+                        c = __fmul2_rn(G[k], v);
+                        G[k] = v;
+                    }
+                    T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
+#pragma unroll
+                    for (int k = 0; k < kGateGroup; ++k, dx -= p.dim, df -= p.dim) {
+                        const float2 x = load(2, X, k, 0), before = load(3, H, k, 1);
+                        const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
+                        const float2 w = __fmul2_rn(__fmul2_rn(G[k], diff), u[k]);
+                        dlow = __fadd2_rn(dlow, w);
+                        if (ch.active[0]) {
+                            ch.store(dx, __fmul2_rn(u[k], G[k]));
+                            ch.store(df, __fmul2_rn(w, r[k]));
+                        }
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int k = 0; k < kGateGroup && hi - 1 - k >= s0; ++k) {
+                    const int t = hi - 1 - k;
+                    const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
+                    if constexpr (kEnds) {
+                        c = __ffma2_rn(gate.a, c, __fmul2_rn(gate.a, load(1, DY, k, 0)));
+                        P = __fmul2_rn(P, gate.a);
+                    } else {
+                        const float2 G = __fadd2_rn(load(1, DY, k, 0), c);
+                        const bool begins = seq.start == t;
+                        const float2 x = load(2, X, k, 0), before = begins ? first_h : load(3, H, k, 1);
+                        const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
+                        const float2 w = __fmul2_rn(__fmul2_rn(G, diff), gate.u);
+                        dlow = __fadd2_rn(dlow, w);
+                        c = __fmul2_rn(gate.a, G);
+                        if (ch.active[0]) {
+                            ch.store(DX + static_cast<size_t>(t) * p.dim, __fmul2_rn(gate.u, G));
+                            ch.store(DF + static_cast<size_t>(t) * p.dim, __fmul2_rn(w, gate.r));
+                        }
+                        if (begins) {
+                            store_dinit(seq.seq, c);
+                            seq = next;
+                            c = next_c;
+                            if (t > s0) look_ahead();
+                        }
                     }
                 }
             }
-            if (inside) run.P = above_zero(run.P);
-            if constexpr (kWords) cp_async_wait<kStages - 3>();  // the next tiles, which the join's barrier makes everyone's
-            const float2 start = gate_join(sm.join, turn, g.cluster, rank, run, carry, lost);
-            copy(step + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);  // into the tiles of the step before: all are done with them
-            auto finish = [&](int k, float2 Gk, float2 before) {
-                const size_t at = static_cast<size_t>(t1 - k) * p.dim;
-                const float2 x = load(1, X, k, 0);
-                const float2 diff = make_float2(before.x - x.x, before.y - x.y);
-                const float2 w = __fmul2_rn(__fmul2_rn(Gk, diff), u[k]);
-                if (ch.active[0]) {
-                    ch.store(DX + at, __fmul2_rn(u[k], Gk));
-                    ch.store(DF + at, __fmul2_rn(w, r[k]));
-                }
-                dlow = __fadd2_rn(dlow, w);
-            };
-            if (inside && __all_sync(kFullMask, finite2(start))) {
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) finish(k, __ffma2_rn(P[k], start, G[k]), load(3, H, k, 1));
-            } else {
-                SeqAt at = seq;
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    if (k >= left) break;
-                    if (at.start > t1 - k) at = seq_at(q, t1 - k);
-                    const float2 Gk = join_any(GatePair{inside ? above_zero(P[k]) : P[k], G[k]}, start);
-                    const bool begins = at.start == t1 - k;
-                    finish(k, Gk, begins ? state_row(p.init, at.seq) : load(3, H, k, 1));
-                    if (begins) store_dinit(at.seq, __fmul2_rn(__ffma2_rn(rest, r[k], low), Gk));
-                }
-            }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+        if constexpr (kEnds) {
+            g.P[pair(j)] = above_zero(P);
+            g.h[pair(j)] = c;
         }
         cp_async_wait<0>();
-        __syncthreads();  // (the ring is filled anew)
+        __syncwarp();  // (the ring is filled anew)
     }
-    if (g.cluster > 1) {
-        if (lost && threadIdx.x == 0) atomicAdd(&g_gate_grad_wait_failures, 1u);
-        cluster_barrier();
+    if (!kEnds && part != nullptr)  // da (1 - a) = da (1 - bound) sigmoid(-f)
+        ch.store_floats(part + static_cast<size_t>(slot * segs + j) * p.dim, make_float2(dlow.x / rest.x, dlow.y / rest.y));
+}
+
+template <typename T, bool kWords>
+cudaError_t launch_words(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
+    if (g.segments > 1) {
+        const cudaError_t e = launch_gate(gate_grad_kernel<T, kWords, true>, sizeof(GradSmem<T, kWords, true>), g,
+                                          g.segments - 1, stream, a, g, part);
+        if (e != cudaSuccess) return e;
     }
-    if (part != nullptr) {  // the block's sum, the warps' added in order
-        sm.join.warp[0][warp][lane].h = dlow;
-        __syncthreads();
-        if (warp == 0) {
-            float2 sum = both(0.0f);
-            for (int w = 0; w < kWarps; ++w) sum = __fadd2_rn(sum, sm.join.warp[0][w][lane].h);
-            sum = make_float2(sum.x / rest.x, sum.y / rest.y);  // da (1 - a) = da (1 - bound) sigmoid(-f)
-            ch.store_floats(part + static_cast<size_t>(slot * g.cluster + rank) * p.dim, sum);
-        }
-    }
+    return launch_gate(gate_grad_kernel<T, kWords, false>, sizeof(GradSmem<T, kWords, false>), g, g.segments, stream, a, g,
+                       part);
 }
 
 template <typename T>
-cudaError_t launch_type(const GateGradArgs &a, float *part, const GateSpans &g, cudaStream_t stream) {
+cudaError_t launch_type(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
     if (a.dim * sizeof(T) % 16 == 0 && aligned16(a.dy) && aligned16(a.x) && aligned16(a.f) && aligned16(a.y) &&
         aligned16(a.dx) && aligned16(a.df))
-        return launch_gate_clusters(gate_grad_kernel<T, true>, kThreads, sizeof(GradSmem<T, true>), g, stream, a, g, part);
-    return launch_gate_clusters(gate_grad_kernel<T, false>, kThreads, sizeof(GradSmem<T, false>), g, stream, a, g, part);
+        return launch_words<T, true>(a, g, part, stream);
+    return launch_words<T, false>(a, g, part, stream);
 }
+
+GateCut cut_of(const GateGradArgs &a) { return gate_cut(a.seq, a.dim, a.want_dbound ? kMaxParts : INT_MAX); }
 
 }  // namespace
 
-cudaError_t gate_grad_take_wait_failures(unsigned int *count) {
-    cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) {
-        gate_grad_swap_failures<<<1, 1>>>();
-        e = cudaGetLastError();
-    }
-    return e == cudaSuccess ? cudaMemcpyFromSymbol(count, g_gate_grad_failures_taken, sizeof(*count)) : e;
-}
-
 size_t gated_recurrence_grad_workspace(const GateGradArgs &a) {
-    if (!a.want_dbound || a.dim == 0) return 0;
-    const GateSpans g = gate_spans(a.seq, a.dim, kTokens);
-    const size_t parts = static_cast<size_t>(g.width) * g.cluster;
-    return parts > 1 ? parts * a.dim * sizeof(float) : 0;
+    if (a.dim == 0) return 0;
+    const GateCut g = cut_of(a);
+    const size_t parts = static_cast<size_t>(g.width) * g.segments;
+    return 2 * gate_pairs(g) * sizeof(float2) + (a.want_dbound && parts > 1 ? parts * a.dim * sizeof(float) : 0);
 }
 
 cudaError_t launch_gated_recurrence_grad(const GateGradArgs &a, void *workspace, cudaStream_t stream) {
-    const GateSpans g = gate_spans(a.seq, a.dim, kTokens);
-    const int parts = g.width * g.cluster;
-    float *part = a.dbound == nullptr ? nullptr : parts > 1 ? static_cast<float *>(workspace) : a.dbound;
+    GateCut g = cut_of(a);
+    g.P = static_cast<float2 *>(workspace);
+    g.h = g.P + gate_pairs(g);
+    const int parts = g.width * g.segments;
+    float *part = a.dbound == nullptr ? nullptr : parts > 1 ? reinterpret_cast<float *>(g.h + gate_pairs(g)) : a.dbound;
     cudaError_t e;
     switch (a.io) {
-        case IoType::kBF16: e = launch_type<__nv_bfloat16>(a, part, g, stream); break;
-        case IoType::kF16: e = launch_type<__half>(a, part, g, stream); break;
-        default: e = launch_type<float>(a, part, g, stream);
+        case IoType::kBF16: e = launch_type<__nv_bfloat16>(a, g, part, stream); break;
+        case IoType::kF16: e = launch_type<__half>(a, g, part, stream); break;
+        default: e = launch_type<float>(a, g, part, stream);
     }
     if (e != cudaSuccess || a.dbound == nullptr || parts == 1) return e;
     return launch_column_sums(part, nullptr, parts, a.dim, a.dbound, nullptr, stream);

@@ -1,23 +1,23 @@
 // xm_gate.cuh -- what the gated linear recurrence and its backward pass share: the
-// gate, the walk over sequences, and the scan over the token axis.
+// gate, the walk over sequences, and how a call is cut.
 //
 // Both are first-order recurrences per channel, h <- a h + b, forwards over the
-// tokens or backwards. A lane holds two channels, a warp some consecutive
-// tokens of 64 channels; the block's warps follow one another along the axis, and so
-// do the blocks of a cluster. Each warp runs its tokens from zero and keeps, per
-// token, h and the product P of the a up to it, so that the value with the true start
-// h0 is h + P h0: the start needs to be known only after the loads and exponentials
-// are done. The starts come by joining (P, h) pairs, first over the block's warps in
-// shared memory, then over the cluster's blocks in each other's shared memory, and
-// the cluster walks on with the last value as carry. So the axis is read once, every
-// wait is a hardware barrier, and the order of all operations is fixed.
+// tokens or backwards. A warp is a block of its own: it holds 64 channels, two per
+// lane, and walks tokens in groups of kGroup. The gates of a group do not depend on
+// h, so their exponentials overlap; only one multiply-add per token is in sequence.
+// Tiles of tokens come by asynchronous copies some groups ahead, and no warp waits
+// for another.
+//
+// Where there are too few rows for the device, a row is cut into segments. A first
+// pass then walks the segments that a sequence leaves, from zero, and keeps h at the
+// segment's end with the product P of the a: a start h0 would have added P h0. The
+// second pass joins these pairs from the sequence's start up to its own segment.
 #pragma once
 
 #include <algorithm>
 
 #include "xm_common.cuh"
 #include "xm_sequences.cuh"
-#include "xm_umma.cuh"
 
 namespace xm {
 
@@ -48,25 +48,31 @@ __device__ __forceinline__ Gate2 gate_of(float2 f, float2 low, float2 rest) {
     return g;
 }
 
-constexpr int kGateChannels = 64;  // channels of a block
-constexpr int kGateMaxCluster = 8;
+constexpr int kGateChannels = 64;  // channels of a warp
+constexpr int kGateGroup = 16;     // tokens of a group
 
-// The tokens that a cluster walks: a batch row, several short ones, or the packed row.
-struct GateSpans {
-    int rows;     // spans
-    int length;   // tokens of a span; with cu the span is [cu[0], cu[units])
-    int tiles;    // blocks of channels
-    int cluster;  // blocks of a cluster
-    int width;    // spans walked at the same time
+// How a call is cut. A span is a batch row, several short ones, or the packed row.
+struct GateCut {
+    int spans, length;  // length: tokens of a span; with cu it is [cu[0], cu[units])
+    int width;          // spans walked at the same time
+    int segments;       // of a span
+    int tiles;          // groups of channels
+    float2 *P, *h, *start;  // [spans][segments][tiles][32]: the pairs, and the state that a leaving sequence started from
 };
 
+// Tokens [lo, hi) of segment j of span i.
 struct Span {
     int lo, hi;
 };
-__device__ __forceinline__ Span gate_span(const SeqArgs &q, const GateSpans &s, int i) {
+__device__ __forceinline__ Span gate_span(const SeqArgs &q, const GateCut &g, int i) {
     if (q.cu != nullptr) return Span{seq_start(q, 0), seq_start(q, q.units)};
-    const int lo = i * s.length;
-    return Span{lo, lo + min(s.length, q.tokens - lo)};
+    const int lo = i * g.length;
+    return Span{lo, lo + min(g.length, q.tokens - lo)};
+}
+__device__ __forceinline__ int segment_length(const GateCut &g, Span s) {
+    if (g.segments == 1) return max(s.hi - s.lo, 1);
+    const int n = (max(s.hi - s.lo, 0) + g.segments - 1) / g.segments;
+    return max((n + kGateGroup - 1) / kGateGroup * kGateGroup, kGateGroup);
 }
 
 // The sequence that holds a token: [start, end) of sequence seq.
@@ -81,16 +87,28 @@ __device__ __forceinline__ SeqAt seq_at(const SeqArgs &q, int t) {
     const int next = max(seq_first_from(q, t + 1), 1);  // first that starts behind t
     return SeqAt{next - 1, seq_start(q, next - 1), seq_start(q, next)};
 }
+// The same for the token behind, or before, a sequence that is known.
+__device__ __forceinline__ SeqAt seq_behind(const SeqArgs &q, const SeqAt &s) {
+    if (q.cu != nullptr && s.seq + 2 <= q.units) {
+        const int end = seq_start(q, s.seq + 2);
+        if (end > s.end) return SeqAt{s.seq + 1, s.end, end};
+    }
+    return seq_at(q, s.end);
+}
+__device__ __forceinline__ SeqAt seq_before(const SeqArgs &q, const SeqAt &s) {
+    if (q.cu != nullptr && s.seq >= 1) {
+        const int start = seq_start(q, s.seq - 1);
+        if (start < s.start) return SeqAt{s.seq - 1, start, s.start};
+    }
+    return seq_at(q, s.start - 1);
+}
 
-// Calls f(sequence) for the sequences without tokens, shared out over the warps of all
-// blocks with the same channels (block `block` of `blocks`).
-template <int kWarps, typename F>
-__device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int block, int blocks, F &&f) {
+// Calls f(sequence) for the sequences without tokens, shared out over `warps` warps with the same channels.
+template <typename F>
+__device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int warp, int warps, F &&f) {
     if (q.cu == nullptr && q.seqlen > 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (long long s0 = (static_cast<long long>(block) * kWarps + warp) * 32; s0 < q.units;
-         s0 += 32LL * kWarps * blocks) {
-        const int s = static_cast<int>(s0) + lane;
+    for (long long s0 = static_cast<long long>(warp) * 32; s0 < q.units; s0 += 32LL * warps) {
+        const int s = static_cast<int>(s0) + static_cast<int>(threadIdx.x);
         bool empty = false;
         if (s < q.units) {
             const int t = seq_start(q, s);
@@ -101,174 +119,14 @@ __device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int block,
     }
 }
 
-// A (P, h) pair stands for h0 -> P h0 + h. Where a sequence starts inside, P is zero
-// and nothing of h0 may get through; elsewhere products of gates are kept above zero,
-// so that an infinite h0 outlasts their underflow as it does step by step. As long as
-// h0 is finite a multiply-add does both, and it only gives a finite value if h0 was
-// one; values that come out infinite or NaN are joined once more with `join_any`.
-struct GatePair {
-    float2 P, h;
-};
-constexpr float kLeast = 1.4e-45f;
-__device__ __forceinline__ float2 above_zero(float2 P) { return make_float2(fmaxf(P.x, kLeast), fmaxf(P.y, kLeast)); }
-__device__ __forceinline__ bool finite2(float2 v) { return fabsf(v.x) <= 3.4028235e38f && fabsf(v.y) <= 3.4028235e38f; }
-__device__ __forceinline__ float2 join(const GatePair &p, float2 h0) { return __ffma2_rn(p.P, h0, p.h); }
-__device__ __forceinline__ float2 join_any(const GatePair &p, float2 h0) {
-    return make_float2(p.P.x == 0.0f ? p.h.x : fmaf(p.P.x, h0.x, p.h.x), p.P.y == 0.0f ? p.h.y : fmaf(p.P.y, h0.y, p.h.y));
-}
-__device__ __forceinline__ float2 product(float2 P, float2 before) {
-    const float2 v = __fmul2_rn(P, before);
-    return make_float2(P.x == 0.0f || before.x == 0.0f ? 0.0f : fmaxf(v.x, kLeast),
-                       P.y == 0.0f || before.y == 0.0f ? 0.0f : fmaxf(v.y, kLeast));
-}
-
-// Shared memory of the join; parity alternates from step to step.
-template <int kWarps>
-struct GateJoin {
-    GatePair warp[2][kWarps][32];
-    GatePair block[2][kGateMaxCluster][32];
-    uint64_t arrived[2];  // the cluster's pairs of a step are here
-};
-
-__device__ __forceinline__ GatePair load_pair(const GatePair &p) {
-    const float4 w = *reinterpret_cast<const float4 *>(&p);
-    return GatePair{make_float2(w.x, w.y), make_float2(w.z, w.w)};
-}
-
-__device__ __forceinline__ unsigned cluster_rank() {
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ uint32_t address_in_block(const void *smem, unsigned rank) {
-    uint32_t there;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;"
-        : "=r"(there)
-        : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "r"(rank));
-    return there;
-}
-// A pair into another block's shared memory; its bytes count on that block's `arrived`. (A cluster barrier per step,
-// whose release waits for the block's own stores to global memory, took two to five microseconds under load.)
-__device__ __forceinline__ void send_pair(uint32_t there, uint32_t arrived, const GatePair &p) {
-    asm volatile(
-        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there),
-        "f"(p.P.x), "f"(p.P.y), "f"(p.h.x), "f"(p.h.y), "r"(arrived)
-        : "memory");
-}
-// Waits for a phase of `arrived`, a bounded number of times.
-__device__ __forceinline__ bool wait_arrived(uint64_t *arrived, uint32_t phase) {
-    const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(arrived));
-    for (uint32_t i = 0; i < (1u << 22); ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t"
-            ".reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t"
-            "}\n"
-            : "=r"(done)
-            : "r"(a), "r"(phase)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
-}
-
-// Before the first join and behind the last, by all threads of a cluster of several blocks: every block has begun, and
-// none has left, while others write into its shared memory.
-template <int kWarps>
-__device__ __forceinline__ void gate_join_begin(GateJoin<kWarps> &s) {
-    if (threadIdx.x == 0) {
-        umma::mbar_init(&s.arrived[0], 1);
-        umma::mbar_init(&s.arrived[1], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    cluster_barrier();
-}
-
-// The values before and behind this block's part of the step.
-template <int K, int kWarps>
-__device__ __forceinline__ void join_blocks(const GateJoin<kWarps> &s, int parity, unsigned rank, float2 &start,
-                                            float2 &carry) {
-    const int lane = threadIdx.x & 31;
-    GatePair p[K];
-#pragma unroll
-    for (int r = 0; r < K; ++r) p[r] = load_pair(s.block[parity][r][lane]);
-#pragma unroll
-    for (int r = 0; r < K; ++r) {
-        if (r == static_cast<int>(rank)) start = carry;
-        carry = join(p[r], carry);
-    }
-}
-
-// Joins the warps' pairs of step `turn`, counted from 0 over the kernel. Returns the
-// value that this warp's tokens start from and moves `carry` from the step's start to
-// its end. Called by all threads of the cluster; also a __syncthreads() of the block.
-// `lost`: a wait gave up, here or before.
-template <int kWarps>
-__device__ __forceinline__ float2 gate_join(GateJoin<kWarps> &s, unsigned turn, int cluster, unsigned rank,
-                                            const GatePair &mine, float2 &carry, bool &lost) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, parity = turn & 1;
-    *reinterpret_cast<float4 *>(&s.warp[parity][warp][lane]) = make_float4(mine.P.x, mine.P.y, mine.h.x, mine.h.y);
-    __syncthreads();
-    float2 start = carry, behind = carry;
-    if (cluster > 1) {
-        if (warp == kWarps - 1) {  // the block's pair, to every block
-            GatePair p[kWarps];
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) p[w] = load_pair(s.warp[parity][w][lane]);
-            GatePair b = p[0];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) b.h = join(p[w], b.h), b.P = product(p[w].P, b.P);
-            if (!finite2(b.h)) {
-                b.h = p[0].h;
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) b.h = join_any(p[w], b.h);
-            }
-            for (int r = 0; r < cluster; ++r)
-                send_pair(address_in_block(&s.block[parity][rank][lane], r), address_in_block(&s.arrived[parity], r), b);
-            if (lane == 0) umma::mbar_arrive_expect_tx(&s.arrived[parity], cluster * 32 * sizeof(GatePair));
-        }
-        if (!lost) lost = !wait_arrived(&s.arrived[parity], turn >> 1 & 1);
-        if (cluster == 2) join_blocks<2>(s, parity, rank, start, behind);
-        else if (cluster == 4) join_blocks<4>(s, parity, rank, start, behind);
-        else join_blocks<8>(s, parity, rank, start, behind);
-#pragma unroll
-        for (int w = 0; w < kWarps - 1; ++w)
-            if (w < warp) start = join(load_pair(s.warp[parity][w][lane]), start);
-    } else {
-        GatePair p[kWarps];
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) p[w] = load_pair(s.warp[parity][w][lane]);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w == warp) start = behind;
-            behind = join(p[w], behind);
-        }
-    }
-    if (!__all_sync(kFullMask, finite2(start) && finite2(behind))) {
-        behind = start = carry;
-        for (int r = 0; r < (cluster > 1 ? cluster : 0); ++r) {
-            if (r == static_cast<int>(rank)) start = behind;
-            behind = join_any(load_pair(s.block[parity][r][lane]), behind);
-        }
-        for (int w = 0; w < kWarps; ++w) {
-            if (cluster == 1) behind = join_any(load_pair(s.warp[parity][w][lane]), behind);
-            if (w < warp) start = join_any(load_pair(s.warp[parity][w][lane]), start);
-        }
-    }
-    carry = behind;
-    return start;
-}
+// Products of gates are kept above zero, so that an infinite start outlasts their underflow as it does step by step.
+__device__ __forceinline__ float2 above_zero(float2 P) { return make_float2(fmaxf(P.x, 1.4e-45f), fmaxf(P.y, 1.4e-45f)); }
 
 // A lane's two channels: neighbours, moved as one word (kWords: rows of whole 16-byte
 // words, aligned to them), else 32 apart and moved one by one.
 template <typename T, bool kWords>
 struct Lane {
-    int c[2];        // channels (0 where there is none)
+    int c[2];  // channels (0 where there is none)
     bool active[2];
     __device__ __forceinline__ Lane(int tile, int lane, int dim) {
 #pragma unroll
@@ -299,68 +157,49 @@ struct Lane {
     }
 };
 
-// A block's tokens of one tensor in shared memory, and the copy that fills it: 16-byte
-// words of consecutive threads.
-template <typename T, int kTokens>
+// A group's tokens of one tensor in shared memory, and the warp's copy that fills it.
+template <typename T>
 struct GateTile {
-    T v[kTokens][kGateChannels];
-    __device__ __forceinline__ float2 at(int row, int lane) const {
-        if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][2 * lane]));
-        else return *reinterpret_cast<const float2 *>(&v[row][2 * lane]);
+    T v[kGateGroup][kGateChannels];
+    __device__ __forceinline__ float2 at(int row) const {
+        if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][2 * threadIdx.x]));
+        else return *reinterpret_cast<const float2 *>(&v[row][2 * threadIdx.x]);
     }
 };
-// Rows first + 0 .. kTokens - 1 of a tensor's channels; those outside [lo, hi) are left out.
-template <int kThreads, typename T, int kTokens>
-__device__ __forceinline__ void copy_tile(GateTile<T, kTokens> &dst, const T *src, int first, int lo, int hi, int dim,
-                                          int tile) {
+// Rows first .. first + kGateGroup - 1 of a tensor's channels; those outside [lo, hi) are left out.
+template <typename T>
+__device__ __forceinline__ void copy_tile(GateTile<T> &dst, const T *src, int first, int lo, int hi, int dim, int tile) {
     constexpr int kPer = 16 / static_cast<int>(sizeof(T)), kWordsRow = kGateChannels / kPer;
-    constexpr int kRows = kThreads / kWordsRow;  // rows per pass
+    constexpr int kRows = 32 / kWordsRow;  // rows per pass
     const int col = threadIdx.x % kWordsRow * kPer, row = threadIdx.x / kWordsRow;
     if (tile * kGateChannels + col >= dim) return;
     const T *p = src + static_cast<int64_t>(first + row) * dim + tile * kGateChannels + col;
-    if (first >= lo && first + kTokens <= hi) {
+    if (first >= lo && first + kGateGroup <= hi) {
 #pragma unroll
-        for (int k = 0; k < kTokens; k += kRows, p += static_cast<int64_t>(kRows) * dim) cp_async16(&dst.v[row + k][col], p, 16);
+        for (int k = 0; k < kGateGroup; k += kRows, p += static_cast<int64_t>(kRows) * dim)
+            cp_async16(&dst.v[row + k][col], p, 16);
         return;
     }
 #pragma unroll
-    for (int k = 0; k < kTokens; k += kRows, p += static_cast<int64_t>(kRows) * dim) {
+    for (int k = 0; k < kGateGroup; k += kRows, p += static_cast<int64_t>(kRows) * dim) {
         const int t = first + row + k;
         if (t >= lo && t < hi) cp_async16(&dst.v[row + k][col], p, 16);
     }
 }
 
-// Zeros where copy_tile leaves channels behind the last one out: what is computed of them stays finite.
-template <typename R>
-__device__ __forceinline__ void clear_ring(R &ring, int dim, int tile) {
-    if ((tile + 1) * kGateChannels <= dim) return;
-    for (unsigned i = threadIdx.x; i < sizeof(R) / 16; i += blockDim.x)
-        reinterpret_cast<float4 *>(&ring)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    __syncthreads();
+// The cut of a call (without pointers). parts: at most as many warps per tile.
+GateCut gate_cut(const SeqArgs &q, int dim, int parts);
+inline size_t gate_pairs(const GateCut &g) {  // elements of each of P, h and start
+    return g.segments > 1 ? static_cast<size_t>(g.spans) * g.segments * g.tiles * 32 : 0;
 }
 
-// How a call is cut: blocks of channels, spans, and the cluster along the tokens, of which a block takes `tokens` at a
-// time.
-GateSpans gate_spans(const SeqArgs &q, int dim, int tokens);
-
 template <typename... Params, typename... Args>
-cudaError_t launch_gate_clusters(void (*kernel)(Params...), int threads, size_t smem, const GateSpans &g, cudaStream_t stream,
-                                 const Args &...args) {
+cudaError_t launch_gate(void (*kernel)(Params...), size_t smem, const GateCut &g, int segments, cudaStream_t stream,
+                        const Args &...args) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(g.width) * g.tiles * g.cluster);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = g.cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = g.cluster > 1 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    return e == cudaSuccess ? cudaGetLastError() : e;
+    kernel<<<static_cast<unsigned>(g.width) * segments * g.tiles, 32, smem, stream>>>(args...);
+    return cudaGetLastError();
 }
 
 }  // namespace xm

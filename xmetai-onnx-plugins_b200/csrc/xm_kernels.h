@@ -180,7 +180,9 @@ struct GateArgs {
     float *final_state;  // or null
     void *out;
 };
-cudaError_t launch_gated_recurrence(const GateArgs &a, cudaStream_t stream);
+size_t gated_recurrence_workspace(const GateArgs &a);
+// `workspace` must hold gated_recurrence_workspace(a) bytes, 256-byte aligned.
+cudaError_t launch_gated_recurrence(const GateArgs &a, void *workspace, cudaStream_t stream);
 // One token per sequence: x, f, out [units, dim]; init and final_state both given.
 cudaError_t launch_gated_recurrence_update(const GateArgs &a, cudaStream_t stream);
 
@@ -198,11 +200,6 @@ struct GateGradArgs {
 size_t gated_recurrence_grad_workspace(const GateGradArgs &a);
 // `workspace` must hold gated_recurrence_grad_workspace(a) bytes, 256-byte aligned.
 cudaError_t launch_gated_recurrence_grad(const GateGradArgs &a, void *workspace, cudaStream_t stream);
-
-// Blocks of the two whose wait for another block of their cluster gave up on the current device (their outputs are
-// incomplete); reads and clears the counts, after synchronising the device.
-cudaError_t gate_take_wait_failures(unsigned int *count);
-cudaError_t gate_grad_take_wait_failures(unsigned int *count);
 
 // out0[d] = sum over r of part0[r][d], and the same of part1 into out1 (null: not there), in a fixed order.
 cudaError_t launch_column_sums(const float *part0, const float *part1, int rows, int dim, float *out0, float *out1,
