@@ -12,11 +12,16 @@
 namespace xm {
 namespace {
 
-constexpr int kStages = 6;  // groups of x and f in use and under way
+constexpr int kStages = 6;      // groups of x and f in use and under way, of a warp with a row or segment
+// And of a warp in a ring: what leaves an SM as many blocks as its registers do (16-bit types: five; 8 x 2048 x 4096
+// takes 71 us, and 83 with three stages and four blocks), or its copies (float32: two; 8 x 1024 x 4096 takes 70 us, and
+// 78 with two stages and four blocks).
+template <typename T>
+constexpr int kRingStages = sizeof(T) == 4 ? 3 : 2;
 
 template <typename T, bool kWords>
 struct ScanSmem {
-    GateTile<T> ring[kWords ? kStages : 0][2];
+    GateTile<T, kGateGroup> ring[kWords ? kStages : 0][2];
 };
 
 // kEnds: the first pass over segments (all but a span's last).
@@ -27,7 +32,7 @@ __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const Gat
     const SeqArgs &q = p.seq;
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs, slot = blockIdx.x / g.tiles / segs;
-    const Lane<T, kWords> ch(tile, threadIdx.x, p.dim);
+    const Lane<T, kWords> ch(tile, threadIdx.x & 31, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
     T *const Y = static_cast<T *>(p.out);
@@ -158,6 +163,120 @@ __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const Gat
     }
 }
 
+template <typename T, bool kWords>
+struct RingSmem {
+    Ring hand;
+    GateTile<T, kGateGroup> ring[kWords ? kRingWarps : 0][kRingStages<T>][2];
+};
+
+template <typename T, bool kWords>
+__global__ void __launch_bounds__(32 * kRingWarps, 5) gate_ring_kernel(const GateArgs p, const GateCut g) {
+    extern __shared__ float4 smem_f4[];
+    constexpr int kStages = kRingStages<T>;
+    auto &sm = *reinterpret_cast<RingSmem<T, kWords> *>(smem_f4);
+    const SeqArgs &q = p.seq;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
+    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
+    T *const Y = static_cast<T *>(p.out);
+    auto init_of = [&](int seq) {
+        const long long row = seq_row(q, seq);
+        return ch.floats(p.init != nullptr && seq_live(q, seq, row) ? p.init + row * p.dim : nullptr, 0.0f);
+    };
+    auto store_final = [&](int seq, float2 h) {
+        const long long row = seq_row(q, seq);
+        if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
+    };
+    if (p.final_state != nullptr)  // sequences without tokens keep their starting states
+        for_empty_sequences(q, slot * kRingWarps + warp, g.width * kRingWarps, [&](int s) { store_final(s, init_of(s)); });
+    for (int i = slot; i < g.spans; i += g.width) {
+        const Span span = gate_span(q, g, i);
+        constexpr int kTurn = kRingWarps * kGateGroup;  // tokens of a round
+        const int first = span.lo + warp * kGateGroup;
+        auto copy = [&](int t, int stage) {
+            if constexpr (kWords) {
+                if (t < span.hi) {
+                    copy_tile(sm.ring[warp][stage][0], X, t, 0, span.hi, p.dim, tile);
+                    copy_tile(sm.ring[warp][stage][1], F, t, 0, span.hi, p.dim, tile);
+                }
+                cp_async_commit();
+            }
+        };
+        for (int k = 0; k < kStages - 1; ++k) copy(first + k * kTurn, k);
+        SeqAt seq{0, 0, 0};
+        int stage = 0;
+        for (int t = first; t < span.hi; t += kTurn) {
+            if constexpr (kWords) {
+                cp_async_wait<kStages - 2>();
+                __syncwarp();
+            }
+            copy(t + (kStages - 1) * kTurn, stage == 0 ? kStages - 1 : stage - 1);  // read by all a round ago
+            auto token = [&](int k, float2 &x, float2 &f) {
+                if constexpr (kWords) {
+                    x = sm.ring[warp][stage][0].at(k);
+                    f = sm.ring[warp][stage][1].at(k);
+                } else {
+                    const size_t at = static_cast<size_t>(t + k) * p.dim;
+                    x = ch.load(X + at);
+                    f = ch.load(F + at);
+                }
+            };
+            if (seq.end <= t) seq = seq_at(q, t);
+            const bool more = t + kGateGroup < span.hi;  // a group behind
+            const int next = warp + 1 == kRingWarps ? 0 : warp + 1;
+            // (whether a group takes and gives depends on t alone, so that offsets that descend leave nobody waiting)
+            if (t > span.lo && t + kGateGroup <= span.hi && seq.start < t && seq.end > t + kGateGroup) {
+                float2 P[kGateGroup], h[kGateGroup];
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k) {
+                    float2 x, f;
+                    token(k, x, f);
+                    const Gate2 gate = gate_of(f, low, rest);
+                    P[k] = gate.a;
+                    h[k] = __fmul2_rn(gate.u, x);
+                }
+#pragma unroll
+                for (int k = 1; k < kGateGroup; ++k) {
+                    h[k] = __ffma2_rn(P[k], h[k - 1], h[k]);
+                    P[k] = __fmul2_rn(P[k], P[k - 1]);
+                }
+                const float2 start = sm.hand.take(warp);
+                const bool finite = __all_sync(kFullMask, finite2(start));
+                if (!finite) {
+#pragma unroll
+                    for (int k = 0; k < kGateGroup; ++k) P[k] = above_zero(P[k]);
+                }
+                if (more) sm.hand.give(next, __ffma2_rn(P[kGateGroup - 1], start, h[kGateGroup - 1]));
+                if (ch.active[0]) {
+                    T *y = Y + static_cast<size_t>(t) * p.dim;
+#pragma unroll
+                    for (int k = 0; k < kGateGroup; ++k, y += p.dim) ch.store(y, __ffma2_rn(P[k], start, h[k]));
+                }
+            } else {
+                SeqAt at = seq;
+                float2 h = t > span.lo ? sm.hand.take(warp) : both(0.0f);
+#pragma unroll 1
+                for (int k = 0; k < kGateGroup && t + k < span.hi; ++k) {
+                    if (at.end <= t + k) at = seq_at(q, t + k);
+                    if (at.start == t + k) h = init_of(at.seq);
+                    float2 x, f;
+                    token(k, x, f);
+                    const Gate2 gate = gate_of(f, low, rest);
+                    h = __ffma2_rn(gate.a, h, __fmul2_rn(gate.u, x));
+                    if (ch.active[0]) ch.store(Y + static_cast<size_t>(t + k) * p.dim, h);
+                    if (at.end == t + k + 1) store_final(at.seq, h);
+                }
+                if (more) sm.hand.give(next, h);
+            }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+        cp_async_wait<0>();
+        __syncthreads();  // the rings are filled anew, the hands start anew
+    }
+}
+
 constexpr int kTokenThreads = 128;
 
 template <typename T>
@@ -180,11 +299,13 @@ __global__ void __launch_bounds__(kTokenThreads) gate_token_kernel(const GateArg
 template <typename T, bool kWords>
 cudaError_t launch_words(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
     constexpr size_t kSmem = sizeof(ScanSmem<T, kWords>);
+    if (g.ring)
+        return launch_gate(gate_ring_kernel<T, kWords>, kRingWarps, sizeof(RingSmem<T, kWords>), g, 1, stream, a, g);
     if (g.segments > 1) {
-        const cudaError_t e = launch_gate(gate_kernel<T, kWords, true>, kSmem, g, g.segments - 1, stream, a, g);
+        const cudaError_t e = launch_gate(gate_kernel<T, kWords, true>, 1, kSmem, g, g.segments - 1, stream, a, g);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate(gate_kernel<T, kWords, false>, kSmem, g, g.segments, stream, a, g);
+    return launch_gate(gate_kernel<T, kWords, false>, 1, kSmem, g, g.segments, stream, a, g);
 }
 
 template <typename T>
@@ -216,9 +337,14 @@ GateCut gate_cut(const SeqArgs &q, int dim, int parts) {
         g.spans = g.length > 0 ? static_cast<int>((static_cast<int64_t>(q.tokens) + g.length - 1) / g.length) : 1;
     }
     const int64_t warps = static_cast<int64_t>(g.spans) * g.tiles, sms = current_device_sm_count();
+    // A row per block needs four fifths of the device's blocks to be the faster (8 x 2048 x 1024, 128 blocks: 40 us
+    // against 38 in eight segments; 2 x 8192 x 4096, 128 blocks: 131 against 121; 4 x 2048 x 4096, 256 blocks: 50
+    // against 64). With fewer, one wave of eight warps an SM (16384 x 4096 packed: 119 to 121 us in 16 or 18 segments, 147
+    // in 24), of 32 tokens at least (512 x 4096: 10 us in 16, 14 in 32). Rows below 128 tokens: a warp each.
     g.segments = 1;
-    if (warps * 10 < sms * 24 && g.length > 128)
-        g.segments = static_cast<int>(std::min<int64_t>((8 * sms + warps - 1) / warps, (g.length + 63) / 64));
+    g.ring = g.length >= 128 && warps * 5 >= sms * 4;
+    if (!g.ring && g.length >= 128)
+        g.segments = static_cast<int>(std::min<int64_t>(std::max<int64_t>(sms * 81 / 10 / warps, 1), (g.length + 31) / 32));
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(parts, (int64_t(1) << 30) / g.tiles) / g.segments);
     g.width = static_cast<int>(std::min<int64_t>(g.spans, most));
     return g;

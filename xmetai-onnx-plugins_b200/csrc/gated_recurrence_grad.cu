@@ -24,7 +24,7 @@ template <typename T, bool kWords, bool kEnds>
 struct GradSmem {
     static constexpr int kStages = sizeof(T) == 4 ? 3 : 5;  // groups in use and under way
     static constexpr int kTensors = kEnds ? 2 : 4;          // f, dy; x, and y of the token before
-    GateTile<T> ring[kWords ? kStages : 0][kTensors];
+    GateTile<T, kGateGroup> ring[kWords ? kStages : 0][kTensors];
 };
 
 // kEnds: the first pass over segments (all but a span's first).
@@ -192,14 +192,161 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
         ch.store_floats(part + static_cast<size_t>(slot * segs + j) * p.dim, make_float2(dlow.x / rest.x, dlow.y / rest.y));
 }
 
+constexpr int kRingGroup = 8;  // tokens of a group of a ring: what is kept of more does not fit beside four blocks
+
+template <typename T, bool kWords>
+struct GradRingSmem {
+    static constexpr int kStages = 2;
+    Ring hand;
+    GateTile<T, kRingGroup> ring[kWords ? kRingWarps : 0][kStages][4];  // f, dy, x, and y of the token before
+};
+
+// part: [width][dim] sums of d_bound, or null.
+template <typename T, bool kWords>
+__global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(const GateGradArgs p, const GateCut g,
+                                                                           float *part) {
+    extern __shared__ float4 smem_f4[];
+    auto &sm = *reinterpret_cast<GradRingSmem<T, kWords> *>(smem_f4);
+    constexpr int kStages = GradRingSmem<T, kWords>::kStages;
+    const SeqArgs &q = p.seq;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
+    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
+                   *const F = static_cast<const T *>(p.f), *const H = static_cast<const T *>(p.y);
+    T *const DX = static_cast<T *>(p.dx), *const DF = static_cast<T *>(p.df);
+    auto state_row = [&](const float *base, int seq) {
+        return ch.floats(base != nullptr ? base + static_cast<size_t>(seq) * p.dim : nullptr, 0.0f);
+    };
+    auto store_dinit = [&](int seq, float2 c) {
+        if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
+    };
+    if (p.dinit != nullptr)  // sequences without tokens: the gradient passes through
+        for_empty_sequences(q, slot * kRingWarps + warp, g.width * kRingWarps,
+                            [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
+    float2 dlow = both(0.0f);  // sum of da (1 - a)
+    for (int i = slot; i < g.spans; i += g.width) {
+        const Span span = gate_span(q, g, i);
+        constexpr int kTurn = kRingWarps * kRingGroup;  // tokens of a round
+        const int first = span.hi - warp * kRingGroup;
+        auto copy = [&](int hi, int stage) {
+            if constexpr (kWords) {
+                const int t = hi - kRingGroup;
+                if (hi > span.lo) {
+                    copy_tile(sm.ring[warp][stage][0], F, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile(sm.ring[warp][stage][1], DY, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile(sm.ring[warp][stage][2], X, t, span.lo, span.hi, p.dim, tile);
+                    copy_tile(sm.ring[warp][stage][3], H, t - 1, span.lo, span.hi, p.dim, tile);
+                }
+                cp_async_commit();
+            }
+        };
+        for (int k = 0; k < kStages - 1; ++k) copy(first - k * kTurn, k);
+        SeqAt seq{0, span.hi, 0};
+        int stage = 0;
+        for (int hi = first; hi > span.lo; hi -= kTurn) {
+            if constexpr (kWords) {
+                cp_async_wait<kStages - 2>();
+                __syncwarp();
+            }
+            copy(hi - (kStages - 1) * kTurn, stage == 0 ? kStages - 1 : stage - 1);  // read by all a round ago
+            // token hi - 1 - k of a tensor
+            auto load = [&](int which, const T *base, int k, int back) {
+                if constexpr (kWords) return sm.ring[warp][stage][which].at(kRingGroup - 1 - k);
+                else return ch.load(base + static_cast<size_t>(hi - 1 - k - back) * p.dim);
+            };
+            if (seq.start >= hi) seq = seq_at(q, hi - 1);
+            const bool more = hi - kRingGroup > span.lo;  // a group before
+            const int next = warp + 1 == kRingWarps ? 0 : warp + 1;
+            // (whether a group takes and gives depends on hi alone, so that offsets that descend leave nobody waiting)
+            if (hi < span.hi && hi - kRingGroup >= span.lo && seq.end > hi && seq.start < hi - kRingGroup) {
+                float2 P[kRingGroup], G[kRingGroup], u[kRingGroup], r[kRingGroup];
+#pragma unroll
+                for (int k = 0; k < kRingGroup; ++k) {
+                    const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
+                    P[k] = gate.a;
+                    u[k] = gate.u;
+                    r[k] = gate.r;
+                }
+                // P[k] becomes the product up to and with token k, G[k] is run from zero
+                float2 c = both(0.0f);
+#pragma unroll
+                for (int k = 0; k < kRingGroup; ++k) {
+                    G[k] = __fadd2_rn(load(1, DY, k, 0), c);
+                    c = __fmul2_rn(P[k], G[k]);
+                    if (k > 0) P[k] = __fmul2_rn(P[k], P[k - 1]);
+                }
+                const float2 start = sm.hand.take(warp);
+                if (!__all_sync(kFullMask, finite2(start))) {
+#pragma unroll
+                    for (int k = 0; k < kRingGroup; ++k) P[k] = above_zero(P[k]);
+                }
+                if (more) sm.hand.give(next, __ffma2_rn(P[kRingGroup - 1], start, c));
+                T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
+#pragma unroll
+                for (int k = 0; k < kRingGroup; ++k, dx -= p.dim, df -= p.dim) {
+                    const float2 Gk = k == 0 ? __fadd2_rn(G[0], start) : __ffma2_rn(P[k - 1], start, G[k]);
+                    const float2 x = load(2, X, k, 0), before = load(3, H, k, 1);
+                    const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
+                    const float2 w = __fmul2_rn(__fmul2_rn(Gk, diff), u[k]);
+                    dlow = __fadd2_rn(dlow, w);
+                    if (ch.active[0]) {
+                        ch.store(dx, __fmul2_rn(u[k], Gk));
+                        ch.store(df, __fmul2_rn(w, r[k]));
+                    }
+                }
+            } else {
+                SeqAt at = seq;
+                float2 c = hi < span.hi ? sm.hand.take(warp) : both(0.0f);
+#pragma unroll 1
+                for (int k = 0; k < kRingGroup && hi - 1 - k >= span.lo; ++k) {
+                    const int t = hi - 1 - k;
+                    if (at.start > t) at = seq_at(q, t);
+                    if (at.end == t + 1) c = state_row(p.dfinal, at.seq);
+                    const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
+                    const float2 G = __fadd2_rn(load(1, DY, k, 0), c);
+                    const bool begins = at.start == t;
+                    const float2 x = load(2, X, k, 0), before = begins ? state_row(p.init, at.seq) : load(3, H, k, 1);
+                    const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
+                    const float2 w = __fmul2_rn(__fmul2_rn(G, diff), gate.u);
+                    dlow = __fadd2_rn(dlow, w);
+                    c = __fmul2_rn(gate.a, G);
+                    if (ch.active[0]) {
+                        ch.store(DX + static_cast<size_t>(t) * p.dim, __fmul2_rn(gate.u, G));
+                        ch.store(DF + static_cast<size_t>(t) * p.dim, __fmul2_rn(w, gate.r));
+                    }
+                    if (begins) store_dinit(at.seq, c);
+                }
+                if (more) sm.hand.give(next, c);
+            }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+        cp_async_wait<0>();
+        __syncthreads();  // the rings are filled anew, the hands start anew
+    }
+    if (part != nullptr) {  // the block's sum, the warps' added in order
+        sm.hand.slot[warp][lane] = dlow;
+        __syncthreads();
+        if (warp == 0) {
+            float2 sum = sm.hand.slot[0][lane];
+            for (int w = 1; w < kRingWarps; ++w) sum = __fadd2_rn(sum, sm.hand.slot[w][lane]);
+            ch.store_floats(part + static_cast<size_t>(slot) * p.dim, make_float2(sum.x / rest.x, sum.y / rest.y));
+        }
+    }
+}
+
 template <typename T, bool kWords>
 cudaError_t launch_words(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
+    if (g.ring)
+        return launch_gate(gate_grad_ring_kernel<T, kWords>, kRingWarps, sizeof(GradRingSmem<T, kWords>), g, 1, stream, a, g,
+                           part);
     if (g.segments > 1) {
-        const cudaError_t e = launch_gate(gate_grad_kernel<T, kWords, true>, sizeof(GradSmem<T, kWords, true>), g,
+        const cudaError_t e = launch_gate(gate_grad_kernel<T, kWords, true>, 1, sizeof(GradSmem<T, kWords, true>), g,
                                           g.segments - 1, stream, a, g, part);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate(gate_grad_kernel<T, kWords, false>, sizeof(GradSmem<T, kWords, false>), g, g.segments, stream, a, g,
+    return launch_gate(gate_grad_kernel<T, kWords, false>, 1, sizeof(GradSmem<T, kWords, false>), g, g.segments, stream, a, g,
                        part);
 }
 

@@ -2,16 +2,21 @@
 // gate, the walk over sequences, and how a call is cut.
 //
 // Both are first-order recurrences per channel, h <- a h + b, forwards over the
-// tokens or backwards. A warp is a block of its own: it holds 64 channels, two per
-// lane, and walks tokens in groups of kGroup. The gates of a group do not depend on
-// h, so their exponentials overlap; only one multiply-add per token is in sequence.
-// Tiles of tokens come by asynchronous copies some groups ahead, and no warp waits
-// for another.
+// tokens or backwards. A warp holds 64 channels, two per lane, and takes groups of
+// tokens, whose tiles come by asynchronous copies some groups ahead. A group is run
+// from zero, with the product P of the a up to each token beside it: the value with
+// the true start h0 is h + P h0, so everything but one multiply-add per group can be
+// done before h0 is known.
 //
-// Where there are too few rows for the device, a row is cut into segments. A first
-// pass then walks the segments that a sequence leaves, from zero, and keeps h at the
-// segment's end with the product P of the a: a start h0 would have added P h0. The
-// second pass joins these pairs from the sequence's start up to its own segment.
+// With rows enough for the device, a block's warps take a row's groups in turn (ring):
+// each waits for its start, which the warp before leaves in shared memory, hands the
+// value at its group's end on at once and then stores its outputs. Every operand is
+// read once.
+//
+// With fewer rows, a row is cut into segments of a warp each. A first pass walks the
+// segments that a sequence leaves, from zero, and keeps h and P at the segment's end;
+// the second joins these pairs from the sequence's start up to its own segment and
+// walks with the true start.
 #pragma once
 
 #include <algorithm>
@@ -49,13 +54,15 @@ __device__ __forceinline__ Gate2 gate_of(float2 f, float2 low, float2 rest) {
 }
 
 constexpr int kGateChannels = 64;  // channels of a warp
-constexpr int kGateGroup = 16;     // tokens of a group
+constexpr int kGateGroup = 16;     // tokens that segments are whole multiples of
+constexpr int kRingWarps = 4;      // warps of a block that share a row
 
 // How a call is cut. A span is a batch row, several short ones, or the packed row.
 struct GateCut {
     int spans, length;  // length: tokens of a span; with cu it is [cu[0], cu[units])
     int width;          // spans walked at the same time
     int segments;       // of a span
+    bool ring;          // a block's warps share a span (segments is 1)
     int tiles;          // groups of channels
     float2 *P, *h, *start;  // [spans][segments][tiles][32]: the pairs, and the state that a leaving sequence started from
 };
@@ -108,7 +115,7 @@ template <typename F>
 __device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int warp, int warps, F &&f) {
     if (q.cu == nullptr && q.seqlen > 0) return;
     for (long long s0 = static_cast<long long>(warp) * 32; s0 < q.units; s0 += 32LL * warps) {
-        const int s = static_cast<int>(s0) + static_cast<int>(threadIdx.x);
+        const int s = static_cast<int>(s0) + static_cast<int>(threadIdx.x & 31);
         bool empty = false;
         if (s < q.units) {
             const int t = seq_start(q, s);
@@ -158,30 +165,32 @@ struct Lane {
 };
 
 // A group's tokens of one tensor in shared memory, and the warp's copy that fills it.
-template <typename T>
+template <typename T, int kRows>
 struct GateTile {
-    T v[kGateGroup][kGateChannels];
+    T v[kRows][kGateChannels];
     __device__ __forceinline__ float2 at(int row) const {
-        if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][2 * threadIdx.x]));
-        else return *reinterpret_cast<const float2 *>(&v[row][2 * threadIdx.x]);
+        const int lane = threadIdx.x & 31;
+        if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][2 * lane]));
+        else return *reinterpret_cast<const float2 *>(&v[row][2 * lane]);
     }
 };
-// Rows first .. first + kGateGroup - 1 of a tensor's channels; those outside [lo, hi) are left out.
-template <typename T>
-__device__ __forceinline__ void copy_tile(GateTile<T> &dst, const T *src, int first, int lo, int hi, int dim, int tile) {
+// Rows first .. first + kGroup - 1 of a tensor's channels; those outside [lo, hi) are left out.
+template <typename T, int kGroup>
+__device__ __forceinline__ void copy_tile(GateTile<T, kGroup> &dst, const T *src, int first, int lo, int hi, int dim,
+                                          int tile) {
     constexpr int kPer = 16 / static_cast<int>(sizeof(T)), kWordsRow = kGateChannels / kPer;
     constexpr int kRows = 32 / kWordsRow;  // rows per pass
-    const int col = threadIdx.x % kWordsRow * kPer, row = threadIdx.x / kWordsRow;
+    const int lane = threadIdx.x & 31, col = lane % kWordsRow * kPer, row = lane / kWordsRow;
     if (tile * kGateChannels + col >= dim) return;
     const T *p = src + static_cast<int64_t>(first + row) * dim + tile * kGateChannels + col;
-    if (first >= lo && first + kGateGroup <= hi) {
+    if (first >= lo && first + kGroup <= hi) {
 #pragma unroll
-        for (int k = 0; k < kGateGroup; k += kRows, p += static_cast<int64_t>(kRows) * dim)
+        for (int k = 0; k < kGroup; k += kRows, p += static_cast<int64_t>(kRows) * dim)
             cp_async16(&dst.v[row + k][col], p, 16);
         return;
     }
 #pragma unroll
-    for (int k = 0; k < kGateGroup; k += kRows, p += static_cast<int64_t>(kRows) * dim) {
+    for (int k = 0; k < kGroup; k += kRows, p += static_cast<int64_t>(kRows) * dim) {
         const int t = first + row + k;
         if (t >= lo && t < hi) cp_async16(&dst.v[row + k][col], p, 16);
     }
@@ -193,12 +202,38 @@ inline size_t gate_pairs(const GateCut &g) {  // elements of each of P, h and st
     return g.segments > 1 ? static_cast<size_t>(g.spans) * g.segments * g.tiles * 32 : 0;
 }
 
+// Hands a value on from the warp of group n to that of group n + 1 of a ring: slot and barrier are the receiver's. The
+// giver only arrives; it writes the slot again a round later, when the receiver is long past its wait. (Barriers by
+// number known to the compiler: a block that may use any holds all sixteen, and four blocks an SM's.)
+struct Ring {
+    float2 slot[kRingWarps][32];
+    __device__ __forceinline__ void give(int warp, float2 v) {
+        slot[warp][threadIdx.x & 31] = v;
+        if (warp == 0) asm volatile("bar.arrive 1, 64;" ::: "memory");
+        else if (warp == 1) asm volatile("bar.arrive 2, 64;" ::: "memory");
+        else if (warp == 2) asm volatile("bar.arrive 3, 64;" ::: "memory");
+        else asm volatile("bar.arrive 4, 64;" ::: "memory");
+    }
+    __device__ __forceinline__ float2 take(int warp) const {
+        if (warp == 0) asm volatile("bar.sync 1, 64;" ::: "memory");
+        else if (warp == 1) asm volatile("bar.sync 2, 64;" ::: "memory");
+        else if (warp == 2) asm volatile("bar.sync 3, 64;" ::: "memory");
+        else asm volatile("bar.sync 4, 64;" ::: "memory");
+        return slot[warp][threadIdx.x & 31];
+    }
+};
+static_assert(kRingWarps == 4, "a barrier for each");
+__device__ __forceinline__ bool finite2(float2 v) { return fabsf(v.x) <= 3.4028235e38f && fabsf(v.y) <= 3.4028235e38f; }
+
 template <typename... Params, typename... Args>
-cudaError_t launch_gate(void (*kernel)(Params...), size_t smem, const GateCut &g, int segments, cudaStream_t stream,
-                        const Args &...args) {
+cudaError_t launch_gate(void (*kernel)(Params...), int warps, size_t smem, const GateCut &g, int segments,
+                        cudaStream_t stream, const Args &...args) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // (the driver's own split of the cache left room for fewer blocks than registers and copies allow)
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
-    kernel<<<static_cast<unsigned>(g.width) * segments * g.tiles, 32, smem, stream>>>(args...);
+    kernel<<<static_cast<unsigned>(g.width) * segments * g.tiles, 32 * warps, smem, stream>>>(args...);
     return cudaGetLastError();
 }
 
