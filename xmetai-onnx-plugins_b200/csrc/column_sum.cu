@@ -20,6 +20,7 @@ __global__ void __launch_bounds__(32 * kWarps) column_sum_kernel(const float *pa
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int d = blockIdx.x * 32 + lane;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    wait_for_before();
     if (d < dim) {
         const float *const p = part + d;
         int r = warp;
@@ -43,8 +44,7 @@ __global__ void __launch_bounds__(32 * kWarps) column_sum_kernel(const float *pa
 cudaError_t launch_column_sums(const float *part0, const float *part1, int rows, int dim, float *out0, float *out1,
                                cudaStream_t stream) {
     const dim3 grid((dim + 31) / 32, part1 != nullptr ? 2 : 1);
-    column_sum_kernel<<<grid, 32 * kWarps, 0, stream>>>(part0, part1, rows, dim, out0, out1);
-    return cudaGetLastError();
+    return launch_behind(column_sum_kernel, grid, dim3(32 * kWarps), 0, stream, part0, part1, rows, dim, out0, out1);
 }
 
 }  // namespace xm

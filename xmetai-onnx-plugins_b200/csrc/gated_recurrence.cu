@@ -21,7 +21,7 @@ constexpr int kRingStages = sizeof(T) == 4 ? 3 : 2;
 
 template <typename T, bool kWords>
 struct ScanSmem {
-    GateTile<T, kGateGroup> ring[kWords ? kStages : 0][2];
+    GateTile<T, kGateGroup, kWords> ring[kStages][2];
 };
 
 // kEnds: the first pass over segments (all but a span's last).
@@ -29,6 +29,7 @@ template <typename T, bool kWords, bool kEnds>
 __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const GateCut g) {
     extern __shared__ float4 smem_f4[];
     auto &sm = *reinterpret_cast<ScanSmem<T, kWords> *>(smem_f4);
+    if (kEnds) dependents_may_launch();
     const SeqArgs &q = p.seq;
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs, slot = blockIdx.x / g.tiles / segs;
@@ -42,6 +43,12 @@ __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const Gat
     auto store_final = [&](long long row, float2 h) {
         if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
     };
+    bool waited = kEnds;
+    auto first_pass = [&] {  // is through: nothing is stored, and nothing of it read, before
+        if (!waited) wait_for_before();
+        waited = true;
+    };
+    if (!kEnds && p.final_state != nullptr && (q.cu != nullptr || q.seqlen == 0)) first_pass();
     if (!kEnds && p.final_state != nullptr)  // sequences without tokens keep their starting states
         for_empty_sequences(q, slot * segs + j, g.width * segs, [&](int s) {
             const long long row = seq_row(q, s);
@@ -61,15 +68,14 @@ __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const Gat
             begin = max(s0, seq.start);
         }
         auto copy = [&](int t, int stage) {
-            if constexpr (kWords) {
-                if (t < s1) {
-                    copy_tile(sm.ring[stage][0], X, t, 0, s1, p.dim, tile);
-                    copy_tile(sm.ring[stage][1], F, t, 0, s1, p.dim, tile);
-                }
-                cp_async_commit();
+            if (t < s1) {
+                copy_tile(sm.ring[stage][0], X, t, 0, s1, p.dim, tile);
+                copy_tile(sm.ring[stage][1], F, t, 0, s1, p.dim, tile);
             }
+            cp_async_commit();
         };
         for (int k = 0; k < kStages - 1; ++k) copy(begin + k * kGateGroup, k);
+        first_pass();
         float2 h = both(0.0f), P = both(1.0f);
         long long row = seq_row(q, seq.seq);
         // where the warp's first token does not begin a sequence, the state comes from the segments before
@@ -95,20 +101,12 @@ __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const Gat
         look_ahead();
         int stage = 0;
         for (int t = begin; t < s1; t += kGateGroup) {
-            if constexpr (kWords) {
-                cp_async_wait<kStages - 2>();
-                __syncwarp();
-            }
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
             copy(t + (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
             auto token = [&](int k, float2 &x, float2 &f) {
-                if constexpr (kWords) {
-                    x = sm.ring[stage][0].at(k);
-                    f = sm.ring[stage][1].at(k);
-                } else {
-                    const size_t at = static_cast<size_t>(t + k) * p.dim;
-                    x = ch.load(X + at);
-                    f = ch.load(F + at);
-                }
+                x = sm.ring[stage][0].at(k, shift_of<T, kWords>(X, t + k, p.dim));
+                f = sm.ring[stage][1].at(k, shift_of<T, kWords>(F, t + k, p.dim));
             };
             if (t + kGateGroup <= s1 && (kEnds || seq.end > t + kGateGroup)) {
                 float2 a[kGateGroup], b[kGateGroup];
@@ -161,12 +159,13 @@ __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const Gat
         cp_async_wait<0>();
         __syncwarp();  // (the ring is filled anew)
     }
+    first_pass();  // (also warps without tokens: what follows waits for this kernel only)
 }
 
 template <typename T, bool kWords>
 struct RingSmem {
     Ring hand;
-    GateTile<T, kGateGroup> ring[kWords ? kRingWarps : 0][kRingStages<T>][2];
+    GateTile<T, kGateGroup, kWords> ring[kRingWarps][kRingStages<T>][2];
 };
 
 template <typename T, bool kWords>
@@ -196,32 +195,22 @@ __global__ void __launch_bounds__(32 * kRingWarps, 5) gate_ring_kernel(const Gat
         constexpr int kTurn = kRingWarps * kGateGroup;  // tokens of a round
         const int first = span.lo + warp * kGateGroup;
         auto copy = [&](int t, int stage) {
-            if constexpr (kWords) {
-                if (t < span.hi) {
-                    copy_tile(sm.ring[warp][stage][0], X, t, 0, span.hi, p.dim, tile);
-                    copy_tile(sm.ring[warp][stage][1], F, t, 0, span.hi, p.dim, tile);
-                }
-                cp_async_commit();
+            if (t < span.hi) {
+                copy_tile(sm.ring[warp][stage][0], X, t, 0, span.hi, p.dim, tile);
+                copy_tile(sm.ring[warp][stage][1], F, t, 0, span.hi, p.dim, tile);
             }
+            cp_async_commit();
         };
         for (int k = 0; k < kStages - 1; ++k) copy(first + k * kTurn, k);
         SeqAt seq{0, 0, 0};
         int stage = 0;
         for (int t = first; t < span.hi; t += kTurn) {
-            if constexpr (kWords) {
-                cp_async_wait<kStages - 2>();
-                __syncwarp();
-            }
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
             copy(t + (kStages - 1) * kTurn, stage == 0 ? kStages - 1 : stage - 1);  // read by all a round ago
             auto token = [&](int k, float2 &x, float2 &f) {
-                if constexpr (kWords) {
-                    x = sm.ring[warp][stage][0].at(k);
-                    f = sm.ring[warp][stage][1].at(k);
-                } else {
-                    const size_t at = static_cast<size_t>(t + k) * p.dim;
-                    x = ch.load(X + at);
-                    f = ch.load(F + at);
-                }
+                x = sm.ring[warp][stage][0].at(k, shift_of<T, kWords>(X, t + k, p.dim));
+                f = sm.ring[warp][stage][1].at(k, shift_of<T, kWords>(F, t + k, p.dim));
             };
             if (seq.end <= t) seq = seq_at(q, t);
             const bool more = t + kGateGroup < span.hi;  // a group behind
@@ -300,12 +289,12 @@ template <typename T, bool kWords>
 cudaError_t launch_words(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
     constexpr size_t kSmem = sizeof(ScanSmem<T, kWords>);
     if (g.ring)
-        return launch_gate(gate_ring_kernel<T, kWords>, kRingWarps, sizeof(RingSmem<T, kWords>), g, 1, stream, a, g);
+        return launch_gate(gate_ring_kernel<T, kWords>, kRingWarps, sizeof(RingSmem<T, kWords>), g, 1, false, stream, a, g);
     if (g.segments > 1) {
-        const cudaError_t e = launch_gate(gate_kernel<T, kWords, true>, 1, kSmem, g, g.segments - 1, stream, a, g);
+        const cudaError_t e = launch_gate(gate_kernel<T, kWords, true>, 1, kSmem, g, g.segments - 1, false, stream, a, g);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate(gate_kernel<T, kWords, false>, 1, kSmem, g, g.segments, stream, a, g);
+    return launch_gate(gate_kernel<T, kWords, false>, 1, kSmem, g, g.segments, gate_behind(g), stream, a, g);
 }
 
 template <typename T>

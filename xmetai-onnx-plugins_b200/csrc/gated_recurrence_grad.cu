@@ -24,7 +24,7 @@ template <typename T, bool kWords, bool kEnds>
 struct GradSmem {
     static constexpr int kStages = sizeof(T) == 4 ? 3 : 5;  // groups in use and under way
     static constexpr int kTensors = kEnds ? 2 : 4;          // f, dy; x, and y of the token before
-    GateTile<T, kGateGroup> ring[kWords ? kStages : 0][kTensors];
+    GateTile<T, kGateGroup, kWords> ring[kStages][kTensors];
 };
 
 // kEnds: the first pass over segments (all but a span's first).
@@ -34,6 +34,7 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
     extern __shared__ float4 smem_f4[];
     auto &sm = *reinterpret_cast<GradSmem<T, kWords, kEnds> *>(smem_f4);
     constexpr int kStages = GradSmem<T, kWords, kEnds>::kStages;
+    dependents_may_launch();
     const SeqArgs &q = p.seq;
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs + (kEnds ? 1 : 0), slot = blockIdx.x / g.tiles / segs;
@@ -47,6 +48,11 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
     };
     auto store_dinit = [&](int seq, float2 c) {
         if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
+    };
+    bool waited = kEnds;
+    auto first_pass = [&] {  // is through: nothing of it is read before
+        if (!waited) wait_for_before();
+        waited = true;
     };
     if (!kEnds && p.dinit != nullptr)  // sequences without tokens: the gradient passes through
         for_empty_sequences(q, slot * segs + j, g.width * segs, [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
@@ -65,20 +71,19 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
             end = min(s1, seq.end);
         }
         auto copy = [&](int hi, int stage) {
-            if constexpr (kWords) {
-                const int t = hi - kGateGroup;
-                if (hi > s0) {
-                    copy_tile(sm.ring[stage][0], F, t, s0, s1, p.dim, tile);
-                    copy_tile(sm.ring[stage][1], DY, t, s0, s1, p.dim, tile);
-                    if constexpr (!kEnds) {
-                        copy_tile(sm.ring[stage][2], X, t, s0, s1, p.dim, tile);
-                        copy_tile(sm.ring[stage][3], H, t - 1, span.lo, s1, p.dim, tile);
-                    }
+            const int t = hi - kGateGroup;
+            if (hi > s0) {
+                copy_tile(sm.ring[stage][0], F, t, s0, s1, p.dim, tile);
+                copy_tile(sm.ring[stage][1], DY, t, s0, s1, p.dim, tile);
+                if constexpr (!kEnds) {
+                    copy_tile(sm.ring[stage][2], X, t, s0, s1, p.dim, tile);
+                    copy_tile(sm.ring[stage][3], H, t - 1, span.lo, s1, p.dim, tile);
                 }
-                cp_async_commit();
             }
+            cp_async_commit();
         };
         for (int k = 0; k < kStages - 1; ++k) copy(end - k * kGateGroup, k);
+        first_pass();
         float2 c = both(0.0f), P = both(1.0f);
         if (seq.end <= end) {  // (== unless the offsets descend)
             c = state_row(p.dfinal, seq.seq);
@@ -99,15 +104,12 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
         look_ahead();
         int stage = 0;
         for (int hi = end; hi > s0; hi -= kGateGroup) {
-            if constexpr (kWords) {
-                cp_async_wait<kStages - 2>();
-                __syncwarp();
-            }
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
             copy(hi - (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
             // token hi - 1 - k of a tensor
             auto load = [&](int which, const T *base, int k, int back) {
-                if constexpr (kWords) return sm.ring[stage][which].at(kGateGroup - 1 - k);
-                else return ch.load(base + static_cast<size_t>(hi - 1 - k - back) * p.dim);
+                return sm.ring[stage][which].at(kGateGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
             };
             if (hi - kGateGroup >= s0 && (kEnds || seq.start < hi - kGateGroup)) {
                 if constexpr (kEnds) {
@@ -188,6 +190,7 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
         cp_async_wait<0>();
         __syncwarp();  // (the ring is filled anew)
     }
+    first_pass();  // (also by warps without tokens: what follows waits for this kernel only)
     if (!kEnds && part != nullptr)  // da (1 - a) = da (1 - bound) sigmoid(-f)
         ch.store_floats(part + static_cast<size_t>(slot * segs + j) * p.dim, make_float2(dlow.x / rest.x, dlow.y / rest.y));
 }
@@ -198,7 +201,7 @@ template <typename T, bool kWords>
 struct GradRingSmem {
     static constexpr int kStages = 2;
     Ring hand;
-    GateTile<T, kRingGroup> ring[kWords ? kRingWarps : 0][kStages][4];  // f, dy, x, and y of the token before
+    GateTile<T, kRingGroup, kWords> ring[kRingWarps][kStages][4];  // f, dy, x, and y of the token before
 };
 
 // part: [width][dim] sums of d_bound, or null.
@@ -208,6 +211,7 @@ __global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(cons
     extern __shared__ float4 smem_f4[];
     auto &sm = *reinterpret_cast<GradRingSmem<T, kWords> *>(smem_f4);
     constexpr int kStages = GradRingSmem<T, kWords>::kStages;
+    dependents_may_launch();
     const SeqArgs &q = p.seq;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
@@ -231,30 +235,25 @@ __global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(cons
         constexpr int kTurn = kRingWarps * kRingGroup;  // tokens of a round
         const int first = span.hi - warp * kRingGroup;
         auto copy = [&](int hi, int stage) {
-            if constexpr (kWords) {
-                const int t = hi - kRingGroup;
-                if (hi > span.lo) {
-                    copy_tile(sm.ring[warp][stage][0], F, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile(sm.ring[warp][stage][1], DY, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile(sm.ring[warp][stage][2], X, t, span.lo, span.hi, p.dim, tile);
-                    copy_tile(sm.ring[warp][stage][3], H, t - 1, span.lo, span.hi, p.dim, tile);
-                }
-                cp_async_commit();
+            const int t = hi - kRingGroup;
+            if (hi > span.lo) {
+                copy_tile(sm.ring[warp][stage][0], F, t, span.lo, span.hi, p.dim, tile);
+                copy_tile(sm.ring[warp][stage][1], DY, t, span.lo, span.hi, p.dim, tile);
+                copy_tile(sm.ring[warp][stage][2], X, t, span.lo, span.hi, p.dim, tile);
+                copy_tile(sm.ring[warp][stage][3], H, t - 1, span.lo, span.hi, p.dim, tile);
             }
+            cp_async_commit();
         };
         for (int k = 0; k < kStages - 1; ++k) copy(first - k * kTurn, k);
         SeqAt seq{0, span.hi, 0};
         int stage = 0;
         for (int hi = first; hi > span.lo; hi -= kTurn) {
-            if constexpr (kWords) {
-                cp_async_wait<kStages - 2>();
-                __syncwarp();
-            }
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
             copy(hi - (kStages - 1) * kTurn, stage == 0 ? kStages - 1 : stage - 1);  // read by all a round ago
             // token hi - 1 - k of a tensor
             auto load = [&](int which, const T *base, int k, int back) {
-                if constexpr (kWords) return sm.ring[warp][stage][which].at(kRingGroup - 1 - k);
-                else return ch.load(base + static_cast<size_t>(hi - 1 - k - back) * p.dim);
+                return sm.ring[warp][stage][which].at(kRingGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
             };
             if (seq.start >= hi) seq = seq_at(q, hi - 1);
             const bool more = hi - kRingGroup > span.lo;  // a group before
@@ -339,15 +338,15 @@ __global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(cons
 template <typename T, bool kWords>
 cudaError_t launch_words(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
     if (g.ring)
-        return launch_gate(gate_grad_ring_kernel<T, kWords>, kRingWarps, sizeof(GradRingSmem<T, kWords>), g, 1, stream, a, g,
-                           part);
+        return launch_gate(gate_grad_ring_kernel<T, kWords>, kRingWarps, sizeof(GradRingSmem<T, kWords>), g, 1, false, stream, a,
+                           g, part);
     if (g.segments > 1) {
         const cudaError_t e = launch_gate(gate_grad_kernel<T, kWords, true>, 1, sizeof(GradSmem<T, kWords, true>), g,
-                                          g.segments - 1, stream, a, g, part);
+                                          g.segments - 1, false, stream, a, g, part);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate(gate_grad_kernel<T, kWords, false>, 1, sizeof(GradSmem<T, kWords, false>), g, g.segments, stream, a, g,
-                       part);
+    return launch_gate(gate_grad_kernel<T, kWords, false>, 1, sizeof(GradSmem<T, kWords, false>), g, g.segments,
+                       gate_behind(g), stream, a, g, part);
 }
 
 template <typename T>

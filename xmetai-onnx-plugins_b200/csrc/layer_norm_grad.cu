@@ -28,6 +28,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), 512 / threads_of(kGroup)) 
     constexpr int kThreads = threads_of(kGroup), kRows = kThreads / kGroup;
     using Part = RowPart<T, VE, kGroup>;
     constexpr int kElems = Part::kElems, kPairs = kElems / 2;
+    dependents_may_launch();
     __shared__ float2 part[kGroup > 32 ? 2 * (kGroup / 32) : 1];
     __shared__ float2 sums[kRows > 1 ? kThreads * kPairs : 1];
     const int g = threadIdx.x % kGroup, dim = p.dim;

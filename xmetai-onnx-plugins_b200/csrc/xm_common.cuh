@@ -336,6 +336,29 @@ __device__ __forceinline__ UnitSpan unit_span(const void *cu, bool cu64, int n, 
 
 // ---------------------------------------------------------------- shared helpers
 
+// Device: a kernel launched with launch_behind may begin once every block of the one before has called
+// dependents_may_launch (or ended), and sees that one's writes, and may overwrite what it reads, behind wait_for_before.
+__device__ __forceinline__ void dependents_may_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Host: a launch whose blocks may begin while the kernel before it on the stream ends.
+template <typename... Params, typename... Args>
+cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                          const Args &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
 // Host: 16-byte alignment of a device pointer (vectorised and TMA paths).
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -129,16 +129,15 @@ __device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int warp, 
 // Products of gates are kept above zero, so that an infinite start outlasts their underflow as it does step by step.
 __device__ __forceinline__ float2 above_zero(float2 P) { return make_float2(fmaxf(P.x, 1.4e-45f), fmaxf(P.y, 1.4e-45f)); }
 
-// A lane's two channels: neighbours, moved as one word (kWords: rows of whole 16-byte
-// words, aligned to them), else 32 apart and moved one by one.
+// A lane's two neighbouring channels. kWords: rows of whole 16-byte words, aligned to them.
 template <typename T, bool kWords>
 struct Lane {
-    int c[2];  // channels (0 where there is none)
+    int c[2];  // (0 where there is none)
     bool active[2];
     __device__ __forceinline__ Lane(int tile, int lane, int dim) {
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
-            const int at = tile * kGateChannels + (kWords ? 2 * lane + v : lane + 32 * v);
+            const int at = tile * kGateChannels + 2 * lane + v;
             active[v] = at < dim;
             c[v] = active[v] ? at : 0;
         }
@@ -150,49 +149,76 @@ struct Lane {
         if (active[0]) p[c[0]] = v.x;
         if (active[1]) p[c[1]] = v.y;
     }
-    // `row`: a token's first channel
-    __device__ __forceinline__ float2 load(const T *row) const { return make_float2(to_f32<T>(row[c[0]]), to_f32<T>(row[c[1]])); }
-    // (words: only by active lanes)
+    // `row`: a token's first channel; only by lanes whose first channel is active
     __device__ __forceinline__ void store(T *row, float2 v) const {
         if constexpr (kWords) {
             if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t *>(row + c[0]) = pack2<T>(v.x, v.y);
             else *reinterpret_cast<float2 *>(row + c[0]) = v;
         } else {
-            if (active[0]) row[c[0]] = from_f32<T>(v.x);
+            row[c[0]] = from_f32<T>(v.x);
             if (active[1]) row[c[1]] = from_f32<T>(v.y);
         }
     }
 };
 
-// A group's tokens of one tensor in shared memory, and the warp's copy that fills it.
-template <typename T, int kRows>
+// A group's tokens of one tensor in shared memory, and the warp's copy that fills it. Rows that are not whole 16-byte
+// words are copied in 4-byte ones, from the word that holds their first element: a row of a 16-bit type may then begin
+// in the middle of its first word (`shift`).
+template <typename T, int kRows, bool kWords>
 struct GateTile {
-    T v[kRows][kGateChannels];
-    __device__ __forceinline__ float2 at(int row) const {
-        const int lane = threadIdx.x & 31;
-        if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][2 * lane]));
-        else return *reinterpret_cast<const float2 *>(&v[row][2 * lane]);
+    static constexpr bool kShifts = !kWords && sizeof(T) == 2;
+    T v[kRows][kGateChannels + (kShifts ? 2 : 0)];
+    __device__ __forceinline__ float2 at(int row, int shift) const {
+        const int c = 2 * (threadIdx.x & 31);
+        if constexpr (kShifts) return make_float2(to_f32<T>(v[row][c + shift]), to_f32<T>(v[row][c + 1 + shift]));
+        else if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][c]));
+        else return *reinterpret_cast<const float2 *>(&v[row][c]);
     }
 };
-// Rows first .. first + kGroup - 1 of a tensor's channels; those outside [lo, hi) are left out.
-template <typename T, int kGroup>
-__device__ __forceinline__ void copy_tile(GateTile<T, kGroup> &dst, const T *src, int first, int lo, int hi, int dim,
+// The shift of a token's row.
+template <typename T, bool kWords>
+__device__ __forceinline__ int shift_of(const T *src, int t, int dim) {
+    if (kWords || sizeof(T) != 2) return 0;
+    return (static_cast<int>(reinterpret_cast<uintptr_t>(src) >> 1) ^ (t & dim)) & 1;  // (a tile's first channel is even)
+}
+// Rows first .. first + kRows - 1 of a tensor's channels; those outside [lo, hi) are left out.
+template <typename T, int kRows, bool kWords>
+__device__ __forceinline__ void copy_tile(GateTile<T, kRows, kWords> &dst, const T *src, int first, int lo, int hi, int dim,
                                           int tile) {
-    constexpr int kPer = 16 / static_cast<int>(sizeof(T)), kWordsRow = kGateChannels / kPer;
-    constexpr int kRows = 32 / kWordsRow;  // rows per pass
-    const int lane = threadIdx.x & 31, col = lane % kWordsRow * kPer, row = lane / kWordsRow;
-    if (tile * kGateChannels + col >= dim) return;
-    const T *p = src + static_cast<int64_t>(first + row) * dim + tile * kGateChannels + col;
-    if (first >= lo && first + kGroup <= hi) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (kWords) {
+        constexpr int kPer = 16 / static_cast<int>(sizeof(T)), kWordsRow = kGateChannels / kPer;
+        constexpr int kStep = 32 / kWordsRow;  // rows per pass
+        const int col = lane % kWordsRow * kPer, row = lane / kWordsRow;
+        if (tile * kGateChannels + col >= dim) return;
+        const T *p = src + static_cast<int64_t>(first + row) * dim + tile * kGateChannels + col;
+        if (first >= lo && first + kRows <= hi) {
 #pragma unroll
-        for (int k = 0; k < kGroup; k += kRows, p += static_cast<int64_t>(kRows) * dim)
-            cp_async16(&dst.v[row + k][col], p, 16);
-        return;
-    }
+            for (int k = 0; k < kRows; k += kStep, p += static_cast<int64_t>(kStep) * dim)
+                cp_async16(&dst.v[row + k][col], p, 16);
+            return;
+        }
 #pragma unroll
-    for (int k = 0; k < kGroup; k += kRows, p += static_cast<int64_t>(kRows) * dim) {
-        const int t = first + row + k;
-        if (t >= lo && t < hi) cp_async16(&dst.v[row + k][col], p, 16);
+        for (int k = 0; k < kRows; k += kStep, p += static_cast<int64_t>(kStep) * dim) {
+            const int t = first + row + k;
+            if (t >= lo && t < hi) cp_async16(&dst.v[row + k][col], p, 16);
+        }
+    } else {
+        const int n = min(kGateChannels, dim - tile * kGateChannels);
+        const T *row = src + static_cast<int64_t>(first) * dim + tile * kGateChannels;
+#pragma unroll 4
+        for (int k = 0; k < kRows; ++k, row += dim) {
+            if (first + k < lo || first + k >= hi) continue;
+            if constexpr (sizeof(T) == 2) {
+                const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1;
+                const T *const word = row - shift;
+                if (2 * lane < n + shift) cp_async4(&dst.v[k][2 * lane], word + 2 * lane, 4);
+                if (lane == 0 && n + shift > kGateChannels) cp_async4(&dst.v[k][kGateChannels], word + kGateChannels, 4);
+            } else {
+                if (lane < n) cp_async4(&dst.v[k][lane], row + lane, 4);
+                if (lane + 32 < n) cp_async4(&dst.v[k][lane + 32], row + lane + 32, 4);
+            }
+        }
     }
 }
 
@@ -201,6 +227,11 @@ GateCut gate_cut(const SeqArgs &q, int dim, int parts);
 inline size_t gate_pairs(const GateCut &g) {  // elements of each of P, h and start
     return g.segments > 1 ? static_cast<size_t>(g.spans) * g.segments * g.tiles * 32 : 0;
 }
+
+// Whether the second pass's blocks may begin while the first ends: worth a microsecond where segments are short (512 x
+// 4096 in 16: 9.4 us against 10.2). Long ones want their blocks spread evenly, which slots that fall free one by one do
+// not give (16384 x 4096 packed in 18: 131 us against 121).
+inline bool gate_behind(const GateCut &g) { return g.segments > 1 && g.length / g.segments <= 64; }
 
 // Hands a value on from the warp of group n to that of group n + 1 of a ring: slot and barrier are the receiver's. The
 // giver only arrives; it writes the slot again a round later, when the receiver is long past its wait. (Barriers by
@@ -225,15 +256,18 @@ struct Ring {
 static_assert(kRingWarps == 4, "a barrier for each");
 __device__ __forceinline__ bool finite2(float2 v) { return fabsf(v.x) <= 3.4028235e38f && fabsf(v.y) <= 3.4028235e38f; }
 
+// behind: the kernel waits by itself for the one before.
 template <typename... Params, typename... Args>
-cudaError_t launch_gate(void (*kernel)(Params...), int warps, size_t smem, const GateCut &g, int segments,
+cudaError_t launch_gate(void (*kernel)(Params...), int warps, size_t smem, const GateCut &g, int segments, bool behind,
                         cudaStream_t stream, const Args &...args) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     // (the driver's own split of the cache left room for fewer blocks than registers and copies allow)
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
-    kernel<<<static_cast<unsigned>(g.width) * segments * g.tiles, 32 * warps, smem, stream>>>(args...);
+    const dim3 grid(static_cast<unsigned>(g.width) * segments * g.tiles), block(32 * warps);
+    if (behind) return launch_behind(kernel, grid, block, smem, stream, args...);
+    kernel<<<grid, block, smem, stream>>>(args...);
     return cudaGetLastError();
 }
 

@@ -201,7 +201,8 @@ size_t gated_recurrence_grad_workspace(const GateGradArgs &a);
 // `workspace` must hold gated_recurrence_grad_workspace(a) bytes, 256-byte aligned.
 cudaError_t launch_gated_recurrence_grad(const GateGradArgs &a, void *workspace, cudaStream_t stream);
 
-// out0[d] = sum over r of part0[r][d], and the same of part1 into out1 (null: not there), in a fixed order.
+// out0[d] = sum over r of part0[r][d], and the same of part1 into out1 (null: not there), in a fixed order. Follows the
+// kernel that leaves the partial sums directly.
 cudaError_t launch_column_sums(const float *part0, const float *part1, int rows, int dim, float *out0, float *out1,
                                cudaStream_t stream);
 
