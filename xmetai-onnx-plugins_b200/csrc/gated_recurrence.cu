@@ -13,11 +13,11 @@ namespace xm {
 namespace {
 
 constexpr int kStages = 6;      // groups of x and f in use and under way, of a warp with a row or segment
-// And of a warp in a ring: what leaves an SM as many blocks as its registers do (16-bit types: five; 8 x 2048 x 4096
-// takes 71 us, and 83 with three stages and four blocks), or its copies (float32: two; 8 x 1024 x 4096 takes 70 us, and
-// 78 with two stages and four blocks).
-template <typename T>
-constexpr int kRingStages = sizeof(T) == 4 ? 3 : 2;
+// And of a warp in a ring. Of four: what leaves an SM as many blocks as its registers do (16-bit types: five; 8 x 2048 x
+// 4096 takes 71 us, and 83 with three stages and four blocks), or its copies (float32: two; 8 x 1024 x 4096 takes 70 us,
+// and 78 with two stages and four blocks). Of eight, an SM has two at most.
+template <typename T, int kWarps>
+constexpr int kRingStages = kWarps == 8 || sizeof(T) == 4 ? 3 : 2;
 
 template <typename T, bool kWords>
 struct ScanSmem {
@@ -162,17 +162,17 @@ __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const Gat
     first_pass();  // (also warps without tokens: what follows waits for this kernel only)
 }
 
-template <typename T, bool kWords>
+template <typename T, bool kWords, int kWarps>
 struct RingSmem {
-    Ring hand;
-    GateTile<T, kGateGroup, kWords> ring[kRingWarps][kRingStages<T>][2];
+    Ring<kWarps> hand;
+    GateTile<T, kGateGroup, kWords> ring[kWarps][kRingStages<T, kWarps>][2];
 };
 
-template <typename T, bool kWords>
-__global__ void __launch_bounds__(32 * kRingWarps, 5) gate_ring_kernel(const GateArgs p, const GateCut g) {
+template <typename T, bool kWords, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? 5 : 2) gate_ring_kernel(const GateArgs p, const GateCut g) {
     extern __shared__ float4 smem_f4[];
-    constexpr int kStages = kRingStages<T>;
-    auto &sm = *reinterpret_cast<RingSmem<T, kWords> *>(smem_f4);
+    constexpr int kStages = kRingStages<T, kWarps>;
+    auto &sm = *reinterpret_cast<RingSmem<T, kWords, kWarps> *>(smem_f4);
     const SeqArgs &q = p.seq;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
@@ -189,10 +189,10 @@ __global__ void __launch_bounds__(32 * kRingWarps, 5) gate_ring_kernel(const Gat
         if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
     };
     if (p.final_state != nullptr)  // sequences without tokens keep their starting states
-        for_empty_sequences(q, slot * kRingWarps + warp, g.width * kRingWarps, [&](int s) { store_final(s, init_of(s)); });
+        for_empty_sequences(q, slot * kWarps + warp, g.width * kWarps, [&](int s) { store_final(s, init_of(s)); });
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(q, g, i);
-        constexpr int kTurn = kRingWarps * kGateGroup;  // tokens of a round
+        constexpr int kTurn = kWarps * kGateGroup;  // tokens of a round
         const int first = span.lo + warp * kGateGroup;
         auto copy = [&](int t, int stage) {
             if (t < span.hi) {
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(32 * kRingWarps, 5) gate_ring_kernel(const Gat
             };
             if (seq.end <= t) seq = seq_at(q, t);
             const bool more = t + kGateGroup < span.hi;  // a group behind
-            const int next = warp + 1 == kRingWarps ? 0 : warp + 1;
+            const int next = warp + 1 == kWarps ? 0 : warp + 1;
             // (whether a group takes and gives depends on t alone, so that offsets that descend leave nobody waiting)
             if (t > span.lo && t + kGateGroup <= span.hi && seq.start < t && seq.end > t + kGateGroup) {
                 float2 P[kGateGroup], h[kGateGroup];
@@ -288,8 +288,10 @@ __global__ void __launch_bounds__(kTokenThreads) gate_token_kernel(const GateArg
 template <typename T, bool kWords>
 cudaError_t launch_words(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
     constexpr size_t kSmem = sizeof(ScanSmem<T, kWords>);
-    if (g.ring)
-        return launch_gate(gate_ring_kernel<T, kWords>, kRingWarps, sizeof(RingSmem<T, kWords>), g, 1, false, stream, a, g);
+    if (g.ring == 4)
+        return launch_gate(gate_ring_kernel<T, kWords, 4>, 4, sizeof(RingSmem<T, kWords, 4>), g, 1, false, stream, a, g);
+    if (g.ring == 8)
+        return launch_gate(gate_ring_kernel<T, kWords, 8>, 8, sizeof(RingSmem<T, kWords, 8>), g, 1, false, stream, a, g);
     if (g.segments > 1) {
         const cudaError_t e = launch_gate(gate_kernel<T, kWords, true>, 1, kSmem, g, g.segments - 1, false, stream, a, g);
         if (e != cudaSuccess) return e;
@@ -326,14 +328,16 @@ GateCut gate_cut(const SeqArgs &q, int dim, int parts) {
         g.spans = g.length > 0 ? static_cast<int>((static_cast<int64_t>(q.tokens) + g.length - 1) / g.length) : 1;
     }
     const int64_t warps = static_cast<int64_t>(g.spans) * g.tiles, sms = current_device_sm_count();
-    // A row per block needs four fifths of the device's blocks to be the faster (8 x 2048 x 1024, 128 blocks: 40 us
-    // against 38 in eight segments; 2 x 8192 x 4096, 128 blocks: 131 against 121; 4 x 2048 x 4096, 256 blocks: 50
-    // against 64). With fewer, one wave of eight warps an SM (16384 x 4096 packed: 119 to 121 us in 16 or 18 segments, 147
-    // in 24), of 32 tokens at least (512 x 4096: 10 us in 16, 14 in 32). Rows below 128 tokens: a warp each.
+    // A row per block needs four fifths of the device's blocks to be the faster (8 x 2048 x 1024, 128 blocks: 34 us, and
+    // 38 in eight segments; 4 x 2048 x 4096, 256 blocks: 42 and 64), of eight warps up to two blocks an SM (those 256: 50
+    // with four; 6 x 2048 x 4096, 384 blocks: 75 with eight and 58 with four). With fewer, one wave of eight warps an SM
+    // (16384 x 4096 packed: 119 to 121 us in 16 or 18 segments, 147 in 24), of 32 tokens at least (512 x 4096: 10 us in
+    // 16, 14 in 32). Rows below 128 tokens: a warp each.
     g.segments = 1;
-    g.ring = g.length >= 128 && warps * 5 >= sms * 4;
-    if (!g.ring && g.length >= 128)
-        g.segments = static_cast<int>(std::min<int64_t>(std::max<int64_t>(sms * 81 / 10 / warps, 1), (g.length + 31) / 32));
+    if (g.length >= 128) {
+        if (warps * 5 >= sms * 4) g.ring = warps > 2 * sms ? 4 : 8;
+        else g.segments = static_cast<int>(std::min<int64_t>(std::max<int64_t>(sms * 81 / 10 / warps, 1), (g.length + 31) / 32));
+    }
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(parts, (int64_t(1) << 30) / g.tiles) / g.segments);
     g.width = static_cast<int>(std::min<int64_t>(g.spans, most));
     return g;

@@ -197,20 +197,20 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
 
 constexpr int kRingGroup = 8;  // tokens of a group of a ring: what is kept of more does not fit beside four blocks
 
-template <typename T, bool kWords>
+template <typename T, bool kWords, int kWarps>
 struct GradRingSmem {
-    static constexpr int kStages = 2;
-    Ring hand;
-    GateTile<T, kRingGroup, kWords> ring[kRingWarps][kStages][4];  // f, dy, x, and y of the token before
+    static constexpr int kStages = kWarps == 8 && sizeof(T) == 2 ? 3 : 2;
+    Ring<kWarps> hand;
+    GateTile<T, kRingGroup, kWords> ring[kWarps][kStages][4];  // f, dy, x, and y of the token before
 };
 
 // part: [width][dim] sums of d_bound, or null.
-template <typename T, bool kWords>
-__global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(const GateGradArgs p, const GateCut g,
+template <typename T, bool kWords, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kernel(const GateGradArgs p, const GateCut g,
                                                                            float *part) {
     extern __shared__ float4 smem_f4[];
-    auto &sm = *reinterpret_cast<GradRingSmem<T, kWords> *>(smem_f4);
-    constexpr int kStages = GradRingSmem<T, kWords>::kStages;
+    auto &sm = *reinterpret_cast<GradRingSmem<T, kWords, kWarps> *>(smem_f4);
+    constexpr int kStages = GradRingSmem<T, kWords, kWarps>::kStages;
     dependents_may_launch();
     const SeqArgs &q = p.seq;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -227,12 +227,12 @@ __global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(cons
         if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
     };
     if (p.dinit != nullptr)  // sequences without tokens: the gradient passes through
-        for_empty_sequences(q, slot * kRingWarps + warp, g.width * kRingWarps,
+        for_empty_sequences(q, slot * kWarps + warp, g.width * kWarps,
                             [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
     float2 dlow = both(0.0f);  // sum of da (1 - a)
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(q, g, i);
-        constexpr int kTurn = kRingWarps * kRingGroup;  // tokens of a round
+        constexpr int kTurn = kWarps * kRingGroup;  // tokens of a round
         const int first = span.hi - warp * kRingGroup;
         auto copy = [&](int hi, int stage) {
             const int t = hi - kRingGroup;
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(cons
             };
             if (seq.start >= hi) seq = seq_at(q, hi - 1);
             const bool more = hi - kRingGroup > span.lo;  // a group before
-            const int next = warp + 1 == kRingWarps ? 0 : warp + 1;
+            const int next = warp + 1 == kWarps ? 0 : warp + 1;
             // (whether a group takes and gives depends on hi alone, so that offsets that descend leave nobody waiting)
             if (hi < span.hi && hi - kRingGroup >= span.lo && seq.end > hi && seq.start < hi - kRingGroup) {
                 float2 P[kRingGroup], G[kRingGroup], u[kRingGroup], r[kRingGroup];
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(cons
         __syncthreads();
         if (warp == 0) {
             float2 sum = sm.hand.slot[0][lane];
-            for (int w = 1; w < kRingWarps; ++w) sum = __fadd2_rn(sum, sm.hand.slot[w][lane]);
+            for (int w = 1; w < kWarps; ++w) sum = __fadd2_rn(sum, sm.hand.slot[w][lane]);
             ch.store_floats(part + static_cast<size_t>(slot) * p.dim, make_float2(sum.x / rest.x, sum.y / rest.y));
         }
     }
@@ -337,9 +337,12 @@ __global__ void __launch_bounds__(32 * kRingWarps, 4) gate_grad_ring_kernel(cons
 
 template <typename T, bool kWords>
 cudaError_t launch_words(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
-    if (g.ring)
-        return launch_gate(gate_grad_ring_kernel<T, kWords>, kRingWarps, sizeof(GradRingSmem<T, kWords>), g, 1, false, stream, a,
-                           g, part);
+    if (g.ring == 4)
+        return launch_gate(gate_grad_ring_kernel<T, kWords, 4>, 4, sizeof(GradRingSmem<T, kWords, 4>), g, 1, false, stream,
+                           a, g, part);
+    if (g.ring == 8)
+        return launch_gate(gate_grad_ring_kernel<T, kWords, 8>, 8, sizeof(GradRingSmem<T, kWords, 8>), g, 1, false, stream,
+                           a, g, part);
     if (g.segments > 1) {
         const cudaError_t e = launch_gate(gate_grad_kernel<T, kWords, true>, 1, sizeof(GradSmem<T, kWords, true>), g,
                                           g.segments - 1, false, stream, a, g, part);

@@ -55,14 +55,13 @@ __device__ __forceinline__ Gate2 gate_of(float2 f, float2 low, float2 rest) {
 
 constexpr int kGateChannels = 64;  // channels of a warp
 constexpr int kGateGroup = 16;     // tokens that segments are whole multiples of
-constexpr int kRingWarps = 4;      // warps of a block that share a row
 
 // How a call is cut. A span is a batch row, several short ones, or the packed row.
 struct GateCut {
     int spans, length;  // length: tokens of a span; with cu it is [cu[0], cu[units])
     int width;          // spans walked at the same time
     int segments;       // of a span
-    bool ring;          // a block's warps share a span (segments is 1)
+    int ring;           // warps of the block that shares a span (segments is 1); 0: a segment to each warp
     int tiles;          // groups of channels
     float2 *P, *h, *start;  // [spans][segments][tiles][32]: the pairs, and the state that a leaving sequence started from
 };
@@ -236,24 +235,32 @@ inline bool gate_behind(const GateCut &g) { return g.segments > 1 && g.length / 
 // Hands a value on from the warp of group n to that of group n + 1 of a ring: slot and barrier are the receiver's. The
 // giver only arrives; it writes the slot again a round later, when the receiver is long past its wait. (Barriers by
 // number known to the compiler: a block that may use any holds all sixteen, and four blocks an SM's.)
+template <int kWarps>
 struct Ring {
-    float2 slot[kRingWarps][32];
+    float2 slot[kWarps][32];
+    template <int kAt>
+    __device__ __forceinline__ static void arrive(int warp) {
+        if constexpr (kAt + 1 < kWarps) {
+            if (warp != kAt) return arrive<kAt + 1>(warp);
+        }
+        asm volatile("bar.arrive %0, 64;" ::"n"(kAt + 1) : "memory");
+    }
+    template <int kAt>
+    __device__ __forceinline__ static void sync(int warp) {
+        if constexpr (kAt + 1 < kWarps) {
+            if (warp != kAt) return sync<kAt + 1>(warp);
+        }
+        asm volatile("bar.sync %0, 64;" ::"n"(kAt + 1) : "memory");
+    }
     __device__ __forceinline__ void give(int warp, float2 v) {
         slot[warp][threadIdx.x & 31] = v;
-        if (warp == 0) asm volatile("bar.arrive 1, 64;" ::: "memory");
-        else if (warp == 1) asm volatile("bar.arrive 2, 64;" ::: "memory");
-        else if (warp == 2) asm volatile("bar.arrive 3, 64;" ::: "memory");
-        else asm volatile("bar.arrive 4, 64;" ::: "memory");
+        arrive<0>(warp);
     }
     __device__ __forceinline__ float2 take(int warp) const {
-        if (warp == 0) asm volatile("bar.sync 1, 64;" ::: "memory");
-        else if (warp == 1) asm volatile("bar.sync 2, 64;" ::: "memory");
-        else if (warp == 2) asm volatile("bar.sync 3, 64;" ::: "memory");
-        else asm volatile("bar.sync 4, 64;" ::: "memory");
+        sync<0>(warp);
         return slot[warp][threadIdx.x & 31];
     }
 };
-static_assert(kRingWarps == 4, "a barrier for each");
 __device__ __forceinline__ bool finite2(float2 v) { return fabsf(v.x) <= 3.4028235e38f && fabsf(v.y) <= 3.4028235e38f; }
 
 // behind: the kernel waits by itself for the one before.
