@@ -7,6 +7,7 @@
 #include "xm_common.cuh"
 #include "xm_gate.cuh"
 #include "xm_kernels.h"
+#include "xm_rows.cuh"
 #include "xm_sequences.cuh"
 
 namespace xm {
@@ -266,22 +267,70 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? 5 : 2) gate_ring_ke
     }
 }
 
+// One token per sequence: bound by memory, 8 bytes of state and three elements per channel. A thread takes kVec
+// neighbouring channels (a word of the I/O type, or one where rows are not whole words) of kRows sequences, whose loads
+// are issued together.
 constexpr int kTokenThreads = 128;
 
-template <typename T>
+template <int kVec>
+__device__ __forceinline__ void load_state(const float *p, float (&v)[kVec]) {
+    if constexpr (kVec == 1) {
+        v[0] = *p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; i += 4) {
+            const float4 w = *reinterpret_cast<const float4 *>(p + i);
+            v[i] = w.x; v[i + 1] = w.y; v[i + 2] = w.z; v[i + 3] = w.w;
+        }
+    }
+}
+
+template <typename T, int kVec, int kRows>
 __global__ void __launch_bounds__(kTokenThreads) gate_token_kernel(const GateArgs p) {
-    const int d = blockIdx.x * kTokenThreads + threadIdx.x;
+    using Word = Chunk<T, kVec>;
+    const int d = (blockIdx.x * kTokenThreads + threadIdx.x) * kVec;
     if (d >= p.dim) return;
-    const float low = p.bound != nullptr ? p.bound[d] : 0.0f;
-    for (unsigned i = blockIdx.y; i < static_cast<unsigned>(p.seq.units); i += gridDim.y) {
-        const long long row = seq_row(p.seq, i);
-        if (row < 0) continue;
-        const size_t at = static_cast<size_t>(i) * p.dim + d;
-        const Gate2 g = gate_of(both(to_f32<T>(static_cast<const T *>(p.f)[at])), both(low), both(1.0f - low));
-        const float x = to_f32<T>(static_cast<const T *>(p.x)[at]);
-        const float h = fmaf(g.a.x, p.init[row * p.dim + d], g.u.x * x);
-        p.final_state[row * p.dim + d] = h;
-        static_cast<T *>(p.out)[at] = from_f32<T>(h);
+    // (sequences are counted in 31 bits, the steps past the last one need the 32nd)
+    const unsigned units = p.seq.units;
+    for (unsigned i0 = blockIdx.y * kRows; i0 < units; i0 += gridDim.y * kRows) {
+        long long row[kRows];
+        Word x[kRows], f[kRows];
+        float h[kRows][kVec];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const unsigned i = min(i0 + r, units - 1);
+            const size_t at = static_cast<size_t>(i) * p.dim + d;
+            row[r] = i0 + r < units ? seq_row(p.seq, i) : -1;
+            x[r] = *reinterpret_cast<const Word *>(static_cast<const T *>(p.x) + at);
+            f[r] = *reinterpret_cast<const Word *>(static_cast<const T *>(p.f) + at);
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+            if (row[r] >= 0) load_state<kVec>(p.init + row[r] * p.dim + d, h[r]);
+        float low[kVec];
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) low[k] = 0.0f;
+        if (p.bound != nullptr) load_state<kVec>(p.bound + d, low);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            if (row[r] < 0) continue;
+            float xs[kVec], fs[kVec];
+            chunk_floats<T, kVec>(x[r], xs);
+            chunk_floats<T, kVec>(f[r], fs);
+#pragma unroll
+            for (int k = 0; k < kVec; k += 2) {
+                constexpr int kNext = kVec > 1 ? 1 : 0;
+                const float2 b = make_float2(low[k], low[k + kNext]);
+                const Gate2 g = gate_of(make_float2(fs[k], fs[k + kNext]), b, make_float2(1.0f - b.x, 1.0f - b.y));
+                const float2 v = __ffma2_rn(g.a, make_float2(h[r][k], h[r][k + kNext]),
+                                            __fmul2_rn(g.u, make_float2(xs[k], xs[k + kNext])));
+                h[r][k] = v.x;
+                if (kVec > 1) h[r][k + kNext] = v.y;
+            }
+            store_row_floats<kVec>(p.final_state + row[r] * p.dim + d, h[r]);
+            *reinterpret_cast<Word *>(static_cast<T *>(p.out) + static_cast<size_t>(i0 + r) * p.dim + d) =
+                to_chunk<T, kVec>(h[r]);
+        }
     }
 }
 
@@ -306,11 +355,24 @@ cudaError_t launch_type(const GateArgs &a, const GateCut &g, cudaStream_t stream
     return launch_words<T, false>(a, g, stream);
 }
 
+// Several sequences per thread where that leaves each SM eight blocks; below, one.
+template <typename T, int kVec, int kRows>
+cudaError_t launch_token_rows(const GateArgs &a, cudaStream_t stream) {
+    const int64_t blocks = (a.dim + static_cast<int64_t>(kTokenThreads) * kVec - 1) / (kTokenThreads * kVec);
+    const int64_t rows = (static_cast<int64_t>(a.seq.units) + kRows - 1) / kRows;
+    if (kRows > 1 && blocks * rows < 8LL * current_device_sm_count()) return launch_token_rows<T, kVec, 1>(a, stream);
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(rows, 65535)));
+    gate_token_kernel<T, kVec, kRows><<<grid, kTokenThreads, 0, stream>>>(a);
+    return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t launch_token_type(const GateArgs &a, cudaStream_t stream) {
-    const dim3 grid((a.dim + kTokenThreads - 1) / kTokenThreads, std::min(a.seq.units, 65535));
-    gate_token_kernel<T><<<grid, kTokenThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+    constexpr int kWord = 16 / static_cast<int>(sizeof(T));
+    if (a.dim % kWord == 0 && aligned16(a.x) && aligned16(a.f) && aligned16(a.out) && aligned16(a.init) &&
+        aligned16(a.final_state) && aligned16(a.bound))
+        return launch_token_rows<T, kWord, 2>(a, stream);
+    return launch_token_rows<T, 1, 4>(a, stream);
 }
 
 }  // namespace
