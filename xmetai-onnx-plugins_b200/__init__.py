@@ -466,12 +466,6 @@ def _invalid(message):
     raise XmError(XM_ERR_INVALID_ARGUMENT, message)
 
 
-def _float32():
-    import torch
-
-    return torch.float32
-
-
 _pycall = None
 
 
@@ -538,7 +532,7 @@ def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
     index = x.get_device() if isinstance(x, torch.Tensor) else -1
     if index < 0:
         _invalid(f"{op.names[0]} must be a CUDA tensor")
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return _serve(op, attrs, tensors, out, state, state_shape, with_state, stream)
     handle = torch._C._cuda_getCurrentRawStream(index)
@@ -559,21 +553,16 @@ def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
             state = tensors[inplace] if state_shape is None else x.new_empty(
                 state_shape, dtype=torch.float32 if op.kinds[op.state] == "f" else x.dtype)
         outs = (out, state)
-    _launch(op, attrs, tensors, outs, index, inplace, handle)
+    _launch(op, ctypes.addressof(attrs), tensors, outs, index, inplace, handle)
     return outs if with_state else out
 
 
 def _launch(op, attrs, tensors, outs, index, inplace, handle):
-    """Call xm_<op>_fwd on the current device `index` and the current stream `handle`."""
-    import torch
-
+    """Call xm_<op>_fwd on the current device `index` and the current stream `handle`; attrs: the struct's address."""
     x = tensors[0]
-    alloc = None
-    if op.workspace:
-        alloc = lambda n: x.new_empty(n, dtype=torch.uint8)  # noqa: E731
     blank = op.blank.get(x.dtype)
-    status, which = op.call(op.fwd, op.size, ctypes.addressof(attrs), tensors,
-                            op.blank[None] if blank is None else blank, outs, index, inplace, alloc, handle)
+    status, which = op.call(op.fwd, op.size, attrs, tensors, op.blank[None] if blank is None else blank, outs, index,
+                            inplace, _scratch(x) if op.workspace else None, handle)
     if status:
         if status == -1:
             _invalid(f"{op.names[which]} must be a tensor on cuda:{index}")
@@ -584,9 +573,15 @@ def _launch(op, attrs, tensors, outs, index, inplace, handle):
         _check(status)
 
 
-def _serve_many(op, attrs, tensors, outputs, stream, inplace=-1):
-    """_serve for operators with other outputs than a tensor and a state: `outputs` holds what the caller gave, or
-    (shape, dtype) of a tensor to allocate. Returns them."""
+def _scratch(x):
+    import torch
+
+    return lambda n: x.new_empty(n, dtype=torch.uint8)
+
+
+def _serve_many(op, attrs, tensors, make, stream, inplace=-1):
+    """_serve for operators with other outputs than a tensor and a state: make() gives their tuple, on the device and the
+    stream that the call runs on. attrs: the struct's address. Returns the outputs."""
     import torch
 
     if op.call is None:
@@ -595,19 +590,34 @@ def _serve_many(op, attrs, tensors, outputs, stream, inplace=-1):
     index = x.get_device() if isinstance(x, torch.Tensor) else -1
     if index < 0:
         _invalid(f"{op.names[0]} must be a CUDA tensor")
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            return _serve_many(op, attrs, tensors, outputs, stream, inplace)
+            return _serve_many(op, attrs, tensors, make, stream, inplace)
     handle = torch._C._cuda_getCurrentRawStream(index)
     if stream is not None:
         if stream.device_index != index:
             _invalid("stream belongs to another device")
         if stream.cuda_stream != handle:
             with torch.cuda.stream(stream):
-                return _serve_many(op, attrs, tensors, outputs, None, inplace)
-    outs = tuple([x.new_empty(o[0], dtype=o[1]) if type(o) is tuple else o for o in outputs])
+                return _serve_many(op, attrs, tensors, make, None, inplace)
+    outs = make()
     _launch(op, attrs, tensors, outs, index, inplace, handle)
     return outs
+
+
+_attrs = {}
+
+
+def _address(kind, *values):
+    """Address of an attribute struct with these values, which stays as it is."""
+    key = (kind, *values)
+    a = _attrs.get(key)
+    if a is None:
+        if len(_attrs) > 1000:
+            _attrs.clear()
+        a = kind(*values)
+        a = _attrs[key] = (a, ctypes.addressof(a))
+    return a
 
 
 _CONV = _ServeOp("causal_conv1d", ("x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices",
@@ -753,23 +763,31 @@ def GatedRecurrenceGradFn(dy, x, f, y, lower_bound=None, initial_state=None, cu_
     else None. A sequence that started from zeros has a row of zeros in initial_state. out: a tuple of outputs in the
     same order, None where one is to be allocated.
     """
+    import torch
+
     if getattr(dy, "ndim", 0) != 3:
         _invalid("dy must have rank 3")
     units = cu_seqlens.numel() - 1 if _given(cu_seqlens) else dy.shape[0]
     lb = _given(lower_bound) if output_lower_bound_grad is None else bool(output_lower_bound_grad)
     st = bool(output_initial_state_grad) if output_initial_state_grad is not None else (
         _given(initial_state) or (initial_state is not None and units == 0))
-    f32 = _float32()
-    want = [(tuple(dy.shape), dy.dtype)] * 2 + [((dy.shape[2],), f32) if lb else None,
-                                                ((units, dy.shape[2]), f32) if st else None]
-    if out is not None:
-        if len(out) != 4:
-            _invalid("out must hold 4 outputs (None: allocate)")
-        want = [w if o is None or w is None else o for o, w in zip(out, want)]
-    got = iter(_serve_many(_GATE_GRAD, GatedRecurrenceGradAttrs(int(lb), int(st)),
-                           (dy, x, f, y, lower_bound, initial_state, cu_seqlens, d_final_state),
-                           [w for w in want if w is not None], stream))
-    return tuple([None if w is None else next(got) for w in want])
+    if out is None:
+        out = (None, None, None, None)
+    elif len(out) != 4:
+        _invalid("out must hold 4 outputs (None: allocate)")
+
+    def make():
+        outs = [torch.empty_like(dy, memory_format=torch.contiguous_format) if o is None else o for o in out[:2]]
+        if lb:
+            outs.append(dy.new_empty(dy.shape[2], dtype=torch.float32) if out[2] is None else out[2])
+        if st:
+            outs.append(dy.new_empty((units, dy.shape[2]), dtype=torch.float32) if out[3] is None else out[3])
+        return tuple(outs)
+
+    attrs = _address(GatedRecurrenceGradAttrs, int(lb), int(st))
+    got = _serve_many(_GATE_GRAD, attrs[1], (dy, x, f, y, lower_bound, initial_state, cu_seqlens, d_final_state), make,
+                      stream)
+    return got[0], got[1], got[2] if lb else None, got[-1] if st else None
 
 
 def GatedRecurrenceUpdateFn(x, f, lower_bound=None, state=None, state_indices=None, *, stream=None, out=None,
@@ -793,21 +811,27 @@ def LayerNormFn(x, weight=None, bias=None, residual=None, *, eps: float = 1e-5, 
     tuple: (y, s) with a residual, and with output_stats=1 the float32 [..., 2] of every row's mean and rstd at its
     end, which LayerNormGradFn takes. residual_out may be the residual itself: the residual stream in place.
     """
-    if not hasattr(x, "shape") or len(x.shape) == 0:
+    import torch
+
+    if getattr(x, "ndim", 0) == 0:
         _invalid("x must have at least one axis")
     if residual is not None and not _given(residual) and not _given(x):  # no rows: the sum is as empty as its terms
         y = LayerNormFn(x, weight, bias, eps=eps, rms=rms, output_stats=output_stats, stream=stream, out=out, stats=stats)
         y = y if output_stats else (y,)
         return y[:1] + (x.new_empty(x.shape) if residual_out is None else residual_out,) + y[1:]
     many = _given(residual)
-    shape = tuple(x.shape)
-    outs = [(shape, x.dtype) if out is None else out]
-    if many:
-        outs.append((shape, x.dtype) if residual_out is None else residual_out)
-    if output_stats:
-        outs.append((shape[:-1] + (2,), _float32()) if stats is None else stats)
-    got = _serve_many(_NORM, LayerNormAttrs(float(eps), int(rms), int(output_stats)), (x, weight, bias, residual), outs,
-                      stream, 3 if many and residual_out is residual else -1)
+
+    def make():
+        outs = [torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else out]
+        if many:
+            outs.append(torch.empty_like(x, memory_format=torch.contiguous_format) if residual_out is None else residual_out)
+        if output_stats:
+            outs.append(x.new_empty((*x.shape[:-1], 2), dtype=torch.float32) if stats is None else stats)
+        return tuple(outs)
+
+    attrs = _address(LayerNormAttrs, float(eps), int(rms), int(output_stats))
+    got = _serve_many(_NORM, attrs[1], (x, weight, bias, residual), make, stream,
+                      3 if many and residual_out is residual else -1)
     return got if len(got) > 1 else got[0]
 
 
@@ -822,17 +846,27 @@ def LayerNormGradFn(dy, x, weight=None, stats=None, d_residual=None, *, rms: int
     """
     if stats is None:
         _invalid("LayerNormGradFn needs the forward call's stats")
-    if not hasattr(dy, "shape") or len(dy.shape) == 0:
+    import torch
+
+    if getattr(dy, "ndim", 0) == 0:
         _invalid("dy must have at least one axis")
-    row = ((dy.shape[-1],), _float32())
-    want = [(tuple(dy.shape), dy.dtype), row if _given(weight) else None, row if output_bias_grad else None]
-    if out is not None:
-        if len(out) != 3:
-            _invalid("out must hold 3 outputs (None: allocate)")
-        want = [w if o is None or w is None else o for o, w in zip(out, want)]
-    got = iter(_serve_many(_NORM_GRAD, LayerNormGradAttrs(int(rms), int(output_bias_grad)),
-                           (dy, x, weight, stats, d_residual), [w for w in want if w is not None], stream))
-    return tuple([None if w is None else next(got) for w in want])
+    many = _given(weight)
+    if out is None:
+        out = (None, None, None)
+    elif len(out) != 3:
+        _invalid("out must hold 3 outputs (None: allocate)")
+
+    def make():
+        outs = [torch.empty_like(dy, memory_format=torch.contiguous_format) if out[0] is None else out[0]]
+        if many:
+            outs.append(dy.new_empty(dy.shape[-1], dtype=torch.float32) if out[1] is None else out[1])
+        if output_bias_grad:
+            outs.append(dy.new_empty(dy.shape[-1], dtype=torch.float32) if out[2] is None else out[2])
+        return tuple(outs)
+
+    attrs = _address(LayerNormGradAttrs, int(rms), int(output_bias_grad))
+    got = _serve_many(_NORM_GRAD, attrs[1], (dy, x, weight, stats, d_residual), make, stream)
+    return got[0], got[1] if many else None, got[-1] if output_bias_grad else None
 
 
 def device_wait_failures() -> int:

@@ -338,14 +338,14 @@ template <typename T, bool kWords>
 cudaError_t launch_words(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
     constexpr size_t kSmem = sizeof(ScanSmem<T, kWords>);
     if (g.ring == 4)
-        return launch_gate(gate_ring_kernel<T, kWords, 4>, 4, sizeof(RingSmem<T, kWords, 4>), g, 1, false, stream, a, g);
+        return launch_gate<gate_ring_kernel<T, kWords, 4>>(4, sizeof(RingSmem<T, kWords, 4>), g, 1, false, stream, a, g);
     if (g.ring == 8)
-        return launch_gate(gate_ring_kernel<T, kWords, 8>, 8, sizeof(RingSmem<T, kWords, 8>), g, 1, false, stream, a, g);
+        return launch_gate<gate_ring_kernel<T, kWords, 8>>(8, sizeof(RingSmem<T, kWords, 8>), g, 1, false, stream, a, g);
     if (g.segments > 1) {
-        const cudaError_t e = launch_gate(gate_kernel<T, kWords, true>, 1, kSmem, g, g.segments - 1, false, stream, a, g);
+        const cudaError_t e = launch_gate<gate_kernel<T, kWords, true>>(1, kSmem, g, g.segments - 1, false, stream, a, g);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate(gate_kernel<T, kWords, false>, 1, kSmem, g, g.segments, gate_behind(g), stream, a, g);
+    return launch_gate<gate_kernel<T, kWords, false>>(1, kSmem, g, g.segments, gate_behind(g), stream, a, g);
 }
 
 template <typename T>

@@ -338,17 +338,17 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
 template <typename T, bool kWords>
 cudaError_t launch_words(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
     if (g.ring == 4)
-        return launch_gate(gate_grad_ring_kernel<T, kWords, 4>, 4, sizeof(GradRingSmem<T, kWords, 4>), g, 1, false, stream,
+        return launch_gate<gate_grad_ring_kernel<T, kWords, 4>>(4, sizeof(GradRingSmem<T, kWords, 4>), g, 1, false, stream,
                            a, g, part);
     if (g.ring == 8)
-        return launch_gate(gate_grad_ring_kernel<T, kWords, 8>, 8, sizeof(GradRingSmem<T, kWords, 8>), g, 1, false, stream,
+        return launch_gate<gate_grad_ring_kernel<T, kWords, 8>>(8, sizeof(GradRingSmem<T, kWords, 8>), g, 1, false, stream,
                            a, g, part);
     if (g.segments > 1) {
-        const cudaError_t e = launch_gate(gate_grad_kernel<T, kWords, true>, 1, sizeof(GradSmem<T, kWords, true>), g,
+        const cudaError_t e = launch_gate<gate_grad_kernel<T, kWords, true>>(1, sizeof(GradSmem<T, kWords, true>), g,
                                           g.segments - 1, false, stream, a, g, part);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate(gate_grad_kernel<T, kWords, false>, 1, sizeof(GradSmem<T, kWords, false>), g, g.segments,
+    return launch_gate<gate_grad_kernel<T, kWords, false>>(1, sizeof(GradSmem<T, kWords, false>), g, g.segments,
                        gate_behind(g), stream, a, g, part);
 }
 
