@@ -394,10 +394,11 @@ GateCut gate_cut(const SeqArgs &q, int dim, int parts) {
     // 38 in eight segments; 4 x 2048 x 4096, 256 blocks: 42 and 64), of eight warps up to two blocks an SM (those 256: 50
     // with four; 6 x 2048 x 4096, 384 blocks: 75 with eight and 58 with four). With fewer, one wave of eight warps an SM
     // (16384 x 4096 packed: 119 to 121 us in 16 or 18 segments, 147 in 24), of 32 tokens at least (512 x 4096: 10 us in
-    // 16, 14 in 32). Rows below 128 tokens: a warp each.
+    // 16, 14 in 32). Rows of fewer
+    // than 256 tokens, or 128 where there are few: a warp each (8 x 128 x 4096: 8.9 us, 10.9 in rings).
     g.segments = 1;
     if (g.length >= 128) {
-        if (warps * 5 >= sms * 4) g.ring = warps > 2 * sms ? 4 : 8;
+        if (warps * 5 >= sms * 4) g.ring = g.length < 256 ? 0 : warps > 2 * sms ? 4 : 8;
         else g.segments = static_cast<int>(std::min<int64_t>(std::max<int64_t>(sms * 81 / 10 / warps, 1), (g.length + 31) / 32));
     }
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(parts, (int64_t(1) << 30) / g.tiles) / g.segments);

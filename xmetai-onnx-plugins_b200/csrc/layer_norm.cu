@@ -7,7 +7,8 @@
 // Bound by memory: x and the residual are read once and y and s written once. A row
 // stays in the registers of its group of threads between the sum, the squares and the
 // output, so it is not read again; rows that do not fit (above 16384 elements of
-// the 16-bit types, 8192 of float32 or unaligned) are, from the caches.
+// the 16-bit types, 8192 of float32) are, from the caches. Rows that are not whole
+// words are staged in shared memory.
 #include <algorithm>
 
 #include "xm_common.cuh"
@@ -20,7 +21,7 @@ namespace {
 constexpr int threads_of(int group) { return group < 128 ? 128 : group; }
 
 template <typename T, int VE, int kGroup>
-__global__ void __launch_bounds__(threads_of(kGroup)) norm_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup)) norm_kernel(const NormArgs p) {
     constexpr int kThreads = threads_of(kGroup), kRows = kThreads / kGroup;
     using Part = RowPart<T, VE, kGroup>;
     constexpr int kPairs = Part::kElems / 2;
@@ -93,6 +94,79 @@ __global__ void __launch_bounds__(threads_of(kGroup)) norm_kernel(const NormArgs
     }
 }
 
+// Rows that are not whole words, above 1024 elements: staged some rows ahead, and read from shared memory for every
+// pass. (In registers, one element a load, 16384 rows of 4097 took 247 us.)
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 2048 / kThreads) norm_staged_kernel(const NormArgs p, int stages) {
+    extern __shared__ float4 smem_f4[];
+    __shared__ float2 part[2 * (kThreads / 32)];
+    const int dim = p.dim;
+    const size_t pitch = staged_pitch<T>(dim);
+    const T *const X = static_cast<const T *>(p.x), *const R = static_cast<const T *>(p.residual);
+    T *const ring = reinterpret_cast<T *>(smem_f4);  // [stages][x, residual where there is one][pitch]
+    const size_t tensors = R != nullptr ? 2 : 1;
+    const float inv = 1.0f / static_cast<float>(dim);
+    auto copy = [&](long long row, int stage) {
+        if (row < p.rows) {
+            stage_row<kThreads>(ring + tensors * stage * pitch, X, static_cast<unsigned>(row), dim);
+            if (R != nullptr) stage_row<kThreads>(ring + (2 * stage + 1) * pitch, R, static_cast<unsigned>(row), dim);
+        }
+        cp_async_commit();
+    };
+    for (int k = 0; k < stages - 1; ++k) copy(blockIdx.x + static_cast<long long>(k) * gridDim.x, k);
+    int turn = 0, stage = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        // (all but the last stages - 2 copies are here; two or three stages)
+        if (stages == 2) cp_async_wait<0>();
+        else cp_async_wait<1>();
+        __syncthreads();
+        copy(row + static_cast<long long>(stages - 1) * gridDim.x, stage == 0 ? stages - 1 : stage - 1);
+        T *const s = ring + tensors * stage * pitch + staged_shift(X, static_cast<unsigned>(row), dim);
+        const T *const r = ring + (2 * stage + 1) * pitch + (R != nullptr ? staged_shift(R, static_cast<unsigned>(row), dim) : 0);
+        const size_t at = static_cast<size_t>(row) * dim;
+        // (an element is read again only by the thread that wrote it)
+        float sum = 0.0f;
+        if (R != nullptr) {
+            T *const kept = static_cast<T *>(p.sum) + at;
+#pragma unroll 4
+            for (int d = threadIdx.x; d < dim; d += kThreads) {
+                const T v = from_f32<T>(to_f32<T>(s[d]) + to_f32<T>(r[d]));
+                kept[d] = v;
+                s[d] = v;
+                sum += to_f32<T>(v);
+            }
+        } else if (!p.rms) {
+#pragma unroll 4
+            for (int d = threadIdx.x; d < dim; d += kThreads) sum += to_f32<T>(s[d]);
+        }
+        float mean = 0.0f;
+        if (!p.rms) {
+            mean = group_sum<kThreads>(make_float2(sum, 0.0f), part, turn).x * inv;
+            turn ^= 1;
+        }
+        float sq = 0.0f;
+#pragma unroll 4
+        for (int d = threadIdx.x; d < dim; d += kThreads) {
+            const float v = to_f32<T>(s[d]) - mean;
+            sq = fmaf(v, v, sq);
+        }
+        const float rstd = 1.0f / sqrtf(group_sum<kThreads>(make_float2(sq, 0.0f), part, turn).x * inv + p.eps);
+        turn ^= 1;
+        T *const out = static_cast<T *>(p.out) + at;
+#pragma unroll 4
+        for (int d = threadIdx.x; d < dim; d += kThreads) {
+            const float v = (to_f32<T>(s[d]) - mean) * rstd;
+            out[d] = from_f32<T>(
+                fmaf(v, p.weight != nullptr ? __ldg(p.weight + d) : 1.0f, p.bias != nullptr ? __ldg(p.bias + d) : 0.0f));
+        }
+        if (p.stats != nullptr && threadIdx.x == 0) {
+            p.stats[2 * static_cast<size_t>(row)] = mean;
+            p.stats[2 * static_cast<size_t>(row) + 1] = rstd;
+        }
+        stage = stage + 1 == stages ? 0 : stage + 1;
+    }
+}
+
 constexpr int kWideThreads = 1024;
 
 // Rows of any length: a block per row, three passes over it.
@@ -146,15 +220,37 @@ cudaError_t launch_group(const NormArgs &a, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
+template <typename T, int kThreads>
+cudaError_t launch_staged(const NormArgs &a, cudaStream_t stream) {
+    const size_t row = (a.residual != nullptr ? 2 : 1) * staged_pitch<T>(a.dim) * sizeof(T);
+    const int stages = 3 * row <= kStagedBytes / 2 ? 3 : 2;
+    const size_t smem = stages * row;
+    const cudaError_t e = prepare_staged<norm_staged_kernel<T, kThreads>>();
+    if (e != cudaSuccess) return e;
+    const int64_t most = static_cast<int64_t>(current_device_sm_count()) *
+                         std::min<int64_t>(kStagedBytes / smem, 2048 / kThreads);
+    norm_staged_kernel<T, kThreads><<<static_cast<unsigned>(std::min<int64_t>(a.rows, most)), kThreads, smem, stream>>>(
+        a, stages);
+    return cudaGetLastError();
+}
+
 template <typename T, int VE>
 cudaError_t launch_rows(const NormArgs &a, cudaStream_t stream) {
-    constexpr int kElems = kRowElems<T, VE>;
-    if (a.dim <= 8 * kElems) return launch_group<T, VE, 8>(a, stream);
-    if (a.dim <= 32 * kElems) return launch_group<T, VE, 32>(a, stream);
-    if (a.dim <= 128 * kElems) return launch_group<T, VE, 128>(a, stream);
-    if (a.dim <= 256 * kElems) return launch_group<T, VE, 256>(a, stream);
-    if (a.dim <= 512 * kElems) return launch_group<T, VE, 512>(a, stream);
-    if (a.dim <= 1024 * kElems) return launch_group<T, VE, 1024>(a, stream);
+    if (a.dim <= 8 * kRowElems<T, VE, 8>) return launch_group<T, VE, 8>(a, stream);
+    if (a.dim <= 16 * kRowElems<T, VE, 16>) return launch_group<T, VE, 16>(a, stream);
+    if (a.dim <= 32 * kRowElems<T, VE, 32>) return launch_group<T, VE, 32>(a, stream);
+    if (a.dim <= 128 * kRowElems<T, VE, 128>) return launch_group<T, VE, 128>(a, stream);
+    if constexpr (VE == 1) {
+        if (2 * 2 * staged_pitch<T>(a.dim) * sizeof(T) <= kStagedBytes) {
+            if (staged_threads(a.dim) == 128) return launch_staged<T, 128>(a, stream);
+            if (staged_threads(a.dim) == 256) return launch_staged<T, 256>(a, stream);
+            return launch_staged<T, 512>(a, stream);
+        }
+    } else {
+        if (a.dim <= 256 * kRowElems<T, VE, 256>) return launch_group<T, VE, 256>(a, stream);
+        if (a.dim <= 512 * kRowElems<T, VE, 512>) return launch_group<T, VE, 512>(a, stream);
+        if (a.dim <= 1024 * kRowElems<T, VE, 1024>) return launch_group<T, VE, 1024>(a, stream);
+    }
     norm_wide_kernel<T><<<std::min(a.rows, 2 * current_device_sm_count()), kWideThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }

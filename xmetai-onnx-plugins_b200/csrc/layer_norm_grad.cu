@@ -7,9 +7,9 @@
 // Bound by memory: dy, x and d_residual are read once and dx written once. A thread
 // keeps the same columns for all rows that its block walks, so the sums over rows stay
 // in registers next to the row itself; each block leaves one row of partial sums, which
-// column_sum.cu adds in a fixed order. Rows that do not fit (above 8192 elements of the
-// 16-bit types, 4096 of float32 or unaligned) take a kernel for dx and one for the
-// columns.
+// column_sum.cu adds in a fixed order. Rows that are not whole words are staged in
+// shared memory. Rows that do not fit (above 8192 elements of the 16-bit types, 4096 of
+// float32 in whole words) take a kernel for dx and one for the columns.
 #include <algorithm>
 
 #include "xm_common.cuh"
@@ -118,6 +118,86 @@ __global__ void __launch_bounds__(threads_of(kGroup), 512 / threads_of(kGroup)) 
     if (part_b != nullptr) leave(part_b, sb);
 }
 
+// Rows that are not whole words, above 1024 elements: staged some rows ahead, kPer columns to a thread.
+template <typename T, int kThreads, int kPer>
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_grad_staged_kernel(const NormGradArgs p, int stages, float *part_w,
+                                                                         float *part_b) {
+    extern __shared__ float4 smem_f4[];
+    __shared__ float2 part[2 * (kThreads / 32)];
+    dependents_may_launch();
+    const int dim = p.dim;
+    const size_t pitch = staged_pitch<T>(dim);
+    T *const ring = reinterpret_cast<T *>(smem_f4);  // [stages][dy, x, d_residual][pitch]
+    const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
+                   *const DR = static_cast<const T *>(p.dres);
+    const float inv = 1.0f / static_cast<float>(dim);
+    float weight[kPer], sw[kPer], sb[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int d = threadIdx.x + k * kThreads;
+        weight[k] = p.weight != nullptr && d < dim ? p.weight[d] : 1.0f;
+        sw[k] = sb[k] = 0.0f;
+    }
+    auto copy = [&](long long row, int stage) {
+        if (row < p.rows) {
+            const unsigned i = static_cast<unsigned>(row);
+            stage_row<kThreads>(ring + 3 * stage * pitch, DY, i, dim);
+            stage_row<kThreads>(ring + (3 * stage + 1) * pitch, X, i, dim);
+            if (DR != nullptr) stage_row<kThreads>(ring + (3 * stage + 2) * pitch, DR, i, dim);
+        }
+        cp_async_commit();
+    };
+    for (int k = 0; k < stages - 1; ++k) copy(blockIdx.x + static_cast<long long>(k) * gridDim.x, k);
+    int turn = 0, stage = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        // (all but the last stages - 2 copies are here; two or three stages)
+        if (stages == 2) cp_async_wait<0>();
+        else cp_async_wait<1>();
+        __syncthreads();
+        copy(row + static_cast<long long>(stages - 1) * gridDim.x, stage == 0 ? stages - 1 : stage - 1);
+        const unsigned i = static_cast<unsigned>(row);
+        const T *const dy = ring + 3 * stage * pitch + staged_shift(DY, i, dim),
+                       *const x = ring + (3 * stage + 1) * pitch + staged_shift(X, i, dim),
+                       *const dr = ring + (3 * stage + 2) * pitch + (DR != nullptr ? staged_shift(DR, i, dim) : 0);
+        const float mean = p.rms ? 0.0f : p.stats[2 * static_cast<size_t>(row)];
+        const float rstd = p.stats[2 * static_cast<size_t>(row) + 1];
+        float2 total = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int d = threadIdx.x + k * kThreads;
+            if (d < dim) {
+                const float v = to_f32<T>(dy[d]), h = (to_f32<T>(x[d]) - mean) * rstd;
+                sw[k] = fmaf(v, h, sw[k]);
+                sb[k] += v;
+                const float gr = v * weight[k];
+                total.x += gr;
+                total.y = fmaf(gr, h, total.y);
+            }
+        }
+        total = group_sum<kThreads>(total, part, turn);
+        const float ag = p.rms ? 0.0f : total.x * inv, ax = total.y * inv;
+        T *const out = static_cast<T *>(p.dx) + static_cast<size_t>(row) * dim;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int d = threadIdx.x + k * kThreads;
+            if (d < dim) {
+                const float h = (to_f32<T>(x[d]) - mean) * rstd;
+                out[d] = from_f32<T>(
+                    fmaf(rstd, to_f32<T>(dy[d]) * weight[k] - ag - h * ax, DR != nullptr ? to_f32<T>(dr[d]) : 0.0f));
+            }
+        }
+        stage = stage + 1 == stages ? 0 : stage + 1;
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int d = threadIdx.x + k * kThreads;
+        if (d < dim) {
+            if (part_w != nullptr) part_w[static_cast<size_t>(blockIdx.x) * dim + d] = sw[k];
+            if (part_b != nullptr) part_b[static_cast<size_t>(blockIdx.x) * dim + d] = sb[k];
+        }
+    }
+}
+
 constexpr int kWideThreads = 1024;
 
 // Rows of any length: a block per row, two passes over it.
@@ -166,11 +246,18 @@ __global__ void __launch_bounds__(kColThreads) norm_grad_columns_kernel(const No
     if (part_b != nullptr) part_b[static_cast<size_t>(blockIdx.y) * p.dim + d] = sb;
 }
 
-// Threads per row; 0: the rows do not fit.
-int group_of(int dim, int elems) {
-    for (int group : {8, 32, 128, 256, 512})
-        if (dim <= group * elems) return group;
-    return 0;
+constexpr int kStagedMax = 16 * 512;  // longest staged row
+
+// Threads per row held in registers; -1: staged, 0: neither fits.
+template <typename T, int VE>
+int group_of(int dim) {
+    if (dim <= 8 * kRowElems<T, VE, 8>) return 8;
+    if (dim <= 16 * kRowElems<T, VE, 16>) return 16;
+    if (dim <= 32 * kRowElems<T, VE, 32>) return 32;
+    if (dim <= 128 * kRowElems<T, VE, 128>) return 128;
+    if (VE == 1) return dim <= kStagedMax && 2 * 3 * staged_pitch<T>(dim) * sizeof(T) <= kStagedBytes ? -1 : 0;
+    if (dim <= 256 * kRowElems<T, VE, 256>) return 256;
+    return dim <= 512 * kRowElems<T, VE, 512> ? 512 : 0;
 }
 
 // Whether all tensors move in words.
@@ -178,19 +265,44 @@ bool words_of(const NormGradArgs &a) {
     return a.dim % (a.io == IoType::kF32 ? 4 : 8) == 0 && aligned16(a.dy) && aligned16(a.x) && aligned16(a.dres) &&
            aligned16(a.weight);
 }
-int elems_of(const NormGradArgs &a, bool words) {
-    return !words ? kRowElems<float, 1> : a.io == IoType::kF32 ? kRowElems<float, 4> : kRowElems<__half, 8>;
+
+// Stages of a staged row, and blocks of an SM.
+template <typename T>
+int stages_of(int dim, int *blocks) {
+    const size_t row = 3 * staged_pitch<T>(dim) * sizeof(T);
+    const int stages = 3 * row <= kStagedBytes / 2 ? 3 : 2;
+    *blocks = static_cast<int>(std::min<size_t>(kStagedBytes / (stages * row), 512 / staged_threads(dim)));
+    return stages;
 }
 
 // Blocks that leave partial sums: as many as are resident, fewer for few rows.
-int parts_of(const NormGradArgs &a, bool words) {
-    const int group = group_of(a.dim, elems_of(a, words)), sms = current_device_sm_count();
+template <typename T, int VE>
+int parts_of(const NormGradArgs &a) {
+    const int group = group_of<T, VE>(a.dim), sms = current_device_sm_count();
     if (group == 0) {
         const int tiles = (a.dim + kColThreads - 1) / kColThreads;
         return std::max(1, std::min(a.rows, (8 * sms + tiles - 1) / tiles));
     }
+    if (group < 0) {
+        int blocks = 1;
+        stages_of<T>(a.dim, &blocks);
+        return std::max(1, std::min(a.rows, sms * blocks));
+    }
     const int threads = threads_of(group), rows = threads / group;
     return std::max(1, std::min((a.rows + rows - 1) / rows, sms * (512 / threads)));
+}
+int parts_of(const NormGradArgs &a, bool words) {
+    if (a.io == IoType::kF32) return words ? parts_of<float, 4>(a) : parts_of<float, 1>(a);
+    return words ? parts_of<__half, 8>(a) : parts_of<__half, 1>(a);
+}
+
+template <typename T, int kThreads, int kPer>
+void launch_staged(const NormGradArgs &a, int parts, float *part_w, float *part_b, cudaStream_t stream) {
+    int blocks = 1;
+    const int stages = stages_of<T>(a.dim, &blocks);
+    if (prepare_staged<norm_grad_staged_kernel<T, kThreads, kPer>>() != cudaSuccess) return;  // (the last error says so)
+    norm_grad_staged_kernel<T, kThreads, kPer>
+        <<<parts, kThreads, stages * 3 * staged_pitch<T>(a.dim) * sizeof(T), stream>>>(a, stages, part_w, part_b);
 }
 
 template <typename T, int VE, int kGroup>
@@ -200,12 +312,21 @@ void launch_group(const NormGradArgs &a, int parts, float *part_w, float *part_b
 
 template <typename T, int VE>
 void launch_rows(const NormGradArgs &a, int parts, float *part_w, float *part_b, cudaStream_t stream) {
-    switch (group_of(a.dim, kRowElems<T, VE>)) {
+    switch (group_of<T, VE>(a.dim)) {
         case 8: return launch_group<T, VE, 8>(a, parts, part_w, part_b, stream);
+        case 16: return launch_group<T, VE, 16>(a, parts, part_w, part_b, stream);
         case 32: return launch_group<T, VE, 32>(a, parts, part_w, part_b, stream);
         case 128: return launch_group<T, VE, 128>(a, parts, part_w, part_b, stream);
-        case 256: return launch_group<T, VE, 256>(a, parts, part_w, part_b, stream);
-        case 512: return launch_group<T, VE, 512>(a, parts, part_w, part_b, stream);
+    }
+    if constexpr (VE == 1) {
+        if (group_of<T, VE>(a.dim) < 0) {
+            if (staged_threads(a.dim) == 128) return launch_staged<T, 128, 16>(a, parts, part_w, part_b, stream);
+            if (staged_threads(a.dim) == 256) return launch_staged<T, 256, 20>(a, parts, part_w, part_b, stream);
+            return launch_staged<T, 512, 16>(a, parts, part_w, part_b, stream);
+        }
+    } else {
+        if (group_of<T, VE>(a.dim) == 256) return launch_group<T, VE, 256>(a, parts, part_w, part_b, stream);
+        if (group_of<T, VE>(a.dim) == 512) return launch_group<T, VE, 512>(a, parts, part_w, part_b, stream);
     }
     if (a.rows > 0)
         norm_grad_wide_kernel<T><<<std::min(a.rows, 2 * current_device_sm_count()), kWideThreads, 0, stream>>>(a);

@@ -359,6 +359,23 @@ cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
+// Host: lets a kernel use `bytes` of dynamic shared memory, and as many blocks of an SM as that allows (the driver's own
+// share of the cache left room for fewer than registers do). Set once per kernel and device.
+template <auto kKernel>
+cudaError_t allow_shared(size_t bytes) {
+    static std::atomic<unsigned long long> set{0};  // a bit per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (bit != 0 && (set.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kKernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) set.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+
 // Host: 16-byte alignment of a device pointer (vectorised and TMA paths).
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -20,7 +20,6 @@
 #pragma once
 
 #include <algorithm>
-#include <atomic>
 
 #include "xm_common.cuh"
 #include "xm_sequences.cuh"
@@ -264,23 +263,12 @@ struct Ring {
 };
 __device__ __forceinline__ bool finite2(float2 v) { return fabsf(v.x) <= 3.4028235e38f && fabsf(v.y) <= 3.4028235e38f; }
 
-// Launches kKernel with `warps` to a block. behind: it waits by itself for the kernel before. Its limit and share of
-// shared memory are set once per device (the driver's own share left room for fewer blocks than registers allow).
+// Launches kKernel with `warps` to a block. behind: it waits by itself for the kernel before.
 template <auto kKernel, typename... Args>
 cudaError_t launch_gate(int warps, size_t smem, const GateCut &g, int segments, bool behind, cudaStream_t stream,
                         const Args &...args) {
-    static std::atomic<unsigned long long> set{0};  // a bit per device
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    const cudaError_t e = allow_shared<kKernel>(smem);
     if (e != cudaSuccess) return e;
-    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
-    if (bit == 0 || (set.load(std::memory_order_acquire) & bit) == 0) {
-        e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kKernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        if (e != cudaSuccess) return e;
-        set.fetch_or(bit, std::memory_order_release);
-    }
     const dim3 grid(static_cast<unsigned>(g.width) * segments * g.tiles), block(32 * warps);
     if (behind) return launch_behind(kKernel, grid, block, smem, stream, args...);
     kKernel<<<grid, block, smem, stream>>>(args...);

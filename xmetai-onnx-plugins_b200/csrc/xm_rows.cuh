@@ -10,9 +10,10 @@
 
 namespace xm {
 
-// Elements of a row that a thread holds: two words of each tensor, or eight single elements.
-template <typename T, int VE>
-constexpr int kRowElems = VE == 1 ? 8 : 32 / static_cast<int>(sizeof(T));
+// Elements of a row that a thread holds: two words of each tensor (one in groups of up to 16, whose rows are short), or
+// eight single elements.
+template <typename T, int VE, int kGroup>
+constexpr int kRowElems = VE == 1 ? 8 : kGroup <= 16 ? VE : 2 * VE;
 
 template <typename T, int VE>
 struct Chunk;  // VE elements as they are stored
@@ -80,7 +81,7 @@ __device__ __forceinline__ void store_row_floats(float *p, const float *v) {
 // A row's chunks of one thread, as they are stored; zeros behind its end.
 template <typename T, int VE, int kGroup>
 struct RowPart {
-    static constexpr int kElems = kRowElems<T, VE>, kChunks = kElems / VE;
+    static constexpr int kElems = kRowElems<T, VE, kGroup>, kChunks = kElems / VE;
     Chunk<T, VE> c[kChunks];
     __device__ __forceinline__ static int at(int k, int g) { return (k * kGroup + g) * VE; }
     __device__ __forceinline__ void clear() {
@@ -138,6 +139,33 @@ struct RowPart {
 };
 
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+
+// Rows that are not whole words, staged in shared memory: 4-byte asynchronous copies from the word that holds a row's
+// first element, so that a row of a 16-bit type may begin in the middle of its first word. Elements are read from there
+// by consecutive threads, about sixteen to each: fewer leave most of a row's time to its barriers (32768 x 1026, backward:
+// 229 us with 512 threads), more too few warps.
+constexpr int staged_threads(int dim) { return dim <= 2048 ? 128 : dim <= 5120 ? 256 : 512; }
+
+template <typename T>
+__host__ __device__ constexpr size_t staged_pitch(int dim) {  // elements of a staged row, in whole 16-byte words
+    return (static_cast<size_t>(dim) + 2 + 16 / sizeof(T) - 1) / (16 / sizeof(T)) * (16 / sizeof(T));
+}
+constexpr size_t kStagedBytes = 220 * 1024;  // of shared memory on an SM
+template <auto kKernel>
+cudaError_t prepare_staged() { return allow_shared<kKernel>(kStagedBytes); }
+// Where row `row` of a tensor begins in its stage.
+template <typename T>
+__device__ __forceinline__ int staged_shift(const T *src, unsigned row, int dim) {
+    if (sizeof(T) != 2) return 0;
+    return static_cast<int>((reinterpret_cast<uintptr_t>(src) >> 1) ^ (row & static_cast<unsigned>(dim))) & 1;
+}
+template <int kThreads, typename T>
+__device__ __forceinline__ void stage_row(T *dst, const T *src, unsigned row, int dim) {
+    constexpr int kPer = 4 / static_cast<int>(sizeof(T));
+    const int shift = staged_shift(src, row, dim);
+    const T *const first = src + static_cast<size_t>(row) * dim - shift;
+    for (int i = threadIdx.x * kPer; i < dim + shift; i += kThreads * kPer) cp_async4(dst + i, first + i, 4);
+}
 
 // Sums of two values over a group, the same in all its threads and whatever the number of rows. `part`: shared memory
 // of 2 x (kGroup / 32) pairs, used in turn (`turn` alternates), so that one barrier is enough.
