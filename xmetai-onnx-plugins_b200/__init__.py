@@ -458,8 +458,8 @@ def GatedDeltaNet2Fn(q, k, v, g, beta, w, initial_state=None, *, scale: float = 
 # ---------------------------------------------------------------- serving operators
 #
 # A decode step calls these for every layer, so their host path is short: the
-# descriptors are filled and the entry point is called in C (csrc/pycall.c), and
-# validation happens once, in the library.
+# descriptors are filled, outputs and workspace allocated and the entry point
+# called in C++ (csrc/pycall.cpp), and validation happens once, in the library.
 
 
 def _invalid(message):
@@ -482,13 +482,13 @@ def _load_pycall():
         path = _PKG_DIR / ("_xm_call" + sysconfig.get_config_var("EXT_SUFFIX"))
         if not path.exists():
             raise XmError(XM_ERR_UNSUPPORTED, f"{path} not found; build it with `make -C {_PKG_DIR} "
-                                              f"PYTHON={sys.executable}` (needs this Python's headers)")
+                                              f"PYTHON={sys.executable}` (needs its headers and its torch's)")
         spec = importlib.util.spec_from_file_location("_xm_call", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        mod.setup(torch.Tensor, ((torch.float32, DTYPE_FLOAT), (torch.bfloat16, DTYPE_BFLOAT16),
-                                 (torch.float16, DTYPE_FLOAT16), (torch.int32, DTYPE_INT32),
-                                 (torch.int64, DTYPE_INT64)))
+        if mod.torch_version.split("+")[0] != torch.__version__.split("+")[0]:
+            raise XmError(XM_ERR_UNSUPPORTED, f"{path} was built for torch {mod.torch_version}, this is "
+                                              f"{torch.__version__}; build it with `make -C {_PKG_DIR}`")
         _pycall = mod
     return _pycall
 
@@ -504,120 +504,89 @@ class _ServeOp:
         self.call = None
 
     def load(self):
-        import torch
-
         lib = load_library()
         address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
         self.fwd = address(getattr(lib, f"xm_{self.name}_fwd"))
         self.size = address(getattr(lib, f"xm_{self.name}_workspace_size")) if self.workspace else 0
-        self.blank = {}  # by the activations' type: the descriptors of absent inputs
-        for io, code in ((torch.float32, DTYPE_FLOAT), (torch.bfloat16, DTYPE_BFLOAT16),
-                         (torch.float16, DTYPE_FLOAT16), (None, 0)):
+        blanks = []  # by the activations' type: the descriptors of absent inputs
+        for code in (DTYPE_FLOAT, DTYPE_BFLOAT16, DTYPE_FLOAT16, 0):
             descs = (XmTensor * len(self.names))()
             for i, k in enumerate(self.kinds):
                 descs[i].rank, descs[i].dtype = 1, {"x": code, "f": DTYPE_FLOAT, "i": DTYPE_INT64}[k]
-            self.blank[io] = bytes(descs)
-        self.call = _load_pycall().call
+            blanks.append(bytes(descs))
+        self.blanks = tuple(blanks)
+        self.call = _load_pycall().serve
 
-
-def _serve(op, attrs, tensors, out, state, state_shape, with_state, stream):
-    """Call xm_<op>_fwd on the device of tensors[0]. The state output is `state`, a new tensor of state_shape, or
-    (state_shape None) the state input itself, which then has to be contiguous: a copy would lose the update.
-    Everything allocated here belongs to the stream that the call runs on."""
-    import torch
-
-    if op.call is None:
-        op.load()
-    x = tensors[0]
-    index = x.get_device() if isinstance(x, torch.Tensor) else -1
-    if index < 0:
-        _invalid(f"{op.names[0]} must be a CUDA tensor")
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            return _serve(op, attrs, tensors, out, state, state_shape, with_state, stream)
-    handle = torch._C._cuda_getCurrentRawStream(index)
-    if stream is not None:
-        if stream.device_index != index:  # (default streams of all devices have the same handle)
-            _invalid("stream belongs to another device")
-        if stream.cuda_stream != handle:
-            with torch.cuda.stream(stream):
-                return _serve(op, attrs, tensors, out, state, state_shape, with_state, None)
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    inplace = -1
-    outs = (out,)
-    if with_state:
-        if state_shape is None:
-            inplace = op.state
-        if state is None:
-            state = tensors[inplace] if state_shape is None else x.new_empty(
-                state_shape, dtype=torch.float32 if op.kinds[op.state] == "f" else x.dtype)
-        outs = (out, state)
-    _launch(op, ctypes.addressof(attrs), tensors, outs, index, inplace, handle)
-    return outs if with_state else out
-
-
-def _launch(op, attrs, tensors, outs, index, inplace, handle):
-    """Call xm_<op>_fwd on the current device `index` and the current stream `handle`; attrs: the struct's address."""
-    x = tensors[0]
-    blank = op.blank.get(x.dtype)
-    status, which = op.call(op.fwd, op.size, attrs, tensors, op.blank[None] if blank is None else blank, outs, index,
-                            inplace, _scratch(x) if op.workspace else None, handle)
-    if status:
+    def refused(self, status, which, tensors):
+        """Raise what a call's status says."""
+        if status == -4:
+            _invalid(f"{self.names[0]} must be a CUDA tensor")
+        device = f"cuda:{tensors[0].get_device()}"
         if status == -1:
-            _invalid(f"{op.names[which]} must be a tensor on cuda:{index}")
+            _invalid(f"{self.names[which]} must be a tensor on {device}")
         if status == -2:
-            _invalid(f"{op.names[which]} is updated in place and must be contiguous")
+            _invalid(f"{self.names[which]} is updated in place and must be contiguous")
         if status == -3:
-            _invalid(f"{op.outs[which]} must be a contiguous tensor on cuda:{index}")
+            _invalid(f"{self.outs[which]} must be a contiguous tensor on {device}")
         _check(status)
 
 
-def _scratch(x):
-    import torch
-
-    return lambda n: x.new_empty(n, dtype=torch.uint8)
-
-
-def _serve_many(op, attrs, tensors, make, stream, inplace=-1):
-    """_serve for operators with other outputs than a tensor and a state: make() gives their tuple, on the device and the
-    stream that the call runs on. attrs: the struct's address. Returns the outputs."""
-    import torch
-
+def _serve(op, attrs, tensors, outs, shapes, stream, inplace=-1):
+    """Call xm_<op>_fwd on the device of tensors[0]; attrs: the attribute struct's address. An output that is None is
+    allocated: with the shape and type of tensors[0], or where `shapes` says (own, sizes...), float32, or with own=1 of
+    that type. Everything allocated belongs to the stream that the call runs on. inplace: an input that must not be
+    copied. Returns the outputs."""
     if op.call is None:
         op.load()
-    x = tensors[0]
-    index = x.get_device() if isinstance(x, torch.Tensor) else -1
-    if index < 0:
-        _invalid(f"{op.names[0]} must be a CUDA tensor")
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            return _serve_many(op, attrs, tensors, make, stream, inplace)
-    handle = torch._C._cuda_getCurrentRawStream(index)
     if stream is not None:
-        if stream.device_index != index:
-            _invalid("stream belongs to another device")
-        if stream.cuda_stream != handle:
-            with torch.cuda.stream(stream):
-                return _serve_many(op, attrs, tensors, make, None, inplace)
-    outs = make()
-    _launch(op, attrs, tensors, outs, index, inplace, handle)
-    return outs
+        import torch
+
+        x = tensors[0]
+        index = x.get_device() if isinstance(x, torch.Tensor) else -1
+        if index >= 0:
+            if stream.device_index != index:  # (default streams of all devices have the same handle)
+                _invalid("stream belongs to another device")
+            with torch.cuda.device(index):
+                if stream.cuda_stream != torch._C._cuda_getCurrentRawStream(index):
+                    with torch.cuda.stream(stream):
+                        return _serve(op, attrs, tensors, outs, shapes, None, inplace)
+                return _serve(op, attrs, tensors, outs, shapes, None, inplace)
+    got = op.call(op.fwd, op.size, attrs, tensors, op.blanks, outs, shapes, inplace)
+    if len(got) == 2 and type(got[0]) is int:
+        if got[0] == -5:
+            import torch
+
+            with torch.cuda.device(tensors[0].get_device()):
+                return _serve(op, attrs, tensors, outs, shapes, None, inplace)
+        op.refused(got[0], got[1], tensors)
+    return got
+
+
+def _serve_state(op, attrs, tensors, out, state, state_shape, with_state, stream):
+    """_serve with an output and a state: `state`, a new tensor of state_shape, or (state_shape None) the state input
+    itself, which then has to be contiguous: a copy would lose the update."""
+    if not with_state:
+        return _serve(op, attrs, tensors, (out,), (None,), stream)[0]
+    inplace = -1
+    if state_shape is None:
+        inplace = op.state
+        if state is None:
+            state = tensors[inplace]
+    return _serve(op, attrs, tensors, (out, state),
+                  (None, None if state_shape is None else (int(op.kinds[op.state] == "x"), *state_shape)), stream, inplace)
 
 
 _attrs = {}
 
 
 def _address(kind, *values):
-    """Address of an attribute struct with these values, which stays as it is."""
+    """Address of an attribute struct with these values, which stays as it is (and lives as long as the process)."""
     key = (kind, *values)
     a = _attrs.get(key)
     if a is None:
-        if len(_attrs) > 1000:
-            _attrs.clear()
         a = kind(*values)
-        a = _attrs[key] = (a, ctypes.addressof(a))
-    return a
+        a = _attrs[key] = (ctypes.addressof(a), a)
+    return a[0]
 
 
 _CONV = _ServeOp("causal_conv1d", ("x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices",
@@ -663,14 +632,14 @@ def CausalConv1dFn(x, weight, bias=None, initial_state=None, cu_seqlens=None, st
     output_final_state=1 its final state replaces that row in place (the result is (out, initial_state)). An index
     outside the pool owns no row: zeros, and no final state is kept. No slot may be named twice in a call.
     """
-    attrs = CausalConv1dAttrs(int(silu), int(channels_last), int(output_final_state))
+    attrs = _address(CausalConv1dAttrs, int(silu), int(channels_last), int(output_final_state))
     shape = None
     if output_final_state:
         if getattr(x, "ndim", 0) != 3 or getattr(weight, "ndim", 0) != 2:
             _invalid("x must have rank 3 and weight shape (dim, width)")
         shape = _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state,
                                     (x.shape[2 if channels_last else 1], max(0, weight.shape[1] - 1)))
-    return _serve(_CONV, attrs, (x, weight, bias, initial_state, cu_seqlens, state_indices, has_initial_state), out,
+    return _serve_state(_CONV, attrs, (x, weight, bias, initial_state, cu_seqlens, state_indices, has_initial_state), out,
                   final_state, shape, bool(output_final_state), stream)
 
 
@@ -682,7 +651,7 @@ def CausalConv1dUpdateFn(x, weight, bias=None, state=None, state_indices=None, *
     skipped and their output rows left as they were."""
     if state is None:
         _invalid("CausalConv1dUpdateFn needs a state")
-    return _serve(_CONV_UPDATE, CausalConv1dUpdateAttrs(int(silu)), (x, weight, bias, state, state_indices), out,
+    return _serve_state(_CONV_UPDATE, _address(CausalConv1dUpdateAttrs, int(silu)), (x, weight, bias, state, state_indices), out,
                   new_state, None if new_state is None or new_state is state else (), True, stream)
 
 
@@ -697,14 +666,14 @@ def SelectiveScanVarlenFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, in
     initial_state is float32 [sequences, dim, d_state] (SelectiveScanFn's last_state); output_final_state,
     cu_seqlens, state_indices and has_initial_state work as in CausalConv1dFn.
     """
-    attrs = SelectiveScanVarlenAttrs(int(delta_softplus), int(output_final_state))
+    attrs = _address(SelectiveScanVarlenAttrs, int(delta_softplus), int(output_final_state))
     shape = None
     if output_final_state:
         if getattr(u, "ndim", 0) != 3 or getattr(A, "ndim", 0) != 2:
             _invalid("u must have rank 3 and A shape (dim, d_state)")
         shape = _prompt_state_shape(u, cu_seqlens, state_indices, initial_state, final_state,
                                     (u.shape[2], A.shape[1]))
-    return _serve(_SCAN, attrs, (u, delta, A, B, C, D, z, delta_bias, initial_state, cu_seqlens, state_indices,
+    return _serve_state(_SCAN, attrs, (u, delta, A, B, C, D, z, delta_bias, initial_state, cu_seqlens, state_indices,
                                  has_initial_state), out, final_state, shape, bool(output_final_state), stream)
 
 
@@ -716,7 +685,7 @@ def SelectiveStateUpdateFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, s
     receives it instead. Rows whose index is outside the pool are skipped and their output rows left as they were."""
     if state is None:
         _invalid("SelectiveStateUpdateFn needs a state")
-    return _serve(_UPDATE, SelectiveStateUpdateAttrs(int(delta_softplus)),
+    return _serve_state(_UPDATE, _address(SelectiveStateUpdateAttrs, int(delta_softplus)),
                   (u, delta, A, B, C, D, z, delta_bias, state, state_indices), out, new_state,
                   None if new_state is None or new_state is state else (), True, stream)
 
@@ -747,7 +716,7 @@ def GatedRecurrenceFn(x, f, lower_bound=None, initial_state=None, cu_seqlens=Non
         if getattr(x, "ndim", 0) != 3:
             _invalid("x must have rank 3")
         shape = _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state, (x.shape[2],))
-    return _serve(_GATE, GatedRecurrenceAttrs(int(output_final_state)),
+    return _serve_state(_GATE, _address(GatedRecurrenceAttrs, int(output_final_state)),
                   (x, f, lower_bound, initial_state, cu_seqlens, state_indices, has_initial_state), out, final_state,
                   shape, bool(output_final_state), stream)
 
@@ -763,11 +732,9 @@ def GatedRecurrenceGradFn(dy, x, f, y, lower_bound=None, initial_state=None, cu_
     else None. A sequence that started from zeros has a row of zeros in initial_state. out: a tuple of outputs in the
     same order, None where one is to be allocated.
     """
-    import torch
-
     if getattr(dy, "ndim", 0) != 3:
         _invalid("dy must have rank 3")
-    units = cu_seqlens.numel() - 1 if _given(cu_seqlens) else dy.shape[0]
+    units, dim = cu_seqlens.numel() - 1 if _given(cu_seqlens) else dy.shape[0], dy.shape[2]
     lb = _given(lower_bound) if output_lower_bound_grad is None else bool(output_lower_bound_grad)
     st = bool(output_initial_state_grad) if output_initial_state_grad is not None else (
         _given(initial_state) or (initial_state is not None and units == 0))
@@ -775,18 +742,10 @@ def GatedRecurrenceGradFn(dy, x, f, y, lower_bound=None, initial_state=None, cu_
         out = (None, None, None, None)
     elif len(out) != 4:
         _invalid("out must hold 4 outputs (None: allocate)")
-
-    def make():
-        outs = [torch.empty_like(dy, memory_format=torch.contiguous_format) if o is None else o for o in out[:2]]
-        if lb:
-            outs.append(dy.new_empty(dy.shape[2], dtype=torch.float32) if out[2] is None else out[2])
-        if st:
-            outs.append(dy.new_empty((units, dy.shape[2]), dtype=torch.float32) if out[3] is None else out[3])
-        return tuple(outs)
-
-    attrs = _address(GatedRecurrenceGradAttrs, int(lb), int(st))
-    got = _serve_many(_GATE_GRAD, attrs[1], (dy, x, f, y, lower_bound, initial_state, cu_seqlens, d_final_state), make,
-                      stream)
+    got = _serve(_GATE_GRAD, _address(GatedRecurrenceGradAttrs, int(lb), int(st)),
+                 (dy, x, f, y, lower_bound, initial_state, cu_seqlens, d_final_state),
+                 (*out[:2], *out[2:3 if lb else 2], *out[3:4 if st else 3]),
+                 (None, None, *(((0, dim),) if lb else ()), *(((0, units, dim),) if st else ())), stream)
     return got[0], got[1], got[2] if lb else None, got[-1] if st else None
 
 
@@ -798,7 +757,7 @@ def GatedRecurrenceUpdateFn(x, f, lower_bound=None, state=None, state_indices=No
     they were."""
     if state is None:
         _invalid("GatedRecurrenceUpdateFn needs a state")
-    return _serve(_GATE_UPDATE, GatedRecurrenceUpdateAttrs(0), (x, f, lower_bound, state, state_indices), out, new_state,
+    return _serve_state(_GATE_UPDATE, _address(GatedRecurrenceUpdateAttrs, 0), (x, f, lower_bound, state, state_indices), out, new_state,
                   None if new_state is None or new_state is state else (), True, stream)
 
 
@@ -811,27 +770,23 @@ def LayerNormFn(x, weight=None, bias=None, residual=None, *, eps: float = 1e-5, 
     tuple: (y, s) with a residual, and with output_stats=1 the float32 [..., 2] of every row's mean and rstd at its
     end, which LayerNormGradFn takes. residual_out may be the residual itself: the residual stream in place.
     """
-    import torch
-
     if getattr(x, "ndim", 0) == 0:
         _invalid("x must have at least one axis")
-    if residual is not None and not _given(residual) and not _given(x):  # no rows: the sum is as empty as its terms
-        y = LayerNormFn(x, weight, bias, eps=eps, rms=rms, output_stats=output_stats, stream=stream, out=out, stats=stats)
-        y = y if output_stats else (y,)
-        return y[:1] + (x.new_empty(x.shape) if residual_out is None else residual_out,) + y[1:]
-    many = _given(residual)
-
-    def make():
-        outs = [torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else out]
-        if many:
-            outs.append(torch.empty_like(x, memory_format=torch.contiguous_format) if residual_out is None else residual_out)
-        if output_stats:
-            outs.append(x.new_empty((*x.shape[:-1], 2), dtype=torch.float32) if stats is None else stats)
-        return tuple(outs)
-
-    attrs = _address(LayerNormAttrs, float(eps), int(rms), int(output_stats))
-    got = _serve_many(_NORM, attrs[1], (x, weight, bias, residual), make, stream,
-                      3 if many and residual_out is residual else -1)
+    outs, shapes, inplace = (out,), (None,), -1
+    if residual is not None:
+        if not _given(residual) and not _given(x):  # no rows: the sum is as empty as its terms
+            y = LayerNormFn(x, weight, bias, eps=eps, rms=rms, output_stats=output_stats, stream=stream, out=out,
+                            stats=stats)
+            y = y if output_stats else (y,)
+            return y[:1] + (x.new_empty(x.shape) if residual_out is None else residual_out,) + y[1:]
+        if _given(residual):
+            outs, shapes = (out, residual_out), (None, None)
+            if residual_out is residual:
+                inplace = 3
+    if output_stats:
+        outs, shapes = (*outs, stats), (*shapes, (0, *x.shape[:-1], 2))
+    got = _serve(_NORM, _address(LayerNormAttrs, float(eps), int(rms), int(output_stats)), (x, weight, bias, residual),
+                 outs, shapes, stream, inplace)
     return got if len(got) > 1 else got[0]
 
 
@@ -846,26 +801,18 @@ def LayerNormGradFn(dy, x, weight=None, stats=None, d_residual=None, *, rms: int
     """
     if stats is None:
         _invalid("LayerNormGradFn needs the forward call's stats")
-    import torch
-
     if getattr(dy, "ndim", 0) == 0:
         _invalid("dy must have at least one axis")
-    many = _given(weight)
+    many, dim = _given(weight), dy.shape[-1]
     if out is None:
         out = (None, None, None)
     elif len(out) != 3:
         _invalid("out must hold 3 outputs (None: allocate)")
-
-    def make():
-        outs = [torch.empty_like(dy, memory_format=torch.contiguous_format) if out[0] is None else out[0]]
-        if many:
-            outs.append(dy.new_empty(dy.shape[-1], dtype=torch.float32) if out[1] is None else out[1])
-        if output_bias_grad:
-            outs.append(dy.new_empty(dy.shape[-1], dtype=torch.float32) if out[2] is None else out[2])
-        return tuple(outs)
-
-    attrs = _address(LayerNormGradAttrs, int(rms), int(output_bias_grad))
-    got = _serve_many(_NORM_GRAD, attrs[1], (dy, x, weight, stats, d_residual), make, stream)
+    sums = int(many) + bool(output_bias_grad)
+    got = _serve(_NORM_GRAD, _address(LayerNormGradAttrs, int(rms), int(output_bias_grad)),
+                 (dy, x, weight, stats, d_residual),
+                 (out[0], *out[1:2 if many else 1], *out[2:3 if output_bias_grad else 2]), (None,) + ((0, dim),) * sums,
+                 stream)
     return got[0], got[1] if many else None, got[-1] if output_bias_grad else None
 
 
