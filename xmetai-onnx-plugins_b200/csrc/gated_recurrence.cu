@@ -21,146 +21,191 @@ template <typename T, int kWarps>
 constexpr int kRingStages = kWarps == 8 || sizeof(T) == 4 ? 3 : 2;
 
 template <typename T, bool kWords>
-struct ScanSmem {
-    GateTile<T, kGateGroup, kWords> ring[kStages][2];
-};
+using ScanTile = GateTile<T, kGateGroup, kWords>;
 
-// kEnds: the first pass over segments (all but a span's last).
+template <typename T, bool kWords>
+__device__ __forceinline__ float2 init_of(const GateArgs &p, const Lane<T, kWords> &ch, long long row) {
+    return ch.floats(p.init != nullptr && row >= 0 ? p.init + row * p.dim : nullptr, 0.0f);
+}
+template <typename T, bool kWords>
+__device__ __forceinline__ void store_final(const GateArgs &p, const Lane<T, kWords> &ch, long long row, float2 h) {
+    if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
+}
+// Sequences without tokens keep their starting states; warp of warps with the same channels.
+template <typename T, bool kWords>
+__device__ __forceinline__ void keep_empty(const GateArgs &p, const Lane<T, kWords> &ch, int warp, int warps) {
+    if (p.final_state == nullptr) return;
+    for_empty_sequences(p.seq, warp, warps, [&](int s) {
+        long long from;
+        const long long row = seq_rows(p.seq, s, &from);
+        store_final(p, ch, row, init_of(p, ch, from));
+    });
+}
+
+// A warp walks segment j of a span. kEnds: the first pass. first_pass(): it is through; nothing is stored, and nothing
+// of it read, before.
+template <typename T, bool kWords, bool kEnds, int kStages, typename Wait>
+__device__ __forceinline__ void walk_segment(const GateArgs &p, const GateCut &g, ScanTile<T, kWords> (*ring)[2],
+                                             const Lane<T, kWords> &ch, int tile, float2 low, float2 rest, Span span,
+                                             int length, int j, const GatePairs &pairs, Wait &&first_pass) {
+    const SeqArgs &q = p.seq;
+    const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
+    T *const Y = static_cast<T *>(p.out);
+    const int s0 = span.lo + min(static_cast<long long>(j) * length, static_cast<long long>(max(span.hi - span.lo, 0)));
+    const int s1 = min(static_cast<long long>(s0) + length, static_cast<long long>(span.hi));
+    if (s0 >= s1) return;
+    int begin = s0;
+    SeqAt seq = seq_at(q, kEnds ? s1 - 1 : s0);
+    if (kEnds) {
+        if (seq.end <= s1 || s1 >= span.hi) return;  // no sequence leaves the segment
+        begin = max(s0, seq.start);
+    }
+    auto copy = [&](int t, int stage) {
+        if (t < s1) {
+            copy_tile(ring[stage][0], X, t, 0, s1, p.dim, tile);
+            copy_tile(ring[stage][1], F, t, 0, s1, p.dim, tile);
+        }
+        cp_async_commit();
+    };
+    for (int k = 0; k < kStages - 1; ++k) copy(begin + k * kGateGroup, k);
+    first_pass();
+    float2 h = both(0.0f), P = both(1.0f);
+    long long from, row = seq_rows(q, seq.seq, &from);
+    // where the warp's first token does not begin a sequence, the state comes from the segments before
+    SeqAt next{0, 0, 0};
+    long long next_row = -1;
+    float2 next_h = both(0.0f);
+    if (seq.start >= begin) {  // (== unless the offsets descend)
+        h = init_of(p, ch, from);
+        if (kEnds) pairs.start(j) = h;
+        else if (seq.end > s1 && g.segments > 1) h = pairs.start(j);
+    } else if (!kEnds && j > 0) {
+        int k = max(seq.start - span.lo, 0) / length;
+        h = pairs.h(k);
+        for (++k; k < j; ++k) h = __ffma2_rn(pairs.P(k), h, pairs.h(k));
+    }
+    auto look_ahead = [&] {  // the sequence behind this one, and its starting state
+        if (kEnds || seq.end >= s1) return;
+        next = seq_behind(q, seq);
+        next_row = seq_rows(q, next.seq, &from);
+        // one that leaves the segment: its last warp may have stored its final state in the same place
+        next_h = next.end > s1 && g.segments > 1 ? pairs.start(j) : init_of(p, ch, from);
+    };
+    look_ahead();
+    int stage = 0;
+    for (int t = begin; t < s1; t += kGateGroup) {
+        cp_async_wait<kStages - 2>();
+        __syncwarp();
+        copy(t + (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
+        auto token = [&](int k, float2 &x, float2 &f) {
+            x = ring[stage][0].at(k, shift_of<T, kWords>(X, t + k, p.dim));
+            f = ring[stage][1].at(k, shift_of<T, kWords>(F, t + k, p.dim));
+        };
+        if (t + kGateGroup <= s1 && (kEnds || seq.end > t + kGateGroup)) {
+            float2 a[kGateGroup], b[kGateGroup];
+#pragma unroll
+            for (int k = 0; k < kGateGroup; ++k) {
+                float2 x, f;
+                token(k, x, f);
+                const Gate2 gate = gate_of(f, low, rest);
+                a[k] = gate.a;
+                b[k] = __fmul2_rn(gate.u, x);
+            }
+#pragma unroll
+            for (int k = 0; k < kGateGroup; ++k) {
+                h = __ffma2_rn(a[k], h, b[k]);
+                if (kEnds) P = __fmul2_rn(P, a[k]);
+                b[k] = h;
+            }
+            if (!kEnds && ch.active[0]) {
+                T *y = Y + static_cast<size_t>(t) * p.dim;
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k, y += p.dim) ch.store(y, b[k]);
+            }
+        } else {
+#pragma unroll 1
+            for (int k = 0; k < kGateGroup && t + k < s1; ++k) {
+                float2 x, f;
+                token(k, x, f);
+                const Gate2 gate = gate_of(f, low, rest);
+                h = __ffma2_rn(gate.a, h, __fmul2_rn(gate.u, x));
+                if (kEnds) {
+                    P = __fmul2_rn(P, gate.a);
+                    continue;
+                }
+                if (ch.active[0]) ch.store(Y + static_cast<size_t>(t + k) * p.dim, h);
+                if (seq.end == t + k + 1) {
+                    store_final(p, ch, row, h);
+                    seq = next;
+                    row = next_row;
+                    h = next_h;
+                    look_ahead();
+                }
+            }
+        }
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    if (kEnds) {
+        pairs.P(j) = above_zero(P);
+        pairs.h(j) = h;
+    }
+    cp_async_wait<0>();
+    __syncwarp();  // (the ring is filled anew)
+}
+
+// A segment to each warp. kEnds: the first pass over segments (all but a span's last).
 template <typename T, bool kWords, bool kEnds>
 __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const GateCut g) {
     extern __shared__ float4 smem_f4[];
-    auto &sm = *reinterpret_cast<ScanSmem<T, kWords> *>(smem_f4);
     if (kEnds) dependents_may_launch();
-    const SeqArgs &q = p.seq;
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs, slot = blockIdx.x / g.tiles / segs;
     const Lane<T, kWords> ch(tile, threadIdx.x & 31, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
-    const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
-    T *const Y = static_cast<T *>(p.out);
-    auto init_of = [&](int seq, long long row) {
-        return ch.floats(p.init != nullptr && seq_live(q, seq, row) ? p.init + row * p.dim : nullptr, 0.0f);
-    };
-    auto store_final = [&](long long row, float2 h) {
-        if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
-    };
     bool waited = kEnds;
-    auto first_pass = [&] {  // is through: nothing is stored, and nothing of it read, before
+    auto first_pass = [&] {
         if (!waited) wait_for_before();
         waited = true;
     };
-    if (!kEnds && p.final_state != nullptr && (q.cu != nullptr || q.seqlen == 0)) first_pass();
-    if (!kEnds && p.final_state != nullptr)  // sequences without tokens keep their starting states
-        for_empty_sequences(q, slot * segs + j, g.width * segs, [&](int s) {
-            const long long row = seq_row(q, s);
-            store_final(row, init_of(s, row));
-        });
+    if (!kEnds && p.final_state != nullptr && (p.seq.cu != nullptr || p.seq.seqlen == 0)) first_pass();
+    if (!kEnds) keep_empty(p, ch, slot * segs + j, g.width * segs);
     for (int i = slot; i < g.spans; i += g.width) {
-        const Span span = gate_span(q, g, i);
-        const int length = segment_length(g, span);
-        const int s0 = span.lo + min(static_cast<long long>(j) * length, static_cast<long long>(max(span.hi - span.lo, 0)));
-        const int s1 = min(static_cast<long long>(s0) + length, static_cast<long long>(span.hi));
-        if (s0 >= s1) continue;
-        auto pair = [&](int k) { return ((static_cast<size_t>(i) * g.segments + k) * g.tiles + tile) * 32 + threadIdx.x; };
-        int begin = s0;
-        SeqAt seq = seq_at(q, kEnds ? s1 - 1 : s0);
-        if (kEnds) {
-            if (seq.end <= s1 || s1 >= span.hi) continue;  // no sequence leaves the segment
-            begin = max(s0, seq.start);
-        }
-        auto copy = [&](int t, int stage) {
-            if (t < s1) {
-                copy_tile(sm.ring[stage][0], X, t, 0, s1, p.dim, tile);
-                copy_tile(sm.ring[stage][1], F, t, 0, s1, p.dim, tile);
-            }
-            cp_async_commit();
-        };
-        for (int k = 0; k < kStages - 1; ++k) copy(begin + k * kGateGroup, k);
-        first_pass();
-        float2 h = both(0.0f), P = both(1.0f);
-        long long row = seq_row(q, seq.seq);
-        // where the warp's first token does not begin a sequence, the state comes from the segments before
-        SeqAt next{0, 0, 0};
-        long long next_row = -1;
-        float2 next_h = both(0.0f);
-        if (seq.start >= begin) {  // (== unless the offsets descend)
-            h = init_of(seq.seq, row);
-            if (kEnds) g.start[pair(j)] = h;
-            else if (seq.end > s1 && g.segments > 1) h = g.start[pair(j)];
-        } else if (!kEnds && j > 0) {
-            int k = max(seq.start - span.lo, 0) / length;
-            h = g.h[pair(k)];
-            for (++k; k < j; ++k) h = __ffma2_rn(g.P[pair(k)], h, g.h[pair(k)]);
-        }
-        auto look_ahead = [&] {  // the sequence behind this one, and its starting state
-            if (kEnds || seq.end >= s1) return;
-            next = seq_behind(q, seq);
-            next_row = seq_row(q, next.seq);
-            // one that leaves the segment: its last warp may have stored its final state in the same place
-            next_h = next.end > s1 && g.segments > 1 ? g.start[pair(j)] : init_of(next.seq, next_row);
-        };
-        look_ahead();
-        int stage = 0;
-        for (int t = begin; t < s1; t += kGateGroup) {
-            cp_async_wait<kStages - 2>();
-            __syncwarp();
-            copy(t + (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
-            auto token = [&](int k, float2 &x, float2 &f) {
-                x = sm.ring[stage][0].at(k, shift_of<T, kWords>(X, t + k, p.dim));
-                f = sm.ring[stage][1].at(k, shift_of<T, kWords>(F, t + k, p.dim));
-            };
-            if (t + kGateGroup <= s1 && (kEnds || seq.end > t + kGateGroup)) {
-                float2 a[kGateGroup], b[kGateGroup];
-#pragma unroll
-                for (int k = 0; k < kGateGroup; ++k) {
-                    float2 x, f;
-                    token(k, x, f);
-                    const Gate2 gate = gate_of(f, low, rest);
-                    a[k] = gate.a;
-                    b[k] = __fmul2_rn(gate.u, x);
-                }
-#pragma unroll
-                for (int k = 0; k < kGateGroup; ++k) {
-                    h = __ffma2_rn(a[k], h, b[k]);
-                    if (kEnds) P = __fmul2_rn(P, a[k]);
-                    b[k] = h;
-                }
-                if (!kEnds && ch.active[0]) {
-                    T *y = Y + static_cast<size_t>(t) * p.dim;
-#pragma unroll
-                    for (int k = 0; k < kGateGroup; ++k, y += p.dim) ch.store(y, b[k]);
-                }
-            } else {
-#pragma unroll 1
-                for (int k = 0; k < kGateGroup && t + k < s1; ++k) {
-                    float2 x, f;
-                    token(k, x, f);
-                    const Gate2 gate = gate_of(f, low, rest);
-                    h = __ffma2_rn(gate.a, h, __fmul2_rn(gate.u, x));
-                    if (kEnds) {
-                        P = __fmul2_rn(P, gate.a);
-                        continue;
-                    }
-                    if (ch.active[0]) ch.store(Y + static_cast<size_t>(t + k) * p.dim, h);
-                    if (seq.end == t + k + 1) {
-                        store_final(row, h);
-                        seq = next;
-                        row = next_row;
-                        h = next_h;
-                        look_ahead();
-                    }
-                }
-            }
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-        }
-        if (kEnds) {
-            g.P[pair(j)] = above_zero(P);
-            g.h[pair(j)] = h;
-        }
-        cp_async_wait<0>();
-        __syncwarp();  // (the ring is filled anew)
+        const Span span = gate_span(p.seq, g, i);
+        walk_segment<T, kWords, kEnds, kStages>(p, g, reinterpret_cast<ScanTile<T, kWords>(*)[2]>(smem_f4), ch, tile, low,
+                                                rest, span, segment_length(g, span), j, global_pairs(g, i, tile), first_pass);
     }
     first_pass();  // (also warps without tokens: what follows waits for this kernel only)
+}
+
+// Both passes in one block, a segment to each of its warps: as many as have room for their copies.
+template <typename T>
+struct ScanBlock {
+    static constexpr int kWarps = sizeof(T) == 4 ? 8 : 16, kStages = sizeof(T) == 4 ? 3 : 2;
+};
+template <typename T, bool kWords>
+struct BlockSmem {
+    ScanTile<T, kWords> ring[ScanBlock<T>::kWarps][ScanBlock<T>::kStages][2];
+    BlockPairs<ScanBlock<T>::kWarps> pairs;
+};
+
+template <typename T, bool kWords>
+__global__ void __launch_bounds__(32 * ScanBlock<T>::kWarps, 1) gate_block_kernel(const GateArgs p, const GateCut g) {
+    extern __shared__ float4 smem_f4[];
+    constexpr int kWarps = ScanBlock<T>::kWarps, kStages = ScanBlock<T>::kStages;
+    auto &sm = *reinterpret_cast<BlockSmem<T, kWords> *>(smem_f4);
+    const int warp = threadIdx.x >> 5, tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
+    const Lane<T, kWords> ch(tile, threadIdx.x & 31, p.dim);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    keep_empty(p, ch, slot * kWarps + warp, g.width * kWarps);
+    for (int i = slot; i < g.spans; i += g.width) {
+        const Span span = gate_span(p.seq, g, i);
+        const int length = segment_length(g, span);
+        const GatePairs pairs = sm.pairs.view();
+        walk_segment<T, kWords, true, kStages>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, [] {});
+        __syncthreads();
+        walk_segment<T, kWords, false, kStages>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, [] {});
+        __syncthreads();
+    }
 }
 
 template <typename T, bool kWords, int kWarps>
@@ -181,16 +226,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? 5 : 2) gate_ring_ke
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
     T *const Y = static_cast<T *>(p.out);
-    auto init_of = [&](int seq) {
-        const long long row = seq_row(q, seq);
-        return ch.floats(p.init != nullptr && seq_live(q, seq, row) ? p.init + row * p.dim : nullptr, 0.0f);
-    };
-    auto store_final = [&](int seq, float2 h) {
-        const long long row = seq_row(q, seq);
-        if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
-    };
-    if (p.final_state != nullptr)  // sequences without tokens keep their starting states
-        for_empty_sequences(q, slot * kWarps + warp, g.width * kWarps, [&](int s) { store_final(s, init_of(s)); });
+    keep_empty(p, ch, slot * kWarps + warp, g.width * kWarps);
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(q, g, i);
         constexpr int kTurn = kWarps * kGateGroup;  // tokens of a round
@@ -250,13 +286,17 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? 5 : 2) gate_ring_ke
 #pragma unroll 1
                 for (int k = 0; k < kGateGroup && t + k < span.hi; ++k) {
                     if (at.end <= t + k) at = seq_at(q, t + k);
-                    if (at.start == t + k) h = init_of(at.seq);
+                    if (at.start == t + k) {
+                        long long from;
+                        seq_rows(q, at.seq, &from);
+                        h = init_of(p, ch, from);
+                    }
                     float2 x, f;
                     token(k, x, f);
                     const Gate2 gate = gate_of(f, low, rest);
                     h = __ffma2_rn(gate.a, h, __fmul2_rn(gate.u, x));
                     if (ch.active[0]) ch.store(Y + static_cast<size_t>(t + k) * p.dim, h);
-                    if (at.end == t + k + 1) store_final(at.seq, h);
+                    if (at.end == t + k + 1) store_final(p, ch, seq_row(q, at.seq), h);
                 }
                 if (more) sm.hand.give(next, h);
             }
@@ -336,7 +376,9 @@ __global__ void __launch_bounds__(kTokenThreads) gate_token_kernel(const GateArg
 
 template <typename T, bool kWords>
 cudaError_t launch_words(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
-    constexpr size_t kSmem = sizeof(ScanSmem<T, kWords>);
+    constexpr size_t kSmem = kStages * 2 * sizeof(ScanTile<T, kWords>);
+    if (g.block != 0)
+        return launch_gate<gate_block_kernel<T, kWords>>(g.block, sizeof(BlockSmem<T, kWords>), g, 1, false, stream, a, g);
     if (g.ring == 4)
         return launch_gate<gate_ring_kernel<T, kWords, 4>>(4, sizeof(RingSmem<T, kWords, 4>), g, 1, false, stream, a, g);
     if (g.ring == 8)
@@ -366,6 +408,10 @@ cudaError_t launch_token_rows(const GateArgs &a, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
+int block_of(const GateArgs &a) {
+    return a.io == IoType::kF32 ? ScanBlock<float>::kWarps : ScanBlock<__nv_bfloat16>::kWarps;
+}
+
 template <typename T>
 cudaError_t launch_token_type(const GateArgs &a, cudaStream_t stream) {
     constexpr int kWord = 16 / static_cast<int>(sizeof(T));
@@ -377,7 +423,7 @@ cudaError_t launch_token_type(const GateArgs &a, cudaStream_t stream) {
 
 }  // namespace
 
-GateCut gate_cut(const SeqArgs &q, int dim, int parts) {
+GateCut gate_cut(const SeqArgs &q, int dim, int block, int parts) {
     GateCut g{};
     g.tiles = (dim + kGateChannels - 1) / kGateChannels;
     constexpr int kShort = 64;  // rows shorter than this share a span
@@ -394,12 +440,18 @@ GateCut gate_cut(const SeqArgs &q, int dim, int parts) {
     // 38 in eight segments; 4 x 2048 x 4096, 256 blocks: 42 and 64), of eight warps up to two blocks an SM (those 256: 50
     // with four; 6 x 2048 x 4096, 384 blocks: 75 with eight and 58 with four). With fewer, one wave of eight warps an SM
     // (16384 x 4096 packed: 119 to 121 us in 16 or 18 segments, 147 in 24), of 32 tokens at least (512 x 4096: 10 us in
-    // 16, 14 in 32). Rows of fewer
-    // than 256 tokens, or 128 where there are few: a warp each (8 x 128 x 4096: 8.9 us, 10.9 in rings).
+    // 16, 14 in 32). Many rows of fewer than 256 tokens: a warp each (8 x 128 x 4096: 8.9 us, 10.9 in rings).
     g.segments = 1;
     if (g.length >= 128) {
         if (warps * 5 >= sms * 4) g.ring = g.length < 256 ? 0 : warps > 2 * sms ? 4 : 8;
         else g.segments = static_cast<int>(std::min<int64_t>(std::max<int64_t>(sms * 81 / 10 / warps, 1), (g.length + 31) / 32));
+    }
+    // Short rows in one block and launch: as long as a warp has a group or two (192 x 512: 6.7 us, 7.1 in two kernels;
+    // 384: 9.0 and 8.2, with three microseconds less on the host; 1024: 16 and 9.8), and in the place of rings of an SM
+    // each up to four (4 x 256 x 2048: 7.9 us, 10.5 in rings; 1024: 19 and 21).
+    if (g.length >= 64 && warps <= sms && g.length <= (g.ring != 0 ? 64 : 24) * block) {
+        g.ring = 0;
+        g.block = g.segments = block;
     }
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(parts, (int64_t(1) << 30) / g.tiles) / g.segments);
     g.width = static_cast<int>(std::min<int64_t>(g.spans, most));
@@ -407,11 +459,11 @@ GateCut gate_cut(const SeqArgs &q, int dim, int parts) {
 }
 
 size_t gated_recurrence_workspace(const GateArgs &a) {
-    return a.dim == 0 ? 0 : 3 * gate_pairs(gate_cut(a.seq, a.dim, INT_MAX)) * sizeof(float2);
+    return a.dim == 0 ? 0 : 3 * gate_pairs(gate_cut(a.seq, a.dim, block_of(a), INT_MAX)) * sizeof(float2);
 }
 
 cudaError_t launch_gated_recurrence(const GateArgs &a, void *workspace, cudaStream_t stream) {
-    GateCut g = gate_cut(a.seq, a.dim, INT_MAX);
+    GateCut g = gate_cut(a.seq, a.dim, block_of(a), INT_MAX);
     g.P = static_cast<float2 *>(workspace);
     g.h = g.P + gate_pairs(g);
     g.start = g.h + gate_pairs(g);

@@ -20,179 +20,242 @@ namespace {
 
 constexpr int kMaxParts = 1024;  // partial sums of d_bound per channel
 
-template <typename T, bool kWords, bool kEnds>
-struct GradSmem {
-    static constexpr int kStages = sizeof(T) == 4 ? 3 : 5;  // groups in use and under way
-    static constexpr int kTensors = kEnds ? 2 : 4;          // f, dy; x, and y of the token before
-    GateTile<T, kGateGroup, kWords> ring[kStages][kTensors];
-};
+template <typename T, bool kWords>
+using GradTile = GateTile<T, kGateGroup, kWords>;
 
-// kEnds: the first pass over segments (all but a span's first).
+// Groups in use and under way, of the tensors f, dy; x, and y of the token before.
+template <typename T>
+constexpr int kStages = sizeof(T) == 4 ? 3 : 5;
+
+template <typename T, bool kWords>
+__device__ __forceinline__ float2 state_row(const GateGradArgs &p, const Lane<T, kWords> &ch, const float *base, int seq) {
+    return ch.floats(base != nullptr ? base + static_cast<size_t>(seq) * p.dim : nullptr, 0.0f);
+}
+template <typename T, bool kWords>
+__device__ __forceinline__ void store_dinit(const GateGradArgs &p, const Lane<T, kWords> &ch, int seq, float2 c) {
+    if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
+}
+// Sequences without tokens: the gradient passes through; warp of warps with the same channels.
+template <typename T, bool kWords>
+__device__ __forceinline__ void pass_empty(const GateGradArgs &p, const Lane<T, kWords> &ch, int warp, int warps) {
+    if (p.dinit != nullptr)
+        for_empty_sequences(p.seq, warp, warps, [&](int s) { store_dinit(p, ch, s, state_row(p, ch, p.dfinal, s)); });
+}
+
+// A warp walks segment j of a span. kEnds: the first pass. first_pass(): it is through; nothing of it is read before.
+// dlow: sum of da (1 - a).
+template <typename T, bool kWords, bool kEnds, int kStages, int kTensors, typename Wait>
+__device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCut &g, GradTile<T, kWords> (*ring)[kTensors],
+                                             const Lane<T, kWords> &ch, int tile, float2 low, float2 rest, Span span,
+                                             int length, int j, const GatePairs &pairs, float2 &dlow, Wait &&first_pass) {
+    const SeqArgs &q = p.seq;
+    const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
+                   *const F = static_cast<const T *>(p.f), *const H = static_cast<const T *>(p.y);
+    T *const DX = static_cast<T *>(p.dx), *const DF = static_cast<T *>(p.df);
+    const int s0 = span.lo + min(static_cast<long long>(j) * length, static_cast<long long>(max(span.hi - span.lo, 0)));
+    const int s1 = min(static_cast<long long>(s0) + length, static_cast<long long>(span.hi));
+    if (s0 >= s1) return;
+    int end = s1;
+    SeqAt seq = seq_at(q, kEnds ? s0 : s1 - 1);
+    if (kEnds) {
+        if (seq.start >= s0) return;  // no sequence enters the segment
+        end = min(s1, seq.end);
+    }
+    auto copy = [&](int hi, int stage) {
+        const int t = hi - kGateGroup;
+        if (hi > s0) {
+            copy_tile(ring[stage][0], F, t, s0, s1, p.dim, tile);
+            copy_tile(ring[stage][1], DY, t, s0, s1, p.dim, tile);
+            if constexpr (!kEnds) {
+                copy_tile(ring[stage][2], X, t, s0, s1, p.dim, tile);
+                copy_tile(ring[stage][3], H, t - 1, span.lo, s1, p.dim, tile);
+            }
+        }
+        cp_async_commit();
+    };
+    for (int k = 0; k < kStages - 1; ++k) copy(end - k * kGateGroup, k);
+    first_pass();
+    float2 c = both(0.0f), P = both(1.0f);
+    if (seq.end <= end) {  // (== unless the offsets descend)
+        c = state_row(p, ch, p.dfinal, seq.seq);
+    } else if (!kEnds && j + 1 < g.segments) {  // what comes from the segments behind
+        int k = min(max(seq.end - 1 - span.lo, 0) / length, g.segments - 1);
+        c = pairs.h(k);
+        for (--k; k > j; --k) c = __ffma2_rn(pairs.P(k), c, pairs.h(k));
+    }
+    SeqAt next{0, 0, 0};
+    float2 next_c = both(0.0f), first_h = both(0.0f);
+    auto look_ahead = [&] {  // this sequence's starting state, and the sequence before it
+        if (kEnds || seq.start < s0) return;
+        first_h = state_row(p, ch, p.init, seq.seq);
+        if (seq.start == s0) return;
+        next = seq_before(q, seq);
+        next_c = state_row(p, ch, p.dfinal, next.seq);
+    };
+    look_ahead();
+    int stage = 0;
+    for (int hi = end; hi > s0; hi -= kGateGroup) {
+        cp_async_wait<kStages - 2>();
+        __syncwarp();
+        copy(hi - (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
+        // token hi - 1 - k of a tensor
+        auto load = [&](int which, const T *base, int k, int back) {
+            return ring[stage][which].at(kGateGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
+        };
+        if (hi - kGateGroup >= s0 && (kEnds || seq.start < hi - kGateGroup)) {
+            if constexpr (kEnds) {
+                float2 a[kGateGroup], b[kGateGroup];
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k) {
+                    a[k] = gate_of(load(0, F, k, 0), low, rest).a;
+                    b[k] = __fmul2_rn(a[k], load(1, DY, k, 0));
+                }
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k) {
+                    c = __ffma2_rn(a[k], c, b[k]);
+                    P = __fmul2_rn(P, a[k]);
+                }
+            } else {
+                float2 G[kGateGroup], u[kGateGroup], r[kGateGroup];
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k) {
+                    const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
+                    G[k] = gate.a;
+                    u[k] = gate.u;
+                    r[k] = gate.r;
+                }
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k) {
+                    const float2 v = __fadd2_rn(load(1, DY, k, 0), c);
+                    c = __fmul2_rn(G[k], v);
+                    G[k] = v;
+                }
+                T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k, dx -= p.dim, df -= p.dim) {
+                    const float2 x = load(2, X, k, 0), before = load(3, H, k, 1);
+                    const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
+                    const float2 w = __fmul2_rn(__fmul2_rn(G[k], diff), u[k]);
+                    dlow = __fadd2_rn(dlow, w);
+                    if (ch.active[0]) {
+                        ch.store(dx, __fmul2_rn(u[k], G[k]));
+                        ch.store(df, __fmul2_rn(w, r[k]));
+                    }
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int k = 0; k < kGateGroup && hi - 1 - k >= s0; ++k) {
+                const int t = hi - 1 - k;
+                const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
+                if constexpr (kEnds) {
+                    c = __ffma2_rn(gate.a, c, __fmul2_rn(gate.a, load(1, DY, k, 0)));
+                    P = __fmul2_rn(P, gate.a);
+                } else {
+                    const float2 G = __fadd2_rn(load(1, DY, k, 0), c);
+                    const bool begins = seq.start == t;
+                    const float2 x = load(2, X, k, 0), before = begins ? first_h : load(3, H, k, 1);
+                    const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
+                    const float2 w = __fmul2_rn(__fmul2_rn(G, diff), gate.u);
+                    dlow = __fadd2_rn(dlow, w);
+                    c = __fmul2_rn(gate.a, G);
+                    if (ch.active[0]) {
+                        ch.store(DX + static_cast<size_t>(t) * p.dim, __fmul2_rn(gate.u, G));
+                        ch.store(DF + static_cast<size_t>(t) * p.dim, __fmul2_rn(w, gate.r));
+                    }
+                    if (begins) {
+                        store_dinit(p, ch, seq.seq, c);
+                        seq = next;
+                        c = next_c;
+                        if (t > s0) look_ahead();
+                    }
+                }
+            }
+        }
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    if constexpr (kEnds) {
+        pairs.P(j) = above_zero(P);
+        pairs.h(j) = c;
+    }
+    cp_async_wait<0>();
+    __syncwarp();  // (the ring is filled anew)
+}
+
+// A segment to each warp. kEnds: the first pass over segments (all but a span's first).
 // part: [width x segments][dim] sums of d_bound, or null.
 template <typename T, bool kWords, bool kEnds>
 __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, const GateCut g, float *part) {
     extern __shared__ float4 smem_f4[];
-    auto &sm = *reinterpret_cast<GradSmem<T, kWords, kEnds> *>(smem_f4);
-    constexpr int kStages = GradSmem<T, kWords, kEnds>::kStages;
     dependents_may_launch();
-    const SeqArgs &q = p.seq;
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs + (kEnds ? 1 : 0), slot = blockIdx.x / g.tiles / segs;
-    const Lane<T, kWords> ch(tile, threadIdx.x, p.dim);
+    const Lane<T, kWords> ch(tile, threadIdx.x & 31, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
-    const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
-                   *const F = static_cast<const T *>(p.f), *const H = static_cast<const T *>(p.y);
-    T *const DX = static_cast<T *>(p.dx), *const DF = static_cast<T *>(p.df);
-    auto state_row = [&](const float *base, int seq) {
-        return ch.floats(base != nullptr ? base + static_cast<size_t>(seq) * p.dim : nullptr, 0.0f);
-    };
-    auto store_dinit = [&](int seq, float2 c) {
-        if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
-    };
     bool waited = kEnds;
-    auto first_pass = [&] {  // is through: nothing of it is read before
+    auto first_pass = [&] {
         if (!waited) wait_for_before();
         waited = true;
     };
-    if (!kEnds && p.dinit != nullptr)  // sequences without tokens: the gradient passes through
-        for_empty_sequences(q, slot * segs + j, g.width * segs, [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
-    float2 dlow = both(0.0f);  // sum of da (1 - a)
+    if (!kEnds) pass_empty(p, ch, slot * segs + j, g.width * segs);
+    float2 dlow = both(0.0f);
     for (int i = slot; i < g.spans; i += g.width) {
-        const Span span = gate_span(q, g, i);
-        const int length = segment_length(g, span);
-        const int s0 = span.lo + min(static_cast<long long>(j) * length, static_cast<long long>(max(span.hi - span.lo, 0)));
-        const int s1 = min(static_cast<long long>(s0) + length, static_cast<long long>(span.hi));
-        if (s0 >= s1) continue;
-        auto pair = [&](int k) { return ((static_cast<size_t>(i) * g.segments + k) * g.tiles + tile) * 32 + threadIdx.x; };
-        int end = s1;
-        SeqAt seq = seq_at(q, kEnds ? s0 : s1 - 1);
-        if (kEnds) {
-            if (seq.start >= s0) continue;  // no sequence enters the segment
-            end = min(s1, seq.end);
-        }
-        auto copy = [&](int hi, int stage) {
-            const int t = hi - kGateGroup;
-            if (hi > s0) {
-                copy_tile(sm.ring[stage][0], F, t, s0, s1, p.dim, tile);
-                copy_tile(sm.ring[stage][1], DY, t, s0, s1, p.dim, tile);
-                if constexpr (!kEnds) {
-                    copy_tile(sm.ring[stage][2], X, t, s0, s1, p.dim, tile);
-                    copy_tile(sm.ring[stage][3], H, t - 1, span.lo, s1, p.dim, tile);
-                }
-            }
-            cp_async_commit();
-        };
-        for (int k = 0; k < kStages - 1; ++k) copy(end - k * kGateGroup, k);
-        first_pass();
-        float2 c = both(0.0f), P = both(1.0f);
-        if (seq.end <= end) {  // (== unless the offsets descend)
-            c = state_row(p.dfinal, seq.seq);
-        } else if (!kEnds && j + 1 < g.segments) {  // what comes from the segments behind
-            int k = min(max(seq.end - 1 - span.lo, 0) / length, g.segments - 1);
-            c = g.h[pair(k)];
-            for (--k; k > j; --k) c = __ffma2_rn(g.P[pair(k)], c, g.h[pair(k)]);
-        }
-        SeqAt next{0, 0, 0};
-        float2 next_c = both(0.0f), first_h = both(0.0f);
-        auto look_ahead = [&] {  // this sequence's starting state, and the sequence before it
-            if (kEnds || seq.start < s0) return;
-            first_h = state_row(p.init, seq.seq);
-            if (seq.start == s0) return;
-            next = seq_before(q, seq);
-            next_c = state_row(p.dfinal, next.seq);
-        };
-        look_ahead();
-        int stage = 0;
-        for (int hi = end; hi > s0; hi -= kGateGroup) {
-            cp_async_wait<kStages - 2>();
-            __syncwarp();
-            copy(hi - (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
-            // token hi - 1 - k of a tensor
-            auto load = [&](int which, const T *base, int k, int back) {
-                return sm.ring[stage][which].at(kGateGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
-            };
-            if (hi - kGateGroup >= s0 && (kEnds || seq.start < hi - kGateGroup)) {
-                if constexpr (kEnds) {
-                    float2 a[kGateGroup], b[kGateGroup];
-#pragma unroll
-                    for (int k = 0; k < kGateGroup; ++k) {
-                        a[k] = gate_of(load(0, F, k, 0), low, rest).a;
-                        b[k] = __fmul2_rn(a[k], load(1, DY, k, 0));
-                    }
-#pragma unroll
-                    for (int k = 0; k < kGateGroup; ++k) {
-                        c = __ffma2_rn(a[k], c, b[k]);
-                        P = __fmul2_rn(P, a[k]);
-                    }
-                } else {
-                    float2 G[kGateGroup], u[kGateGroup], r[kGateGroup];
-#pragma unroll
-                    for (int k = 0; k < kGateGroup; ++k) {
-                        const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
-                        G[k] = gate.a;
-                        u[k] = gate.u;
-                        r[k] = gate.r;
-                    }
-#pragma unroll
-                    for (int k = 0; k < kGateGroup; ++k) {
-                        const float2 v = __fadd2_rn(load(1, DY, k, 0), c);
-                        c = __fmul2_rn(G[k], v);
-                        G[k] = v;
-                    }
-                    T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
-#pragma unroll
-                    for (int k = 0; k < kGateGroup; ++k, dx -= p.dim, df -= p.dim) {
-                        const float2 x = load(2, X, k, 0), before = load(3, H, k, 1);
-                        const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
-                        const float2 w = __fmul2_rn(__fmul2_rn(G[k], diff), u[k]);
-                        dlow = __fadd2_rn(dlow, w);
-                        if (ch.active[0]) {
-                            ch.store(dx, __fmul2_rn(u[k], G[k]));
-                            ch.store(df, __fmul2_rn(w, r[k]));
-                        }
-                    }
-                }
-            } else {
-#pragma unroll 1
-                for (int k = 0; k < kGateGroup && hi - 1 - k >= s0; ++k) {
-                    const int t = hi - 1 - k;
-                    const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
-                    if constexpr (kEnds) {
-                        c = __ffma2_rn(gate.a, c, __fmul2_rn(gate.a, load(1, DY, k, 0)));
-                        P = __fmul2_rn(P, gate.a);
-                    } else {
-                        const float2 G = __fadd2_rn(load(1, DY, k, 0), c);
-                        const bool begins = seq.start == t;
-                        const float2 x = load(2, X, k, 0), before = begins ? first_h : load(3, H, k, 1);
-                        const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
-                        const float2 w = __fmul2_rn(__fmul2_rn(G, diff), gate.u);
-                        dlow = __fadd2_rn(dlow, w);
-                        c = __fmul2_rn(gate.a, G);
-                        if (ch.active[0]) {
-                            ch.store(DX + static_cast<size_t>(t) * p.dim, __fmul2_rn(gate.u, G));
-                            ch.store(DF + static_cast<size_t>(t) * p.dim, __fmul2_rn(w, gate.r));
-                        }
-                        if (begins) {
-                            store_dinit(seq.seq, c);
-                            seq = next;
-                            c = next_c;
-                            if (t > s0) look_ahead();
-                        }
-                    }
-                }
-            }
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-        }
-        if constexpr (kEnds) {
-            g.P[pair(j)] = above_zero(P);
-            g.h[pair(j)] = c;
-        }
-        cp_async_wait<0>();
-        __syncwarp();  // (the ring is filled anew)
+        const Span span = gate_span(p.seq, g, i);
+        constexpr int kTensors = kEnds ? 2 : 4;
+        walk_segment<T, kWords, kEnds, kStages<T>, kTensors>(
+            p, g, reinterpret_cast<GradTile<T, kWords>(*)[kTensors]>(smem_f4), ch, tile, low, rest, span,
+            segment_length(g, span), j, global_pairs(g, i, tile), dlow, first_pass);
     }
-    first_pass();  // (also by warps without tokens: what follows waits for this kernel only)
+    first_pass();  // (also warps without tokens: what follows waits for this kernel only)
     if (!kEnds && part != nullptr)  // da (1 - a) = da (1 - bound) sigmoid(-f)
         ch.store_floats(part + static_cast<size_t>(slot * segs + j) * p.dim, make_float2(dlow.x / rest.x, dlow.y / rest.y));
+}
+
+// Both passes in one block, a segment to each of its warps: as many as have room for their copies.
+template <typename T>
+struct GradBlock {
+    static constexpr int kWarps = sizeof(T) == 4 ? 6 : 8, kStages = sizeof(T) == 4 ? 2 : 3;
+};
+template <typename T, bool kWords>
+struct GradBlockSmem {
+    GradTile<T, kWords> ring[GradBlock<T>::kWarps][GradBlock<T>::kStages][4];
+    BlockPairs<GradBlock<T>::kWarps> pairs;
+};
+
+// part: [width][dim] sums of d_bound, or null.
+template <typename T, bool kWords>
+__global__ void __launch_bounds__(32 * GradBlock<T>::kWarps, 1) gate_grad_block_kernel(const GateGradArgs p, const GateCut g,
+                                                                                  float *part) {
+    extern __shared__ float4 smem_f4[];
+    constexpr int kWarps = GradBlock<T>::kWarps, kStages = GradBlock<T>::kStages;
+    auto &sm = *reinterpret_cast<GradBlockSmem<T, kWords> *>(smem_f4);
+    dependents_may_launch();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
+    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    pass_empty(p, ch, slot * kWarps + warp, g.width * kWarps);
+    float2 dlow = both(0.0f);
+    for (int i = slot; i < g.spans; i += g.width) {
+        const Span span = gate_span(p.seq, g, i);
+        const int length = segment_length(g, span);
+        const GatePairs pairs = sm.pairs.view();
+        if (warp > 0)
+            walk_segment<T, kWords, true, kStages, 4>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs,
+                                                      dlow, [] {});
+        __syncthreads();
+        walk_segment<T, kWords, false, kStages, 4>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, dlow,
+                                                   [] {});
+        __syncthreads();
+    }
+    if (part != nullptr) {  // the block's sum, the warps' added in order
+        sm.pairs.h[warp][lane] = dlow;
+        __syncthreads();
+        if (warp == 0) {
+            float2 sum = sm.pairs.h[0][lane];
+            for (int w = 1; w < kWarps; ++w) sum = __fadd2_rn(sum, sm.pairs.h[w][lane]);
+            ch.store_floats(part + static_cast<size_t>(slot) * p.dim, make_float2(sum.x / rest.x, sum.y / rest.y));
+        }
+    }
 }
 
 constexpr int kRingGroup = 8;  // tokens of a group of a ring: what is kept of more does not fit beside four blocks
@@ -343,12 +406,16 @@ cudaError_t launch_words(const GateGradArgs &a, const GateCut &g, float *part, c
     if (g.ring == 8)
         return launch_gate<gate_grad_ring_kernel<T, kWords, 8>>(8, sizeof(GradRingSmem<T, kWords, 8>), g, 1, false, stream,
                            a, g, part);
+    if (g.block != 0)
+        return launch_gate<gate_grad_block_kernel<T, kWords>>(g.block, sizeof(GradBlockSmem<T, kWords>), g, 1, false, stream,
+                                                              a, g, part);
+    constexpr size_t kSmem = kStages<T> * sizeof(GradTile<T, kWords>);  // of one tensor
     if (g.segments > 1) {
-        const cudaError_t e = launch_gate<gate_grad_kernel<T, kWords, true>>(1, sizeof(GradSmem<T, kWords, true>), g,
+        const cudaError_t e = launch_gate<gate_grad_kernel<T, kWords, true>>(1, 2 * kSmem, g,
                                           g.segments - 1, false, stream, a, g, part);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate<gate_grad_kernel<T, kWords, false>>(1, sizeof(GradSmem<T, kWords, false>), g, g.segments,
+    return launch_gate<gate_grad_kernel<T, kWords, false>>(1, 4 * kSmem, g, g.segments,
                        gate_behind(g), stream, a, g, part);
 }
 
@@ -360,14 +427,20 @@ cudaError_t launch_type(const GateGradArgs &a, const GateCut &g, float *part, cu
     return launch_words<T, false>(a, g, part, stream);
 }
 
-GateCut cut_of(const GateGradArgs &a) { return gate_cut(a.seq, a.dim, a.want_dbound ? kMaxParts : INT_MAX); }
+GateCut cut_of(const GateGradArgs &a) {
+    return gate_cut(a.seq, a.dim, a.io == IoType::kF32 ? GradBlock<float>::kWarps : GradBlock<__nv_bfloat16>::kWarps,
+                    a.want_dbound ? kMaxParts : INT_MAX);
+}
+
+// Partial sums of d_bound.
+int parts_of(const GateCut &g) { return g.width * (g.block != 0 ? 1 : g.segments); }
 
 }  // namespace
 
 size_t gated_recurrence_grad_workspace(const GateGradArgs &a) {
     if (a.dim == 0) return 0;
     const GateCut g = cut_of(a);
-    const size_t parts = static_cast<size_t>(g.width) * g.segments;
+    const size_t parts = parts_of(g);
     return 2 * gate_pairs(g) * sizeof(float2) + (a.want_dbound && parts > 1 ? parts * a.dim * sizeof(float) : 0);
 }
 
@@ -375,7 +448,7 @@ cudaError_t launch_gated_recurrence_grad(const GateGradArgs &a, void *workspace,
     GateCut g = cut_of(a);
     g.P = static_cast<float2 *>(workspace);
     g.h = g.P + gate_pairs(g);
-    const int parts = g.width * g.segments;
+    const int parts = parts_of(g);
     float *part = a.dbound == nullptr ? nullptr : parts > 1 ? reinterpret_cast<float *>(g.h + gate_pairs(g)) : a.dbound;
     cudaError_t e;
     switch (a.io) {

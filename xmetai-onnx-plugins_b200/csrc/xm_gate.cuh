@@ -16,7 +16,8 @@
 // With fewer rows, a row is cut into segments of a warp each. A first pass walks the
 // segments that a sequence leaves, from zero, and keeps h and P at the segment's end;
 // the second joins these pairs from the sequence's start up to its own segment and
-// walks with the true start.
+// walks with the true start. Short rows do both in one block, behind one launch, long
+// ones in two kernels.
 #pragma once
 
 #include <algorithm>
@@ -61,7 +62,8 @@ struct GateCut {
     int spans, length;  // length: tokens of a span; with cu it is [cu[0], cu[units])
     int width;          // spans walked at the same time
     int segments;       // of a span
-    int ring;           // warps of the block that shares a span (segments is 1); 0: a segment to each warp
+    int ring;           // warps of a block that take a span's groups in turn (segments is 1), or 0
+    int block;          // warps of a block that shares a span in segments, or 0; without both a segment to each warp
     int tiles;          // groups of channels
     float2 *P, *h, *start;  // [spans][segments][tiles][32]: the pairs, and the state that a leaving sequence started from
 };
@@ -81,7 +83,28 @@ __device__ __forceinline__ int segment_length(const GateCut &g, Span s) {
     return max((n + kGateGroup - 1) / kGateGroup * kGateGroup, kGateGroup);
 }
 
-// The sequence that holds a token: [start, end) of sequence seq.
+// First packed sequence that starts behind t (units: none). A warp looks at 32 offsets at a time: a round of loads for up
+// to 32 sequences, two for a thousand, where halving takes one for every doubling.
+__device__ __forceinline__ int seq_first_behind(const SeqArgs &q, int t) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = q.units;  // it is one of [lo, hi]
+    while (hi - lo > 32) {
+        const int step = (hi - lo - 1) / 32 + 1;  // the last of every `step` offsets
+        const long long at = lo + (lane + 1LL) * step - 1;
+        const unsigned behind = __ballot_sync(kFullMask, at < hi && seq_start(q, static_cast<int>(min(at, hi - 1LL))) > t);
+        if (behind != 0) {
+            const int k = __ffs(behind) - 1;
+            hi = lo + (k + 1) * step - 1;
+            lo += k * step;
+        } else {
+            lo += (hi - lo) / step * step;
+        }
+    }
+    const unsigned behind = __ballot_sync(kFullMask, lo + lane < hi && seq_start(q, min(lo + lane, q.units)) > t);
+    return behind != 0 ? lo + __ffs(behind) - 1 : hi;
+}
+
+// The sequence that holds a token: [start, end) of sequence seq. Called by whole warps.
 struct SeqAt {
     int seq, start, end;
 };
@@ -90,7 +113,7 @@ __device__ __forceinline__ SeqAt seq_at(const SeqArgs &q, int t) {
         const int i = t / q.seqlen;
         return SeqAt{i, i * q.seqlen, (i + 1) * q.seqlen};
     }
-    const int next = max(seq_first_from(q, t + 1), 1);  // first that starts behind t
+    const int next = max(seq_first_behind(q, t), 1);
     return SeqAt{next - 1, seq_start(q, next - 1), seq_start(q, next)};
 }
 // The same for the token behind, or before, a sequence that is known.
@@ -107,6 +130,14 @@ __device__ __forceinline__ SeqAt seq_before(const SeqArgs &q, const SeqAt &s) {
         if (start < s.start) return SeqAt{s.seq - 1, start, s.start};
     }
     return seq_at(q, s.start - 1);
+}
+
+// State row of sequence i, and in *start the one that it starts from (-1: none). Both of its entries are asked for at once.
+__device__ __forceinline__ long long seq_rows(const SeqArgs &q, int i, long long *start) {
+    const bool live = q.live == nullptr || index_at(q.live, q.live64, i) != 0;
+    const long long row = seq_row(q, i);
+    *start = live ? row : -1;
+    return row;
 }
 
 // Calls f(sequence) for the sequences without tokens, shared out over `warps` warps with the same channels.
@@ -221,10 +252,31 @@ __device__ __forceinline__ void copy_tile(GateTile<T, kRows, kWords> &dst, const
     }
 }
 
-// The cut of a call (without pointers). parts: at most as many warps per tile.
-GateCut gate_cut(const SeqArgs &q, int dim, int parts);
+// What the first pass leaves of a span's segments, for one lane: in global memory, or in a block's shared memory.
+struct GatePairs {
+    float2 *P_, *h_, *start_;
+    size_t base, step;
+    __device__ __forceinline__ float2 &P(int k) const { return P_[base + k * step]; }
+    __device__ __forceinline__ float2 &h(int k) const { return h_[base + k * step]; }
+    __device__ __forceinline__ float2 &start(int k) const { return start_[base + k * step]; }
+};
+__device__ __forceinline__ GatePairs global_pairs(const GateCut &g, int span, int tile) {
+    const size_t base = (static_cast<size_t>(span) * g.segments * g.tiles + tile) * 32 + (threadIdx.x & 31);
+    return GatePairs{g.P, g.h, g.start, base, static_cast<size_t>(g.tiles) * 32};
+}
+template <int kWarps>
+struct BlockPairs {
+    float2 P[kWarps][32], h[kWarps][32], start[kWarps][32];
+    __device__ __forceinline__ GatePairs view() {
+        return GatePairs{&P[0][0], &h[0][0], &start[0][0], static_cast<size_t>(threadIdx.x & 31), 32};
+    }
+};
+
+// The cut of a call (without pointers). block: warps of a block of the operator's own; parts: at most as many partial
+// sums per tile.
+GateCut gate_cut(const SeqArgs &q, int dim, int block, int parts);
 inline size_t gate_pairs(const GateCut &g) {  // elements of each of P, h and start
-    return g.segments > 1 ? static_cast<size_t>(g.spans) * g.segments * g.tiles * 32 : 0;
+    return g.segments > 1 && g.block == 0 ? static_cast<size_t>(g.spans) * g.segments * g.tiles * 32 : 0;
 }
 
 // Whether the second pass's blocks may begin while the first ends: worth a microsecond where segments are short (512 x
