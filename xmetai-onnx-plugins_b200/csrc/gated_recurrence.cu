@@ -13,12 +13,16 @@
 namespace xm {
 namespace {
 
-constexpr int kStages = 6;      // groups of x and f in use and under way, of a warp with a row or segment
+constexpr int kStages = 3;  // groups of x and f in use and under way, of a warp with a row or segment
 // And of a warp in a ring. Of four: what leaves an SM as many blocks as its registers do (16-bit types: five; 8 x 2048 x
 // 4096 takes 71 us, and 83 with three stages and four blocks), or its copies (float32: two; 8 x 1024 x 4096 takes 70 us,
 // and 78 with two stages and four blocks). Of eight, an SM has two at most.
 template <typename T, int kWarps>
 constexpr int kRingStages = kWarps == 8 || sizeof(T) == 4 ? 3 : 2;
+
+// Segments of an SM: one wave that fills it, and leaves room for the next pass (16384 x 4096 packed takes 111 us; with six
+// stages, of which nine fit an SM, 119 at best).
+constexpr int kPerSm = 12;
 
 template <typename T, bool kWords>
 using ScanTile = GateTile<T, kGateGroup, kWords>;
@@ -423,7 +427,7 @@ cudaError_t launch_token_type(const GateArgs &a, cudaStream_t stream) {
 
 }  // namespace
 
-GateCut gate_cut(const SeqArgs &q, int dim, int block, int parts) {
+GateCut gate_cut(const SeqArgs &q, int dim, int block, int per_sm, int parts) {
     GateCut g{};
     g.tiles = (dim + kGateChannels - 1) / kGateChannels;
     constexpr int kShort = 64;  // rows shorter than this share a span
@@ -438,13 +442,12 @@ GateCut gate_cut(const SeqArgs &q, int dim, int block, int parts) {
     const int64_t warps = static_cast<int64_t>(g.spans) * g.tiles, sms = current_device_sm_count();
     // A row per block needs four fifths of the device's blocks to be the faster (8 x 2048 x 1024, 128 blocks: 34 us, and
     // 38 in eight segments; 4 x 2048 x 4096, 256 blocks: 42 and 64), of eight warps up to two blocks an SM (those 256: 50
-    // with four; 6 x 2048 x 4096, 384 blocks: 75 with eight and 58 with four). With fewer, one wave of eight warps an SM
-    // (16384 x 4096 packed: 119 to 121 us in 16 or 18 segments, 147 in 24), of 32 tokens at least (512 x 4096: 10 us in
-    // 16, 14 in 32). Many rows of fewer than 256 tokens: a warp each (8 x 128 x 4096: 8.9 us, 10.9 in rings).
+    // with four; 6 x 2048 x 4096, 384 blocks: 75 with eight and 58 with four). With fewer, one wave of per_sm
+    // segments an SM, of 32 tokens at least (512 x 4096: 10 us in 16, 14 in 32). Many rows of fewer than 256 tokens: a warp each (8 x 128 x 4096: 8.9 us, 10.9 in rings).
     g.segments = 1;
     if (g.length >= 128) {
         if (warps * 5 >= sms * 4) g.ring = g.length < 256 ? 0 : warps > 2 * sms ? 4 : 8;
-        else g.segments = static_cast<int>(std::min<int64_t>(std::max<int64_t>(sms * 81 / 10 / warps, 1), (g.length + 31) / 32));
+        else g.segments = static_cast<int>(std::min<int64_t>(std::max<int64_t>(sms * per_sm / warps, 1), (g.length + 31) / 32));
     }
     // Short rows in one block and launch: as long as a warp has a group or two (192 x 512: 6.7 us, 7.1 in two kernels;
     // 384: 9.0 and 8.2, with three microseconds less on the host; 1024: 16 and 9.8), and in the place of rings of an SM
@@ -459,11 +462,11 @@ GateCut gate_cut(const SeqArgs &q, int dim, int block, int parts) {
 }
 
 size_t gated_recurrence_workspace(const GateArgs &a) {
-    return a.dim == 0 ? 0 : 3 * gate_pairs(gate_cut(a.seq, a.dim, block_of(a), INT_MAX)) * sizeof(float2);
+    return a.dim == 0 ? 0 : 3 * gate_pairs(gate_cut(a.seq, a.dim, block_of(a), kPerSm, INT_MAX)) * sizeof(float2);
 }
 
 cudaError_t launch_gated_recurrence(const GateArgs &a, void *workspace, cudaStream_t stream) {
-    GateCut g = gate_cut(a.seq, a.dim, block_of(a), INT_MAX);
+    GateCut g = gate_cut(a.seq, a.dim, block_of(a), kPerSm, INT_MAX);
     g.P = static_cast<float2 *>(workspace);
     g.h = g.P + gate_pairs(g);
     g.start = g.h + gate_pairs(g);

@@ -23,9 +23,13 @@ constexpr int kMaxParts = 1024;  // partial sums of d_bound per channel
 template <typename T, bool kWords>
 using GradTile = GateTile<T, kGateGroup, kWords>;
 
+// Segments of an SM: one wave, as many as it has room for (16384 x 4096 packed takes 187 us; with five stages, of which
+// five warps' fit, 206).
+constexpr int kPerSm = 8;
+
 // Groups in use and under way, of the tensors f, dy; x, and y of the token before.
 template <typename T>
-constexpr int kStages = sizeof(T) == 4 ? 3 : 5;
+constexpr int kStages = sizeof(T) == 4 ? 2 : 3;
 
 template <typename T, bool kWords>
 __device__ __forceinline__ float2 state_row(const GateGradArgs &p, const Lane<T, kWords> &ch, const float *base, int seq) {
@@ -429,7 +433,7 @@ cudaError_t launch_type(const GateGradArgs &a, const GateCut &g, float *part, cu
 
 GateCut cut_of(const GateGradArgs &a) {
     return gate_cut(a.seq, a.dim, a.io == IoType::kF32 ? GradBlock<float>::kWarps : GradBlock<__nv_bfloat16>::kWarps,
-                    a.want_dbound ? kMaxParts : INT_MAX);
+                    kPerSm, a.want_dbound ? kMaxParts : INT_MAX);
 }
 
 // Partial sums of d_bound.

@@ -272,9 +272,9 @@ struct BlockPairs {
     }
 };
 
-// The cut of a call (without pointers). block: warps of a block of the operator's own; parts: at most as many partial
-// sums per tile.
-GateCut gate_cut(const SeqArgs &q, int dim, int block, int parts);
+// The cut of a call (without pointers). block: warps of the operator's block that shares a row; per_sm: segments of a wave
+// on an SM; parts: at most as many partial sums per tile.
+GateCut gate_cut(const SeqArgs &q, int dim, int block, int per_sm, int parts);
 inline size_t gate_pairs(const GateCut &g) {  // elements of each of P, h and start
     return g.segments > 1 && g.block == 0 ? static_cast<size_t>(g.spans) * g.segments * g.tiles * 32 : 0;
 }
