@@ -415,7 +415,7 @@ xm_status xm_selective_state_update_fwd(const xm_selective_state_update_attrs *a
  *   h_t = a_t h_(t-1) + (1 - a_t) x_t,   y_t = h_t.
  * Types, sequences (cu_seqlens, state_indices, has_initial_state), states,
  * absent inputs, overlap and limits are those of the serving operators; the
- * states and lower_bound ([dim], at least 0 and below 1; empty: 0) are float32.
+ * states and lower_bound ([dim], 0 to 1; empty: 0) are float32.
  */
 
 /* GatedRecurrenceFn. Inputs (7, in order): x, f [batch, seqlen, dim],

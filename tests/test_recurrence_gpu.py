@@ -303,6 +303,28 @@ def test_grad_extreme_gates_and_infinities(xm, cuda):
     _close_grads(_grad(xm, cu, dy, x, f2, y, low, init, dl), want, low, init)
 
 
+@pytest.mark.parametrize("batch,seqlen,dim", [(1, 700, 70), (2, 100, 40), (160, 270, 9)])
+def test_lower_bounds_of_one(xm, cuda, batch, seqlen, dim):
+    """Such a channel keeps its state for good; its bound has a gradient, its inputs have (next to) none."""
+    g = gen(20)
+    x, f, low = inputs(g, batch, seqlen, dim, torch.float32)
+    ones = torch.arange(dim) % 3 == 1
+    low[ones] = 1.0
+    init, dl = normal(g, batch, dim), normal(g, batch, dim)
+    y, last = xm.GatedRecurrenceFn(dev(x), dev(f), dev(low), dev(init), output_final_state=1)
+    want = Q.recurrence(x, f, low, init)
+    close(y, *want[:2])
+    assert torch.equal(y[..., ones].cpu(), init[:, None, ones].expand(-1, seqlen, -1))
+    dy = normal(g, batch, seqlen, dim)
+    want = Q.recurrence_grad(dy, x, f, y.cpu(), low, init, None, dl)
+    # G is at most the sum of |dy| and |dl|, h - x at most 12: times 2^-60
+    most = 12 * (dy.abs().sum(1).max() + dl.abs().max()).double() * 2.0**-60
+    for v, b in want[:2]:
+        b[..., ones] += most
+    got = _grad(xm, None, dy, x, f, y.cpu(), low, init, dl)
+    _close_grads(got, want, low, init)
+
+
 def test_grad_misaligned(xm, cuda):
     g = gen(19)
     for dtype in DT.values():
@@ -529,6 +551,114 @@ def test_repeatable_bits(xm, cuda):
     want = _training_step(xm, p)
     for _ in range(20):
         assert not _differing(_training_step(xm, p), want)
+
+
+# ------------------------------------------------------------------ many and few rows, short and long
+
+# (batch, seqlen, dim) or (offsets, None, dim); a row's 64 channels are a warp's or a block's
+CUTS = {
+    "blocks of eight, words": (3, 300, 3264),
+    "blocks of eight, odd rows": (3, 300, 3267),
+    "blocks of four, words": (5, 260, 4000),
+    "blocks of four, odd rows": (5, 261, 3999),
+    "packed, blocks of eight": ([0, 0, 7, 8, 9, 128, 128, 256, 257, 530, 600], None, 9600),
+    "packed, blocks of eight, odd rows": ([3, 4, 100, 411], None, 9607),
+    "packed, blocks of four": ([0, 1, 130, 131, 330, 400], None, 19001),
+    "a block for each SM": (2, 500, 3904),
+    "a warp for each row": (3, 200, 3265),
+    "short rows of two sequences": (9, 32, 70),
+    "short rows, in turns": (290, 32, 64),
+    "segments of several rows": (2, 1200, 130),
+}
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("cut", CUTS)
+def test_every_cut(xm, cuda, dt, cut):
+    """Forward and backward, at sizes that are cut in every way there is; repeated, and from a captured graph."""
+    batch, seqlen, dim = CUTS[cut]
+    cu = batch if seqlen is None else None
+    if cu is not None:
+        batch, seqlen = 1, cu[-1] + 5
+    g = gen(dim + seqlen)
+    x, f, low = inputs(g, batch, seqlen, dim, DT[dt])
+    units = batch if cu is None else len(cu) - 1
+    init, dl = normal(g, units, dim), normal(g, units, dim)
+    hole = torch.full_like(x, 7.0)
+    y, bound, final, fb = Q.recurrence(x, f, low, init, cu, out=hole)
+    ys = y.to(DT[dt])
+    dy = normal(g, batch, seqlen, dim, dtype=DT[dt])
+    want = Q.recurrence_grad(dy, x, f, ys, low, init, cu, dl, dx=hole, df=hole)
+    c = None if cu is None else torch.tensor(cu).cuda()
+    a = [dev(t) for t in (x, f, low, init, ys, dy, dl)]
+    outs = [torch.full_like(a[0], 7.0) for _ in range(3)]
+
+    def run():
+        got = xm.GatedRecurrenceFn(a[0], a[1], a[2], a[3], c, output_final_state=1, out=outs[0])
+        return (*got, *xm.GatedRecurrenceGradFn(a[5], a[0], a[1], a[4], a[2], a[3], c, a[6],
+                                                out=(outs[1], outs[2], None, None)))
+
+    got = run()
+    close(got[0], y, bound)
+    close(got[1], final, fb)
+    _close_grads(got[2:], want, low, init)
+    first = [t.clone() for t in got]
+    assert all(torch.equal(u, v) for u, v in zip(run(), first))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = run()
+    for t in outs:
+        t.fill_(7.0)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(again, first))
+
+
+@pytest.mark.parametrize("dim", [9600, 19001])
+def test_infinities_in_rows_of_blocks(xm, cuda, dim):
+    """What is infinite or NaN lasts to its sequence's end and touches no other sequence or channel."""
+    g = gen(dim)
+    cu = [0, 140, 141, 400]
+    dy, x, f, _, low, init, dl = _grad_inputs(g, 1, 400, dim, torch.float32, cu)
+    f.clamp_(-10, 10)
+    x[0, 20, 3], x[0, 140, 4], x[0, 200, dim - 1] = float("inf"), float("nan"), -float("inf")
+    init[2, 5], init[0, 6] = float("inf"), float("nan")
+    y, bound, final, fb = Q.recurrence(x, f, low, init, cu)
+    c = torch.tensor(cu).cuda()
+    got, last = xm.GatedRecurrenceFn(dev(x), dev(f), dev(low), dev(init), c, output_final_state=1)
+    close(got, y, bound)
+    close(last, final, fb)
+    dy, x, f, y, low, init, dl = _grad_inputs(g, 1, 400, dim, torch.float32, cu)
+    f.clamp_(-10, 10)
+    y = Q.recurrence(x, f, low, init, cu)[0].float()
+    dy[0, 350, 3], dy[0, 100, dim - 1], dl[2, 64], dl[0, 70] = float("inf"), float("nan"), -float("inf"), float("nan")
+    want = Q.recurrence_grad(dy, x, f, y, low, init, cu, dl)
+    _close_grads(_grad(xm, cu, dy, x, f, y, low, init, dl), want, low, init)
+
+
+@pytest.mark.parametrize("seqlen,dim", [(256, 6), (130, 70)])
+def test_more_rows_than_partial_sums(xm, cuda, seqlen, dim):
+    """A row's results do not depend on how many rows there are, and the lower bounds' gradient is the sum over them."""
+    g = gen(61)
+    n, part = 2300, 460
+    x, f, low = (dev(t) for t in inputs(g, n, seqlen, dim, torch.bfloat16))
+    dy, init, dl = (dev(normal(g, *s, dtype=t)) for s, t in (((n, seqlen, dim), torch.bfloat16),
+                                                             ((n, dim), torch.float32), ((n, dim), torch.float32)))
+    y, last = xm.GatedRecurrenceFn(x, f, low, init, output_final_state=1)
+    got = xm.GatedRecurrenceGradFn(dy, x, f, y, low, init, None, dl)
+    total = torch.zeros(dim, dtype=torch.float64)
+    for i in range(0, n, part):
+        r = slice(i, i + part)
+        yr, lr = xm.GatedRecurrenceFn(x[r], f[r], low, init[r], output_final_state=1)
+        assert torch.equal(yr, y[r]) and torch.equal(lr, last[r])
+        gr = xm.GatedRecurrenceGradFn(dy[r], x[r], f[r], y[r], low, init[r], None, dl[r])
+        assert torch.equal(gr[0], got[0][r]) and torch.equal(gr[1], got[1][r]) and torch.equal(gr[3], got[3][r])
+        total += gr[2].cpu().double()
+    # the terms, G (h - x) sigmoid(-f) = df / ((1 - low) sigmoid(f)) with df rounded to bfloat16, are the same bits in both;
+    # a warp adds those of at most three rows in a row, and a column's sum fewer than 100 of such: below 1024 roundings
+    mag = (got[1].double().abs() / ((1 - low.double()) * torch.sigmoid(f.double()))).sum((0, 1)).cpu() * 1.01
+    close(got[2], total, 2 * 1024 * 2.0**-24 * mag)
 
 
 # ------------------------------------------------------------------ sizes and indices at the edges

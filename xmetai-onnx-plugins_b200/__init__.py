@@ -707,7 +707,7 @@ def GatedRecurrenceFn(x, f, lower_bound=None, initial_state=None, cu_seqlens=Non
     """Gated linear recurrence over sequences: h_t = a_t h_(t-1) + (1 - a_t) x_t with
     a_t = lower_bound + (1 - lower_bound) sigmoid(f_t); returns y = h.
 
-    x, f: [batch, seqlen, dim] in float32, bfloat16 or float16; lower_bound [dim], at least 0 and below 1, and the
+    x, f: [batch, seqlen, dim] in float32, bfloat16 or float16; lower_bound [dim], 0 to 1, and the
     states [sequences, dim] are float32. output_final_state, cu_seqlens, state_indices and has_initial_state work as in
     CausalConv1dFn.
     """

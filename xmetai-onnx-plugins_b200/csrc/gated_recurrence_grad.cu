@@ -31,6 +31,12 @@ constexpr int kPerSm = 8;
 template <typename T>
 constexpr int kStages = sizeof(T) == 4 ? 2 : 3;
 
+// 1 - bound, which da (1 - a), summed in place of da sigmoid(-f), is divided by in the end. A bound that training has brought
+// to 1 counts as 1 - 2^-60 (a is 1, dx and df are 2^-60 of what a bound of zero gives), so that it has a gradient too.
+__device__ __forceinline__ float2 rest_of(float2 low) {
+    return make_float2(low.x == 1.0f ? 0x1p-60f : 1.0f - low.x, low.y == 1.0f ? 0x1p-60f : 1.0f - low.y);
+}
+
 template <typename T, bool kWords>
 __device__ __forceinline__ float2 state_row(const GateGradArgs &p, const Lane<T, kWords> &ch, const float *base, int seq) {
     return ch.floats(base != nullptr ? base + static_cast<size_t>(seq) * p.dim : nullptr, 0.0f);
@@ -195,7 +201,7 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs + (kEnds ? 1 : 0), slot = blockIdx.x / g.tiles / segs;
     const Lane<T, kWords> ch(tile, threadIdx.x & 31, p.dim);
-    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
     bool waited = kEnds;
     auto first_pass = [&] {
         if (!waited) wait_for_before();
@@ -236,7 +242,7 @@ __global__ void __launch_bounds__(32 * GradBlock<T>::kWarps, 1) gate_grad_block_
     dependents_may_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
     const Lane<T, kWords> ch(tile, lane, p.dim);
-    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
     pass_empty(p, ch, slot * kWarps + warp, g.width * kWarps);
     float2 dlow = both(0.0f);
     for (int i = slot; i < g.spans; i += g.width) {
@@ -283,7 +289,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
     const Lane<T, kWords> ch(tile, lane, p.dim);
-    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
     const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
                    *const F = static_cast<const T *>(p.f), *const H = static_cast<const T *>(p.y);
     T *const DX = static_cast<T *>(p.dx), *const DF = static_cast<T *>(p.df);
