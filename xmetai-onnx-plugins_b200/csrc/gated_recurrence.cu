@@ -105,16 +105,17 @@ __device__ __forceinline__ void walk_segment(const GateArgs &p, const GateCut &g
             x = ring[stage][0].at(k, shift_of<T, kWords>(X, t + k, p.dim));
             f = ring[stage][1].at(k, shift_of<T, kWords>(F, t + k, p.dim));
         };
-        if (t + kGateGroup <= s1 && (kEnds || seq.end > t + kGateGroup)) {
-            float2 a[kGateGroup], b[kGateGroup];
+        float2 a[kGateGroup], b[kGateGroup];  // (of no meaning behind the segment's end)
 #pragma unroll
-            for (int k = 0; k < kGateGroup; ++k) {
-                float2 x, f;
-                token(k, x, f);
-                const Gate2 gate = gate_of(f, low, rest);
-                a[k] = gate.a;
-                b[k] = __fmul2_rn(gate.u, x);
-            }
+        for (int k = 0; k < kGateGroup; ++k) {
+            float2 x, f;
+            token(k, x, f);
+            const Gate2 gate = gate_of(f, low, rest);
+            a[k] = gate.a;
+            b[k] = __fmul2_rn(gate.u, x);
+        }
+        T *y = Y + static_cast<size_t>(t) * p.dim;
+        if (t + kGateGroup <= s1 && (kEnds || seq.end > t + kGateGroup)) {
 #pragma unroll
             for (int k = 0; k < kGateGroup; ++k) {
                 h = __ffma2_rn(a[k], h, b[k]);
@@ -122,29 +123,32 @@ __device__ __forceinline__ void walk_segment(const GateArgs &p, const GateCut &g
                 b[k] = h;
             }
             if (!kEnds && ch.active[0]) {
-                T *y = Y + static_cast<size_t>(t) * p.dim;
 #pragma unroll
                 for (int k = 0; k < kGateGroup; ++k, y += p.dim) ch.store(y, b[k]);
             }
         } else {
-#pragma unroll 1
-            for (int k = 0; k < kGateGroup && t + k < s1; ++k) {
-                float2 x, f;
-                token(k, x, f);
-                const Gate2 gate = gate_of(f, low, rest);
-                h = __ffma2_rn(gate.a, h, __fmul2_rn(gate.u, x));
-                if (kEnds) {
-                    P = __fmul2_rn(P, gate.a);
-                    continue;
+            const int last = min(kGateGroup, s1 - t);
+            for (int k0 = 0; k0 < last;) {  // the tokens of a sequence, k0 .. k1 - 1
+                const int end = kEnds ? last : seq.end - t, k1 = end > k0 && end < last ? end : last;
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k) {
+                    if (k < k0 || k >= k1) continue;
+                    h = __ffma2_rn(a[k], h, b[k]);
+                    if (kEnds) P = __fmul2_rn(P, a[k]);
+                    b[k] = h;
                 }
-                if (ch.active[0]) ch.store(Y + static_cast<size_t>(t + k) * p.dim, h);
-                if (seq.end == t + k + 1) {
-                    store_final(p, ch, row, h);
-                    seq = next;
-                    row = next_row;
-                    h = next_h;
-                    look_ahead();
-                }
+                k0 = k1;
+                if (kEnds || end != k1) continue;
+                store_final(p, ch, row, h);
+                seq = next;
+                row = next_row;
+                h = next_h;
+                look_ahead();
+            }
+            if (!kEnds && ch.active[0]) {
+#pragma unroll
+                for (int k = 0; k < kGateGroup; ++k, y += p.dim)
+                    if (k < last) ch.store(y, b[k]);
             }
         }
         stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -186,6 +190,7 @@ template <typename T>
 struct ScanBlock {
     static constexpr int kWarps = sizeof(T) == 4 ? 8 : 16, kStages = sizeof(T) == 4 ? 3 : 2;
 };
+constexpr int kShortest = 64;  // tokens of a row that a block shares (48 x 512: 4.8 us by a warp alone, 5.3)
 template <typename T, bool kWords>
 struct BlockSmem {
     ScanTile<T, kWords> ring[ScanBlock<T>::kWarps][ScanBlock<T>::kStages][2];
@@ -427,32 +432,39 @@ cudaError_t launch_token_type(const GateArgs &a, cudaStream_t stream) {
 
 }  // namespace
 
-GateCut gate_cut(const SeqArgs &q, int dim, int block, int per_sm, int parts) {
+GateCut gate_cut(const SeqArgs &q, int dim, int block, int shortest, int per_sm, int parts) {
     GateCut g{};
     g.tiles = (dim + kGateChannels - 1) / kGateChannels;
-    constexpr int kShort = 64;  // rows shorter than this share a span
+    // Rows shorter than this share a span, where that leaves an SM eight warps (5 x 6 x 547: 4.5 us apart, 10 together).
+    constexpr int kShort = 64;
+    const int64_t sms = current_device_sm_count();
     if (q.cu != nullptr) {
         g.spans = 1;
         g.length = q.tokens;
     } else {
-        const int64_t per = q.seqlen > 0 ? std::max<int64_t>(1, kShort / q.seqlen) : q.units;
+        const int64_t share = std::min<int64_t>(kShort / std::max<int64_t>(q.seqlen, 1),
+                                                static_cast<int64_t>(q.units) * g.tiles / (8 * sms));
+        const int64_t per = q.seqlen > 0 ? std::max<int64_t>(1, share) : q.units;
         g.length = static_cast<int>(std::min<int64_t>(per * q.seqlen, q.tokens));
         g.spans = g.length > 0 ? static_cast<int>((static_cast<int64_t>(q.tokens) + g.length - 1) / g.length) : 1;
     }
-    const int64_t warps = static_cast<int64_t>(g.spans) * g.tiles, sms = current_device_sm_count();
+    const int64_t warps = static_cast<int64_t>(g.spans) * g.tiles;
     // A row per block needs four fifths of the device's blocks to be the faster (8 x 2048 x 1024, 128 blocks: 34 us, and
     // 38 in eight segments; 4 x 2048 x 4096, 256 blocks: 42 and 64), of eight warps up to two blocks an SM (those 256: 50
     // with four; 6 x 2048 x 4096, 384 blocks: 75 with eight and 58 with four). With fewer, one wave of per_sm
-    // segments an SM, of 32 tokens at least (512 x 4096: 10 us in 16, 14 in 32). Many rows of fewer than 256 tokens: a warp each (8 x 128 x 4096: 8.9 us, 10.9 in rings).
+    // segments an SM, of 32 tokens at least (512 x 4096: 10 us in 16, 14 in 32), and no more than one join can go through
+    // in good time (32768 x 64: 31 us in 160, 34 in 128, 90 in 1024). Many rows of fewer than 256 tokens: a warp each
+    // (8 x 128 x 4096: 8.9 us, 10.9 in rings).
     g.segments = 1;
     if (g.length >= 128) {
         if (warps * 5 >= sms * 4) g.ring = g.length < 256 ? 0 : warps > 2 * sms ? 4 : 8;
-        else g.segments = static_cast<int>(std::min<int64_t>(std::max<int64_t>(sms * per_sm / warps, 1), (g.length + 31) / 32));
+        else g.segments = static_cast<int>(std::min<int64_t>({std::max<int64_t>(sms * per_sm / warps, 1),
+                                                              (int64_t(g.length) + 31) / 32, 192}));
     }
     // Short rows in one block and launch: as long as a warp has a group or two (192 x 512: 6.7 us, 7.1 in two kernels;
     // 384: 9.0 and 8.2, with three microseconds less on the host; 1024: 16 and 9.8), and in the place of rings of an SM
     // each up to four (4 x 256 x 2048: 7.9 us, 10.5 in rings; 1024: 19 and 21).
-    if (g.length >= 64 && warps <= sms && g.length <= (g.ring != 0 ? 64 : 24) * block) {
+    if (g.length >= shortest && warps <= sms && g.length <= (g.ring != 0 ? 64 : 24) * block) {
         g.ring = 0;
         g.block = g.segments = block;
     }
@@ -462,11 +474,11 @@ GateCut gate_cut(const SeqArgs &q, int dim, int block, int per_sm, int parts) {
 }
 
 size_t gated_recurrence_workspace(const GateArgs &a) {
-    return a.dim == 0 ? 0 : 3 * gate_pairs(gate_cut(a.seq, a.dim, block_of(a), kPerSm, INT_MAX)) * sizeof(float2);
+    return a.dim == 0 ? 0 : 3 * gate_pairs(gate_cut(a.seq, a.dim, block_of(a), kShortest, kPerSm, INT_MAX)) * sizeof(float2);
 }
 
 cudaError_t launch_gated_recurrence(const GateArgs &a, void *workspace, cudaStream_t stream) {
-    GateCut g = gate_cut(a.seq, a.dim, block_of(a), kPerSm, INT_MAX);
+    GateCut g = gate_cut(a.seq, a.dim, block_of(a), kShortest, kPerSm, INT_MAX);
     g.P = static_cast<float2 *>(workspace);
     g.h = g.P + gate_pairs(g);
     g.start = g.h + gate_pairs(g);

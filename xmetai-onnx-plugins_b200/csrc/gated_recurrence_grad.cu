@@ -20,16 +20,20 @@ namespace {
 
 constexpr int kMaxParts = 1024;  // partial sums of d_bound per channel
 
-template <typename T, bool kWords>
-using GradTile = GateTile<T, kGateGroup, kWords>;
+// Tokens of a group: in a ring, what is kept of more does not fit beside four blocks; in a segment 16 take as long, with
+// twice the instructions to fetch in short calls.
+constexpr int kGroup = 8;
 
-// Segments of an SM: one wave, as many as it has room for (16384 x 4096 packed takes 187 us; with five stages, of which
-// five warps' fit, 206).
-constexpr int kPerSm = 8;
+template <typename T, bool kWords>
+using GradTile = GateTile<T, kGroup, kWords>;
+
+// Segments of an SM: one wave, as many as it has room for (16384 x 4096 packed takes 188 us; with six stages, of which
+// eight fit, 197).
+template <typename T>
+constexpr int kPerSm = sizeof(T) == 4 ? 7 : 12;
 
 // Groups in use and under way, of the tensors f, dy; x, and y of the token before.
-template <typename T>
-constexpr int kStages = sizeof(T) == 4 ? 2 : 3;
+constexpr int kStages = 4;
 
 // 1 - bound, which da (1 - a), summed in place of da sigmoid(-f), is divided by in the end. A bound that training has brought
 // to 1 counts as 1 - 2^-60 (a is 1, dx and df are 2^-60 of what a bound of zero gives), so that it has a gradient too.
@@ -72,7 +76,7 @@ __device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCu
         end = min(s1, seq.end);
     }
     auto copy = [&](int hi, int stage) {
-        const int t = hi - kGateGroup;
+        const int t = hi - kGroup;
         if (hi > s0) {
             copy_tile(ring[stage][0], F, t, s0, s1, p.dim, tile);
             copy_tile(ring[stage][1], DY, t, s0, s1, p.dim, tile);
@@ -83,7 +87,7 @@ __device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCu
         }
         cp_async_commit();
     };
-    for (int k = 0; k < kStages - 1; ++k) copy(end - k * kGateGroup, k);
+    for (int k = 0; k < kStages - 1; ++k) copy(end - k * kGroup, k);
     first_pass();
     float2 c = both(0.0f), P = both(1.0f);
     if (seq.end <= end) {  // (== unless the offsets descend)
@@ -104,81 +108,76 @@ __device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCu
     };
     look_ahead();
     int stage = 0;
-    for (int hi = end; hi > s0; hi -= kGateGroup) {
+    for (int hi = end; hi > s0; hi -= kGroup) {
         cp_async_wait<kStages - 2>();
         __syncwarp();
-        copy(hi - (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
+        copy(hi - (kStages - 1) * kGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
         // token hi - 1 - k of a tensor
         auto load = [&](int which, const T *base, int k, int back) {
-            return ring[stage][which].at(kGateGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
+            return ring[stage][which].at(kGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
         };
-        if (hi - kGateGroup >= s0 && (kEnds || seq.start < hi - kGateGroup)) {
-            if constexpr (kEnds) {
-                float2 a[kGateGroup], b[kGateGroup];
+        const int last = min(kGroup, hi - s0);
+        if constexpr (kEnds) {
+            float2 a[kGroup], b[kGroup];  // (of no meaning before the segment)
 #pragma unroll
-                for (int k = 0; k < kGateGroup; ++k) {
-                    a[k] = gate_of(load(0, F, k, 0), low, rest).a;
-                    b[k] = __fmul2_rn(a[k], load(1, DY, k, 0));
+            for (int k = 0; k < kGroup; ++k) {
+                a[k] = gate_of(load(0, F, k, 0), low, rest).a;
+                b[k] = __fmul2_rn(a[k], load(1, DY, k, 0));
+            }
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) {
+                if (k >= last) continue;
+                c = __ffma2_rn(a[k], c, b[k]);
+                P = __fmul2_rn(P, a[k]);
+            }
+        } else {
+            float2 G[kGroup], u[kGroup], r[kGroup];  // (of no meaning before the segment)
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) {
+                const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
+                G[k] = gate.a;
+                u[k] = gate.u;
+                r[k] = gate.r;
+            }
+            T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
+            auto token = [&](int k, float2 before) {
+                const float2 x = load(2, X, k, 0);
+                const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
+                const float2 w = __fmul2_rn(__fmul2_rn(G[k], diff), u[k]);
+                dlow = __fadd2_rn(dlow, w);
+                if (ch.active[0]) {
+                    ch.store(dx, __fmul2_rn(u[k], G[k]));
+                    ch.store(df, __fmul2_rn(w, r[k]));
                 }
+            };
+            if (last == kGroup && seq.start < hi - kGroup) {
 #pragma unroll
-                for (int k = 0; k < kGateGroup; ++k) {
-                    c = __ffma2_rn(a[k], c, b[k]);
-                    P = __fmul2_rn(P, a[k]);
-                }
-            } else {
-                float2 G[kGateGroup], u[kGateGroup], r[kGateGroup];
-#pragma unroll
-                for (int k = 0; k < kGateGroup; ++k) {
-                    const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
-                    G[k] = gate.a;
-                    u[k] = gate.u;
-                    r[k] = gate.r;
-                }
-#pragma unroll
-                for (int k = 0; k < kGateGroup; ++k) {
+                for (int k = 0; k < kGroup; ++k) {
                     const float2 v = __fadd2_rn(load(1, DY, k, 0), c);
                     c = __fmul2_rn(G[k], v);
                     G[k] = v;
                 }
-                T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
 #pragma unroll
-                for (int k = 0; k < kGateGroup; ++k, dx -= p.dim, df -= p.dim) {
-                    const float2 x = load(2, X, k, 0), before = load(3, H, k, 1);
-                    const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
-                    const float2 w = __fmul2_rn(__fmul2_rn(G[k], diff), u[k]);
-                    dlow = __fadd2_rn(dlow, w);
-                    if (ch.active[0]) {
-                        ch.store(dx, __fmul2_rn(u[k], G[k]));
-                        ch.store(df, __fmul2_rn(w, r[k]));
+                for (int k = 0; k < kGroup; ++k, dx -= p.dim, df -= p.dim) token(k, load(3, H, k, 1));
+            } else {
+                for (int k0 = 0; k0 < last;) {  // the tokens of a sequence, k0 .. k1 - 1
+                    const int end = hi - seq.start, k1 = end > k0 && end < last ? end : last;
+#pragma unroll
+                    for (int k = 0; k < kGroup; ++k) {
+                        if (k < k0 || k >= k1) continue;
+                        const float2 v = __fadd2_rn(load(1, DY, k, 0), c);
+                        c = __fmul2_rn(G[k], v);
+                        G[k] = v;
+                        token(k, end == k1 && k == k1 - 1 ? first_h : load(3, H, k, 1));
+                        dx -= p.dim;
+                        df -= p.dim;
                     }
-                }
-            }
-        } else {
-#pragma unroll 1
-            for (int k = 0; k < kGateGroup && hi - 1 - k >= s0; ++k) {
-                const int t = hi - 1 - k;
-                const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
-                if constexpr (kEnds) {
-                    c = __ffma2_rn(gate.a, c, __fmul2_rn(gate.a, load(1, DY, k, 0)));
-                    P = __fmul2_rn(P, gate.a);
-                } else {
-                    const float2 G = __fadd2_rn(load(1, DY, k, 0), c);
-                    const bool begins = seq.start == t;
-                    const float2 x = load(2, X, k, 0), before = begins ? first_h : load(3, H, k, 1);
-                    const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
-                    const float2 w = __fmul2_rn(__fmul2_rn(G, diff), gate.u);
-                    dlow = __fadd2_rn(dlow, w);
-                    c = __fmul2_rn(gate.a, G);
-                    if (ch.active[0]) {
-                        ch.store(DX + static_cast<size_t>(t) * p.dim, __fmul2_rn(gate.u, G));
-                        ch.store(DF + static_cast<size_t>(t) * p.dim, __fmul2_rn(w, gate.r));
-                    }
-                    if (begins) {
-                        store_dinit(p, ch, seq.seq, c);
-                        seq = next;
-                        c = next_c;
-                        if (t > s0) look_ahead();
-                    }
+                    k0 = k1;
+                    if (end != k1) continue;
+                    store_dinit(p, ch, seq.seq, c);
+                    seq = next;
+                    c = next_c;
+                    if (hi - k1 > s0) look_ahead();
                 }
             }
         }
@@ -212,7 +211,7 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(p.seq, g, i);
         constexpr int kTensors = kEnds ? 2 : 4;
-        walk_segment<T, kWords, kEnds, kStages<T>, kTensors>(
+        walk_segment<T, kWords, kEnds, kStages, kTensors>(
             p, g, reinterpret_cast<GradTile<T, kWords>(*)[kTensors]>(smem_f4), ch, tile, low, rest, span,
             segment_length(g, span), j, global_pairs(g, i, tile), dlow, first_pass);
     }
@@ -224,8 +223,9 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
 // Both passes in one block, a segment to each of its warps: as many as have room for their copies.
 template <typename T>
 struct GradBlock {
-    static constexpr int kWarps = sizeof(T) == 4 ? 6 : 8, kStages = sizeof(T) == 4 ? 2 : 3;
+    static constexpr int kWarps = sizeof(T) == 4 ? 6 : 8, kStages = sizeof(T) == 4 ? 4 : 6;
 };
+constexpr int kShortest = 24;  // tokens of a row that a block shares (50 x 386 in float32: 9.7 us, by a warp alone 13.9)
 template <typename T, bool kWords>
 struct GradBlockSmem {
     GradTile<T, kWords> ring[GradBlock<T>::kWarps][GradBlock<T>::kStages][4];
@@ -268,13 +268,11 @@ __global__ void __launch_bounds__(32 * GradBlock<T>::kWarps, 1) gate_grad_block_
     }
 }
 
-constexpr int kRingGroup = 8;  // tokens of a group of a ring: what is kept of more does not fit beside four blocks
-
 template <typename T, bool kWords, int kWarps>
 struct GradRingSmem {
     static constexpr int kStages = kWarps == 8 && sizeof(T) == 2 ? 3 : 2;
     Ring<kWarps> hand;
-    GateTile<T, kRingGroup, kWords> ring[kWarps][kStages][4];  // f, dy, x, and y of the token before
+    GateTile<T, kGroup, kWords> ring[kWarps][kStages][4];  // f, dy, x, and y of the token before
 };
 
 // part: [width][dim] sums of d_bound, or null.
@@ -305,10 +303,10 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
     float2 dlow = both(0.0f);  // sum of da (1 - a)
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(q, g, i);
-        constexpr int kTurn = kWarps * kRingGroup;  // tokens of a round
-        const int first = span.hi - warp * kRingGroup;
+        constexpr int kTurn = kWarps * kGroup;  // tokens of a round
+        const int first = span.hi - warp * kGroup;
         auto copy = [&](int hi, int stage) {
-            const int t = hi - kRingGroup;
+            const int t = hi - kGroup;
             if (hi > span.lo) {
                 copy_tile(sm.ring[warp][stage][0], F, t, span.lo, span.hi, p.dim, tile);
                 copy_tile(sm.ring[warp][stage][1], DY, t, span.lo, span.hi, p.dim, tile);
@@ -326,25 +324,36 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
             copy(hi - (kStages - 1) * kTurn, stage == 0 ? kStages - 1 : stage - 1);  // read by all a round ago
             // token hi - 1 - k of a tensor
             auto load = [&](int which, const T *base, int k, int back) {
-                return sm.ring[warp][stage][which].at(kRingGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
+                return sm.ring[warp][stage][which].at(kGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
             };
             if (seq.start >= hi) seq = seq_at(q, hi - 1);
-            const bool more = hi - kRingGroup > span.lo;  // a group before
+            const bool more = hi - kGroup > span.lo;  // a group before
             const int next = warp + 1 == kWarps ? 0 : warp + 1;
-            // (whether a group takes and gives depends on hi alone, so that offsets that descend leave nobody waiting)
-            if (hi < span.hi && hi - kRingGroup >= span.lo && seq.end > hi && seq.start < hi - kRingGroup) {
-                float2 P[kRingGroup], G[kRingGroup], u[kRingGroup], r[kRingGroup];
+            float2 P[kGroup], G[kGroup], u[kGroup], r[kGroup];  // (of no meaning before the span)
 #pragma unroll
-                for (int k = 0; k < kRingGroup; ++k) {
-                    const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
-                    P[k] = gate.a;
-                    u[k] = gate.u;
-                    r[k] = gate.r;
+            for (int k = 0; k < kGroup; ++k) {
+                const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
+                P[k] = gate.a;
+                u[k] = gate.u;
+                r[k] = gate.r;
+            }
+            T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
+            auto token = [&](int k, float2 Gk, float2 before) {
+                const float2 x = load(2, X, k, 0);
+                const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
+                const float2 w = __fmul2_rn(__fmul2_rn(Gk, diff), u[k]);
+                dlow = __fadd2_rn(dlow, w);
+                if (ch.active[0]) {
+                    ch.store(dx, __fmul2_rn(u[k], Gk));
+                    ch.store(df, __fmul2_rn(w, r[k]));
                 }
+            };
+            // (whether a group takes and gives depends on hi alone, so that offsets that descend leave nobody waiting)
+            if (hi < span.hi && hi - kGroup >= span.lo && seq.end > hi && seq.start < hi - kGroup) {
                 // P[k] becomes the product up to and with token k, G[k] is run from zero
                 float2 c = both(0.0f);
 #pragma unroll
-                for (int k = 0; k < kRingGroup; ++k) {
+                for (int k = 0; k < kGroup; ++k) {
                     G[k] = __fadd2_rn(load(1, DY, k, 0), c);
                     c = __fmul2_rn(P[k], G[k]);
                     if (k > 0) P[k] = __fmul2_rn(P[k], P[k - 1]);
@@ -352,43 +361,32 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
                 const float2 start = sm.hand.take(warp);
                 if (!__all_sync(kFullMask, finite2(start))) {
 #pragma unroll
-                    for (int k = 0; k < kRingGroup; ++k) P[k] = above_zero(P[k]);
+                    for (int k = 0; k < kGroup; ++k) P[k] = above_zero(P[k]);
                 }
-                if (more) sm.hand.give(next, __ffma2_rn(P[kRingGroup - 1], start, c));
-                T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
+                if (more) sm.hand.give(next, __ffma2_rn(P[kGroup - 1], start, c));
 #pragma unroll
-                for (int k = 0; k < kRingGroup; ++k, dx -= p.dim, df -= p.dim) {
-                    const float2 Gk = k == 0 ? __fadd2_rn(G[0], start) : __ffma2_rn(P[k - 1], start, G[k]);
-                    const float2 x = load(2, X, k, 0), before = load(3, H, k, 1);
-                    const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
-                    const float2 w = __fmul2_rn(__fmul2_rn(Gk, diff), u[k]);
-                    dlow = __fadd2_rn(dlow, w);
-                    if (ch.active[0]) {
-                        ch.store(dx, __fmul2_rn(u[k], Gk));
-                        ch.store(df, __fmul2_rn(w, r[k]));
-                    }
-                }
+                for (int k = 0; k < kGroup; ++k, dx -= p.dim, df -= p.dim)
+                    token(k, k == 0 ? __fadd2_rn(G[0], start) : __ffma2_rn(P[k - 1], start, G[k]), load(3, H, k, 1));
             } else {
-                SeqAt at = seq;
+                const int last = min(kGroup, hi - span.lo);
                 float2 c = hi < span.hi ? sm.hand.take(warp) : both(0.0f);
-#pragma unroll 1
-                for (int k = 0; k < kRingGroup && hi - 1 - k >= span.lo; ++k) {
-                    const int t = hi - 1 - k;
-                    if (at.start > t) at = seq_at(q, t);
-                    if (at.end == t + 1) c = state_row(p.dfinal, at.seq);
-                    const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
-                    const float2 G = __fadd2_rn(load(1, DY, k, 0), c);
-                    const bool begins = at.start == t;
-                    const float2 x = load(2, X, k, 0), before = begins ? state_row(p.init, at.seq) : load(3, H, k, 1);
-                    const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
-                    const float2 w = __fmul2_rn(__fmul2_rn(G, diff), gate.u);
-                    dlow = __fadd2_rn(dlow, w);
-                    c = __fmul2_rn(gate.a, G);
-                    if (ch.active[0]) {
-                        ch.store(DX + static_cast<size_t>(t) * p.dim, __fmul2_rn(gate.u, G));
-                        ch.store(DF + static_cast<size_t>(t) * p.dim, __fmul2_rn(w, gate.r));
+                for (int k0 = 0; k0 < last;) {  // the tokens of a sequence, k0 .. k1 - 1
+                    if (seq.start > hi - 1 - k0) seq = seq_at(q, hi - 1 - k0);
+                    if (seq.end == hi - k0) c = state_row(p.dfinal, seq.seq);
+                    const int end = hi - seq.start, k1 = end > k0 && end < last ? end : last;
+                    float2 before = both(0.0f);
+                    if (end == k1) before = state_row(p.init, seq.seq);
+#pragma unroll
+                    for (int k = 0; k < kGroup; ++k) {
+                        if (k < k0 || k >= k1) continue;
+                        const float2 Gk = __fadd2_rn(load(1, DY, k, 0), c);
+                        c = __fmul2_rn(P[k], Gk);
+                        token(k, Gk, end == k1 && k == k1 - 1 ? before : load(3, H, k, 1));
+                        dx -= p.dim;
+                        df -= p.dim;
                     }
-                    if (begins) store_dinit(at.seq, c);
+                    if (end == k1) store_dinit(seq.seq, c);
+                    k0 = k1;
                 }
                 if (more) sm.hand.give(next, c);
             }
@@ -419,7 +417,7 @@ cudaError_t launch_words(const GateGradArgs &a, const GateCut &g, float *part, c
     if (g.block != 0)
         return launch_gate<gate_grad_block_kernel<T, kWords>>(g.block, sizeof(GradBlockSmem<T, kWords>), g, 1, false, stream,
                                                               a, g, part);
-    constexpr size_t kSmem = kStages<T> * sizeof(GradTile<T, kWords>);  // of one tensor
+    constexpr size_t kSmem = kStages * sizeof(GradTile<T, kWords>);  // of one tensor
     if (g.segments > 1) {
         const cudaError_t e = launch_gate<gate_grad_kernel<T, kWords, true>>(1, 2 * kSmem, g,
                                           g.segments - 1, false, stream, a, g, part);
@@ -437,9 +435,12 @@ cudaError_t launch_type(const GateGradArgs &a, const GateCut &g, float *part, cu
     return launch_words<T, false>(a, g, part, stream);
 }
 
+template <typename T>
+GateCut cut_of_type(const GateGradArgs &a) {
+    return gate_cut(a.seq, a.dim, GradBlock<T>::kWarps, kShortest, kPerSm<T>, a.want_dbound ? kMaxParts : INT_MAX);
+}
 GateCut cut_of(const GateGradArgs &a) {
-    return gate_cut(a.seq, a.dim, a.io == IoType::kF32 ? GradBlock<float>::kWarps : GradBlock<__nv_bfloat16>::kWarps,
-                    kPerSm, a.want_dbound ? kMaxParts : INT_MAX);
+    return a.io == IoType::kF32 ? cut_of_type<float>(a) : cut_of_type<__nv_bfloat16>(a);
 }
 
 // Partial sums of d_bound.

@@ -191,13 +191,13 @@ struct Lane {
     }
 };
 
-// A group's tokens of one tensor in shared memory, and the warp's copy that fills it. Rows that are not whole 16-byte
-// words are copied in 4-byte ones, from the word that holds their first element: a row of a 16-bit type may then begin
-// in the middle of its first word (`shift`).
+// A group's tokens of one tensor in shared memory, and the warp's copy that fills it, in 16-byte words. Rows of 16-bit types
+// that are not whole words are copied from the one that holds their first element, and lie behind `shift` others; those of
+// float32 are copied in 4-byte words.
 template <typename T, int kRows, bool kWords>
 struct GateTile {
     static constexpr bool kShifts = !kWords && sizeof(T) == 2;
-    T v[kRows][kGateChannels + (kShifts ? 2 : 0)];
+    alignas(16) T v[kRows][kGateChannels + (kShifts ? 8 : 0)];
     __device__ __forceinline__ float2 at(int row, int shift) const {
         const int c = 2 * (threadIdx.x & 31);
         if constexpr (kShifts) return make_float2(to_f32<T>(v[row][c + shift]), to_f32<T>(v[row][c + 1 + shift]));
@@ -209,9 +209,11 @@ struct GateTile {
 template <typename T, bool kWords>
 __device__ __forceinline__ int shift_of(const T *src, int t, int dim) {
     if (kWords || sizeof(T) != 2) return 0;
-    return (static_cast<int>(reinterpret_cast<uintptr_t>(src) >> 1) ^ (t & dim)) & 1;  // (a tile's first channel is even)
+    const unsigned first = static_cast<unsigned>(reinterpret_cast<uintptr_t>(src) >> 1);
+    return (first + static_cast<unsigned>(t) * static_cast<unsigned>(dim)) & 7;  // (a tile's first channel is a multiple of 8)
 }
-// Rows first .. first + kRows - 1 of a tensor's channels; those outside [lo, hi) are left out.
+// Rows first .. first + kRows - 1 of a tensor's channels; those outside [lo, hi) are left out. Reads nothing outside the
+// tensor's rows 0 .. hi - 1.
 template <typename T, int kRows, bool kWords>
 __device__ __forceinline__ void copy_tile(GateTile<T, kRows, kWords> &dst, const T *src, int first, int lo, int hi, int dim,
                                           int tile) {
@@ -233,21 +235,32 @@ __device__ __forceinline__ void copy_tile(GateTile<T, kRows, kWords> &dst, const
             const int t = first + row + k;
             if (t >= lo && t < hi) cp_async16(&dst.v[row + k][col], p, 16);
         }
+    } else if constexpr (sizeof(T) == 2) {
+        constexpr int kWordsRow = kGateChannels / 8 + 1;
+        const int n = min(kGateChannels, dim - tile * kGateChannels);
+        const T *const end = src + static_cast<int64_t>(hi) * dim;
+#pragma unroll
+        for (int i0 = 0; i0 < kRows * kWordsRow; i0 += 32) {
+            const int i = i0 + lane, row = i / kWordsRow, word = i - row * kWordsRow, t = first + row;
+            if (i >= kRows * kWordsRow || t < lo || t >= hi) continue;
+            const T *const p = src + static_cast<int64_t>(t) * dim + tile * kGateChannels;
+            const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 7;
+            const T *const from = p + (8 * word - shift);
+            if (8 * word >= n + shift) continue;
+            if (from >= src) {
+                cp_async16(&dst.v[row][8 * word], from, static_cast<int>(min(end - from, int64_t(8))) * 2);
+            } else {  // the word in which the tensor begins
+                for (int k = shift; k < min(8, shift + n); ++k) dst.v[row][k] = p[k - shift];
+            }
+        }
     } else {
         const int n = min(kGateChannels, dim - tile * kGateChannels);
         const T *row = src + static_cast<int64_t>(first) * dim + tile * kGateChannels;
 #pragma unroll 4
         for (int k = 0; k < kRows; ++k, row += dim) {
             if (first + k < lo || first + k >= hi) continue;
-            if constexpr (sizeof(T) == 2) {
-                const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1;
-                const T *const word = row - shift;
-                if (2 * lane < n + shift) cp_async4(&dst.v[k][2 * lane], word + 2 * lane, 4);
-                if (lane == 0 && n + shift > kGateChannels) cp_async4(&dst.v[k][kGateChannels], word + kGateChannels, 4);
-            } else {
-                if (lane < n) cp_async4(&dst.v[k][lane], row + lane, 4);
-                if (lane + 32 < n) cp_async4(&dst.v[k][lane + 32], row + lane + 32, 4);
-            }
+            if (lane < n) cp_async4(&dst.v[k][lane], row + lane, 4);
+            if (lane + 32 < n) cp_async4(&dst.v[k][lane + 32], row + lane + 32, 4);
         }
     }
 }
@@ -272,9 +285,9 @@ struct BlockPairs {
     }
 };
 
-// The cut of a call (without pointers). block: warps of the operator's block that shares a row; per_sm: segments of a wave
-// on an SM; parts: at most as many partial sums per tile.
-GateCut gate_cut(const SeqArgs &q, int dim, int block, int per_sm, int parts);
+// The cut of a call (without pointers). block: warps of the operator's block that shares a row, of `shortest` tokens at
+// least; per_sm: segments of a wave on an SM; parts: at most as many partial sums per tile.
+GateCut gate_cut(const SeqArgs &q, int dim, int block, int shortest, int per_sm, int parts);
 inline size_t gate_pairs(const GateCut &g) {  // elements of each of P, h and start
     return g.segments > 1 && g.block == 0 ? static_cast<size_t>(g.spans) * g.segments * g.tiles * 32 : 0;
 }
