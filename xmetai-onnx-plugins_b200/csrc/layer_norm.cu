@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(kThreads, 2048 / kThreads) norm_staged_kernel(
     const float inv = 1.0f / static_cast<float>(dim);
     auto copy = [&](long long row, int stage) {
         if (row < p.rows) {
-            stage_row<kThreads>(ring + tensors * stage * pitch, X, static_cast<unsigned>(row), dim);
-            if (R != nullptr) stage_row<kThreads>(ring + (2 * stage + 1) * pitch, R, static_cast<unsigned>(row), dim);
+            stage_row<kThreads>(ring + tensors * stage * pitch, X, static_cast<unsigned>(row), p.rows, dim);
+            if (R != nullptr) stage_row<kThreads>(ring + (2 * stage + 1) * pitch, R, static_cast<unsigned>(row), p.rows, dim);
         }
         cp_async_commit();
     };

@@ -141,9 +141,9 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_grad_staged_ker
     auto copy = [&](long long row, int stage) {
         if (row < p.rows) {
             const unsigned i = static_cast<unsigned>(row);
-            stage_row<kThreads>(ring + 3 * stage * pitch, DY, i, dim);
-            stage_row<kThreads>(ring + (3 * stage + 1) * pitch, X, i, dim);
-            if (DR != nullptr) stage_row<kThreads>(ring + (3 * stage + 2) * pitch, DR, i, dim);
+            stage_row<kThreads>(ring + 3 * stage * pitch, DY, i, p.rows, dim);
+            stage_row<kThreads>(ring + (3 * stage + 1) * pitch, X, i, p.rows, dim);
+            if (DR != nullptr) stage_row<kThreads>(ring + (3 * stage + 2) * pitch, DR, i, p.rows, dim);
         }
         cp_async_commit();
     };

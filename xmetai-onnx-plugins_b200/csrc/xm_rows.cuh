@@ -140,15 +140,17 @@ struct RowPart {
 
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
 
-// Rows that are not whole words, staged in shared memory: 4-byte asynchronous copies from the word that holds a row's
-// first element, so that a row of a 16-bit type may begin in the middle of its first word. Elements are read from there
-// by consecutive threads, about sixteen to each: fewer leave most of a row's time to its barriers (32768 x 1026, backward:
+// Rows that are not whole words, staged in shared memory: asynchronous copies of 16-byte words, from the one that holds a
+// row's first element, behind up to a word's others. Elements are read from there by consecutive threads, about sixteen to each: fewer leave most of a row's time to its barriers (32768 x 1026, backward:
 // 229 us with 512 threads), more too few warps.
 constexpr int staged_threads(int dim) { return dim <= 2048 ? 128 : dim <= 5120 ? 256 : 512; }
 
 template <typename T>
-__host__ __device__ constexpr size_t staged_pitch(int dim) {  // elements of a staged row, in whole 16-byte words
-    return (static_cast<size_t>(dim) + 2 + 16 / sizeof(T) - 1) / (16 / sizeof(T)) * (16 / sizeof(T));
+constexpr int kStagedWord = 16 / static_cast<int>(sizeof(T));
+template <typename T>
+__host__ __device__ constexpr size_t staged_pitch(int dim) {  // elements of a staged row, in whole words
+    constexpr size_t kWord = kStagedWord<T>;
+    return (static_cast<size_t>(dim) + 2 * kWord - 2) / kWord * kWord;
 }
 constexpr size_t kStagedBytes = 220 * 1024;  // of shared memory on an SM
 template <auto kKernel>
@@ -156,15 +158,23 @@ cudaError_t prepare_staged() { return allow_shared<kKernel>(kStagedBytes); }
 // Where row `row` of a tensor begins in its stage.
 template <typename T>
 __device__ __forceinline__ int staged_shift(const T *src, unsigned row, int dim) {
-    if (sizeof(T) != 2) return 0;
-    return static_cast<int>((reinterpret_cast<uintptr_t>(src) >> 1) ^ (row & static_cast<unsigned>(dim))) & 1;
+    const unsigned first = static_cast<unsigned>(reinterpret_cast<uintptr_t>(src) / sizeof(T));
+    return static_cast<int>((first + row * static_cast<unsigned>(dim)) % kStagedWord<T>);
 }
+// Copies a row of a tensor of `rows` rows, and reads nothing outside of it.
 template <int kThreads, typename T>
-__device__ __forceinline__ void stage_row(T *dst, const T *src, unsigned row, int dim) {
-    constexpr int kPer = 4 / static_cast<int>(sizeof(T));
+__device__ __forceinline__ void stage_row(T *dst, const T *src, unsigned row, unsigned rows, int dim) {
+    constexpr int kWord = kStagedWord<T>;
     const int shift = staged_shift(src, row, dim);
-    const T *const first = src + static_cast<size_t>(row) * dim - shift;
-    for (int i = threadIdx.x * kPer; i < dim + shift; i += kThreads * kPer) cp_async4(dst + i, first + i, 4);
+    const T *const first = src + static_cast<size_t>(row) * dim;
+    for (int i = static_cast<int>(threadIdx.x) * kWord - shift; i < dim; i += kThreads * kWord) {
+        const bool begin = row == 0 && i < 0, end = row + 1 == rows && dim - i < kWord;
+        if (!begin && !end) {
+            cp_async16(dst + shift + i, first + i, 16);
+        } else {  // the words in which the tensor begins and ends
+            for (int k = max(i, 0); k < min(i + kWord, dim); ++k) dst[shift + k] = first[k];
+        }
+    }
 }
 
 // Sums of two values over a group, the same in all its threads and whatever the number of rows. `part`: shared memory
