@@ -790,3 +790,61 @@ def test_malformed_offsets_stay_inside(xm, cuda):
         xm.GatedRecurrenceGradFn(x, x, f, x, low, pool[3:6].clone(), c, out=(guard[1:2], None, None, None))
         torch.cuda.synchronize()
         assert bool((guard[::2] == 5).all()) and bool((pool[:3] == 5).all()) and bool((pool[6:] == 5).all())
+
+
+@pytest.mark.parametrize("dt,tokens,dim", [("bf16", 300, 72), ("bf16", 300, 71), ("f32", 40, 33), ("bf16", 300, 9600),
+                                           ("f32", 300, 9607), ("bf16", 280, 19001)])
+def test_malformed_offsets_in_every_cut(xm, cuda, dt, tokens, dim):
+    """The same where a block, or its warps in turn, takes a row: every call ends and stays inside its outputs."""
+    g = gen(55)
+    x, f, low = (t.cuda() for t in inputs(g, 1, tokens, dim, DT[dt]))
+    guard = torch.full((3, tokens, dim), 5.0, dtype=DT[dt], device="cuda")
+    pool = torch.full((9, dim), 5.0, device="cuda")
+    for cu in ([0, 900, 30, tokens], [-7, 100, 2000, tokens - 1], [tokens - 10, 30, 20, 10], [tokens] * 4, [10, 20, 15, 36],
+               [5, 4, 3, tokens]):
+        c = torch.tensor(cu).cuda()
+        xm.GatedRecurrenceFn(x, f, low, pool[3:6], c, output_final_state=1, out=guard[1:2], final_state=pool[3:6])
+        xm.GatedRecurrenceGradFn(x, x, f, x, low, pool[3:6].clone(), c, out=(guard[1:2], None, None, None))
+        torch.cuda.synchronize()
+        assert bool((guard[::2] == 5).all()) and bool((pool[:3] == 5).all()) and bool((pool[6:] == 5).all())
+    # and the next call is as it should be
+    y, bound, final, fb = Q.recurrence(x.cpu(), f.cpu(), low.cpu())
+    got, last = xm.GatedRecurrenceFn(x, f, low, output_final_state=1)
+    close(got, y, bound)
+    close(last, final, fb)
+
+
+@pytest.mark.parametrize("dim", [61, 66, 71])
+def test_views_at_the_ends_of_a_buffer(xm, cuda, dim):
+    """Tensors that begin off a 16-byte word and end with the buffer's last element, between neighbours that hold NaN."""
+    g = gen(56)
+    for dtype in DT.values():
+        for n, off in ((1, 1), (40, 3), (130, 7)):
+            x, f, low = inputs(g, 1, n, dim, dtype)
+            init, dl = normal(g, 1, dim), normal(g, 1, dim)
+            y, bound, final, fb = Q.recurrence(x, f, low, init)
+            dy, ys = normal(g, 1, n, dim, dtype=dtype), y.to(dtype)
+            want = Q.recurrence_grad(dy, x, f, ys, low, init, None, dl)
+
+            def place(t):
+                buf = torch.full((off + t.numel(),), float("nan"), dtype=t.dtype, device="cuda")
+                buf[off:] = t.flatten().cuda()
+                return buf[off:].view(t.shape)
+
+            a = [place(t) for t in (x, f, low, init, ys, dy, dl)]
+            got, last = xm.GatedRecurrenceFn(*a[:4], output_final_state=1)
+            close(got, y, bound)
+            close(last, final, fb)
+            _close_grads(xm.GatedRecurrenceGradFn(a[5], a[0], a[1], a[4], a[2], a[3], None, a[6]), want, low, init)
+
+
+def test_long_rows_of_few_channels(xm, cuda):
+    """Rows that are cut into as many segments as there may be."""
+    for dt, n, dim, cu in ((torch.float32, 7000, 7, [0, 1, 3500, 7000]), (torch.bfloat16, 9001, 64, [0, 9001])):
+        a = _grad_inputs(gen(57), 1, n, dim, dt, cu)
+        dy, x, f, ys, low, init, dl = a
+        y, bound, final, fb = Q.recurrence(x, f, low, init, cu)
+        got, last = xm.GatedRecurrenceFn(dev(x), dev(f), dev(low), dev(init), torch.tensor(cu).cuda(), output_final_state=1)
+        close(got, y, bound)
+        close(last, final, fb)
+        _close_grads(_grad(xm, cu, *a), Q.recurrence_grad(*a[:6], cu, dl), low, init)
