@@ -13,7 +13,8 @@ pytestmark = pytest.mark.gpu
 
 SHAPES = [((1,), 1), ((3,), 2), ((2, 5), 7), ((4,), 8), ((1, 1, 3), 64), ((33,), 100), ((7,), 128), ((1,), 1000),
           ((300,), 72), ((9,), 1024), ((5,), 1025), ((2,), 2048), ((3,), 4096), ((1,), 4096), ((2,), 5003), ((4,), 8192),
-          ((2,), 16384), ((2,), 16392), ((1,), 40000), ((2,), 100003), ((), 96)]
+          ((2,), 16384), ((2,), 16392), ((1,), 40000), ((2,), 100003), ((), 96),
+          ((5,), 362), ((4,), 1026), ((3,), 2050), ((2,), 4098), ((2,), 8194)]
 
 
 def rows(g, lead, dim, dtype):

@@ -559,16 +559,20 @@ def test_repeatable_bits(xm, cuda):
 CUTS = {
     "blocks of eight, words": (3, 300, 3264),
     "blocks of eight, odd rows": (3, 300, 3267),
+    "blocks of eight, pairs": (3, 300, 3266),
     "blocks of four, words": (5, 260, 4000),
+    "blocks of four, pairs": (5, 261, 3998),
     "blocks of four, odd rows": (5, 261, 3999),
     "packed, blocks of eight": ([0, 0, 7, 8, 9, 128, 128, 256, 257, 530, 600], None, 9600),
     "packed, blocks of eight, odd rows": ([3, 4, 100, 411], None, 9607),
     "packed, blocks of four": ([0, 1, 130, 131, 330, 400], None, 19001),
     "a block for each SM": (2, 500, 3904),
     "a warp for each row": (3, 200, 3265),
+    "a warp for each row, pairs": (3, 200, 3266),
     "short rows of two sequences": (9, 32, 70),
     "short rows, in turns": (290, 32, 64),
     "segments of several rows": (2, 1200, 130),
+    "segments, words": (2, 1200, 136),
 }
 
 

@@ -24,20 +24,20 @@ constexpr int kRingStages = kWarps == 8 || sizeof(T) == 4 ? 3 : 2;
 // stages, of which nine fit an SM, 119 at best).
 constexpr int kPerSm = 12;
 
-template <typename T, bool kWords>
-using ScanTile = GateTile<T, kGateGroup, kWords>;
+template <typename T, int kRow>
+using ScanTile = GateTile<T, kGateGroup, kRow>;
 
-template <typename T, bool kWords>
-__device__ __forceinline__ float2 init_of(const GateArgs &p, const Lane<T, kWords> &ch, long long row) {
+template <typename T, int kRow>
+__device__ __forceinline__ float2 init_of(const GateArgs &p, const Lane<T, kRow> &ch, long long row) {
     return ch.floats(p.init != nullptr && row >= 0 ? p.init + row * p.dim : nullptr, 0.0f);
 }
-template <typename T, bool kWords>
-__device__ __forceinline__ void store_final(const GateArgs &p, const Lane<T, kWords> &ch, long long row, float2 h) {
+template <typename T, int kRow>
+__device__ __forceinline__ void store_final(const GateArgs &p, const Lane<T, kRow> &ch, long long row, float2 h) {
     if (p.final_state != nullptr && row >= 0) ch.store_floats(p.final_state + row * p.dim, h);
 }
 // Sequences without tokens keep their starting states; warp of warps with the same channels.
-template <typename T, bool kWords>
-__device__ __forceinline__ void keep_empty(const GateArgs &p, const Lane<T, kWords> &ch, int warp, int warps) {
+template <typename T, int kRow>
+__device__ __forceinline__ void keep_empty(const GateArgs &p, const Lane<T, kRow> &ch, int warp, int warps) {
     if (p.final_state == nullptr) return;
     for_empty_sequences(p.seq, warp, warps, [&](int s) {
         long long from;
@@ -48,9 +48,9 @@ __device__ __forceinline__ void keep_empty(const GateArgs &p, const Lane<T, kWor
 
 // A warp walks segment j of a span. kEnds: the first pass. first_pass(): it is through; nothing is stored, and nothing
 // of it read, before.
-template <typename T, bool kWords, bool kEnds, int kStages, typename Wait>
-__device__ __forceinline__ void walk_segment(const GateArgs &p, const GateCut &g, ScanTile<T, kWords> (*ring)[2],
-                                             const Lane<T, kWords> &ch, int tile, float2 low, float2 rest, Span span,
+template <typename T, int kRow, bool kEnds, int kStages, typename Wait>
+__device__ __forceinline__ void walk_segment(const GateArgs &p, const GateCut &g, ScanTile<T, kRow> (*ring)[2],
+                                             const Lane<T, kRow> &ch, int tile, float2 low, float2 rest, Span span,
                                              int length, int j, const GatePairs &pairs, Wait &&first_pass) {
     const SeqArgs &q = p.seq;
     const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
@@ -102,8 +102,8 @@ __device__ __forceinline__ void walk_segment(const GateArgs &p, const GateCut &g
         __syncwarp();
         copy(t + (kStages - 1) * kGateGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
         auto token = [&](int k, float2 &x, float2 &f) {
-            x = ring[stage][0].at(k, shift_of<T, kWords>(X, t + k, p.dim));
-            f = ring[stage][1].at(k, shift_of<T, kWords>(F, t + k, p.dim));
+            x = ring[stage][0].at(k, shift_of<T, kRow>(X, t + k, p.dim));
+            f = ring[stage][1].at(k, shift_of<T, kRow>(F, t + k, p.dim));
         };
         float2 a[kGateGroup], b[kGateGroup];  // (of no meaning behind the segment's end)
 #pragma unroll
@@ -162,13 +162,13 @@ __device__ __forceinline__ void walk_segment(const GateArgs &p, const GateCut &g
 }
 
 // A segment to each warp. kEnds: the first pass over segments (all but a span's last).
-template <typename T, bool kWords, bool kEnds>
+template <typename T, int kRow, bool kEnds>
 __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const GateCut g) {
     extern __shared__ float4 smem_f4[];
     if (kEnds) dependents_may_launch();
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs, slot = blockIdx.x / g.tiles / segs;
-    const Lane<T, kWords> ch(tile, threadIdx.x & 31, p.dim);
+    const Lane<T, kRow> ch(tile, threadIdx.x & 31, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     bool waited = kEnds;
     auto first_pass = [&] {
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(32, 8) gate_kernel(const GateArgs p, const Gat
     if (!kEnds) keep_empty(p, ch, slot * segs + j, g.width * segs);
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(p.seq, g, i);
-        walk_segment<T, kWords, kEnds, kStages>(p, g, reinterpret_cast<ScanTile<T, kWords>(*)[2]>(smem_f4), ch, tile, low,
+        walk_segment<T, kRow, kEnds, kStages>(p, g, reinterpret_cast<ScanTile<T, kRow>(*)[2]>(smem_f4), ch, tile, low,
                                                 rest, span, segment_length(g, span), j, global_pairs(g, i, tile), first_pass);
     }
     first_pass();  // (also warps without tokens: what follows waits for this kernel only)
@@ -191,47 +191,47 @@ struct ScanBlock {
     static constexpr int kWarps = sizeof(T) == 4 ? 8 : 16, kStages = sizeof(T) == 4 ? 3 : 2;
 };
 constexpr int kShortest = 64;  // tokens of a row that a block shares (48 x 512: 4.8 us by a warp alone, 5.3)
-template <typename T, bool kWords>
+template <typename T, int kRow>
 struct BlockSmem {
-    ScanTile<T, kWords> ring[ScanBlock<T>::kWarps][ScanBlock<T>::kStages][2];
+    ScanTile<T, kRow> ring[ScanBlock<T>::kWarps][ScanBlock<T>::kStages][2];
     BlockPairs<ScanBlock<T>::kWarps> pairs;
 };
 
-template <typename T, bool kWords>
+template <typename T, int kRow>
 __global__ void __launch_bounds__(32 * ScanBlock<T>::kWarps, 1) gate_block_kernel(const GateArgs p, const GateCut g) {
     extern __shared__ float4 smem_f4[];
     constexpr int kWarps = ScanBlock<T>::kWarps, kStages = ScanBlock<T>::kStages;
-    auto &sm = *reinterpret_cast<BlockSmem<T, kWords> *>(smem_f4);
+    auto &sm = *reinterpret_cast<BlockSmem<T, kRow> *>(smem_f4);
     const int warp = threadIdx.x >> 5, tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
-    const Lane<T, kWords> ch(tile, threadIdx.x & 31, p.dim);
+    const Lane<T, kRow> ch(tile, threadIdx.x & 31, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     keep_empty(p, ch, slot * kWarps + warp, g.width * kWarps);
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(p.seq, g, i);
         const int length = segment_length(g, span);
         const GatePairs pairs = sm.pairs.view();
-        walk_segment<T, kWords, true, kStages>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, [] {});
+        walk_segment<T, kRow, true, kStages>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, [] {});
         __syncthreads();
-        walk_segment<T, kWords, false, kStages>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, [] {});
+        walk_segment<T, kRow, false, kStages>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, [] {});
         __syncthreads();
     }
 }
 
-template <typename T, bool kWords, int kWarps>
+template <typename T, int kRow, int kWarps>
 struct RingSmem {
     Ring<kWarps> hand;
-    GateTile<T, kGateGroup, kWords> ring[kWarps][kRingStages<T, kWarps>][2];
+    GateTile<T, kGateGroup, kRow> ring[kWarps][kRingStages<T, kWarps>][2];
 };
 
-template <typename T, bool kWords, int kWarps>
+template <typename T, int kRow, int kWarps>
 __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? 5 : 2) gate_ring_kernel(const GateArgs p, const GateCut g) {
     extern __shared__ float4 smem_f4[];
     constexpr int kStages = kRingStages<T, kWarps>;
-    auto &sm = *reinterpret_cast<RingSmem<T, kWords, kWarps> *>(smem_f4);
+    auto &sm = *reinterpret_cast<RingSmem<T, kRow, kWarps> *>(smem_f4);
     const SeqArgs &q = p.seq;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
-    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const Lane<T, kRow> ch(tile, lane, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     const T *const X = static_cast<const T *>(p.x), *const F = static_cast<const T *>(p.f);
     T *const Y = static_cast<T *>(p.out);
@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? 5 : 2) gate_ring_ke
             __syncwarp();
             copy(t + (kStages - 1) * kTurn, stage == 0 ? kStages - 1 : stage - 1);  // read by all a round ago
             auto token = [&](int k, float2 &x, float2 &f) {
-                x = sm.ring[warp][stage][0].at(k, shift_of<T, kWords>(X, t + k, p.dim));
-                f = sm.ring[warp][stage][1].at(k, shift_of<T, kWords>(F, t + k, p.dim));
+                x = sm.ring[warp][stage][0].at(k, shift_of<T, kRow>(X, t + k, p.dim));
+                f = sm.ring[warp][stage][1].at(k, shift_of<T, kRow>(F, t + k, p.dim));
             };
             if (seq.end <= t) seq = seq_at(q, t);
             const bool more = t + kGateGroup < span.hi;  // a group behind
@@ -383,27 +383,29 @@ __global__ void __launch_bounds__(kTokenThreads) gate_token_kernel(const GateArg
     }
 }
 
-template <typename T, bool kWords>
-cudaError_t launch_words(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
-    constexpr size_t kSmem = kStages * 2 * sizeof(ScanTile<T, kWords>);
+template <typename T, int kRow>
+cudaError_t launch_row(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
+    constexpr size_t kSmem = kStages * 2 * sizeof(ScanTile<T, kRow>);
     if (g.block != 0)
-        return launch_gate<gate_block_kernel<T, kWords>>(g.block, sizeof(BlockSmem<T, kWords>), g, 1, false, stream, a, g);
+        return launch_gate<gate_block_kernel<T, kRow>>(g.block, sizeof(BlockSmem<T, kRow>), g, 1, false, stream, a, g);
     if (g.ring == 4)
-        return launch_gate<gate_ring_kernel<T, kWords, 4>>(4, sizeof(RingSmem<T, kWords, 4>), g, 1, false, stream, a, g);
+        return launch_gate<gate_ring_kernel<T, kRow, 4>>(4, sizeof(RingSmem<T, kRow, 4>), g, 1, false, stream, a, g);
     if (g.ring == 8)
-        return launch_gate<gate_ring_kernel<T, kWords, 8>>(8, sizeof(RingSmem<T, kWords, 8>), g, 1, false, stream, a, g);
+        return launch_gate<gate_ring_kernel<T, kRow, 8>>(8, sizeof(RingSmem<T, kRow, 8>), g, 1, false, stream, a, g);
     if (g.segments > 1) {
-        const cudaError_t e = launch_gate<gate_kernel<T, kWords, true>>(1, kSmem, g, g.segments - 1, false, stream, a, g);
+        const cudaError_t e = launch_gate<gate_kernel<T, kRow, true>>(1, kSmem, g, g.segments - 1, false, stream, a, g);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate<gate_kernel<T, kWords, false>>(1, kSmem, g, g.segments, gate_behind(g), stream, a, g);
+    return launch_gate<gate_kernel<T, kRow, false>>(1, kSmem, g, g.segments, gate_behind(g), stream, a, g);
 }
 
 template <typename T>
 cudaError_t launch_type(const GateArgs &a, const GateCut &g, cudaStream_t stream) {
-    if (a.dim * sizeof(T) % 16 == 0 && aligned16(a.x) && aligned16(a.f) && aligned16(a.out))
-        return launch_words<T, true>(a, g, stream);
-    return launch_words<T, false>(a, g, stream);
+    switch (row_of(a.dim, sizeof(T), {a.x, a.f, a.out})) {
+        case kRowWords: return launch_row<T, kRowWords>(a, g, stream);
+        case kRowPairs: return launch_row<T, kRowPairs>(a, g, stream);
+        default: return launch_row<T, kRowAny>(a, g, stream);
+    }
 }
 
 // Several sequences per thread where that leaves each SM eight blocks; below, one.

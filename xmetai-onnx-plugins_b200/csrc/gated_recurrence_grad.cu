@@ -24,8 +24,8 @@ constexpr int kMaxParts = 1024;  // partial sums of d_bound per channel
 // twice the instructions to fetch in short calls.
 constexpr int kGroup = 8;
 
-template <typename T, bool kWords>
-using GradTile = GateTile<T, kGroup, kWords>;
+template <typename T, int kRow>
+using GradTile = GateTile<T, kGroup, kRow>;
 
 // Segments of an SM: one wave, as many as it has room for (16384 x 4096 packed takes 188 us; with six stages, of which
 // eight fit, 197).
@@ -41,26 +41,26 @@ __device__ __forceinline__ float2 rest_of(float2 low) {
     return make_float2(low.x == 1.0f ? 0x1p-60f : 1.0f - low.x, low.y == 1.0f ? 0x1p-60f : 1.0f - low.y);
 }
 
-template <typename T, bool kWords>
-__device__ __forceinline__ float2 state_row(const GateGradArgs &p, const Lane<T, kWords> &ch, const float *base, int seq) {
+template <typename T, int kRow>
+__device__ __forceinline__ float2 state_row(const GateGradArgs &p, const Lane<T, kRow> &ch, const float *base, int seq) {
     return ch.floats(base != nullptr ? base + static_cast<size_t>(seq) * p.dim : nullptr, 0.0f);
 }
-template <typename T, bool kWords>
-__device__ __forceinline__ void store_dinit(const GateGradArgs &p, const Lane<T, kWords> &ch, int seq, float2 c) {
+template <typename T, int kRow>
+__device__ __forceinline__ void store_dinit(const GateGradArgs &p, const Lane<T, kRow> &ch, int seq, float2 c) {
     if (p.dinit != nullptr) ch.store_floats(p.dinit + static_cast<size_t>(seq) * p.dim, c);
 }
 // Sequences without tokens: the gradient passes through; warp of warps with the same channels.
-template <typename T, bool kWords>
-__device__ __forceinline__ void pass_empty(const GateGradArgs &p, const Lane<T, kWords> &ch, int warp, int warps) {
+template <typename T, int kRow>
+__device__ __forceinline__ void pass_empty(const GateGradArgs &p, const Lane<T, kRow> &ch, int warp, int warps) {
     if (p.dinit != nullptr)
         for_empty_sequences(p.seq, warp, warps, [&](int s) { store_dinit(p, ch, s, state_row(p, ch, p.dfinal, s)); });
 }
 
 // A warp walks segment j of a span. kEnds: the first pass. first_pass(): it is through; nothing of it is read before.
 // dlow: sum of da (1 - a).
-template <typename T, bool kWords, bool kEnds, int kStages, int kTensors, typename Wait>
-__device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCut &g, GradTile<T, kWords> (*ring)[kTensors],
-                                             const Lane<T, kWords> &ch, int tile, float2 low, float2 rest, Span span,
+template <typename T, int kRow, bool kEnds, int kStages, int kTensors, typename Wait>
+__device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCut &g, GradTile<T, kRow> (*ring)[kTensors],
+                                             const Lane<T, kRow> &ch, int tile, float2 low, float2 rest, Span span,
                                              int length, int j, const GatePairs &pairs, float2 &dlow, Wait &&first_pass) {
     const SeqArgs &q = p.seq;
     const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
@@ -114,7 +114,7 @@ __device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCu
         copy(hi - (kStages - 1) * kGroup, stage == 0 ? kStages - 1 : stage - 1);  // read by all a group ago
         // token hi - 1 - k of a tensor
         auto load = [&](int which, const T *base, int k, int back) {
-            return ring[stage][which].at(kGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
+            return ring[stage][which].at(kGroup - 1 - k, shift_of<T, kRow>(base, hi - 1 - k - back, p.dim));
         };
         const int last = min(kGroup, hi - s0);
         if constexpr (kEnds) {
@@ -193,13 +193,13 @@ __device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCu
 
 // A segment to each warp. kEnds: the first pass over segments (all but a span's first).
 // part: [width x segments][dim] sums of d_bound, or null.
-template <typename T, bool kWords, bool kEnds>
+template <typename T, int kRow, bool kEnds>
 __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, const GateCut g, float *part) {
     extern __shared__ float4 smem_f4[];
     dependents_may_launch();
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs + (kEnds ? 1 : 0), slot = blockIdx.x / g.tiles / segs;
-    const Lane<T, kWords> ch(tile, threadIdx.x & 31, p.dim);
+    const Lane<T, kRow> ch(tile, threadIdx.x & 31, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
     bool waited = kEnds;
     auto first_pass = [&] {
@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(p.seq, g, i);
         constexpr int kTensors = kEnds ? 2 : 4;
-        walk_segment<T, kWords, kEnds, kStages, kTensors>(
-            p, g, reinterpret_cast<GradTile<T, kWords>(*)[kTensors]>(smem_f4), ch, tile, low, rest, span,
+        walk_segment<T, kRow, kEnds, kStages, kTensors>(
+            p, g, reinterpret_cast<GradTile<T, kRow>(*)[kTensors]>(smem_f4), ch, tile, low, rest, span,
             segment_length(g, span), j, global_pairs(g, i, tile), dlow, first_pass);
     }
     first_pass();  // (also warps without tokens: what follows waits for this kernel only)
@@ -226,22 +226,22 @@ struct GradBlock {
     static constexpr int kWarps = sizeof(T) == 4 ? 6 : 8, kStages = sizeof(T) == 4 ? 4 : 6;
 };
 constexpr int kShortest = 24;  // tokens of a row that a block shares (50 x 386 in float32: 9.7 us, by a warp alone 13.9)
-template <typename T, bool kWords>
+template <typename T, int kRow>
 struct GradBlockSmem {
-    GradTile<T, kWords> ring[GradBlock<T>::kWarps][GradBlock<T>::kStages][4];
+    GradTile<T, kRow> ring[GradBlock<T>::kWarps][GradBlock<T>::kStages][4];
     BlockPairs<GradBlock<T>::kWarps> pairs;
 };
 
 // part: [width][dim] sums of d_bound, or null.
-template <typename T, bool kWords>
+template <typename T, int kRow>
 __global__ void __launch_bounds__(32 * GradBlock<T>::kWarps, 1) gate_grad_block_kernel(const GateGradArgs p, const GateCut g,
                                                                                   float *part) {
     extern __shared__ float4 smem_f4[];
     constexpr int kWarps = GradBlock<T>::kWarps, kStages = GradBlock<T>::kStages;
-    auto &sm = *reinterpret_cast<GradBlockSmem<T, kWords> *>(smem_f4);
+    auto &sm = *reinterpret_cast<GradBlockSmem<T, kRow> *>(smem_f4);
     dependents_may_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
-    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const Lane<T, kRow> ch(tile, lane, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
     pass_empty(p, ch, slot * kWarps + warp, g.width * kWarps);
     float2 dlow = both(0.0f);
@@ -250,10 +250,10 @@ __global__ void __launch_bounds__(32 * GradBlock<T>::kWarps, 1) gate_grad_block_
         const int length = segment_length(g, span);
         const GatePairs pairs = sm.pairs.view();
         if (warp > 0)
-            walk_segment<T, kWords, true, kStages, 4>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs,
+            walk_segment<T, kRow, true, kStages, 4>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs,
                                                       dlow, [] {});
         __syncthreads();
-        walk_segment<T, kWords, false, kStages, 4>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, dlow,
+        walk_segment<T, kRow, false, kStages, 4>(p, g, sm.ring[warp], ch, tile, low, rest, span, length, warp, pairs, dlow,
                                                    [] {});
         __syncthreads();
     }
@@ -268,25 +268,25 @@ __global__ void __launch_bounds__(32 * GradBlock<T>::kWarps, 1) gate_grad_block_
     }
 }
 
-template <typename T, bool kWords, int kWarps>
+template <typename T, int kRow, int kWarps>
 struct GradRingSmem {
     static constexpr int kStages = kWarps == 8 && sizeof(T) == 2 ? 3 : 2;
     Ring<kWarps> hand;
-    GateTile<T, kGroup, kWords> ring[kWarps][kStages][4];  // f, dy, x, and y of the token before
+    GateTile<T, kGroup, kRow> ring[kWarps][kStages][4];  // f, dy, x, and y of the token before
 };
 
 // part: [width][dim] sums of d_bound, or null.
-template <typename T, bool kWords, int kWarps>
+template <typename T, int kRow, int kWarps>
 __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kernel(const GateGradArgs p, const GateCut g,
                                                                            float *part) {
     extern __shared__ float4 smem_f4[];
-    auto &sm = *reinterpret_cast<GradRingSmem<T, kWords, kWarps> *>(smem_f4);
-    constexpr int kStages = GradRingSmem<T, kWords, kWarps>::kStages;
+    auto &sm = *reinterpret_cast<GradRingSmem<T, kRow, kWarps> *>(smem_f4);
+    constexpr int kStages = GradRingSmem<T, kRow, kWarps>::kStages;
     dependents_may_launch();
     const SeqArgs &q = p.seq;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
-    const Lane<T, kWords> ch(tile, lane, p.dim);
+    const Lane<T, kRow> ch(tile, lane, p.dim);
     const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
     const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
                    *const F = static_cast<const T *>(p.f), *const H = static_cast<const T *>(p.y);
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
             copy(hi - (kStages - 1) * kTurn, stage == 0 ? kStages - 1 : stage - 1);  // read by all a round ago
             // token hi - 1 - k of a tensor
             auto load = [&](int which, const T *base, int k, int back) {
-                return sm.ring[warp][stage][which].at(kGroup - 1 - k, shift_of<T, kWords>(base, hi - 1 - k - back, p.dim));
+                return sm.ring[warp][stage][which].at(kGroup - 1 - k, shift_of<T, kRow>(base, hi - 1 - k - back, p.dim));
             };
             if (seq.start >= hi) seq = seq_at(q, hi - 1);
             const bool more = hi - kGroup > span.lo;  // a group before
@@ -406,33 +406,34 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
     }
 }
 
-template <typename T, bool kWords>
-cudaError_t launch_words(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
+template <typename T, int kRow>
+cudaError_t launch_row(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
     if (g.ring == 4)
-        return launch_gate<gate_grad_ring_kernel<T, kWords, 4>>(4, sizeof(GradRingSmem<T, kWords, 4>), g, 1, false, stream,
+        return launch_gate<gate_grad_ring_kernel<T, kRow, 4>>(4, sizeof(GradRingSmem<T, kRow, 4>), g, 1, false, stream,
                            a, g, part);
     if (g.ring == 8)
-        return launch_gate<gate_grad_ring_kernel<T, kWords, 8>>(8, sizeof(GradRingSmem<T, kWords, 8>), g, 1, false, stream,
+        return launch_gate<gate_grad_ring_kernel<T, kRow, 8>>(8, sizeof(GradRingSmem<T, kRow, 8>), g, 1, false, stream,
                            a, g, part);
     if (g.block != 0)
-        return launch_gate<gate_grad_block_kernel<T, kWords>>(g.block, sizeof(GradBlockSmem<T, kWords>), g, 1, false, stream,
+        return launch_gate<gate_grad_block_kernel<T, kRow>>(g.block, sizeof(GradBlockSmem<T, kRow>), g, 1, false, stream,
                                                               a, g, part);
-    constexpr size_t kSmem = kStages * sizeof(GradTile<T, kWords>);  // of one tensor
+    constexpr size_t kSmem = kStages * sizeof(GradTile<T, kRow>);  // of one tensor
     if (g.segments > 1) {
-        const cudaError_t e = launch_gate<gate_grad_kernel<T, kWords, true>>(1, 2 * kSmem, g,
+        const cudaError_t e = launch_gate<gate_grad_kernel<T, kRow, true>>(1, 2 * kSmem, g,
                                           g.segments - 1, false, stream, a, g, part);
         if (e != cudaSuccess) return e;
     }
-    return launch_gate<gate_grad_kernel<T, kWords, false>>(1, 4 * kSmem, g, g.segments,
+    return launch_gate<gate_grad_kernel<T, kRow, false>>(1, 4 * kSmem, g, g.segments,
                        gate_behind(g), stream, a, g, part);
 }
 
 template <typename T>
 cudaError_t launch_type(const GateGradArgs &a, const GateCut &g, float *part, cudaStream_t stream) {
-    if (a.dim * sizeof(T) % 16 == 0 && aligned16(a.dy) && aligned16(a.x) && aligned16(a.f) && aligned16(a.y) &&
-        aligned16(a.dx) && aligned16(a.df))
-        return launch_words<T, true>(a, g, part, stream);
-    return launch_words<T, false>(a, g, part, stream);
+    switch (row_of(a.dim, sizeof(T), {a.dy, a.x, a.f, a.y, a.dx, a.df})) {
+        case kRowWords: return launch_row<T, kRowWords>(a, g, part, stream);
+        case kRowPairs: return launch_row<T, kRowPairs>(a, g, part, stream);
+        default: return launch_row<T, kRowAny>(a, g, part, stream);
+    }
 }
 
 template <typename T>

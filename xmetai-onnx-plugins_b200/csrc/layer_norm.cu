@@ -7,8 +7,8 @@
 // Bound by memory: x and the residual are read once and y and s written once. A row
 // stays in the registers of its group of threads between the sum, the squares and the
 // output, so it is not read again; rows that do not fit (above 16384 elements of
-// the 16-bit types, 8192 of float32) are, from the caches. Rows that are not whole
-// words are staged in shared memory.
+// the 16-bit types, 8192 of float32) are, from the caches. Rows of an odd number of
+// elements are staged in shared memory above 1024.
 #include <algorithm>
 
 #include "xm_common.cuh"
@@ -20,8 +20,12 @@ namespace {
 
 constexpr int threads_of(int group) { return group < 128 ? 128 : group; }
 
+// Threads of an SM: pairs of 16-bit elements take more registers than 64 (16384 x 4098: 206 us with 1024).
+template <typename T, int VE>
+constexpr int kThreadsSm = VE == 2 && sizeof(T) == 2 ? 512 : 1024;
+
 template <typename T, int VE, int kGroup>
-__global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup)) norm_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(threads_of(kGroup), kThreadsSm<T, VE> / threads_of(kGroup)) norm_kernel(const NormArgs p) {
     constexpr int kThreads = threads_of(kGroup), kRows = kThreads / kGroup;
     using Part = RowPart<T, VE, kGroup>;
     constexpr int kPairs = Part::kElems / 2;
@@ -94,7 +98,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup))
     }
 }
 
-// Rows that are not whole words, above 1024 elements: staged some rows ahead, and read from shared memory for every
+// Rows that are not pairs of elements, above 1024: staged some rows ahead, and read from shared memory for every
 // pass. (In registers, one element a load, 16384 rows of 4097 took 247 us.)
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads, 2048 / kThreads) norm_staged_kernel(const NormArgs p, int stages) {
@@ -215,7 +219,7 @@ template <typename T, int VE, int kGroup>
 cudaError_t launch_group(const NormArgs &a, cudaStream_t stream) {
     constexpr int kThreads = threads_of(kGroup), kRows = kThreads / kGroup;
     const int64_t blocks = (static_cast<int64_t>(a.rows) + kRows - 1) / kRows;
-    const int64_t most = static_cast<int64_t>(current_device_sm_count()) * (1024 / kThreads);
+    const int64_t most = static_cast<int64_t>(current_device_sm_count()) * (kThreadsSm<T, VE> / kThreads);
     norm_kernel<T, VE, kGroup><<<static_cast<unsigned>(std::min(blocks, most)), kThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }
@@ -240,16 +244,19 @@ cudaError_t launch_rows(const NormArgs &a, cudaStream_t stream) {
     if (a.dim <= 16 * kRowElems<T, VE, 16>) return launch_group<T, VE, 16>(a, stream);
     if (a.dim <= 32 * kRowElems<T, VE, 32>) return launch_group<T, VE, 32>(a, stream);
     if (a.dim <= 128 * kRowElems<T, VE, 128>) return launch_group<T, VE, 128>(a, stream);
-    if constexpr (VE == 1) {
+    if constexpr (VE > 1) {
+        if (a.dim <= 256 * kRowElems<T, VE, 256>) return launch_group<T, VE, 256>(a, stream);
+        if (a.dim <= 512 * kRowElems<T, VE, 512>) return launch_group<T, VE, 512>(a, stream);
+    }
+    if constexpr (kThreadsSm<T, VE> == 1024 && VE > 1) {
+        if (a.dim <= 1024 * kRowElems<T, VE, 1024>) return launch_group<T, VE, 1024>(a, stream);
+    }
+    if constexpr (VE <= 2) {
         if (2 * 2 * staged_pitch<T>(a.dim) * sizeof(T) <= kStagedBytes) {
             if (staged_threads(a.dim) == 128) return launch_staged<T, 128>(a, stream);
             if (staged_threads(a.dim) == 256) return launch_staged<T, 256>(a, stream);
             return launch_staged<T, 512>(a, stream);
         }
-    } else {
-        if (a.dim <= 256 * kRowElems<T, VE, 256>) return launch_group<T, VE, 256>(a, stream);
-        if (a.dim <= 512 * kRowElems<T, VE, 512>) return launch_group<T, VE, 512>(a, stream);
-        if (a.dim <= 1024 * kRowElems<T, VE, 1024>) return launch_group<T, VE, 1024>(a, stream);
     }
     norm_wide_kernel<T><<<std::min(a.rows, 2 * current_device_sm_count()), kWideThreads, 0, stream>>>(a);
     return cudaGetLastError();
@@ -258,10 +265,11 @@ cudaError_t launch_rows(const NormArgs &a, cudaStream_t stream) {
 template <typename T>
 cudaError_t launch_type(const NormArgs &a, cudaStream_t stream) {
     constexpr int kWord = 16 / static_cast<int>(sizeof(T));
-    if (a.dim % kWord == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.out) && aligned16(a.sum) &&
-        aligned16(a.weight) && aligned16(a.bias))
-        return launch_rows<T, kWord>(a, stream);
-    return launch_rows<T, 1>(a, stream);
+    switch (row_unit(a.dim, sizeof(T), {a.x, a.residual, a.out, a.sum}, {a.weight, a.bias})) {
+        case kWord: return launch_rows<T, kWord>(a, stream);
+        case 2: return launch_rows<T, 2>(a, stream);
+        default: return launch_rows<T, 1>(a, stream);
+    }
 }
 
 }  // namespace

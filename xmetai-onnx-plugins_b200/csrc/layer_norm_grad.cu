@@ -7,9 +7,9 @@
 // Bound by memory: dy, x and d_residual are read once and dx written once. A thread
 // keeps the same columns for all rows that its block walks, so the sums over rows stay
 // in registers next to the row itself; each block leaves one row of partial sums, which
-// column_sum.cu adds in a fixed order. Rows that are not whole words are staged in
-// shared memory. Rows that do not fit (above 8192 elements of the 16-bit types, 4096 of
-// float32 in whole words) take a kernel for dx and one for the columns.
+// column_sum.cu adds in a fixed order. Rows of an odd number of elements are staged in
+// shared memory above 1024. Rows that do not fit (above 8192 elements of the 16-bit types, 4096 of
+// float32) take a kernel for dx and one for the columns.
 #include <algorithm>
 
 #include "xm_common.cuh"
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), 512 / threads_of(kGroup)) 
     if (part_b != nullptr) leave(part_b, sb);
 }
 
-// Rows that are not whole words, above 1024 elements: staged some rows ahead, kPer columns to a thread.
+// Rows that are not pairs of elements, above 1024: staged some rows ahead, kPer columns to a thread.
 template <typename T, int kThreads, int kPer>
 __global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_grad_staged_kernel(const NormGradArgs p, int stages, float *part_w,
                                                                          float *part_b) {
@@ -255,15 +255,9 @@ int group_of(int dim) {
     if (dim <= 16 * kRowElems<T, VE, 16>) return 16;
     if (dim <= 32 * kRowElems<T, VE, 32>) return 32;
     if (dim <= 128 * kRowElems<T, VE, 128>) return 128;
-    if (VE == 1) return dim <= kStagedMax && 2 * 3 * staged_pitch<T>(dim) * sizeof(T) <= kStagedBytes ? -1 : 0;
-    if (dim <= 256 * kRowElems<T, VE, 256>) return 256;
-    return dim <= 512 * kRowElems<T, VE, 512> ? 512 : 0;
-}
-
-// Whether all tensors move in words.
-bool words_of(const NormGradArgs &a) {
-    return a.dim % (a.io == IoType::kF32 ? 4 : 8) == 0 && aligned16(a.dy) && aligned16(a.x) && aligned16(a.dres) &&
-           aligned16(a.weight);
+    if (VE > 1 && dim <= 256 * kRowElems<T, VE, 256>) return 256;
+    if (VE > 1 && dim <= 512 * kRowElems<T, VE, 512>) return 512;
+    return VE <= 2 && dim <= kStagedMax && 2 * 3 * staged_pitch<T>(dim) * sizeof(T) <= kStagedBytes ? -1 : 0;
 }
 
 // Stages of a staged row, and blocks of an SM.
@@ -291,9 +285,9 @@ int parts_of(const NormGradArgs &a) {
     const int threads = threads_of(group), rows = threads / group;
     return std::max(1, std::min((a.rows + rows - 1) / rows, sms * (512 / threads)));
 }
-int parts_of(const NormGradArgs &a, bool words) {
-    if (a.io == IoType::kF32) return words ? parts_of<float, 4>(a) : parts_of<float, 1>(a);
-    return words ? parts_of<__half, 8>(a) : parts_of<__half, 1>(a);
+int parts_of(const NormGradArgs &a, int unit) {
+    if (a.io == IoType::kF32) return unit > 2 ? parts_of<float, 4>(a) : unit == 2 ? parts_of<float, 2>(a) : parts_of<float, 1>(a);
+    return unit > 2 ? parts_of<__half, 8>(a) : unit == 2 ? parts_of<__half, 2>(a) : parts_of<__half, 1>(a);
 }
 
 template <typename T, int kThreads, int kPer>
@@ -318,15 +312,16 @@ void launch_rows(const NormGradArgs &a, int parts, float *part_w, float *part_b,
         case 32: return launch_group<T, VE, 32>(a, parts, part_w, part_b, stream);
         case 128: return launch_group<T, VE, 128>(a, parts, part_w, part_b, stream);
     }
-    if constexpr (VE == 1) {
+    if constexpr (VE > 1) {
+        if (group_of<T, VE>(a.dim) == 256) return launch_group<T, VE, 256>(a, parts, part_w, part_b, stream);
+        if (group_of<T, VE>(a.dim) == 512) return launch_group<T, VE, 512>(a, parts, part_w, part_b, stream);
+    }
+    if constexpr (VE <= 2) {
         if (group_of<T, VE>(a.dim) < 0) {
             if (staged_threads(a.dim) == 128) return launch_staged<T, 128, 16>(a, parts, part_w, part_b, stream);
             if (staged_threads(a.dim) == 256) return launch_staged<T, 256, 20>(a, parts, part_w, part_b, stream);
             return launch_staged<T, 512, 16>(a, parts, part_w, part_b, stream);
         }
-    } else {
-        if (group_of<T, VE>(a.dim) == 256) return launch_group<T, VE, 256>(a, parts, part_w, part_b, stream);
-        if (group_of<T, VE>(a.dim) == 512) return launch_group<T, VE, 512>(a, parts, part_w, part_b, stream);
     }
     if (a.rows > 0)
         norm_grad_wide_kernel<T><<<std::min(a.rows, 2 * current_device_sm_count()), kWideThreads, 0, stream>>>(a);
@@ -336,24 +331,26 @@ void launch_rows(const NormGradArgs &a, int parts, float *part_w, float *part_b,
 }
 
 template <typename T>
-void launch_type(const NormGradArgs &a, bool words, int parts, float *part_w, float *part_b, cudaStream_t stream) {
-    if (words) launch_rows<T, 16 / static_cast<int>(sizeof(T))>(a, parts, part_w, part_b, stream);
+void launch_type(const NormGradArgs &a, int unit, int parts, float *part_w, float *part_b, cudaStream_t stream) {
+    if (unit > 2) launch_rows<T, 16 / static_cast<int>(sizeof(T))>(a, parts, part_w, part_b, stream);
+    else if (unit == 2) launch_rows<T, 2>(a, parts, part_w, part_b, stream);
     else launch_rows<T, 1>(a, parts, part_w, part_b, stream);
 }
 
 }  // namespace
 
-// (The partial sums' number depends on alignment; the larger of both.)
+// (The partial sums' number depends on alignment; the largest.)
 size_t layer_norm_grad_workspace(const NormGradArgs &a) {
-    const int sums = (a.weight != nullptr) + a.want_dbias, parts = std::max(parts_of(a, true), parts_of(a, false));
+    const int sums = (a.weight != nullptr) + a.want_dbias, parts = std::max({parts_of(a, 1), parts_of(a, 2), parts_of(a, 16)});
     // rows of the two sums begin on 16-byte words
     return parts > 1 ? static_cast<size_t>(sums) * ((static_cast<size_t>(parts) * a.dim + 3) / 4 * 4) * sizeof(float) : 0;
 }
 
 cudaError_t launch_layer_norm_grad(const NormGradArgs &a, void *workspace, cudaStream_t stream) {
-    bool words = words_of(a) && aligned16(a.dx);
-    if (parts_of(a, words) == 1) words = words && aligned16(a.dweight) && aligned16(a.dbias);
-    const int parts = parts_of(a, words);
+    const size_t size = a.io == IoType::kF32 ? 4 : 2;
+    int unit = row_unit(a.dim, size, {a.dy, a.x, a.dres, a.dx}, {a.weight});
+    if (parts_of(a, unit) == 1) unit = row_unit(a.dim, size, {a.dy, a.x, a.dres, a.dx}, {a.weight, a.dweight, a.dbias});
+    const int parts = parts_of(a, unit);
     float *part_w = a.dweight, *part_b = a.dbias;
     if (parts > 1) {
         float *next = static_cast<float *>(workspace);
@@ -361,9 +358,9 @@ cudaError_t launch_layer_norm_grad(const NormGradArgs &a, void *workspace, cudaS
         if (part_b != nullptr) part_b = next;
     }
     switch (a.io) {
-        case IoType::kBF16: launch_type<__nv_bfloat16>(a, words, parts, part_w, part_b, stream); break;
-        case IoType::kF16: launch_type<__half>(a, words, parts, part_w, part_b, stream); break;
-        default: launch_type<float>(a, words, parts, part_w, part_b, stream);
+        case IoType::kBF16: launch_type<__nv_bfloat16>(a, unit, parts, part_w, part_b, stream); break;
+        case IoType::kF16: launch_type<__half>(a, unit, parts, part_w, part_b, stream); break;
+        default: launch_type<float>(a, unit, parts, part_w, part_b, stream);
     }
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || parts == 1 || (part_w == nullptr && part_b == nullptr)) return e;

@@ -21,6 +21,7 @@
 #pragma once
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "xm_common.cuh"
 #include "xm_sequences.cuh"
@@ -159,8 +160,16 @@ __device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int warp, 
 // Products of gates are kept above zero, so that an infinite start outlasts their underflow as it does step by step.
 __device__ __forceinline__ float2 above_zero(float2 P) { return make_float2(fmaxf(P.x, 1.4e-45f), fmaxf(P.y, 1.4e-45f)); }
 
-// A lane's two neighbouring channels. kWords: rows of whole 16-byte words, aligned to them.
-template <typename T, bool kWords>
+// How rows lie: of whole 16-byte words and aligned to them, of pairs of elements, or anyhow.
+constexpr int kRowWords = 2, kRowPairs = 1, kRowAny = 0;
+inline int row_of(int dim, size_t size, std::initializer_list<const void *> tensors) {
+    uintptr_t all = static_cast<uintptr_t>(dim) * size;
+    for (const void *p : tensors) all |= reinterpret_cast<uintptr_t>(p);
+    return all % 16 == 0 ? kRowWords : all % (2 * size) == 0 ? kRowPairs : kRowAny;
+}
+
+// A lane's two neighbouring channels.
+template <typename T, int kRow>
 struct Lane {
     int c[2];  // (0 where there is none)
     bool active[2];
@@ -181,7 +190,7 @@ struct Lane {
     }
     // `row`: a token's first channel; only by lanes whose first channel is active
     __device__ __forceinline__ void store(T *row, float2 v) const {
-        if constexpr (kWords) {
+        if constexpr (kRow != kRowAny) {
             if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t *>(row + c[0]) = pack2<T>(v.x, v.y);
             else *reinterpret_cast<float2 *>(row + c[0]) = v;
         } else {
@@ -194,31 +203,32 @@ struct Lane {
 // A group's tokens of one tensor in shared memory, and the warp's copy that fills it, in 16-byte words. Rows of 16-bit types
 // that are not whole words are copied from the one that holds their first element, and lie behind `shift` others; those of
 // float32 are copied in 4-byte words.
-template <typename T, int kRows, bool kWords>
+template <typename T, int kRows, int kRow>
 struct GateTile {
-    static constexpr bool kShifts = !kWords && sizeof(T) == 2;
+    static constexpr bool kShifts = kRow != kRowWords && sizeof(T) == 2;
     alignas(16) T v[kRows][kGateChannels + (kShifts ? 8 : 0)];
     __device__ __forceinline__ float2 at(int row, int shift) const {
         const int c = 2 * (threadIdx.x & 31);
-        if constexpr (kShifts) return make_float2(to_f32<T>(v[row][c + shift]), to_f32<T>(v[row][c + 1 + shift]));
-        else if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][c]));
+        if constexpr (kShifts && kRow == kRowAny)
+            return make_float2(to_f32<T>(v[row][c + shift]), to_f32<T>(v[row][c + 1 + shift]));
+        else if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t *>(&v[row][c + shift]));
         else return *reinterpret_cast<const float2 *>(&v[row][c]);
     }
 };
 // The shift of a token's row.
-template <typename T, bool kWords>
+template <typename T, int kRow>
 __device__ __forceinline__ int shift_of(const T *src, int t, int dim) {
-    if (kWords || sizeof(T) != 2) return 0;
+    if (kRow == kRowWords || sizeof(T) != 2) return 0;
     const unsigned first = static_cast<unsigned>(reinterpret_cast<uintptr_t>(src) >> 1);
     return (first + static_cast<unsigned>(t) * static_cast<unsigned>(dim)) & 7;  // (a tile's first channel is a multiple of 8)
 }
 // Rows first .. first + kRows - 1 of a tensor's channels; those outside [lo, hi) are left out. Reads nothing outside the
 // tensor's rows 0 .. hi - 1.
-template <typename T, int kRows, bool kWords>
-__device__ __forceinline__ void copy_tile(GateTile<T, kRows, kWords> &dst, const T *src, int first, int lo, int hi, int dim,
+template <typename T, int kRows, int kRow>
+__device__ __forceinline__ void copy_tile(GateTile<T, kRows, kRow> &dst, const T *src, int first, int lo, int hi, int dim,
                                           int tile) {
     const int lane = threadIdx.x & 31;
-    if constexpr (kWords) {
+    if constexpr (kRow == kRowWords) {
         constexpr int kPer = 16 / static_cast<int>(sizeof(T)), kWordsRow = kGateChannels / kPer;
         constexpr int kStep = 32 / kWordsRow;  // rows per pass
         const int col = lane % kWordsRow * kPer, row = lane / kWordsRow;

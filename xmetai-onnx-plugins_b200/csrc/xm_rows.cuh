@@ -3,8 +3,11 @@
 //
 // A group of kGroup threads owns a row: thread g has the chunks g, g + kGroup, ... of
 // VE consecutive elements. VE is a 16-byte word where rows and tensors are aligned to
-// words, else one element (still consecutive over the threads).
+// words, two elements where they are aligned to those, else one element (still
+// consecutive over the threads).
 #pragma once
+
+#include <initializer_list>
 
 #include "xm_common.cuh"
 
@@ -13,7 +16,17 @@ namespace xm {
 // Elements of a row that a thread holds: two words of each tensor (one in groups of up to 16, whose rows are short), or
 // eight single elements.
 template <typename T, int VE, int kGroup>
-constexpr int kRowElems = VE == 1 ? 8 : kGroup <= 16 ? VE : 2 * VE;
+constexpr int kRowElems = VE == 1 ? 8 : (kGroup <= 16 ? 16 : 32) / static_cast<int>(sizeof(T));
+
+// VE of rows of dim elements of `size` bytes, and of vectors of floats beside them.
+inline int row_unit(int dim, size_t size, std::initializer_list<const void *> tensors,
+                    std::initializer_list<const void *> vectors) {
+    uintptr_t rows = static_cast<uintptr_t>(dim) * size, floats = 0;
+    for (const void *p : tensors) rows |= reinterpret_cast<uintptr_t>(p);
+    for (const void *p : vectors) floats |= reinterpret_cast<uintptr_t>(p);
+    if ((rows | floats) % 16 == 0) return 16 / static_cast<int>(size);
+    return rows % (2 * size) == 0 && floats % 8 == 0 ? 2 : 1;
+}
 
 template <typename T, int VE>
 struct Chunk;  // VE elements as they are stored
@@ -25,6 +38,14 @@ template <typename T>
 struct Chunk<T, 8> {
     uint4 w;
 };
+template <>
+struct Chunk<float, 2> {
+    float2 w;
+};
+template <typename T>
+struct Chunk<T, 2> {
+    uint32_t w;
+};
 template <typename T>
 struct Chunk<T, 1> {
     T w;
@@ -34,6 +55,11 @@ template <typename T, int VE>
 __device__ __forceinline__ void chunk_floats(const Chunk<T, VE> &c, float *v) {
     if constexpr (VE == 1) {
         v[0] = to_f32<T>(c.w);
+    } else if constexpr (VE == 2) {
+        float2 f;
+        if constexpr (sizeof(T) == 4) f = c.w;
+        else f = unpack2<T>(c.w);
+        v[0] = f.x; v[1] = f.y;
     } else if constexpr (VE == 4) {
         v[0] = c.w.x; v[1] = c.w.y; v[2] = c.w.z; v[3] = c.w.w;
     } else {
@@ -50,16 +76,21 @@ template <typename T, int VE>
 __device__ __forceinline__ Chunk<T, VE> to_chunk(const float *v) {
     Chunk<T, VE> c;
     if constexpr (VE == 1) c.w = from_f32<T>(v[0]);
+    else if constexpr (VE == 2 && sizeof(T) == 4) c.w = make_float2(v[0], v[1]);
+    else if constexpr (VE == 2) c.w = pack2<T>(v[0], v[1]);
     else if constexpr (VE == 4) c.w = make_float4(v[0], v[1], v[2], v[3]);
     else c.w = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
     return c;
 }
 
-// VE consecutive floats (aligned to words where VE > 1).
+// VE consecutive floats (aligned to words, or pairs, where VE > 1).
 template <int VE>
 __device__ __forceinline__ void load_row_floats(const float *p, float *v) {
     if constexpr (VE == 1) {
         v[0] = __ldg(p);
+    } else if constexpr (VE == 2) {
+        const float2 w = __ldg(reinterpret_cast<const float2 *>(p));
+        v[0] = w.x; v[1] = w.y;
     } else {
 #pragma unroll
         for (int i = 0; i < VE; i += 4) {
@@ -72,6 +103,8 @@ template <int VE>
 __device__ __forceinline__ void store_row_floats(float *p, const float *v) {
     if constexpr (VE == 1) {
         p[0] = v[0];
+    } else if constexpr (VE == 2) {
+        *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
     } else {
 #pragma unroll
         for (int i = 0; i < VE; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
@@ -140,7 +173,7 @@ struct RowPart {
 
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
 
-// Rows that are not whole words, staged in shared memory: asynchronous copies of 16-byte words, from the one that holds a
+// Rows that are not pairs of elements, staged in shared memory: asynchronous copies of 16-byte words, from the one that holds a
 // row's first element, behind up to a word's others. Elements are read from there by consecutive threads, about sixteen to each: fewer leave most of a row's time to its barriers (32768 x 1026, backward:
 // 229 us with 512 threads), more too few warps.
 constexpr int staged_threads(int dim) { return dim <= 2048 ? 128 : dim <= 5120 ? 256 : 512; }
