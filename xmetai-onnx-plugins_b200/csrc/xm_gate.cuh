@@ -302,9 +302,9 @@ inline size_t gate_pairs(const GateCut &g) {  // elements of each of P, h and st
     return g.segments > 1 && g.block == 0 ? static_cast<size_t>(g.spans) * g.segments * g.tiles * 32 : 0;
 }
 
-// Whether the second pass's blocks may begin while the first ends: worth a microsecond where segments are short (512 x
-// 4096 in 16: 9.4 us against 10.2). Long ones want their blocks spread evenly, which slots that fall free one by one do
-// not give (16384 x 4096 packed in 18: 131 us against 121).
+// Whether the second pass's blocks may begin while the first ends: worth a microsecond or two where segments are short (512 x
+// 4096 in 16: 8.8 us against 9.6; 2 x 257 x 63: 7.2 against 9.2). Long ones want their blocks spread evenly, which slots
+// that fall free one by one do not give (16384 x 4096 packed in 27: 116 us against 110, backward 204 against 188).
 inline bool gate_behind(const GateCut &g) { return g.segments > 1 && g.length / g.segments <= 64; }
 
 // Hands a value on from the warp of group n to that of group n + 1 of a ring: slot and barrier are the receiver's. The
