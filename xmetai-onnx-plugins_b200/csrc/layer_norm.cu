@@ -101,9 +101,9 @@ __global__ void __launch_bounds__(threads_of(kGroup), kThreadsSm<T, VE> / thread
 }
 
 // Rows that are not pairs of elements, above 1024: staged some rows ahead, and read from shared memory for every
-// pass: 16384 x 4097 in bf16 with a residual takes 174 us, 47 % of copy bandwidth (247 in registers, an element a load).
+// pass: 16384 x 4097 in bf16 with a residual takes 163 us, 50 % of copy bandwidth (247 in registers, an element a load).
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads, 2048 / kThreads) norm_staged_kernel(const NormArgs p, int stages) {
+__global__ void __launch_bounds__(kThreads, 1536 / kThreads) norm_staged_kernel(const NormArgs p, int stages) {
     extern __shared__ float4 smem_f4[];
     __shared__ float2 part[2 * (kThreads / 32)];
     const int dim = p.dim;
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 2048 / kThreads) norm_staged_kernel(
         float sum = 0.0f;
         if (R != nullptr) {
             T *const kept = static_cast<T *>(p.sum) + at;
-#pragma unroll 4
+#pragma unroll 8
             for (int d = threadIdx.x; d < dim; d += kThreads) {
                 const T v = from_f32<T>(to_f32<T>(s[d]) + to_f32<T>(r[d]));
                 kept[d] = v;
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 2048 / kThreads) norm_staged_kernel(
                 sum += to_f32<T>(v);
             }
         } else if (!p.rms) {
-#pragma unroll 4
+#pragma unroll 8
             for (int d = threadIdx.x; d < dim; d += kThreads) sum += to_f32<T>(s[d]);
         }
         float mean = 0.0f;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 2048 / kThreads) norm_staged_kernel(
             turn ^= 1;
         }
         float sq = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
         for (int d = threadIdx.x; d < dim; d += kThreads) {
             const float v = to_f32<T>(s[d]) - mean;
             sq = fmaf(v, v, sq);
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 2048 / kThreads) norm_staged_kernel(
         const float rstd = 1.0f / sqrtf(group_sum<kThreads>(make_float2(sq, 0.0f), part, turn).x * inv + p.eps);
         turn ^= 1;
         T *const out = static_cast<T *>(p.out) + at;
-#pragma unroll 4
+#pragma unroll 8
         for (int d = threadIdx.x; d < dim; d += kThreads) {
             const float v = (to_f32<T>(s[d]) - mean) * rstd;
             out[d] = from_f32<T>(
@@ -234,7 +234,7 @@ cudaError_t launch_staged(const NormArgs &a, cudaStream_t stream) {
     const cudaError_t e = prepare_staged<norm_staged_kernel<T, kThreads>>();
     if (e != cudaSuccess) return e;
     const int64_t most = static_cast<int64_t>(current_device_sm_count()) *
-                         std::min<int64_t>(kStagedBytes / smem, 2048 / kThreads);
+                         std::min<int64_t>(kStagedBytes / smem, 1536 / kThreads);
     norm_staged_kernel<T, kThreads><<<static_cast<unsigned>(std::min<int64_t>(a.rows, most)), kThreads, smem, stream>>>(
         a, stages);
     return cudaGetLastError();
