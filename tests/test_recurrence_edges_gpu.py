@@ -1,0 +1,49 @@
+"""Edges of the gated recurrence on the GPU: gates shut on purpose, whose small
+shares decide the result. Definitions and error bounds: recurrence_reference.py."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import recurrence_reference as Q
+from test_recurrence_gpu import DT, close, dev, gen, normal
+
+pytestmark = pytest.mark.gpu
+
+LOGITS = torch.tensor([-60.0, -70.0, -87.0, -200.0])
+BOUNDS = torch.tensor([0.999, 0.99999, 1 - 2.0**-24, 0.0])
+# one of each way that a call is cut: a warp to a row, a block to a row, segments in two kernels, blocks whose warps take
+# turns (of eight and of four)
+CUTS = [(2, 40, 70), (1, 700, 70), (1, 2600, 70), (8, 256, 1280), (8, 256, 2560)]
+
+
+def shut(g, batch, seqlen, dim, dtype):
+    """Gates that keep next to nothing of their own, in channels whose lower bounds keep all but a little: from a state of
+    zero, what is taken up is the whole result."""
+    x = normal(g, batch, seqlen, dim, dtype=dtype)
+    f = LOGITS[torch.randint(0, 4, (batch, seqlen, dim), generator=g)].to(dtype)
+    return x, f, BOUNDS[torch.arange(dim) % 4].contiguous()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("batch,seqlen,dim", CUTS)
+def test_shut_gates(xm, cuda, dt, batch, seqlen, dim):
+    """The share taken up, (1 - lower bound) sigmoid(-f), keeps its relative precision however far f is below zero."""
+    g = gen(71)
+    x, f, low = shut(g, batch, seqlen, dim, DT[dt])
+    y, bound, final, fb = Q.recurrence(x, f, low)
+    got, last = xm.GatedRecurrenceFn(dev(x), dev(f), dev(low), output_final_state=1)
+    close(got, y, bound)
+    close(last, final, fb)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("batch,dim", [(3, 72), (3, 67), (500, 1024)])
+def test_shut_gates_of_single_tokens(xm, cuda, dt, batch, dim):
+    g = gen(72)
+    x, f, low = shut(g, batch, 1, dim, DT[dt])
+    y, bound, final, fb = Q.recurrence(x, f, low)
+    got, state = xm.GatedRecurrenceUpdateFn(dev(x[:, 0]), dev(f[:, 0]), dev(low), torch.zeros(batch, dim, device="cuda"))
+    close(got, y[:, 0], bound[:, 0])
+    close(state, final, fb)

@@ -34,7 +34,9 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // precision: with t = exp(-f), r = 1 / (1 + t) and t r, no difference of nearby values
 // is formed. The exponent stops at 2^126, where r is float32's smallest normal value
 // and t r one: nothing overflows, and NaN stays NaN.
-// For two channels: r' = rest r, a = low + r' (the share kept), u = t r' (taken up).
+// For two channels: a = low + rest r (the share kept), u = (rest t) r (taken up). rest meets t first: where f is far below
+// zero, r is next to the smallest normal value, and rest r would lose its bits below it before t brought them back (bound
+// 0.99999, f = -87: u off by 3e-3). Far above zero r is 1, and rest t loses no more than u itself has to.
 struct Gate2 {
     float2 r, a, u;
 };
@@ -49,9 +51,8 @@ __device__ __forceinline__ Gate2 gate_of(float2 f, float2 low, float2 rest) {
     const float2 s = __fadd2_rn(t, both(1.0f));
     Gate2 g;
     g.r = make_float2(rcp_approx(s.x), rcp_approx(s.y));
-    const float2 k = __fmul2_rn(g.r, rest);
-    g.a = __fadd2_rn(k, low);
-    g.u = __fmul2_rn(k, t);
+    g.a = __ffma2_rn(g.r, rest, low);
+    g.u = __fmul2_rn(__fmul2_rn(t, rest), g.r);
     return g;
 }
 
