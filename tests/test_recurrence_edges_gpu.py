@@ -47,3 +47,21 @@ def test_shut_gates_of_single_tokens(xm, cuda, dt, batch, dim):
     got, state = xm.GatedRecurrenceUpdateFn(dev(x[:, 0]), dev(f[:, 0]), dev(low), torch.zeros(batch, dim, device="cuda"))
     close(got, y[:, 0], bound[:, 0])
     close(state, final, fb)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("batch,seqlen,dim", CUTS)
+@pytest.mark.parametrize("scale", [1.0, 2.0**-80])
+def test_shut_gates_backward(xm, cuda, dt, batch, seqlen, dim, scale):
+    """The lower bounds' gradient is sum G (h - x) sigmoid(-f) whatever the bounds are, 1 among them, and however small G
+    is; behind a bound of 1 the inputs have none."""
+    g = gen(73)
+    x, f, low = shut(g, batch, seqlen, dim, DT[dt])
+    low[low == 0] = 1.0
+    y = Q.recurrence(x, f, low)[0].to(DT[dt])
+    dy = normal(g, batch, seqlen, dim, std=scale).to(DT[dt])  # (2^-80 is below float16's range: zero)
+    want = Q.recurrence_grad(dy, x, f, y, low)
+    got = xm.GatedRecurrenceGradFn(dev(dy), dev(x), dev(f), dev(y), dev(low))
+    for k in range(3):
+        close(got[k], *want[k])
+    assert not bool(got[0][..., low == 1].any()) and not bool(got[1][..., low == 1].any())

@@ -35,12 +35,6 @@ constexpr int kPerSm = sizeof(T) == 4 ? 7 : 12;
 // Groups in use and under way, of the tensors f, dy; x, and y of the token before.
 constexpr int kStages = 4;
 
-// 1 - bound, which da (1 - a), summed in place of da sigmoid(-f), is divided by in the end. A bound that training has brought
-// to 1 counts as 1 - 2^-60 (a is 1, dx and df are 2^-60 of what a bound of zero gives), so that it has a gradient too.
-__device__ __forceinline__ float2 rest_of(float2 low) {
-    return make_float2(low.x == 1.0f ? 0x1p-60f : 1.0f - low.x, low.y == 1.0f ? 0x1p-60f : 1.0f - low.y);
-}
-
 template <typename T, int kRow>
 __device__ __forceinline__ float2 state_row(const GateGradArgs &p, const Lane<T, kRow> &ch, const float *base, int seq) {
     return ch.floats(base != nullptr ? base + static_cast<size_t>(seq) * p.dim : nullptr, 0.0f);
@@ -57,7 +51,7 @@ __device__ __forceinline__ void pass_empty(const GateGradArgs &p, const Lane<T, 
 }
 
 // A warp walks segment j of a span. kEnds: the first pass. first_pass(): it is through; nothing of it is read before.
-// dlow: sum of da (1 - a).
+// dlow: sum of da sigmoid(-f).
 template <typename T, int kRow, bool kEnds, int kStages, int kTensors, typename Wait>
 __device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCut &g, GradTile<T, kRow> (*ring)[kTensors],
                                              const Lane<T, kRow> &ch, int tile, float2 low, float2 rest, Span span,
@@ -131,23 +125,23 @@ __device__ __forceinline__ void walk_segment(const GateGradArgs &p, const GateCu
                 P = __fmul2_rn(P, a[k]);
             }
         } else {
-            float2 G[kGroup], u[kGroup], r[kGroup];  // (of no meaning before the segment)
+            float2 G[kGroup], take[kGroup], keep[kGroup];  // (of no meaning before the segment)
 #pragma unroll
             for (int k = 0; k < kGroup; ++k) {
                 const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
                 G[k] = gate.a;
-                u[k] = gate.u;
-                r[k] = gate.r;
+                take[k] = gate.take;
+                keep[k] = gate.keep;
             }
             T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
             auto token = [&](int k, float2 before) {
                 const float2 x = load(2, X, k, 0);
                 const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
-                const float2 w = __fmul2_rn(__fmul2_rn(G[k], diff), u[k]);
-                dlow = __fadd2_rn(dlow, w);
+                dlow = __fadd2_rn(dlow, __fmul2_rn(__fmul2_rn(G[k], diff), take[k]));
+                const float2 d = __fmul2_rn(__fmul2_rn(G[k], rest), take[k]);
                 if (ch.active[0]) {
-                    ch.store(dx, __fmul2_rn(u[k], G[k]));
-                    ch.store(df, __fmul2_rn(w, r[k]));
+                    ch.store(dx, d);
+                    ch.store(df, __fmul2_rn(__fmul2_rn(d, diff), keep[k]));
                 }
             };
             if (last == kGroup && seq.start < hi - kGroup) {
@@ -201,7 +195,7 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
     const int tile = blockIdx.x % g.tiles, segs = kEnds ? g.segments - 1 : g.segments;
     const int j = blockIdx.x / g.tiles % segs + (kEnds ? 1 : 0), slot = blockIdx.x / g.tiles / segs;
     const Lane<T, kRow> ch(tile, threadIdx.x & 31, p.dim);
-    const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     bool waited = kEnds;
     auto first_pass = [&] {
         if (!waited) wait_for_before();
@@ -217,8 +211,7 @@ __global__ void __launch_bounds__(32, 8) gate_grad_kernel(const GateGradArgs p, 
             segment_length(g, span), j, global_pairs(g, i, tile), dlow, first_pass);
     }
     first_pass();  // (also warps without tokens: what follows waits for this kernel only)
-    if (!kEnds && part != nullptr)  // da (1 - a) = da (1 - bound) sigmoid(-f)
-        ch.store_floats(part + static_cast<size_t>(slot * segs + j) * p.dim, make_float2(dlow.x / rest.x, dlow.y / rest.y));
+    if (!kEnds && part != nullptr) ch.store_floats(part + static_cast<size_t>(slot * segs + j) * p.dim, dlow);
 }
 
 // Both passes in one block, a segment to each of its warps: as many as have room for their copies.
@@ -243,7 +236,7 @@ __global__ void __launch_bounds__(32 * GradBlock<T>::kWarps, 1) gate_grad_block_
     dependents_may_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
     const Lane<T, kRow> ch(tile, lane, p.dim);
-    const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     pass_empty(p, ch, slot * kWarps + warp, g.width * kWarps);
     float2 dlow = both(0.0f);
     for (int i = slot; i < g.spans; i += g.width) {
@@ -264,7 +257,7 @@ __global__ void __launch_bounds__(32 * GradBlock<T>::kWarps, 1) gate_grad_block_
         if (warp == 0) {
             float2 sum = sm.pairs.h[0][lane];
             for (int w = 1; w < kWarps; ++w) sum = __fadd2_rn(sum, sm.pairs.h[w][lane]);
-            ch.store_floats(part + static_cast<size_t>(slot) * p.dim, make_float2(sum.x / rest.x, sum.y / rest.y));
+            ch.store_floats(part + static_cast<size_t>(slot) * p.dim, sum);
         }
     }
 }
@@ -289,7 +282,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile = blockIdx.x % g.tiles, slot = blockIdx.x / g.tiles;
     const Lane<T, kRow> ch(tile, lane, p.dim);
-    const float2 low = ch.floats(p.bound, 0.0f), rest = rest_of(low);
+    const float2 low = ch.floats(p.bound, 0.0f), rest = make_float2(1.0f - low.x, 1.0f - low.y);
     const T *const DY = static_cast<const T *>(p.dy), *const X = static_cast<const T *>(p.x),
                    *const F = static_cast<const T *>(p.f), *const H = static_cast<const T *>(p.y);
     T *const DX = static_cast<T *>(p.dx), *const DF = static_cast<T *>(p.df);
@@ -302,7 +295,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
     if (p.dinit != nullptr)  // sequences without tokens: the gradient passes through
         for_empty_sequences(q, slot * kWarps + warp, g.width * kWarps,
                             [&](int s) { store_dinit(s, state_row(p.dfinal, s)); });
-    float2 dlow = both(0.0f);  // sum of da (1 - a)
+    float2 dlow = both(0.0f);  // sum of da sigmoid(-f)
     for (int i = slot; i < g.spans; i += g.width) {
         const Span span = gate_span(q, g, i);
         constexpr int kTurn = kWarps * kGroup;  // tokens of a round
@@ -331,23 +324,23 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
             if (seq.start >= hi) seq = seq_at(q, hi - 1);
             const bool more = hi - kGroup > span.lo;  // a group before
             const int next = warp + 1 == kWarps ? 0 : warp + 1;
-            float2 P[kGroup], G[kGroup], u[kGroup], r[kGroup];  // (of no meaning before the span)
+            float2 P[kGroup], G[kGroup], take[kGroup], keep[kGroup];  // (of no meaning before the span)
 #pragma unroll
             for (int k = 0; k < kGroup; ++k) {
                 const Gate2 gate = gate_of(load(0, F, k, 0), low, rest);
                 P[k] = gate.a;
-                u[k] = gate.u;
-                r[k] = gate.r;
+                take[k] = gate.take;
+                keep[k] = gate.keep;
             }
             T *dx = DX + static_cast<size_t>(hi - 1) * p.dim, *df = DF + static_cast<size_t>(hi - 1) * p.dim;
             auto token = [&](int k, float2 Gk, float2 before) {
                 const float2 x = load(2, X, k, 0);
                 const float2 diff = __fadd2_rn(before, make_float2(-x.x, -x.y));
-                const float2 w = __fmul2_rn(__fmul2_rn(Gk, diff), u[k]);
-                dlow = __fadd2_rn(dlow, w);
+                dlow = __fadd2_rn(dlow, __fmul2_rn(__fmul2_rn(Gk, diff), take[k]));
+                const float2 d = __fmul2_rn(__fmul2_rn(Gk, rest), take[k]);
                 if (ch.active[0]) {
-                    ch.store(dx, __fmul2_rn(u[k], Gk));
-                    ch.store(df, __fmul2_rn(w, r[k]));
+                    ch.store(dx, d);
+                    ch.store(df, __fmul2_rn(__fmul2_rn(d, diff), keep[k]));
                 }
             };
             // (whether a group takes and gives depends on hi alone, so that offsets that descend leave nobody waiting)
@@ -403,7 +396,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
         if (warp == 0) {
             float2 sum = sm.hand.slot[0][lane];
             for (int w = 1; w < kWarps; ++w) sum = __fadd2_rn(sum, sm.hand.slot[w][lane]);
-            ch.store_floats(part + static_cast<size_t>(slot) * p.dim, make_float2(sum.x / rest.x, sum.y / rest.y));
+            ch.store_floats(part + static_cast<size_t>(slot) * p.dim, sum);
         }
     }
 }

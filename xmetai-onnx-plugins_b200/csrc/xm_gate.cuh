@@ -34,11 +34,11 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // precision: with t = exp(-f), r = 1 / (1 + t) and t r, no difference of nearby values
 // is formed. The exponent stops at 2^126, where r is float32's smallest normal value
 // and t r one: nothing overflows, and NaN stays NaN.
-// For two channels: a = low + rest r (the share kept), u = (rest t) r (taken up). rest meets t first: where f is far below
+// For two channels: a = low + rest keep (the share kept), u = rest take (taken up), as (rest t) r. rest meets t first: where f is far below
 // zero, r is next to the smallest normal value, and rest r would lose its bits below it before t brought them back (bound
 // 0.99999, f = -87: u off by 3e-3). Far above zero r is 1, and rest t loses no more than u itself has to.
 struct Gate2 {
-    float2 r, a, u;
+    float2 keep, take, a, u;
 };
 __device__ __forceinline__ float min_nan(float a, float b) {
     float r;
@@ -50,9 +50,10 @@ __device__ __forceinline__ Gate2 gate_of(float2 f, float2 low, float2 rest) {
     const float2 t = make_float2(ex2_approx(min_nan(e.x, 126.0f)), ex2_approx(min_nan(e.y, 126.0f)));
     const float2 s = __fadd2_rn(t, both(1.0f));
     Gate2 g;
-    g.r = make_float2(rcp_approx(s.x), rcp_approx(s.y));
-    g.a = __ffma2_rn(g.r, rest, low);
-    g.u = __fmul2_rn(__fmul2_rn(t, rest), g.r);
+    g.keep = make_float2(rcp_approx(s.x), rcp_approx(s.y));
+    g.a = __ffma2_rn(g.keep, rest, low);
+    g.u = __fmul2_rn(__fmul2_rn(t, rest), g.keep);
+    g.take = __fmul2_rn(t, g.keep);
     return g;
 }
 
