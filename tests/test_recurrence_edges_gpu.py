@@ -65,3 +65,48 @@ def test_shut_gates_backward(xm, cuda, dt, batch, seqlen, dim, scale):
     for k in range(3):
         close(got[k], *want[k])
     assert not bool(got[0][..., low == 1].any()) and not bool(got[1][..., low == 1].any())
+
+
+def shut_behind_a_group(dim, tokens=256, batch=8):
+    """Gates open for a while, then shut: products of gates that leave float32's range meet states that have not."""
+    f = torch.full((batch, tokens, dim), 30.0)
+    f[:, 40:200] = -30.0
+    return torch.zeros(batch, tokens, dim), f
+
+
+@pytest.mark.parametrize("dim", [1280, 2560])
+def test_channels_do_not_touch_each_other(xm, cuda, dim):
+    """Nor do sequences: an infinite channel leaves every bit of the others as it is, forward and backward."""
+    x, f = (dev(t) for t in shut_behind_a_group(dim))
+    ones = torch.ones(8, dim, device="cuda")
+    odd = ones.clone()
+    odd[::2, ::7] = float("inf")
+    odd[1, 3] = float("nan")
+    same = odd == ones
+    y, last = xm.GatedRecurrenceFn(x, f, None, ones, output_final_state=1)
+    y2, last2 = xm.GatedRecurrenceFn(x, f, None, odd, output_final_state=1)
+    rows = same[:, None].expand_as(y)
+    assert torch.equal(y[rows], y2[rows]) and torch.equal(last[same], last2[same])
+    assert bool(torch.isinf(y2[0, :, 0]).all())
+    got = xm.GatedRecurrenceGradFn(x, x, f, y, None, ones, None, ones)
+    got2 = xm.GatedRecurrenceGradFn(x, x, f, y, None, ones, None, odd)
+    assert all(torch.equal(a[rows], b[rows]) for a, b in zip(got[:2], got2[:2]))
+    assert torch.equal(got[3][same], got2[3][same])
+
+
+@pytest.mark.parametrize("dim", [1250, 1251])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_bits_do_not_depend_on_what_ran_before(xm, cuda, dt, dim):
+    """Channels that are not there are not looked at: shared memory still holds what a kernel before left in their place."""
+    x, f = (dev(t).to(DT[dt]) for t in shut_behind_a_group(dim))
+    ones = torch.ones(8, dim, device="cuda")
+    y = xm.GatedRecurrenceFn(x, f, None, ones)
+    results = []
+    for fill in (0.0, float("inf"), float("nan")):
+        before = torch.full((8, 256, 2560), fill, dtype=DT[dt], device="cuda")
+        xm.GatedRecurrenceFn(before, before)
+        forward = xm.GatedRecurrenceFn(x, f, None, ones, output_final_state=1)
+        xm.GatedRecurrenceGradFn(before, before, before, before)
+        results.append((*forward, *xm.GatedRecurrenceGradFn(x, x, f, y, None, ones, None, ones)))
+    for r in results[1:]:
+        assert all(a is b or torch.equal(a, b) for a, b in zip(r, results[0]))

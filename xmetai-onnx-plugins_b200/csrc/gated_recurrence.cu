@@ -281,10 +281,9 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? 5 : 2) gate_ring_ke
                     P[k] = __fmul2_rn(P[k], P[k - 1]);
                 }
                 const float2 start = sm.hand.take(warp);
-                const bool finite = __all_sync(kFullMask, finite2(start));
-                if (!finite) {
+                if (!__all_sync(kFullMask, finite2(start))) {  // (also for what lanes without channels find)
 #pragma unroll
-                    for (int k = 0; k < kGateGroup; ++k) P[k] = above_zero(P[k]);
+                    for (int k = 0; k < kGateGroup; ++k) P[k] = above_zero(P[k], start);
                 }
                 if (more) sm.hand.give(next, __ffma2_rn(P[kGateGroup - 1], start, h[kGateGroup - 1]));
                 if (ch.active[0]) {

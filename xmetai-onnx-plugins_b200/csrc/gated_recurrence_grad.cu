@@ -354,9 +354,9 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) gate_grad_ring_kerne
                     if (k > 0) P[k] = __fmul2_rn(P[k], P[k - 1]);
                 }
                 const float2 start = sm.hand.take(warp);
-                if (!__all_sync(kFullMask, finite2(start))) {
+                if (!__all_sync(kFullMask, finite2(start))) {  // (also for what lanes without channels find)
 #pragma unroll
-                    for (int k = 0; k < kGroup; ++k) P[k] = above_zero(P[k]);
+                    for (int k = 0; k < kGroup; ++k) P[k] = above_zero(P[k], start);
                 }
                 if (more) sm.hand.give(next, __ffma2_rn(P[kGroup - 1], start, c));
 #pragma unroll

@@ -161,6 +161,13 @@ __device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int warp, 
 
 // Products of gates are kept above zero, so that an infinite start outlasts their underflow as it does step by step.
 __device__ __forceinline__ float2 above_zero(float2 P) { return make_float2(fmaxf(P.x, 1.4e-45f), fmaxf(P.y, 1.4e-45f)); }
+__device__ __forceinline__ bool finite1(float v) { return fabsf(v) <= 3.4028235e38f; }
+__device__ __forceinline__ bool finite2(float2 v) { return finite1(v.x) && finite1(v.y); }
+// The same in the channel whose start is not finite alone: a neighbour's zeros are its own.
+__device__ __forceinline__ float2 above_zero(float2 P, float2 start) {
+    const float2 Q = above_zero(P);
+    return make_float2(finite1(start.x) ? P.x : Q.x, finite1(start.y) ? P.y : Q.y);
+}
 
 // How rows lie: of whole 16-byte words and aligned to them, of pairs of elements, or anyhow.
 constexpr int kRowWords = 2, kRowPairs = 1, kRowAny = 0;
@@ -338,7 +345,6 @@ struct Ring {
         return slot[warp][threadIdx.x & 31];
     }
 };
-__device__ __forceinline__ bool finite2(float2 v) { return fabsf(v.x) <= 3.4028235e38f && fabsf(v.y) <= 3.4028235e38f; }
 
 // Launches kKernel with `warps` to a block. behind: it waits by itself for the kernel before.
 template <auto kKernel, typename... Args>
