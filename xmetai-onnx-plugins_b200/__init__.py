@@ -532,10 +532,10 @@ class _ServeOp:
 
 
 def _serve(op, attrs, tensors, outs, shapes, stream, inplace=-1):
-    """Call xm_<op>_fwd on the device of tensors[0]; attrs: the attribute struct's address. An output that is None is
-    allocated: with the shape and type of tensors[0], or where `shapes` says (own, sizes...), float32, or with own=1 of
-    that type. Everything allocated belongs to the stream that the call runs on. inplace: an input that must not be
-    copied. Returns the outputs."""
+    """Call xm_<op>_fwd on the device of tensors[0]; attrs: the attribute struct, this call's own. An output that is
+    None is allocated: with the shape and type of tensors[0], or where `shapes` says (own, sizes...), float32, or with
+    own=1 of that type. Everything allocated belongs to the stream that the call runs on. inplace: an input that must
+    not be copied. Returns the outputs."""
     if op.call is None:
         op.load()
     if stream is not None:
@@ -551,7 +551,7 @@ def _serve(op, attrs, tensors, outs, shapes, stream, inplace=-1):
                     with torch.cuda.stream(stream):
                         return _serve(op, attrs, tensors, outs, shapes, None, inplace)
                 return _serve(op, attrs, tensors, outs, shapes, None, inplace)
-    got = op.call(op.fwd, op.size, attrs, tensors, op.blanks, outs, shapes, inplace)
+    got = op.call(op.fwd, op.size, ctypes.addressof(attrs), tensors, op.blanks, outs, shapes, inplace)
     if len(got) == 2 and type(got[0]) is int:
         if got[0] == -5:
             import torch
@@ -574,19 +574,6 @@ def _serve_state(op, attrs, tensors, out, state, state_shape, with_state, stream
             state = tensors[inplace]
     return _serve(op, attrs, tensors, (out, state),
                   (None, None if state_shape is None else (int(op.kinds[op.state] == "x"), *state_shape)), stream, inplace)
-
-
-_attrs = {}
-
-
-def _address(kind, *values):
-    """Address of an attribute struct with these values, which stays as it is (and lives as long as the process)."""
-    key = (kind, *values)
-    a = _attrs.get(key)
-    if a is None:
-        a = kind(*values)
-        a = _attrs[key] = (ctypes.addressof(a), a)
-    return a[0]
 
 
 _CONV = _ServeOp("causal_conv1d", ("x", "weight", "bias", "initial_state", "cu_seqlens", "state_indices",
@@ -632,7 +619,7 @@ def CausalConv1dFn(x, weight, bias=None, initial_state=None, cu_seqlens=None, st
     output_final_state=1 its final state replaces that row in place (the result is (out, initial_state)). An index
     outside the pool owns no row: zeros, and no final state is kept. No slot may be named twice in a call.
     """
-    attrs = _address(CausalConv1dAttrs, int(silu), int(channels_last), int(output_final_state))
+    attrs = CausalConv1dAttrs(int(silu), int(channels_last), int(output_final_state))
     shape = None
     if output_final_state:
         if getattr(x, "ndim", 0) != 3 or getattr(weight, "ndim", 0) != 2:
@@ -651,7 +638,7 @@ def CausalConv1dUpdateFn(x, weight, bias=None, state=None, state_indices=None, *
     skipped and their output rows left as they were."""
     if state is None:
         _invalid("CausalConv1dUpdateFn needs a state")
-    return _serve_state(_CONV_UPDATE, _address(CausalConv1dUpdateAttrs, int(silu)), (x, weight, bias, state, state_indices), out,
+    return _serve_state(_CONV_UPDATE, CausalConv1dUpdateAttrs(int(silu)), (x, weight, bias, state, state_indices), out,
                   new_state, None if new_state is None or new_state is state else (), True, stream)
 
 
@@ -666,7 +653,7 @@ def SelectiveScanVarlenFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, in
     initial_state is float32 [sequences, dim, d_state] (SelectiveScanFn's last_state); output_final_state,
     cu_seqlens, state_indices and has_initial_state work as in CausalConv1dFn.
     """
-    attrs = _address(SelectiveScanVarlenAttrs, int(delta_softplus), int(output_final_state))
+    attrs = SelectiveScanVarlenAttrs(int(delta_softplus), int(output_final_state))
     shape = None
     if output_final_state:
         if getattr(u, "ndim", 0) != 3 or getattr(A, "ndim", 0) != 2:
@@ -685,7 +672,7 @@ def SelectiveStateUpdateFn(u, delta, A, B, C, D=None, z=None, delta_bias=None, s
     receives it instead. Rows whose index is outside the pool are skipped and their output rows left as they were."""
     if state is None:
         _invalid("SelectiveStateUpdateFn needs a state")
-    return _serve_state(_UPDATE, _address(SelectiveStateUpdateAttrs, int(delta_softplus)),
+    return _serve_state(_UPDATE, SelectiveStateUpdateAttrs(int(delta_softplus)),
                   (u, delta, A, B, C, D, z, delta_bias, state, state_indices), out, new_state,
                   None if new_state is None or new_state is state else (), True, stream)
 
@@ -716,7 +703,7 @@ def GatedRecurrenceFn(x, f, lower_bound=None, initial_state=None, cu_seqlens=Non
         if getattr(x, "ndim", 0) != 3:
             _invalid("x must have rank 3")
         shape = _prompt_state_shape(x, cu_seqlens, state_indices, initial_state, final_state, (x.shape[2],))
-    return _serve_state(_GATE, _address(GatedRecurrenceAttrs, int(output_final_state)),
+    return _serve_state(_GATE, GatedRecurrenceAttrs(int(output_final_state)),
                   (x, f, lower_bound, initial_state, cu_seqlens, state_indices, has_initial_state), out, final_state,
                   shape, bool(output_final_state), stream)
 
@@ -742,7 +729,7 @@ def GatedRecurrenceGradFn(dy, x, f, y, lower_bound=None, initial_state=None, cu_
         out = (None, None, None, None)
     elif len(out) != 4:
         _invalid("out must hold 4 outputs (None: allocate)")
-    got = _serve(_GATE_GRAD, _address(GatedRecurrenceGradAttrs, int(lb), int(st)),
+    got = _serve(_GATE_GRAD, GatedRecurrenceGradAttrs(int(lb), int(st)),
                  (dy, x, f, y, lower_bound, initial_state, cu_seqlens, d_final_state),
                  (*out[:2], *out[2:3 if lb else 2], *out[3:4 if st else 3]),
                  (None, None, *(((0, dim),) if lb else ()), *(((0, units, dim),) if st else ())), stream)
@@ -757,7 +744,7 @@ def GatedRecurrenceUpdateFn(x, f, lower_bound=None, state=None, state_indices=No
     they were."""
     if state is None:
         _invalid("GatedRecurrenceUpdateFn needs a state")
-    return _serve_state(_GATE_UPDATE, _address(GatedRecurrenceUpdateAttrs, 0), (x, f, lower_bound, state, state_indices), out, new_state,
+    return _serve_state(_GATE_UPDATE, GatedRecurrenceUpdateAttrs(0), (x, f, lower_bound, state, state_indices), out, new_state,
                   None if new_state is None or new_state is state else (), True, stream)
 
 
@@ -785,7 +772,7 @@ def LayerNormFn(x, weight=None, bias=None, residual=None, *, eps: float = 1e-5, 
                 inplace = 3
     if output_stats:
         outs, shapes = (*outs, stats), (*shapes, (0, *x.shape[:-1], 2))
-    got = _serve(_NORM, _address(LayerNormAttrs, float(eps), int(rms), int(output_stats)), (x, weight, bias, residual),
+    got = _serve(_NORM, LayerNormAttrs(float(eps), int(rms), int(output_stats)), (x, weight, bias, residual),
                  outs, shapes, stream, inplace)
     return got if len(got) > 1 else got[0]
 
@@ -809,7 +796,7 @@ def LayerNormGradFn(dy, x, weight=None, stats=None, d_residual=None, *, rms: int
     elif len(out) != 3:
         _invalid("out must hold 3 outputs (None: allocate)")
     sums = int(many) + bool(output_bias_grad)
-    got = _serve(_NORM_GRAD, _address(LayerNormGradAttrs, int(rms), int(output_bias_grad)),
+    got = _serve(_NORM_GRAD, LayerNormGradAttrs(int(rms), int(output_bias_grad)),
                  (dy, x, weight, stats, d_residual),
                  (out[0], *out[1:2 if many else 1], *out[2:3 if output_bias_grad else 2]), (None,) + ((0, dim),) * sums,
                  stream)
