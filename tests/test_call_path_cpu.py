@@ -54,3 +54,24 @@ def test_attributes_live_as_long_as_the_call(xm, monkeypatch, native, op):
     for t in threads:
         t.join(30)
     assert seen == ([0.125] * 2 if op == "norm" else [1] * 2)
+
+
+def _workspace_of(xm, nbytes):
+    """A workspace query that answers with nbytes, as the native call path takes it."""
+    c = xm.ctypes
+
+    @c.CFUNCTYPE(c.c_int, c.c_void_p, c.c_void_p, c.c_int32, c.POINTER(c.c_size_t))
+    def size(attrs, inputs, n, answer):
+        answer[0] = nbytes
+        return 0
+
+    return size, c.cast(size, c.c_void_p).value
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="needs an allocation that fails")
+def test_torch_errors_come_through_as_torch_raises_them(xm):
+    """A workspace that torch cannot allocate: torch's own exception, without a C++ trace in its text."""
+    size, entry = _workspace_of(xm, 1000)
+    with pytest.raises(RuntimeError, match="NVIDIA driver") as caught:
+        xm._load_pycall().call(0, entry, 0, (), b"", (), 0, -1, None, 0)
+    assert "Exception raised from" not in str(caught.value) and "frame #" not in str(caught.value)

@@ -5,18 +5,19 @@
 // method calls through the CPython API (half a microsecond a tensor). Here the
 // tensors are read through torch's C++ API, which also allocates the outputs and
 // the workspace, and the operator's entry point is called with the interpreter
-// lock free. Built against the headers of the Python and the torch that run it.
+// lock free. What torch throws is raised as torch's own functions raise it. Built
+// against the headers of the Python and the torch that run it.
 #include <Python.h>
 
 #include <cstdint>
 #include <cstring>
-#include <exception>
 #include <vector>
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -42,7 +43,7 @@ int32_t code_of(at::ScalarType t) {
 
 void describe(const at::Tensor &t, xm_tensor *d) {
     const auto sizes = t.sizes();
-    if (sizes.size() > XM_MAX_RANK) throw std::runtime_error("tensor rank above 8 is not supported");
+    TORCH_CHECK_VALUE(sizes.size() <= XM_MAX_RANK, "tensor rank above 8 is not supported");
     d->data = t.data_ptr();
     d->rank = static_cast<int32_t>(sizes.size());
     for (size_t i = 0; i < sizes.size(); ++i) d->shape[i] = sizes[i];
@@ -101,18 +102,6 @@ long run(FwdFn fwd, SizeFn size, const void *attrs, const xm_tensor *in, Py_ssiz
     return s;
 }
 
-template <typename F>
-PyObject *guarded(F &&f) {
-    try {
-        return f();
-    } catch (const std::exception &e) {
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
-    } catch (...) {
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "unknown error");
-    }
-    return nullptr;
-}
-
 void *pointer(PyObject *o) { return reinterpret_cast<void *>(static_cast<uintptr_t>(PyLong_AsUnsignedLongLongMask(o))); }
 
 // call(fwd, size, attrs, inputs, blank, outputs, device, inplace, alloc, stream) -> (status, which)
@@ -123,6 +112,7 @@ void *pointer(PyObject *o) { return reinterpret_cast<void *>(static_cast<uintptr
 //   inplace     index of an input that must not be copied, or -1
 //   alloc       not used: the workspace is allocated here
 PyObject *call(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
     if (n != 10 || !PyTuple_Check(a[3]) || !PyBytes_Check(a[4]) || !PyTuple_Check(a[5])) {
         PyErr_SetString(PyExc_TypeError, "call: wrong arguments");
         return nullptr;
@@ -139,19 +129,18 @@ PyObject *call(PyObject *, PyObject *const *a, Py_ssize_t n) {
         PyErr_SetString(PyExc_TypeError, "call: wrong number of tensors");
         return nullptr;
     }
-    return guarded([&]() -> PyObject * {
-        xm_tensor in[kMaxTensors], out[kMaxTensors];
-        std::memcpy(in, PyBytes_AS_STRING(a[4]), static_cast<size_t>(n_in) * sizeof(xm_tensor));
-        std::vector<at::Tensor> keep;
-        Answer answer = describe_inputs(a[3], index, inplace, in, keep);
-        for (Py_ssize_t i = 0; answer.status == 0 && i < n_out; ++i) {
-            PyObject *o = PyTuple_GET_ITEM(a[5], i);
-            if (!on_device(o, index) || !THPVariable_Unpack(o).is_contiguous()) answer = Answer{-3, static_cast<long>(i)};
-            else describe(THPVariable_Unpack(o), &out[i]);
-        }
-        if (answer.status == 0) answer.status = run(fwd, size, attrs, in, n_in, out, index, stream, keep);
-        return Py_BuildValue("(ll)", answer.status, answer.which);
-    });
+    xm_tensor in[kMaxTensors], out[kMaxTensors];
+    std::memcpy(in, PyBytes_AS_STRING(a[4]), static_cast<size_t>(n_in) * sizeof(xm_tensor));
+    std::vector<at::Tensor> keep;
+    Answer answer = describe_inputs(a[3], index, inplace, in, keep);
+    for (Py_ssize_t i = 0; answer.status == 0 && i < n_out; ++i) {
+        PyObject *o = PyTuple_GET_ITEM(a[5], i);
+        if (!on_device(o, index) || !THPVariable_Unpack(o).is_contiguous()) answer = Answer{-3, static_cast<long>(i)};
+        else describe(THPVariable_Unpack(o), &out[i]);
+    }
+    if (answer.status == 0) answer.status = run(fwd, size, attrs, in, n_in, out, index, stream, keep);
+    return Py_BuildValue("(ll)", answer.status, answer.which);
+    END_HANDLE_TH_ERRORS
 }
 
 // serve(fwd, size, attrs, inputs, blanks, outputs, shapes, inplace) -> outputs, or (status, which) as integers
@@ -160,6 +149,7 @@ PyObject *call(PyObject *, PyObject *const *a, Py_ssize_t n) {
 //   shapes      per output None (the shape and type of input 0) or (own, sizes...): float32, or with own 1 input 0's type
 // Further statuses: -4: input 0 is not a CUDA tensor, -5: it is not on the current device.
 PyObject *serve(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
     if (n != 8 || !PyTuple_Check(a[3]) || !PyTuple_Check(a[4]) || PyTuple_GET_SIZE(a[4]) != 4 || !PyTuple_Check(a[5]) ||
         !PyTuple_Check(a[6]) || PyTuple_GET_SIZE(a[5]) != PyTuple_GET_SIZE(a[6])) {
         PyErr_SetString(PyExc_TypeError, "serve: wrong arguments");
@@ -175,60 +165,59 @@ PyObject *serve(PyObject *, PyObject *const *a, Py_ssize_t n) {
         PyErr_SetString(PyExc_TypeError, "serve: wrong number of tensors");
         return nullptr;
     }
-    return guarded([&]() -> PyObject * {
-        PyObject *first = PyTuple_GET_ITEM(a[3], 0);
-        if (!THPVariable_Check(first) || !THPVariable_Unpack(first).is_cuda()) return Py_BuildValue("(ll)", -4L, 0L);
-        const at::Tensor &x = THPVariable_Unpack(first);
-        const int64_t index = x.get_device();
-        if (index != c10::cuda::current_device()) return Py_BuildValue("(ll)", -5L, 0L);
-        const int32_t code = code_of(x.scalar_type());
-        PyObject *blank = PyTuple_GET_ITEM(
-            a[4], code == XM_DTYPE_FLOAT ? 0 : code == XM_DTYPE_BFLOAT16 ? 1 : code == XM_DTYPE_FLOAT16 ? 2 : 3);
-        if (!PyBytes_Check(blank) || PyBytes_GET_SIZE(blank) != static_cast<Py_ssize_t>(n_in * sizeof(xm_tensor)))
-            throw std::runtime_error("serve: wrong descriptors");
-        xm_tensor in[kMaxTensors], out[kMaxTensors];
-        std::memcpy(in, PyBytes_AS_STRING(blank), static_cast<size_t>(n_in) * sizeof(xm_tensor));
-        std::vector<at::Tensor> keep;
-        Answer answer = describe_inputs(a[3], index, inplace, in, keep);
-        if (answer.status != 0) return Py_BuildValue("(ll)", answer.status, answer.which);
-        at::Tensor made[kMaxTensors];
-        for (Py_ssize_t i = 0; i < n_out; ++i) {
-            PyObject *o = PyTuple_GET_ITEM(a[5], i), *shape = PyTuple_GET_ITEM(a[6], i);
-            if (o != Py_None) {
-                if (!on_device(o, index) || !THPVariable_Unpack(o).is_contiguous())
-                    return Py_BuildValue("(ll)", -3L, static_cast<long>(i));
-                made[i] = THPVariable_Unpack(o);
-            } else if (shape == Py_None) {
-                made[i] = at::empty(x.sizes(), x.options());
-            } else {
-                int64_t sizes[XM_MAX_RANK];
-                const Py_ssize_t rank = PyTuple_Check(shape) ? PyTuple_GET_SIZE(shape) - 1 : -1;
-                if (rank < 0 || rank > XM_MAX_RANK) throw std::runtime_error("serve: wrong shape");
-                for (Py_ssize_t k = 0; k < rank; ++k) sizes[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, k + 1));
-                const long own = PyLong_AsLong(PyTuple_GET_ITEM(shape, 0));
-                if (PyErr_Occurred()) return nullptr;
-                made[i] = at::empty(at::IntArrayRef(sizes, static_cast<size_t>(rank)),
-                                    x.options().dtype(own != 0 ? x.scalar_type() : at::kFloat));
-            }
-            describe(made[i], &out[i]);
+    PyObject *first = PyTuple_GET_ITEM(a[3], 0);
+    if (!THPVariable_Check(first) || !THPVariable_Unpack(first).is_cuda()) return Py_BuildValue("(ll)", -4L, 0L);
+    const at::Tensor &x = THPVariable_Unpack(first);
+    const int64_t index = x.get_device();
+    if (index != c10::cuda::current_device()) return Py_BuildValue("(ll)", -5L, 0L);
+    const int32_t code = code_of(x.scalar_type());
+    PyObject *blank = PyTuple_GET_ITEM(
+        a[4], code == XM_DTYPE_FLOAT ? 0 : code == XM_DTYPE_BFLOAT16 ? 1 : code == XM_DTYPE_FLOAT16 ? 2 : 3);
+    if (!PyBytes_Check(blank) || PyBytes_GET_SIZE(blank) != static_cast<Py_ssize_t>(n_in * sizeof(xm_tensor)))
+        TORCH_CHECK(false, "serve: wrong descriptors");
+    xm_tensor in[kMaxTensors], out[kMaxTensors];
+    std::memcpy(in, PyBytes_AS_STRING(blank), static_cast<size_t>(n_in) * sizeof(xm_tensor));
+    std::vector<at::Tensor> keep;
+    Answer answer = describe_inputs(a[3], index, inplace, in, keep);
+    if (answer.status != 0) return Py_BuildValue("(ll)", answer.status, answer.which);
+    at::Tensor made[kMaxTensors];
+    for (Py_ssize_t i = 0; i < n_out; ++i) {
+        PyObject *o = PyTuple_GET_ITEM(a[5], i), *shape = PyTuple_GET_ITEM(a[6], i);
+        if (o != Py_None) {
+            if (!on_device(o, index) || !THPVariable_Unpack(o).is_contiguous())
+                return Py_BuildValue("(ll)", -3L, static_cast<long>(i));
+            made[i] = THPVariable_Unpack(o);
+        } else if (shape == Py_None) {
+            made[i] = at::empty(x.sizes(), x.options());
+        } else {
+            int64_t sizes[XM_MAX_RANK];
+            const Py_ssize_t rank = PyTuple_Check(shape) ? PyTuple_GET_SIZE(shape) - 1 : -1;
+            if (rank < 0 || rank > XM_MAX_RANK) TORCH_CHECK(false, "serve: wrong shape");
+            for (Py_ssize_t k = 0; k < rank; ++k) sizes[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, k + 1));
+            const long own = PyLong_AsLong(PyTuple_GET_ITEM(shape, 0));
+            if (PyErr_Occurred()) return nullptr;
+            made[i] = at::empty(at::IntArrayRef(sizes, static_cast<size_t>(rank)),
+                                x.options().dtype(own != 0 ? x.scalar_type() : at::kFloat));
         }
-        void *stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(index)).stream();
-        answer.status = run(fwd, size, attrs, in, n_in, out, index, stream, keep);
-        if (answer.status != 0) return Py_BuildValue("(ll)", answer.status, answer.which);
-        PyObject *result = PyTuple_New(n_out);
-        if (result == nullptr) return nullptr;
-        for (Py_ssize_t i = 0; i < n_out; ++i) {
-            PyObject *o = PyTuple_GET_ITEM(a[5], i);
-            if (o != Py_None) Py_INCREF(o);
-            else o = THPVariable_Wrap(std::move(made[i]));
-            if (o == nullptr) {
-                Py_DECREF(result);
-                return nullptr;
-            }
-            PyTuple_SET_ITEM(result, i, o);
+        describe(made[i], &out[i]);
+    }
+    void *stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(index)).stream();
+    answer.status = run(fwd, size, attrs, in, n_in, out, index, stream, keep);
+    if (answer.status != 0) return Py_BuildValue("(ll)", answer.status, answer.which);
+    PyObject *result = PyTuple_New(n_out);
+    if (result == nullptr) return nullptr;
+    for (Py_ssize_t i = 0; i < n_out; ++i) {
+        PyObject *o = PyTuple_GET_ITEM(a[5], i);
+        if (o != Py_None) Py_INCREF(o);
+        else o = THPVariable_Wrap(std::move(made[i]));
+        if (o == nullptr) {
+            Py_DECREF(result);
+            return nullptr;
         }
-        return result;
-    });
+        PyTuple_SET_ITEM(result, i, o);
+    }
+    return result;
+    END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {
