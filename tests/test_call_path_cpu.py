@@ -4,6 +4,7 @@ native entry is replaced by a Python function where one is needed."""
 from __future__ import annotations
 
 import threading
+import time
 import weakref
 
 import pytest
@@ -75,3 +76,17 @@ def test_torch_errors_come_through_as_torch_raises_them(xm):
     with pytest.raises(RuntimeError, match="NVIDIA driver") as caught:
         xm._load_pycall().call(0, entry, 0, (), b"", (), 0, -1, None, 0)
     assert "Exception raised from" not in str(caught.value) and "frame #" not in str(caught.value)
+
+
+def test_the_workspace_query_lets_other_threads_run(xm):
+    """The interpreter is free from the workspace query on, so that allocations that wait for the device hold nobody up
+    (libc's usleep stands in for the query; it sleeps as many microseconds as its first argument says)."""
+    entry = xm.ctypes.cast(xm.ctypes.CDLL(None).usleep, xm.ctypes.c_void_p).value
+    none = xm.ctypes.cast(xm.ctypes.CDLL(None).getppid, xm.ctypes.c_void_p).value
+    ran = []
+    other = threading.Thread(target=lambda: (time.sleep(0.05), ran.append(time.monotonic())))
+    other.start()
+    xm._load_pycall().call(none, entry, 900_000, (), b"", (), 0, -1, None, 0)
+    done = time.monotonic()
+    other.join()
+    assert ran[0] < done - 0.1

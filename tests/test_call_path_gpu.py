@@ -3,6 +3,9 @@ come from torch, other threads."""
 
 from __future__ import annotations
 
+import threading
+import time
+
 import pytest
 import torch
 
@@ -34,3 +37,50 @@ def test_too_many_axes(xm, cuda):
     with pytest.raises(ValueError, match="tensor rank above 8 is not supported"):
         xm.CausalConv1dUpdateFn(x, x, None, x)
     assert xm.LayerNormFn(x[0]).shape == x.shape[1:]
+
+
+def test_other_threads_run_during_a_call(xm, cuda):
+    """serve() with libc's usleep in place of the workspace query (which sleeps as long as its first argument says)."""
+    xm._NORM.load()
+    entry, none = (xm.ctypes.cast(f, xm.ctypes.c_void_p).value for f in (xm.ctypes.CDLL(None).usleep,
+                                                                       xm.ctypes.CDLL(None).getppid))
+    x = torch.rand(3, 8, device="cuda")
+    ran = []
+    other = threading.Thread(target=lambda: (time.sleep(0.05), ran.append(time.monotonic())))
+    other.start()
+    xm._load_pycall().serve(none, entry, 900_000, (x, None, None, None), xm._NORM.blanks, (None,), (None,), -1)
+    done = time.monotonic()
+    other.join()
+    assert ran[0] < done - 0.1
+
+
+def test_calls_from_several_threads(xm, cuda):
+    """Threads with a stream each call with attributes, strides and outputs of their own; all get what one thread gets."""
+    x = torch.rand(64, 100, device="cuda")
+    cases = [(x[:, i:i + 40], 10.0**-i, i % 2) for i in range(6)]
+
+    def run(case):
+        v, eps, rms = case
+        y, stats = xm.LayerNormFn(v, eps=eps, rms=rms, output_stats=1)
+        s = torch.ones(64, 40, device="cuda")
+        return y, stats, *xm.GatedRecurrenceUpdateFn(v, y, None, s), xm.GatedRecurrenceFn(v[None], y[None]), \
+            xm.LayerNormGradFn(y, v, None, stats, rms=rms, output_bias_grad=1)[2]
+
+    want = [run(c) for c in cases]
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(len(cases))
+
+    def worker(case, expected):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait(30)
+            for _ in range(200):
+                got = run(case)
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(k for k, (a, b) in enumerate(zip(got, expected)) if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=worker, args=a) for a in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert wrong == [] and not any(t.is_alive() for t in threads)

@@ -4,13 +4,15 @@
 // a tensor to the C ABI takes several Python operations each through ctypes, or
 // method calls through the CPython API (half a microsecond a tensor). Here the
 // tensors are read through torch's C++ API, which also allocates the outputs and
-// the workspace, and the operator's entry point is called with the interpreter
+// the workspace and calls the operator's entry point, all with the interpreter
 // lock free. What torch throws is raised as torch's own functions raise it. Built
 // against the headers of the Python and the torch that run it.
 #include <Python.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <utility>
 #include <vector>
 
 #include <ATen/core/Tensor.h>
@@ -41,9 +43,11 @@ int32_t code_of(at::ScalarType t) {
     }
 }
 
+constexpr const char *kRank = "tensor rank above 8 is not supported";
+
 void describe(const at::Tensor &t, xm_tensor *d) {
     const auto sizes = t.sizes();
-    TORCH_CHECK_VALUE(sizes.size() <= XM_MAX_RANK, "tensor rank above 8 is not supported");
+    TORCH_CHECK_VALUE(sizes.size() <= XM_MAX_RANK, kRank);
     d->data = t.data_ptr();
     d->rank = static_cast<int32_t>(sizes.size());
     for (size_t i = 0; i < sizes.size(); ++i) d->shape[i] = sizes[i];
@@ -62,45 +66,77 @@ struct Answer {
     long status, which;
 };
 
-// Describes the inputs over the descriptors of absent ones; copies of those that are not contiguous go to `keep`.
-Answer describe_inputs(PyObject *tensors, int64_t index, long inplace, xm_tensor *in, std::vector<at::Tensor> &keep) {
-    const Py_ssize_t n = PyTuple_GET_SIZE(tensors);
-    for (Py_ssize_t i = 0; i < n; ++i) {
-        PyObject *o = PyTuple_GET_ITEM(tensors, i);
-        if (o == Py_None) continue;
-        if (!on_device(o, index)) return Answer{-1, static_cast<long>(i)};
-        const at::Tensor &t = THPVariable_Unpack(o);
-        if (t.is_contiguous()) {
-            describe(t, &in[i]);
-        } else {
-            if (i == inplace) return Answer{-2, static_cast<long>(i)};
-            keep.push_back(t.contiguous());
-            describe(keep.back(), &in[i]);
-        }
-    }
-    return Answer{0, 0};
-}
-
-// Asks for the workspace, allocates it on the current stream and calls the entry point.
-long run(FwdFn fwd, SizeFn size, const void *attrs, const xm_tensor *in, Py_ssize_t n_in, xm_tensor *out, int64_t index,
-         void *stream, std::vector<at::Tensor> &keep) {
-    size_t bytes = 0;
-    void *ws = nullptr;
-    if (size != nullptr) {
-        const xm_status s = size(attrs, in, static_cast<int32_t>(n_in), &bytes);
-        if (s != XM_OK) return s;
-        if (bytes > 0) {
-            keep.push_back(at::empty({static_cast<int64_t>(bytes)},
-                                     at::TensorOptions(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(index))));
-            ws = keep.back().data_ptr();
-        }
-    }
-    // a launch may wait for room in its queue: other threads run meanwhile (the caller's tuples hold the tensors)
+// Other threads run while one of these is there.
+struct Unlocked {
     PyThreadState *const thread = PyEval_SaveThread();
-    const xm_status s = fwd(attrs, in, static_cast<int32_t>(n_in), out, ws, bytes, stream);
-    PyEval_RestoreThread(thread);
-    return s;
-}
+    ~Unlocked() { PyEval_RestoreThread(thread); }
+};
+
+// A call in two steps: what the tuples hold is read under the interpreter lock; copies, allocations and the entry point,
+// each of which may wait for the device or for room in its queue, come without it (the caller's tuples hold the tensors).
+struct Call {
+    xm_tensor in[kMaxTensors], out[kMaxTensors];
+    Py_ssize_t n_in = 0, n_out = 0;
+    struct Copy {
+        Py_ssize_t at;
+        at::Tensor t;
+    };
+    std::vector<Copy> copies;  // inputs that are not contiguous
+    enum Make : char { kGiven, kOwn, kFloat } make[kMaxTensors] = {};  // outputs to allocate: in input 0's type, in float32
+    at::TensorOptions options;  // of input 0
+    at::Tensor made[kMaxTensors], workspace;
+
+    // Describes the inputs over the descriptors of absent ones.
+    Answer inputs(PyObject *tensors, PyObject *blank, int64_t index, long inplace) {
+        n_in = PyTuple_GET_SIZE(tensors);
+        std::memcpy(in, PyBytes_AS_STRING(blank), static_cast<size_t>(n_in) * sizeof(xm_tensor));
+        for (Py_ssize_t i = 0; i < n_in; ++i) {
+            PyObject *o = PyTuple_GET_ITEM(tensors, i);
+            if (o == Py_None) continue;
+            if (!on_device(o, index)) return Answer{-1, static_cast<long>(i)};
+            const at::Tensor &t = THPVariable_Unpack(o);
+            if (t.is_contiguous()) {
+                describe(t, &in[i]);
+            } else {
+                if (i == inplace) return Answer{-2, static_cast<long>(i)};
+                copies.push_back(Copy{i, t});
+            }
+        }
+        return Answer{0, 0};
+    }
+    // Describes an output that is given.
+    bool output(Py_ssize_t i, PyObject *o, int64_t index) {
+        if (!on_device(o, index) || !THPVariable_Unpack(o).is_contiguous()) return false;
+        describe(THPVariable_Unpack(o), &out[i]);
+        return true;
+    }
+    // The rest, on the current stream's allocations. stream: what the entry point is given.
+    long run(FwdFn fwd, SizeFn size, const void *attrs, int64_t index, void *stream) {
+        const Unlocked unlocked;
+        for (Copy &c : copies) {
+            c.t = c.t.contiguous();
+            describe(c.t, &in[c.at]);
+        }
+        for (Py_ssize_t i = 0; i < n_out; ++i) {
+            if (make[i] == kGiven) continue;
+            made[i] = at::empty(at::IntArrayRef(out[i].shape, static_cast<size_t>(out[i].rank)),
+                                make[i] == kOwn ? options : options.dtype(at::kFloat));
+            describe(made[i], &out[i]);
+        }
+        size_t bytes = 0;
+        void *ws = nullptr;
+        if (size != nullptr) {
+            const xm_status s = size(attrs, in, static_cast<int32_t>(n_in), &bytes);
+            if (s != XM_OK) return s;
+            if (bytes > 0) {
+                workspace = at::empty({static_cast<int64_t>(bytes)},
+                                      at::TensorOptions(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(index)));
+                ws = workspace.data_ptr();
+            }
+        }
+        return fwd(attrs, in, static_cast<int32_t>(n_in), out, ws, bytes, stream);
+    }
+};
 
 void *pointer(PyObject *o) { return reinterpret_cast<void *>(static_cast<uintptr_t>(PyLong_AsUnsignedLongLongMask(o))); }
 
@@ -129,16 +165,12 @@ PyObject *call(PyObject *, PyObject *const *a, Py_ssize_t n) {
         PyErr_SetString(PyExc_TypeError, "call: wrong number of tensors");
         return nullptr;
     }
-    xm_tensor in[kMaxTensors], out[kMaxTensors];
-    std::memcpy(in, PyBytes_AS_STRING(a[4]), static_cast<size_t>(n_in) * sizeof(xm_tensor));
-    std::vector<at::Tensor> keep;
-    Answer answer = describe_inputs(a[3], index, inplace, in, keep);
-    for (Py_ssize_t i = 0; answer.status == 0 && i < n_out; ++i) {
-        PyObject *o = PyTuple_GET_ITEM(a[5], i);
-        if (!on_device(o, index) || !THPVariable_Unpack(o).is_contiguous()) answer = Answer{-3, static_cast<long>(i)};
-        else describe(THPVariable_Unpack(o), &out[i]);
-    }
-    if (answer.status == 0) answer.status = run(fwd, size, attrs, in, n_in, out, index, stream, keep);
+    Call c;
+    Answer answer = c.inputs(a[3], a[4], index, inplace);
+    c.n_out = n_out;
+    for (Py_ssize_t i = 0; answer.status == 0 && i < n_out; ++i)
+        if (!c.output(i, PyTuple_GET_ITEM(a[5], i), index)) answer = Answer{-3, static_cast<long>(i)};
+    if (answer.status == 0) answer.status = c.run(fwd, size, attrs, index, stream);
     return Py_BuildValue("(ll)", answer.status, answer.which);
     END_HANDLE_TH_ERRORS
 }
@@ -175,41 +207,40 @@ PyObject *serve(PyObject *, PyObject *const *a, Py_ssize_t n) {
         a[4], code == XM_DTYPE_FLOAT ? 0 : code == XM_DTYPE_BFLOAT16 ? 1 : code == XM_DTYPE_FLOAT16 ? 2 : 3);
     if (!PyBytes_Check(blank) || PyBytes_GET_SIZE(blank) != static_cast<Py_ssize_t>(n_in * sizeof(xm_tensor)))
         TORCH_CHECK(false, "serve: wrong descriptors");
-    xm_tensor in[kMaxTensors], out[kMaxTensors];
-    std::memcpy(in, PyBytes_AS_STRING(blank), static_cast<size_t>(n_in) * sizeof(xm_tensor));
-    std::vector<at::Tensor> keep;
-    Answer answer = describe_inputs(a[3], index, inplace, in, keep);
-    if (answer.status != 0) return Py_BuildValue("(ll)", answer.status, answer.which);
-    at::Tensor made[kMaxTensors];
-    for (Py_ssize_t i = 0; i < n_out; ++i) {
+    Call c;
+    Answer answer = c.inputs(a[3], blank, index, inplace);
+    c.n_out = n_out;
+    c.options = x.options();
+    for (Py_ssize_t i = 0; answer.status == 0 && i < n_out; ++i) {
         PyObject *o = PyTuple_GET_ITEM(a[5], i), *shape = PyTuple_GET_ITEM(a[6], i);
         if (o != Py_None) {
-            if (!on_device(o, index) || !THPVariable_Unpack(o).is_contiguous())
-                return Py_BuildValue("(ll)", -3L, static_cast<long>(i));
-            made[i] = THPVariable_Unpack(o);
-        } else if (shape == Py_None) {
-            made[i] = at::empty(x.sizes(), x.options());
-        } else {
-            int64_t sizes[XM_MAX_RANK];
-            const Py_ssize_t rank = PyTuple_Check(shape) ? PyTuple_GET_SIZE(shape) - 1 : -1;
-            if (rank < 0 || rank > XM_MAX_RANK) TORCH_CHECK(false, "serve: wrong shape");
-            for (Py_ssize_t k = 0; k < rank; ++k) sizes[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, k + 1));
-            const long own = PyLong_AsLong(PyTuple_GET_ITEM(shape, 0));
-            if (PyErr_Occurred()) return nullptr;
-            made[i] = at::empty(at::IntArrayRef(sizes, static_cast<size_t>(rank)),
-                                x.options().dtype(own != 0 ? x.scalar_type() : at::kFloat));
+            if (!c.output(i, o, index)) answer = Answer{-3, static_cast<long>(i)};
+            continue;
         }
-        describe(made[i], &out[i]);
+        xm_tensor &d = c.out[i];  // (its data once it is there)
+        c.make[i] = Call::kOwn;
+        const Py_ssize_t rank = shape == Py_None ? x.dim() : PyTuple_Check(shape) ? PyTuple_GET_SIZE(shape) - 1 : -1;
+        TORCH_CHECK(rank >= 0, "serve: wrong shape");
+        TORCH_CHECK_VALUE(rank <= XM_MAX_RANK, kRank);
+        d.rank = static_cast<int32_t>(rank);
+        if (shape == Py_None) {
+            std::copy(x.sizes().begin(), x.sizes().end(), d.shape);
+            continue;
+        }
+        for (Py_ssize_t k = 0; k < rank; ++k) d.shape[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, k + 1));
+        if (PyLong_AsLong(PyTuple_GET_ITEM(shape, 0)) == 0) c.make[i] = Call::kFloat;
+        if (PyErr_Occurred()) return nullptr;
     }
-    void *stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(index)).stream();
-    answer.status = run(fwd, size, attrs, in, n_in, out, index, stream, keep);
+    if (answer.status == 0)
+        answer.status = c.run(fwd, size, attrs, index,
+                              c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(index)).stream());
     if (answer.status != 0) return Py_BuildValue("(ll)", answer.status, answer.which);
     PyObject *result = PyTuple_New(n_out);
     if (result == nullptr) return nullptr;
     for (Py_ssize_t i = 0; i < n_out; ++i) {
         PyObject *o = PyTuple_GET_ITEM(a[5], i);
         if (o != Py_None) Py_INCREF(o);
-        else o = THPVariable_Wrap(std::move(made[i]));
+        else o = THPVariable_Wrap(std::move(c.made[i]));
         if (o == nullptr) {
             Py_DECREF(result);
             return nullptr;
