@@ -3,12 +3,20 @@ native entry is replaced by a Python function where one is needed."""
 
 from __future__ import annotations
 
+import pathlib
+import shutil
+import subprocess
+import sys
+import sysconfig
 import threading
 import time
 import weakref
 
 import pytest
 import torch
+
+ROOT = pathlib.Path(__file__).resolve().parents[1]
+SUFFIX = sysconfig.get_config_var("EXT_SUFFIX")
 
 
 @pytest.fixture
@@ -90,3 +98,34 @@ def test_the_workspace_query_lets_other_threads_run(xm):
     done = time.monotonic()
     other.join()
     assert ran[0] < done - 0.1
+
+
+# ------------------------------------------------------------------ building and loading
+
+
+def _make(where, *args):
+    return subprocess.run(["make", "-C", str(where), f"PYTHON={sys.executable}", *args], check=True, capture_output=True,
+                          text=True).stdout
+
+
+@pytest.fixture
+def built(tmp_path):
+    """A copy of the package that counts as built against torch 1.0."""
+    pkg = tmp_path / "pkg"
+    shutil.copytree(ROOT / "include", tmp_path / "include")
+    shutil.copytree(ROOT / "xmetai-onnx-plugins_b200" / "csrc", pkg / "csrc")
+    shutil.copy(ROOT / "xmetai-onnx-plugins_b200" / "Makefile", pkg)
+    (pkg / "_build").mkdir()
+    _make(pkg, "-t", "TORCH_VERSION=1.0")
+    return pkg
+
+
+def test_the_call_path_is_built_anew_for_another_torch(built):
+    assert "pycall" not in _make(built, "-n", "TORCH_VERSION=1.0")
+    plan = _make(built, "-n", "TORCH_VERSION=2.0")
+    assert "pycall.cpp" in plan and "-o libxm_ops.so" not in plan
+    # and once more when the first one comes back
+    stamp = f"_build/call{SUFFIX}.torch-%s"
+    _make(built, "TORCH_VERSION=2.0", stamp % "2.0")
+    assert (built / (stamp % "2.0")).exists() and not (built / (stamp % "1.0")).exists()
+    assert "pycall.cpp" in _make(built, "-n", "TORCH_VERSION=1.0")
