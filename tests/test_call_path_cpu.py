@@ -129,3 +129,10 @@ def test_the_call_path_is_built_anew_for_another_torch(built):
     _make(built, "TORCH_VERSION=2.0", stamp % "2.0")
     assert (built / (stamp % "2.0")).exists() and not (built / (stamp % "1.0")).exists()
     assert "pycall.cpp" in _make(built, "-n", "TORCH_VERSION=1.0")
+
+
+def test_the_c_library_builds_beside_a_torch_without_cuda(built, tmp_path):
+    (tmp_path / "torch" / "include" / "ATen").mkdir(parents=True)
+    (tmp_path / "torch" / "lib").mkdir()
+    plan = _make(built, "-n", "-B", f"TORCH={tmp_path / 'torch'}")
+    assert "-o libxm_ops.so" in plan and "pycall.cpp" not in plan
