@@ -136,3 +136,23 @@ def test_the_c_library_builds_beside_a_torch_without_cuda(built, tmp_path):
     (tmp_path / "torch" / "lib").mkdir()
     plan = _make(built, "-n", "-B", f"TORCH={tmp_path / 'torch'}")
     assert "-o libxm_ops.so" in plan and "pycall.cpp" not in plan
+
+
+def test_a_call_path_of_another_torch_is_refused(xm, monkeypatch, tmp_path):
+    """With how to build it, whether it can be loaded or not."""
+    how = f"build it with `make -C .* PYTHON={sys.executable}`"
+    monkeypatch.setattr(xm, "_pycall", None)
+    with monkeypatch.context() as m:
+        m.setattr(torch, "__version__", "0.0.1")
+        with pytest.raises(xm.XmError, match=f"was built for torch .*, this is 0.0.1; {how}"):
+            xm._load_pycall()
+    monkeypatch.setattr(xm, "_PKG_DIR", tmp_path)
+    with pytest.raises(xm.XmError, match=f"not found; {how}"):
+        xm._load_pycall()
+    # a module that needs what this torch does not have
+    (tmp_path / "m.c").write_text("void missing(void); void *PyInit__xm_call(void) { missing(); return 0; }")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(tmp_path / ("_xm_call" + SUFFIX)), str(tmp_path / "m.c")], check=True)
+    with pytest.raises(xm.XmError, match=f"cannot be loaded.*missing.*; {how}"):
+        xm._load_pycall()
+    monkeypatch.undo()
+    assert xm._load_pycall() is not None

@@ -480,15 +480,18 @@ def _load_pycall():
         import torch
 
         path = _PKG_DIR / ("_xm_call" + sysconfig.get_config_var("EXT_SUFFIX"))
+        how = f"build it with `make -C {_PKG_DIR} PYTHON={sys.executable}` (needs its headers and its torch's)"
         if not path.exists():
-            raise XmError(XM_ERR_UNSUPPORTED, f"{path} not found; build it with `make -C {_PKG_DIR} "
-                                              f"PYTHON={sys.executable}` (needs its headers and its torch's)")
+            raise XmError(XM_ERR_UNSUPPORTED, f"{path} not found; {how}")
         spec = importlib.util.spec_from_file_location("_xm_call", path)
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
+        try:
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+        except ImportError as e:  # (another torch may lack what the module links with)
+            raise XmError(XM_ERR_UNSUPPORTED, f"{path} cannot be loaded ({e}); {how}") from e
         if mod.torch_version.split("+")[0] != torch.__version__.split("+")[0]:
             raise XmError(XM_ERR_UNSUPPORTED, f"{path} was built for torch {mod.torch_version}, this is "
-                                              f"{torch.__version__}; build it with `make -C {_PKG_DIR}`")
+                                              f"{torch.__version__}; {how}")
         _pycall = mod
     return _pycall
 
