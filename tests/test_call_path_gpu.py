@@ -84,3 +84,24 @@ def test_calls_from_several_threads(xm, cuda):
     for t in threads:
         t.join(120)
     assert wrong == [] and not any(t.is_alive() for t in threads)
+
+
+def test_a_residual_without_rows(xm, cuda):
+    """It counts as a residual, and is checked like one, where it has x's shape; any other empty tensor is absent."""
+    x, w = torch.empty(0, 24, device="cuda"), torch.rand(24, device="cuda")
+    none = torch.empty(0, device="cuda")
+    y, s, st = xm.LayerNormFn(x, w, None, x.clone(), output_stats=1)
+    assert y.shape == s.shape == x.shape and st.shape == (0, 2)
+    kept = torch.empty(0, 24, device="cuda")
+    assert xm.LayerNormFn(x, w, None, kept, residual_out=kept)[1] is kept
+    # absent: the same results as where x has rows
+    assert xm.LayerNormFn(x, w, None, none).shape == x.shape
+    y, st = xm.LayerNormFn(x, w, None, none, output_stats=1)
+    assert y.shape == x.shape and st.shape == (0, 2)
+    rows = torch.rand(2, 24, device="cuda")
+    assert torch.equal(xm.LayerNormFn(rows, w, None, none), xm.LayerNormFn(rows, w))
+    for residual, into, match in ((x.half(), None, "float32"), (x.cpu(), None, "residual must be a tensor on cuda:0"),
+                                  (x.clone(), rows, "shape and type of x"), (x.clone(), x.half(), "shape and type of x"),
+                                  (x.clone(), x.cpu(), "an output must be a contiguous tensor on cuda:0")):
+        with pytest.raises(xm.XmError, match=match):
+            xm.LayerNormFn(x, w, None, residual, residual_out=into)

@@ -763,20 +763,24 @@ def LayerNormFn(x, weight=None, bias=None, residual=None, *, eps: float = 1e-5, 
     if getattr(x, "ndim", 0) == 0:
         _invalid("x must have at least one axis")
     outs, shapes, inplace = (out,), (None,), -1
-    if residual is not None:
-        if not _given(residual) and not _given(x):  # no rows: the sum is as empty as its terms
-            y = LayerNormFn(x, weight, bias, eps=eps, rms=rms, output_stats=output_stats, stream=stream, out=out,
-                            stats=stats)
-            y = y if output_stats else (y,)
-            return y[:1] + (x.new_empty(x.shape) if residual_out is None else residual_out,) + y[1:]
-        if _given(residual):
-            outs, shapes = (out, residual_out), (None, None)
-            if residual_out is residual:
-                inplace = 3
+    given = _given(residual)
+    # no rows: a residual of x's shape, which the library takes for an absent one, has a sum as empty as it is
+    empty = residual is not None and not given and getattr(residual, "shape", None) == x.shape
+    if given:
+        outs, shapes = (out, residual_out), (None, None)
+    elif empty and residual_out is not None:
+        if not hasattr(residual_out, "dtype") or (residual_out.shape, residual_out.dtype) != (x.shape, x.dtype):
+            _invalid("output must have the shape and type of x")
+        if residual_out.device != x.device:
+            _invalid(f"an output must be a contiguous tensor on {x.device}")
+    if residual is not None and residual_out is residual:
+        inplace = 3
     if output_stats:
         outs, shapes = (*outs, stats), (*shapes, (0, *x.shape[:-1], 2))
     got = _serve(_NORM, LayerNormAttrs(float(eps), int(rms), int(output_stats)), (x, weight, bias, residual),
                  outs, shapes, stream, inplace)
+    if empty:
+        got = (got[0], x.new_empty(x.shape) if residual_out is None else residual_out, *got[1:])
     return got if len(got) > 1 else got[0]
 
 
