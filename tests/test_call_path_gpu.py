@@ -105,3 +105,70 @@ def test_a_residual_without_rows(xm, cuda):
                                   (x.clone(), x.cpu(), "an output must be a contiguous tensor on cuda:0")):
         with pytest.raises(xm.XmError, match=match):
             xm.LayerNormFn(x, w, None, residual, residual_out=into)
+
+
+def _functions(xm):
+    """The operators and their gradients in autograd's terms, as a program that uses it wires them."""
+
+    class GatedRecurrence(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, f, lower_bound, h0, cu):
+            y, h_last = xm.GatedRecurrenceFn(x, f, lower_bound, h0, cu, output_final_state=1)
+            ctx.save_for_backward(x, f, y, lower_bound, h0, cu)
+            return y, h_last
+
+        @staticmethod
+        def backward(ctx, dy, d_last):
+            x, f, y, lower_bound, h0, cu = ctx.saved_tensors
+            return (*xm.GatedRecurrenceGradFn(dy, x, f, y, lower_bound, h0, cu, d_last), None)
+
+    class ResidualNorm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias, residual):
+            y, s, stats = xm.LayerNormFn(x, weight, bias, residual, output_stats=1)
+            ctx.save_for_backward(s, weight, stats)
+            return y, s
+
+        @staticmethod
+        def backward(ctx, dy, ds):
+            s, weight, stats = ctx.saved_tensors
+            dx, d_weight, d_bias = xm.LayerNormGradFn(dy, s, weight, stats, ds, output_bias_grad=1)
+            return dx, d_weight, d_bias, dx
+
+    return GatedRecurrence.apply, ResidualNorm.apply
+
+
+def test_in_autograd_functions(xm, cuda):
+    """A layer of both in a program that uses autograd: the gradients are those of the formulas, by autograd in 64 bits.
+    Every operator is off by about 2^-20 of what it sums, and gates of at most 1 - 0.3 / (1 + e^4) keep some two hundred
+    tokens at most: 2^-13 of the largest value."""
+    recurrence, norm = _functions(xm)
+    g = torch.Generator().manual_seed(81)
+    n, dim = 130, 24
+    leaves = [torch.randn(1, n, dim, generator=g), 1 + 0.1 * torch.randn(dim, generator=g), torch.randn(dim, generator=g),
+              torch.randn(1, n, dim, generator=g), 0.7 * torch.rand(dim, generator=g), torch.randn(2, dim, generator=g)]
+    cu, weights = [0, 50, n], torch.randn(n, 1, dim, generator=g)
+    dev = [t.cuda().requires_grad_() for t in leaves]
+    x, w, b, r, low, h0 = dev
+    h, s = norm(x, w, b, r)
+    y, last = recurrence(h, s.clamp(-4, 4), low, h0, torch.tensor(cu).cuda())
+    # (a transposed gradient: not contiguous)
+    loss = (y.transpose(0, 1) * weights.cuda()).sum() + (last * last).sum() + s.sum()
+    got = torch.autograd.grad(loss, dev)
+
+    x, w, b, r, low, h0 = exact = [t.double().requires_grad_() for t in leaves]
+    s = x + r
+    d = s - s.mean(-1, keepdim=True)
+    h = d / torch.sqrt((d * d).mean(-1, keepdim=True) + 1e-5) * w + b
+    a = low + (1 - low) * torch.sigmoid(s.clamp(-4, 4))
+    ys, last = [], []
+    for i, (p, q) in enumerate(zip(cu, cu[1:])):
+        state = h0[i]
+        for t in range(p, q):
+            state = a[0, t] * state + (1 - a[0, t]) * h[0, t]
+            ys.append(state)
+        last.append(state)
+    last = torch.stack(last)
+    loss = (torch.stack(ys).unsqueeze(1) * weights.double()).sum() + (last * last).sum() + s.sum()
+    for k, (u, v) in enumerate(zip(got, torch.autograd.grad(loss, exact))):
+        assert float((u.cpu().double() - v).abs().max()) <= 2.0**-13 * float(v.abs().max()), k

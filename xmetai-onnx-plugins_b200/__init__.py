@@ -26,7 +26,8 @@ attribute is set (an extension: the reference rejects those attributes). Optiona
 carrying the reference's own message.
 
 torch is only the plumbing for device memory and streams here; the work runs
-in the library's sm_100a kernels. There is no fallback: if the library is
+in the library's sm_100a kernels. Outputs are plain tensors outside autograd's
+graph, whatever the inputs require: gradients come from the ...GradFn operators. There is no fallback: if the library is
 missing, every call raises.
 """
 
@@ -714,7 +715,8 @@ def GatedRecurrenceFn(x, f, lower_bound=None, initial_state=None, cu_seqlens=Non
 def GatedRecurrenceGradFn(dy, x, f, y, lower_bound=None, initial_state=None, cu_seqlens=None, d_final_state=None, *,
                           output_lower_bound_grad: int | None = None, output_initial_state_grad: int | None = None,
                           stream=None, out=None):
-    """GatedRecurrenceFn's backward pass: returns (dx, df, d_lower_bound, d_initial_state).
+    """GatedRecurrenceFn's backward pass, for the caller's autograd function: returns (dx, df, d_lower_bound,
+    d_initial_state).
 
     dy is the gradient of y, d_final_state (float32 [sequences, dim], None: zero) that of the final states; x, f,
     lower_bound, initial_state and cu_seqlens are what the forward call took, y what it returned. d_lower_bound [dim]
@@ -786,7 +788,7 @@ def LayerNormFn(x, weight=None, bias=None, residual=None, *, eps: float = 1e-5, 
 
 def LayerNormGradFn(dy, x, weight=None, stats=None, d_residual=None, *, rms: int = 0, output_bias_grad: int = 0,
                     stream=None, out=None):
-    """LayerNormFn's backward pass: returns (dx, d_weight, d_bias).
+    """LayerNormFn's backward pass, for the caller's autograd function: returns (dx, d_weight, d_bias).
 
     dy is the gradient of y, d_residual (None: zero) that of the residual sum; x is what was normalised (the residual
     sum where there was a residual), weight what the forward call took, stats what it returned. dx is the gradient of
