@@ -15,7 +15,7 @@ namespace {
 
 constexpr int kStages = 3;  // groups of x and f in use and under way, of a warp with a row or segment
 // And of a warp in a ring. Of four: what leaves an SM as many blocks as its registers do (16-bit types: five; 8 x 2048 x
-// 4096 takes 71 us, and 83 with three stages and four blocks), or its copies (float32: two; 8 x 1024 x 4096 takes 70 us,
+// 4096 takes 72 us, and 83 with three stages and four blocks), or its copies (float32: two; 8 x 1024 x 4096 takes 70 us,
 // and 78 with two stages and four blocks). Of eight, an SM has two at most.
 template <typename T, int kWarps>
 constexpr int kRingStages = kWarps == 8 || sizeof(T) == 4 ? 3 : 2;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(32 * ScanBlock<T>::kWarps, 1) gate_block_kerne
     }
 }
 
-// A row to a block, its warps' groups in turn: x, f and y move once. 8 x 2048 x 4096 in bf16, 403 MB: 71 us, 86 % of copy
+// A row to a block, its warps' groups in turn: x, f and y move once. 8 x 2048 x 4096 in bf16, 403 MB: 72 us, 85 % of copy
 // bandwidth, with an instruction issued every second cycle.
 template <typename T, int kRow, int kWarps>
 struct RingSmem {

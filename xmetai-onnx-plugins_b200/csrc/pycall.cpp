@@ -141,12 +141,13 @@ struct Call {
 void *pointer(PyObject *o) { return reinterpret_cast<void *>(static_cast<uintptr_t>(PyLong_AsUnsignedLongLongMask(o))); }
 
 // call(fwd, size, attrs, inputs, blank, outputs, device, inplace, alloc, stream) -> (status, which)
+// A call with outputs, device and stream of the caller's choosing; the operators go through serve.
 //   fwd, size   entry points as integers (size 0: the operator takes no workspace)
 //   attrs       address of the attribute struct
 //   inputs      tuple of tensors or None; blank: the descriptors of absent inputs, as bytes
 //   outputs     tuple of contiguous tensors
 //   inplace     index of an input that must not be copied, or -1
-//   alloc       not used: the workspace is allocated here
+//   alloc       ignored (the workspace is allocated here)
 PyObject *call(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 10 || !PyTuple_Check(a[3]) || !PyBytes_Check(a[4]) || !PyTuple_Check(a[5])) {

@@ -34,9 +34,10 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // precision: with t = exp(-f), r = 1 / (1 + t) and t r, no difference of nearby values
 // is formed. The exponent stops at 2^126, where r is float32's smallest normal value
 // and t r one: nothing overflows, and NaN stays NaN.
-// For two channels: a = low + rest keep (the share kept), u = rest take (taken up), as (rest t) r. rest meets t first: where f is far below
-// zero, r is next to the smallest normal value, and rest r would lose its bits below it before t brought them back (bound
-// 0.99999, f = -87: u off by 3e-3). Far above zero r is 1, and rest t loses no more than u itself has to.
+// For two channels: a = low + rest keep (the share kept), u = rest take (taken up), as (rest t) r. rest meets t first:
+// where f is far below zero, r is next to the smallest normal value, and rest r would lose its bits below it before t
+// brought them back (bound 0.99999, f = -87: u off by 3e-3). Far above zero r is 1, and rest t loses no more than u itself
+// has to.
 struct Gate2 {
     float2 keep, take, a, u;
 };
@@ -159,7 +160,8 @@ __device__ __forceinline__ void for_empty_sequences(const SeqArgs &q, int warp, 
     }
 }
 
-// Products of gates are kept above zero, so that an infinite start outlasts their underflow as it does step by step.
+// Products of gates are kept above zero, so that an infinite start outlasts their underflow as it does step by step. (To a
+// finite start this adds 2^-149 of it, no more than the last bits of products next to underflow do.)
 __device__ __forceinline__ float2 above_zero(float2 P) { return make_float2(fmaxf(P.x, 1.4e-45f), fmaxf(P.y, 1.4e-45f)); }
 __device__ __forceinline__ bool finite1(float v) { return fabsf(v) <= 3.4028235e38f; }
 __device__ __forceinline__ bool finite2(float2 v) { return finite1(v.x) && finite1(v.y); }

@@ -173,9 +173,10 @@ struct RowPart {
 
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
 
-// Rows that are not pairs of elements, staged in shared memory: asynchronous copies of 16-byte words, from the one that holds a
-// row's first element, behind up to a word's others. Elements are read from there by consecutive threads, about sixteen to each: fewer leave most of a row's time to its barriers (32768 x 1026, backward:
-// 229 us with 512 threads), more too few warps.
+// Rows that are too long for registers in pairs or single elements, staged in shared memory: asynchronous copies of 16-byte
+// words, from the one that holds a row's first element, behind up to a word's others. Elements are read from there by
+// consecutive threads, eight to twenty to each up to 8192: fewer leave most of a row's time to its barriers (32768 x 1027 in
+// bf16: 95 us, and 230 with 512 threads; backward 147 and 406), more too few warps.
 constexpr int staged_threads(int dim) { return dim <= 2048 ? 128 : dim <= 5120 ? 256 : 512; }
 
 template <typename T>
