@@ -27,8 +27,8 @@ carrying the reference's own message.
 
 torch is only the plumbing for device memory and streams here; the work runs
 in the library's sm_100a kernels. Outputs are plain tensors outside autograd's
-graph, whatever the inputs require: gradients come from the ...GradFn operators. There is no fallback: if the library is
-missing, every call raises.
+graph, whatever the inputs require: gradients come from the ...GradFn operators.
+There is no fallback: if the library is missing, every call raises.
 """
 
 from __future__ import annotations

@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 4 ? 5 : 2) gate_ring_ke
 
 // One token per sequence: bound by memory, 8 bytes of state and three elements per channel. A thread takes kVec
 // neighbouring channels (a word of the I/O type, or one where rows are not whole words) of kRows sequences, whose loads
-// are issued together. 256 x 4096 in fp16, 15 MB: 3.3 us in a graph, 67 % of copy bandwidth.
+// are issued together. 256 x 4096 in fp16, 15 MB: 3.5 us in a graph, 64 % of copy bandwidth.
 constexpr int kTokenThreads = 128;
 
 template <int kVec>
